@@ -68,6 +68,30 @@ int32_t check_decode_desc(const enigma_decode_layer_desc* d);
 
 cudaError_t qwen_decode_f32_launch(const enigma_qwen_decode_f32_desc& q, cudaStream_t s);
 
+// Serving attention: bf16 shapes that fit the tensor-core kernels' tiles go there, the rest to
+// the CUDA-core kernels.
+cudaError_t sdpa_packed_launch(const enigma_sdpa_packed_desc& d, cudaStream_t s);
+cudaError_t sdpa_packed_simt_launch(const enigma_sdpa_packed_desc& d, cudaStream_t s);
+size_t sdpa_shared_prefix_workspace(const enigma_sdpa_shared_prefix_desc& d);
+cudaError_t sdpa_shared_prefix_launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s);
+cudaError_t sdpa_paged_simt_launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s);
+
+// Paged cache (kv_cache.cu).
+size_t kv_cache_workspace_bytes(const enigma_kv_cache_desc& d);
+cudaError_t kv_cache_fork(const enigma_kv_cache_desc& d, const int32_t* parents,
+                          const int32_t* children, int64_t n, cudaStream_t s);
+cudaError_t kv_cache_free(const enigma_kv_cache_desc& d, const int32_t* slots, int64_t n,
+                          cudaStream_t s);
+cudaError_t kv_cache_reserve(const enigma_kv_cache_desc& d, const int32_t* slots,
+                             const int32_t* lens, int64_t n, cudaStream_t s);
+cudaError_t kv_cache_write(const enigma_kv_cache_desc& d, int64_t layer, const void* new_k,
+                           const void* new_v, const int64_t* strides4, const int32_t* slots,
+                           const int32_t* starts, const int32_t* cu, int64_t n, int64_t tokens,
+                           cudaStream_t s);
+cudaError_t kv_cache_compact(const enigma_kv_cache_desc& d, cudaStream_t s);
+cudaError_t kv_cache_copy_pages(const enigma_kv_cache_desc& d, const int32_t* src,
+                                const int32_t* dst, int64_t n, cudaStream_t s);
+
 cudaError_t elementwise_launch(int op, int dtype, const void* a, const void* b, void* c, int64_t n,
                                cudaStream_t s);
 

@@ -27,7 +27,7 @@ from .tuple import product, repeat_like, select
 from .typing import (BFloat16, Bool, Float16, Float32, Int8, Int16, Int32, Int64, Scalar, UInt8,
                      UInt16, UInt32, UInt64, b1, bf16, f16, f32, i8, i16, i32, i64, u8, u16, u32,
                      u64)
-from . import benchmark, cuda_ops, ops, testing  # noqa: F401
+from . import benchmark, cuda_ops, kv_cache, ops, testing  # noqa: F401
 from .ops import (dequantize_int8, gemm, pack_int4x2, pack_uint8x4, unpack_int4x2,
                   unpack_uint8x4)
 

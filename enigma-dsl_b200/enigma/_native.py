@@ -18,6 +18,8 @@ _LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libenigma_cuda.so"
 OK, ERR_LAUNCH, ERR_EXEC, ERR_TIMEOUT, ERR_BADARG, ERR_DEVICE = 0, -1, -2, -3, -4, -5
 DTYPE_F32, DTYPE_BF16 = 0, 1
 KERNEL_RMSNORM, KERNEL_GEMM, KERNEL_SDPA = 1, 2, 3
+PACKED_PLAN_HEADER = 8
+CACHE_FULL, CACHE_BAD_REQUEST = 1, 2
 
 _STATUS_NAMES = {
     ERR_LAUNCH: "launch failed",
@@ -68,6 +70,20 @@ PROTOTYPES = {
     "enigma_qwen_decode_f32": [_vp, _vp],
     "enigma_decode_layer_bf16_noalloc": [_vp, _vp, _vp, _vp],
     "enigma_decode_noalloc_check_timeout_path": [_i64, _vp],
+    "enigma_sdpa_packed_plan": [_c.POINTER(_i64), _c.POINTER(_i64), _i64, _i64, _i64, _i32,
+                                _c.POINTER(_i32), _i64, _c.POINTER(_i64)],
+    "enigma_sdpa_packed_workspace_bytes": [_c.POINTER(_i32), _i64, _c.POINTER(_sz)],
+    "enigma_sdpa_packed": [_vp, _vp],
+    "enigma_sdpa_shared_prefix_workspace_bytes": [_vp, _c.POINTER(_sz)],
+    "enigma_sdpa_shared_prefix": [_vp, _vp],
+    "enigma_kv_cache_workspace_bytes": [_vp, _c.POINTER(_sz)],
+    "enigma_kv_cache_fork": [_vp, _vp, _vp, _i64, _vp],
+    "enigma_kv_cache_free": [_vp, _vp, _i64, _vp],
+    "enigma_kv_cache_reserve": [_vp, _vp, _vp, _i64, _vp],
+    "enigma_kv_cache_write": [_vp, _i64, _vp, _vp, _c.POINTER(_i64), _vp, _vp, _vp, _i64, _i64,
+                              _vp],
+    "enigma_kv_cache_compact": [_vp, _vp],
+    "enigma_kv_cache_copy_pages": [_vp, _vp, _vp, _i64, _vp],
     "enigma_dispatch": [_i32, _c.POINTER(_vp), _i32, _c.POINTER(_i64), _i32, _c.POINTER(_f32),
                         _i32, _u32p, _u32p, _vp],
     "enigma_dispatch_timed": [_i32, _c.POINTER(_vp), _i32, _c.POINTER(_i64), _i32,

@@ -126,6 +126,192 @@ def sdpa(q, k, v, scale: Optional[float] = None, causal: bool = False, out=None)
     return out
 
 
+class PackedPlan:
+    """The work list of `sdpa_packed` for prompts of these lengths, made once per batch.
+
+    lens_q / lens_k: tokens of each sequence's queries and keys (lens_k defaults to lens_q; a
+    sequence with more keys than queries continues an earlier part of its context).
+    """
+
+    def __init__(self, lens_q, lens_k=None, *, heads_q: int, heads_kv: int, causal: bool = True,
+                 device="cuda"):
+        torch = _torch()
+        lens_q = [int(n) for n in lens_q]
+        lens_k = lens_q if lens_k is None else [int(n) for n in lens_k]
+        if len(lens_q) != len(lens_k):
+            raise ValueError("PackedPlan: lens_q and lens_k differ in number")
+        n = len(lens_q)
+        c_q, c_k = (ctypes.c_int64 * n)(*lens_q), (ctypes.c_int64 * n)(*lens_k)
+        count = ctypes.c_int64()
+        args = (c_q, c_k, n, heads_q, heads_kv, int(causal))
+        _native.call("enigma_sdpa_packed_plan", *args, None, 0, ctypes.byref(count))
+        ints = torch.empty(count.value, dtype=torch.int32)
+        _native.call("enigma_sdpa_packed_plan", *args,
+                     ctypes.cast(ints.data_ptr(), ctypes.POINTER(ctypes.c_int32)), count.value,
+                     ctypes.byref(count))
+        self.heads_q, self.heads_kv, self.causal = int(heads_q), int(heads_kv), bool(causal)
+        self.tokens_q, self.tokens_k = sum(lens_q), sum(lens_k)
+        self.header = (ctypes.c_int32 * _native.PACKED_PLAN_HEADER)(
+            *ints[:_native.PACKED_PLAN_HEADER].tolist())
+        self.ints = ints.to(device)
+
+    def workspace_bytes(self, head_dim: int) -> int:
+        """Device memory that a call with this plan needs (0 unless it splits rows)."""
+        need = ctypes.c_size_t()
+        _native.call("enigma_sdpa_packed_workspace_bytes", self.header, head_dim,
+                     ctypes.byref(need))
+        return need.value
+
+
+class _PackedDesc(ctypes.Structure):
+    """Mirror of enigma_sdpa_packed_desc (include/enigma_cuda.h)."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("tokens_q", "tokens_k", "heads_q", "heads_kv",
+                                              "head_dim", "q_token", "q_head", "k_token",
+                                              "k_head", "v_token", "v_head", "o_token",
+                                              "o_head")] + \
+               [("scale", ctypes.c_float)] + \
+               [(n, ctypes.c_int32) for n in ("causal", "dtype", "reserved")] + \
+               [("header", ctypes.c_int32 * _native.PACKED_PLAN_HEADER)] + \
+               [(n, ctypes.c_void_p) for n in ("plan", "q", "k", "v", "out", "lse",
+                                               "workspace")] + \
+               [("workspace_bytes", ctypes.c_size_t)]
+
+
+def _check_rows(name, *ts):
+    """CUDA tensors of one device and dtype whose last axis is contiguous."""
+    for t in ts:
+        if not t.is_cuda:
+            raise ValueError("enigma CUDA operators take CUDA tensors (no CPU fallback)")
+        if t.device != ts[0].device:
+            raise ValueError("all tensors must be on the same device")
+        if t.dtype != ts[0].dtype:
+            raise TypeError(f"{name}: tensors must share a dtype")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{name}: the last axis must be contiguous")
+    index = ts[0].device.index
+    ensure_device(index if index is not None else 0)
+
+
+def sdpa_packed(q, k, v, plan: PackedPlan, scale: Optional[float] = None, out=None,
+                return_lse: bool = False, workspace=None):
+    """Attention over whole prompts packed one after the other.
+
+    q [tokens_q, Hq, D], k / v [tokens_k, Hkv, D] (GQA when Hkv < Hq), any token and head
+    strides, e.g. slices of one fused projection's output.  Row i of a sequence sees its keys
+    j <= i + len_k - len_q (all of them with a plan made with causal=False); a row that sees
+    none is zero.  scale defaults to 1/sqrt(D).  workspace: a uint8 tensor of
+    plan.workspace_bytes(D) bytes to use instead of an allocation per call.  Returns out
+    [tokens_q, Hq, D], and with return_lse the fp32 log-sum-exp [tokens_q, Hq] too.
+    """
+    torch = _torch()
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError("sdpa_packed: expected [tokens, heads, head_dim] tensors")
+    tq, hq, d = q.shape
+    tk, hk, dk = k.shape
+    if dk != d or v.shape != k.shape:
+        raise ValueError("sdpa_packed: K/V shapes do not match Q")
+    if (hq, hk) != (plan.heads_q, plan.heads_kv):
+        raise ValueError("sdpa_packed: the plan was made for other heads")
+    if (tq, tk) != (plan.tokens_q, plan.tokens_k):
+        raise ValueError(f"sdpa_packed: the plan's lengths sum to {plan.tokens_q} / "
+                         f"{plan.tokens_k} tokens, the tensors hold {tq} / {tk}")
+    if out is None:
+        out = torch.empty((tq, hq, d), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError("sdpa_packed: out must have q's shape")
+    dtype = _dtype_code(q)
+    _check_rows("sdpa_packed", q, k, v, out)
+    if plan.ints.device != q.device:
+        raise ValueError("all tensors must be on the same device")
+    lse = torch.empty((tq, hq), dtype=torch.float32, device=q.device) if return_lse else None
+    if workspace is None:
+        workspace = torch.empty(plan.workspace_bytes(d), dtype=torch.uint8, device=q.device)
+    elif workspace.device != q.device or not workspace.is_contiguous():
+        raise ValueError("sdpa_packed: workspace must be contiguous on the data's device")
+    desc = _PackedDesc(tq, tk, hq, hk, d, *q.stride()[:2], *k.stride()[:2],
+                       *v.stride()[:2], *out.stride()[:2],
+                       1.0 / math.sqrt(d) if scale is None else scale, int(plan.causal), dtype, 0,
+                       plan.header, plan.ints.data_ptr(), q.data_ptr(), k.data_ptr(),
+                       v.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None,
+                       workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    _native.call("enigma_sdpa_packed", ctypes.byref(desc), _stream_ptr(q))
+    return (out, lse) if return_lse else out
+
+
+class _SharedPrefixDesc(ctypes.Structure):
+    """Mirror of enigma_sdpa_shared_prefix_desc (include/enigma_cuda.h)."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("batch", "heads_q", "heads_kv", "head_dim", "page",
+                                              "pages", "table_width", "n_slots", "prefix_len",
+                                              "q_batch", "q_head", "o_batch", "o_head", "k_page",
+                                              "v_page")] + \
+               [("scale", ctypes.c_float), ("dtype", ctypes.c_int32)] + \
+               [(n, ctypes.c_void_p) for n in ("table", "lens", "slots", "q", "k_pages",
+                                               "v_pages", "out", "workspace")] + \
+               [("workspace_bytes", ctypes.c_size_t)]
+
+
+def _check_int32(name, device, *ts):
+    torch = _torch()
+    for t in ts:
+        if t.dtype != torch.int32 or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"{name}: tables, lengths and slots are contiguous int32 tensors on "
+                             f"the data's device")
+
+
+def sdpa_shared_prefix(q, k_pages, v_pages, table, lens, prefix_len: int = 0, slots=None,
+                       scale: Optional[float] = None, out=None, workspace=None):
+    """One new token per sequence over a paged cache whose sequences share their first tokens.
+
+    q [B, Hq, D]; k_pages / v_pages [pages, Hkv, page, D] (one layer of a cache); table
+    [n, width] int32 page numbers, lens [n] int32; sequence b uses row slots[b] (default: row
+    b).  Sequence b attends to its first lens keys; those below prefix_len are the same for
+    the whole batch and are read once for all, through sequence 0's row.  A sequence without
+    keys gives zeros.  workspace: a uint8 tensor to use instead of an allocation per call
+    (as many bytes as enigma_sdpa_shared_prefix_workspace_bytes says).  Returns out [B, Hq, D].
+    """
+    torch = _torch()
+    if q.dim() != 3 or k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+        raise ValueError("sdpa_shared_prefix: expected q [B, Hq, D] and pages [P, Hkv, page, D]")
+    b, hq, d = q.shape
+    pages, hk, page, dk = k_pages.shape
+    if dk != d:
+        raise ValueError("sdpa_shared_prefix: K/V head_dim does not match Q")
+    if table.dim() != 2 or lens.dim() != 1 or lens.shape[0] != table.shape[0]:
+        raise ValueError("sdpa_shared_prefix: expected table [n, width] and lens [n]")
+    if slots is not None and tuple(slots.shape) != (b,):
+        raise ValueError("sdpa_shared_prefix: slots must name one row per sequence")
+    if out is None:
+        out = torch.empty((b, hq, d), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError("sdpa_shared_prefix: out must have q's shape")
+    dtype = _dtype_code(q)
+    _check_rows("sdpa_shared_prefix", q, k_pages, v_pages, out)
+    for t in (k_pages, v_pages):
+        if t.stride()[1:] != (page * d, d, 1):
+            raise ValueError("sdpa_shared_prefix: a page must be contiguous")
+    _check_int32("sdpa_shared_prefix", q.device, table, lens, *(() if slots is None else (slots,)))
+    desc = _SharedPrefixDesc(b, hq, hk, d, page, pages, table.shape[1], table.shape[0],
+                             int(prefix_len), *q.stride()[:2], *out.stride()[:2],
+                             k_pages.stride(0), v_pages.stride(0),
+                             1.0 / math.sqrt(d) if scale is None else scale, dtype,
+                             table.data_ptr(), lens.data_ptr(),
+                             None if slots is None else slots.data_ptr(), q.data_ptr(),
+                             k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr())
+    if workspace is None:
+        need = ctypes.c_size_t()
+        _native.call("enigma_sdpa_shared_prefix_workspace_bytes", ctypes.byref(desc),
+                     ctypes.byref(need))
+        workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+    elif workspace.device != q.device or not workspace.is_contiguous():
+        raise ValueError("sdpa_shared_prefix: workspace must be contiguous on the data's device")
+    desc.workspace = workspace.data_ptr()
+    desc.workspace_bytes = workspace.numel() * workspace.element_size()
+    _native.call("enigma_sdpa_shared_prefix", ctypes.byref(desc), _stream_ptr(q))
+    return out
+
+
 def synchronize(device_index: int = 0) -> None:
     """Synchronize the device and raise if a kernel reported a device-side timeout."""
     ensure_device(device_index)

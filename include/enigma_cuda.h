@@ -222,6 +222,108 @@ int32_t enigma_decode_layer_bf16_noalloc(const enigma_decode_layer_desc* desc, c
  * no-allocation entry's status word. */
 int32_t enigma_decode_noalloc_check_timeout_path(int64_t polls, void* stream);
 
+/* ---- serving: prompts of different lengths, and a cache in pages ----
+ * (No counterpart in the reference, whose one decode example owns a dense cache of one
+ * sequence, examples/qwen_megakernel.py:228-269.) */
+
+/* Attention over whole prompts packed one after the other: sequence s owns lens_q[s] rows of
+ * q [tokens_q, heads_q, head_dim] and lens_k[s] rows of k, v [tokens_k, heads_kv, head_dim].
+ *   out_i = sum_j softmax_j(scale q_i . k_j) v_j  over the sequence's keys,
+ * with causal j <= i + lens_k[s] - lens_q[s]; query head h reads kv head h / (heads_q /
+ * heads_kv).  A row that sees no key gives zeros and lse -inf.  Token and head strides are
+ * in elements, head_dim is contiguous; lse (may be NULL) is [tokens_q, heads_q], natural log.
+ * Keys of other sequences are never read into a result, whatever they hold; a masked key of a
+ * row's own sequence must be finite in v.
+ *
+ * enigma_sdpa_packed_plan (host only) lays out the work for these lengths, so a batch's layers
+ * share one plan: which thread block does what, evenly, with long rows split over their keys
+ * where there are few.  It writes *n_ints ints into plan[capacity] (plan NULL: only counts),
+ * the first ENIGMA_PACKED_PLAN_HEADER of them the header.  The caller keeps the plan in device
+ * memory (16-byte aligned) and gives the header with every call; a plan that splits rows needs a workspace of
+ * enigma_sdpa_packed_workspace_bytes() bytes, 256-byte aligned. */
+#define ENIGMA_PACKED_PLAN_HEADER 8
+#define ENIGMA_PACKED_TILE_ROWS 128
+int32_t enigma_sdpa_packed_plan(const int64_t* lens_q, const int64_t* lens_k, int64_t n_seqs,
+                                int64_t heads_q, int64_t heads_kv, int32_t causal, int32_t* plan,
+                                int64_t capacity, int64_t* n_ints);
+int32_t enigma_sdpa_packed_workspace_bytes(const int32_t* header, int64_t head_dim, size_t* bytes);
+typedef struct enigma_sdpa_packed_desc {
+  int64_t tokens_q, tokens_k, heads_q, heads_kv, head_dim;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;
+  float scale;
+  int32_t causal, dtype, reserved;
+  int32_t header[ENIGMA_PACKED_PLAN_HEADER];
+  const int32_t* plan;
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+} enigma_sdpa_packed_desc;
+int32_t enigma_sdpa_packed(const enigma_sdpa_packed_desc* desc, void* stream);
+
+/* One new token per sequence over a paged cache: q, out [batch, heads_q, head_dim]; pages
+ * [pages, heads_kv, page, head_dim] (contiguous but for the page strides, in elements);
+ * table [n_slots, table_width] int32 page numbers, lens [n_slots] int32 keys of each sequence;
+ * sequence b uses row slots[b] (slots NULL: row b).  The first prefix_len keys are the same for
+ * the whole batch: they are read once, through the row of sequence 0.  A sequence attends
+ * to its first min(lens, table_width * page) keys; none gives zeros.  page is 16, 32, 64 or
+ * 128; batch <= 4096.  workspace: caller-owned device memory of
+ * enigma_sdpa_shared_prefix_workspace_bytes() bytes, 256-byte aligned. */
+typedef struct enigma_sdpa_shared_prefix_desc {
+  int64_t batch, heads_q, heads_kv, head_dim, page, pages, table_width, n_slots, prefix_len;
+  int64_t q_batch, q_head, o_batch, o_head, k_page, v_page;
+  float scale;
+  int32_t dtype;
+  const int32_t *table, *lens, *slots;
+  const void *q, *k_pages, *v_pages;
+  void *out, *workspace;
+  size_t workspace_bytes;
+} enigma_sdpa_shared_prefix_desc;
+int32_t enigma_sdpa_shared_prefix_workspace_bytes(const enigma_sdpa_shared_prefix_desc* desc,
+                                                  size_t* bytes);
+int32_t enigma_sdpa_shared_prefix(const enigma_sdpa_shared_prefix_desc* desc, void* stream);
+
+/* A paged cache: k, v [layers, pages, heads_kv, page, head_dim]; table [slots, table_width]
+ * (-1: none), lens [slots], refs [pages] (rows that hold the page; 0: free), status [1], all
+ * int32 on the device.  Requests (n entries) are int32 device arrays.  New pages are the lowest
+ * free ones in the order of the request.  A request that cannot be met changes nothing and
+ * sets ENIGMA_CACHE_FULL or ENIGMA_CACHE_BAD_REQUEST in *status (a slot out of range or named
+ * twice, a parent among the children, a length below the current one or past the table).
+ *   fork     children[i] lets go of its pages and continues parents[i]: full pages are
+ *            shared, the valid rows of a partly filled last page are copied to a new page.
+ *   free     the slots let go of their pages.
+ *   reserve  slots[i] grows to lens[i] tokens.
+ *   write    rows of new_k / new_v (strides4: k token, k head, v token, v head, in elements)
+ *            of one layer: rows cu[i] .. cu[i + 1] are tokens starts[i], ... of slots[i];
+ *            a token without a page is left out and sets ENIGMA_CACHE_BAD_REQUEST.
+ *   compact  the n live pages take the numbers below n; rows are rewritten to match.
+ *   copy_pages  whole pages src[i] -> dst[i], all layers; no page both source and destination.
+ * workspace: enigma_kv_cache_workspace_bytes() bytes; calls that share it run in one order. */
+#define ENIGMA_CACHE_FULL 1
+#define ENIGMA_CACHE_BAD_REQUEST 2
+typedef struct enigma_kv_cache_desc {
+  int64_t layers, pages, heads_kv, page, head_dim, elem_bytes, slots, table_width;
+  void *k, *v;
+  int32_t *table, *lens, *refs, *status;
+  void* workspace;
+  size_t workspace_bytes;
+} enigma_kv_cache_desc;
+int32_t enigma_kv_cache_workspace_bytes(const enigma_kv_cache_desc* desc, size_t* bytes);
+int32_t enigma_kv_cache_fork(const enigma_kv_cache_desc* desc, const int32_t* parents,
+                             const int32_t* children, int64_t n, void* stream);
+int32_t enigma_kv_cache_free(const enigma_kv_cache_desc* desc, const int32_t* slots, int64_t n,
+                             void* stream);
+int32_t enigma_kv_cache_reserve(const enigma_kv_cache_desc* desc, const int32_t* slots,
+                                const int32_t* lens, int64_t n, void* stream);
+int32_t enigma_kv_cache_write(const enigma_kv_cache_desc* desc, int64_t layer, const void* new_k,
+                              const void* new_v, const int64_t* strides4, const int32_t* slots,
+                              const int32_t* starts, const int32_t* cu, int64_t n, int64_t tokens,
+                              void* stream);
+int32_t enigma_kv_cache_compact(const enigma_kv_cache_desc* desc, void* stream);
+int32_t enigma_kv_cache_copy_pages(const enigma_kv_cache_desc* desc, const int32_t* src,
+                                   const int32_t* dst, int64_t n, void* stream);
+
 /* ---- generic dispatch by kernel id: replaces enigma_dispatch /
  *      enigma_dispatch_timed (libenigma_runtime.swift:132-214).
  *      grid / threads are Metal-style totals (threads per axis, not groups),
