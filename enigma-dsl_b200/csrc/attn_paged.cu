@@ -1,12 +1,660 @@
 // attn_paged.cu — one new token per sequence over a paged cache with a shared prefix.
-#include "attn_serving.cuh"
+//
+// The prefix is a matrix product: all sequences' heads of a kv head's group against the same
+// keys (attn_tc.cuh, split over the keys so that every SM has a part).  Each sequence's own
+// keys are read once for few rows, which is bound by memory: paged_decode_kernel streams them.
+// Both leave partial results (maximum, sum, unnormalised O); paged_join_kernel joins them.
+#include <algorithm>
+
+#include "attn_tc.cuh"
+
+namespace {
+
+using namespace enigma_tc;
+
+// ============================================================================ own keys
+// The work is the flattened list of (unit, 64-key chunk) pairs, unit = (sequence, kv head, block
+// of up to 16 query heads); CTA c of P takes the contiguous range [c T / P, (c + 1) T / P), so
+// every SM streams the same number of chunks whatever the lengths are.  A producer warp loads
+// chunks by TMA (one box per page and 64 columns) into a ring; four warps take 16 keys of each
+// chunk: S = Q K^T (mma.sync, the heads as the 16-row operand), online softmax, O += P V.  At
+// the end of a unit's run of chunks the warps' states are merged and stored in slot c + u
+// (segments in order advance c or u, so the slots are distinct).
+constexpr int CHUNK = 64;
+constexpr int DWARPS = 4;
+constexpr int DTHREADS = (DWARPS + 1) * 32;
+constexpr int ROWS = 16;                     // query heads of a unit
+
+template <int D>
+struct DCfg {
+  static constexpr int ATOMS = D / 64;
+  static constexpr int TILE = CHUNK * D * 2;            // one of K or V
+  static constexpr int STAGES = D == 64 ? 4 : 3;
+  static constexpr int MERGE = (DWARPS - 1) * 8 * D * 4;
+  static constexpr int SMEM = STAGES * 2 * TILE + MERGE + 1024;   // + (batch + 1) ints
+};
+
+struct DecodeParams {
+  const __nv_bfloat16* q;
+  int64_t q_batch, q_head;
+  const int32_t *table, *lens, *slots;
+  int batch, heads_kv, group, blocks, rows;  // blocks of `rows` <= 16 heads per group
+  int width, n_slots, pages, page_shift, box_shift, prefix, base;
+  float scale_log2;
+  float* opart;                              // [slot][rows][D]
+  float2* ml;                                // [slot][rows]
+  int32_t* starts;                           // [batch + 1] chunks (of one unit) before b
+  uint32_t* status;
+};
+
+// Element c (16 bytes) of row r in a 128-byte-swizzled tile.
+__device__ __forceinline__ uint32_t sw128(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void warps_sync() {   // the DWARPS consumer warps
+  asm volatile("bar.sync 1, %0;" ::"n"(DWARPS * 32) : "memory");
+}
+__device__ __forceinline__ bool warps_all(bool ok) {   // the same, and whether all say yes
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %1, 0;\n\t"
+      "barrier.cta.red.and.pred b, 1, %2, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
+      : "=r"(all) : "r"(ok ? 1u : 0u), "n"(DWARPS * 32) : "memory");
+  return all != 0;
+}
+
+// floor(n c / P) for n c < 2^53 without a 64-bit division.
+__device__ __forceinline__ int64_t share(int64_t n, int64_t c, int64_t P) {
+  const int64_t x = n * c;
+  int64_t q = int64_t(double(x) / double(P));
+  if ((q + 1) * P <= x) ++q;
+  if (q * P > x) --q;
+  return q;
+}
+
+// The CTA that owns chunk x of T over P CTAs.
+__device__ __forceinline__ int owner(int64_t x, int64_t T, int64_t P) {
+  return int(((x + 1) * P - 1) / T);
+}
+
+// Chunks of sequence b's own keys.
+__device__ __forceinline__ int chunks_of(int len, int prefix, int base) {
+  return len > prefix ? (len - base + CHUNK - 1) / CHUNK : 0;
+}
+
+// A run of one unit's chunks.
+struct Segment {
+  int b, kvh, block, unit;
+  int j0, n;                    // first chunk within the unit, number of chunks
+};
+
+// The segment that begins at chunk x of the CTA's range [x, end).  starts[b] * units_per_b is
+// the first chunk of sequence b.
+__device__ __forceinline__ Segment segment_at(const int* starts, int batch, int per_b, int blocks,
+                                              int64_t x, int64_t end) {
+  int lo = 0, hi = batch;       // the last b with starts[b] * per_b <= x
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (int64_t(starts[mid]) * per_b <= x) lo = mid;
+    else hi = mid;
+  }
+  Segment s;
+  s.b = lo;
+  const int n = starts[lo + 1] - starts[lo];
+  const int64_t in_b = x - int64_t(starts[lo]) * per_b;
+  const int u = int(in_b / n);
+  s.j0 = int(in_b - int64_t(u) * n);
+  s.kvh = u / blocks;
+  s.block = u - s.kvh * blocks;
+  s.unit = lo * per_b + u;
+  s.n = int(min(int64_t(n - s.j0), end - x));
+  return s;
+}
+
+template <int D>
+__global__ void __launch_bounds__(DTHREADS)
+paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const DecodeParams p) {
+  using C = DCfg<D>;
+  constexpr int ST = C::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* s_o = reinterpret_cast<float*>(ring + ST * 2 * C::TILE);     // [DWARPS - 1][8][D]
+  int* s_starts = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(s_o) + C::MERGE);
+  __shared__ uint64_t full[ST], empty[ST];
+  __shared__ float s_m[DWARPS][ROWS], s_l[DWARPS][ROWS];
+  __shared__ int s_warp[DWARPS + 1];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t most = int64_t(p.width) << p.page_shift;
+
+  if (tid == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], DWARPS);
+    }
+    fence_barrier_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  // Chunk counts before each sequence.
+  int run = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += DTHREADS) {
+    const int b = b0 + tid;
+    int v = 0;
+    if (b < p.batch)
+      v = chunks_of(len_of(p.lens, p.slots, p.n_slots, most, b), p.prefix, p.base);
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    int before = run;
+    for (int w = 0; w < warp; ++w) before += s_warp[w];
+    if (b < p.batch) s_starts[b] = before + x - v;
+    for (int w = 0; w <= DWARPS; ++w) run += s_warp[w];
+    __syncthreads();
+  }
+  if (tid == 0) s_starts[p.batch] = run;
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int b = tid; b <= p.batch; b += DTHREADS) p.starts[b] = s_starts[b];
+
+  const int per_b = p.heads_kv * p.blocks;
+  const int64_t T = int64_t(run) * per_b;
+  const int64_t P = min(int64_t(gridDim.x), T);
+  if (int64_t(blockIdx.x) >= P) return;
+  const int64_t c0 = share(T, blockIdx.x, P), c1 = share(T, int64_t(blockIdx.x) + 1, P);
+
+  if (warp == DWARPS) {
+    // ---------------------------------------------------------------- producer
+    // Lanes 0 .. 15 load K's boxes, 16 .. 31 V's: box x = rows [(x / ATOMS) << box_shift, ...),
+    // columns 64 (x % ATOMS).
+    const int x = lane & 15, box = x / C::ATOMS, atom = x % C::ATOMS;
+    const bool is_v = lane >= 16;
+    int i = 0;
+    for (int64_t at = c0; at < c1;) {
+      const Segment s = segment_at(s_starts, p.batch, per_b, p.blocks, at, c1);
+      const int len = len_of(p.lens, p.slots, p.n_slots, most, s.b);
+      auto look_up = [&](int j) {
+        const int key = p.base + j * CHUNK + (box << p.box_shift);
+        return page_at(p.table, p.slots, p.n_slots, p.width, p.pages, s.b, key >> p.page_shift);
+      };
+      const bool can = box < (CHUNK >> p.box_shift);
+      int page = can ? look_up(s.j0) : 0;
+      for (int j = s.j0; j < s.j0 + s.n; ++j, ++i) {
+        const int key0 = p.base + j * CHUNK;
+        const int boxes = (min(CHUNK, len - key0) + (1 << p.box_shift) - 1) >> p.box_shift;
+        const int page_now = page;
+        if (can && j + 1 < s.j0 + s.n) page = look_up(j + 1);
+        const int st = i % ST;
+        if (!__all_sync(0xffffffffu, mbar_wait(&empty[st], ((i / ST) & 1) ^ 1, p.status))) {
+          at = c1;
+          break;
+        }
+        if (lane == 0)
+          mbar_arrive_expect_tx(&full[st], (uint32_t(2 * boxes * C::ATOMS) * 128u) << p.box_shift);
+        __syncwarp();
+        if (box < boxes)
+          tma_load_4d(ring + (2 * st + (is_v ? 1 : 0)) * C::TILE + atom * CHUNK * 128 +
+                          ((box << p.box_shift) * 128),
+                      is_v ? &tmV : &tmK, &full[st], atom * 64,
+                      (key0 + (box << p.box_shift)) & ((1 << p.page_shift) - 1), s.kvh, page_now);
+        __syncwarp();
+      }
+      at += s.n;
+    }
+    return;
+  }
+
+  // ------------------------------------------------------------------ consumers
+  const int g = lane >> 2, quad = lane & 3;
+  int i = 0;
+  for (int64_t at = c0; at < c1;) {
+    const Segment s = segment_at(s_starts, p.batch, per_b, p.blocks, at, c1);
+    const int len = len_of(p.lens, p.slots, p.n_slots, most, s.b);
+    const int rows = min(p.rows, p.group - s.block * p.rows);
+    uint32_t q[D / 16][4];
+    {
+      const __nv_bfloat16* qb = p.q + s.b * p.q_batch +
+                                int64_t(s.kvh * p.group + s.block * p.rows) * p.q_head;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = g + (e & 1) * 8, d = kk * 16 + quad * 2 + (e >> 1) * 8;
+          q[kk][e] = row < rows ? *reinterpret_cast<const uint32_t*>(qb + row * p.q_head + d) : 0u;
+        }
+    }
+    float o[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    bool ok = true;
+    for (int j = s.j0; j < s.j0 + s.n; ++j, ++i) {
+      const int st = i % ST;
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[st], (i / ST) & 1, p.status));
+      if (!ok) break;
+      uint8_t* tile_k = ring + 2 * st * C::TILE;
+      uint8_t* tile_v = tile_k + C::TILE;
+      const int key0 = p.base + j * CHUNK + warp * 16;      // this warp's first key
+      float sc[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+      const int mi = lane >> 3, mr = lane & 7;              // ldmatrix: matrix, row
+      const uint32_t ka = smem_u32(tile_k);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t b[4];
+        ldsm_x4(ka + (kk / 4) * CHUNK * 128 +
+                    sw128(warp * 16 + (mi >> 1) * 8 + mr, (kk % 4) * 2 + (mi & 1)), b);
+        mma_16816(sc[0], q[kk], b[0], b[1]);
+        mma_16816(sc[1], q[kk], b[2], b[3]);
+      }
+      if (key0 + 16 > len || key0 < p.prefix) {             // warp-uniform
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + n * 8 + quad * 2 + (e & 1);
+            if (key >= len || key < p.prefix) sc[n][e] = -INFINITY;
+          }
+        // Rows past the end hold whatever the page or the ring held, rows of the prefix
+        // whatever this sequence's page has there: 0 * NaN must not be.
+        for (int x = lane; x < 16 * 8 * C::ATOMS; x += 32) {
+          const int row = x >> 3 & 15;
+          if (key0 + row >= len || key0 + row < p.prefix)
+            *reinterpret_cast<uint4*>(tile_v + (x >> 7) * CHUNK * 128 + (warp * 16 + row) * 128 +
+                                      (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();                           // before the next TMA write here
+        __syncwarp();
+      }
+      float mc[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {                         // rows g and g + 8
+        float mx = max3f(max3f(sc[0][2 * h], sc[0][2 * h + 1], sc[1][2 * h]), sc[1][2 * h + 1], m[h]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        mc[h] = mx == -INFINITY ? 0.f : mx * p.scale_log2;
+        const float f = ex2(m[h] * p.scale_log2 - mc[h]);   // m = -inf: 0
+        m[h] = mx;
+        l[h] *= f;
+        if (__any_sync(0xffffffffu, f != 1.f)) {
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            o[n][2 * h] *= f;
+            o[n][2 * h + 1] *= f;
+          }
+        }
+      }
+      uint32_t pa[4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float e0 = ex2(fmaf(sc[n][2 * h], p.scale_log2, -mc[h]));
+          const float e1 = ex2(fmaf(sc[n][2 * h + 1], p.scale_log2, -mc[h]));
+          l[h] += e0 + e1;                                  // this lane's share of the row's sum
+          pa[2 * n + h] = pack_bf16x2(e0, e1);
+        }
+      const uint32_t va = smem_u32(tile_v);
+#pragma unroll
+      for (int dd = 0; dd < D / 16; ++dd) {
+        uint32_t b[4];
+        ldsm_x4_trans(va + (dd / 4) * CHUNK * 128 +
+                          sw128(warp * 16 + (mi & 1) * 8 + mr, (dd % 4) * 2 + (mi >> 1)), b);
+        mma_16816(o[2 * dd], pa, b[0], b[1]);
+        mma_16816(o[2 * dd + 1], pa, b[2], b[3]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+    if (!warps_all(ok)) return;                             // a wait ran out (status is set)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      if (quad == 0) {
+        s_m[warp][g + 8 * h] = m[h] == -INFINITY ? -INFINITY : m[h] * p.scale_log2;
+        s_l[warp][g + 8 * h] = l[h];
+      }
+    }
+    // Merge the warps' states, 8 rows at a time: the others' through shared memory to warp 0.
+    const int64_t slot = int64_t(blockIdx.x) + s.unit;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (h * 8 >= rows) break;                             // uniform
+      if (warp > 0) {
+        float* mine = s_o + ((warp - 1) * 8 + g) * D + quad * 2;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+          *reinterpret_cast<float2*>(mine + n * 8) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+      }
+      warps_sync();
+      if (warp == 0) {
+        const int row = g + 8 * h;
+        float M = s_m[0][row];
+#pragma unroll
+        for (int w = 1; w < DWARPS; ++w) M = fmaxf(M, s_m[w][row]);
+        float f[DWARPS], L = 0.f;
+#pragma unroll
+        for (int w = 0; w < DWARPS; ++w) {
+          f[w] = s_m[w][row] == -INFINITY ? 0.f : ex2(s_m[w][row] - M);
+          L = fmaf(s_l[w][row], f[w], L);
+        }
+        if (row < rows) {
+          float* to = p.opart + (slot * p.rows + row) * D + quad * 2;
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            float a = o[n][2 * h] * f[0], b = o[n][2 * h + 1] * f[0];
+#pragma unroll
+            for (int w = 1; w < DWARPS; ++w) {
+              const float2 v = *reinterpret_cast<const float2*>(s_o + ((w - 1) * 8 + g) * D +
+                                                                quad * 2 + n * 8);
+              a = fmaf(v.x, f[w], a);
+              b = fmaf(v.y, f[w], b);
+            }
+            *reinterpret_cast<float2*>(to + n * 8) = make_float2(a, b);
+          }
+          if (quad == 0) p.ml[slot * p.rows + row] = make_float2(M, L);
+        }
+      }
+      warps_sync();
+    }
+    at += s.n;
+  }
+}
+
+// ============================================================================ join
+struct JoinParams {
+  __nv_bfloat16* out;
+  int64_t o_batch, o_head;
+  int batch, heads_q, heads_kv, group;
+  // prefix: pairs x splits items, two states each (0 splits: no prefix)
+  const float* p_opart;
+  const float2* p_ml;
+  int pairs, splits, row_tiles, tokens;
+  // own keys
+  const float* d_opart;
+  const float2* d_ml;
+  const int32_t* starts;
+  int blocks, rows, ctas;
+};
+
+// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a row's partial results, always in the
+// same order.  One warp per (sequence, query head).
+template <int D>
+__global__ void __launch_bounds__(128) paged_join_kernel(const JoinParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t id = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (id >= int64_t(p.batch) * p.heads_q) return;
+  const int b = int(id / p.heads_q), h = int(id - int64_t(b) * p.heads_q);
+  const int kvh = h / p.group, gh = h - kvh * p.group;
+  // Prefix partials: rows pf + i * p_step of [slot * 128 + row].
+  int n_p = 0;
+  int64_t p_at = 0, p_step = 0;
+  if (p.splits > 0) {
+    const int tile = b / p.tokens, pair = tile >> 1;
+    const bool alt = 2 * pair + 1 >= p.row_tiles;
+    const int row = (b - tile * p.tokens) * p.group + gh;
+    const int64_t slot = int64_t(kvh * p.pairs + pair) * p.splits * 2 + (alt ? 0 : (tile & 1));
+    n_p = alt ? 2 * p.splits : p.splits;
+    p_step = (alt ? 1 : 2) * BM;
+    p_at = slot * BM + row;
+  }
+  // Own partials: the slots of the CTAs that hold the unit's chunks.
+  int n_d = 0;
+  int64_t d_at = 0;
+  const int per_b = p.heads_kv * p.blocks;
+  const int64_t T = int64_t(p.starts[p.batch]) * per_b;
+  const int n = p.starts[b + 1] - p.starts[b];
+  if (n > 0) {
+    const int block = gh / p.rows, u = kvh * p.blocks + block;
+    const int64_t x0 = int64_t(p.starts[b]) * per_b + int64_t(u) * n;
+    const int64_t P = min(int64_t(p.ctas), T);
+    const int first = owner(x0, T, P), last = owner(x0 + n - 1, T, P);
+    n_d = last - first + 1;
+    d_at = (int64_t(first) + b * per_b + u) * p.rows + (gh - block * p.rows);
+  }
+  float M = -INFINITY;
+  for (int i = lane; i < n_p; i += 32) M = fmaxf(M, p.p_ml[p_at + i * p_step].x);
+  for (int i = lane; i < n_d; i += 32) M = fmaxf(M, p.d_ml[d_at + int64_t(i) * p.rows].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  constexpr int V = D / 32;
+  float acc[V] = {};
+  float l = 0.f;
+  auto add = [&](const float2* ml, const float* opart, int64_t at) {
+    const float2 x = ml[at];
+    if (x.x == -INFINITY) return;                           // this part saw no key
+    const float f = ex2(x.x - M);
+    l = fmaf(x.y, f, l);
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = fmaf(opart[at * D + lane * V + v], f, acc[v]);
+  };
+  for (int i = 0; i < n_p; ++i) add(p.p_ml, p.p_opart, p_at + i * p_step);
+  for (int i = 0; i < n_d; ++i) add(p.d_ml, p.d_opart, d_at + int64_t(i) * p.rows);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __nv_bfloat16* out = p.out + b * p.o_batch + h * p.o_head + lane * V;
+#pragma unroll
+  for (int v = 0; v < V; v += 2)
+    *reinterpret_cast<uint32_t*>(out + v) = pack_bf16x2(acc[v] * inv, acc[v + 1] * inv);
+}
+
+// ============================================================================ host
+bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// The tensor-core kernels take bf16 heads of 64 or 128 whose rows TMA can address (base and
+// strides multiples of 16 bytes), and a group that fits a tile.
+bool tc_takes(const enigma_sdpa_shared_prefix_desc& d) {
+  const int64_t st[6] = {d.q_batch, d.q_head, d.o_batch, d.o_head, d.k_page, d.v_page};
+  for (int i = 0; i < 6; ++i)
+    if (st[i] % 8 != 0 || st[i] <= 0 || st[i] >= (int64_t(1) << 39)) return false;
+  return d.dtype == ENIGMA_DTYPE_BF16 && (d.head_dim == 64 || d.head_dim == 128) &&
+         d.heads_q / d.heads_kv <= BM && aligned_to(d.q, 16) && aligned_to(d.k_pages, 16) &&
+         aligned_to(d.v_pages, 16) && aligned_to(d.out, 16);
+}
+
+int log2_of(int64_t x) {
+  int n = 0;
+  while ((int64_t(1) << n) < x) ++n;
+  return n;
+}
+
+struct Layout {
+  int group, tokens, row_tiles, pairs, splits, prefix;    // prefix part
+  int blocks, rows, ctas;                                 // own part
+  size_t p_opart, p_ml, d_opart, d_ml, starts, total;     // byte offsets
+};
+
+Layout layout_of(const enigma_sdpa_shared_prefix_desc& d) {
+  Layout y = {};
+  const int sms = enigma::sm_count();
+  y.group = int(d.heads_q / d.heads_kv);
+  y.tokens = std::max(1, BM / y.group);
+  // One sequence shares its prefix with nobody.
+  y.prefix = d.batch > 1 ? int(d.prefix_len) : 0;
+  y.row_tiles = int((d.batch + y.tokens - 1) / y.tokens);
+  y.pairs = (y.row_tiles + 1) / 2;
+  const int tiles = (y.prefix + BN - 1) / BN;
+  if (tiles > 0) {
+    // As many parts of the keys as there are SMs, each at least two tiles.
+    const int64_t units = int64_t(d.heads_kv) * y.pairs;
+    y.splits = int(std::max<int64_t>(1, std::min<int64_t>(sms / std::max<int64_t>(units, 1),
+                                                          (tiles + 1) / 2)));
+  }
+  const int64_t p_slots = int64_t(d.heads_kv) * y.pairs * y.splits * 2;
+  y.blocks = (y.group + ROWS - 1) / ROWS;
+  y.rows = (y.group + y.blocks - 1) / y.blocks;
+  y.ctas = sms * (d.head_dim == 64 ? 3 : 2);
+  const int64_t d_slots = int64_t(y.ctas) + d.batch * d.heads_kv * y.blocks;
+  size_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const size_t here = at;
+    at += (size_t(bytes) + 255) & ~size_t(255);
+    return here;
+  };
+  y.p_opart = take(p_slots * BM * d.head_dim * 4);
+  y.p_ml = take(p_slots * BM * 8);
+  y.d_opart = take(d_slots * y.rows * d.head_dim * 4);
+  y.d_ml = take(d_slots * y.rows * 8);
+  y.starts = take((d.batch + 1) * 4);
+  y.total = at;
+  return y;
+}
+
+bool pages_map(CUtensorMap* m, const void* base, const enigma_sdpa_shared_prefix_desc& d,
+               int64_t page_stride, int box_rows) {
+  const cuuint64_t dims[4] = {cuuint64_t(d.head_dim), cuuint64_t(d.page), cuuint64_t(d.heads_kv),
+                              cuuint64_t(d.pages)};
+  const cuuint64_t strides[3] = {cuuint64_t(d.head_dim * 2), cuuint64_t(d.page * d.head_dim * 2),
+                                 cuuint64_t(page_stride * 2)};
+  const cuuint32_t box[4] = {64, cuuint32_t(box_rows), 1, 1};
+  return make_map(m, base, 4, dims, strides, box);
+}
+
+template <int D>
+cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
+  const Layout y = layout_of(d);
+  uint8_t* ws = static_cast<uint8_t*>(d.workspace);
+  uint32_t* status = enigma::device_status();
+  if (status == nullptr) return cudaErrorMemoryAllocation;      // the bounded waits need it
+  const int box_rows = int(std::min<int64_t>(d.page, 64));
+  CUtensorMap mk, mv;
+  if (!pages_map(&mk, d.k_pages, d, d.k_page, box_rows) ||
+      !pages_map(&mv, d.v_pages, d, d.v_page, box_rows))
+    return cudaErrorInvalidValue;
+  const float scale_log2 = d.scale * 1.4426950408889634f;
+  const int page_shift = log2_of(d.page), box_shift = log2_of(box_rows);
+  cudaError_t e;
+  if (y.splits > 0) {
+    CUtensorMap mq;
+    const cuuint64_t dims[3] = {cuuint64_t(D), cuuint64_t(d.heads_q), cuuint64_t(d.batch)};
+    const cuuint64_t strides[2] = {cuuint64_t(d.q_head * 2), cuuint64_t(d.q_batch * 2)};
+    const cuuint32_t box[3] = {64, cuuint32_t(y.group), cuuint32_t(y.tokens)};
+    if (!make_map(&mq, d.q, 3, dims, strides, box)) return cudaErrorInvalidValue;
+    e = prepare_kernel<D, true>();
+    if (e != cudaSuccess) return e;
+    Params p = {};
+    p.scale_log2 = scale_log2;
+    p.group = y.group;
+    p.tokens = y.tokens;
+    p.status = status;
+    p.opart = reinterpret_cast<float*>(ws + y.p_opart);
+    p.ml = reinterpret_cast<float2*>(ws + y.p_ml);
+    p.table = d.table;
+    p.lens = d.lens;
+    p.slots = d.slots;
+    p.width = int(d.table_width);
+    p.n_slots = int(d.n_slots);
+    p.pages = int(d.pages);
+    p.page_shift = page_shift;
+    p.box_shift = box_shift;
+    p.prefix = y.prefix;
+    p.batch = int(d.batch);
+    p.heads_kv = int(d.heads_kv);
+    p.pairs = y.pairs;
+    p.splits = y.splits;
+    p.row_tiles = y.row_tiles;
+    const int items = int(d.heads_kv) * y.pairs * y.splits;
+    attn_tc_kernel<D, true><<<unsigned(items), THREADS, Cfg<D>::SMEM, s>>>(mq, mk, mv, p, items);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  DecodeParams p = {};
+  p.q = static_cast<const __nv_bfloat16*>(d.q);
+  p.q_batch = d.q_batch;
+  p.q_head = d.q_head;
+  p.table = d.table;
+  p.lens = d.lens;
+  p.slots = d.slots;
+  p.batch = int(d.batch);
+  p.heads_kv = int(d.heads_kv);
+  p.group = y.group;
+  p.blocks = y.blocks;
+  p.rows = y.rows;
+  p.width = int(d.table_width);
+  p.n_slots = int(d.n_slots);
+  p.pages = int(d.pages);
+  p.page_shift = page_shift;
+  p.box_shift = box_shift;
+  p.prefix = y.prefix;
+  p.base = y.prefix / CHUNK * CHUNK;
+  p.scale_log2 = scale_log2;
+  p.opart = reinterpret_cast<float*>(ws + y.d_opart);
+  p.ml = reinterpret_cast<float2*>(ws + y.d_ml);
+  p.starts = reinterpret_cast<int32_t*>(ws + y.starts);
+  p.status = status;
+  const int smem = DCfg<D>::SMEM + int(d.batch + 1) * 4;
+  e = cudaFuncSetAttribute(paged_decode_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           DCfg<D>::SMEM + 4097 * 4);
+  if (e != cudaSuccess) return e;
+  paged_decode_kernel<D><<<unsigned(y.ctas), DTHREADS, smem, s>>>(mk, mv, p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  JoinParams j = {};
+  j.out = static_cast<__nv_bfloat16*>(d.out);
+  j.o_batch = d.o_batch;
+  j.o_head = d.o_head;
+  j.batch = int(d.batch);
+  j.heads_q = int(d.heads_q);
+  j.heads_kv = int(d.heads_kv);
+  j.group = y.group;
+  j.p_opart = reinterpret_cast<const float*>(ws + y.p_opart);
+  j.p_ml = reinterpret_cast<const float2*>(ws + y.p_ml);
+  j.pairs = y.pairs;
+  j.splits = y.splits;
+  j.row_tiles = y.row_tiles;
+  j.tokens = y.tokens;
+  j.d_opart = p.opart;
+  j.d_ml = p.ml;
+  j.starts = p.starts;
+  j.blocks = y.blocks;
+  j.rows = y.rows;
+  j.ctas = y.ctas;
+  const unsigned grid = unsigned((d.batch * d.heads_q + 3) / 4);
+  paged_join_kernel<D><<<grid, 128, 0, s>>>(j);
+  return cudaGetLastError();
+}
+
+}  // namespace
 
 namespace enigma {
 
-size_t sdpa_shared_prefix_workspace(const enigma_sdpa_shared_prefix_desc&) { return 0; }
+size_t sdpa_shared_prefix_workspace(const enigma_sdpa_shared_prefix_desc& d) {
+  return d.batch > 0 && (d.head_dim == 64 || d.head_dim == 128) &&
+                 d.dtype == ENIGMA_DTYPE_BF16 && d.heads_q / d.heads_kv <= BM
+             ? layout_of(d).total
+             : 0;
+}
 
 cudaError_t sdpa_shared_prefix_launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
-  return sdpa_paged_simt_launch(d, s);
+  if (!tc_takes(d)) return sdpa_paged_simt_launch(d, s);
+  note_kernel(d.prefix_len > 0 && d.batch > 1 ? "attn_tc_kernel" : "paged_decode_kernel");
+  return d.head_dim == 128 ? launch<128>(d, s) : launch<64>(d, s);
 }
 
 }  // namespace enigma

@@ -1,0 +1,676 @@
+// attn_tc.cuh — attention on the sm_100a tensor cores for the serving operators.
+//
+//   O_r = sum_j softmax_j(scale q_r . k_j) v_j,   keys j < lim(r)
+//
+// A row r is one (token, query head) of a kv head's group: a tile takes `tokens` = 128 / G
+// tokens with all G heads of their group, so every row of a tile reads the same K and V, a
+// short sequence does not pay a tile per head, and a causal tile's rows end within
+// `tokens` keys of each other.  A work item is two row tiles (256 rows) of one kv head and a
+// range of 128-key tiles; or one row tile twice (alt), the even key tiles with one softmax
+// state and the odd ones with the other, when there is no second row tile to fill the SM.
+//
+//   warp 0      TMA: both Q tiles, then K and V tiles into rings of C::STAGES
+//   warp 1      one thread issues tcgen05.mma, S_i = Q_i K_j^T and O_i += P_i V_j (P from
+//               TMEM over S_i's columns), PV_0 S_0 PV_1 S_1 in turn, so the tensor core works
+//               for one tile while the other's softmax runs
+//   warp 2      clears V rows past the sequence's end: what lies behind it (a neighbour's
+//               tokens, a page's unwritten rows) may be NaN, and 0 * NaN would reach the sum
+//   warps 4-7, 8-11   softmax of the two tiles, one thread per row, fp32
+//
+// The softmax takes the running maximum that the tiles before left and starts its exponentials
+// at once; this tile's maximum is found beside them (they do not depend on it) and only has to
+// show that no weight exceeds 2^kGrow.  If one does, O and the sum are rescaled and the tile's
+// exponentials are done again.  Any base within fp32's range gives the same quotient, so this
+// is exact; it takes the row maximum (400 to 450 cycles of 128 dependent comparisons) out of
+// the chain S -> P -> PV -> S that bounds this kernel.
+//
+// P is rounded to bf16, the operand type of the PV product; sums, maxima and O stay fp32.
+// Every mbarrier wait is bounded (sm100.cuh).
+#pragma once
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "attn_serving.cuh"
+
+namespace enigma_tc {
+
+using namespace enigma_sm100;
+
+constexpr int BM = 128;            // rows per tile (two tiles per item)
+constexpr int BN = 128;            // keys per tile
+constexpr int THREADS = 384;       // warpgroup 0: TMA, MMA, V tail, idle; WG 1, 2: softmax
+// Register split: 384 x 168 at launch; warpgroup 0 drops to 104, the softmax warpgroups rise to
+// 200: 128 * 104 + 256 * 200 = 384 * 168 exactly.
+constexpr int LAUNCH_REGS = 168, WG0_REGS = 104, SOFTMAX_REGS = 200;
+static_assert(128 * WG0_REGS + 256 * SOFTMAX_REGS <= THREADS * LAUNCH_REGS, "register split");
+constexpr float kGrow = 24.f;      // log2 units a weight may exceed 1 by before a rescale
+
+template <int D>
+struct Cfg {
+  static constexpr int STAGES = D == 64 ? 4 : 2;
+  static constexpr int Q_BYTES = BM * D * 2;
+  static constexpr int KV_BYTES = BN * D * 2;
+  static constexpr int ATOMS = D / 64;           // 128-byte swizzle atoms along D
+  static constexpr int SMEM = 2 * Q_BYTES + 2 * STAGES * KV_BYTES + 1024 + 512;
+  static constexpr uint32_t TMEM_COLS = 512;     // S0 | S1 | O0 | O1
+  static constexpr uint32_t O_COL = 2 * BN;
+};
+
+struct Params {
+  float scale_log2;
+  int group, tokens;               // G, tokens per row tile (G * tokens <= 128)
+  uint32_t* status;
+  float* opart;                    // [slot][128][D] fp32, not normalised
+  float2* ml;                      // [slot][128] (maximum in log2 units, sum)
+  // packed prompts
+  const int32_t *offsets, *list;   // each CTA's range of items, the items
+  __nv_bfloat16* out;
+  float* lse;
+  int64_t o_token, o_head;
+  int heads_q, causal, tokens_q, tokens_k;
+  // paged prefix
+  const int32_t *table, *lens, *slots;
+  int width, n_slots, pages, page_shift, box_shift, prefix, batch, heads_kv;
+  int pairs, splits, row_tiles;
+};
+
+// One item, as every role sees it.
+struct Work {
+  int tok0, tok_end;     // first token of tile 0; end of the sequence (batch)
+  int kvh, k0, lk;       // kv head, first key row, number of keys
+  int off;               // a token's keys: min(lk, token - seq0 + off); off >= lk: all
+  int seq0;
+  int j0;                // first key tile
+  int cnt0, cnt1;        // key tiles of each softmax state
+  int all;               // key tiles streamed
+  bool alt;
+  int slot;              // first partial slot, or -1: final result
+};
+
+template <bool PAGED>
+__device__ __forceinline__ Work make_work(const Params& p, int t) {
+  Work w;
+  if (PAGED) {
+    const int split = t % p.splits, unit = t / p.splits;
+    const int pair = unit % p.pairs;
+    w.kvh = unit / p.pairs;
+    w.tok0 = pair * 2 * p.tokens;
+    w.tok_end = p.batch;
+    w.seq0 = 0;
+    w.k0 = 0;
+    w.lk = p.prefix;
+    w.off = p.prefix;
+    const int tiles = (p.prefix + BN - 1) / BN;
+    w.j0 = int(int64_t(tiles) * split / p.splits);
+    w.all = int(int64_t(tiles) * (split + 1) / p.splits) - w.j0;
+    w.alt = 2 * pair + 1 >= p.row_tiles;
+    w.cnt0 = w.alt ? (w.all + 1) / 2 : w.all;
+    w.cnt1 = w.alt ? w.all / 2 : w.all;
+    w.slot = 2 * t;
+  } else {
+    const int4* it = reinterpret_cast<const int4*>(p.list) +
+                     int64_t(t) * (enigma_serving::kItemInts / 4);
+    const int4 a = __ldg(it), b = __ldg(it + 1), c = __ldg(it + 2);
+    // q0 lq k0 lk | t0 tokens j0 j1 | kvh alt slot -
+    w.seq0 = a.x;
+    w.tok0 = a.x + b.x;
+    w.tok_end = a.x + a.y;
+    w.k0 = a.z;
+    w.lk = a.w;
+    w.off = p.causal ? a.w - a.y + 1 : a.w;
+    w.kvh = c.x;
+    w.alt = c.y != 0;
+    w.slot = c.z;
+    w.j0 = b.z;
+    if (w.alt) {
+      w.all = max(b.w - b.z, 0);
+      w.cnt0 = (w.all + 1) / 2;
+      w.cnt1 = w.all / 2;
+    } else {
+      auto tiles = [&](int first) {
+        const int last = min(first + p.tokens, w.tok_end) - 1;
+        const int keys = p.causal ? min(w.lk, last - w.seq0 + w.off) : w.lk;
+        const int end = first < w.tok_end && keys > 0 ? (keys + BN - 1) / BN : 0;
+        return max(min(end, b.w) - b.z, 0);
+      };
+      w.cnt0 = tiles(w.tok0);
+      w.cnt1 = tiles(w.tok0 + p.tokens);
+      w.all = max(w.cnt0, w.cnt1);
+    }
+  }
+  return w;
+}
+
+// ------------------------------------------------------------------ packed fp32 math
+__device__ __forceinline__ float2 f2fma(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+      "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 f2add(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "add.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 4-D tiled load (pages: head_dim, row, kv head, page).
+__device__ __forceinline__ void tma_load_4d(void* dst, const void* desc, uint64_t* bar, int32_t c0,
+                                            int32_t c1, int32_t c2, int32_t c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(desc)), "r"(smem_u32(bar)), "r"(c0),
+        "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// The number of a page, or `pages` (out of the tensor map's range: reads as zeros) where the
+// table holds none.
+__device__ __forceinline__ int page_at(const int32_t* table, const int32_t* slots, int n_slots,
+                                       int width, int pages, int seq, int col) {
+  const int slot = slots != nullptr ? slots[seq] : seq;
+  if (slot < 0 || slot >= n_slots || col >= width) return pages;
+  const int at = table[int64_t(slot) * width + col];
+  return at < 0 || at >= pages ? pages : at;
+}
+
+// Keys of sequence b.
+__device__ __forceinline__ int len_of(const int32_t* lens, const int32_t* slots, int n_slots,
+                                      int64_t most, int b) {
+  const int slot = slots != nullptr ? slots[b] : b;
+  if (slot < 0 || slot >= n_slots) return 0;
+  const int n = lens[slot];
+  return n < 0 ? 0 : int(n < most ? n : most);
+}
+
+template <int D, bool PAGED>
+__global__ void __launch_bounds__(THREADS, 1)
+attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+               const __grid_constant__ CUtensorMap tmV, const Params p, const int items) {
+  using C = Cfg<D>;
+  constexpr int ST = C::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                                   // Q0 | Q1
+  uint8_t* sK = sQ + 2 * C::Q_BYTES;
+  uint8_t* sV = sK + ST * C::KV_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * C::KV_BYTES);
+  uint64_t* q_full = bars;                   // [1]
+  uint64_t* q_empty = q_full + 1;            // [1] the item's last S product has read Q
+  uint64_t* k_full = q_empty + 1;            // [ST]
+  uint64_t* k_empty = k_full + ST;
+  uint64_t* v_full = k_empty + ST;
+  uint64_t* v_empty = v_full + ST;
+  uint64_t* v_tail = v_empty + ST;           // [ST] a sequence's last V tile has landed
+  uint64_t* s_full = v_tail + ST;            // [2] one per softmax state
+  uint64_t* p_full = s_full + 2;             // [2 states][2 halves of the keys]
+  uint64_t* o_done = p_full + 4;             // [2]
+  uint64_t* o_free = o_done + 2;             // [2] the epilogue has read O_i
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 2);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  // Packed: the plan lists each CTA's items.  Paged: one item per CTA.
+  const int t_begin = PAGED ? int(blockIdx.x) : __ldg(p.offsets + blockIdx.x);
+  const int t_end = PAGED ? min(t_begin + 1, items) : __ldg(p.offsets + blockIdx.x + 1);
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+      mbar_init(&v_tail[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[2 * i], 128);
+      mbar_init(&p_full[2 * i + 1], 128);
+      mbar_init(&o_done[i], 1);
+      mbar_init(&o_free[i], 128);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(WG0_REGS));
+    if (warp == 0) {
+      // ------------------------------------------------------------ TMA producer
+      int jg = 0, it = 0;                    // key tiles loaded so far; items with work
+      bool ok = true;
+      const uint32_t q_bytes = uint32_t(p.group * p.tokens) * 128u;   // one atom of a Q tile
+      for (int t = t_begin; t < t_end && ok; ++t) {
+        const Work w = make_work<PAGED>(p, t);
+        if (w.all == 0) continue;
+        if (it > 0 && !__all_sync(0xffffffffu, mbar_wait(q_empty, (it - 1) & 1, p.status))) break;
+        const int q_tiles = w.alt ? 1 : 2;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(q_full, q_bytes * C::ATOMS * q_tiles);
+          for (int i = 0; i < q_tiles; ++i)
+#pragma unroll
+            for (int a = 0; a < C::ATOMS; ++a)
+              tma_load_3d(sQ + i * C::Q_BYTES + a * BM * 128, &tmQ, q_full, a * 64,
+                          w.kvh * p.group, w.tok0 + i * p.tokens);
+        }
+        // Paged: lane x loads box x of each tile, rows [(x / ATOMS) << box_shift, ...), atom
+        // x % ATOMS; the page number of the next tile is read one tile ahead.
+        const int box = PAGED ? lane / C::ATOMS : 0, atom = PAGED ? lane % C::ATOMS : 0;
+        int at = 0, row_in_page = 0;
+        auto look_up = [&](int j) {
+          const int key = j * BN + (box << p.box_shift);
+          row_in_page = key & ((1 << p.page_shift) - 1);
+          at = page_at(p.table, p.slots, p.n_slots, p.width, p.pages, 0, key >> p.page_shift);
+        };
+        if (PAGED && box < (BN >> p.box_shift)) look_up(w.j0);
+        for (int j = 0; j < w.all; ++j, ++jg) {
+          const int s = jg % ST;
+          const uint32_t ph = (jg / ST) & 1;
+          const int key0 = (w.j0 + j) * BN;
+          const int at_now = at, row_now = row_in_page;
+          int boxes = 0;
+          bool mine = false;
+          if (PAGED) {
+            boxes = (min(BN, w.lk - key0) + (1 << p.box_shift) - 1) >> p.box_shift;
+            mine = box < boxes;
+            if (j + 1 < w.all && box < (BN >> p.box_shift)) look_up(w.j0 + j + 1);
+          }
+          const uint32_t bytes = PAGED ? (uint32_t(boxes * C::ATOMS) * 128u) << p.box_shift
+                                       : uint32_t(C::KV_BYTES);
+          auto load = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* full, uint64_t* empty) {
+            if (!__all_sync(0xffffffffu, mbar_wait(empty, ph ^ 1, p.status))) return false;
+            if (lane == 0) mbar_arrive_expect_tx(full, bytes);
+            __syncwarp();
+            if (PAGED) {
+              if (mine)
+                tma_load_4d(dst + atom * BN * 128 + ((box << p.box_shift) * 128), map, full,
+                            atom * 64, row_now, w.kvh, at_now);
+            } else if (lane == 0) {
+#pragma unroll
+              for (int a = 0; a < C::ATOMS; ++a)
+                tma_load_3d(dst + a * BN * 128, map, full, a * 64, w.kvh, w.k0 + key0);
+            }
+            __syncwarp();
+            return true;
+          };
+          // A last V tile with rows past the end goes to warp 2 first.
+          uint64_t* v_bar = key0 + BN > w.lk ? &v_tail[s] : &v_full[s];
+          if (!load(&tmK, sK + s * C::KV_BYTES, &k_full[s], &k_empty[s]) ||
+              !load(&tmV, sV + s * C::KV_BYTES, v_bar, &v_empty[s])) {
+            ok = false;
+            break;
+          }
+        }
+        ++it;
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer
+      if (lane == 0) {
+        constexpr uint32_t idesc_s = idesc_bf16_f32(BM, BN, false, false);
+        constexpr uint32_t idesc_o = idesc_bf16_f32(BM, D, false, true);
+        const uint32_t q_addr = smem_u32(sQ), k_addr = smem_u32(sK), v_addr = smem_u32(sV);
+        int jg = 0, it = 0;
+        int pv_g[2] = {0, 0}, acc_items[2] = {0, 0};
+        bool ok = true;
+        for (int t = t_begin; t < t_end && ok; ++t) {
+          const Work w = make_work<PAGED>(p, t);
+          if (w.all == 0) continue;
+          const int step = w.alt ? 2 : 1;
+          if (!mbar_wait(q_full, it & 1, p.status)) break;
+          auto issue_s = [&](int i, int st) {
+            const int s = st % ST;
+            const uint32_t s_tmem = tmem + uint32_t(i * BN);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t offq = (w.alt ? 0 : i) * C::Q_BYTES + (kk / 4) * (BM * 128) + (kk % 4) * 32;
+              const uint32_t offk = s * C::KV_BYTES + (kk / 4) * (BN * 128) + (kk % 4) * 32;
+              mma_bf16_ss(s_tmem, smem_desc_sw128(q_addr + offq, 16, 1024),
+                          smem_desc_sw128(k_addr + offk, 16, 1024), idesc_s, kk != 0 ? 1u : 0u);
+            }
+            mma_commit(&s_full[i]);
+          };
+          // P arrives in two halves of the keys, so the first half's products start while the
+          // softmax finishes the second.  An item's first PV overwrites O_i: it waits until
+          // the previous item's epilogue has read it.
+          auto issue_pv = [&](int i, int j, int st) -> bool {
+            const int s = st % ST;
+            if (!mbar_wait(&v_full[s], (st / ST) & 1, p.status)) return false;
+            if (j == 0 && acc_items[i] > 0 &&
+                !mbar_wait(&o_free[i], (acc_items[i] - 1) & 1, p.status))
+              return false;
+            const uint32_t p_tmem = tmem + uint32_t(i * BN);
+            const uint64_t dv = smem_desc_sw128(v_addr + s * C::KV_BYTES, BN * 128, 1024);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (!mbar_wait(&p_full[2 * i + half], pv_g[i] & 1, p.status)) return false;
+              tc_fence_after();
+#pragma unroll
+              for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+                mma_bf16_ts(tmem + C::O_COL + i * D, p_tmem + kk * 8,
+                            dv + uint64_t((kk * 2048) >> 4), idesc_o, (j | kk) != 0 ? 1u : 0u);
+            }
+            ++pv_g[i];
+            return true;
+          };
+          const int cnt[2] = {w.cnt0, w.cnt1}, steps = max(w.cnt0, w.cnt1);
+          for (int j = 0; j <= steps && ok; ++j) {
+#pragma unroll
+            for (int i = 0; i < 2 && ok; ++i) {
+              const int st = jg + step * j + (w.alt ? i : 0);
+              if (j >= 1 && j - 1 < cnt[i]) {
+                ok = issue_pv(i, j - 1, st - step);
+                if (ok && j == cnt[i]) {
+                  mma_commit(&o_done[i]);
+                  ++acc_items[i];
+                }
+                if (ok && w.alt) mma_commit(&v_empty[(st - step) % ST]);
+              }
+              if (ok && j < cnt[i]) {
+                ok = mbar_wait(&k_full[st % ST], (st / ST) & 1, p.status);
+                if (ok) {
+                  tc_fence_after();
+                  issue_s(i, st);
+                  if (w.alt) mma_commit(&k_empty[st % ST]);
+                }
+              }
+            }
+            if (!ok) break;
+            if (!w.alt && j < steps) mma_commit(&k_empty[(jg + j) % ST]);
+            if (j == steps - 1) mma_commit(q_empty);    // the item's last S was just issued
+            if (!w.alt && j >= 1) mma_commit(&v_empty[(jg + j - 1) % ST]);
+          }
+          jg += w.all;
+          ++it;
+        }
+      }
+      __syncwarp();
+    } else if (warp == 2) {
+      // ------------------------------------------------------------ V rows past the end
+      // The stage's v_full is signalled here instead of by the load.  v_tail[s] completes once
+      // per tail in stage s, and the stage is not reused before the MMA warp has seen v_full.
+      int jg = 0;
+      uint32_t phase = 0;                    // bit s: parity of v_tail[s]'s next completion
+      for (int t = t_begin; t < t_end; ++t) {
+        const Work w = make_work<PAGED>(p, t);
+        if (w.all == 0) continue;
+        const int tail = (w.lk - 1) / BN - w.j0, live = w.lk % BN;
+        if (live != 0 && tail < w.all) {
+          const int s = (jg + tail) % ST;
+          if (!__all_sync(0xffffffffu, mbar_wait(&v_tail[s], phase >> s & 1u, p.status))) break;
+          phase ^= 1u << s;
+#pragma unroll 1
+          for (int a = 0; a < C::ATOMS; ++a) {
+            uint4* rows = reinterpret_cast<uint4*>(sV + s * C::KV_BYTES + a * BN * 128);
+            for (int x = live * 8 + lane; x < BN * 8; x += 32) rows[x] = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_full[s]);
+        }
+        jg += w.all;
+      }
+      __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
+    // ------------------------------------------------------------ softmax / epilogue
+    const int ti = (warp - 4) >> 2;           // softmax state of this warpgroup
+    const int quarter = warp & 3;             // TMEM lane quarter this warp may access
+    const int r = quarter * 32 + lane;        // row of the tile owned by this thread
+    const uint32_t lane_off = uint32_t(quarter * 32) << 16;
+    const uint32_t s_addr = tmem + lane_off + uint32_t(ti * BN);
+    const uint32_t o_addr = tmem + lane_off + C::O_COL + uint32_t(ti * D);
+    const float c = p.scale_log2;
+    const int r_tok = r / p.group, r_head = r - r_tok * p.group;
+    int sg = 0, acc_items = 0;                // S tiles seen, items whose O accumulated
+    bool ok = true;
+    for (int t = t_begin; t < t_end && ok; ++t) {
+      const Work w = make_work<PAGED>(p, t);
+      const int n_my = ti == 0 ? w.cnt0 : w.cnt1;
+      const int tok = w.tok0 + (w.alt ? 0 : ti * p.tokens) + r_tok;
+      const bool live = r_tok < p.tokens && tok < w.tok_end && (PAGED || tok < p.tokens_q);
+      int keys = 0;                           // keys this row sees
+      if (live) {
+        keys = PAGED ? min(w.lk, len_of(p.lens, p.slots, p.n_slots,
+                                        int64_t(p.width) << p.page_shift, tok))
+                     : min(w.lk, tok - w.seq0 + w.off);
+      }
+      float m_used = -INFINITY, l = 0.f;      // m in raw score units
+      for (int j = 0; j < n_my; ++j, ++sg) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[ti], sg & 1, p.status));
+        if (!ok) break;
+        tc_fence_after();
+        float x[BN];
+#pragma unroll
+        for (int k = 0; k < BN; k += 32) tmem_ld32(s_addr + k, reinterpret_cast<uint32_t*>(&x[k]));
+        tmem_wait_ld();
+        const int lim = keys - (w.j0 + (w.alt ? 2 * j + ti : j)) * BN;
+        // Warp-uniform: the loop below holds warp-collective tcgen05.st.  Rows of no token
+        // are left as they are; nobody reads their result.
+        if (__any_sync(0xffffffffu, live && lim < BN)) {
+#pragma unroll
+          for (int k = 0; k < BN; ++k) x[k] = (k < lim) ? x[k] : -INFINITY;
+        }
+        float2 sum2[4];
+        float mq[4];
+        auto row_max = [&](int k0, int k1) {       // folds x[k0 .. k1) into mq
+#pragma unroll
+          for (int k = k0; k < k1; k += 8)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) mq[u] = max3f(mq[u], x[k + u], x[k + 4 + u]);
+        };
+        // p = 2^(s c - m c) in fp32 for 16 keys, summed in fp32, stored as bf16 pairs.
+        auto weigh = [&](int k, float2 cc, float2 nmc) {
+          uint32_t pk[8];
+#pragma unroll
+          for (int t2 = 0; t2 < 8; ++t2) {
+            const float2 y = f2fma(make_float2(x[k + 2 * t2], x[k + 2 * t2 + 1]), cc, nmc);
+            const float2 e = make_float2(ex2(y.x), ex2(y.y));
+            sum2[t2 & 3] = f2add(sum2[t2 & 3], e);
+            pk[t2] = pack_bf16x2(e.x, e.y);
+          }
+          tmem_st8(s_addr + k / 2, pk);
+        };
+        const float2 cc = make_float2(c, c);
+        float2 nmc;
+        auto rebase = [&](float m_new, bool need) {    // warp-uniform call
+          const float f = need ? ex2((m_used - m_new) * c) : 1.0f;   // m_used = -inf: f = 0
+          l *= f;
+          if (j > 0) {
+            // "S_i(j) done" implies PV_i(j-1) done (commit order), so O is complete here.
+#pragma unroll 1
+            for (int k = 0; k < D; k += 16) {
+              uint32_t o[16];
+              tmem_ld16(o_addr + k, o);
+              tmem_wait_ld();
+              uint32_t lo[8], hi[8];
+#pragma unroll
+              for (int t2 = 0; t2 < 8; ++t2) {
+                lo[t2] = __float_as_uint(__uint_as_float(o[t2]) * f);
+                hi[t2] = __float_as_uint(__uint_as_float(o[8 + t2]) * f);
+              }
+              tmem_st8(o_addr + k, lo);
+              tmem_st8(o_addr + k + 8, hi);
+            }
+            tmem_wait_st();
+          }
+          if (need) m_used = m_new;
+        };
+        if (j == 0) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mq[u] = -INFINITY;
+          row_max(0, BN);
+          m_used = max3f(mq[0], mq[1], fmaxf(mq[2], mq[3]));
+        }
+#pragma unroll 1
+        for (int pass = 0; ; ++pass) {
+          const float mc = (m_used == -INFINITY) ? 0.f : m_used * c;
+          nmc = make_float2(-mc, -mc);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            sum2[u] = make_float2(0.f, 0.f);
+            mq[u] = -INFINITY;
+          }
+#pragma unroll
+          for (int k = 0; k < BN / 2; k += 16) {
+            weigh(k, cc, nmc);
+            row_max(2 * k, 2 * k + 32);
+          }
+          const float mx = max3f(mq[0], mq[1], fmaxf(mq[2], mq[3]));
+          const bool need = (mx - m_used) * c > kGrow;    // m_used = -inf and a key: true
+          if (pass > 0 || !__any_sync(0xffffffffu, need)) break;
+          rebase(mx, need);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[2 * ti]);
+#pragma unroll
+        for (int k = BN / 2; k < BN; k += 16) weigh(k, cc, nmc);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[2 * ti + 1]);
+        const float2 s01 = f2add(sum2[0], sum2[1]), s23 = f2add(sum2[2], sum2[3]);
+        l += (s01.x + s23.x) + (s01.y + s23.y);
+      }
+      if (!ok) break;
+      if (n_my > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&o_done[ti], acc_items & 1, p.status));
+        if (!ok) break;
+        tc_fence_after();
+      }
+      const bool none = n_my == 0 || keys <= 0;     // the row saw nothing
+      if (w.slot < 0) {
+        const float inv = none || l == 0.f ? 0.f : 1.0f / l;
+        const int h = w.kvh * p.group + r_head;
+        const int64_t row = live ? int64_t(tok) : 0;
+        __nv_bfloat16* o_row = p.out + row * p.o_token + int64_t(live ? h : 0) * p.o_head;
+        if (p.lse != nullptr && live)
+          p.lse[row * p.heads_q + h] =
+              none ? -INFINITY : (m_used * c + log2f(l)) * 0.6931471805599453f;
+#pragma unroll 1
+        for (int k = 0; k < D; k += 16) {
+          uint32_t o[16];
+          if (n_my > 0) {  // warp-uniform: the collective load runs on every lane
+            tmem_ld16(o_addr + k, o);
+            tmem_wait_ld();
+          }
+          uint32_t u[8];
+#pragma unroll
+          for (int t2 = 0; t2 < 8; ++t2)
+            u[t2] = none ? 0u : pack_bf16x2(__uint_as_float(o[2 * t2]) * inv,
+                                            __uint_as_float(o[2 * t2 + 1]) * inv);
+          if (live) {
+            reinterpret_cast<uint4*>(o_row + k)[0] = make_uint4(u[0], u[1], u[2], u[3]);
+            reinterpret_cast<uint4*>(o_row + k)[1] = make_uint4(u[4], u[5], u[6], u[7]);
+          }
+        }
+      } else {
+        const int64_t row = int64_t(w.slot + ti) * BM + r;
+        if (live) p.ml[row] = none ? make_float2(-INFINITY, 0.f) : make_float2(m_used * c, l);
+        if (n_my > 0) {
+#pragma unroll 1
+          for (int k = 0; k < D; k += 16) {
+            uint32_t o[16];
+            tmem_ld16(o_addr + k, o);
+            tmem_wait_ld();
+            if (live && !none) {
+              uint4* to = reinterpret_cast<uint4*>(p.opart + row * D + k);
+#pragma unroll
+              for (int t2 = 0; t2 < 4; ++t2)
+                to[t2] = make_uint4(o[4 * t2], o[4 * t2 + 1], o[4 * t2 + 2], o[4 * t2 + 3]);
+            }
+          }
+        }
+      }
+      if (n_my > 0) {
+        // O_i has been read: the next item's first PV may overwrite it.
+        tc_fence_before();
+        mbar_arrive(&o_free[ti]);
+        ++acc_items;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  if (fn == nullptr) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }
+  return fn;
+}
+
+// bf16 map of `rank` dimensions, innermost contiguous; strides in bytes of dimensions 1, ...
+inline bool make_map(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims,
+                     const cuuint64_t* strides, const cuuint32_t* box) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, cuuint32_t(rank), const_cast<void*>(base), dims,
+            strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Launch attributes of one instantiation (shared memory, registers enough for the split).
+template <int D, bool PAGED>
+cudaError_t prepare_kernel() {
+  const auto kernel = attn_tc_kernel<D, PAGED>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       Cfg<D>::SMEM);
+  if (e != cudaSuccess) return e;
+  static int regs = -1;
+  if (regs < 0) {
+    cudaFuncAttributes fa;
+    e = cudaFuncGetAttributes(&fa, kernel);
+    if (e != cudaSuccess) return e;
+    regs = fa.numRegs;
+  }
+  return regs < LAUNCH_REGS ? cudaErrorInvalidConfiguration : cudaSuccess;
+}
+
+}  // namespace enigma_tc

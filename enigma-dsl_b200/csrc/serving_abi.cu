@@ -41,6 +41,9 @@ int32_t check_heads(int64_t heads_q, int64_t heads_kv, int64_t head_dim) {
   return ENIGMA_OK;
 }
 
+// The kernels take a row's maximum before they scale it.
+bool good_scale(float s) { return s > 0.f && s < 1e30f; }
+
 int32_t check_shared(const enigma_sdpa_shared_prefix_desc* d) {
   if (d == nullptr) return bad("sdpa_shared_prefix: desc is NULL");
   if (d->dtype != ENIGMA_DTYPE_F32 && d->dtype != ENIGMA_DTYPE_BF16)
@@ -144,6 +147,7 @@ int32_t enigma_sdpa_packed(const enigma_sdpa_packed_desc* d, void* stream) {
     return bad("sdpa_packed: dtype");
   int32_t e = check_heads(d->heads_q, d->heads_kv, d->head_dim);
   if (e != ENIGMA_OK) return e;
+  if (!good_scale(d->scale)) return bad("sdpa_packed: scale must be positive and finite");
   if (d->tokens_q < 0 || d->tokens_k < 0) return bad("sdpa_packed: negative size");
   if (d->tokens_q > kInt31 - 256 || d->tokens_k > kInt31 - 256)
     return bad("sdpa_packed: sizes must fit in int32");
@@ -183,6 +187,7 @@ int32_t enigma_sdpa_shared_prefix_workspace_bytes(const enigma_sdpa_shared_prefi
 int32_t enigma_sdpa_shared_prefix(const enigma_sdpa_shared_prefix_desc* d, void* stream) {
   const int32_t e = check_shared(d);
   if (e != ENIGMA_OK) return e;
+  if (!good_scale(d->scale)) return bad("sdpa_shared_prefix: scale must be positive and finite");
   if (d->q_batch < 0 || d->q_head < 0 || d->o_batch < 0 || d->o_head < 0 || d->k_page < 0 ||
       d->v_page < 0)
     return bad("sdpa_shared_prefix: negative stride");

@@ -233,7 +233,7 @@ int32_t enigma_decode_noalloc_check_timeout_path(int64_t polls, void* stream);
  * heads_kv).  A row that sees no key gives zeros and lse -inf.  Token and head strides are
  * in elements, head_dim is contiguous; lse (may be NULL) is [tokens_q, heads_q], natural log.
  * Keys of other sequences are never read into a result, whatever they hold; a masked key of a
- * row's own sequence must be finite in v.
+ * row's own sequence must be finite in v.  scale must be positive.
  *
  * enigma_sdpa_packed_plan (host only) lays out the work for these lengths, so a batch's layers
  * share one plan: which thread block does what, evenly, with long rows split over their keys
@@ -267,8 +267,8 @@ int32_t enigma_sdpa_packed(const enigma_sdpa_packed_desc* desc, void* stream);
  * table [n_slots, table_width] int32 page numbers, lens [n_slots] int32 keys of each sequence;
  * sequence b uses row slots[b] (slots NULL: row b).  The first prefix_len keys are the same for
  * the whole batch: they are read once, through the row of sequence 0.  A sequence attends
- * to its first min(lens, table_width * page) keys; none gives zeros.  page is 16, 32, 64 or
- * 128; batch <= 4096.  workspace: caller-owned device memory of
+ * to its first min(lens, table_width * page) keys; none gives zeros.  scale is positive, page
+ * 16, 32, 64 or 128, batch <= 4096.  workspace: caller-owned device memory of
  * enigma_sdpa_shared_prefix_workspace_bytes() bytes, 256-byte aligned. */
 typedef struct enigma_sdpa_shared_prefix_desc {
   int64_t batch, heads_q, heads_kv, head_dim, page, pages, table_width, n_slots, prefix_len;

@@ -9,7 +9,7 @@ from __future__ import annotations
 import numpy as np
 
 U32 = 2.0 ** -24      # unit roundoff of fp32
-UBF = 2.0 ** -9       # of bf16
+UBF = 2.0 ** -8       # of bf16 (8 significant bits)
 
 
 def attend(q, k, v, scale, seen):
@@ -77,8 +77,8 @@ def bound(out, mag, err, keys, bf16):
 
     With fp32 scores, weights and sums over `keys` keys: each weight is off by the score's error
     (twice: numerator and normaliser), each sum by keys * u of its magnitude; a few u more for
-    exp and the division.  In bf16 each weight is rounded once before it meets its value (2^-9
-    of the magnitude) and the result once (2^-9 of the result)."""
+    exp and the division.  In bf16 each weight is rounded once before it meets its value (2^-8
+    of the magnitude) and the result once (2^-8 of the result)."""
     fp32 = 4 * (err[..., None] + (keys + 16) * U32) * mag
     return fp32 + (UBF * (mag + np.abs(out)) * 1.01 if bf16 else 2 * U32 * np.abs(out)) + 1e-30
 

@@ -201,6 +201,9 @@ def test_packed_refusals(cuda):
         cuda_ops.sdpa_packed(q.cpu(), k.cpu(), k.cpu(), plan)
     with pytest.raises(ValueError, match="shapes"):
         cuda_ops.sdpa_packed(q, k, k[:6], plan)
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(_native.EnigmaCudaError, match="scale"):
+            cuda_ops.sdpa_packed(q, k, k, plan, scale=scale)
     wide = torch.zeros(7, 2, 257, device=cuda)
     with pytest.raises(_native.EnigmaCudaError, match="head_dim"):
         cuda_ops.sdpa_packed(torch.zeros(7, 4, 257, device=cuda), wide, wide, plan)
