@@ -10,19 +10,27 @@
 // state and the odd ones with the other, when there is no second row tile to fill the SM.
 //
 //   warp 0      TMA: both Q tiles, then K and V tiles into rings of C::STAGES
-//   warp 1      one thread issues tcgen05.mma, S_i = Q_i K_j^T and O_i += P_i V_j (P from
-//               TMEM over S_i's columns), PV_0 S_0 PV_1 S_1 in turn, so the tensor core works
-//               for one tile while the other's softmax runs
-//   warp 2      clears V rows past the sequence's end: what lies behind it (a neighbour's
-//               tokens, a page's unwritten rows) may be NaN, and 0 * NaN would reach the sum
+//   warps 1, 2  one thread each issues the tcgen05.mma of softmax state i = warp - 1:
+//               S_i = Q_i K_j^T, O_i += P_i V_j (P from TMEM over S_i's columns); the tensor
+//               core works for one state while the other's softmax runs
 //   warps 4-7, 8-11   softmax of the two tiles, one thread per row, fp32
 //
+// What bounds it: per 128 keys of both tiles the tensor core needs 2048 cycles and the
+// exponential units 2048 (256 x 128 at 16 a cycle), each tile's chain S -> softmax -> P V -> S
+// about 3500.  So the two states work in turns: one weighs its tile (its exponentials) while the
+// other's products run.  Without turns they fall into step, both at the exponentials and then
+// both waiting for the tensor core: 4300 cycles a step against 3550 (8192 tokens, 32 / 8 heads of
+// 128, causal: 573 -> 457 us = 1200 TFLOP/s; one issuing thread for both states, in turns or not,
+// 573 to 583 us).  The turn passes on after kHandOver of the 128 keys: 96 keys 457 us, 64 479,
+// 80 480, all 128 482.
+//
 // The softmax takes the running maximum that the tiles before left and starts its exponentials
-// at once; this tile's maximum is found beside them (they do not depend on it) and only has to
-// show that no weight exceeds 2^kGrow.  If one does, O and the sum are rescaled and the tile's
-// exponentials are done again.  Any base within fp32's range gives the same quotient, so this
-// is exact; it takes the row maximum (400 to 450 cycles of 128 dependent comparisons) out of
-// the chain S -> P -> PV -> S that bounds this kernel.
+// at once; this tile's maximum is found beside them and only has to show that no weight exceeds
+// 2^kGrow.  If one does, O and the sum are rescaled and the tile's exponentials are done again.
+// Any base within fp32's range gives the same quotient, so this is exact (the maximum first:
+// 463 us).  Not kept: a degree-4 polynomial on the FMA pipe for 1/8, 1/4, 3/8 of the exponentials
+// (480, 511, 535 us: a turn is bound by one warp's instructions); the row sum after P's release
+// (467 us); P released once, or at 96 keys (470 us).
 //
 // P is rounded to bf16, the operand type of the PV product; sums, maxima and O stay fp32.
 // Every mbarrier wait is bounded (sm100.cuh).
@@ -38,11 +46,12 @@ using namespace enigma_sm100;
 
 constexpr int BM = 128;            // rows per tile (two tiles per item)
 constexpr int BN = 128;            // keys per tile
-constexpr int THREADS = 384;       // warpgroup 0: TMA, MMA, V tail, idle; WG 1, 2: softmax
+constexpr int THREADS = 384;       // warpgroup 0: TMA, 2 MMA, idle; WG 1, 2: softmax
 // Register split: 384 x 168 at launch; warpgroup 0 drops to 104, the softmax warpgroups rise to
 // 200: 128 * 104 + 256 * 200 = 384 * 168 exactly.
 constexpr int LAUNCH_REGS = 168, WG0_REGS = 104, SOFTMAX_REGS = 200;
 static_assert(128 * WG0_REGS + 256 * SOFTMAX_REGS <= THREADS * LAUNCH_REGS, "register split");
+constexpr int kHandOver = 96;      // keys of a tile weighed when the other state's turn begins
 constexpr float kGrow = 24.f;      // log2 units a weight may exceed 1 by before a rescale
 
 template <int D>
@@ -214,18 +223,18 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   uint8_t* sK = sQ + 2 * C::Q_BYTES;
   uint8_t* sV = sK + ST * C::KV_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * C::KV_BYTES);
-  uint64_t* q_full = bars;                   // [1]
-  uint64_t* q_empty = q_full + 1;            // [1] the item's last S product has read Q
-  uint64_t* k_full = q_empty + 1;            // [ST]
+  uint64_t* q_full = bars;                   // [2] one Q tile per softmax state
+  uint64_t* q_empty = q_full + 2;            // [2] the item's last S product has read Q_i
+  uint64_t* k_full = q_empty + 2;            // [ST]
   uint64_t* k_empty = k_full + ST;
   uint64_t* v_full = k_empty + ST;
   uint64_t* v_empty = v_full + ST;
-  uint64_t* v_tail = v_empty + ST;           // [ST] a sequence's last V tile has landed
-  uint64_t* s_full = v_tail + ST;            // [2] one per softmax state
+  uint64_t* s_full = v_empty + ST;            // [2] one per softmax state
   uint64_t* p_full = s_full + 2;             // [2 states][2 halves of the keys]
   uint64_t* o_done = p_full + 4;             // [2]
   uint64_t* o_free = o_done + 2;             // [2] the epilogue has read O_i
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 2);
+  uint64_t* turn = o_free + 2;               // [2] state i may take the exponential units
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -237,21 +246,21 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
     for (int s = 0; s < ST; ++s) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
+      mbar_init(&k_empty[s], 2);
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], 1);
-      mbar_init(&v_tail[s], 1);
+      mbar_init(&v_empty[s], 2);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[2 * i], 128);
       mbar_init(&p_full[2 * i + 1], 128);
       mbar_init(&o_done[i], 1);
       mbar_init(&o_free[i], 128);
+      mbar_init(&turn[i], 4);
     }
     fence_barrier_init();
   }
@@ -268,22 +277,31 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(WG0_REGS));
     if (warp == 0) {
       // ------------------------------------------------------------ TMA producer
-      int jg = 0, it = 0;                    // key tiles loaded so far; items with work
+      int jg = 0;                            // key tiles loaded so far
+      int q_items[2] = {0, 0};               // items with work per softmax state
       bool ok = true;
       const uint32_t q_bytes = uint32_t(p.group * p.tokens) * 128u;   // one atom of a Q tile
       for (int t = t_begin; t < t_end && ok; ++t) {
         const Work w = make_work<PAGED>(p, t);
         if (w.all == 0) continue;
-        if (it > 0 && !__all_sync(0xffffffffu, mbar_wait(q_empty, (it - 1) & 1, p.status))) break;
-        const int q_tiles = w.alt ? 1 : 2;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(q_full, q_bytes * C::ATOMS * q_tiles);
-          for (int i = 0; i < q_tiles; ++i)
+        auto load_q = [&](int i, int n) {    // an alt item's one tile goes to both states
+          if (n == 0) return true;
+          if (q_items[i] > 0 &&
+              !__all_sync(0xffffffffu, mbar_wait(&q_empty[i], (q_items[i] - 1) & 1, p.status)))
+            return false;
+          ++q_items[i];
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&q_full[i], q_bytes * C::ATOMS);
 #pragma unroll
             for (int a = 0; a < C::ATOMS; ++a)
-              tma_load_3d(sQ + i * C::Q_BYTES + a * BM * 128, &tmQ, q_full, a * 64,
-                          w.kvh * p.group, w.tok0 + i * p.tokens);
-        }
+              tma_load_3d(sQ + i * C::Q_BYTES + a * BM * 128, &tmQ, &q_full[i], a * 64,
+                          w.kvh * p.group, w.tok0 + (w.alt ? 0 : i * p.tokens));
+          }
+          __syncwarp();
+          return true;
+        };
+        ok = load_q(0, w.cnt0);
+        if (!ok) break;
         // Paged: lane x loads box x of each tile, rows [(x / ATOMS) << box_shift, ...), atom
         // x % ATOMS; the page number of the next tile is read one tile ahead.
         const int box = PAGED ? lane / C::ATOMS : 0, atom = PAGED ? lane % C::ATOMS : 0;
@@ -324,122 +342,107 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
             __syncwarp();
             return true;
           };
-          // A last V tile with rows past the end goes to warp 2 first.
-          uint64_t* v_bar = key0 + BN > w.lk ? &v_tail[s] : &v_full[s];
           if (!load(&tmK, sK + s * C::KV_BYTES, &k_full[s], &k_empty[s]) ||
-              !load(&tmV, sV + s * C::KV_BYTES, v_bar, &v_empty[s])) {
+              (j == 0 && !load_q(1, w.cnt1)) ||
+              !load(&tmV, sV + s * C::KV_BYTES, &v_full[s], &v_empty[s])) {
             ok = false;
             break;
           }
         }
-        ++it;
       }
       __syncwarp();
-    } else if (warp == 1) {
-      // ------------------------------------------------------------ MMA issuer
+    } else if (warp <= 2) {
+      // ------------------------------------------------------------ MMA issuers
+      // Warp 1 + i issues for softmax state i: S_0 | PV_0 S_1 | PV_1 S_2 ...  Each state's
+      // products wait for its own softmax only; the tensor core takes them as they come.
       if (lane == 0) {
+        const int i = warp - 1;
         constexpr uint32_t idesc_s = idesc_bf16_f32(BM, BN, false, false);
         constexpr uint32_t idesc_o = idesc_bf16_f32(BM, D, false, true);
-        const uint32_t q_addr = smem_u32(sQ), k_addr = smem_u32(sK), v_addr = smem_u32(sV);
-        int jg = 0, it = 0;
-        int pv_g[2] = {0, 0}, acc_items[2] = {0, 0};
+        const uint32_t s_tmem = tmem + uint32_t(i * BN), o_tmem = tmem + C::O_COL + uint32_t(i * D);
+        const uint64_t dk0 = smem_desc_sw128(smem_u32(sK), 16, 1024);
+        const uint64_t dv0 = smem_desc_sw128(smem_u32(sV), BN * 128, 1024);
+        const uint64_t dq = smem_desc_sw128(smem_u32(sQ) + uint32_t(i) * C::Q_BYTES, 16, 1024);
+        int jg = 0, pv = 0, items_done = 0;  // items_done: with work for this state
         bool ok = true;
         for (int t = t_begin; t < t_end && ok; ++t) {
           const Work w = make_work<PAGED>(p, t);
           if (w.all == 0) continue;
+          const int n = i == 0 ? w.cnt0 : w.cnt1;
+          // A stage is free again after one arrival from each issuer; the only user of an
+          // alt item's stage arrives twice.
+          auto release = [&](uint64_t* empty) {
+            mma_commit(empty);
+            if (w.alt) mma_commit(empty);
+          };
+          int st = jg + (w.alt ? i : 0);
           const int step = w.alt ? 2 : 1;
-          if (!mbar_wait(q_full, it & 1, p.status)) break;
-          auto issue_s = [&](int i, int st) {
-            const int s = st % ST;
-            const uint32_t s_tmem = tmem + uint32_t(i * BN);
+          auto issue_s = [&](int at) -> bool {
+            const int sk = at % ST;
+            tc_fence_after();
+            const uint64_t dk = dk0 + uint64_t((sk * C::KV_BYTES) >> 4);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t offq = (w.alt ? 0 : i) * C::Q_BYTES + (kk / 4) * (BM * 128) + (kk % 4) * 32;
-              const uint32_t offk = s * C::KV_BYTES + (kk / 4) * (BN * 128) + (kk % 4) * 32;
-              mma_bf16_ss(s_tmem, smem_desc_sw128(q_addr + offq, 16, 1024),
-                          smem_desc_sw128(k_addr + offk, 16, 1024), idesc_s, kk != 0 ? 1u : 0u);
+              const uint64_t off = uint64_t(((kk / 4) * (BM * 128) + (kk % 4) * 32) >> 4);
+              mma_bf16_ss(s_tmem, dq + off, dk + off, idesc_s, kk != 0 ? 1u : 0u);
             }
             mma_commit(&s_full[i]);
+            return true;
           };
-          // P arrives in two halves of the keys, so the first half's products start while the
-          // softmax finishes the second.  An item's first PV overwrites O_i: it waits until
-          // the previous item's epilogue has read it.
-          auto issue_pv = [&](int i, int j, int st) -> bool {
-            const int s = st % ST;
-            if (!mbar_wait(&v_full[s], (st / ST) & 1, p.status)) return false;
-            if (j == 0 && acc_items[i] > 0 &&
-                !mbar_wait(&o_free[i], (acc_items[i] - 1) & 1, p.status))
-              return false;
-            const uint32_t p_tmem = tmem + uint32_t(i * BN);
-            const uint64_t dv = smem_desc_sw128(v_addr + s * C::KV_BYTES, BN * 128, 1024);
+          if (n > 0) {
+            ok = mbar_wait(&q_full[i], items_done & 1, p.status) &&
+                 mbar_wait(&k_full[st % ST], (st / ST) & 1, p.status);
+            if (!ok) break;
+            issue_s(st);
+            if (n == 1) mma_commit(&q_empty[i]);
+            release(&k_empty[st % ST]);
+          }
+          for (int j = 0; j < n; ++j, st += step) {
+            const int sv = st % ST, next = st + step;
+            // What the products of this step need besides P, before P is waited for.
+            ok = mbar_wait(&v_full[sv], (st / ST) & 1, p.status) &&
+                 (j + 1 == n || mbar_wait(&k_full[next % ST], (next / ST) & 1, p.status)) &&
+                 (j > 0 || items_done == 0 || mbar_wait(&o_free[i], (items_done - 1) & 1, p.status));
+            if (!ok) break;
+            const uint64_t dv = dv0 + uint64_t((sv * C::KV_BYTES) >> 4);
+            // P arrives in two halves of the keys, so the first half's products start while
+            // the softmax finishes the second.
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              if (!mbar_wait(&p_full[2 * i + half], pv_g[i] & 1, p.status)) return false;
+              ok = mbar_wait(&p_full[2 * i + half], pv & 1, p.status);
+              if (!ok) break;
               tc_fence_after();
 #pragma unroll
               for (int kk = half * 4; kk < half * 4 + 4; ++kk)
-                mma_bf16_ts(tmem + C::O_COL + i * D, p_tmem + kk * 8,
-                            dv + uint64_t((kk * 2048) >> 4), idesc_o, (j | kk) != 0 ? 1u : 0u);
-            }
-            ++pv_g[i];
-            return true;
-          };
-          const int cnt[2] = {w.cnt0, w.cnt1}, steps = max(w.cnt0, w.cnt1);
-          for (int j = 0; j <= steps && ok; ++j) {
-#pragma unroll
-            for (int i = 0; i < 2 && ok; ++i) {
-              const int st = jg + step * j + (w.alt ? i : 0);
-              if (j >= 1 && j - 1 < cnt[i]) {
-                ok = issue_pv(i, j - 1, st - step);
-                if (ok && j == cnt[i]) {
-                  mma_commit(&o_done[i]);
-                  ++acc_items[i];
-                }
-                if (ok && w.alt) mma_commit(&v_empty[(st - step) % ST]);
-              }
-              if (ok && j < cnt[i]) {
-                ok = mbar_wait(&k_full[st % ST], (st / ST) & 1, p.status);
-                if (ok) {
-                  tc_fence_after();
-                  issue_s(i, st);
-                  if (w.alt) mma_commit(&k_empty[st % ST]);
-                }
-              }
+                mma_bf16_ts(o_tmem, s_tmem + kk * 8, dv + uint64_t((kk * 2048) >> 4), idesc_o,
+                            (j | kk) != 0 ? 1u : 0u);
             }
             if (!ok) break;
-            if (!w.alt && j < steps) mma_commit(&k_empty[(jg + j) % ST]);
-            if (j == steps - 1) mma_commit(q_empty);    // the item's last S was just issued
-            if (!w.alt && j >= 1) mma_commit(&v_empty[(jg + j - 1) % ST]);
+            ++pv;
+            if (j + 1 == n) {
+              mma_commit(&o_done[i]);
+            } else {
+              issue_s(next);
+              if (j + 2 == n) mma_commit(&q_empty[i]);    // the item's last S was just issued
+              release(&k_empty[next % ST]);
+            }
+            release(&v_empty[sv]);
+          }
+          if (!ok) break;
+          if (n > 0) ++items_done;
+          // Key tiles that only the other state needs.
+          if (!w.alt) {
+            for (int j = n; j < w.all; ++j, ++st) {
+              ok = mbar_wait(&k_full[st % ST], (st / ST) & 1, p.status);
+              if (!ok) break;
+              mbar_arrive(&k_empty[st % ST]);
+              ok = mbar_wait(&v_full[st % ST], (st / ST) & 1, p.status);
+              if (!ok) break;
+              mbar_arrive(&v_empty[st % ST]);
+            }
           }
           jg += w.all;
-          ++it;
         }
-      }
-      __syncwarp();
-    } else if (warp == 2) {
-      // ------------------------------------------------------------ V rows past the end
-      // The stage's v_full is signalled here instead of by the load.  v_tail[s] completes once
-      // per tail in stage s, and the stage is not reused before the MMA warp has seen v_full.
-      int jg = 0;
-      uint32_t phase = 0;                    // bit s: parity of v_tail[s]'s next completion
-      for (int t = t_begin; t < t_end; ++t) {
-        const Work w = make_work<PAGED>(p, t);
-        if (w.all == 0) continue;
-        const int tail = (w.lk - 1) / BN - w.j0, live = w.lk % BN;
-        if (live != 0 && tail < w.all) {
-          const int s = (jg + tail) % ST;
-          if (!__all_sync(0xffffffffu, mbar_wait(&v_tail[s], phase >> s & 1u, p.status))) break;
-          phase ^= 1u << s;
-#pragma unroll 1
-          for (int a = 0; a < C::ATOMS; ++a) {
-            uint4* rows = reinterpret_cast<uint4*>(sV + s * C::KV_BYTES + a * BN * 128);
-            for (int x = live * 8 + lane; x < BN * 8; x += 32) rows[x] = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&v_full[s]);
-        }
-        jg += w.all;
       }
       __syncwarp();
     }
@@ -455,6 +458,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     const float c = p.scale_log2;
     const int r_tok = r / p.group, r_head = r - r_tok * p.group;
     int sg = 0, acc_items = 0;                // S tiles seen, items whose O accumulated
+    int jg = 0;                               // key tiles streamed before this item
+    int turns = 0;                            // turns taken
+    if (ti == 1 && lane == 0) mbar_arrive(&turn[0]);   // state 0 begins
     bool ok = true;
     for (int t = t_begin; t < t_end && ok; ++t) {
       const Work w = make_work<PAGED>(p, t);
@@ -468,6 +474,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                      : min(w.lk, tok - w.seq0 + w.off);
       }
       float m_used = -INFINITY, l = 0.f;      // m in raw score units
+      const int both = min(w.cnt0, w.cnt1);   // tiles that both states have: taken in turns
       for (int j = 0; j < n_my; ++j, ++sg) {
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[ti], sg & 1, p.status));
         if (!ok) break;
@@ -476,7 +483,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
 #pragma unroll
         for (int k = 0; k < BN; k += 32) tmem_ld32(s_addr + k, reinterpret_cast<uint32_t*>(&x[k]));
         tmem_wait_ld();
-        const int lim = keys - (w.j0 + (w.alt ? 2 * j + ti : j)) * BN;
+        const int tile = w.alt ? 2 * j + ti : j;     // within the item
+        const int lim = keys - (w.j0 + tile) * BN;
         // Warp-uniform: the loop below holds warp-collective tcgen05.st.  Rows of no token
         // are left as they are; nobody reads their result.
         if (__any_sync(0xffffffffu, live && lim < BN)) {
@@ -534,6 +542,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           row_max(0, BN);
           m_used = max3f(mq[0], mq[1], fmaxf(mq[2], mq[3]));
         }
+        if (j < both) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&turn[ti], turns & 1, p.status));
+          if (!ok) break;
+          ++turns;
+        }
 #pragma unroll 1
         for (int pass = 0; ; ++pass) {
           const float mc = (m_used == -INFINITY) ? 0.f : m_used * c;
@@ -553,11 +566,30 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           if (pass > 0 || !__any_sync(0xffffffffu, need)) break;
           rebase(mx, need);
         }
+        // The sequence's last tile: what lies behind its end in V (a neighbour's tokens, a
+        // page's unwritten rows) may be NaN, and 0 * NaN would reach the sum.  Row r is
+        // cleared here, before P is released; the stage stays until PV has read it.
+        const int end = w.lk - (w.j0 + tile) * BN;
+        if (end < BN) {
+          const int st = jg + tile, s = st % ST;
+          ok = __all_sync(0xffffffffu, mbar_wait(&v_full[s], (st / ST) & 1, p.status));
+          if (!ok) break;
+          if (r >= end) {
+#pragma unroll
+            for (int y = 0; y < D / 8; ++y)
+              *reinterpret_cast<uint4*>(sV + s * C::KV_BYTES + (y / 8) * BN * 128 + r * 128 +
+                                        (y % 8) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&p_full[2 * ti]);
 #pragma unroll
-        for (int k = BN / 2; k < BN; k += 16) weigh(k, cc, nmc);
+        for (int k = BN / 2; k < BN; k += 16) {
+          if (k == kHandOver && j < both && lane == 0) mbar_arrive(&turn[1 - ti]);
+          weigh(k, cc, nmc);
+        }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&p_full[2 * ti + 1]);
@@ -565,6 +597,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         l += (s01.x + s23.x) + (s01.y + s23.y);
       }
       if (!ok) break;
+      jg += w.all;
       if (n_my > 0) {
         ok = __all_sync(0xffffffffu, mbar_wait(&o_done[ti], acc_items & 1, p.status));
         if (!ok) break;
