@@ -1,5 +1,5 @@
 // attn_packed.cu — attention over packed prompts: the tensor-core kernel of attn_tc.cuh over the
-// plan's items, and the join of rows whose keys the plan split.
+// plan's items, or the CUDA-core one, then the join of rows whose keys the plan split.
 #include <algorithm>
 
 #include "attn_tc.cuh"
@@ -8,47 +8,6 @@ namespace {
 
 using namespace enigma_tc;
 using namespace enigma_serving;
-
-// Joins the partial results of split rows: O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in
-// the order of the parts.  One warp per row; grid (groups, row blocks).
-template <int D>
-__global__ void __launch_bounds__(256)
-packed_join_kernel(const PackedGroup* __restrict__ groups, const float* __restrict__ opart,
-                   const float2* __restrict__ ml, const Params p) {
-  const int lane = threadIdx.x & 31;
-  const int r = int(blockIdx.y) * 8 + (threadIdx.x >> 5);       // row of the pair of tiles
-  const PackedGroup g = groups[blockIdx.x];
-  const int state = r / BM, row = r % BM;
-  const int tok = g.tok0 + state * g.tokens + row / p.group;
-  if (row >= g.tokens * p.group || tok >= g.tok_end || (g.alt && state > 0)) return;
-  const int n = g.alt ? 2 * g.parts : g.parts, step = g.alt ? 1 : 2;
-  const int64_t first = g.slot + (g.alt ? 0 : state);
-  float M = -INFINITY;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, ml[(first + i * step) * BM + row].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  constexpr int V = D / 32;
-  float acc[V] = {};
-  float l = 0.f;
-  for (int i = 0; i < n; ++i) {
-    const int64_t at = (first + i * step) * BM + row;
-    const float2 x = ml[at];
-    if (x.x == -INFINITY) continue;                             // this part saw no key
-    const float f = ex2(x.x - M);
-    l = fmaf(x.y, f, l);
-#pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] = fmaf(opart[at * D + lane * V + v], f, acc[v]);
-  }
-  const int h = g.kvh * p.group + row % p.group;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  __nv_bfloat16* out = p.out + tok * p.o_token + h * p.o_head + lane * V;
-#pragma unroll
-  for (int v = 0; v < V; v += 2)
-    *reinterpret_cast<uint32_t*>(out + v) = pack_bf16x2(acc[v] * inv, acc[v + 1] * inv);
-  if (p.lse != nullptr && lane == 0)
-    p.lse[int64_t(tok) * p.heads_q + h] =
-        l == 0.f ? -INFINITY : (M + log2f(l)) * 0.6931471805599453f;
-}
 
 bool a16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -103,10 +62,6 @@ cudaError_t launch(const enigma_sdpa_packed_desc& d, cudaStream_t s) {
   p.tokens_k = int(d.tokens_k);
   attn_tc_kernel<D, false><<<unsigned(d.header[kCtas]), THREADS, Cfg<D>::SMEM, s>>>(
       mq, mk, mv, p, d.header[kItems]);
-  e = cudaGetLastError();
-  if (e != cudaSuccess || d.header[kGroups] == 0) return e;
-  packed_join_kernel<D><<<dim3(unsigned(d.header[kGroups]), 2 * BM / 8), 256, 0, s>>>(
-      reinterpret_cast<const PackedGroup*>(d.plan + d.header[kGroupsAt]), p.opart, p.ml, p);
   return cudaGetLastError();
 }
 
@@ -115,9 +70,14 @@ cudaError_t launch(const enigma_sdpa_packed_desc& d, cudaStream_t s) {
 namespace enigma {
 
 cudaError_t sdpa_packed_launch(const enigma_sdpa_packed_desc& d, cudaStream_t s) {
-  if (!tc_takes(d)) return sdpa_packed_simt_launch(d, s);
-  note_kernel("attn_tc_kernel");
-  return d.head_dim == 128 ? launch<128>(d, s) : launch<64>(d, s);
+  cudaError_t e;
+  if (!tc_takes(d)) {
+    e = sdpa_packed_simt_launch(d, s);
+  } else {
+    note_kernel("attn_tc_kernel");
+    e = d.head_dim == 128 ? launch<128>(d, s) : launch<64>(d, s);
+  }
+  return e == cudaSuccess ? sdpa_packed_join_launch(d, s) : e;
 }
 
 }  // namespace enigma
