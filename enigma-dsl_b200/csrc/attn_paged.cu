@@ -18,8 +18,10 @@ using namespace enigma_tc;
 // every SM streams the same number of chunks whatever the lengths are.  A producer warp loads
 // chunks by TMA (one box per page and 64 columns) into a ring; four warps take 16 keys of each
 // chunk: S = Q K^T (mma.sync, the heads as the 16-row operand), online softmax, O += P V.  At
-// the end of a unit's run of chunks the warps' states are merged and stored in slot c + u
-// (segments in order advance c or u, so the slots are distinct).
+// the end of a unit's run of chunks each warp stores its state, in slot (c + u) * 4 + warp
+// (segments in order advance c or u, so the slots are distinct).  Merging the warps first cost
+// two barriers and a second pass per run (92 against 60 us for 128 sequences of 5 to 1024 keys);
+// four partials of a few KB next to a run's 100 KB and more of K and V cost less.
 constexpr int CHUNK = 64;
 constexpr int DWARPS = 4;
 constexpr int DTHREADS = (DWARPS + 1) * 32;
@@ -30,8 +32,7 @@ struct DCfg {
   static constexpr int ATOMS = D / 64;
   static constexpr int TILE = CHUNK * D * 2;            // one of K or V
   static constexpr int STAGES = D == 64 ? 4 : 3;
-  static constexpr int MERGE = (DWARPS - 1) * 8 * D * 4;
-  static constexpr int SMEM = STAGES * 2 * TILE + MERGE + 1024;   // + (batch + 1) ints
+  static constexpr int SMEM = STAGES * 2 * TILE + 1024;   // + 2 batch + 1 ints
 };
 
 struct DecodeParams {
@@ -66,18 +67,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void warps_sync() {   // the DWARPS consumer warps
-  asm volatile("bar.sync 1, %0;" ::"n"(DWARPS * 32) : "memory");
-}
-__device__ __forceinline__ bool warps_all(bool ok) {   // the same, and whether all say yes
-  uint32_t all;
-  asm volatile(
-      "{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %1, 0;\n\t"
-      "barrier.cta.red.and.pred b, 1, %2, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
-      : "=r"(all) : "r"(ok ? 1u : 0u), "n"(DWARPS * 32) : "memory");
-  return all != 0;
-}
-
 // floor(n c / P) for n c < 2^53 without a 64-bit division.
 __device__ __forceinline__ int64_t share(int64_t n, int64_t c, int64_t P) {
   const int64_t x = n * c;
@@ -135,10 +124,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* s_o = reinterpret_cast<float*>(ring + ST * 2 * C::TILE);     // [DWARPS - 1][8][D]
-  int* s_starts = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(s_o) + C::MERGE);
+  int* s_starts = reinterpret_cast<int*>(ring + ST * 2 * C::TILE);    // [batch + 1]
+  int* s_len = s_starts + p.batch + 1;                                // [batch]
   __shared__ uint64_t full[ST], empty[ST];
-  __shared__ float s_m[DWARPS][ROWS], s_l[DWARPS][ROWS];
   __shared__ int s_warp[DWARPS + 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t most = int64_t(p.width) << p.page_shift;
@@ -157,8 +145,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   for (int b0 = 0; b0 < p.batch; b0 += DTHREADS) {
     const int b = b0 + tid;
     int v = 0;
-    if (b < p.batch)
-      v = chunks_of(len_of(p.lens, p.slots, p.n_slots, most, b), p.prefix, p.base);
+    if (b < p.batch) {
+      const int len = len_of(p.lens, p.slots, p.n_slots, most, b);
+      s_len[b] = len;
+      v = chunks_of(len, p.prefix, p.base);
+    }
     int x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -193,7 +184,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     int i = 0;
     for (int64_t at = c0; at < c1;) {
       const Segment s = segment_at(s_starts, p.batch, per_b, p.blocks, at, c1);
-      const int len = len_of(p.lens, p.slots, p.n_slots, most, s.b);
+      const int len = s_len[s.b];
       auto look_up = [&](int j) {
         const int key = p.base + j * CHUNK + (box << p.box_shift);
         return page_at(p.table, p.slots, p.n_slots, p.width, p.pages, s.b, key >> p.page_shift);
@@ -230,7 +221,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   int i = 0;
   for (int64_t at = c0; at < c1;) {
     const Segment s = segment_at(s_starts, p.batch, per_b, p.blocks, at, c1);
-    const int len = len_of(p.lens, p.slots, p.n_slots, most, s.b);
+    const int len = s_len[s.b];
     const int rows = min(p.rows, p.group - s.block * p.rows);
     uint32_t q[D / 16][4];
     {
@@ -332,57 +323,25 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
     }
-    if (!warps_all(ok)) return;                             // a wait ran out (status is set)
+    if (!ok) return;                                        // a wait ran out (status is set)
+    const int64_t slot = (int64_t(blockIdx.x) + s.unit) * DWARPS + warp;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      if (quad == 0) {
-        s_m[warp][g + 8 * h] = m[h] == -INFINITY ? -INFINITY : m[h] * p.scale_log2;
-        s_l[warp][g + 8 * h] = l[h];
-      }
-    }
-    // Merge the warps' states, 8 rows at a time: the others' through shared memory to warp 0.
-    const int64_t slot = int64_t(blockIdx.x) + s.unit;
+      const int row = g + 8 * h;
+      if (row >= rows) continue;
+      // None of its keys: only says so.  (Nothing but NaN scores: l = NaN, no maximum.)
+      const bool none = m[h] == -INFINITY && l[h] == 0.f;
+      if (quad == 0)
+        p.ml[slot * p.rows + row] =
+            none ? make_float2(-INFINITY, 0.f)
+                 : make_float2(m[h] == -INFINITY ? 0.f : m[h] * p.scale_log2, l[h]);
+      if (none) continue;
+      float* to = p.opart + (slot * p.rows + row) * D + quad * 2;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (h * 8 >= rows) break;                             // uniform
-      if (warp > 0) {
-        float* mine = s_o + ((warp - 1) * 8 + g) * D + quad * 2;
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-          *reinterpret_cast<float2*>(mine + n * 8) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-      }
-      warps_sync();
-      if (warp == 0) {
-        const int row = g + 8 * h;
-        float M = s_m[0][row];
-#pragma unroll
-        for (int w = 1; w < DWARPS; ++w) M = fmaxf(M, s_m[w][row]);
-        float f[DWARPS], L = 0.f;
-#pragma unroll
-        for (int w = 0; w < DWARPS; ++w) {
-          f[w] = s_m[w][row] == -INFINITY ? 0.f : ex2(s_m[w][row] - M);
-          L = fmaf(s_l[w][row], f[w], L);
-        }
-        if (row < rows) {
-          float* to = p.opart + (slot * p.rows + row) * D + quad * 2;
-#pragma unroll
-          for (int n = 0; n < D / 8; ++n) {
-            float a = o[n][2 * h] * f[0], b = o[n][2 * h + 1] * f[0];
-#pragma unroll
-            for (int w = 1; w < DWARPS; ++w) {
-              const float2 v = *reinterpret_cast<const float2*>(s_o + ((w - 1) * 8 + g) * D +
-                                                                quad * 2 + n * 8);
-              a = fmaf(v.x, f[w], a);
-              b = fmaf(v.y, f[w], b);
-            }
-            *reinterpret_cast<float2*>(to + n * 8) = make_float2(a, b);
-          }
-          if (quad == 0) p.ml[slot * p.rows + row] = make_float2(M, L);
-        }
-      }
-      warps_sync();
+      for (int n = 0; n < D / 8; ++n)
+        *reinterpret_cast<float2*>(to + n * 8) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
     }
     at += s.n;
   }
@@ -404,8 +363,7 @@ struct JoinParams {
   int blocks, rows, ctas;
 };
 
-// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a row's partial results, always in the
-// same order.  One warp per (sequence, query head).
+// Joins a row's partial results.  One warp per (sequence, query head).
 template <int D>
 __global__ void __launch_bounds__(128) paged_join_kernel(const JoinParams p) {
   const int lane = threadIdx.x & 31;
@@ -436,32 +394,20 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const JoinParams p) {
     const int64_t x0 = int64_t(p.starts[b]) * per_b + int64_t(u) * n;
     const int64_t P = min(int64_t(p.ctas), T);
     const int first = owner(x0, T, P), last = owner(x0 + n - 1, T, P);
-    n_d = last - first + 1;
-    d_at = (int64_t(first) + b * per_b + u) * p.rows + (gh - block * p.rows);
+    n_d = (last - first + 1) * DWARPS;
+    d_at = (int64_t(first) + b * per_b + u) * DWARPS * p.rows + (gh - block * p.rows);
   }
-  float M = -INFINITY;
-  for (int i = lane; i < n_p; i += 32) M = fmaxf(M, p.p_ml[p_at + i * p_step].x);
-  for (int i = lane; i < n_d; i += 32) M = fmaxf(M, p.d_ml[d_at + int64_t(i) * p.rows].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   constexpr int V = D / 32;
-  float acc[V] = {};
-  float l = 0.f;
-  auto add = [&](const float2* ml, const float* opart, int64_t at) {
-    const float2 x = ml[at];
-    if (x.x == -INFINITY) return;                           // this part saw no key
-    const float f = ex2(x.x - M);
-    l = fmaf(x.y, f, l);
+  enigma_serving::RowJoin<V> join;
+  join.best(p.p_ml + p_at, p_step, n_p, lane);
+  join.best(p.d_ml + d_at, p.rows, n_d, lane);
+  join.seal();
+  join.add(p.p_ml + p_at, p_step, p.p_opart + p_at * D, p_step * D, n_p, D, lane);
+  join.add(p.d_ml + d_at, p.rows, p.d_opart + d_at * D, int64_t(p.rows) * D, n_d, D, lane);
+  const float inv = join.l == 0.f ? 0.f : 1.f / join.l;
+  __nv_bfloat16* out = p.out + b * p.o_batch + h * p.o_head + lane;
 #pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] = fmaf(opart[at * D + lane * V + v], f, acc[v]);
-  };
-  for (int i = 0; i < n_p; ++i) add(p.p_ml, p.p_opart, p_at + i * p_step);
-  for (int i = 0; i < n_d; ++i) add(p.d_ml, p.d_opart, d_at + int64_t(i) * p.rows);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  __nv_bfloat16* out = p.out + b * p.o_batch + h * p.o_head + lane * V;
-#pragma unroll
-  for (int v = 0; v < V; v += 2)
-    *reinterpret_cast<uint32_t*>(out + v) = pack_bf16x2(acc[v] * inv, acc[v + 1] * inv);
+  for (int v = 0; v < V; ++v) out[32 * v] = __float2bfloat16_rn(join.acc[v] * inv);
 }
 
 // ============================================================================ host
@@ -510,7 +456,7 @@ Layout layout_of(const enigma_sdpa_shared_prefix_desc& d) {
   y.blocks = (y.group + ROWS - 1) / ROWS;
   y.rows = (y.group + y.blocks - 1) / y.blocks;
   y.ctas = sms * (d.head_dim == 64 ? 3 : 2);
-  const int64_t d_slots = int64_t(y.ctas) + d.batch * d.heads_kv * y.blocks;
+  const int64_t d_slots = (int64_t(y.ctas) + d.batch * d.heads_kv * y.blocks) * DWARPS;
   size_t at = 0;
   auto take = [&](int64_t bytes) {
     const size_t here = at;
@@ -608,10 +554,19 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
   p.ml = reinterpret_cast<float2*>(ws + y.d_ml);
   p.starts = reinterpret_cast<int32_t*>(ws + y.starts);
   p.status = status;
-  const int smem = DCfg<D>::SMEM + int(d.batch + 1) * 4;
-  e = cudaFuncSetAttribute(paged_decode_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           DCfg<D>::SMEM + 4097 * 4);
-  if (e != cudaSuccess) return e;
+  const int smem = DCfg<D>::SMEM + int(2 * d.batch + 1) * 4;
+  {
+    static std::atomic<uint64_t> ready{0};                  // devices where the attribute is set
+    int dev = 0;
+    e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && !(dev < 64 && (ready.load() >> dev & 1))) {
+      e = cudaFuncSetAttribute(paged_decode_kernel<D>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               DCfg<D>::SMEM + 8193 * 4);
+      if (e == cudaSuccess && dev < 64) ready.fetch_or(uint64_t(1) << dev);
+    }
+    if (e != cudaSuccess) return e;
+  }
   paged_decode_kernel<D><<<unsigned(y.ctas), DTHREADS, smem, s>>>(mk, mv, p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;

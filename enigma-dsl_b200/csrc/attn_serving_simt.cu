@@ -278,9 +278,8 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec) {
   }
 }
 
-// Joins the partial results of split rows: O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in
-// the order of the parts.  One warp per row; grid (groups, rows / 8).
-template <typename T>
+// Joins the partial results of split rows.  One warp per row; grid (groups, rows / 8).
+template <typename T, int V>
 __global__ void __launch_bounds__(256)
 packed_join_kernel(const enigma_sdpa_packed_desc p) {
   const int lane = threadIdx.x & 31, D = int(p.head_dim), G = int(p.heads_q / p.heads_kv);
@@ -293,33 +292,28 @@ packed_join_kernel(const enigma_sdpa_packed_desc p) {
   const int state = r / 128, row = r % 128;
   const int tok = g.tok0 + state * g.tokens + row / G;
   if (row >= g.tokens * G || tok >= g.tok_end || tok >= p.tokens_q || (g.alt && state > 0)) return;
-  const int n = g.alt ? 2 * g.parts : g.parts, step = g.alt ? 1 : 2;
-  const int64_t first = g.slot + (g.alt ? 0 : state);
-  float M = -INFINITY;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, ml[(first + i * step) * 128 + row].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  float acc[kMaxDPerLane] = {};
-  float l = 0.f;
-  for (int i = 0; i < n; ++i) {
-    const int64_t at = (first + i * step) * 128 + row;
-    const float2 x = ml[at];
-    if (x.x == -INFINITY) continue;                             // this part saw no key
-    const float f = exp2f(x.x - M);
-    l = fmaf(x.y, f, l);
-#pragma unroll
-    for (int v = 0; v < kMaxDPerLane; ++v)
-      if (lane + 32 * v < D) acc[v] = fmaf(opart[at * D + lane + 32 * v], f, acc[v]);
-  }
+  const int n = g.alt ? 2 * g.parts : g.parts, step = (g.alt ? 1 : 2) * 128;
+  const int64_t at = int64_t(g.slot + (g.alt ? 0 : state)) * 128 + row;
+  enigma_serving::RowJoin<V> join;
+  join.best(ml + at, step, n, lane);
+  join.seal();
+  join.add(ml + at, step, opart + at * D, int64_t(step) * D, n, D, lane);
   const int h = g.kvh * G + row % G;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = join.l == 0.f ? 0.f : 1.f / join.l;
   T* out = static_cast<T*>(p.out) + tok * p.o_token + h * p.o_head;
 #pragma unroll
-  for (int v = 0; v < kMaxDPerLane; ++v)
-    if (lane + 32 * v < D) store(out + lane + 32 * v, acc[v] * inv);
+  for (int v = 0; v < V; ++v)
+    if (lane + 32 * v < D) store(out + lane + 32 * v, join.acc[v] * inv);
   if (p.lse != nullptr && lane == 0)
     p.lse[int64_t(tok) * p.heads_q + h] =
-        l == 0.f ? -INFINITY : (M + log2f(l)) * 0.6931471805599453f;
+        join.l == 0.f ? -INFINITY : (join.M + log2f(join.l)) * 0.6931471805599453f;
+}
+
+template <typename T>
+void launch_join(const enigma_sdpa_packed_desc& d, const dim3 grid, cudaStream_t s) {
+  if (d.head_dim <= 64) packed_join_kernel<T, 2><<<grid, 256, 0, s>>>(d);
+  else if (d.head_dim <= 128) packed_join_kernel<T, 4><<<grid, 256, 0, s>>>(d);
+  else packed_join_kernel<T, 8><<<grid, 256, 0, s>>>(d);
 }
 
 template <typename T, int DP>
@@ -404,8 +398,8 @@ cudaError_t sdpa_packed_join_launch(const enigma_sdpa_packed_desc& d, cudaStream
   const int groups = d.header[enigma_serving::kGroups];
   if (groups == 0) return cudaSuccess;
   const dim3 grid(unsigned(groups), 2 * ENIGMA_PACKED_TILE_ROWS / 8);
-  if (d.dtype == ENIGMA_DTYPE_F32) packed_join_kernel<float><<<grid, 256, 0, s>>>(d);
-  else packed_join_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(d);
+  if (d.dtype == ENIGMA_DTYPE_F32) launch_join<float>(d, grid, s);
+  else launch_join<__nv_bfloat16>(d, grid, s);
   return cudaGetLastError();
 }
 

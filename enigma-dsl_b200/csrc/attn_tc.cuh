@@ -38,6 +38,8 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
+
 #include "attn_serving.cuh"
 
 namespace enigma_tc {
@@ -631,7 +633,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         }
       } else {
         const int64_t row = int64_t(w.slot + ti) * BM + r;
-        if (live) p.ml[row] = none ? make_float2(-INFINITY, 0.f) : make_float2(m_used * c, l);
+        // (A row of nothing but NaN scores has l = NaN and no maximum: it is not empty.)
+        if (live)
+          p.ml[row] = none || l == 0.f ? make_float2(-INFINITY, 0.f)
+                                       : make_float2(m_used == -INFINITY ? 0.f : m_used * c, l);
         if (n_my > 0) {
 #pragma unroll 1
           for (int k = 0; k < D; k += 16) {
@@ -689,21 +694,24 @@ inline bool make_map(CUtensorMap* m, const void* base, int rank, const cuuint64_
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Launch attributes of one instantiation (shared memory, registers enough for the split).
+// Launch attributes of one instantiation (shared memory, registers enough for the split), set
+// once per device: they outlast the call, and setting them costs a microsecond.
 template <int D, bool PAGED>
 cudaError_t prepare_kernel() {
   const auto kernel = attn_tc_kernel<D, PAGED>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       Cfg<D>::SMEM);
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  static int regs = -1;
-  if (regs < 0) {
-    cudaFuncAttributes fa;
-    e = cudaFuncGetAttributes(&fa, kernel);
-    if (e != cudaSuccess) return e;
-    regs = fa.numRegs;
-  }
-  return regs < LAUNCH_REGS ? cudaErrorInvalidConfiguration : cudaSuccess;
+  if (dev < 64 && (ready.load() >> dev & 1)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+  if (e != cudaSuccess) return e;
+  cudaFuncAttributes fa;
+  e = cudaFuncGetAttributes(&fa, kernel);
+  if (e != cudaSuccess) return e;
+  if (fa.numRegs < LAUNCH_REGS) return cudaErrorInvalidConfiguration;
+  if (dev < 64) ready.fetch_or(uint64_t(1) << dev);
+  return cudaSuccess;
 }
 
 }  // namespace enigma_tc

@@ -8,7 +8,9 @@ Inputs must be contiguous CUDA tensors; there is no CPU path.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
+import struct
 from typing import Optional
 
 from . import _native
@@ -151,46 +153,57 @@ class PackedPlan:
                      ctypes.byref(count))
         self.heads_q, self.heads_kv, self.causal = int(heads_q), int(heads_kv), bool(causal)
         self.tokens_q, self.tokens_k = sum(lens_q), sum(lens_k)
-        self.header = (ctypes.c_int32 * _native.PACKED_PLAN_HEADER)(
-            *ints[:_native.PACKED_PLAN_HEADER].tolist())
+        self.header = tuple(ints[:_native.PACKED_PLAN_HEADER].tolist())
         self.ints = ints.to(device)
+        self._workspace = {}
 
     def workspace_bytes(self, head_dim: int) -> int:
         """Device memory that a call with this plan needs (0 unless it splits rows)."""
-        need = ctypes.c_size_t()
-        _native.call("enigma_sdpa_packed_workspace_bytes", self.header, head_dim,
-                     ctypes.byref(need))
-        return need.value
+        if head_dim not in self._workspace:
+            need = ctypes.c_size_t()
+            _native.call("enigma_sdpa_packed_workspace_bytes",
+                         (ctypes.c_int32 * len(self.header))(*self.header), head_dim,
+                         ctypes.byref(need))
+            self._workspace[head_dim] = need.value
+        return self._workspace[head_dim]
 
 
-class _PackedDesc(ctypes.Structure):
-    """Mirror of enigma_sdpa_packed_desc (include/enigma_cuda.h)."""
+# enigma_sdpa_packed_desc (include/enigma_cuda.h): sizes and strides, scale and flags, the plan's
+# header, pointers.  Packed bytes cost a third of filling a ctypes structure.
+_PACKED_DESC = struct.Struct(f"13qf3i{_native.PACKED_PLAN_HEADER}i8Q")
 
-    _fields_ = [(n, ctypes.c_int64) for n in ("tokens_q", "tokens_k", "heads_q", "heads_kv",
-                                              "head_dim", "q_token", "q_head", "k_token",
-                                              "k_head", "v_token", "v_head", "o_token",
-                                              "o_head")] + \
-               [("scale", ctypes.c_float)] + \
-               [(n, ctypes.c_int32) for n in ("causal", "dtype", "reserved")] + \
-               [("header", ctypes.c_int32 * _native.PACKED_PLAN_HEADER)] + \
-               [(n, ctypes.c_void_p) for n in ("plan", "q", "k", "v", "out", "lse",
-                                               "workspace")] + \
-               [("workspace_bytes", ctypes.c_size_t)]
+
+def _raw_stream(t) -> int:
+    """The current stream of t's device, without the Stream object that _stream_ptr makes."""
+    return _torch()._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _check_rows(name, *ts):
     """CUDA tensors of one device and dtype whose last axis is contiguous."""
+    first = ts[0]
+    device, dtype = first.device, first.dtype
+    if device.type != "cuda":
+        raise ValueError("enigma CUDA operators take CUDA tensors (no CPU fallback)")
     for t in ts:
-        if not t.is_cuda:
-            raise ValueError("enigma CUDA operators take CUDA tensors (no CPU fallback)")
-        if t.device != ts[0].device:
-            raise ValueError("all tensors must be on the same device")
-        if t.dtype != ts[0].dtype:
+        if t.device != device:
+            raise ValueError("enigma CUDA operators take CUDA tensors of one device")
+        if t.dtype != dtype:
             raise TypeError(f"{name}: tensors must share a dtype")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
+        if t.stride(-1) != 1 and t.shape[-1] > 1:
             raise ValueError(f"{name}: the last axis must be contiguous")
-    index = ts[0].device.index
-    ensure_device(index if index is not None else 0)
+    if device.index not in _initialised:
+        ensure_device(device.index)
+
+
+def _scratch(name, workspace, need, like):
+    """(address, bytes) of the caller's workspace or of a new one, and what keeps it alive."""
+    if workspace is None:
+        if need == 0:
+            return 0, 0, None
+        workspace = like.new_empty(need, dtype=_torch().uint8)
+    elif workspace.device != like.device or not workspace.is_contiguous():
+        raise ValueError(f"{name}: workspace must be contiguous on the data's device")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
 def sdpa_packed(q, k, v, plan: PackedPlan, scale: Optional[float] = None, out=None,
@@ -216,40 +229,38 @@ def sdpa_packed(q, k, v, plan: PackedPlan, scale: Optional[float] = None, out=No
     if (tq, tk) != (plan.tokens_q, plan.tokens_k):
         raise ValueError(f"sdpa_packed: the plan's lengths sum to {plan.tokens_q} / "
                          f"{plan.tokens_k} tokens, the tensors hold {tq} / {tk}")
+    dtype = _dtype_code(q)
     if out is None:
-        out = torch.empty((tq, hq, d), dtype=q.dtype, device=q.device)
+        out = q.new_empty((tq, hq, d))
     elif out.shape != q.shape:
         raise ValueError("sdpa_packed: out must have q's shape")
-    dtype = _dtype_code(q)
     _check_rows("sdpa_packed", q, k, v, out)
     if plan.ints.device != q.device:
-        raise ValueError("all tensors must be on the same device")
-    lse = torch.empty((tq, hq), dtype=torch.float32, device=q.device) if return_lse else None
-    if workspace is None:
-        workspace = torch.empty(plan.workspace_bytes(d), dtype=torch.uint8, device=q.device)
-    elif workspace.device != q.device or not workspace.is_contiguous():
-        raise ValueError("sdpa_packed: workspace must be contiguous on the data's device")
-    desc = _PackedDesc(tq, tk, hq, hk, d, *q.stride()[:2], *k.stride()[:2],
-                       *v.stride()[:2], *out.stride()[:2],
-                       1.0 / math.sqrt(d) if scale is None else scale, int(plan.causal), dtype, 0,
-                       plan.header, plan.ints.data_ptr(), q.data_ptr(), k.data_ptr(),
-                       v.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None,
-                       workspace.data_ptr(), workspace.numel() * workspace.element_size())
-    _native.call("enigma_sdpa_packed", ctypes.byref(desc), _stream_ptr(q))
+        raise ValueError("sdpa_packed: the plan is on another device")
+    lse = q.new_empty((tq, hq), dtype=torch.float32) if return_lse else None
+    ws, ws_bytes, keep = _scratch("sdpa_packed", workspace, plan.workspace_bytes(d), q)
+    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+    desc = _PACKED_DESC.pack(tq, tk, hq, hk, d, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0],
+                             os[1], 1.0 / math.sqrt(d) if scale is None else scale, plan.causal,
+                             dtype, 0, *plan.header, plan.ints.data_ptr(), q.data_ptr(),
+                             k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                             lse.data_ptr() if return_lse else 0, ws, ws_bytes)
+    _native.call("enigma_sdpa_packed", desc, _raw_stream(q))
     return (out, lse) if return_lse else out
 
 
-class _SharedPrefixDesc(ctypes.Structure):
-    """Mirror of enigma_sdpa_shared_prefix_desc (include/enigma_cuda.h)."""
+# enigma_sdpa_shared_prefix_desc: sizes and strides, scale and dtype, pointers, workspace.
+_SHARED_DESC = struct.Struct("15qfi9Q")
 
-    _fields_ = [(n, ctypes.c_int64) for n in ("batch", "heads_q", "heads_kv", "head_dim", "page",
-                                              "pages", "table_width", "n_slots", "prefix_len",
-                                              "q_batch", "q_head", "o_batch", "o_head", "k_page",
-                                              "v_page")] + \
-               [("scale", ctypes.c_float), ("dtype", ctypes.c_int32)] + \
-               [(n, ctypes.c_void_p) for n in ("table", "lens", "slots", "q", "k_pages",
-                                               "v_pages", "out", "workspace")] + \
-               [("workspace_bytes", ctypes.c_size_t)]
+
+@functools.lru_cache(maxsize=4096)
+def _shared_workspace_bytes(device_index, *sizes) -> int:
+    """enigma_sdpa_shared_prefix_workspace_bytes for the desc's sizes (it reads nothing else)."""
+    need = ctypes.c_size_t()
+    _native.call("enigma_sdpa_shared_prefix_workspace_bytes",
+                 _SHARED_DESC.pack(*sizes[:9], 0, 0, 0, 0, 0, 0, 1.0, sizes[9], *([0] * 9)),
+                 ctypes.byref(need))
+    return need.value
 
 
 def _check_int32(name, device, *ts):
@@ -282,33 +293,26 @@ def sdpa_shared_prefix(q, k_pages, v_pages, table, lens, prefix_len: int = 0, sl
         raise ValueError("sdpa_shared_prefix: expected table [n, width] and lens [n]")
     if slots is not None and tuple(slots.shape) != (b,):
         raise ValueError("sdpa_shared_prefix: slots must name one row per sequence")
+    dtype = _dtype_code(q)
     if out is None:
-        out = torch.empty((b, hq, d), dtype=q.dtype, device=q.device)
+        out = q.new_empty((b, hq, d))
     elif out.shape != q.shape:
         raise ValueError("sdpa_shared_prefix: out must have q's shape")
-    dtype = _dtype_code(q)
     _check_rows("sdpa_shared_prefix", q, k_pages, v_pages, out)
-    for t in (k_pages, v_pages):
-        if t.stride()[1:] != (page * d, d, 1):
-            raise ValueError("sdpa_shared_prefix: a page must be contiguous")
+    ks, vs = k_pages.stride(), v_pages.stride()
+    if ks[1:] != (page * d, d, 1) or vs[1:] != (page * d, d, 1):
+        raise ValueError("sdpa_shared_prefix: a page must be contiguous")
     _check_int32("sdpa_shared_prefix", q.device, table, lens, *(() if slots is None else (slots,)))
-    desc = _SharedPrefixDesc(b, hq, hk, d, page, pages, table.shape[1], table.shape[0],
-                             int(prefix_len), *q.stride()[:2], *out.stride()[:2],
-                             k_pages.stride(0), v_pages.stride(0),
+    sizes = (b, hq, hk, d, page, pages, table.shape[1], table.shape[0], int(prefix_len))
+    need = _shared_workspace_bytes(q.device.index, *sizes, dtype)
+    ws, ws_bytes, keep = _scratch("sdpa_shared_prefix", workspace, need, q)
+    qs, os = q.stride(), out.stride()
+    desc = _SHARED_DESC.pack(*sizes, qs[0], qs[1], os[0], os[1], ks[0], vs[0],
                              1.0 / math.sqrt(d) if scale is None else scale, dtype,
                              table.data_ptr(), lens.data_ptr(),
-                             None if slots is None else slots.data_ptr(), q.data_ptr(),
-                             k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr())
-    if workspace is None:
-        need = ctypes.c_size_t()
-        _native.call("enigma_sdpa_shared_prefix_workspace_bytes", ctypes.byref(desc),
-                     ctypes.byref(need))
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-    elif workspace.device != q.device or not workspace.is_contiguous():
-        raise ValueError("sdpa_shared_prefix: workspace must be contiguous on the data's device")
-    desc.workspace = workspace.data_ptr()
-    desc.workspace_bytes = workspace.numel() * workspace.element_size()
-    _native.call("enigma_sdpa_shared_prefix", ctypes.byref(desc), _stream_ptr(q))
+                             0 if slots is None else slots.data_ptr(), q.data_ptr(),
+                             k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), ws, ws_bytes)
+    _native.call("enigma_sdpa_shared_prefix", desc, _raw_stream(q))
     return out
 
 

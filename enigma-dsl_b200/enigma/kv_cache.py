@@ -79,6 +79,9 @@ class PagedKVCache:
         import torch
         if not isinstance(values, torch.Tensor):
             values = torch.as_tensor(values, dtype=torch.int32)
+        if values.dtype == torch.int32 and values.device == self.k.device and values.dim() == 1 \
+                and values.is_contiguous() and (like is None or values.shape == like.shape):
+            return values
         if values.dim() != 1:
             raise ValueError(f"{name}: expected one number per sequence")
         if like is not None and values.shape != like.shape:
@@ -88,7 +91,7 @@ class PagedKVCache:
         return values.contiguous()
 
     def _call(self, name, *args):
-        _native.call(name, self._ref, *args, cuda_ops._stream_ptr(self.k))
+        _native.call(name, self._ref, *args, cuda_ops._raw_stream(self.k))
 
     def fork(self, parents, children) -> None:
         """Slot children[i] continues slot parents[i]: it lets go of what it held, shares the
