@@ -26,6 +26,7 @@ constexpr int CHUNK = 64;
 constexpr int DWARPS = 4;
 constexpr int DTHREADS = (DWARPS + 1) * 32;
 constexpr int ROWS = 16;                     // query heads of a unit
+constexpr int PAGES = 128;                   // page numbers looked up at once
 
 template <int D>
 struct DCfg {
@@ -41,6 +42,10 @@ struct DecodeParams {
   const int32_t *table, *lens, *slots;
   int batch, heads_kv, group, blocks, rows;  // blocks of `rows` <= 16 heads per group
   int width, n_slots, pages, page_shift, box_shift, prefix, base;
+  int fold;                                  // the prefix's keys are read here too
+  int direct;                                // a CTA per unit, which writes the final result
+  __nv_bfloat16* out;
+  int64_t o_batch, o_head;
   float scale_log2;
   float* opart;                              // [slot][rows][D]
   float2* ml;                                // [slot][rows]
@@ -67,6 +72,16 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Barrier over the DWARPS consumer warps; whether all say yes.
+__device__ __forceinline__ bool warps_all(bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %1, 0;\n\t"
+      "barrier.cta.red.and.pred b, 1, %2, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
+      : "=r"(all) : "r"(ok ? 1u : 0u), "n"(DWARPS * 32) : "memory");
+  return all != 0;
+}
+
 // floor(n c / P) for n c < 2^53 without a 64-bit division.
 __device__ __forceinline__ int64_t share(int64_t n, int64_t c, int64_t P) {
   const int64_t x = n * c;
@@ -81,9 +96,34 @@ __device__ __forceinline__ int owner(int64_t x, int64_t T, int64_t P) {
   return int(((x + 1) * P - 1) / T);
 }
 
-// Chunks of sequence b's own keys.
-__device__ __forceinline__ int chunks_of(int len, int prefix, int base) {
-  return len > prefix ? (len - base + CHUNK - 1) / CHUNK : 0;
+// Chunks of a sequence: of the prefix, if it is read here, then of its own keys (from `base`, the
+// prefix's end rounded down to a chunk).
+__device__ __forceinline__ int prefix_chunks(const DecodeParams& p, int len) {
+  return p.fold ? (min(len, p.prefix) + CHUNK - 1) / CHUNK : 0;
+}
+__device__ __forceinline__ int chunks_of(const DecodeParams& p, int len) {
+  return prefix_chunks(p, len) + (len > p.prefix ? (len - p.base + CHUNK - 1) / CHUNK : 0);
+}
+
+// Chunk j of a sequence: its first key, and the keys [lo, hi) that count.
+struct Chunk {
+  int key0, lo, hi, seq;       // seq: whose table row holds its pages
+};
+__device__ __forceinline__ Chunk chunk_at(const DecodeParams& p, int b, int len, int j) {
+  const int np = prefix_chunks(p, len);
+  Chunk c;
+  if (j < np) {
+    c.key0 = j * CHUNK;
+    c.lo = 0;
+    c.hi = min(len, p.prefix);
+    c.seq = 0;
+  } else {
+    c.key0 = p.base + (j - np) * CHUNK;
+    c.lo = p.prefix;
+    c.hi = len;
+    c.seq = b;
+  }
+  return c;
 }
 
 // A run of one unit's chunks.
@@ -127,9 +167,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   int* s_starts = reinterpret_cast<int*>(ring + ST * 2 * C::TILE);    // [batch + 1]
   int* s_len = s_starts + p.batch + 1;                                // [batch]
   __shared__ uint64_t full[ST], empty[ST];
-  __shared__ int s_warp[DWARPS + 1];
+  __shared__ float s_m[DWARPS][ROWS], s_l[DWARPS][ROWS];    // direct
+  __shared__ int s_warp[DWARPS + 1], s_pages[PAGES];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t most = int64_t(p.width) << p.page_shift;
+  griddep_launch_dependents();
 
   if (tid == 0) {
     for (int s = 0; s < ST; ++s) {
@@ -148,7 +190,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     if (b < p.batch) {
       const int len = len_of(p.lens, p.slots, p.n_slots, most, b);
       s_len[b] = len;
-      v = chunks_of(len, p.prefix, p.base);
+      v = chunks_of(p, len);
     }
     int x = v;
 #pragma unroll
@@ -166,14 +208,37 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   }
   if (tid == 0) s_starts[p.batch] = run;
   __syncthreads();
-  if (blockIdx.x == 0)
+  if (blockIdx.x == 0 && !p.direct)
     for (int b = tid; b <= p.batch; b += DTHREADS) p.starts[b] = s_starts[b];
 
   const int per_b = p.heads_kv * p.blocks;
   const int64_t T = int64_t(run) * per_b;
   const int64_t P = min(int64_t(gridDim.x), T);
-  if (int64_t(blockIdx.x) >= P) return;
-  const int64_t c0 = share(T, blockIdx.x, P), c1 = share(T, int64_t(blockIdx.x) + 1, P);
+  // This kernel reads nothing of the prefix kernel's, with which it shares the SMs, but the join
+  // waits only for this one: so it ends after that one.
+  if (!p.direct && int64_t(blockIdx.x) >= P) {
+    griddep_wait();
+    return;
+  }
+  int64_t c0, c1;
+  if (p.direct) {                            // unit blockIdx.x; without keys: zeros
+    const int b = int(blockIdx.x) / per_b, n = s_starts[b + 1] - s_starts[b];
+    c0 = int64_t(s_starts[b]) * per_b + int64_t(int(blockIdx.x) - b * per_b) * n;
+    c1 = c0 + n;
+    if (n == 0) {
+      const int u = int(blockIdx.x) - b * per_b, block = u % p.blocks;
+      const int rows = min(p.rows, p.group - block * p.rows);
+      __nv_bfloat16* to = p.out + b * p.o_batch +
+                          int64_t(u / p.blocks * p.group + block * p.rows) * p.o_head;
+      for (int x = tid; x < rows * (D / 8); x += DTHREADS)
+        *reinterpret_cast<uint4*>(to + x / (D / 8) * p.o_head + x % (D / 8) * 8) =
+            make_uint4(0, 0, 0, 0);
+      return;
+    }
+  } else {
+    c0 = share(T, blockIdx.x, P);
+    c1 = share(T, int64_t(blockIdx.x) + 1, P);
+  }
 
   if (warp == DWARPS) {
     // ---------------------------------------------------------------- producer
@@ -181,21 +246,33 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     // columns 64 (x % ATOMS).
     const int x = lane & 15, box = x / C::ATOMS, atom = x % C::ATOMS;
     const bool is_v = lane >= 16;
+    const int per = CHUNK >> p.box_shift, ahead = PAGES / per;   // boxes per chunk; chunks looked up
     int i = 0;
     for (int64_t at = c0; at < c1;) {
       const Segment s = segment_at(s_starts, p.batch, per_b, p.blocks, at, c1);
       const int len = s_len[s.b];
-      auto look_up = [&](int j) {
-        const int key = p.base + j * CHUNK + (box << p.box_shift);
-        return page_at(p.table, p.slots, p.n_slots, p.width, p.pages, s.b, key >> p.page_shift);
-      };
-      const bool can = box < (CHUNK >> p.box_shift);
-      int page = can ? look_up(s.j0) : 0;
       for (int j = s.j0; j < s.j0 + s.n; ++j, ++i) {
-        const int key0 = p.base + j * CHUNK;
-        const int boxes = (min(CHUNK, len - key0) + (1 << p.box_shift) - 1) >> p.box_shift;
-        const int page_now = page;
-        if (can && j + 1 < s.j0 + s.n) page = look_up(j + 1);
+        const Chunk c = chunk_at(p, s.b, len, j);
+        const int key0 = c.key0;
+        const int boxes = (min(CHUNK, c.hi - key0) + (1 << p.box_shift) - 1) >> p.box_shift;
+        // Page numbers of the next `ahead` chunks at once: one look-up per chunk, even if made a
+        // chunk ahead, left the ring waiting for the table's latency.
+        const int in = (j - s.j0) % ahead;
+        if (in == 0) {
+          __syncwarp();
+#pragma unroll
+          for (int y = 0; y < PAGES; y += 32) {
+            const int jj = j + (y + lane) / per;
+            if (jj < s.j0 + s.n) {
+              const Chunk cc = chunk_at(p, s.b, len, jj);
+              const int key = cc.key0 + (((y + lane) % per) << p.box_shift);
+              s_pages[y + lane] = page_at(p.table, p.slots, p.n_slots, p.width, p.pages, cc.seq,
+                                          key >> p.page_shift);
+            }
+          }
+          __syncwarp();
+        }
+        const int page_now = box < boxes ? s_pages[in * per + box] : 0;
         const int st = i % ST;
         if (!__all_sync(0xffffffffu, mbar_wait(&empty[st], ((i / ST) & 1) ^ 1, p.status))) {
           at = c1;
@@ -213,6 +290,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       }
       at += s.n;
     }
+    griddep_wait();
     return;
   }
 
@@ -248,7 +326,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       if (!ok) break;
       uint8_t* tile_k = ring + 2 * st * C::TILE;
       uint8_t* tile_v = tile_k + C::TILE;
-      const int key0 = p.base + j * CHUNK + warp * 16;      // this warp's first key
+      const Chunk ch = chunk_at(p, s.b, len, j);
+      const int key0 = ch.key0 + warp * 16;                 // this warp's first key
       float sc[2][4];
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -264,19 +343,19 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         mma_16816(sc[0], q[kk], b[0], b[1]);
         mma_16816(sc[1], q[kk], b[2], b[3]);
       }
-      if (key0 + 16 > len || key0 < p.prefix) {             // warp-uniform
+      if (key0 + 16 > ch.hi || key0 < ch.lo) {              // warp-uniform
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int key = key0 + n * 8 + quad * 2 + (e & 1);
-            if (key >= len || key < p.prefix) sc[n][e] = -INFINITY;
+            if (key >= ch.hi || key < ch.lo) sc[n][e] = -INFINITY;
           }
         // Rows past the end hold whatever the page or the ring held, rows of the prefix
         // whatever this sequence's page has there: 0 * NaN must not be.
         for (int x = lane; x < 16 * 8 * C::ATOMS; x += 32) {
           const int row = x >> 3 & 15;
-          if (key0 + row >= len || key0 + row < p.prefix)
+          if (key0 + row >= ch.hi || key0 + row < ch.lo)
             *reinterpret_cast<uint4*>(tile_v + (x >> 7) * CHUNK * 128 + (warp * 16 + row) * 128 +
                                       (x & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
@@ -322,6 +401,49 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
+    }
+    if (p.direct) {
+      // The ring is idle once every warp is here: it takes the warps' states, each thread sums
+      // two columns of a row over the warps, in their order.
+      if (!warps_all(ok)) return;                           // a wait ran out (status is set)
+      float* s_o = reinterpret_cast<float*>(ring);          // [DWARPS][ROWS][D]
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        const int row = g + 8 * h;
+        if (quad == 0) {
+          s_m[warp][row] = m[h] == -INFINITY ? (l[h] == 0.f ? -INFINITY : 0.f) : m[h] * p.scale_log2;
+          s_l[warp][row] = l[h];
+        }
+        if (row >= rows) continue;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+          *reinterpret_cast<float2*>(s_o + (warp * ROWS + row) * D + quad * 2 + n * 8) =
+              make_float2(o[n][2 * h], o[n][2 * h + 1]);
+      }
+      warps_all(true);
+      for (int x = tid; x < rows * (D / 2); x += DWARPS * 32) {
+        const int row = x / (D / 2), d = x % (D / 2) * 2;
+        float M = s_m[0][row];
+#pragma unroll
+        for (int w = 1; w < DWARPS; ++w) M = fmaxf(M, s_m[w][row]);
+        float2 acc = make_float2(0.f, 0.f);
+        float L = 0.f;
+#pragma unroll
+        for (int w = 0; w < DWARPS; ++w) {
+          const float f = s_m[w][row] == -INFINITY ? 0.f : ex2(s_m[w][row] - M);
+          const float2 v = *reinterpret_cast<const float2*>(s_o + (w * ROWS + row) * D + d);
+          acc.x = fmaf(v.x, f, acc.x);
+          acc.y = fmaf(v.y, f, acc.y);
+          L = fmaf(s_l[w][row], f, L);
+        }
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const int64_t at = s.b * p.o_batch +
+                           int64_t(s.kvh * p.group + s.block * p.rows + row) * p.o_head + d;
+        *reinterpret_cast<uint32_t*>(p.out + at) = pack_bf16x2(acc.x * inv, acc.y * inv);
+      }
+      return;
     }
     if (!ok) return;                                        // a wait ran out (status is set)
     const int64_t slot = (int64_t(blockIdx.x) + s.unit) * DWARPS + warp;
@@ -369,6 +491,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const JoinParams p) {
   const int lane = threadIdx.x & 31;
   const int64_t id = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
   if (id >= int64_t(p.batch) * p.heads_q) return;
+  griddep_wait();
   const int b = int(id / p.heads_q), h = int(id - int64_t(b) * p.heads_q);
   const int kvh = h / p.group, gh = h - kvh * p.group;
   // Prefix partials: rows pf + i * p_step of [slot * 128 + row].
@@ -430,9 +553,12 @@ int log2_of(int64_t x) {
   return n;
 }
 
+constexpr int64_t kFoldBytes = 128ll << 20, kDirectKeys = 1024;
+
 struct Layout {
   int group, tokens, row_tiles, pairs, splits, prefix;    // prefix part
   int blocks, rows, ctas;                                 // own part
+  bool fold, direct;
   size_t p_opart, p_ml, d_opart, d_ml, starts, total;     // byte offsets
 };
 
@@ -446,7 +572,14 @@ Layout layout_of(const enigma_sdpa_shared_prefix_desc& d) {
   y.row_tiles = int((d.batch + y.tokens - 1) / y.tokens);
   y.pairs = (y.row_tiles + 1) / 2;
   const int tiles = (y.prefix + BN - 1) / BN;
-  if (tiles > 0) {
+  // Short rows: one CTA per unit reads all its keys, the prefix's too, and writes the result; no
+  // second and third launch, no partial results.  Measured (graph, us, alone / with the prefix
+  // apart): 4 x 512 keys, 2 kv heads of 64: 10.5 / 12.4; 16 x 512, 8 of 128: 10.7 / 14.6; 32 x 1024
+  // + 128: 19.1 / 23.8; but 8 x 2048 + 128: 26.2 / 15.2, 32 x 2048 + 64, 2 of 64: 27.0 / 16.3.
+  y.direct = d.table_width * d.page <= kDirectKeys &&
+             d.batch * y.prefix * d.heads_kv * d.head_dim * 4 <= kFoldBytes;
+  y.fold = y.direct && y.prefix > 0;
+  if (tiles > 0 && !y.fold) {
     // As many parts of the keys as there are SMs, each at least two tiles.
     const int64_t units = int64_t(d.heads_kv) * y.pairs;
     y.splits = int(std::max<int64_t>(1, std::min<int64_t>(sms / std::max<int64_t>(units, 1),
@@ -456,6 +589,10 @@ Layout layout_of(const enigma_sdpa_shared_prefix_desc& d) {
   y.blocks = (y.group + ROWS - 1) / ROWS;
   y.rows = (y.group + y.blocks - 1) / y.blocks;
   y.ctas = sms * (d.head_dim == 64 ? 3 : 2);
+  if (y.direct) {
+    y.ctas = int(d.batch * d.heads_kv) * y.blocks;
+    return y;
+  }
   const int64_t d_slots = (int64_t(y.ctas) + d.batch * d.heads_kv * y.blocks) * DWARPS;
   size_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -549,6 +686,11 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
   p.box_shift = box_shift;
   p.prefix = y.prefix;
   p.base = y.prefix / CHUNK * CHUNK;
+  p.fold = y.fold;
+  p.direct = y.direct;
+  p.out = static_cast<__nv_bfloat16*>(d.out);
+  p.o_batch = d.o_batch;
+  p.o_head = d.o_head;
   p.scale_log2 = scale_log2;
   p.opart = reinterpret_cast<float*>(ws + y.d_opart);
   p.ml = reinterpret_cast<float2*>(ws + y.d_ml);
@@ -567,9 +709,13 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
     }
     if (e != cudaSuccess) return e;
   }
-  paged_decode_kernel<D><<<unsigned(y.ctas), DTHREADS, smem, s>>>(mk, mv, p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+  if (y.splits > 0) {
+    e = enigma::launch_dependent(paged_decode_kernel<D>, unsigned(y.ctas), DTHREADS, smem, s, mk, mv, p);
+  } else {
+    paged_decode_kernel<D><<<unsigned(y.ctas), DTHREADS, smem, s>>>(mk, mv, p);
+    e = cudaGetLastError();
+  }
+  if (e != cudaSuccess || y.direct) return e;
   JoinParams j = {};
   j.out = static_cast<__nv_bfloat16*>(d.out);
   j.o_batch = d.o_batch;
@@ -591,8 +737,7 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
   j.rows = y.rows;
   j.ctas = y.ctas;
   const unsigned grid = unsigned((d.batch * d.heads_q + 3) / 4);
-  paged_join_kernel<D><<<grid, 128, 0, s>>>(j);
-  return cudaGetLastError();
+  return enigma::launch_dependent(paged_join_kernel<D>, grid, 128, 0, s, j);
 }
 
 }  // namespace
@@ -608,7 +753,7 @@ size_t sdpa_shared_prefix_workspace(const enigma_sdpa_shared_prefix_desc& d) {
 
 cudaError_t sdpa_shared_prefix_launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
   if (!tc_takes(d)) return sdpa_paged_simt_launch(d, s);
-  note_kernel(d.prefix_len > 0 && d.batch > 1 ? "attn_tc_kernel" : "paged_decode_kernel");
+  note_kernel(layout_of(d).splits > 0 ? "attn_tc_kernel" : "paged_decode_kernel");
   return d.head_dim == 128 ? launch<128>(d, s) : launch<64>(d, s);
 }
 

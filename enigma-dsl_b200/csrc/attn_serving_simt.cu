@@ -7,6 +7,8 @@
 
 namespace {
 
+using enigma_sm100::griddep_launch_dependents;
+using enigma_sm100::griddep_wait;
 using enigma_serving::PackedGroup;
 using enigma_serving::PackedItem;
 
@@ -57,18 +59,20 @@ struct Row {
 };
 
 // ============================================================================ packed
-// A CTA takes 64 rows (token, head) of an item against its keys, 64 at a time.  128 threads, each
-// with 8 rows x 4 keys of S and 8 rows x DP / 16 columns of O, rows in pairs for the packed fp32
-// FMA.  Q, K and P lie transposed in shared memory, so a step of either product reads 8 rows
-// with two and 4 keys or columns with one 16-byte load for 32 multiply-adds.  Bound by the
-// FMA pipe and, next to it, by shared memory.
-constexpr int TR = 64, TK = 64, TT = 128;
+// A CTA takes 64 rows (token, head) of an item against its keys, TK at a time.  128 threads, each
+// with 8 rows x TK / 16 keys of S and 8 rows x DP / 16 columns of O.  Products run on the packed
+// fp32 FMA: S over pairs of the head dimension, so that neither operand has to be doubled, O over
+// pairs of rows.  K of the next tile is fetched while the softmax and P V run, V while S does.
+// Bound by the FMA pipe's issue and, next to it, by shared memory.
+constexpr int TR = 64, TT = 128;
 
 template <int DP>
 struct TileCfg {
-  static constexpr int QT = DP * TR, KT = DP * (TK + 4), VT = TK * DP, PT = TK * TR;   // floats
-  static constexpr int SMEM = (QT + (KT > PT ? KT : PT) + VT) * 4;
-  static constexpr int CPT = DP / 16;                     // columns of O per thread
+  static constexpr int TK = DP <= 64 ? 64 : 32;           // keys per tile
+  static constexpr int LD = DP + 4;                       // row of Q or K: 8 lanes meet all banks
+  static constexpr int SMEM = (TR * LD + TK * LD + TK * DP + TK * TR) * 4;
+  static constexpr int KPT = TK / 16, CPT = DP / 16;      // keys, columns of O per thread
+  static constexpr int CTAS = DP <= 128 ? 2 : 1;   // per SM, by shared memory
 };
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -96,14 +100,36 @@ __device__ __forceinline__ float4 row4(const T* p, int d, int D, bool vec) {
                      d + 2 < D ? load(p + d + 2) : 0.f, d + 3 < D ? load(p + d + 3) : 0.f);
 }
 
+// Four elements of a row to shared memory; fp32 rows of aligned tensors by an asynchronous copy
+// (zeros where there is no row), waited for by rows_landed.
+__device__ __forceinline__ void put4(float* dst, const float* p, int d, int D, bool vec, bool there) {
+  if (vec && (d + 4 <= D || !there)) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                 ::"r"(enigma_sm100::smem_u32(dst)), "l"(there ? p + d : p), "r"(there ? 16 : 0)
+                 : "memory");
+  } else {
+    *reinterpret_cast<float4*>(dst) = there ? row4(p, d, D, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+}
+__device__ __forceinline__ void put4(float* dst, const __nv_bfloat16* p, int d, int D, bool vec,
+                                     bool there) {
+  *reinterpret_cast<float4*>(dst) = there ? row4(p, d, D, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+__device__ __forceinline__ void rows_landed() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
 template <typename T, int DP>
-__global__ void __launch_bounds__(TT)
+__global__ void __launch_bounds__(TT, TileCfg<DP>::CTAS)
 packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec) {
   using C = TileCfg<DP>;
+  constexpr int TK = C::TK, LD = C::LD, KPT = C::KPT;
   extern __shared__ float4 smem4[];
-  float* s_q = reinterpret_cast<float*>(smem4);           // [DP][TR]
-  float* s_k = s_q + C::QT;                               // [DP][TK + 4]; then P [TK][TR]
-  float* s_v = s_k + (C::KT > C::PT ? C::KT : C::PT);     // [TK][DP]
+  griddep_launch_dependents();
+  float* s_q = reinterpret_cast<float*>(smem4);           // [TR][LD]
+  float* s_k = s_q + TR * LD;                             // [TK][LD]
+  float* s_v = s_k + TK * LD;                             // [TK][DP]
+  float* s_p = s_v + TK * DP;                             // [TK][TR]
   const int tid = threadIdx.x;
   const PackedItem it = reinterpret_cast<const PackedItem*>(
       p.plan + p.header[enigma_serving::kItemsAt])[blockIdx.x];
@@ -118,29 +144,45 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec) {
   if (r0 >= n) return;
   const int off = p.causal ? it.lk - it.lq + 1 : it.lk;   // a token's keys: min(lk, token + off)
   const int t_last = it.t0 + (min(r0 + TR, n) - 1) / G;
-  const int k_end = min(min(it.lk, t_last + off), it.j1 * 128);
+  const int k_begin = it.j0 * 128, k_end = min(min(it.lk, t_last + off), it.j1 * 128);
   const T* kb = static_cast<const T*>(p.k) + it.k0 * p.k_token + kvh * p.k_head;
   const T* vb = static_cast<const T*>(p.v) + it.k0 * p.v_token + kvh * p.v_head;
+  // Keys past the end are zeros in K and V; their weights are zero too.
+  auto fetch_k = [&](int k0) {
+    for (int x = tid; x < TK * (DP / 4); x += TT) {
+      const int key = x / (DP / 4), d = x % (DP / 4) * 4;
+      const bool there = k0 + key < it.lk && d < D;
+      put4(s_k + key * LD + d, there ? kb + (k0 + key) * p.k_token : kb, d, D, vec, there);
+    }
+  };
+  auto fetch_v = [&](int k0) {
+    for (int x = tid; x < TK * (DP / 4); x += TT) {
+      const int key = x / (DP / 4), d = x % (DP / 4) * 4;
+      const bool there = k0 + key < it.lk && d < D;
+      put4(s_v + key * DP + d, there ? vb + (k0 + key) * p.v_token : vb, d, D, vec, there);
+    }
+  };
   for (int x = tid; x < TR * (DP / 4); x += TT) {
-    const int r = x % TR, d = x / TR * 4, row = r0 + r;
+    const int r = x / (DP / 4), d = x % (DP / 4) * 4, row = r0 + r;
     float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
     if (row < n)
       q = row4(static_cast<const T*>(p.q) + (int64_t(it.q0) + it.t0 + row / G) * p.q_token +
                    (kvh * G + row % G) * p.q_head, d, D, vec);
-    s_q[d * TR + r] = q.x;
-    s_q[(d + 1) * TR + r] = q.y;
-    s_q[(d + 2) * TR + r] = q.z;
-    s_q[(d + 3) * TR + r] = q.w;
+    *reinterpret_cast<float4*>(s_q + r * LD + d) = q;
   }
-  const int rg = tid / 16, cg = tid % 16;                 // rows rg * 8 .., keys / columns cg * 4 ..
-  int keys[8];                                            // keys each row sees
+  if (k_begin < k_end) {
+    fetch_k(k_begin);
+    fetch_v(k_begin);
+  }
+  const int rg = tid / 16, cg = tid % 16;    // rows rg * 8 .., keys cg + 16 c, columns cg * 4 ..
+  int keys[8];                               // keys each row sees
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
     const int row = r0 + rg * 8 + r;
     keys[r] = row < n ? min(it.lk, it.t0 + row / G + off) : 0;
   }
   float2 o[4][C::CPT];
-  float m[8], l[8];                                       // l: this thread's keys only
+  float m[8], l[8];                          // l: this thread's keys only
 #pragma unroll
   for (int r = 0; r < 8; ++r) m[r] = -INFINITY, l[r] = 0.f;
 #pragma unroll
@@ -148,52 +190,43 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec) {
 #pragma unroll
     for (int c = 0; c < C::CPT; ++c) o[r][c] = make_float2(0.f, 0.f);
   const float c_log2 = p.scale * 1.4426950408889634f;
-  for (int k0 = it.j0 * 128; k0 < k_end; k0 += TK) {
+  for (int k0 = k_begin; k0 < k_end; k0 += TK) {
+    rows_landed();                           // K (and, one tile late, nothing else)
     __syncthreads();
-    // Keys past the end are zeros in K and V; their weights are zero too.
-    for (int x = tid; x < TK * (DP / 4); x += TT) {
-      const int key = x % TK, d = x / TK * 4;
-      float4 k = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (k0 + key < it.lk) k = row4(kb + (k0 + key) * p.k_token, d, D, vec);
-      s_k[d * (TK + 4) + key] = k.x;
-      s_k[(d + 1) * (TK + 4) + key] = k.y;
-      s_k[(d + 2) * (TK + 4) + key] = k.z;
-      s_k[(d + 3) * (TK + 4) + key] = k.w;
+    if (k0 > k_begin) fetch_v(k0);           // the last tile's P V is done
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    float2 s2[8][KPT];                       // sums over even and odd elements
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+      for (int c = 0; c < KPT; ++c) s2[r][c] = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int d = 0; d < DP; d += 4) {
+      float4 k[KPT];
+#pragma unroll
+      for (int c = 0; c < KPT; ++c)
+        k[c] = *reinterpret_cast<const float4*>(s_k + (cg + 16 * c) * LD + d);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const float4 q = *reinterpret_cast<const float4*>(s_q + (rg * 8 + r) * LD + d);
+#pragma unroll
+        for (int c = 0; c < KPT; ++c) {
+          s2[r][c] = fma2(make_float2(q.x, q.y), make_float2(k[c].x, k[c].y), s2[r][c]);
+          s2[r][c] = fma2(make_float2(q.z, q.w), make_float2(k[c].z, k[c].w), s2[r][c]);
+        }
+      }
     }
-    for (int x = tid; x < TK * (DP / 4); x += TT) {
-      const int key = x / (DP / 4), d = x % (DP / 4) * 4;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (k0 + key < it.lk) v = row4(vb + (k0 + key) * p.v_token, d, D, vec);
-      *reinterpret_cast<float4*>(s_v + key * DP + d) = v;
-    }
-    __syncthreads();
-    float2 s[4][4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) s[r][c] = make_float2(0.f, 0.f);
-#pragma unroll 8
-    for (int d = 0; d < DP; ++d) {
-      const float4 qa = *reinterpret_cast<const float4*>(s_q + d * TR + rg * 8);
-      const float4 qb = *reinterpret_cast<const float4*>(s_q + d * TR + rg * 8 + 4);
-      const float4 k = *reinterpret_cast<const float4*>(s_k + d * (TK + 4) + cg * 4);
-      const float2 q[4] = {{qa.x, qa.y}, {qa.z, qa.w}, {qb.x, qb.y}, {qb.z, qb.w}};
-      const float kk[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[r][c] = fma2(q[r], make_float2(kk[c], kk[c]), s[r][c]);
-    }
-    __syncthreads();                                      // K is read: P takes its place
+    __syncthreads();                         // K is read
+    if (k0 + TK < k_end) fetch_k(k0 + TK);
+    float e[8][KPT];
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-      float v[4];
       float mx = m[r];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        v[c] = (r & 1) ? s[r / 2][c].y : s[r / 2][c].x;
-        if (k0 + cg * 4 + c >= keys[r]) v[c] = -INFINITY;
-        mx = fmaxf(mx, v[c]);
+      for (int c = 0; c < KPT; ++c) {
+        e[r][c] = s2[r][c].x + s2[r][c].y;
+        if (k0 + cg + 16 * c >= keys[r]) e[r][c] = -INFINITY;
+        mx = fmaxf(mx, e[r][c]);
       }
 #pragma unroll
       for (int x = 1; x < 16; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
@@ -207,27 +240,28 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec) {
         else o[r / 2][c].x *= f;
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float e = exp2f(fmaf(v[c], c_log2, -base));
-        l[r] += e;
-        if (r & 1) s[r / 2][c].y = e;
-        else s[r / 2][c].x = e;
+      for (int c = 0; c < KPT; ++c) {
+        e[r][c] = exp2f(fmaf(e[r][c], c_log2, -base));
+        l[r] += e[r][c];
       }
     }
-    // Four rows at once; their place in a key's row is turned by the key's group, so that the 8
-    // lanes of one store phase meet all banks.
+    // Four rows at once; their place in a key's row is turned by the key, so that the 8 lanes of
+    // one store phase meet all banks.
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < KPT; ++c)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<float4*>(s_k + (cg * 4 + c) * TR + (((rg * 2 + h) ^ (cg & 7)) * 4)) =
-            make_float4(s[2 * h][c].x, s[2 * h][c].y, s[2 * h + 1][c].x, s[2 * h + 1][c].y);
+        *reinterpret_cast<float4*>(s_p + (cg + 16 * c) * TR + (((rg * 2 + h) ^ (cg & 7)) * 4)) =
+            make_float4(e[4 * h][c], e[4 * h + 1][c], e[4 * h + 2][c], e[4 * h + 3][c]);
+    if (k0 + TK < k_end)                     // V, but not the K tile just asked for
+      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 1;" ::: "memory");
+    else
+      rows_landed();
     __syncthreads();
 #pragma unroll 4
     for (int j = 0; j < TK; ++j) {
-      const int turn = j >> 2 & 7;
-      const float4 pa = *reinterpret_cast<const float4*>(s_k + j * TR + ((rg * 2) ^ turn) * 4);
-      const float4 pb = *reinterpret_cast<const float4*>(s_k + j * TR + ((rg * 2 + 1) ^ turn) * 4);
+      const float4 pa = *reinterpret_cast<const float4*>(s_p + j * TR + ((rg * 2) ^ (j & 7)) * 4);
+      const float4 pb = *reinterpret_cast<const float4*>(s_p + j * TR + ((rg * 2 + 1) ^ (j & 7)) * 4);
       const float2 w[4] = {{pa.x, pa.y}, {pa.z, pa.w}, {pb.x, pb.y}, {pb.z, pb.w}};
 #pragma unroll
       for (int c4 = 0; c4 < C::CPT; c4 += 4) {
@@ -292,6 +326,7 @@ packed_join_kernel(const enigma_sdpa_packed_desc p) {
   const int state = r / 128, row = r % 128;
   const int tok = g.tok0 + state * g.tokens + row / G;
   if (row >= g.tokens * G || tok >= g.tok_end || tok >= p.tokens_q || (g.alt && state > 0)) return;
+  griddep_wait();                                               // the parts are written
   const int n = g.alt ? 2 * g.parts : g.parts, step = (g.alt ? 1 : 2) * 128;
   const int64_t at = int64_t(g.slot + (g.alt ? 0 : state)) * 128 + row;
   enigma_serving::RowJoin<V> join;
@@ -310,10 +345,10 @@ packed_join_kernel(const enigma_sdpa_packed_desc p) {
 }
 
 template <typename T>
-void launch_join(const enigma_sdpa_packed_desc& d, const dim3 grid, cudaStream_t s) {
-  if (d.head_dim <= 64) packed_join_kernel<T, 2><<<grid, 256, 0, s>>>(d);
-  else if (d.head_dim <= 128) packed_join_kernel<T, 4><<<grid, 256, 0, s>>>(d);
-  else packed_join_kernel<T, 8><<<grid, 256, 0, s>>>(d);
+cudaError_t launch_join(const enigma_sdpa_packed_desc& d, const dim3 grid, cudaStream_t s) {
+  if (d.head_dim <= 64) return enigma::launch_dependent(packed_join_kernel<T, 2>, grid, 256, 0, s, d);
+  if (d.head_dim <= 128) return enigma::launch_dependent(packed_join_kernel<T, 4>, grid, 256, 0, s, d);
+  return enigma::launch_dependent(packed_join_kernel<T, 8>, grid, 256, 0, s, d);
 }
 
 template <typename T, int DP>
@@ -398,9 +433,8 @@ cudaError_t sdpa_packed_join_launch(const enigma_sdpa_packed_desc& d, cudaStream
   const int groups = d.header[enigma_serving::kGroups];
   if (groups == 0) return cudaSuccess;
   const dim3 grid(unsigned(groups), 2 * ENIGMA_PACKED_TILE_ROWS / 8);
-  if (d.dtype == ENIGMA_DTYPE_F32) launch_join<float>(d, grid, s);
-  else launch_join<__nv_bfloat16>(d, grid, s);
-  return cudaGetLastError();
+  return d.dtype == ENIGMA_DTYPE_F32 ? launch_join<float>(d, grid, s)
+                                     : launch_join<__nv_bfloat16>(d, grid, s);
 }
 
 cudaError_t sdpa_paged_simt_launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {

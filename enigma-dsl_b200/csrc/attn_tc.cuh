@@ -240,6 +240,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  griddep_launch_dependents();               // the next kernel may take SMs that are free
   // Packed: the plan lists each CTA's items.  Paged: one item per CTA.
   const int t_begin = PAGED ? int(blockIdx.x) : __ldg(p.offsets + blockIdx.x);
   const int t_end = PAGED ? min(t_begin + 1, items) : __ldg(p.offsets + blockIdx.x + 1);

@@ -96,6 +96,24 @@ cudaError_t kv_cache_copy_pages(const enigma_kv_cache_desc& d, const int32_t* sr
 cudaError_t elementwise_launch(int op, int dtype, const void* a, const void* b, void* c, int64_t n,
                                cudaStream_t s);
 
+// Launches `kernel` as a programmatic dependent of the kernel before it on the stream: it may
+// start while that one still runs, and waits (griddep_wait) before it reads what that one wrote.
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,
+                             cudaStream_t s, Args&&... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = block;
+  c.dynamicSmemBytes = smem;
+  c.stream = s;
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = a;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, static_cast<Params>(args)...);
+}
+
 // Records the name of the device kernel an operator launcher chose, for
 // enigma_last_kernel on the calling thread (a static string).
 void note_kernel(const char* name);

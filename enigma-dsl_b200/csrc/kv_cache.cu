@@ -87,6 +87,8 @@ cache_map_kernel(const Map m, const int32_t* __restrict__ a, const int32_t* __re
   const uint32_t rank = cluster_ctarank();
   const int tid = threadIdx.x, gtid = int(rank) * MAP_THREADS + tid;
   constexpr int GT = MAP_CTAS * MAP_THREADS;
+  griddep_launch_dependents();
+  griddep_wait();
 
   // Check the request; every CTA does it for itself and comes to the same answer, since
   // nothing is written before the barrier that follows.
@@ -261,6 +263,8 @@ cache_compact_kernel(const Map m) {
   constexpr int GT = MAP_CTAS * MAP_THREADS;
   const int per = (m.pages + MAP_CTAS - 1) / MAP_CTAS;
   const int p0 = min(int(rank) * per, m.pages), p1 = min(p0 + per, m.pages);
+  griddep_launch_dependents();
+  griddep_wait();
   cluster_sync();                      // every CTA runs before its shared memory is written
   int mine = 0, counted = 0;
   for (int p = p0 + tid; p < p1; p += MAP_THREADS) mine += m.refs[p] > 0;
@@ -331,6 +335,8 @@ struct Copy {
 // Units of one (copy, layer, K or V, head): fill * row_bytes contiguous bytes.
 template <typename V>
 __global__ void __launch_bounds__(256) cache_copy_kernel(const Copy c) {
+  griddep_launch_dependents();
+  griddep_wait();
   const int n = c.count != nullptr ? *c.count : c.n;
   const int64_t units = int64_t(n) * c.layers * 2 * c.heads;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
@@ -371,6 +377,8 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const Write w) {
   const int lane = threadIdx.x & 31;
   const int warps = int(gridDim.x) * 8;
   const int per = w.row_bytes / int(sizeof(V));
+  griddep_launch_dependents();
+  griddep_wait();
   for (int t = int(blockIdx.x) * 8 + (threadIdx.x >> 5); t < w.tokens; t += warps) {
     int lo = 0, hi = w.n;              // the last i with cu[i] <= t
     while (hi - lo > 1) {
@@ -439,18 +447,16 @@ cudaError_t launch_copy(const enigma_kv_cache_desc& d, const int32_t* src, const
   const unsigned grid = unsigned(std::min<int64_t>(units, int64_t(enigma::sm_count()) * 8));
   if (grid == 0) return cudaSuccess;
   if (c.row_bytes % 16 == 0 && a16(d.k) && a16(d.v))
-    cache_copy_kernel<uint4><<<grid, 256, 0, s>>>(c);
-  else
-    cache_copy_kernel<uint16_t><<<grid, 256, 0, s>>>(c);
-  return cudaGetLastError();
+    return enigma::launch_dependent(cache_copy_kernel<uint4>, grid, 256, 0, s, c);
+  return enigma::launch_dependent(cache_copy_kernel<uint16_t>, grid, 256, 0, s, c);
 }
 
 template <int MODE>
 cudaError_t launch_map(const enigma_kv_cache_desc& d, const int32_t* a, const int32_t* b, int64_t n,
                        cudaStream_t s) {
   const size_t bits = size_t((d.slots + 31) / 32) * 4;
-  cache_map_kernel<MODE><<<MAP_CTAS, MAP_THREADS, bits, s>>>(make_map(d), a, b, int(n));
-  return cudaGetLastError();
+  return enigma::launch_dependent(cache_map_kernel<MODE>, MAP_CTAS, MAP_THREADS, bits, s, make_map(d),
+                                  a, b, int(n));
 }
 
 }  // namespace
@@ -485,8 +491,8 @@ cudaError_t kv_cache_reserve(const enigma_kv_cache_desc& d, const int32_t* slots
 cudaError_t kv_cache_compact(const enigma_kv_cache_desc& d, cudaStream_t s) {
   note_kernel("cache_compact_kernel");
   const Map m = make_map(d);
-  cache_compact_kernel<<<MAP_CTAS, MAP_THREADS, 0, s>>>(m);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e =
+      enigma::launch_dependent(cache_compact_kernel, MAP_CTAS, MAP_THREADS, 0, s, m);
   if (e != cudaSuccess) return e;
   // At most half of the pages move: each moved page has a hole of its own.
   return launch_copy(d, m.src(), m.dst(), nullptr, m.ws, d.pages / 2, s);
@@ -532,9 +538,8 @@ cudaError_t kv_cache_write(const enigma_kv_cache_desc& d, int64_t layer, const v
   const bool vec = w.row_bytes % 16 == 0 && a16(w.k) && a16(w.v) && a16(new_k) && a16(new_v) &&
                    w.k_token % 16 == 0 && w.k_head % 16 == 0 && w.v_token % 16 == 0 &&
                    w.v_head % 16 == 0;
-  if (vec) cache_write_kernel<uint4><<<grid, 256, 0, s>>>(w);
-  else cache_write_kernel<uint16_t><<<grid, 256, 0, s>>>(w);
-  return cudaGetLastError();
+  return vec ? enigma::launch_dependent(cache_write_kernel<uint4>, grid, 256, 0, s, w)
+             : enigma::launch_dependent(cache_write_kernel<uint16_t>, grid, 256, 0, s, w);
 }
 
 }  // namespace enigma

@@ -80,8 +80,7 @@ PROTOTYPES = {
     "enigma_kv_cache_fork": [_vp, _vp, _vp, _i64, _vp],
     "enigma_kv_cache_free": [_vp, _vp, _i64, _vp],
     "enigma_kv_cache_reserve": [_vp, _vp, _vp, _i64, _vp],
-    "enigma_kv_cache_write": [_vp, _i64, _vp, _vp, _c.POINTER(_i64), _vp, _vp, _vp, _i64, _i64,
-                              _vp],
+    "enigma_kv_cache_write": [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp],
     "enigma_kv_cache_compact": [_vp, _vp],
     "enigma_kv_cache_copy_pages": [_vp, _vp, _vp, _i64, _vp],
     "enigma_dispatch": [_i32, _c.POINTER(_vp), _i32, _c.POINTER(_i64), _i32, _c.POINTER(_f32),

@@ -18,10 +18,15 @@ from . import _native
 _initialised: set = set()
 
 
-def _torch():
-    import torch  # local: the package imports without torch for host-only use
+_torch_module = None
 
-    return torch
+
+def _torch():
+    global _torch_module
+    if _torch_module is None:
+        import torch  # on first use: the package imports without torch for host-only use
+        _torch_module = torch
+    return _torch_module
 
 
 def ensure_device(device_index: int) -> None:
@@ -173,16 +178,19 @@ class PackedPlan:
 _PACKED_DESC = struct.Struct(f"13qf3i{_native.PACKED_PLAN_HEADER}i8Q")
 
 
+_CUDA = "cuda"
+
+
 def _raw_stream(t) -> int:
     """The current stream of t's device, without the Stream object that _stream_ptr makes."""
     return _torch()._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _check_rows(name, *ts):
-    """CUDA tensors of one device and dtype whose last axis is contiguous."""
+    """CUDA tensors of one device and dtype whose last axis is contiguous; the dtype's code."""
     first = ts[0]
     device, dtype = first.device, first.dtype
-    if device.type != "cuda":
+    if device.type != _CUDA:
         raise ValueError("enigma CUDA operators take CUDA tensors (no CPU fallback)")
     for t in ts:
         if t.device != device:
@@ -193,6 +201,7 @@ def _check_rows(name, *ts):
             raise ValueError(f"{name}: the last axis must be contiguous")
     if device.index not in _initialised:
         ensure_device(device.index)
+    return _dtype_code(first)
 
 
 def _scratch(name, workspace, need, like):
@@ -201,7 +210,8 @@ def _scratch(name, workspace, need, like):
         if need == 0:
             return 0, 0, None
         workspace = like.new_empty(need, dtype=_torch().uint8)
-    elif workspace.device != like.device or not workspace.is_contiguous():
+        return workspace.data_ptr(), need, workspace
+    if workspace.device != like.device or not workspace.is_contiguous():
         raise ValueError(f"{name}: workspace must be contiguous on the data's device")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
@@ -229,12 +239,13 @@ def sdpa_packed(q, k, v, plan: PackedPlan, scale: Optional[float] = None, out=No
     if (tq, tk) != (plan.tokens_q, plan.tokens_k):
         raise ValueError(f"sdpa_packed: the plan's lengths sum to {plan.tokens_q} / "
                          f"{plan.tokens_k} tokens, the tensors hold {tq} / {tk}")
-    dtype = _dtype_code(q)
     if out is None:
+        dtype = _check_rows("sdpa_packed", q, k, v)
         out = q.new_empty((tq, hq, d))
     elif out.shape != q.shape:
         raise ValueError("sdpa_packed: out must have q's shape")
-    _check_rows("sdpa_packed", q, k, v, out)
+    else:
+        dtype = _check_rows("sdpa_packed", q, k, v, out)
     if plan.ints.device != q.device:
         raise ValueError("sdpa_packed: the plan is on another device")
     lse = q.new_empty((tq, hq), dtype=torch.float32) if return_lse else None
@@ -264,9 +275,9 @@ def _shared_workspace_bytes(device_index, *sizes) -> int:
 
 
 def _check_int32(name, device, *ts):
-    torch = _torch()
+    int32 = _torch().int32
     for t in ts:
-        if t.dtype != torch.int32 or not t.is_contiguous() or t.device != device:
+        if t.dtype != int32 or t.device != device or not t.is_contiguous():
             raise ValueError(f"{name}: tables, lengths and slots are contiguous int32 tensors on "
                              f"the data's device")
 
@@ -293,12 +304,13 @@ def sdpa_shared_prefix(q, k_pages, v_pages, table, lens, prefix_len: int = 0, sl
         raise ValueError("sdpa_shared_prefix: expected table [n, width] and lens [n]")
     if slots is not None and tuple(slots.shape) != (b,):
         raise ValueError("sdpa_shared_prefix: slots must name one row per sequence")
-    dtype = _dtype_code(q)
     if out is None:
+        dtype = _check_rows("sdpa_shared_prefix", q, k_pages, v_pages)
         out = q.new_empty((b, hq, d))
     elif out.shape != q.shape:
         raise ValueError("sdpa_shared_prefix: out must have q's shape")
-    _check_rows("sdpa_shared_prefix", q, k_pages, v_pages, out)
+    else:
+        dtype = _check_rows("sdpa_shared_prefix", q, k_pages, v_pages, out)
     ks, vs = k_pages.stride(), v_pages.stride()
     if ks[1:] != (page * d, d, 1) or vs[1:] != (page * d, d, 1):
         raise ValueError("sdpa_shared_prefix: a page must be contiguous")

@@ -10,6 +10,7 @@ with `write`, `cuda_ops.sdpa_shared_prefix` reads it (`attend`).
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 from . import _native, cuda_ops
@@ -24,6 +25,9 @@ class _CacheDesc(ctypes.Structure):
                [(n, ctypes.c_void_p) for n in ("k", "v", "table", "lens", "refs", "status",
                                                "workspace")] + \
                [("workspace_bytes", ctypes.c_size_t)]
+
+
+_STRIDES = struct.Struct("4q")
 
 
 class PagedKVCache:
@@ -45,6 +49,7 @@ class PagedKVCache:
         self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
         self.layers, self.pages, self.heads_kv, self.page, self.head_dim = k.shape
         self.slots, self.width = table.shape
+        self._device, self._row = k.device, (self.heads_kv, self.head_dim)
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         self._desc = _CacheDesc(layers, pages, heads, page, head_dim, k.element_size(),
                                 self.slots, self.width, k.data_ptr(), v.data_ptr(),
@@ -76,11 +81,12 @@ class PagedKVCache:
 
     def _ints(self, name, values, like=None):
         """A request as an int32 device tensor (lists and host tensors are copied there)."""
-        import torch
+        torch = cuda_ops._torch()
         if not isinstance(values, torch.Tensor):
             values = torch.as_tensor(values, dtype=torch.int32)
-        if values.dtype == torch.int32 and values.device == self.k.device and values.dim() == 1 \
-                and values.is_contiguous() and (like is None or values.shape == like.shape):
+        elif values.dtype == torch.int32 and values.device == self._device \
+                and values.dim() == 1 and values.is_contiguous() \
+                and (like is None or values.shape == like.shape):
             return values
         if values.dim() != 1:
             raise ValueError(f"{name}: expected one number per sequence")
@@ -99,37 +105,38 @@ class PagedKVCache:
         parents = self._ints("fork", parents)
         children = self._ints("fork", children, parents)
         self._call("enigma_kv_cache_fork", parents.data_ptr(), children.data_ptr(),
-                   parents.numel())
+                   parents.shape[0])
 
     def free(self, slots) -> None:
         """The slots let go of their pages; a page that no slot holds is free."""
         slots = self._ints("free", slots)
-        self._call("enigma_kv_cache_free", slots.data_ptr(), slots.numel())
+        self._call("enigma_kv_cache_free", slots.data_ptr(), slots.shape[0])
 
     def reserve(self, slots, lens) -> None:
         """Slot slots[i] grows to lens[i] tokens, taking the lowest free pages."""
         slots = self._ints("reserve", slots)
         lens = self._ints("reserve", lens, slots)
-        self._call("enigma_kv_cache_reserve", slots.data_ptr(), lens.data_ptr(), slots.numel())
+        self._call("enigma_kv_cache_reserve", slots.data_ptr(), lens.data_ptr(), slots.shape[0])
 
     def write(self, layer: int, new_k, new_v, slots, starts, cu) -> None:
         """Rows cu[i] .. cu[i + 1] of new_k / new_v [tokens, heads_kv, head_dim] are tokens
         starts[i], starts[i] + 1, ... of slot slots[i] in `layer` (reserved before)."""
-        want = (self.heads_kv, self.head_dim)
-        if new_k.dim() != 3 or new_k.shape != new_v.shape or tuple(new_k.shape[1:]) != want:
-            raise ValueError(f"write: expected rows [tokens, {want[0]}, {want[1]}]")
+        shape = new_k.shape
+        if len(shape) != 3 or shape != new_v.shape or shape[1:] != self._row:
+            raise ValueError(f"write: expected rows [tokens, {self._row[0]}, {self._row[1]}]")
         cuda_ops._check_rows("write", self.k, new_k, new_v)
         if not 0 <= layer < self.layers:
             raise ValueError(f"write: layer {layer} of {self.layers}")
         slots = self._ints("write", slots)
         starts = self._ints("write", starts, slots)
         cu = self._ints("write", cu)
-        if cu.numel() != slots.numel() + 1:
+        n = slots.shape[0]
+        if cu.shape[0] != n + 1:
             raise ValueError("write: cu holds one number more than there are slots")
-        strides = (ctypes.c_int64 * 4)(*new_k.stride()[:2], *new_v.stride()[:2])
-        self._call("enigma_kv_cache_write", layer, new_k.data_ptr(), new_v.data_ptr(), strides,
-                   slots.data_ptr(), starts.data_ptr(), cu.data_ptr(), slots.numel(),
-                   new_k.shape[0])
+        ks, vs = new_k.stride(), new_v.stride()
+        self._call("enigma_kv_cache_write", layer, new_k.data_ptr(), new_v.data_ptr(),
+                   _STRIDES.pack(ks[0], ks[1], vs[0], vs[1]), slots.data_ptr(),
+                   starts.data_ptr(), cu.data_ptr(), n, shape[0])
 
     def compact(self) -> None:
         """The n pages in use take the numbers below n (rows are rewritten to match)."""
