@@ -16,8 +16,9 @@ using namespace enigma_tc;
 // The work is the flattened list of (unit, 64-key chunk) pairs, unit = (sequence, kv head, block
 // of up to 16 query heads); CTA c of P takes the contiguous range [c T / P, (c + 1) T / P), so
 // every SM streams the same number of chunks whatever the lengths are.  A producer warp loads
-// chunks by TMA (one box per page and 64 columns) into a ring; four warps take 16 keys of each
-// chunk: S = Q K^T (mma.sync, the heads as the 16-row operand), online softmax, O += P V.  At
+// chunks by TMA (one box per page and 64 columns) into a ring; two warps take 32 keys each of
+// the even chunks, two of the odd ones (16 keys of every chunk per warp: 1.2x the time, a chunk's
+// chain of dependent steps is longer than its work): S = Q K^T (mma.sync, the heads as the 16-row operand), online softmax, O += P V.  At
 // the end of a unit's run of chunks each warp stores its state, in slot (c + u) * 4 + warp
 // (segments in order advance c or u, so the slots are distinct).  Merging the warps first cost
 // two barriers and a second pass per run (92 against 60 us for 128 sequences of 5 to 1024 keys);
@@ -25,6 +26,7 @@ using namespace enigma_tc;
 constexpr int CHUNK = 64;
 constexpr int DWARPS = 4;
 constexpr int DTHREADS = (DWARPS + 1) * 32;
+constexpr int WKEYS = 32;                    // keys of a chunk that one warp takes
 constexpr int ROWS = 16;                     // query heads of a unit
 constexpr int PAGES = 128;                   // page numbers looked up at once
 
@@ -156,7 +158,7 @@ __device__ __forceinline__ Segment segment_at(const int* starts, int batch, int 
 }
 
 template <int D>
-__global__ void __launch_bounds__(DTHREADS)
+__global__ void __launch_bounds__(DTHREADS, D == 64 ? 3 : 2)
 paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const DecodeParams p) {
   using C = DCfg<D>;
@@ -166,7 +168,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   int* s_starts = reinterpret_cast<int*>(ring + ST * 2 * C::TILE);    // [batch + 1]
   int* s_len = s_starts + p.batch + 1;                                // [batch]
-  __shared__ uint64_t full[ST], empty[ST];
+  __shared__ uint64_t full[ST][2], empty[ST];   // a stage's chunks for either team
   __shared__ float s_m[DWARPS][ROWS], s_l[DWARPS][ROWS];    // direct
   __shared__ int s_warp[DWARPS + 1], s_pages[PAGES];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -175,8 +177,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 
   if (tid == 0) {
     for (int s = 0; s < ST; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], DWARPS);
+      mbar_init(&full[s][0], 1);
+      mbar_init(&full[s][1], 1);
+      mbar_init(&empty[s], 2);               // the chunk's two warps
     }
     fence_barrier_init();
     tma_prefetch_desc(&tmK);
@@ -279,12 +282,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           break;
         }
         if (lane == 0)
-          mbar_arrive_expect_tx(&full[st], (uint32_t(2 * boxes * C::ATOMS) * 128u) << p.box_shift);
+          mbar_arrive_expect_tx(&full[st][i & 1], (uint32_t(2 * boxes * C::ATOMS) * 128u) << p.box_shift);
         __syncwarp();
         if (box < boxes)
           tma_load_4d(ring + (2 * st + (is_v ? 1 : 0)) * C::TILE + atom * CHUNK * 128 +
                           ((box << p.box_shift) * 128),
-                      is_v ? &tmV : &tmK, &full[st], atom * 64,
+                      is_v ? &tmV : &tmK, &full[st][i & 1], atom * 64,
                       (key0 + (box << p.box_shift)) & ((1 << p.page_shift) - 1), s.kvh, page_now);
         __syncwarp();
       }
@@ -296,6 +299,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 
   // ------------------------------------------------------------------ consumers
   const int g = lane >> 2, quad = lane & 3;
+  const int team = warp >> 1;                               // takes every second chunk
   int i = 0;
   for (int64_t at = c0; at < c1;) {
     const Segment s = segment_at(s_starts, p.batch, per_b, p.blocks, at, c1);
@@ -321,31 +325,38 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     bool ok = true;
     for (int j = s.j0; j < s.j0 + s.n; ++j, ++i) {
+      if ((i & 1) != team) continue;
       const int st = i % ST;
-      ok = __all_sync(0xffffffffu, mbar_wait(&full[st], (i / ST) & 1, p.status));
+      // A team sees its own chunks only, so each has its own barrier per stage: the parity of
+      // one that also counted the other team's could be a phase old.
+      const int uses = ST % 2 == 0 ? i / ST : i / ST / 2;   // of this barrier before
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[st][team], uses & 1, p.status));
       if (!ok) break;
       uint8_t* tile_k = ring + 2 * st * C::TILE;
       uint8_t* tile_v = tile_k + C::TILE;
       const Chunk ch = chunk_at(p, s.b, len, j);
-      const int key0 = ch.key0 + warp * 16;                 // this warp's first key
-      float sc[2][4];
+      const int row0 = (warp & 1) * WKEYS;                  // this warp's first row of the chunk
+      const int key0 = ch.key0 + row0;
+      float sc[WKEYS / 8][4];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < WKEYS / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
       const int mi = lane >> 3, mr = lane & 7;              // ldmatrix: matrix, row
       const uint32_t ka = smem_u32(tile_k);
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        uint32_t b[4];
-        ldsm_x4(ka + (kk / 4) * CHUNK * 128 +
-                    sw128(warp * 16 + (mi >> 1) * 8 + mr, (kk % 4) * 2 + (mi & 1)), b);
-        mma_16816(sc[0], q[kk], b[0], b[1]);
-        mma_16816(sc[1], q[kk], b[2], b[3]);
-      }
-      if (key0 + 16 > ch.hi || key0 < ch.lo) {              // warp-uniform
+      for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < WKEYS / 16; ++n) {
+          uint32_t b[4];
+          ldsm_x4(ka + (kk / 4) * CHUNK * 128 +
+                      sw128(row0 + n * 16 + (mi >> 1) * 8 + mr, (kk % 4) * 2 + (mi & 1)), b);
+          mma_16816(sc[2 * n], q[kk], b[0], b[1]);
+          mma_16816(sc[2 * n + 1], q[kk], b[2], b[3]);
+        }
+      if (key0 + WKEYS > ch.hi || key0 < ch.lo) {           // warp-uniform
+#pragma unroll
+        for (int n = 0; n < WKEYS / 8; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int key = key0 + n * 8 + quad * 2 + (e & 1);
@@ -353,11 +364,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           }
         // Rows past the end hold whatever the page or the ring held, rows of the prefix
         // whatever this sequence's page has there: 0 * NaN must not be.
-        for (int x = lane; x < 16 * 8 * C::ATOMS; x += 32) {
-          const int row = x >> 3 & 15;
+        for (int x = lane; x < WKEYS * 8 * C::ATOMS; x += 32) {
+          const int row = (x >> 3) % WKEYS;
           if (key0 + row >= ch.hi || key0 + row < ch.lo)
-            *reinterpret_cast<uint4*>(tile_v + (x >> 7) * CHUNK * 128 + (warp * 16 + row) * 128 +
-                                      (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(tile_v + x / (WKEYS * 8) * CHUNK * 128 +
+                                      (row0 + row) * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();                           // before the next TMA write here
         __syncwarp();
@@ -365,7 +376,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       float mc[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {                         // rows g and g + 8
-        float mx = max3f(max3f(sc[0][2 * h], sc[0][2 * h + 1], sc[1][2 * h]), sc[1][2 * h + 1], m[h]);
+        float mx = m[h];
+#pragma unroll
+        for (int n = 0; n < WKEYS / 8; ++n) mx = max3f(mx, sc[n][2 * h], sc[n][2 * h + 1]);
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         mc[h] = mx == -INFINITY ? 0.f : mx * p.scale_log2;
@@ -380,24 +393,27 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           }
         }
       }
-      uint32_t pa[4];
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float e0 = ex2(fmaf(sc[n][2 * h], p.scale_log2, -mc[h]));
-          const float e1 = ex2(fmaf(sc[n][2 * h + 1], p.scale_log2, -mc[h]));
-          l[h] += e0 + e1;                                  // this lane's share of the row's sum
-          pa[2 * n + h] = pack_bf16x2(e0, e1);
-        }
       const uint32_t va = smem_u32(tile_v);
 #pragma unroll
-      for (int dd = 0; dd < D / 16; ++dd) {
-        uint32_t b[4];
-        ldsm_x4_trans(va + (dd / 4) * CHUNK * 128 +
-                          sw128(warp * 16 + (mi & 1) * 8 + mr, (dd % 4) * 2 + (mi >> 1)), b);
-        mma_16816(o[2 * dd], pa, b[0], b[1]);
-        mma_16816(o[2 * dd + 1], pa, b[2], b[3]);
+      for (int n = 0; n < WKEYS / 16; ++n) {
+        uint32_t pa[4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float e0 = ex2(fmaf(sc[2 * n + t][2 * h], p.scale_log2, -mc[h]));
+            const float e1 = ex2(fmaf(sc[2 * n + t][2 * h + 1], p.scale_log2, -mc[h]));
+            l[h] += e0 + e1;                                // this lane's share of the row's sum
+            pa[2 * t + h] = pack_bf16x2(e0, e1);
+          }
+#pragma unroll
+        for (int dd = 0; dd < D / 16; ++dd) {
+          uint32_t b[4];
+          ldsm_x4_trans(va + (dd / 4) * CHUNK * 128 +
+                            sw128(row0 + n * 16 + (mi & 1) * 8 + mr, (dd % 4) * 2 + (mi >> 1)), b);
+          mma_16816(o[2 * dd], pa, b[0], b[1]);
+          mma_16816(o[2 * dd + 1], pa, b[2], b[3]);
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);

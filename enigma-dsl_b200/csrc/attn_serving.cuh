@@ -19,18 +19,17 @@ struct PackedItem {
   int tokens;        // tokens in each of its (at most) two tiles
   int j0, j1;
   int kvh;
-  int alt;           // one row tile; even and odd key tiles have a softmax state each
-  int slot;          // first of its two partial results, or -1: it computes the final one
-  int pad;
+  int slot;          // first of its two tiles' partial results, or -1: it computes the final one
+  int pad[2];
 };
 constexpr int kItemInts = sizeof(PackedItem) / 4;
 
 // The items of one pair of tiles whose keys were split: partial results slot, slot + 2, ... of
-// `parts` items (and slot + 1, slot + 3, ... of the second state) make its rows.
+// `parts` items make the first tile's rows, slot + 1, slot + 3, ... the second's.
 struct PackedGroup {
   int tok0, tok_end;  // first token of the first tile, end of the sequence (packed rows)
   int tokens, kvh;
-  int slot, parts, alt, pad;
+  int slot, parts, pad[2];
 };
 constexpr int kGroupInts = sizeof(PackedGroup) / 4;
 

@@ -139,7 +139,7 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec) {
       it.k0 + int64_t(it.lk) > p.tokens_k || it.t0 < 0 || kvh < 0 || kvh >= p.heads_kv ||
       it.slot >= p.header[enigma_serving::kSlots])
     return;
-  const int n = min((it.alt ? 1 : 2) * it.tokens, it.lq - it.t0) * G;   // rows of the item
+  const int n = min(2 * it.tokens, it.lq - it.t0) * G;    // rows of the item
   const int r0 = blockIdx.y * TR;
   if (r0 >= n) return;
   const int off = p.causal ? it.lk - it.lq + 1 : it.lk;   // a token's keys: min(lk, token + off)
@@ -287,8 +287,7 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec) {
     const int h = kvh * G + row % G;
     const bool final = it.slot < 0;
     const float inv = !final ? 1.f : l[r] == 0.f ? 0.f : 1.f / l[r];   // no keys: zeros
-    // Partial results: rows of the item's second tile go to the next slot, as do an alt item's
-    // odd key tiles, which this kernel does not treat apart (that state is empty).
+    // Partial results: rows of the item's second tile go to the next slot.
     const int tile = row / (it.tokens * G), in_tile = row - tile * it.tokens * G;
     const int64_t at = (int64_t(it.slot) + tile) * 128 + in_tile;
     T* out = static_cast<T*>(p.out) + tok * p.o_token + h * p.o_head;
@@ -304,7 +303,6 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec) {
     if (cg == 0) {
       if (!final) {
         ml[at] = make_float2(m[r] * c_log2, l[r]);
-        if (it.alt) ml[at + 128] = make_float2(-INFINITY, 0.f);
       } else if (p.lse != nullptr) {
         p.lse[tok * p.heads_q + h] = (m[r] * c_log2 + log2f(l[r])) * 0.6931471805599453f;
       }
@@ -325,10 +323,10 @@ packed_join_kernel(const enigma_sdpa_packed_desc p) {
       reinterpret_cast<const float2*>(opart + int64_t(p.header[enigma_serving::kSlots]) * 128 * D);
   const int state = r / 128, row = r % 128;
   const int tok = g.tok0 + state * g.tokens + row / G;
-  if (row >= g.tokens * G || tok >= g.tok_end || tok >= p.tokens_q || (g.alt && state > 0)) return;
+  if (row >= g.tokens * G || tok >= g.tok_end || tok >= p.tokens_q) return;
   griddep_wait();                                               // the parts are written
-  const int n = g.alt ? 2 * g.parts : g.parts, step = (g.alt ? 1 : 2) * 128;
-  const int64_t at = int64_t(g.slot + (g.alt ? 0 : state)) * 128 + row;
+  const int n = g.parts, step = 2 * 128;
+  const int64_t at = int64_t(g.slot + state) * 128 + row;
   enigma_serving::RowJoin<V> join;
   join.best(ml + at, step, n, lane);
   join.seal();

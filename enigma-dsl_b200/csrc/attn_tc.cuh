@@ -6,8 +6,10 @@
 // tokens with all G heads of their group, so every row of a tile reads the same K and V, a
 // short sequence does not pay a tile per head, and a causal tile's rows end within
 // `tokens` keys of each other.  A work item is two row tiles (256 rows) of one kv head and a
-// range of 128-key tiles; or one row tile twice (alt), the even key tiles with one softmax
-// state and the odd ones with the other, when there is no second row tile to fill the SM.
+// range of 128-key tiles; or (paged, alt) one row tile twice, the even key tiles with one softmax
+// state and the odd ones with the other, when there is no second row tile to fill the SM.  An alt
+// item is its CTA's only one and the rings are even, so a state meets the same stages throughout
+// and waits for every phase of their barriers.
 //
 //   warp 0      TMA: both Q tiles, then K and V tiles into rings of C::STAGES
 //   warps 1, 2  one thread each issues the tcgen05.mma of softmax state i = warp - 1:
@@ -122,7 +124,7 @@ __device__ __forceinline__ Work make_work(const Params& p, int t) {
     const int4* it = reinterpret_cast<const int4*>(p.list) +
                      int64_t(t) * (enigma_serving::kItemInts / 4);
     const int4 a = __ldg(it), b = __ldg(it + 1), c = __ldg(it + 2);
-    // q0 lq k0 lk | t0 tokens j0 j1 | kvh alt slot -
+    // q0 lq k0 lk | t0 tokens j0 j1 | kvh slot - -
     w.seq0 = a.x;
     w.tok0 = a.x + b.x;
     w.tok_end = a.x + a.y;
@@ -130,24 +132,18 @@ __device__ __forceinline__ Work make_work(const Params& p, int t) {
     w.lk = a.w;
     w.off = p.causal ? a.w - a.y + 1 : a.w;
     w.kvh = c.x;
-    w.alt = c.y != 0;
-    w.slot = c.z;
+    w.alt = false;
+    w.slot = c.y;
     w.j0 = b.z;
-    if (w.alt) {
-      w.all = max(b.w - b.z, 0);
-      w.cnt0 = (w.all + 1) / 2;
-      w.cnt1 = w.all / 2;
-    } else {
-      auto tiles = [&](int first) {
-        const int last = min(first + p.tokens, w.tok_end) - 1;
-        const int keys = p.causal ? min(w.lk, last - w.seq0 + w.off) : w.lk;
-        const int end = first < w.tok_end && keys > 0 ? (keys + BN - 1) / BN : 0;
-        return max(min(end, b.w) - b.z, 0);
-      };
-      w.cnt0 = tiles(w.tok0);
-      w.cnt1 = tiles(w.tok0 + p.tokens);
-      w.all = max(w.cnt0, w.cnt1);
-    }
+    auto tiles = [&](int first) {
+      const int last = min(first + p.tokens, w.tok_end) - 1;
+      const int keys = p.causal ? min(w.lk, last - w.seq0 + w.off) : w.lk;
+      const int end = first < w.tok_end && keys > 0 ? (keys + BN - 1) / BN : 0;
+      return max(min(end, b.w) - b.z, 0);
+    };
+    w.cnt0 = tiles(w.tok0);
+    w.cnt1 = tiles(w.tok0 + p.tokens);
+    w.all = max(w.cnt0, w.cnt1);
   }
   return w;
 }

@@ -22,15 +22,7 @@ constexpr int64_t kItemCost = 2;
 // fp32 partial results.
 constexpr int64_t kMinPart = 4;
 
-struct Pair {
-  PackedItem item;
-  bool single;         // one row tile only
-};
-
-int64_t steps(const PackedItem& it) {
-  const int64_t tiles = std::max(0, it.j1 - it.j0);
-  return it.alt ? (tiles + 1) / 2 : tiles;
-}
+int64_t steps(const PackedItem& it) { return std::max(0, it.j1 - it.j0); }
 
 }  // namespace
 
@@ -38,26 +30,25 @@ int64_t steps(const PackedItem& it) {
 std::vector<int32_t> make_packed_plan(const int64_t* lens_q, const int64_t* lens_k, int64_t n,
                                       int group, int heads_kv, bool causal, int sms) {
   const int64_t tokens = std::max(1, ENIGMA_PACKED_TILE_ROWS / group);
-  std::vector<Pair> pairs;
+  std::vector<PackedItem> pairs;
   int64_t q0 = 0, k0 = 0, total = 0, longest = 0;
   for (int64_t s = 0; s < n; ++s) {
     const int64_t lq = lens_q[s], lk = lens_k[s];
     for (int64_t t0 = 0; t0 < lq; t0 += 2 * tokens) {
-      Pair p;
+      PackedItem p;
       std::memset(&p, 0, sizeof(p));
-      p.item.q0 = int(q0);
-      p.item.lq = int(lq);
-      p.item.k0 = int(k0);
-      p.item.lk = int(lk);
-      p.item.t0 = int(t0);
-      p.item.tokens = int(tokens);
+      p.q0 = int(q0);
+      p.lq = int(lq);
+      p.k0 = int(k0);
+      p.lk = int(lk);
+      p.t0 = int(t0);
+      p.tokens = int(tokens);
       const int64_t last = std::min(t0 + 2 * tokens, lq) - 1;
       const int64_t keys = causal ? std::min(lk, last + lk - lq + 1) : lk;
-      p.item.j1 = keys > 0 ? int((keys + 127) / 128) : 0;
-      p.item.slot = -1;
-      p.single = t0 + tokens >= lq;
-      total += (steps(p.item) + kItemCost) * heads_kv;
-      longest = std::max(longest, steps(p.item) + kItemCost);
+      p.j1 = keys > 0 ? int((keys + 127) / 128) : 0;
+      p.slot = -1;
+      total += (steps(p) + kItemCost) * heads_kv;
+      longest = std::max(longest, steps(p) + kItemCost);
       pairs.push_back(p);
     }
     q0 += lq;
@@ -70,15 +61,13 @@ std::vector<int32_t> make_packed_plan(const int64_t* lens_q, const int64_t* lens
   std::vector<PackedItem> items;
   std::vector<PackedGroup> groups;
   int64_t slots = 0;
-  for (const Pair& p : pairs) {
+  for (const PackedItem& p : pairs) {
     for (int h = 0; h < heads_kv; ++h) {
-      PackedItem it = p.item;
+      PackedItem it = p;
       it.kvh = h;
       const int64_t tiles = it.j1;
-      const bool alt = split && p.single && tiles > kMinPart;
-      const int64_t per = alt ? 2 * part : part;
-      const int64_t parts = split ? std::max<int64_t>(1, (tiles + per - 1) / per) : 1;
-      if (parts == 1 && !alt) {
+      const int64_t parts = split ? std::max<int64_t>(1, (tiles + part - 1) / part) : 1;
+      if (parts == 1) {
         items.push_back(it);
         continue;
       }
@@ -90,9 +79,7 @@ std::vector<int32_t> make_packed_plan(const int64_t* lens_q, const int64_t* lens
       g.kvh = h;
       g.slot = int(slots);
       g.parts = int(parts);
-      g.alt = alt;
       groups.push_back(g);
-      it.alt = alt;
       for (int64_t x = 0; x < parts; ++x) {
         it.j0 = int(tiles * x / parts);
         it.j1 = int(tiles * (x + 1) / parts);

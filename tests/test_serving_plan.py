@@ -34,12 +34,11 @@ def test_plan_covers_every_pair_of_row_and_key_once(heads_q, heads_kv, causal, l
     group = heads_q // heads_kv
     starts_q, starts_k = np.cumsum([0] + lens_q), np.cumsum([0] + lens_k)
     seen, used = {}, set()
-    for q0, lq, k0, lk, t0, tokens, j0, j1, kvh, alt, slot, _ in items:
+    for q0, lq, k0, lk, t0, tokens, j0, j1, kvh, slot, _, _ in items:
         assert tokens == max(1, 128 // group) and 0 <= kvh < heads_kv and 0 <= t0 < lq
         assert any((starts_q[i], lens_q[i], starts_k[i], lens_k[i]) == (q0, lq, k0, lk)
                    for i in range(len(lens_q)))
-        assert not alt or t0 + tokens >= lq
-        seen.setdefault((q0 + t0, kvh), []).append((j0, j1, slot, alt))
+        seen.setdefault((q0 + t0, kvh), []).append((j0, j1, slot))
         if slot >= 0:
             assert 0 <= slot < slots and slot % 2 == 0 and slot not in used
             used.add(slot)
@@ -59,9 +58,9 @@ def test_plan_covers_every_pair_of_row_and_key_once(heads_q, heads_kv, causal, l
             g = by_group[tok, kvh]
             assert g[1] == starts_q[i] + lens_q[i] and g[2] == tokens and g[5] == len(parts)
             assert [p[2] for p in parts] == list(range(g[4], g[4] + 2 * len(parts), 2))
-            assert all(p[3] == g[6] for p in parts) and group <= 128
+            assert group <= 128
         else:
-            assert len(parts) == 1 and (tok, kvh) not in by_group and not parts[0][3]
+            assert len(parts) == 1 and (tok, kvh) not in by_group
 
 
 def test_plan_is_even():
@@ -71,7 +70,7 @@ def test_plan_is_even():
                         ([1] * 5, (14, 2)), ([20000], (14, 2))):
         offsets, items, _, _ = _parts(cuda_ops.PackedPlan(lens, heads_q=heads[0],
                                                           heads_kv=heads[1], device="cpu"))
-        cost = [(i[7] - i[6]) / (1 + i[9]) + 2 for i in items]
+        cost = [i[7] - i[6] + 2 for i in items]
         load = [sum(cost[a:b]) for a, b in zip(offsets, offsets[1:])]
         assert max(load) <= sum(cost) / len(load) + 1.5 * max(cost)
 
