@@ -58,6 +58,7 @@ cudaError_t launch(const enigma_sdpa_packed_desc& d, cudaStream_t s) {
   p.o_head = d.o_head;
   p.heads_q = int(d.heads_q);
   p.causal = d.causal != 0;
+  p.one = d.header[kItems] == d.header[kCtas];
   p.tokens_q = int(d.tokens_q);
   p.tokens_k = int(d.tokens_k);
   attn_tc_kernel<D, false><<<unsigned(d.header[kCtas]), THREADS, Cfg<D>::SMEM, s>>>(

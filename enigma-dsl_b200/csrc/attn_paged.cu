@@ -34,8 +34,8 @@ template <int D>
 struct DCfg {
   static constexpr int ATOMS = D / 64;
   static constexpr int TILE = CHUNK * D * 2;            // one of K or V
-  static constexpr int STAGES = D == 64 ? 4 : 3;
-  static constexpr int SMEM = STAGES * 2 * TILE + 1024;   // + 2 batch + 1 ints
+  static constexpr int STAGES = D == 64 ? 4 : 3;          // 3 or 2 CTAs on an SM
+  static constexpr int DEEP = D == 64 ? 12 : 6;           // one CTA on an SM
 };
 
 struct DecodeParams {
@@ -45,14 +45,14 @@ struct DecodeParams {
   int batch, heads_kv, group, blocks, rows;  // blocks of `rows` <= 16 heads per group
   int width, n_slots, pages, page_shift, box_shift, prefix, base;
   int fold;                                  // the prefix's keys are read here too
-  int direct;                                // a CTA per unit, which writes the final result
-  __nv_bfloat16* out;
+  __nv_bfloat16* out;                        // DIRECT
   int64_t o_batch, o_head;
   float scale_log2;
   float* opart;                              // [slot][rows][D]
   float2* ml;                                // [slot][rows]
   int32_t* starts;                           // [batch + 1] chunks (of one unit) before b
   uint32_t* status;
+  int stages;
 };
 
 // Element c (16 bytes) of row r in a 128-byte-swizzled tile.
@@ -111,9 +111,8 @@ __device__ __forceinline__ int chunks_of(const DecodeParams& p, int len) {
 struct Chunk {
   int key0, lo, hi, seq;       // seq: whose table row holds its pages
 };
-__device__ __forceinline__ Chunk chunk_at(const DecodeParams& p, int b, int len, int j) {
-  const int np = prefix_chunks(p, len);
-  Chunk c;
+__device__ __forceinline__ Chunk chunk_at(const DecodeParams& p, int b, int len, int np, int j) {
+  Chunk c;                     // np: chunks of the prefix
   if (j < np) {
     c.key0 = j * CHUNK;
     c.lo = 0;
@@ -157,153 +156,171 @@ __device__ __forceinline__ Segment segment_at(const int* starts, int batch, int 
   return s;
 }
 
-template <int D>
+// DIRECT: a CTA per unit, which writes the final result; no work list, nothing to join.
+template <int D, bool DIRECT>
 __global__ void __launch_bounds__(DTHREADS, D == 64 ? 3 : 2)
 paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const DecodeParams p) {
   using C = DCfg<D>;
-  constexpr int ST = C::STAGES;
+  const int ST = p.stages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   int* s_starts = reinterpret_cast<int*>(ring + ST * 2 * C::TILE);    // [batch + 1]
   int* s_len = s_starts + p.batch + 1;                                // [batch]
-  __shared__ uint64_t full[ST][2], empty[ST];   // a stage's chunks for either team
+  __shared__ uint64_t full[C::DEEP][2], empty[C::DEEP];   // a stage's chunks for either team
   __shared__ float s_m[DWARPS][ROWS], s_l[DWARPS][ROWS];    // direct
   __shared__ int s_warp[DWARPS + 1], s_pages[PAGES];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t most = int64_t(p.width) << p.page_shift;
   griddep_launch_dependents();
 
-  if (tid == 0) {
-    for (int s = 0; s < ST; ++s) {
-      mbar_init(&full[s][0], 1);
-      mbar_init(&full[s][1], 1);
-      mbar_init(&empty[s], 2);               // the chunk's two warps
-    }
+  if (tid < ST) {
+    mbar_init(&full[tid][0], 1);
+    mbar_init(&full[tid][1], 1);
+    mbar_init(&empty[tid], 2);               // the chunk's two warps
     fence_barrier_init();
+  }
+  if (tid == DWARPS * 32) {
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
-  // Chunk counts before each sequence.
-  int run = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += DTHREADS) {
-    const int b = b0 + tid;
-    int v = 0;
-    if (b < p.batch) {
-      const int len = len_of(p.lens, p.slots, p.n_slots, most, b);
-      s_len[b] = len;
-      v = chunks_of(p, len);
-    }
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) s_warp[warp] = x;
-    __syncthreads();
-    int before = run;
-    for (int w = 0; w < warp; ++w) before += s_warp[w];
-    if (b < p.batch) s_starts[b] = before + x - v;
-    for (int w = 0; w <= DWARPS; ++w) run += s_warp[w];
-    __syncthreads();
-  }
-  if (tid == 0) s_starts[p.batch] = run;
-  __syncthreads();
-  if (blockIdx.x == 0 && !p.direct)
-    for (int b = tid; b <= p.batch; b += DTHREADS) p.starts[b] = s_starts[b];
-
   const int per_b = p.heads_kv * p.blocks;
-  const int64_t T = int64_t(run) * per_b;
-  const int64_t P = min(int64_t(gridDim.x), T);
-  // This kernel reads nothing of the prefix kernel's, with which it shares the SMs, but the join
-  // waits only for this one: so it ends after that one.
-  if (!p.direct && int64_t(blockIdx.x) >= P) {
-    griddep_wait();
-    return;
-  }
-  int64_t c0, c1;
-  if (p.direct) {                            // unit blockIdx.x; without keys: zeros
-    const int b = int(blockIdx.x) / per_b, n = s_starts[b + 1] - s_starts[b];
-    c0 = int64_t(s_starts[b]) * per_b + int64_t(int(blockIdx.x) - b * per_b) * n;
-    c1 = c0 + n;
-    if (n == 0) {
-      const int u = int(blockIdx.x) - b * per_b, block = u % p.blocks;
-      const int rows = min(p.rows, p.group - block * p.rows);
-      __nv_bfloat16* to = p.out + b * p.o_batch +
-                          int64_t(u / p.blocks * p.group + block * p.rows) * p.o_head;
+  int64_t c0 = 0, c1 = 0;
+  Segment unit = {};                         // DIRECT: unit blockIdx.x
+  int unit_len = 0;
+  if (DIRECT) {
+    unit.b = int(blockIdx.x) / per_b;
+    const int u = int(blockIdx.x) - unit.b * per_b;
+    unit.kvh = u / p.blocks;
+    unit.block = u - unit.kvh * p.blocks;
+    unit_len = len_of(p.lens, p.slots, p.n_slots, most, unit.b);
+    unit.n = chunks_of(p, unit_len);
+    c1 = unit.n;
+    if (unit.n == 0) {                       // no keys: zeros
+      const int rows = min(p.rows, p.group - unit.block * p.rows);
+      __nv_bfloat16* to = p.out + unit.b * p.o_batch +
+                          int64_t(unit.kvh * p.group + unit.block * p.rows) * p.o_head;
       for (int x = tid; x < rows * (D / 8); x += DTHREADS)
         *reinterpret_cast<uint4*>(to + x / (D / 8) * p.o_head + x % (D / 8) * 8) =
             make_uint4(0, 0, 0, 0);
       return;
     }
+    __syncthreads();
   } else {
+    // Chunk counts before each sequence.
+    int run = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += DTHREADS) {
+      const int b = b0 + tid;
+      int v = 0;
+      if (b < p.batch) {
+        const int len = len_of(p.lens, p.slots, p.n_slots, most, b);
+        s_len[b] = len;
+        v = chunks_of(p, len);
+      }
+      int x = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (lane == 31) s_warp[warp] = x;
+      __syncthreads();
+      int before = run;
+      for (int w = 0; w < warp; ++w) before += s_warp[w];
+      if (b < p.batch) s_starts[b] = before + x - v;
+      for (int w = 0; w <= DWARPS; ++w) run += s_warp[w];
+      __syncthreads();
+    }
+    if (tid == 0) s_starts[p.batch] = run;
+    __syncthreads();
+    if (blockIdx.x == 0)
+      for (int b = tid; b <= p.batch; b += DTHREADS) p.starts[b] = s_starts[b];
+    const int64_t T = int64_t(run) * per_b;
+    const int64_t P = min(int64_t(gridDim.x), T);
+    // This kernel reads nothing of the prefix kernel's, with which it shares the SMs, but the join
+    // waits only for this one: so it ends after that one.
+    if (int64_t(blockIdx.x) >= P) {
+      griddep_wait();
+      return;
+    }
     c0 = share(T, blockIdx.x, P);
     c1 = share(T, int64_t(blockIdx.x) + 1, P);
   }
+  auto segment = [&](int64_t at) {
+    return DIRECT ? unit : segment_at(s_starts, p.batch, per_b, p.blocks, at, c1);
+  };
 
   if (warp == DWARPS) {
     // ---------------------------------------------------------------- producer
-    // Lanes 0 .. 15 load K's boxes, 16 .. 31 V's: box x = rows [(x / ATOMS) << box_shift, ...),
-    // columns 64 (x % ATOMS).
-    const int x = lane & 15, box = x / C::ATOMS, atom = x % C::ATOMS;
-    const bool is_v = lane >= 16;
-    const int per = CHUNK >> p.box_shift, ahead = PAGES / per;   // boxes per chunk; chunks looked up
-    int i = 0;
+    // One lane issues all boxes of a chunk: each lane its own costs 150 cycles a box, which left
+    // the ring empty.
+    const int per_shift = 6 - p.box_shift, per = 1 << per_shift;   // boxes per chunk
+    const int ahead = PAGES >> per_shift;                            // chunks looked up at once
+    // Stages, parities and places in the look-up are counted on: a division here, in a warp with
+    // nothing else to run, held up every chunk (1300 cycles a chunk with five of them, 500 without).
+    int st = 0, wraps = 0, team = 0;
     for (int64_t at = c0; at < c1;) {
-      const Segment s = segment_at(s_starts, p.batch, per_b, p.blocks, at, c1);
-      const int len = s_len[s.b];
-      for (int j = s.j0; j < s.j0 + s.n; ++j, ++i) {
-        const Chunk c = chunk_at(p, s.b, len, j);
+      const Segment s = segment(at);
+      const int len = DIRECT ? unit_len : s_len[s.b], np = prefix_chunks(p, len);
+      int in = ahead;
+      for (int j = s.j0; j < s.j0 + s.n; ++j) {
+        const Chunk c = chunk_at(p, s.b, len, np, j);
         const int key0 = c.key0;
         const int boxes = (min(CHUNK, c.hi - key0) + (1 << p.box_shift) - 1) >> p.box_shift;
         // Page numbers of the next `ahead` chunks at once: one look-up per chunk, even if made a
-        // chunk ahead, left the ring waiting for the table's latency.
-        const int in = (j - s.j0) % ahead;
-        if (in == 0) {
+        // chunk ahead, leaves the ring waiting for the table's latency.
+        if (in == ahead) {
+          in = 0;
           __syncwarp();
 #pragma unroll
           for (int y = 0; y < PAGES; y += 32) {
-            const int jj = j + (y + lane) / per;
+            const int jj = j + ((y + lane) >> per_shift);
             if (jj < s.j0 + s.n) {
-              const Chunk cc = chunk_at(p, s.b, len, jj);
-              const int key = cc.key0 + (((y + lane) % per) << p.box_shift);
+              const Chunk cc = chunk_at(p, s.b, len, np, jj);
+              const int key = cc.key0 + (((y + lane) & (per - 1)) << p.box_shift);
               s_pages[y + lane] = page_at(p.table, p.slots, p.n_slots, p.width, p.pages, cc.seq,
                                           key >> p.page_shift);
             }
           }
           __syncwarp();
         }
-        const int page_now = box < boxes ? s_pages[in * per + box] : 0;
-        const int st = i % ST;
-        if (!__all_sync(0xffffffffu, mbar_wait(&empty[st], ((i / ST) & 1) ^ 1, p.status))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&empty[st], (wraps & 1) ^ 1, p.status))) {
           at = c1;
           break;
         }
-        if (lane == 0)
-          mbar_arrive_expect_tx(&full[st][i & 1], (uint32_t(2 * boxes * C::ATOMS) * 128u) << p.box_shift);
+        uint64_t* bar = &full[st][team];
+        if (elect_one()) {
+          mbar_arrive_expect_tx(bar, (uint32_t(2 * boxes * C::ATOMS) * 128u) << p.box_shift);
+          for (int x = 0; x < boxes; ++x) {
+            const int page = s_pages[in * per + x];
+            const int row = (key0 + (x << p.box_shift)) & ((1 << p.page_shift) - 1);
+            uint8_t* dst = ring + 2 * st * C::TILE + ((x << p.box_shift) * 128);
+#pragma unroll
+            for (int a = 0; a < C::ATOMS; ++a) {
+              tma_load_4d(dst + a * CHUNK * 128, &tmK, bar, a * 64, row, s.kvh, page);
+              tma_load_4d(dst + C::TILE + a * CHUNK * 128, &tmV, bar, a * 64, row, s.kvh, page);
+            }
+          }
+        }
         __syncwarp();
-        if (box < boxes)
-          tma_load_4d(ring + (2 * st + (is_v ? 1 : 0)) * C::TILE + atom * CHUNK * 128 +
-                          ((box << p.box_shift) * 128),
-                      is_v ? &tmV : &tmK, &full[st][i & 1], atom * 64,
-                      (key0 + (box << p.box_shift)) & ((1 << p.page_shift) - 1), s.kvh, page_now);
-        __syncwarp();
+        ++in;
+        team ^= 1;
+        if (++st == ST) st = 0, ++wraps;
       }
       at += s.n;
     }
-    griddep_wait();
+    if (!DIRECT) griddep_wait();
     return;
   }
 
   // ------------------------------------------------------------------ consumers
   const int g = lane >> 2, quad = lane & 3;
   const int team = warp >> 1;                               // takes every second chunk
-  int i = 0;
+  int turn = 0, st = -1, wraps = 0;                         // whose chunk is next, its stage
   for (int64_t at = c0; at < c1;) {
-    const Segment s = segment_at(s_starts, p.batch, per_b, p.blocks, at, c1);
-    const int len = s_len[s.b];
+    const Segment s = segment(at);
+    const int len = DIRECT ? unit_len : s_len[s.b], np = prefix_chunks(p, len);
     const int rows = min(p.rows, p.group - s.block * p.rows);
     uint32_t q[D / 16][4];
     {
@@ -324,17 +341,18 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     bool ok = true;
-    for (int j = s.j0; j < s.j0 + s.n; ++j, ++i) {
-      if ((i & 1) != team) continue;
-      const int st = i % ST;
+    for (int j = s.j0; j < s.j0 + s.n; ++j) {
+      if (++st == ST) st = 0, ++wraps;
+      turn ^= 1;
+      if ((turn ^ 1) != team) continue;
       // A team sees its own chunks only, so each has its own barrier per stage: the parity of
       // one that also counted the other team's could be a phase old.
-      const int uses = ST % 2 == 0 ? i / ST : i / ST / 2;   // of this barrier before
+      const int uses = ST % 2 == 0 ? wraps : wraps >> 1;    // of this barrier before
       ok = __all_sync(0xffffffffu, mbar_wait(&full[st][team], uses & 1, p.status));
       if (!ok) break;
       uint8_t* tile_k = ring + 2 * st * C::TILE;
       uint8_t* tile_v = tile_k + C::TILE;
-      const Chunk ch = chunk_at(p, s.b, len, j);
+      const Chunk ch = chunk_at(p, s.b, len, np, j);
       const int row0 = (warp & 1) * WKEYS;                  // this warp's first row of the chunk
       const int key0 = ch.key0 + row0;
       float sc[WKEYS / 8][4];
@@ -418,7 +436,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
     }
-    if (p.direct) {
+    if (DIRECT) {
       // The ring is idle once every warp is here: it takes the warps' states, each thread sums
       // two columns of a row over the warps, in their order.
       if (!warps_all(ok)) return;                           // a wait ran out (status is set)
@@ -678,6 +696,9 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
     p.pairs = y.pairs;
     p.splits = y.splits;
     p.row_tiles = y.row_tiles;
+    const int tiles = (y.prefix + BN - 1) / BN;
+    p.per_split = tiles / y.splits;
+    p.extra = tiles % y.splits;
     const int items = int(d.heads_kv) * y.pairs * y.splits;
     attn_tc_kernel<D, true><<<unsigned(items), THREADS, Cfg<D>::SMEM, s>>>(mq, mk, mv, p, items);
     e = cudaGetLastError();
@@ -703,7 +724,6 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
   p.prefix = y.prefix;
   p.base = y.prefix / CHUNK * CHUNK;
   p.fold = y.fold;
-  p.direct = y.direct;
   p.out = static_cast<__nv_bfloat16*>(d.out);
   p.o_batch = d.o_batch;
   p.o_head = d.o_head;
@@ -712,23 +732,29 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
   p.ml = reinterpret_cast<float2*>(ws + y.d_ml);
   p.starts = reinterpret_cast<int32_t*>(ws + y.starts);
   p.status = status;
-  const int smem = DCfg<D>::SMEM + int(2 * d.batch + 1) * 4;
+  // A CTA that has the SM to itself needs the whole ring to cover the loads' latency.
+  p.stages = y.ctas <= enigma::sm_count() ? DCfg<D>::DEEP : DCfg<D>::STAGES;
+  const int smem = p.stages * 2 * DCfg<D>::TILE + 1024 + (y.direct ? 0 : int(2 * d.batch + 1) * 4);
+  const auto kernel = y.direct ? paged_decode_kernel<D, true> : paged_decode_kernel<D, false>;
   {
     static std::atomic<uint64_t> ready{0};                  // devices where the attribute is set
     int dev = 0;
     e = cudaGetDevice(&dev);
     if (e == cudaSuccess && !(dev < 64 && (ready.load() >> dev & 1))) {
-      e = cudaFuncSetAttribute(paged_decode_kernel<D>,
-                               cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               DCfg<D>::SMEM + 8193 * 4);
+      const int most = DCfg<D>::DEEP * 2 * DCfg<D>::TILE + 1024 + 8193 * 4;
+      e = cudaFuncSetAttribute(paged_decode_kernel<D, true>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(paged_decode_kernel<D, false>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, most);
       if (e == cudaSuccess && dev < 64) ready.fetch_or(uint64_t(1) << dev);
     }
     if (e != cudaSuccess) return e;
   }
   if (y.splits > 0) {
-    e = enigma::launch_dependent(paged_decode_kernel<D>, unsigned(y.ctas), DTHREADS, smem, s, mk, mv, p);
+    e = enigma::launch_dependent(kernel, unsigned(y.ctas), DTHREADS, smem, s, mk, mv, p);
   } else {
-    paged_decode_kernel<D><<<unsigned(y.ctas), DTHREADS, smem, s>>>(mk, mv, p);
+    kernel<<<unsigned(y.ctas), DTHREADS, smem, s>>>(mk, mv, p);
     e = cudaGetLastError();
   }
   if (e != cudaSuccess || y.direct) return e;

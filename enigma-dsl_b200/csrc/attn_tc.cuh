@@ -81,10 +81,12 @@ struct Params {
   float* lse;
   int64_t o_token, o_head;
   int heads_q, causal, tokens_q, tokens_k;
+  int one;                         // each CTA has exactly one item
   // paged prefix
   const int32_t *table, *lens, *slots;
   int width, n_slots, pages, page_shift, box_shift, prefix, batch, heads_kv;
   int pairs, splits, row_tiles;
+  int per_split, extra;            // key tiles of a part; the first `extra` have one more
 };
 
 // One item, as every role sees it.
@@ -113,9 +115,8 @@ __device__ __forceinline__ Work make_work(const Params& p, int t) {
     w.k0 = 0;
     w.lk = p.prefix;
     w.off = p.prefix;
-    const int tiles = (p.prefix + BN - 1) / BN;
-    w.j0 = int(int64_t(tiles) * split / p.splits);
-    w.all = int(int64_t(tiles) * (split + 1) / p.splits) - w.j0;
+    w.j0 = split * p.per_split + min(split, p.extra);
+    w.all = p.per_split + (split < p.extra ? 1 : 0);
     w.alt = 2 * pair + 1 >= p.row_tiles;
     w.cnt0 = w.alt ? (w.all + 1) / 2 : w.all;
     w.cnt1 = w.alt ? w.all / 2 : w.all;
@@ -238,8 +239,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   const int lane = threadIdx.x & 31;
   griddep_launch_dependents();               // the next kernel may take SMs that are free
   // Packed: the plan lists each CTA's items.  Paged: one item per CTA.
-  const int t_begin = PAGED ? int(blockIdx.x) : __ldg(p.offsets + blockIdx.x);
-  const int t_end = PAGED ? min(t_begin + 1, items) : __ldg(p.offsets + blockIdx.x + 1);
+  const bool one = PAGED || p.one;
+  const int t_begin = one ? int(blockIdx.x) : __ldg(p.offsets + blockIdx.x);
+  const int t_end = one ? min(t_begin + 1, items) : __ldg(p.offsets + blockIdx.x + 1);
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmQ);
@@ -301,27 +303,24 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         };
         ok = load_q(0, w.cnt0);
         if (!ok) break;
-        // Paged: lane x loads box x of each tile, rows [(x / ATOMS) << box_shift, ...), atom
-        // x % ATOMS; the page number of the next tile is read one tile ahead.
-        const int box = PAGED ? lane / C::ATOMS : 0, atom = PAGED ? lane % C::ATOMS : 0;
-        int at = 0, row_in_page = 0;
+        // Paged: lane x knows the page of box x of the next tile, read one tile ahead.  One lane
+        // issues all boxes: each lane its own costs 150 cycles a box.
+        int at = 0;
         auto look_up = [&](int j) {
-          const int key = j * BN + (box << p.box_shift);
-          row_in_page = key & ((1 << p.page_shift) - 1);
-          at = page_at(p.table, p.slots, p.n_slots, p.width, p.pages, 0, key >> p.page_shift);
+          at = page_at(p.table, p.slots, p.n_slots, p.width, p.pages, 0,
+                       (j * BN + (lane << p.box_shift)) >> p.page_shift);
         };
-        if (PAGED && box < (BN >> p.box_shift)) look_up(w.j0);
+        const bool looks = PAGED && lane < (BN >> p.box_shift);
+        if (looks) look_up(w.j0);
         for (int j = 0; j < w.all; ++j, ++jg) {
           const int s = jg % ST;
           const uint32_t ph = (jg / ST) & 1;
           const int key0 = (w.j0 + j) * BN;
-          const int at_now = at, row_now = row_in_page;
+          const int at_now = at;
           int boxes = 0;
-          bool mine = false;
           if (PAGED) {
             boxes = (min(BN, w.lk - key0) + (1 << p.box_shift) - 1) >> p.box_shift;
-            mine = box < boxes;
-            if (j + 1 < w.all && box < (BN >> p.box_shift)) look_up(w.j0 + j + 1);
+            if (looks && j + 1 < w.all) look_up(w.j0 + j + 1);
           }
           const uint32_t bytes = PAGED ? (uint32_t(boxes * C::ATOMS) * 128u) << p.box_shift
                                        : uint32_t(C::KV_BYTES);
@@ -330,9 +329,17 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
             if (lane == 0) mbar_arrive_expect_tx(full, bytes);
             __syncwarp();
             if (PAGED) {
-              if (mine)
-                tma_load_4d(dst + atom * BN * 128 + ((box << p.box_shift) * 128), map, full,
-                            atom * 64, row_now, w.kvh, at_now);
+              for (int x = 0; x < boxes; ++x) {
+                const int page = __shfl_sync(0xffffffffu, at_now, x);
+                const int row = (key0 + (x << p.box_shift)) & ((1 << p.page_shift) - 1);
+                if (elect_one()) {
+#pragma unroll
+                  for (int a = 0; a < C::ATOMS; ++a)
+                    tma_load_4d(dst + a * BN * 128 + ((x << p.box_shift) * 128), map, full, a * 64,
+                                row, w.kvh, page);
+                }
+                __syncwarp();
+              }
             } else if (lane == 0) {
 #pragma unroll
               for (int a = 0; a < C::ATOMS; ++a)
