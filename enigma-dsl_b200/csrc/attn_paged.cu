@@ -45,8 +45,12 @@ struct DecodeParams {
   int batch, heads_kv, group, blocks, rows;  // blocks of `rows` <= 16 heads per group
   int width, n_slots, pages, page_shift, box_shift, prefix, base;
   int fold;                                  // the prefix's keys are read here too
-  __nv_bfloat16* out;                        // DIRECT
+  // DIRECT: where the result goes, and the prefix kernel's partial results (0 splits: none)
+  __nv_bfloat16* out;
   int64_t o_batch, o_head;
+  const float* p_opart;
+  const float2* p_ml;
+  int pairs, splits, row_tiles, tokens;
   float scale_log2;
   float* opart;                              // [slot][rows][D]
   float2* ml;                                // [slot][rows]
@@ -127,6 +131,25 @@ __device__ __forceinline__ Chunk chunk_at(const DecodeParams& p, int b, int len,
   return c;
 }
 
+// Where the prefix kernel left the partial results of sequence b's heads of kv head kvh: n rows of
+// its [slot][128], `step` apart; head h of the group is row at + h.
+struct PrefixRows {
+  int64_t at;
+  int n, step;
+};
+__device__ __forceinline__ PrefixRows prefix_rows(int splits, int tokens, int row_tiles, int pairs,
+                                                  int group, int b, int kvh) {
+  PrefixRows r = {0, 0, 0};
+  if (splits == 0) return r;
+  const int tile = b / tokens, pair = tile >> 1;
+  const bool alt = 2 * pair + 1 >= row_tiles;
+  r.n = alt ? 2 * splits : splits;
+  r.step = (alt ? 1 : 2) * BM;
+  r.at = (int64_t(kvh * pairs + pair) * splits * 2 + (alt ? 0 : (tile & 1))) * BM +
+         (b - tile * tokens) * group;
+  return r;
+}
+
 // A run of one unit's chunks.
 struct Segment {
   int b, kvh, block, unit;
@@ -196,8 +219,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     unit.block = u - unit.kvh * p.blocks;
     unit_len = len_of(p.lens, p.slots, p.n_slots, most, unit.b);
     unit.n = chunks_of(p, unit_len);
-    c1 = unit.n;
-    if (unit.n == 0) {                       // no keys: zeros
+    c1 = max(unit.n, 1);                     // one segment, if an empty one
+    if (unit.n == 0 && p.splits == 0) {      // no keys: zeros
       const int rows = min(p.rows, p.group - unit.block * p.rows);
       __nv_bfloat16* to = p.out + unit.b * p.o_batch +
                           int64_t(unit.kvh * p.group + unit.block * p.rows) * p.o_head;
@@ -456,26 +479,58 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           *reinterpret_cast<float2*>(s_o + (warp * ROWS + row) * D + quad * 2 + n * 8) =
               make_float2(o[n][2 * h], o[n][2 * h + 1]);
       }
+      // The prefix kernel ran beside this one; its partial results of these rows join in.
+      const PrefixRows pr = prefix_rows(p.splits, p.tokens, p.row_tiles, p.pairs, p.group, s.b, s.kvh);
+      float2* s_pre = reinterpret_cast<float2*>(s_o + DWARPS * ROWS * D);   // [rows][pr.n]
+      if (pr.n > 0) {
+        griddep_wait();
+        for (int x = tid; x < rows * pr.n; x += DWARPS * 32) {
+          const int row = x / pr.n, i = x - row * pr.n;
+          s_pre[x] = p.p_ml[pr.at + i * pr.step + s.block * p.rows + row];
+        }
+      }
       warps_all(true);
       for (int x = tid; x < rows * (D / 2); x += DWARPS * 32) {
         const int row = x / (D / 2), d = x % (D / 2) * 2;
+        const float2* pre = s_pre + row * pr.n;
         float M = s_m[0][row];
 #pragma unroll
         for (int w = 1; w < DWARPS; ++w) M = fmaxf(M, s_m[w][row]);
+        for (int i = 0; i < pr.n; ++i) M = fmaxf(M, pre[i].x);
         float2 acc = make_float2(0.f, 0.f);
         float L = 0.f;
 #pragma unroll
         for (int w = 0; w < DWARPS; ++w) {
-          const float f = s_m[w][row] == -INFINITY ? 0.f : ex2(s_m[w][row] - M);
+          if (s_m[w][row] == -INFINITY) continue;           // saw no key; o is not written
+          const float f = ex2(s_m[w][row] - M);
           const float2 v = *reinterpret_cast<const float2*>(s_o + (w * ROWS + row) * D + d);
           acc.x = fmaf(v.x, f, acc.x);
           acc.y = fmaf(v.y, f, acc.y);
           L = fmaf(s_l[w][row], f, L);
         }
+        const float* po = p.p_opart + (pr.at + s.block * p.rows + row) * D + d;
+        for (int i0 = 0; i0 < pr.n; i0 += 8) {              // 8 loads in flight
+          float2 v[8];
+          float f[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const float m_i = i0 + u < pr.n ? pre[i0 + u].x : -INFINITY;
+            f[u] = m_i == -INFINITY ? 0.f : ex2(m_i - M);
+            v[u] = make_float2(0.f, 0.f);
+            if (f[u] != 0.f)
+              v[u] = __ldcg(reinterpret_cast<const float2*>(po + (i0 + u) * pr.step * D));
+          }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            acc.x = fmaf(v[u].x, f[u], acc.x);
+            acc.y = fmaf(v[u].y, f[u], acc.y);
+            if (f[u] != 0.f) L = fmaf(pre[i0 + u].y, f[u], L);
+          }
+        }
         const float inv = L == 0.f ? 0.f : 1.f / L;
-        const int64_t at = s.b * p.o_batch +
-                           int64_t(s.kvh * p.group + s.block * p.rows + row) * p.o_head + d;
-        *reinterpret_cast<uint32_t*>(p.out + at) = pack_bf16x2(acc.x * inv, acc.y * inv);
+        const int64_t at_out = s.b * p.o_batch +
+                               int64_t(s.kvh * p.group + s.block * p.rows + row) * p.o_head + d;
+        *reinterpret_cast<uint32_t*>(p.out + at_out) = pack_bf16x2(acc.x * inv, acc.y * inv);
       }
       return;
     }
@@ -528,18 +583,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const JoinParams p) {
   griddep_wait();
   const int b = int(id / p.heads_q), h = int(id - int64_t(b) * p.heads_q);
   const int kvh = h / p.group, gh = h - kvh * p.group;
-  // Prefix partials: rows pf + i * p_step of [slot * 128 + row].
-  int n_p = 0;
-  int64_t p_at = 0, p_step = 0;
-  if (p.splits > 0) {
-    const int tile = b / p.tokens, pair = tile >> 1;
-    const bool alt = 2 * pair + 1 >= p.row_tiles;
-    const int row = (b - tile * p.tokens) * p.group + gh;
-    const int64_t slot = int64_t(kvh * p.pairs + pair) * p.splits * 2 + (alt ? 0 : (tile & 1));
-    n_p = alt ? 2 * p.splits : p.splits;
-    p_step = (alt ? 1 : 2) * BM;
-    p_at = slot * BM + row;
-  }
+  const PrefixRows pr =
+      prefix_rows(p.splits, p.tokens, p.row_tiles, p.pairs, p.group, b, kvh);
   // Own partials: the slots of the CTAs that hold the unit's chunks.
   int n_d = 0;
   int64_t d_at = 0;
@@ -556,10 +601,11 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const JoinParams p) {
   }
   constexpr int V = D / 32;
   enigma_serving::RowJoin<V> join;
-  join.best(p.p_ml + p_at, p_step, n_p, lane);
+  const int64_t p_at = pr.at + gh;
+  join.best(p.p_ml + p_at, pr.step, pr.n, lane);
   join.best(p.d_ml + d_at, p.rows, n_d, lane);
   join.seal();
-  join.add(p.p_ml + p_at, p_step, p.p_opart + p_at * D, p_step * D, n_p, D, lane);
+  join.add(p.p_ml + p_at, pr.step, p.p_opart + p_at * D, int64_t(pr.step) * D, pr.n, D, lane);
   join.add(p.d_ml + d_at, p.rows, p.d_opart + d_at * D, int64_t(p.rows) * D, n_d, D, lane);
   const float inv = join.l == 0.f ? 0.f : 1.f / join.l;
   __nv_bfloat16* out = p.out + b * p.o_batch + h * p.o_head + lane;
@@ -587,7 +633,7 @@ int log2_of(int64_t x) {
   return n;
 }
 
-constexpr int64_t kFoldBytes = 128ll << 20, kDirectKeys = 1024;
+constexpr int64_t kFoldBytes = 128ll << 20, kDirectKeys = 1536;
 
 struct Layout {
   int group, tokens, row_tiles, pairs, splits, prefix;    // prefix part
@@ -607,12 +653,15 @@ Layout layout_of(const enigma_sdpa_shared_prefix_desc& d) {
   y.pairs = (y.row_tiles + 1) / 2;
   const int tiles = (y.prefix + BN - 1) / BN;
   // Short rows: one CTA per unit reads all its keys, the prefix's too, and writes the result; no
-  // second and third launch, no partial results.  Measured (graph, us, alone / with the prefix
-  // apart): 4 x 512 keys, 2 kv heads of 64: 10.5 / 12.4; 16 x 512, 8 of 128: 10.7 / 14.6; 32 x 1024
-  // + 128: 19.1 / 23.8; but 8 x 2048 + 128: 26.2 / 15.2, 32 x 2048 + 64, 2 of 64: 27.0 / 16.3.
-  y.direct = d.table_width * d.page <= kDirectKeys &&
-             d.batch * y.prefix * d.heads_kv * d.head_dim * 4 <= kFoldBytes;
-  y.fold = y.direct && y.prefix > 0;
+  // second launch, no partial results.  Measured (graph, us, so / with the prefix apart): 4 x 512
+  // shared keys, 2 kv heads of 64: 7.9 / 12.4; 16 x 512, 8 of 128: 9.8 / 14.6; 32 x 1024: 16.7 /
+  // 23.8; with longer rows a CTA's chain of chunks is: 8 x 2048: 26 / 12.8, 8 x 2048, 2 of 64: 27 / 13.8.
+  const int64_t most = d.table_width * d.page;
+  y.fold = y.prefix > 0 && most <= kDirectKeys &&
+           d.batch * y.prefix * d.heads_kv * d.head_dim * 4 <= kFoldBytes;
+  // A CTA per unit reads the own keys too, and joins them with the prefix's partial results, where
+  // no row has many of them; else they are split over the SMs and joined by a third launch.
+  y.direct = y.fold || most - y.prefix <= kDirectKeys;
   if (tiles > 0 && !y.fold) {
     // As many parts of the keys as there are SMs, each at least two tiles.
     const int64_t units = int64_t(d.heads_kv) * y.pairs;
@@ -623,11 +672,9 @@ Layout layout_of(const enigma_sdpa_shared_prefix_desc& d) {
   y.blocks = (y.group + ROWS - 1) / ROWS;
   y.rows = (y.group + y.blocks - 1) / y.blocks;
   y.ctas = sms * (d.head_dim == 64 ? 3 : 2);
-  if (y.direct) {
-    y.ctas = int(d.batch * d.heads_kv) * y.blocks;
-    return y;
-  }
-  const int64_t d_slots = (int64_t(y.ctas) + d.batch * d.heads_kv * y.blocks) * DWARPS;
+  if (y.direct) y.ctas = int(d.batch * d.heads_kv) * y.blocks;
+  const int64_t d_slots =
+      y.direct ? 0 : (int64_t(y.ctas) + d.batch * d.heads_kv * y.blocks) * DWARPS;
   size_t at = 0;
   auto take = [&](int64_t bytes) {
     const size_t here = at;
@@ -638,7 +685,7 @@ Layout layout_of(const enigma_sdpa_shared_prefix_desc& d) {
   y.p_ml = take(p_slots * BM * 8);
   y.d_opart = take(d_slots * y.rows * d.head_dim * 4);
   y.d_ml = take(d_slots * y.rows * 8);
-  y.starts = take((d.batch + 1) * 4);
+  y.starts = take(y.direct ? 0 : (d.batch + 1) * 4);
   y.total = at;
   return y;
 }
@@ -727,6 +774,12 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
   p.out = static_cast<__nv_bfloat16*>(d.out);
   p.o_batch = d.o_batch;
   p.o_head = d.o_head;
+  p.p_opart = reinterpret_cast<const float*>(ws + y.p_opart);
+  p.p_ml = reinterpret_cast<const float2*>(ws + y.p_ml);
+  p.pairs = y.pairs;
+  p.splits = y.splits;
+  p.row_tiles = y.row_tiles;
+  p.tokens = y.tokens;
   p.scale_log2 = scale_log2;
   p.opart = reinterpret_cast<float*>(ws + y.d_opart);
   p.ml = reinterpret_cast<float2*>(ws + y.d_ml);
