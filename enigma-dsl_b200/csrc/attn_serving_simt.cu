@@ -310,36 +310,81 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec) {
   }
 }
 
-// Joins the partial results of split rows.  One warp per row; grid (groups, rows / 8).
+// Joins the partial results of split rows: O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, always in
+// the same order.  A warp takes four rows: 8 lanes each have a row's (m, l), and the four rows'
+// loads of a part are in flight together (one row per warp: the loads' latency is the time, 13 us
+// for 72 pairs of tiles in 2 parts).  grid (groups, rows / 32).
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
 packed_join_kernel(const enigma_sdpa_packed_desc p) {
+  constexpr int R = 4;
   const int lane = threadIdx.x & 31, D = int(p.head_dim), G = int(p.heads_q / p.heads_kv);
-  const int r = int(blockIdx.y) * 8 + (threadIdx.x >> 5);       // row of the pair of tiles
+  const int r0 = (int(blockIdx.y) * 8 + (threadIdx.x >> 5)) * R;   // first row, of 2 * 128
   const PackedGroup g = reinterpret_cast<const PackedGroup*>(
       p.plan + p.header[enigma_serving::kGroupsAt])[blockIdx.x];
   const float* opart = static_cast<const float*>(p.workspace);
   const float2* ml =
       reinterpret_cast<const float2*>(opart + int64_t(p.header[enigma_serving::kSlots]) * 128 * D);
-  const int state = r / 128, row = r % 128;
-  const int tok = g.tok0 + state * g.tokens + row / G;
-  if (row >= g.tokens * G || tok >= g.tok_end || tok >= p.tokens_q) return;
-  griddep_wait();                                               // the parts are written
-  const int n = g.parts, step = 2 * 128;
-  const int64_t at = int64_t(g.slot + state) * 128 + row;
-  enigma_serving::RowJoin<V> join;
-  join.best(ml + at, step, n, lane);
-  join.seal();
-  join.add(ml + at, step, opart + at * D, int64_t(step) * D, n, D, lane);
-  const int h = g.kvh * G + row % G;
-  const float inv = join.l == 0.f ? 0.f : 1.f / join.l;
-  T* out = static_cast<T*>(p.out) + tok * p.o_token + h * p.o_head;
+  const int state = r0 / 128;
+  const int row0 = r0 % 128, mine = row0 + (lane >> 3);            // this lane's row of (m, l)
+  const int tok = g.tok0 + state * g.tokens + mine / G;
+  const bool live = mine < g.tokens * G && tok < g.tok_end && tok < p.tokens_q;
+  if (!__any_sync(0xffffffffu, live)) return;
+  const int n = g.parts;
+  const int64_t step = 2 * 128, at = int64_t(g.slot + state) * 128;
+  griddep_wait();                                                  // the parts are written
+  float M = -INFINITY, l = 0.f;
+  float acc[R][V];
 #pragma unroll
-  for (int v = 0; v < V; ++v)
-    if (lane + 32 * v < D) store(out + lane + 32 * v, join.acc[v] * inv);
-  if (p.lse != nullptr && lane == 0)
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[r][v] = 0.f;
+  if (live)
+    for (int i = lane & 7; i < n; i += 8) M = fmaxf(M, ml[at + mine + i * step].x);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  for (int i0 = 0; i0 < n; i0 += 8) {
+    const int i = i0 + (lane & 7);
+    const float2 x = live && i < n ? ml[at + mine + i * step] : make_float2(-INFINITY, 0.f);
+    const float w = x.x == -INFINITY ? 0.f : exp2f(x.x - M);       // this part saw no key: 0
+    if (w != 0.f) l = fmaf(x.y, w, l);
+    const int here = min(8, n - i0);
+    for (int y = 0; y < here; ++y) {
+      float f[R], o[R][V];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        f[r] = __shfl_sync(0xffffffffu, w, r * 8 + y);
+        const float* from = opart + (at + row0 + r + (i0 + y) * step) * D;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          o[r][v] = 0.f;
+          if (f[r] != 0.f && lane + 32 * v < D) o[r][v] = from[lane + 32 * v];
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[r][v] = fmaf(o[r][v], f[r], acc[r][v]);
+    }
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  const int h = g.kvh * G + mine % G;
+  if (p.lse != nullptr && live && (lane & 7) == 0)
     p.lse[int64_t(tok) * p.heads_q + h] =
-        join.l == 0.f ? -INFINITY : (join.M + log2f(join.l)) * 0.6931471805599453f;
+        l == 0.f ? -INFINITY : (M + log2f(l)) * 0.6931471805599453f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t to = int64_t(tok) * p.o_token + int64_t(h) * p.o_head;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float s = __shfl_sync(0xffffffffu, inv, r * 8);
+    const int64_t row = __shfl_sync(0xffffffffu, to, r * 8);
+    if (__shfl_sync(0xffffffffu, live ? 1 : 0, r * 8) == 0) continue;
+    T* out = static_cast<T*>(p.out) + row;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (lane + 32 * v < D) store(out + lane + 32 * v, acc[r][v] * s);
+  }
 }
 
 template <typename T>
@@ -430,7 +475,7 @@ cudaError_t sdpa_packed_simt_launch(const enigma_sdpa_packed_desc& d, cudaStream
 cudaError_t sdpa_packed_join_launch(const enigma_sdpa_packed_desc& d, cudaStream_t s) {
   const int groups = d.header[enigma_serving::kGroups];
   if (groups == 0) return cudaSuccess;
-  const dim3 grid(unsigned(groups), 2 * ENIGMA_PACKED_TILE_ROWS / 8);
+  const dim3 grid(unsigned(groups), 2 * ENIGMA_PACKED_TILE_ROWS / 32);
   return d.dtype == ENIGMA_DTYPE_F32 ? launch_join<float>(d, grid, s)
                                      : launch_join<__nv_bfloat16>(d, grid, s);
 }
