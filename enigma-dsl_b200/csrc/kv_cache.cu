@@ -6,13 +6,16 @@
 // shared: a fork copies the partly filled last page, so a slot may append without looking
 // whether somebody else reads the page.
 //
-// Every change of the map is one launch of one 8-CTA cluster (cache_map_kernel): the phases
-// "check the request", "change refs", "count and list the free pages", "write rows" need each
-// other's results, and a cluster barrier (well under a microsecond) is the cheapest way to
-// order them; the map itself is small (a few hundred KB).  New pages are the lowest free
-// ones, in the order of the request, so the result does not depend on timing.  A request that
-// is malformed or does not fit changes nothing but the status word.
+// Every change of the map is one launch of one 8-CTA cluster (cache_map_kernel): "check the
+// request", "change refs" and "write rows" need each other's results, and a cluster barrier (well
+// under a microsecond) is the cheapest way to order them.  It is bound by the latency of its
+// dependent loads (request -> lengths | table rows | refs | free list), so each is made once, the
+// request is kept in shared memory, and every CTA lists the free pages for itself instead of
+// waiting for the others' counts.  New pages are the lowest free ones, in the order of the
+// request, so the result does not depend on timing.  A request that is malformed or does not fit
+// changes nothing but the status word.
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 
@@ -23,19 +26,19 @@ using namespace enigma_sm100;
 constexpr int MAP_CTAS = 8;
 constexpr int MAP_THREADS = 1024;
 constexpr int WS_HEAD = 64;            // ints before the lists: [0] = number of page copies
+constexpr int MAX_REQUEST = ENIGMA_CACHE_MAX_REQUEST;
 
 enum Mode { kFork, kFree, kReserve };
 
 struct Map {
   int32_t *table, *lens, *refs, *status;
-  int32_t* ws;                         // WS_HEAD + 5 lists of `cap` ints
+  int32_t* ws;                         // WS_HEAD + 4 lists of `cap` ints
   int64_t cap;                         // max(slots, pages)
   int slots, pages, width, page;
   __host__ __device__ int32_t* src() const { return ws + WS_HEAD; }
   __host__ __device__ int32_t* dst() const { return src() + cap; }
   __host__ __device__ int32_t* fill() const { return dst() + cap; }
-  __host__ __device__ int32_t* start() const { return fill() + cap; }
-  __host__ __device__ int32_t* freed() const { return start() + cap; }
+  __host__ __device__ int32_t* freed() const { return fill() + cap; }
 };
 
 // Exclusive prefix sum of v over the block (MAP_THREADS threads); *total gets the sum.
@@ -81,56 +84,51 @@ __device__ __forceinline__ int pages_of(int len, int page) {
 template <int MODE>
 __global__ void __cluster_dims__(MAP_CTAS, 1, 1) __launch_bounds__(MAP_THREADS, 1)
 cache_map_kernel(const Map m, const int32_t* __restrict__ a, const int32_t* __restrict__ b, int n) {
-  extern __shared__ uint32_t s_bits[];           // one bit per slot: a child / a named slot
+  extern __shared__ int s_req[];                 // [n] each: slot, parent or target, tokens, start
+  int *s_slot = s_req, *s_other = s_req + n, *s_len = s_req + 2 * n, *s_start = s_req + 3 * n;
+  uint32_t* s_bits = reinterpret_cast<uint32_t*>(s_req + 4 * n);    // one bit per slot: named
   __shared__ int s_warp[32];
-  __shared__ int s_all[MAP_CTAS];
+  __shared__ unsigned long long s_need;          // pages asked for: may be more than an int holds
   const uint32_t rank = cluster_ctarank();
-  const int tid = threadIdx.x, gtid = int(rank) * MAP_THREADS + tid;
-  constexpr int GT = MAP_CTAS * MAP_THREADS;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = int(rank) * (MAP_THREADS / 32) + (tid >> 5);     // of the cluster
+  constexpr int WARPS = MAP_CTAS * MAP_THREADS / 32;
   griddep_launch_dependents();
+  for (int i = tid; i < (m.slots + 31) / 32; i += MAP_THREADS) s_bits[i] = 0;
+  if (tid == 0) s_need = 0;
   griddep_wait();
 
   // Check the request; every CTA does it for itself and comes to the same answer, since
-  // nothing is written before the barrier that follows.
-  for (int i = tid; i < (m.slots + 31) / 32; i += MAP_THREADS) s_bits[i] = 0;
-  __syncthreads();
+  // nothing is written before the barrier that follows.  s_len: tokens of the parent (fork), of
+  // the slot (free, reserve).
   bool bad = false;
-  int need_mine = 0;
   for (int i = tid; i < n; i += MAP_THREADS) {
     const int c = MODE == kFork ? b[i] : a[i];
-    if (c < 0 || c >= m.slots) {
-      bad = true;
-    } else {
-      const uint32_t bit = 1u << (c & 31);
-      bad |= (atomicOr(&s_bits[c >> 5], bit) & bit) != 0;       // named twice
-      const int held = m.lens[c];
-      bad |= held < 0 || pages_of(held, m.page) > m.width;
-      if (MODE == kReserve) {
-        const int target = b[i];
-        bad |= target < held || int64_t(target) > int64_t(m.width) * m.page;
-        if (!bad) need_mine += pages_of(target, m.page) - pages_of(held, m.page);
-      }
-    }
+    const int other = MODE == kFork ? a[i] : MODE == kReserve ? b[i] : 0;
+    const int from = MODE == kFork ? other : c;
+    const bool in = c >= 0 && c < m.slots && from >= 0 && from < m.slots;
+    const int len = in ? m.lens[from] : 0;
+    bad |= !in || len < 0 || int64_t(len) > int64_t(m.width) * m.page;
+    if (MODE == kReserve) bad |= other < len || int64_t(other) > int64_t(m.width) * m.page;
+    s_slot[i] = c;
+    s_other[i] = other;
+    s_len[i] = len;
   }
   __syncthreads();
+  for (int i = tid; i < n; i += MAP_THREADS) {
+    const int c = s_slot[i];
+    const uint32_t bit = 1u << (c & 31);
+    if (c >= 0 && c < m.slots) bad |= (atomicOr(&s_bits[c >> 5], bit) & bit) != 0;   // named twice
+  }
   if (MODE == kFork) {
+    __syncthreads();
     for (int i = tid; i < n; i += MAP_THREADS) {
-      const int p = a[i];
-      if (p < 0 || p >= m.slots || (s_bits[p >> 5] >> (p & 31) & 1u)) {
-        bad = true;                                             // a parent among the children
-      } else {
-        const int len = m.lens[p];
-        bad |= len < 0 || int64_t(len) > int64_t(m.width) * m.page;
-        if (!bad && len % m.page) {
-          const int e = m.table[int64_t(p) * m.width + len / m.page];
-          bad |= e < 0 || e >= m.pages;
-          need_mine += 1;
-        }
-      }
+      const int p = s_other[i];
+      bad |= p >= 0 && p < m.slots && (s_bits[p >> 5] >> (p & 31) & 1u);   // a parent among them
     }
   }
   if (__syncthreads_or(bad)) {
-    if (gtid == 0) {
+    if (rank == 0 && tid == 0) {
       atomicOr(m.status, ENIGMA_CACHE_BAD_REQUEST);
       m.ws[0] = 0;
     }
@@ -138,117 +136,93 @@ cache_map_kernel(const Map m, const int32_t* __restrict__ a, const int32_t* __re
   }
   cluster_sync();
 
-  // References: children (or freed slots) let go of their pages, parents' full pages gain one.
-  const int64_t cells = int64_t(n) * m.width;
-  if (MODE != kReserve) {
-    for (int64_t x = gtid; x < cells; x += GT) {
-      const int i = int(x / m.width), col = int(x % m.width);
-      const int c = MODE == kFork ? b[i] : a[i];
-      int32_t* row = m.table + int64_t(c) * m.width;
-      const int e = row[col];
-      if (e >= 0 && e < m.pages) atomicSub(&m.refs[e], 1);
-      if (MODE == kFree) {
-        row[col] = -1;
-        if (col == 0) m.lens[c] = 0;
-      } else if (col < m.lens[a[i]] / m.page) {
-        const int f = m.table[int64_t(a[i]) * m.width + col];
-        if (f >= 0 && f < m.pages) atomicAdd(&m.refs[f], 1);
+  // References: children (or freed slots) let go of their pages, parents' full pages gain one.  A
+  // warp per entry, its lanes along the row.
+  auto change_refs = [&](int by) {
+    for (int i = warp; i < n; i += WARPS) {
+      int32_t* row = m.table + int64_t(s_slot[i]) * m.width;
+      const int32_t* from = m.table + int64_t(s_other[i]) * m.width;
+      const int full = MODE == kFork ? s_len[i] / m.page : 0;
+      for (int col = lane; col < m.width; col += 32) {
+        const int e = row[col];
+        const int f = col < full ? from[col] : -1;
+        if (e >= 0 && e < m.pages) atomicAdd(&m.refs[e], -by);
+        if (f >= 0 && f < m.pages) atomicAdd(&m.refs[f], by);
+        if (MODE == kFree) row[col] = -1;
       }
+      if (MODE == kFree && lane == 0) m.lens[s_slot[i]] = 0;
     }
-  }
+  };
+  if (MODE != kReserve) change_refs(1);
   if (MODE == kFree) return;
-  cluster_sync();
 
-  // Free pages of this CTA's range; refs were changed by atomics, so they are read from L2.
+  // Pages each entry needs, and where its first one is in the list.
   int need = 0;
-  block_scan(need_mine, s_warp, &need);
-  const int per = (m.pages + MAP_CTAS - 1) / MAP_CTAS;
-  const int p0 = min(int(rank) * per, m.pages), p1 = min(p0 + per, m.pages);
-  int mine = 0;
-  for (int p = p0 + tid; p < p1; p += MAP_THREADS) mine += __ldcg(&m.refs[p]) == 0;
-  int counted = 0;
-  block_scan(mine, s_warp, &counted);
-  publish(s_all, rank, counted);
-  cluster_sync();
-  int before = 0, total = 0;
-#pragma unroll
-  for (int r = 0; r < MAP_CTAS; ++r) {
-    if (r < int(rank)) before += s_all[r];
-    total += s_all[r];
+  for (int i0 = 0; i0 < n; i0 += MAP_THREADS) {
+    const int i = i0 + tid;
+    int w = 0, got = 0;
+    if (i < n)
+      w = MODE == kFork ? (s_len[i] % m.page ? 1 : 0)
+                        : pages_of(s_other[i], m.page) - pages_of(s_len[i], m.page);
+    if (w > 0) atomicAdd(&s_need, static_cast<unsigned long long>(w));
+    const int at = need + block_scan(w, s_warp, &got);
+    if (i < n) s_start[i] = at;
+    need += got;                                 // (wraps only where s_need says "does not fit")
   }
-  if (need > total) {                                           // does not fit: as it was
-    if (MODE == kFork) {
-      for (int64_t x = gtid; x < cells; x += GT) {
-        const int i = int(x / m.width), col = int(x % m.width);
-        const int e = m.table[int64_t(b[i]) * m.width + col];
-        if (e >= 0 && e < m.pages) atomicAdd(&m.refs[e], 1);
-        if (col < m.lens[a[i]] / m.page) {
-          const int f = m.table[int64_t(a[i]) * m.width + col];
-          if (f >= 0 && f < m.pages) atomicSub(&m.refs[f], 1);
-        }
-      }
-    }
-    if (gtid == 0) {
+  if (MODE == kFork) cluster_sync();             // every change of refs is made (reserve: none was)
+
+  // The `need` lowest free pages.  A thread looks at a run of pages; refs were changed by
+  // atomics, so they are read from L2.  Every CTA writes the same list.
+  const int per = (m.pages + MAP_THREADS - 1) / MAP_THREADS;
+  const int p0 = min(tid * per, m.pages), p1 = min(p0 + per, m.pages);
+  int mine = 0, total = 0;
+  for (int p = p0; p < p1; ++p) mine += __ldcg(&m.refs[p]) == 0;
+  int at = block_scan(mine, s_warp, &total);
+  if (s_need > static_cast<unsigned long long>(total)) {   // does not fit: as it was
+    cluster_sync();                              // everyone has counted
+    if (MODE == kFork) change_refs(-1);
+    if (rank == 0 && tid == 0) {
       atomicOr(m.status, ENIGMA_CACHE_FULL);
       m.ws[0] = 0;
     }
     return;
   }
-  // The `need` lowest free pages, in order; the first of each request's pages (CTA 0).
-  for (int p = p0; p < p1 && before < need; p += MAP_THREADS) {
-    const bool is_free = p + tid < p1 && __ldcg(&m.refs[p + tid]) == 0;
-    int got = 0;
-    const int r = before + block_scan(is_free ? 1 : 0, s_warp, &got);
-    if (is_free && r < need) m.freed()[r] = p + tid;
-    before += got;
-  }
-  if (rank == 0) {
-    int run = 0;
-    for (int i0 = 0; i0 < n; i0 += MAP_THREADS) {
-      const int i = i0 + tid;
-      int w = 0, got = 0;
-      if (i < n) {
-        if (MODE == kFork) w = m.lens[a[i]] % m.page ? 1 : 0;
-        else w = pages_of(b[i], m.page) - pages_of(m.lens[a[i]], m.page);
-      }
-      const int s = run + block_scan(w, s_warp, &got);
-      if (i < n) m.start()[i] = s;
-      run += got;
-    }
-    if (tid == 0) m.ws[0] = MODE == kFork ? need : 0;
-  }
-  cluster_sync();
+  for (int p = p0; p < p1 && at < need && mine > 0; ++p)
+    if (__ldcg(&m.refs[p]) == 0) m.freed()[at++] = p;
+  if (rank == 0 && tid == 0) m.ws[0] = MODE == kFork ? need : 0;
+  cluster_sync();                                // refs are read, the list is written
 
-  for (int64_t x = gtid; x < cells; x += GT) {
-    const int i = int(x / m.width), col = int(x % m.width);
+  for (int i = warp; i < n; i += WARPS) {
+    int32_t* row = m.table + int64_t(s_slot[i]) * m.width;
+    const int start = s_start[i];
     if (MODE == kFork) {
-      const int len = m.lens[a[i]], full = len / m.page, part = len % m.page;
-      int e = -1;
-      if (col < full) {
-        e = m.table[int64_t(a[i]) * m.width + col];
-      } else if (col == full && part) {
-        const int at = __ldcg(&m.start()[i]);
-        e = __ldcg(&m.freed()[at]);
-        m.refs[e] = 1;
-        m.src()[at] = m.table[int64_t(a[i]) * m.width + col];
-        m.dst()[at] = e;
-        m.fill()[at] = part;
+      const int32_t* from = m.table + int64_t(s_other[i]) * m.width;
+      const int len = s_len[i], full = len / m.page, part = len % m.page;
+      for (int col = lane; col < m.width; col += 32) {
+        int e = col <= full ? from[col] : -1;
+        if (col == full) {
+          if (part) {
+            m.src()[start] = e;
+            e = __ldcg(&m.freed()[start]);
+            m.dst()[start] = e;
+            m.fill()[start] = part;
+            m.refs[e] = 1;
+          } else {
+            e = -1;
+          }
+        }
+        row[col] = e;
       }
-      m.table[int64_t(b[i]) * m.width + col] = e;
-      if (col == 0) m.lens[b[i]] = len;
+      if (lane == 0) m.lens[s_slot[i]] = len;
     } else {
-      // lens[a[i]] changes below only after the last barrier, by the one thread that owns i.
-      const int held = pages_of(m.lens[a[i]], m.page), want = pages_of(b[i], m.page);
-      if (col >= held && col < want) {
-        const int e = __ldcg(&m.freed()[__ldcg(&m.start()[i]) + col - held]);
+      const int held = pages_of(s_len[i], m.page), want = pages_of(s_other[i], m.page);
+      for (int col = held + lane; col < want; col += 32) {
+        const int e = __ldcg(&m.freed()[start + col - held]);
         m.refs[e] = 1;
-        m.table[int64_t(a[i]) * m.width + col] = e;
+        row[col] = e;
       }
+      if (lane == 0) m.lens[s_slot[i]] = s_other[i];
     }
-  }
-  if (MODE == kReserve) {
-    cluster_sync();
-    for (int i = gtid; i < n; i += GT) m.lens[a[i]] = b[i];
   }
 }
 
@@ -356,7 +330,17 @@ __global__ void __launch_bounds__(256) cache_copy_kernel(const Copy c) {
     const V* from = reinterpret_cast<const V*>(at + s * page_bytes);
     V* to = reinterpret_cast<V*>(at + d * page_bytes);
     const int vecs = int(int64_t(rows) * c.row_bytes / int64_t(sizeof(V)));
-    for (int x = threadIdx.x; x < vecs; x += 256) to[x] = from[x];
+    // Four loads in flight before their stores (the two may not overlap, which the compiler
+    // cannot know).
+    for (int x = threadIdx.x; x < vecs; x += 4 * 256) {
+      V v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (x + u * 256 < vecs) v[u] = from[x + u * 256];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (x + u * 256 < vecs) to[x + u * 256] = v[u];
+    }
   }
 }
 
@@ -371,20 +355,32 @@ struct Write {
   int n, tokens, heads, slots_total, pages, width, page, row_bytes;
 };
 
-// One warp per token: its sequence by bisection of cu, then heads x row bytes of K and V.
+// One warp per token, its lanes along the rows of K, then V.  The row's first loads are made before
+// its place is known: sequence (cu is searched 32 ways at once), table, page, store.
 template <typename V>
 __global__ void __launch_bounds__(256) cache_write_kernel(const Write w) {
   const int lane = threadIdx.x & 31;
   const int warps = int(gridDim.x) * 8;
-  const int per = w.row_bytes / int(sizeof(V));
+  const int per = w.row_bytes / int(sizeof(V)), row = w.heads * per;     // vectors: head, token
   griddep_launch_dependents();
   griddep_wait();
   for (int t = int(blockIdx.x) * 8 + (threadIdx.x >> 5); t < w.tokens; t += warps) {
-    int lo = 0, hi = w.n;              // the last i with cu[i] <= t
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (w.cu[mid] <= t) lo = mid;
-      else hi = mid;
+    auto source = [&](int x) {
+      const bool is_v = x >= row;
+      const int y = is_v ? x - row : x, h = y / per, e = y - h * per;
+      return reinterpret_cast<const V*>(is_v ? w.new_v + t * w.v_token + h * w.v_head
+                                             : w.new_k + t * w.k_token + h * w.k_head) + e;
+    };
+    V first = V();
+    if (lane < 2 * row) first = *source(lane);
+    // The last i in [0, n) with cu[i] <= t, in [lo, lo + span).
+    int lo = 0, span = w.n;
+    while (span > 1) {
+      const int step = (span + 31) / 32, i = lo + (lane + 1) * step;
+      const bool past = i >= lo + span || w.cu[i] > t;
+      const int k = __ffs(__ballot_sync(0xffffffffu, past)) - 1;         // lane 31 is always past
+      span = min(step, lo + span - (lo + k * step));
+      lo += k * step;
     }
     const int slot = w.slots[lo];
     const int64_t pos = int64_t(w.starts[lo]) + t - w.cu[lo];
@@ -396,14 +392,12 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const Write w) {
       if (lane == 0) atomicOr(w.status, ENIGMA_CACHE_BAD_REQUEST);
       continue;
     }
-    const int64_t row = at * w.head_bytes * w.heads + (pos % w.page) * w.row_bytes;
-    for (int x = lane; x < w.heads * per; x += 32) {
-      const int h = x / per, e = x - h * per;
-      const int64_t to = row + h * w.head_bytes;
-      reinterpret_cast<V*>(w.k + to)[e] =
-          reinterpret_cast<const V*>(w.new_k + t * w.k_token + h * w.k_head)[e];
-      reinterpret_cast<V*>(w.v + to)[e] =
-          reinterpret_cast<const V*>(w.new_v + t * w.v_token + h * w.v_head)[e];
+    const int64_t to = at * w.head_bytes * w.heads + (pos % w.page) * w.row_bytes;
+    for (int x = lane; x < 2 * row; x += 32) {
+      const bool is_v = x >= row;
+      const int y = is_v ? x - row : x, h = y / per, e = y - h * per;
+      const V v = x == lane ? first : *source(x);
+      reinterpret_cast<V*>((is_v ? w.v : w.k) + to + h * w.head_bytes)[e] = v;
     }
   }
 }
@@ -454,8 +448,17 @@ cudaError_t launch_copy(const enigma_kv_cache_desc& d, const int32_t* src, const
 template <int MODE>
 cudaError_t launch_map(const enigma_kv_cache_desc& d, const int32_t* a, const int32_t* b, int64_t n,
                        cudaStream_t s) {
-  const size_t bits = size_t((d.slots + 31) / 32) * 4;
-  return enigma::launch_dependent(cache_map_kernel<MODE>, MAP_CTAS, MAP_THREADS, bits, s, make_map(d),
+  const size_t smem = size_t(n) * 16 + size_t((d.slots + 31) / 32) * 4;
+  static std::atomic<uint64_t> ready{0};                    // devices where the attribute is set
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && !(dev < 64 && (ready.load() >> dev & 1))) {
+    e = cudaFuncSetAttribute(cache_map_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             MAX_REQUEST * 16 + 262144 / 8);
+    if (e == cudaSuccess && dev < 64) ready.fetch_or(uint64_t(1) << dev);
+  }
+  if (e != cudaSuccess) return e;
+  return enigma::launch_dependent(cache_map_kernel<MODE>, MAP_CTAS, MAP_THREADS, smem, s, make_map(d),
                                   a, b, int(n));
 }
 
@@ -464,7 +467,7 @@ cudaError_t launch_map(const enigma_kv_cache_desc& d, const int32_t* a, const in
 namespace enigma {
 
 size_t kv_cache_workspace_bytes(const enigma_kv_cache_desc& d) {
-  return size_t(WS_HEAD + 5 * std::max(d.slots, d.pages)) * sizeof(int32_t);
+  return size_t(WS_HEAD + 4 * std::max(d.slots, d.pages)) * sizeof(int32_t);
 }
 
 cudaError_t kv_cache_fork(const enigma_kv_cache_desc& d, const int32_t* parents,

@@ -92,6 +92,7 @@ int32_t check_request(const enigma_kv_cache_desc* d, const void* a, const void* 
   const int32_t e = check_cache(d, true);
   if (e != ENIGMA_OK) return e;
   if (n < 0 || n > d->slots) return bad("kv_cache: a request names each slot at most once");
+  if (n > ENIGMA_CACHE_MAX_REQUEST) return bad("kv_cache: a request has at most 8192 entries");
   if (n > 0 && (a == nullptr || b == nullptr)) return bad("kv_cache: NULL request");
   return ENIGMA_OK;
 }

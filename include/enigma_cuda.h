@@ -302,6 +302,7 @@ int32_t enigma_sdpa_shared_prefix(const enigma_sdpa_shared_prefix_desc* desc, vo
  * workspace: enigma_kv_cache_workspace_bytes() bytes; calls that share it run in one order. */
 #define ENIGMA_CACHE_FULL 1
 #define ENIGMA_CACHE_BAD_REQUEST 2
+#define ENIGMA_CACHE_MAX_REQUEST 8192   /* entries of one fork, free or reserve */
 typedef struct enigma_kv_cache_desc {
   int64_t layers, pages, heads_kv, page, head_dim, elem_bytes, slots, table_width;
   void *k, *v;

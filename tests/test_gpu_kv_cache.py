@@ -204,3 +204,42 @@ def test_refusals(cuda):
         PagedKVCache(cache.k, cache.v, cache.table, cache.lens, cache.refs[:4].contiguous())
     with pytest.raises(TypeError, match="unsupported dtype"):
         PagedKVCache(cache.k.half(), cache.v.half(), cache.table, cache.lens, cache.refs)
+
+
+def test_many_pages_and_requests(cuda):
+    """More pages than threads, requests of hundreds of entries, long rows."""
+    rng = np.random.default_rng(9)
+    lens = [int(x) for x in rng.integers(0, 300, 700)]
+    cache, want = _make(cuda, rng, 1, 60000, 1, 4, 2, 2300, 80, lens, "f32")
+    parents = [int(x) for x in rng.integers(0, 700, 1400)]
+    children = [int(x) for x in 700 + rng.permutation(1600)[:1400]]
+    cache.fork(parents, children)
+    want.fork(parents, children)
+    cache.check()
+    _same(cache, want)
+    slots = [int(x) for x in rng.permutation(2300)[:1100]]
+    grown = [int(min(320, want.lens[s] + x)) for s, x in zip(slots, rng.integers(0, 90, 1100))]
+    cache.reserve(slots, grown)
+    want.reserve(slots, grown)
+    cache.free(slots[::2])
+    want.free(slots[::2])
+    cache.compact()
+    want.compact()
+    cache.check()
+    _same(cache, want)
+
+
+def test_more_pages_asked_for_than_an_int_holds(cuda):
+    """The sum of what a request needs does not wrap into something that fits."""
+    import torch
+    from enigma import EnigmaError
+    from enigma.kv_cache import PagedKVCache
+    n, width = 4096, 1 << 20
+    k = torch.zeros(1, 8, 1, 1, 2, device=cuda)
+    cache = PagedKVCache(k, k.clone(), torch.full((n, width), -1, dtype=torch.int32, device=cuda),
+                         torch.zeros(n, dtype=torch.int32, device=cuda),
+                         torch.zeros(8, dtype=torch.int32, device=cuda))
+    cache.reserve(list(range(n)), [width] * n)              # 2^32 pages
+    with pytest.raises(EnigmaError, match="free pages"):
+        cache.check()
+    assert int(cache.refs.sum()) == 0 and int(cache.lens.sum()) == 0
