@@ -121,7 +121,7 @@ __device__ __forceinline__ void rows_landed() {
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(TT, TileCfg<DP>::CTAS)
-packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec) {
+packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec, const int row_blocks) {
   using C = TileCfg<DP>;
   constexpr int TK = C::TK, LD = C::LD, KPT = C::KPT;
   extern __shared__ float4 smem4[];
@@ -132,7 +132,7 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec) {
   float* s_p = s_v + TK * DP;                             // [TK][TR]
   const int tid = threadIdx.x;
   const PackedItem it = reinterpret_cast<const PackedItem*>(
-      p.plan + p.header[enigma_serving::kItemsAt])[blockIdx.x];
+      p.plan + p.header[enigma_serving::kItemsAt])[blockIdx.x / row_blocks];
   const int G = int(p.heads_q / p.heads_kv), D = int(p.head_dim), kvh = it.kvh;
   // An item that does not lie inside the tensors is no work of theirs.
   if (it.q0 < 0 || it.q0 + int64_t(it.lq) > p.tokens_q || it.k0 < 0 ||
@@ -140,7 +140,8 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec) {
       it.slot >= p.header[enigma_serving::kSlots])
     return;
   const int n = min(2 * it.tokens, it.lq - it.t0) * G;    // rows of the item
-  const int r0 = blockIdx.y * TR;
+  // An item's row blocks side by side: the heaviest items start first.
+  const int r0 = int(blockIdx.x % row_blocks) * TR;
   if (r0 >= n) return;
   const int off = p.causal ? it.lk - it.lq + 1 : it.lk;   // a token's keys: min(lk, token + off)
   const int t_last = it.t0 + (min(r0 + TR, n) - 1) / G;
@@ -210,10 +211,11 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec) {
       for (int r = 0; r < 8; ++r) {
         const float4 q = *reinterpret_cast<const float4*>(s_q + (rg * 8 + r) * LD + d);
 #pragma unroll
-        for (int c = 0; c < KPT; ++c) {
+        for (int c = 0; c < KPT; ++c)
           s2[r][c] = fma2(make_float2(q.x, q.y), make_float2(k[c].x, k[c].y), s2[r][c]);
+#pragma unroll
+        for (int c = 0; c < KPT; ++c)
           s2[r][c] = fma2(make_float2(q.z, q.w), make_float2(k[c].z, k[c].w), s2[r][c]);
-        }
       }
     }
     __syncthreads();                         // K is read
@@ -408,8 +410,10 @@ cudaError_t launch_packed(const enigma_sdpa_packed_desc& d, cudaStream_t s) {
     vec &= x % 4 == 0;
   const int64_t group = d.heads_q / d.heads_kv;
   const int64_t rows = 2 * std::max<int64_t>(1, ENIGMA_PACKED_TILE_ROWS / group) * group;
-  const dim3 grid(unsigned(d.header[enigma_serving::kItems]), unsigned((rows + TR - 1) / TR));
-  packed_simt_kernel<T, DP><<<grid, TT, C::SMEM, s>>>(d, vec);
+  const int row_blocks = int((rows + TR - 1) / TR);
+  const int64_t grid = int64_t(d.header[enigma_serving::kItems]) * row_blocks;
+  if (grid > (int64_t(1) << 31) - 1) return cudaErrorInvalidConfiguration;
+  packed_simt_kernel<T, DP><<<unsigned(grid), TT, C::SMEM, s>>>(d, vec, row_blocks);
   return cudaGetLastError();
 }
 

@@ -306,9 +306,13 @@ struct Copy {
   int n, layers, heads, pages, page, row_bytes;   // row_bytes: head_dim * element size
 };
 
-// Units of one (copy, layer, K or V, head): fill * row_bytes contiguous bytes.
+// Units of one (copy, layer, K or V, head): fill * row_bytes contiguous bytes.  Bound by HBM; small
+// blocks and many of them, so that the hardware keeps all SMs' requests going: 128 threads, up
+// to 256 blocks per SM 6.4 TB/s (1 GB moved, read and written; 8 blocks of 256 threads per SM:
+// 5.8), while as many blocks as there could be copies costs their start (131072: 5.4).
+constexpr int COPY_THREADS = 128;
 template <typename V>
-__global__ void __launch_bounds__(256) cache_copy_kernel(const Copy c) {
+__global__ void __launch_bounds__(COPY_THREADS) cache_copy_kernel(const Copy c) {
   griddep_launch_dependents();
   griddep_wait();
   const int n = c.count != nullptr ? *c.count : c.n;
@@ -332,14 +336,14 @@ __global__ void __launch_bounds__(256) cache_copy_kernel(const Copy c) {
     const int vecs = int(int64_t(rows) * c.row_bytes / int64_t(sizeof(V)));
     // Four loads in flight before their stores (the two may not overlap, which the compiler
     // cannot know).
-    for (int x = threadIdx.x; x < vecs; x += 4 * 256) {
+    for (int x = threadIdx.x; x < vecs; x += 4 * COPY_THREADS) {
       V v[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (x + u * 256 < vecs) v[u] = from[x + u * 256];
+        if (x + u * COPY_THREADS < vecs) v[u] = from[x + u * COPY_THREADS];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (x + u * 256 < vecs) to[x + u * 256] = v[u];
+        if (x + u * COPY_THREADS < vecs) to[x + u * COPY_THREADS] = v[u];
     }
   }
 }
@@ -438,11 +442,11 @@ cudaError_t launch_copy(const enigma_kv_cache_desc& d, const int32_t* src, const
   c.pages = int(d.pages);
   c.page = int(d.page);
   const int64_t units = n * d.layers * 2 * d.heads_kv;
-  const unsigned grid = unsigned(std::min<int64_t>(units, int64_t(enigma::sm_count()) * 8));
+  const unsigned grid = unsigned(std::min<int64_t>(units, int64_t(enigma::sm_count()) * 256));
   if (grid == 0) return cudaSuccess;
   if (c.row_bytes % 16 == 0 && a16(d.k) && a16(d.v))
-    return enigma::launch_dependent(cache_copy_kernel<uint4>, grid, 256, 0, s, c);
-  return enigma::launch_dependent(cache_copy_kernel<uint16_t>, grid, 256, 0, s, c);
+    return enigma::launch_dependent(cache_copy_kernel<uint4>, grid, COPY_THREADS, 0, s, c);
+  return enigma::launch_dependent(cache_copy_kernel<uint16_t>, grid, COPY_THREADS, 0, s, c);
 }
 
 template <int MODE>

@@ -174,6 +174,20 @@ def test_packed_long(cuda):
             assert ((out[i, h].double() - ref).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("dtype,d", [("bf16", 64), ("f32", 8)])
+def test_packed_many_sequences(cuda, dtype, d):
+    """More items than a grid's second axis holds; each of one token, whose result is its value."""
+    import torch
+    from enigma import cuda_ops
+    n = 9000
+    g = torch.Generator(device=cuda).manual_seed(3)
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float32
+    q, k, v = (torch.randn(n, h, d, device=cuda, generator=g).to(dt) for h in (16, 8, 8))
+    plan = cuda_ops.PackedPlan([1] * n, heads_q=16, heads_kv=8)
+    out = cuda_ops.sdpa_packed(q, k, v, plan)
+    assert torch.equal(out, v.repeat_interleave(2, 1))
+
+
 def test_packed_empty(cuda):
     import torch
     from enigma import cuda_ops
