@@ -160,48 +160,58 @@ class PackedPlan:
         self.tokens_q, self.tokens_k = sum(lens_q), sum(lens_k)
         self.header = tuple(ints[:_native.PACKED_PLAN_HEADER].tolist())
         self.ints = ints.to(device)
-        self._workspace = {}
+        self.heads = {}          # checked calls' sizes, strides and types
 
     def workspace_bytes(self, head_dim: int) -> int:
         """Device memory that a call with this plan needs (0 unless it splits rows)."""
-        if head_dim not in self._workspace:
-            need = ctypes.c_size_t()
-            _native.call("enigma_sdpa_packed_workspace_bytes",
-                         (ctypes.c_int32 * len(self.header))(*self.header), head_dim,
-                         ctypes.byref(need))
-            self._workspace[head_dim] = need.value
-        return self._workspace[head_dim]
+        need = ctypes.c_size_t()
+        _native.call("enigma_sdpa_packed_workspace_bytes",
+                     (ctypes.c_int32 * len(self.header))(*self.header), head_dim,
+                     ctypes.byref(need))
+        return need.value
 
 
+# The serving operators are called for every layer and token, on calls of a few microseconds: what
+# depends on sizes, strides and types alone is checked and packed once per combination.
+#
 # enigma_sdpa_packed_desc (include/enigma_cuda.h): sizes and strides, scale and flags, the plan's
-# header, pointers.  Packed bytes cost a third of filling a ctypes structure.
-_PACKED_DESC = struct.Struct(f"13qf3i{_native.PACKED_PLAN_HEADER}i8Q")
+# header; then pointers.
+_PACKED_HEAD = struct.Struct(f"13qf3i{_native.PACKED_PLAN_HEADER}i")
+_PACKED_PTRS = struct.Struct("8Q")
+# enigma_sdpa_shared_prefix_desc: sizes and strides, scale and dtype; then pointers.
+_SHARED_HEAD = struct.Struct("15qfi")
+_SHARED_PTRS = struct.Struct("9Q")
 
 
-_CUDA = "cuda"
+def _raw_stream(index: int) -> int:
+    """The current stream of device `index`, without the Stream object that _stream_ptr makes."""
+    return _torch()._C._cuda_getCurrentRawStream(index)
 
 
-def _raw_stream(t) -> int:
-    """The current stream of t's device, without the Stream object that _stream_ptr makes."""
-    return _torch()._C._cuda_getCurrentRawStream(t.device.index)
-
-
-def _check_rows(name, *ts):
-    """CUDA tensors of one device and dtype whose last axis is contiguous; the dtype's code."""
-    first = ts[0]
-    device, dtype = first.device, first.dtype
-    if device.type != _CUDA:
+def _same_device(name, first, *others) -> int:
+    """Index of the CUDA device that all tensors are on."""
+    index = first.get_device()
+    if index < 0:
         raise ValueError("enigma CUDA operators take CUDA tensors (no CPU fallback)")
-    for t in ts:
-        if t.device != device:
-            raise ValueError("enigma CUDA operators take CUDA tensors of one device")
-        if t.dtype != dtype:
+    for t in others:
+        if t.get_device() != index:
+            raise ValueError(f"{name}: all tensors must be on the same device")
+    if index not in _initialised:
+        ensure_device(index)
+    return index
+
+
+def _check_rows(name, dtype, *tensors):
+    """(shape, stride, dtype) of tensors: one dtype, a contiguous last axis.  The dtype's code."""
+    torch = _torch()
+    for shape, stride, other in tensors:
+        if other != dtype:
             raise TypeError(f"{name}: tensors must share a dtype")
-        if t.stride(-1) != 1 and t.shape[-1] > 1:
+        if stride[-1] != 1 and shape[-1] > 1:
             raise ValueError(f"{name}: the last axis must be contiguous")
-    if device.index not in _initialised:
-        ensure_device(device.index)
-    return _dtype_code(first)
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"unsupported dtype {dtype}: expected float32 or bfloat16")
+    return _native.DTYPE_F32 if dtype == torch.float32 else _native.DTYPE_BF16
 
 
 def _scratch(name, workspace, need, like):
@@ -211,9 +221,32 @@ def _scratch(name, workspace, need, like):
             return 0, 0, None
         workspace = like.new_empty(need, dtype=_torch().uint8)
         return workspace.data_ptr(), need, workspace
-    if workspace.device != like.device or not workspace.is_contiguous():
+    if workspace.get_device() != like.get_device() or not workspace.is_contiguous():
         raise ValueError(f"{name}: workspace must be contiguous on the data's device")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
+
+
+def _packed_head(plan, q, k, v, out, scale):
+    """Checks the (shape, stride, dtype) of a call with this plan and packs the desc's head."""
+    if len(q[0]) != 3 or len(k[0]) != 3 or len(v[0]) != 3:
+        raise ValueError("sdpa_packed: expected [tokens, heads, head_dim] tensors")
+    tq, hq, d = q[0]
+    tk, hk, dk = k[0]
+    if dk != d or v[0] != k[0]:
+        raise ValueError("sdpa_packed: K/V shapes do not match Q")
+    if (hq, hk) != (plan.heads_q, plan.heads_kv):
+        raise ValueError("sdpa_packed: the plan was made for other heads")
+    if (tq, tk) != (plan.tokens_q, plan.tokens_k):
+        raise ValueError(f"sdpa_packed: the plan's lengths sum to {plan.tokens_q} / "
+                         f"{plan.tokens_k} tokens, the tensors hold {tq} / {tk}")
+    if out is None:
+        out = (q[0], (hq * d, d, 1), q[2])
+    elif out[0] != q[0]:
+        raise ValueError("sdpa_packed: out must have q's shape")
+    dtype = _check_rows("sdpa_packed", q[2], q, k, v, out)
+    return (_PACKED_HEAD.pack(tq, tk, hq, hk, d, *q[1][:2], *k[1][:2], *v[1][:2], *out[1][:2],
+                              1.0 / math.sqrt(d) if scale is None else scale, plan.causal, dtype,
+                              0, *plan.header), plan.workspace_bytes(d))
 
 
 def sdpa_packed(q, k, v, plan: PackedPlan, scale: Optional[float] = None, out=None,
@@ -227,59 +260,64 @@ def sdpa_packed(q, k, v, plan: PackedPlan, scale: Optional[float] = None, out=No
     plan.workspace_bytes(D) bytes to use instead of an allocation per call.  Returns out
     [tokens_q, Hq, D], and with return_lse the fp32 log-sum-exp [tokens_q, Hq] too.
     """
-    torch = _torch()
-    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
-        raise ValueError("sdpa_packed: expected [tokens, heads, head_dim] tensors")
-    tq, hq, d = q.shape
-    tk, hk, dk = k.shape
-    if dk != d or v.shape != k.shape:
-        raise ValueError("sdpa_packed: K/V shapes do not match Q")
-    if (hq, hk) != (plan.heads_q, plan.heads_kv):
-        raise ValueError("sdpa_packed: the plan was made for other heads")
-    if (tq, tk) != (plan.tokens_q, plan.tokens_k):
-        raise ValueError(f"sdpa_packed: the plan's lengths sum to {plan.tokens_q} / "
-                         f"{plan.tokens_k} tokens, the tensors hold {tq} / {tk}")
+    key = ((q.shape, q.stride(), q.dtype), (k.shape, k.stride(), k.dtype),
+           (v.shape, v.stride(), v.dtype),
+           None if out is None else (out.shape, out.stride(), out.dtype), scale)
+    head = plan.heads.get(key)
+    if head is None:
+        head = _packed_head(plan, *key)
+        if len(plan.heads) >= 64:
+            plan.heads.clear()
+        plan.heads[key] = head
     if out is None:
-        dtype = _check_rows("sdpa_packed", q, k, v)
-        out = q.new_empty((tq, hq, d))
-    elif out.shape != q.shape:
-        raise ValueError("sdpa_packed: out must have q's shape")
+        out = q.new_empty(q.shape)
+        index = _same_device("sdpa_packed", q, k, v, plan.ints)
     else:
-        dtype = _check_rows("sdpa_packed", q, k, v, out)
-    if plan.ints.device != q.device:
-        raise ValueError("sdpa_packed: the plan is on another device")
-    lse = q.new_empty((tq, hq), dtype=torch.float32) if return_lse else None
-    ws, ws_bytes, keep = _scratch("sdpa_packed", workspace, plan.workspace_bytes(d), q)
-    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
-    desc = _PACKED_DESC.pack(tq, tk, hq, hk, d, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0],
-                             os[1], 1.0 / math.sqrt(d) if scale is None else scale, plan.causal,
-                             dtype, 0, *plan.header, plan.ints.data_ptr(), q.data_ptr(),
-                             k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                             lse.data_ptr() if return_lse else 0, ws, ws_bytes)
-    _native.call("enigma_sdpa_packed", desc, _raw_stream(q))
+        index = _same_device("sdpa_packed", q, k, v, plan.ints, out)
+    lse = q.new_empty(q.shape[:2], dtype=_torch().float32) if return_lse else None
+    ws, ws_bytes, keep = _scratch("sdpa_packed", workspace, head[1], q)
+    desc = head[0] + _PACKED_PTRS.pack(plan.ints.data_ptr(), q.data_ptr(), k.data_ptr(),
+                                       v.data_ptr(), out.data_ptr(),
+                                       lse.data_ptr() if return_lse else 0, ws, ws_bytes)
+    status = _native.lib().enigma_sdpa_packed(desc, _raw_stream(index))
+    if status:
+        _native.check(status, "enigma_sdpa_packed")
     return (out, lse) if return_lse else out
 
 
-# enigma_sdpa_shared_prefix_desc: sizes and strides, scale and dtype, pointers, workspace.
-_SHARED_DESC = struct.Struct("15qfi9Q")
-
-
-@functools.lru_cache(maxsize=4096)
-def _shared_workspace_bytes(device_index, *sizes) -> int:
-    """enigma_sdpa_shared_prefix_workspace_bytes for the desc's sizes (it reads nothing else)."""
-    need = ctypes.c_size_t()
-    _native.call("enigma_sdpa_shared_prefix_workspace_bytes",
-                 _SHARED_DESC.pack(*sizes[:9], 0, 0, 0, 0, 0, 0, 1.0, sizes[9], *([0] * 9)),
-                 ctypes.byref(need))
-    return need.value
-
-
-def _check_int32(name, device, *ts):
+@functools.lru_cache(maxsize=1024)
+def _shared_head(index, q, k, v, table, lens, slots, out, prefix_len, scale):
+    """Checks the (shape, stride, dtype) of a call and packs the desc's head; bytes of workspace."""
     int32 = _torch().int32
-    for t in ts:
-        if t.dtype != int32 or t.device != device or not t.is_contiguous():
-            raise ValueError(f"{name}: tables, lengths and slots are contiguous int32 tensors on "
-                             f"the data's device")
+    name = "sdpa_shared_prefix"
+    if len(q[0]) != 3 or len(k[0]) != 4 or v[0] != k[0]:
+        raise ValueError(f"{name}: expected q [B, Hq, D] and pages [P, Hkv, page, D]")
+    b, hq, d = q[0]
+    pages, hk, page, dk = k[0]
+    if dk != d:
+        raise ValueError(f"{name}: K/V head_dim does not match Q")
+    if len(table[0]) != 2 or len(lens[0]) != 1 or lens[0][0] != table[0][0]:
+        raise ValueError(f"{name}: expected table [n, width] and lens [n]")
+    if slots is not None and slots[0] != (b,):
+        raise ValueError(f"{name}: slots must name one row per sequence")
+    if out is None:
+        out = (q[0], (hq * d, d, 1), q[2])
+    elif out[0] != q[0]:
+        raise ValueError(f"{name}: out must have q's shape")
+    dtype = _check_rows(name, q[2], q, k, v, out)
+    if k[1][1:] != (page * d, d, 1) or v[1][1:] != (page * d, d, 1):
+        raise ValueError(f"{name}: a page must be contiguous")
+    for shape, stride, other in (table, lens) + (() if slots is None else (slots,)):
+        dense = stride[-1] == 1 and (len(shape) == 1 or stride[0] == shape[1])
+        if other != int32 or not (dense or 0 in shape):
+            raise ValueError(f"{name}: tables, lengths and slots are contiguous int32 tensors")
+    head = _SHARED_HEAD.pack(b, hq, hk, d, page, pages, table[0][1], table[0][0], prefix_len,
+                             *q[1][:2], *out[1][:2], k[1][0], v[1][0],
+                             1.0 / math.sqrt(d) if scale is None else scale, dtype)
+    need = ctypes.c_size_t()
+    _native.call("enigma_sdpa_shared_prefix_workspace_bytes", head + _SHARED_PTRS.pack(*([0] * 9)),
+                 ctypes.byref(need))
+    return head, need.value
 
 
 def sdpa_shared_prefix(q, k_pages, v_pages, table, lens, prefix_len: int = 0, slots=None,
@@ -290,41 +328,30 @@ def sdpa_shared_prefix(q, k_pages, v_pages, table, lens, prefix_len: int = 0, sl
     [n, width] int32 page numbers, lens [n] int32; sequence b uses row slots[b] (default: row
     b).  Sequence b attends to its first lens keys; those below prefix_len are the same for
     the whole batch and are read once for all, through sequence 0's row.  A sequence without
-    keys gives zeros.  workspace: a uint8 tensor to use instead of an allocation per call
-    (as many bytes as enigma_sdpa_shared_prefix_workspace_bytes says).  Returns out [B, Hq, D].
+    keys gives zeros.  workspace: a uint8 tensor to use instead of an allocation per call (as
+    many bytes as enigma_sdpa_shared_prefix_workspace_bytes says).  Returns out [B, Hq, D].
     """
-    torch = _torch()
-    if q.dim() != 3 or k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
-        raise ValueError("sdpa_shared_prefix: expected q [B, Hq, D] and pages [P, Hkv, page, D]")
-    b, hq, d = q.shape
-    pages, hk, page, dk = k_pages.shape
-    if dk != d:
-        raise ValueError("sdpa_shared_prefix: K/V head_dim does not match Q")
-    if table.dim() != 2 or lens.dim() != 1 or lens.shape[0] != table.shape[0]:
-        raise ValueError("sdpa_shared_prefix: expected table [n, width] and lens [n]")
-    if slots is not None and tuple(slots.shape) != (b,):
-        raise ValueError("sdpa_shared_prefix: slots must name one row per sequence")
+    index = _same_device("sdpa_shared_prefix", q, k_pages, v_pages, table, lens)
+    head, need = _shared_head(
+        index, (q.shape, q.stride(), q.dtype), (k_pages.shape, k_pages.stride(), k_pages.dtype),
+        (v_pages.shape, v_pages.stride(), v_pages.dtype),
+        (table.shape, table.stride(), table.dtype), (lens.shape, lens.stride(), lens.dtype),
+        None if slots is None else (slots.shape, slots.stride(), slots.dtype),
+        None if out is None else (out.shape, out.stride(), out.dtype), prefix_len, scale)
     if out is None:
-        dtype = _check_rows("sdpa_shared_prefix", q, k_pages, v_pages)
-        out = q.new_empty((b, hq, d))
-    elif out.shape != q.shape:
-        raise ValueError("sdpa_shared_prefix: out must have q's shape")
+        out = q.new_empty(q.shape)
     else:
-        dtype = _check_rows("sdpa_shared_prefix", q, k_pages, v_pages, out)
-    ks, vs = k_pages.stride(), v_pages.stride()
-    if ks[1:] != (page * d, d, 1) or vs[1:] != (page * d, d, 1):
-        raise ValueError("sdpa_shared_prefix: a page must be contiguous")
-    _check_int32("sdpa_shared_prefix", q.device, table, lens, *(() if slots is None else (slots,)))
-    sizes = (b, hq, hk, d, page, pages, table.shape[1], table.shape[0], int(prefix_len))
-    need = _shared_workspace_bytes(q.device.index, *sizes, dtype)
+        _same_device("sdpa_shared_prefix", q, out)
     ws, ws_bytes, keep = _scratch("sdpa_shared_prefix", workspace, need, q)
-    qs, os = q.stride(), out.stride()
-    desc = _SHARED_DESC.pack(*sizes, qs[0], qs[1], os[0], os[1], ks[0], vs[0],
-                             1.0 / math.sqrt(d) if scale is None else scale, dtype,
-                             table.data_ptr(), lens.data_ptr(),
-                             0 if slots is None else slots.data_ptr(), q.data_ptr(),
-                             k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), ws, ws_bytes)
-    _native.call("enigma_sdpa_shared_prefix", desc, _raw_stream(q))
+    if slots is not None:
+        _same_device("sdpa_shared_prefix", q, slots)
+    desc = head + _SHARED_PTRS.pack(table.data_ptr(), lens.data_ptr(),
+                                    0 if slots is None else slots.data_ptr(), q.data_ptr(),
+                                    k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), ws,
+                                    ws_bytes)
+    status = _native.lib().enigma_sdpa_shared_prefix(desc, _raw_stream(index))
+    if status:
+        _native.check(status, "enigma_sdpa_shared_prefix")
     return out
 
 

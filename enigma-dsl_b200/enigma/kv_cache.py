@@ -40,7 +40,8 @@ class PagedKVCache:
             raise ValueError("PagedKVCache: k and v must be [layers, pages, heads, page, head_dim]")
         cuda_ops._dtype_code(k)
         cuda_ops._check_cuda(k, v, table, lens, refs)
-        cuda_ops._check_int32("PagedKVCache", k.device, table, lens, refs)
+        if any(t.dtype != torch.int32 for t in (table, lens, refs)):
+            raise ValueError("PagedKVCache: table, lens and refs are int32")
         layers, pages, heads, page, head_dim = k.shape
         if table.dim() != 2 or tuple(lens.shape) != (table.shape[0],) \
                 or tuple(refs.shape) != (pages,):
@@ -49,7 +50,7 @@ class PagedKVCache:
         self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
         self.layers, self.pages, self.heads_kv, self.page, self.head_dim = k.shape
         self.slots, self.width = table.shape
-        self._device, self._row = k.device, (self.heads_kv, self.head_dim)
+        self._index, self._row = k.get_device(), (self.heads_kv, self.head_dim)
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         self._desc = _CacheDesc(layers, pages, heads, page, head_dim, k.element_size(),
                                 self.slots, self.width, k.data_ptr(), v.data_ptr(),
@@ -84,7 +85,7 @@ class PagedKVCache:
         torch = cuda_ops._torch()
         if not isinstance(values, torch.Tensor):
             values = torch.as_tensor(values, dtype=torch.int32)
-        elif values.dtype == torch.int32 and values.device == self._device \
+        elif values.dtype is torch.int32 and values.get_device() == self._index \
                 and values.dim() == 1 and values.is_contiguous() \
                 and (like is None or values.shape == like.shape):
             return values
@@ -97,7 +98,9 @@ class PagedKVCache:
         return values.contiguous()
 
     def _call(self, name, *args):
-        _native.call(name, self._ref, *args, cuda_ops._raw_stream(self.k))
+        status = getattr(_native.lib(), name)(self._ref, *args, cuda_ops._raw_stream(self._index))
+        if status:
+            _native.check(status, name)
 
     def fork(self, parents, children) -> None:
         """Slot children[i] continues slot parents[i]: it lets go of what it held, shares the
@@ -121,10 +124,14 @@ class PagedKVCache:
     def write(self, layer: int, new_k, new_v, slots, starts, cu) -> None:
         """Rows cu[i] .. cu[i + 1] of new_k / new_v [tokens, heads_kv, head_dim] are tokens
         starts[i], starts[i] + 1, ... of slot slots[i] in `layer` (reserved before)."""
-        shape = new_k.shape
+        shape, ks, vs = new_k.shape, new_k.stride(), new_v.stride()
         if len(shape) != 3 or shape != new_v.shape or shape[1:] != self._row:
             raise ValueError(f"write: expected rows [tokens, {self._row[0]}, {self._row[1]}]")
-        cuda_ops._check_rows("write", self.k, new_k, new_v)
+        if new_k.dtype is not self.k.dtype or new_v.dtype is not self.k.dtype:
+            raise TypeError("write: tensors must share a dtype")
+        if (ks[2] != 1 or vs[2] != 1) and shape[2] > 1:
+            raise ValueError("write: the last axis must be contiguous")
+        cuda_ops._same_device("write", self.k, new_k, new_v)
         if not 0 <= layer < self.layers:
             raise ValueError(f"write: layer {layer} of {self.layers}")
         slots = self._ints("write", slots)
@@ -133,7 +140,6 @@ class PagedKVCache:
         n = slots.shape[0]
         if cu.shape[0] != n + 1:
             raise ValueError("write: cu holds one number more than there are slots")
-        ks, vs = new_k.stride(), new_v.stride()
         self._call("enigma_kv_cache_write", layer, new_k.data_ptr(), new_v.data_ptr(),
                    _STRIDES.pack(ks[0], ks[1], vs[0], vs[1]), slots.data_ptr(),
                    starts.data_ptr(), cu.data_ptr(), n, shape[0])
