@@ -45,12 +45,10 @@ struct DecodeParams {
   int batch, heads_kv, group, blocks, rows;  // blocks of `rows` <= 16 heads per group
   int width, n_slots, pages, page_shift, box_shift, prefix, base;
   int fold;                                  // the prefix's keys are read here too
-  // DIRECT: where the result goes, and the prefix kernel's partial results (0 splits: none)
+  // DIRECT: where the result goes; or, part: one partial result per unit, slot = unit
   __nv_bfloat16* out;
   int64_t o_batch, o_head;
-  const float* p_opart;
-  const float2* p_ml;
-  int pairs, splits, row_tiles, tokens;
+  int part;
   float scale_log2;
   float* opart;                              // [slot][rows][D]
   float2* ml;                                // [slot][rows]
@@ -179,7 +177,8 @@ __device__ __forceinline__ Segment segment_at(const int* starts, int batch, int 
   return s;
 }
 
-// DIRECT: a CTA per unit, which writes the final result; no work list, nothing to join.
+// DIRECT: a CTA per unit, which writes the final result, or the unit's one partial result; no
+// work list.
 template <int D, bool DIRECT>
 __global__ void __launch_bounds__(DTHREADS, D == 64 ? 3 : 2)
 paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -192,7 +191,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   int* s_starts = reinterpret_cast<int*>(ring + ST * 2 * C::TILE);    // [batch + 1]
   int* s_len = s_starts + p.batch + 1;                                // [batch]
   __shared__ uint64_t full[C::DEEP][2], empty[C::DEEP];   // a stage's chunks for either team
-  __shared__ float s_m[DWARPS][ROWS], s_l[DWARPS][ROWS];    // direct
+  __shared__ float s_m[DWARPS][ROWS], s_l[DWARPS][ROWS];    // DIRECT
   __shared__ int s_warp[DWARPS + 1], s_pages[PAGES];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t most = int64_t(p.width) << p.page_shift;
@@ -219,9 +218,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     unit.block = u - unit.kvh * p.blocks;
     unit_len = len_of(p.lens, p.slots, p.n_slots, most, unit.b);
     unit.n = chunks_of(p, unit_len);
-    c1 = max(unit.n, 1);                     // one segment, if an empty one
-    if (unit.n == 0 && p.splits == 0) {      // no keys: zeros
+    c1 = unit.n;
+    if (unit.n == 0) {                       // no keys: zeros, or a part that says so
       const int rows = min(p.rows, p.group - unit.block * p.rows);
+      if (p.part) {
+        if (tid < rows) p.ml[int64_t(blockIdx.x) * p.rows + tid] = make_float2(-INFINITY, 0.f);
+        griddep_wait();
+        return;
+      }
       __nv_bfloat16* to = p.out + unit.b * p.o_batch +
                           int64_t(unit.kvh * p.group + unit.block * p.rows) * p.o_head;
       for (int x = tid; x < rows * (D / 8); x += DTHREADS)
@@ -333,7 +337,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       }
       at += s.n;
     }
-    if (!DIRECT) griddep_wait();
+    griddep_wait();
     return;
   }
 
@@ -479,58 +483,36 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           *reinterpret_cast<float2*>(s_o + (warp * ROWS + row) * D + quad * 2 + n * 8) =
               make_float2(o[n][2 * h], o[n][2 * h + 1]);
       }
-      // The prefix kernel ran beside this one; its partial results of these rows join in.
-      const PrefixRows pr = prefix_rows(p.splits, p.tokens, p.row_tiles, p.pairs, p.group, s.b, s.kvh);
-      float2* s_pre = reinterpret_cast<float2*>(s_o + DWARPS * ROWS * D);   // [rows][pr.n]
-      if (pr.n > 0) {
-        griddep_wait();
-        for (int x = tid; x < rows * pr.n; x += DWARPS * 32) {
-          const int row = x / pr.n, i = x - row * pr.n;
-          s_pre[x] = p.p_ml[pr.at + i * pr.step + s.block * p.rows + row];
-        }
-      }
       warps_all(true);
-      for (int x = tid; x < rows * (D / 2); x += DWARPS * 32) {
-        const int row = x / (D / 2), d = x % (D / 2) * 2;
-        const float2* pre = s_pre + row * pr.n;
+      for (int x = tid; x < rows * (D / 4); x += DWARPS * 32) {
+        const int row = x / (D / 4), d = x % (D / 4) * 4;
         float M = s_m[0][row];
 #pragma unroll
         for (int w = 1; w < DWARPS; ++w) M = fmaxf(M, s_m[w][row]);
-        for (int i = 0; i < pr.n; ++i) M = fmaxf(M, pre[i].x);
-        float2 acc = make_float2(0.f, 0.f);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         float L = 0.f;
 #pragma unroll
         for (int w = 0; w < DWARPS; ++w) {
-          if (s_m[w][row] == -INFINITY) continue;           // saw no key; o is not written
+          if (s_m[w][row] == -INFINITY) continue;           // saw no key: o is not written
           const float f = ex2(s_m[w][row] - M);
-          const float2 v = *reinterpret_cast<const float2*>(s_o + (w * ROWS + row) * D + d);
+          const float4 v = *reinterpret_cast<const float4*>(s_o + (w * ROWS + row) * D + d);
           acc.x = fmaf(v.x, f, acc.x);
           acc.y = fmaf(v.y, f, acc.y);
+          acc.z = fmaf(v.z, f, acc.z);
+          acc.w = fmaf(v.w, f, acc.w);
           L = fmaf(s_l[w][row], f, L);
         }
-        const float* po = p.p_opart + (pr.at + s.block * p.rows + row) * D + d;
-        for (int i0 = 0; i0 < pr.n; i0 += 8) {              // 8 loads in flight
-          float2 v[8];
-          float f[8];
-#pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const float m_i = i0 + u < pr.n ? pre[i0 + u].x : -INFINITY;
-            f[u] = m_i == -INFINITY ? 0.f : ex2(m_i - M);
-            v[u] = make_float2(0.f, 0.f);
-            if (f[u] != 0.f)
-              v[u] = __ldcg(reinterpret_cast<const float2*>(po + (i0 + u) * pr.step * D));
-          }
-#pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            acc.x = fmaf(v[u].x, f[u], acc.x);
-            acc.y = fmaf(v[u].y, f[u], acc.y);
-            if (f[u] != 0.f) L = fmaf(pre[i0 + u].y, f[u], L);
-          }
+        if (p.part) {
+          const int64_t at_part = int64_t(blockIdx.x) * p.rows + row;
+          *reinterpret_cast<float4*>(p.opart + at_part * D + d) = acc;
+          if (d == 0) p.ml[at_part] = make_float2(M, L);
+        } else {
+          const float inv = L == 0.f ? 0.f : 1.f / L;
+          const int64_t at_out = s.b * p.o_batch +
+                                 int64_t(s.kvh * p.group + s.block * p.rows + row) * p.o_head + d;
+          *reinterpret_cast<uint2*>(p.out + at_out) = make_uint2(
+              pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
         }
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        const int64_t at_out = s.b * p.o_batch +
-                               int64_t(s.kvh * p.group + s.block * p.rows + row) * p.o_head + d;
-        *reinterpret_cast<uint32_t*>(p.out + at_out) = pack_bf16x2(acc.x * inv, acc.y * inv);
       }
       return;
     }
@@ -570,47 +552,95 @@ struct JoinParams {
   // own keys
   const float* d_opart;
   const float2* d_ml;
-  const int32_t* starts;
+  const int32_t* starts;                   // NULL: one part per unit
   int blocks, rows, ctas;
 };
 
-// Joins a row's partial results.  One warp per (sequence, query head).
+// Joins a row's partial results,
+//   O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, M = max_i m_i (m in log2 units),
+// the prefix's in their order, then the own ones.  One warp per (sequence, query head).  It is all
+// latency (L2 answers in half a microsecond, and a row has a few dozen parts): 16 parts' rows are
+// in flight together, the first 16 already beside their (m, l).  A part that saw no key (m = -inf)
+// may hold anything.
 template <int D>
 __global__ void __launch_bounds__(128) paged_join_kernel(const JoinParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t id = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (id >= int64_t(p.batch) * p.heads_q) return;
-  griddep_wait();
-  const int b = int(id / p.heads_q), h = int(id - int64_t(b) * p.heads_q);
-  const int kvh = h / p.group, gh = h - kvh * p.group;
-  const PrefixRows pr =
-      prefix_rows(p.splits, p.tokens, p.row_tiles, p.pairs, p.group, b, kvh);
-  // Own partials: the slots of the CTAs that hold the unit's chunks.
-  int n_d = 0;
-  int64_t d_at = 0;
-  const int per_b = p.heads_kv * p.blocks;
-  const int64_t T = int64_t(p.starts[p.batch]) * per_b;
-  const int n = p.starts[b + 1] - p.starts[b];
-  if (n > 0) {
-    const int block = gh / p.rows, u = kvh * p.blocks + block;
-    const int64_t x0 = int64_t(p.starts[b]) * per_b + int64_t(u) * n;
-    const int64_t P = min(int64_t(p.ctas), T);
-    const int first = owner(x0, T, P), last = owner(x0 + n - 1, T, P);
-    n_d = (last - first + 1) * DWARPS;
-    d_at = (int64_t(first) + b * per_b + u) * DWARPS * p.rows + (gh - block * p.rows);
-  }
   constexpr int V = D / 32;
-  enigma_serving::RowJoin<V> join;
+  const int lane = threadIdx.x & 31;
+  const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 5);     // batch * heads_q < 2^28
+  if (id >= uint32_t(p.batch) * uint32_t(p.heads_q)) return;
+  const int b = int(id / uint32_t(p.heads_q)), h = int(id - uint32_t(b) * uint32_t(p.heads_q));
+  const int kvh = h / p.group, gh = h - kvh * p.group;
+  const PrefixRows pr = prefix_rows(p.splits, p.tokens, p.row_tiles, p.pairs, p.group, b, kvh);
   const int64_t p_at = pr.at + gh;
-  join.best(p.p_ml + p_at, pr.step, pr.n, lane);
-  join.best(p.d_ml + d_at, p.rows, n_d, lane);
-  join.seal();
-  join.add(p.p_ml + p_at, pr.step, p.p_opart + p_at * D, int64_t(pr.step) * D, pr.n, D, lane);
-  join.add(p.d_ml + d_at, p.rows, p.d_opart + d_at * D, int64_t(p.rows) * D, n_d, D, lane);
-  const float inv = join.l == 0.f ? 0.f : 1.f / join.l;
-  __nv_bfloat16* out = p.out + b * p.o_batch + h * p.o_head + lane;
+  const int per_b = p.heads_kv * p.blocks, block = gh / p.rows, u = kvh * p.blocks + block;
+  const int64_t unit = int64_t(b) * per_b + u;
+  int n_d = 1;
+  int64_t d_at = unit * p.rows + (gh - block * p.rows);
+  griddep_wait();
+  if (p.starts != nullptr) {
+    // The slots of the CTAs that hold the unit's chunks.
+    const int64_t T = int64_t(p.starts[p.batch]) * per_b;
+    const int start = p.starts[b], chunks = p.starts[b + 1] - start;
+    n_d = 0;
+    if (chunks > 0) {
+      const int64_t x0 = int64_t(start) * per_b + int64_t(u) * chunks;
+      const int64_t P = min(int64_t(p.ctas), T);
+      const int first = owner(x0, T, P), last = owner(x0 + chunks - 1, T, P);
+      n_d = (last - first + 1) * DWARPS;
+      d_at = (int64_t(first) + unit) * DWARPS * p.rows + (gh - block * p.rows);
+    }
+  }
+  const int n = pr.n + n_d;
+  auto row_at = [&](int i) {                       // row of part i in its workspace
+    return i < pr.n ? p_at + int64_t(i) * pr.step : d_at + int64_t(i - pr.n) * p.rows;
+  };
+  auto ml_at = [&](int i) { return __ldcg((i < pr.n ? p.p_ml : p.d_ml) + row_at(i)); };
+  constexpr int BATCH = 16;
+  float v[BATCH][V];
+  auto fetch = [&](int base) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) out[32 * v] = __float2bfloat16_rn(join.acc[v] * inv);
+    for (int u = 0; u < BATCH; ++u) {
+      if (base + u >= n) break;
+      const float* from = (base + u < pr.n ? p.p_opart : p.d_opart) + row_at(base + u) * D + lane * V;
+      if constexpr (V == 4) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(from));
+        v[u][0] = x.x, v[u][1] = x.y, v[u][2] = x.z, v[u][3] = x.w;
+      } else {
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(from));
+        v[u][0] = x.x, v[u][1] = x.y;
+      }
+    }
+  };
+  fetch(0);
+  float2 mine = lane < n ? ml_at(lane) : make_float2(-INFINITY, 0.f);
+  float M = mine.x;
+  for (int i = lane + 32; i < n; i += 32) M = fmaxf(M, ml_at(i).x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  float acc[V] = {}, l = 0.f, w = 0.f;
+  for (int base = 0; base < n; base += BATCH) {
+    if (base > 0) fetch(base);
+    if (base % 32 == 0) {
+      if (base > 0) mine = base + lane < n ? ml_at(base + lane) : make_float2(-INFINITY, 0.f);
+      w = mine.x == -INFINITY ? 0.f : ex2(mine.x - M);
+      if (w != 0.f) l = fmaf(w, mine.y, l);        // this lane's parts
+    }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const float f = __shfl_sync(0xffffffffu, w, (base + u) & 31);
+      if (base + u < n && f != 0.f) {
+#pragma unroll
+        for (int x = 0; x < V; ++x) acc[x] = fmaf(v[u][x], f, acc[x]);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __nv_bfloat16* out = p.out + b * p.o_batch + h * p.o_head + lane * V;
+#pragma unroll
+  for (int x = 0; x < V; x += 2)
+    *reinterpret_cast<uint32_t*>(out + x) = pack_bf16x2(acc[x] * inv, acc[x + 1] * inv);
 }
 
 // ============================================================================ host
@@ -634,11 +664,15 @@ int log2_of(int64_t x) {
 }
 
 constexpr int64_t kFoldBytes = 128ll << 20, kDirectKeys = 1536;
+// Work of less is done one after the other: two streams cost four more host calls.  (32 sequences,
+// 4096 shared and up to 512 own keys, 8 kv heads of 128: 22.1 us side by side, 29.5 one after
+// the other; 128, 32768 and 1024: 117 / 134; 8, 2048 and 128: 12.6 / 13.6.)
+constexpr double kBesideUs = 3.0;
 
 struct Layout {
   int group, tokens, row_tiles, pairs, splits, prefix;    // prefix part
   int blocks, rows, ctas;                                 // own part
-  bool fold, direct;
+  bool fold, direct, beside;
   size_t p_opart, p_ml, d_opart, d_ml, starts, total;     // byte offsets
 };
 
@@ -659,22 +693,33 @@ Layout layout_of(const enigma_sdpa_shared_prefix_desc& d) {
   const int64_t most = d.table_width * d.page;
   y.fold = y.prefix > 0 && most <= kDirectKeys &&
            d.batch * y.prefix * d.heads_kv * d.head_dim * 4 <= kFoldBytes;
-  // A CTA per unit reads the own keys too, and joins them with the prefix's partial results, where
-  // no row has many of them; else they are split over the SMs and joined by a third launch.
+  // A CTA per unit reads the own keys where no row has many of them; else they are split over the
+  // SMs.  Where the prefix is apart, a third launch joins the parts of both.
   y.direct = y.fold || most - y.prefix <= kDirectKeys;
+  y.blocks = (y.group + ROWS - 1) / ROWS;
+  y.rows = (y.group + y.blocks - 1) / y.blocks;
+  const int64_t d_units = d.batch * d.heads_kv * y.blocks;
   if (tiles > 0 && !y.fold) {
-    // As many parts of the keys as there are SMs, each at least two tiles.
+    // The prefix is bound by the tensor cores, the own keys by memory, which a few SMs can keep
+    // busy: so each gets SMs by its work, side by side.  Per SM, a step of the prefix (128 keys for
+    // 256 rows) takes 1.9 us, own keys come at 0.1 MB/us; half of what the table has room for is taken
+    // as the own keys' number.  Parts of at least two tiles.
     const int64_t units = int64_t(d.heads_kv) * y.pairs;
-    y.splits = int(std::max<int64_t>(1, std::min<int64_t>(sms / std::max<int64_t>(units, 1),
+    const double steps = double(d.heads_kv) * double(tiles) * (double(y.pairs) - (y.row_tiles % 2) * 0.5);
+    const double prefix = 1.9 * steps;
+    const double own = double(d.batch * d.heads_kv) * double(most - y.prefix) / 2 *
+                       double(d.head_dim) * 4 / 1e5;
+    y.beside = y.direct && (prefix + own) / sms > kBesideUs;
+    const int64_t share = std::max<int64_t>(
+        sms / 4, y.beside ? int64_t(sms * prefix / (prefix + own) + 0.5) : sms);
+    y.splits = int(std::max<int64_t>(1, std::min<int64_t>(share / std::max<int64_t>(units, 1),
                                                           (tiles + 1) / 2)));
   }
   const int64_t p_slots = int64_t(d.heads_kv) * y.pairs * y.splits * 2;
-  y.blocks = (y.group + ROWS - 1) / ROWS;
-  y.rows = (y.group + y.blocks - 1) / y.blocks;
-  y.ctas = sms * (d.head_dim == 64 ? 3 : 2);
-  if (y.direct) y.ctas = int(d.batch * d.heads_kv) * y.blocks;
-  const int64_t d_slots =
-      y.direct ? 0 : (int64_t(y.ctas) + d.batch * d.heads_kv * y.blocks) * DWARPS;
+  y.ctas = y.direct ? int(d_units) : sms * (d.head_dim == 64 ? 3 : 2);
+  const int64_t d_slots = !y.direct      ? (int64_t(y.ctas) + d_units) * DWARPS
+                          : y.splits > 0 ? d_units
+                                         : 0;
   size_t at = 0;
   auto take = [&](int64_t bytes) {
     const size_t here = at;
@@ -700,6 +745,19 @@ bool pages_map(CUtensorMap* m, const void* base, const enigma_sdpa_shared_prefix
   return make_map(m, base, 4, dims, strides, box);
 }
 
+// The calling thread's two events on the current device, for a fork to the second stream and back
+// (a wait takes the event's state when it is made, so the next call may record it again).
+cudaError_t fork_events(cudaEvent_t** events) {
+  thread_local cudaEvent_t kept[64][2] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev >= 64) e = cudaErrorInvalidDevice;
+  for (int i = 0; i < 2 && e == cudaSuccess; ++i)
+    if (kept[dev][i] == nullptr) e = cudaEventCreateWithFlags(&kept[dev][i], cudaEventDisableTiming);
+  if (e == cudaSuccess) *events = kept[dev];
+  return e;
+}
+
 template <int D>
 cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
   const Layout y = layout_of(d);
@@ -714,6 +772,12 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
   const float scale_log2 = d.scale * 1.4426950408889634f;
   const int page_shift = log2_of(d.page), box_shift = log2_of(box_rows);
   cudaError_t e;
+  cudaEvent_t* fork = nullptr;
+  if (y.beside) {
+    e = fork_events(&fork);
+    if (e == cudaSuccess) e = cudaEventRecord(fork[0], s);
+    if (e != cudaSuccess) return e;
+  }
   if (y.splits > 0) {
     CUtensorMap mq;
     const cuuint64_t dims[3] = {cuuint64_t(D), cuuint64_t(d.heads_q), cuuint64_t(d.batch)};
@@ -774,19 +838,14 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
   p.out = static_cast<__nv_bfloat16*>(d.out);
   p.o_batch = d.o_batch;
   p.o_head = d.o_head;
-  p.p_opart = reinterpret_cast<const float*>(ws + y.p_opart);
-  p.p_ml = reinterpret_cast<const float2*>(ws + y.p_ml);
-  p.pairs = y.pairs;
-  p.splits = y.splits;
-  p.row_tiles = y.row_tiles;
-  p.tokens = y.tokens;
+  p.part = y.splits > 0;
   p.scale_log2 = scale_log2;
   p.opart = reinterpret_cast<float*>(ws + y.d_opart);
   p.ml = reinterpret_cast<float2*>(ws + y.d_ml);
   p.starts = reinterpret_cast<int32_t*>(ws + y.starts);
   p.status = status;
   // A CTA that has the SM to itself needs the whole ring to cover the loads' latency.
-  p.stages = y.ctas <= enigma::sm_count() ? DCfg<D>::DEEP : DCfg<D>::STAGES;
+  p.stages = y.direct && y.ctas <= enigma::sm_count() ? DCfg<D>::DEEP : DCfg<D>::STAGES;
   const int smem = p.stages * 2 * DCfg<D>::TILE + 1024 + (y.direct ? 0 : int(2 * d.batch + 1) * 4);
   const auto kernel = y.direct ? paged_decode_kernel<D, true> : paged_decode_kernel<D, false>;
   {
@@ -794,23 +853,36 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
     int dev = 0;
     e = cudaGetDevice(&dev);
     if (e == cudaSuccess && !(dev < 64 && (ready.load() >> dev & 1))) {
-      const int most = DCfg<D>::DEEP * 2 * DCfg<D>::TILE + 1024 + 8193 * 4;
       e = cudaFuncSetAttribute(paged_decode_kernel<D, true>,
-                               cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+                               cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               DCfg<D>::DEEP * 2 * DCfg<D>::TILE + 1024);
       if (e == cudaSuccess)
         e = cudaFuncSetAttribute(paged_decode_kernel<D, false>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 DCfg<D>::STAGES * 2 * DCfg<D>::TILE + 1024 + 8193 * 4);
       if (e == cudaSuccess && dev < 64) ready.fetch_or(uint64_t(1) << dev);
     }
     if (e != cudaSuccess) return e;
   }
-  if (y.splits > 0) {
+  if (y.beside) {
+    // On the library's second stream, after the work before this call and before the join, which
+    // waits for it even if the launch failed: a stream that captures must come back.
+    cudaStream_t side = enigma::aux_stream();
+    if (side == nullptr) return cudaErrorMemoryAllocation;
+    e = cudaStreamWaitEvent(side, fork[0], 0);
+    if (e != cudaSuccess) return e;
+    kernel<<<unsigned(y.ctas), DTHREADS, smem, side>>>(mk, mv, p);
+    e = cudaGetLastError();
+    cudaError_t back = cudaEventRecord(fork[1], side);
+    if (back == cudaSuccess) back = cudaStreamWaitEvent(s, fork[1], 0);
+    if (e == cudaSuccess) e = back;
+  } else if (y.splits > 0) {
     e = enigma::launch_dependent(kernel, unsigned(y.ctas), DTHREADS, smem, s, mk, mv, p);
   } else {
     kernel<<<unsigned(y.ctas), DTHREADS, smem, s>>>(mk, mv, p);
     e = cudaGetLastError();
   }
-  if (e != cudaSuccess || y.direct) return e;
+  if (e != cudaSuccess || (y.direct && y.splits == 0)) return e;
   JoinParams j = {};
   j.out = static_cast<__nv_bfloat16*>(d.out);
   j.o_batch = d.o_batch;
@@ -827,11 +899,15 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
   j.tokens = y.tokens;
   j.d_opart = p.opart;
   j.d_ml = p.ml;
-  j.starts = p.starts;
+  j.starts = y.direct ? nullptr : p.starts;
   j.blocks = y.blocks;
   j.rows = y.rows;
   j.ctas = y.ctas;
   const unsigned grid = unsigned((d.batch * d.heads_q + 3) / 4);
+  if (y.beside) {
+    paged_join_kernel<D><<<grid, 128, 0, s>>>(j);
+    return cudaGetLastError();
+  }
   return enigma::launch_dependent(paged_join_kernel<D>, grid, 128, 0, s, j);
 }
 

@@ -33,53 +33,4 @@ struct PackedGroup {
 };
 constexpr int kGroupInts = sizeof(PackedGroup) / 4;
 
-// Joins partial results of one row, a warp's work:
-//   O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, M = max_i m_i (m in log2 units),
-// always in the same order.  add() folds n partials in, `ml` + i * ml_step and `o` + i * o_step
-// (D floats, lane takes every 32nd); best() must have seen the same ones first.  The lanes
-// load 32 pairs (m, l) at once and 8 partials' rows are in flight together: one after the other
-// the loads' latency is the whole time (20 partials: 24 us, now 3).  A partial that saw no key
-// (m = -inf) may hold anything.
-template <int V>
-struct RowJoin {
-  float acc[V] = {};
-  float M = -INFINITY, l = 0.f;
-  __device__ void best(const float2* ml, int64_t ml_step, int n, int lane) {
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, ml[i * ml_step].x);
-  }
-  __device__ void seal() {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  }
-  __device__ void add(const float2* ml, int64_t ml_step, const float* o, int64_t o_step, int n, int D,
-                      int lane) {
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const float2 mine = i0 + lane < n ? ml[(i0 + lane) * ml_step] : make_float2(-INFINITY, 0.f);
-      const float w = mine.x == -INFINITY ? 0.f : exp2f(mine.x - M);
-      float part = w == 0.f ? 0.f : w * mine.y;
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) part += __shfl_xor_sync(0xffffffffu, part, x);
-      l += part;
-      const int here = min(32, n - i0);
-      for (int i = 0; i < here; i += 8) {
-        float f[8], v[8][V];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          f[u] = __shfl_sync(0xffffffffu, w, (i + u) & 31);
-          if (i + u >= here) f[u] = 0.f;
-#pragma unroll
-          for (int x = 0; x < V; ++x) {
-            v[u][x] = 0.f;
-            if (f[u] != 0.f && lane + 32 * x < D) v[u][x] = o[(i0 + i + u) * o_step + lane + 32 * x];
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-#pragma unroll
-          for (int x = 0; x < V; ++x) acc[x] = fmaf(v[u][x], f[u], acc[x]);
-      }
-    }
-  }
-};
-
 }  // namespace enigma_serving

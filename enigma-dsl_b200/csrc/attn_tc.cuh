@@ -190,6 +190,14 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const void* desc, uint64_
       : "memory");
 }
 
+// The same box fetched into L2 only.
+__device__ __forceinline__ void prefetch_l2_4d(const void* desc, int32_t c0, int32_t c1, int32_t c2,
+                                               int32_t c3) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];"
+               ::"l"(reinterpret_cast<uint64_t>(desc)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+
 // The number of a page, or `pages` (out of the tensor map's range: reads as zeros) where the
 // table holds none.
 __device__ __forceinline__ int page_at(const int32_t* table, const int32_t* slots, int n_slots,
@@ -303,24 +311,43 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         };
         ok = load_q(0, w.cnt0);
         if (!ok) break;
-        // Paged: lane x knows the page of box x of the next tile, read one tile ahead.  One lane
+        // Paged: lane x knows the page of box x of the next tiles, read AHEAD tiles ahead, and asks
+        // for the tile's bytes in L2 then: two stages cover L2's latency, not HBM's.  One lane
         // issues all boxes: each lane its own costs 150 cycles a box.
-        int at = 0;
-        auto look_up = [&](int j) {
-          at = page_at(p.table, p.slots, p.n_slots, p.width, p.pages, 0,
-                       (j * BN + (lane << p.box_shift)) >> p.page_shift);
-        };
+        constexpr int AHEAD = 3;
+        int at[AHEAD + 1];                   // pages of tiles j .. j + AHEAD
         const bool looks = PAGED && lane < (BN >> p.box_shift);
-        if (looks) look_up(w.j0);
+        auto look_up = [&](int j) {          // the j-th tile of the item; none past its end
+          if (!looks || j >= w.all) return p.pages;
+          return page_at(p.table, p.slots, p.n_slots, p.width, p.pages, 0,
+                         ((w.j0 + j) * BN + (lane << p.box_shift)) >> p.page_shift);
+        };
+        auto row_of = [&](int j) {           // first row of this lane's box in its page
+          return ((w.j0 + j) * BN + (lane << p.box_shift)) & ((1 << p.page_shift) - 1);
+        };
+        if (PAGED) {
+#pragma unroll
+          for (int x = 0; x <= AHEAD; ++x) at[x] = look_up(x);
+        }
         for (int j = 0; j < w.all; ++j, ++jg) {
           const int s = jg % ST;
           const uint32_t ph = (jg / ST) & 1;
           const int key0 = (w.j0 + j) * BN;
-          const int at_now = at;
           int boxes = 0;
+          int at_now = 0;
           if (PAGED) {
             boxes = (min(BN, w.lk - key0) + (1 << p.box_shift) - 1) >> p.box_shift;
-            if (looks && j + 1 < w.all) look_up(w.j0 + j + 1);
+            at_now = at[0];
+#pragma unroll
+            for (int x = 0; x < AHEAD; ++x) at[x] = at[x + 1];
+            at[AHEAD] = look_up(j + AHEAD + 1);
+            if (at[AHEAD - 1] < p.pages) {   // tile j + AHEAD
+#pragma unroll
+              for (int a = 0; a < C::ATOMS; ++a) {
+                prefetch_l2_4d(&tmK, a * 64, row_of(j + AHEAD), w.kvh, at[AHEAD - 1]);
+                prefetch_l2_4d(&tmV, a * 64, row_of(j + AHEAD), w.kvh, at[AHEAD - 1]);
+              }
+            }
           }
           const uint32_t bytes = PAGED ? (uint32_t(boxes * C::ATOMS) * 128u) << p.box_shift
                                        : uint32_t(C::KV_BYTES);

@@ -400,3 +400,34 @@ def test_shared_prefix_refusals(cuda):
         run(q.repeat(2, 1, 1), k, k, table, lens)
     with pytest.raises(ValueError, match="slots"):
         run(q, k, k, table, lens, slots=lens[:1])
+
+
+def test_shared_prefix_side_by_side_in_a_graph_and_on_streams(cuda):
+    """Large enough for the prefix and the own keys to run on two streams: captured, replayed with
+    other lengths, and called on several streams at once."""
+    import torch
+    from enigma import cuda_ops
+    rng = np.random.default_rng(21)
+    k, v, table, lens = _paged_case(rng, 40, 3000, [1 + 11 * b for b in range(40)], 64, 4, 128, "bf16")
+    kd, vd = _dev(k, "bf16", cuda), _dev(v, "bf16", cuda)
+    td, ld = torch.from_numpy(table).to(cuda), torch.from_numpy(lens).to(cuda)
+    q = _dev(_values(rng, (40, 16, 128), "bf16"), "bf16", cuda)
+    want = cuda_ops.sdpa_shared_prefix(q, kd, vd, td, ld, prefix_len=3000)
+    short = cuda_ops.sdpa_shared_prefix(q, kd, vd, td, ld - 20, prefix_len=3000)
+    out = torch.empty_like(want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cuda_ops.sdpa_shared_prefix(q, kd, vd, td, ld, prefix_len=3000, out=out)
+    graph.replay()
+    assert torch.equal(out, want)
+    ld -= 20
+    graph.replay()
+    assert torch.equal(out, short)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for s in streams * 2:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(cuda_ops.sdpa_shared_prefix(q, kd, vd, td, ld, prefix_len=3000))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, short) for g in got)
