@@ -17,12 +17,16 @@ using namespace enigma_tc;
 // of up to 16 query heads); CTA c of P takes the contiguous range [c T / P, (c + 1) T / P), so
 // every SM streams the same number of chunks whatever the lengths are.  A producer warp loads
 // chunks by TMA (one box per page and 64 columns) into a ring; two warps take 32 keys each of
-// the even chunks, two of the odd ones (16 keys of every chunk per warp: 1.2x the time, a chunk's
-// chain of dependent steps is longer than its work): S = Q K^T (mma.sync, the heads as the 16-row operand), online softmax, O += P V.  At
-// the end of a unit's run of chunks each warp stores its state, in slot (c + u) * 4 + warp
-// (segments in order advance c or u, so the slots are distinct).  Merging the warps first cost
-// two barriers and a second pass per run (92 against 60 us for 128 sequences of 5 to 1024 keys);
-// four partials of a few KB next to a run's 100 KB and more of K and V cost less.
+// the even chunks, two of the odd ones.  Both products have the keys or the elements as the
+// 16-row operand and the heads, at most 16, as the 8-column one: S^T = K Q^T, O^T += V^T P^T with
+// P^T's fragments turned by movmatrix.  For up to 8 heads that is half the products and half the
+// registers of the form with the heads as rows (128 sequences of 1 to 1024 keys, 32 / 8 heads of
+// 128: 52.9 -> 50.4 us, 5.3 TB/s; next to a shared prefix, where it has a third of the SMs, 32768
+// shared keys and those: 117.5 -> 109.5).  Statistics and O in fp32; P is rounded to bf16,
+// as the product takes it, its sum is of the unrounded values.  At the end of a unit's run of
+// chunks each warp stores its state, in slot (c + u) * 4 + warp (segments in order advance c or
+// u, so the slots are distinct): merging the warps first would cost two barriers and a second pass
+// per run, four partials of a few KB next to a run's 100 KB and more of K and V cost less.
 constexpr int CHUNK = 64;
 constexpr int DWARPS = 4;
 constexpr int DTHREADS = (DWARPS + 1) * 32;
@@ -34,7 +38,8 @@ template <int D>
 struct DCfg {
   static constexpr int ATOMS = D / 64;
   static constexpr int TILE = CHUNK * D * 2;            // one of K or V
-  static constexpr int STAGES = D == 64 ? 4 : 3;          // 3 or 2 CTAs on an SM
+  static constexpr int CTAS = D == 64 ? 3 : 2;            // on an SM, with STAGES each
+  static constexpr int STAGES = 4 - D / 128;
   static constexpr int DEEP = D == 64 ? 12 : 6;           // one CTA on an SM
 };
 
@@ -75,6 +80,17 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t turn_8x8(uint32_t x) {   // an 8 x 8 fragment, transposed
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// Sum over the lanes that hold the same heads.
+__device__ __forceinline__ float over_keys(float x) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
 }
 // Barrier over the DWARPS consumer warps; whether all say yes.
 __device__ __forceinline__ bool warps_all(bool ok) {
@@ -178,9 +194,9 @@ __device__ __forceinline__ Segment segment_at(const int* starts, int batch, int 
 }
 
 // DIRECT: a CTA per unit, which writes the final result, or the unit's one partial result; no
-// work list.
-template <int D, bool DIRECT>
-__global__ void __launch_bounds__(DTHREADS, D == 64 ? 3 : 2)
+// work list.  NT: tiles of 8 heads.
+template <int D, bool DIRECT, int NT>
+__global__ void __launch_bounds__(DTHREADS, DCfg<D>::CTAS)
 paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const DecodeParams p) {
   using C = DCfg<D>;
@@ -280,12 +296,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 
   if (warp == DWARPS) {
     // ---------------------------------------------------------------- producer
-    // One lane issues all boxes of a chunk: each lane its own costs 150 cycles a box, which left
-    // the ring empty.
+    // One lane issues all boxes of a chunk; each lane its own was no faster.
     const int per_shift = 6 - p.box_shift, per = 1 << per_shift;   // boxes per chunk
     const int ahead = PAGES >> per_shift;                            // chunks looked up at once
     // Stages, parities and places in the look-up are counted on: a division here, in a warp with
-    // nothing else to run, held up every chunk (1300 cycles a chunk with five of them, 500 without).
+    // nothing else to run, holds up every chunk (16 sequences of 512 shared keys, 8 kv heads of 128:
+    // 14.6 us with five of them, 12.3 without).
     int st = 0, wraps = 0, team = 0;
     for (int64_t at = c0; at < c1;) {
       const Segment s = segment(at);
@@ -349,24 +365,34 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const Segment s = segment(at);
     const int len = DIRECT ? unit_len : s_len[s.b], np = prefix_chunks(p, len);
     const int rows = min(p.rows, p.group - s.block * p.rows);
-    uint32_t q[D / 16][4];
+    uint32_t q[D / 16][NT][2];                              // Q^T: head g, elements 2 quad ..
     {
       const __nv_bfloat16* qb = p.q + s.b * p.q_batch +
                                 int64_t(s.kvh * p.group + s.block * p.rows) * p.q_head;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = g + (e & 1) * 8, d = kk * 16 + quad * 2 + (e >> 1) * 8;
-          q[kk][e] = row < rows ? *reinterpret_cast<const uint32_t*>(qb + row * p.q_head + d) : 0u;
-        }
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = t * 8 + g, d = kk * 16 + quad * 2 + e * 8;
+            q[kk][t][e] =
+                row < rows ? *reinterpret_cast<const uint32_t*>(qb + row * p.q_head + d) : 0u;
+          }
     }
-    float o[D / 8][4];
+    // A lane's heads: t * 8 + 2 quad + {0, 1}; of O^T the elements dd * 16 + g + {0, 8}.
+    float o[D / 16][NT][4];
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n)
+    for (int dd = 0; dd < D / 16; ++dd)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[dd][t][e] = 0.f;
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) m[t][h] = -INFINITY, l[t][h] = 0.f;
     bool ok = true;
     for (int j = s.j0; j < s.j0 + s.n; ++j) {
       if (++st == ST) st = 0, ++wraps;
@@ -382,30 +408,34 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       const Chunk ch = chunk_at(p, s.b, len, np, j);
       const int row0 = (warp & 1) * WKEYS;                  // this warp's first row of the chunk
       const int key0 = ch.key0 + row0;
-      float sc[WKEYS / 8][4];
+      float sc[WKEYS / 16][NT][4];                          // S^T: keys g and g + 8 of each 16
 #pragma unroll
-      for (int n = 0; n < WKEYS / 8; ++n)
+      for (int n = 0; n < WKEYS / 16; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[n][t][e] = 0.f;
       const int mi = lane >> 3, mr = lane & 7;              // ldmatrix: matrix, row
       const uint32_t ka = smem_u32(tile_k);
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
         for (int n = 0; n < WKEYS / 16; ++n) {
-          uint32_t b[4];
+          uint32_t a[4];
           ldsm_x4(ka + (kk / 4) * CHUNK * 128 +
-                      sw128(row0 + n * 16 + (mi >> 1) * 8 + mr, (kk % 4) * 2 + (mi & 1)), b);
-          mma_16816(sc[2 * n], q[kk], b[0], b[1]);
-          mma_16816(sc[2 * n + 1], q[kk], b[2], b[3]);
+                      sw128(row0 + n * 16 + (mi & 1) * 8 + mr, (kk % 4) * 2 + (mi >> 1)), a);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_16816(sc[n][t], a, q[kk][t][0], q[kk][t][1]);
         }
       if (key0 + WKEYS > ch.hi || key0 < ch.lo) {           // warp-uniform
 #pragma unroll
-        for (int n = 0; n < WKEYS / 8; ++n)
+        for (int n = 0; n < WKEYS / 16; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int key = key0 + n * 8 + quad * 2 + (e & 1);
-            if (key >= ch.hi || key < ch.lo) sc[n][e] = -INFINITY;
+            const int key = key0 + n * 16 + g + (e >> 1) * 8;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              if (key >= ch.hi || key < ch.lo) sc[n][t][e] = -INFINITY;
           }
         // Rows past the end hold whatever the page or the ring held, rows of the prefix
         // whatever this sequence's page has there: 0 * NaN must not be.
@@ -418,46 +448,49 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         fence_proxy_async_smem();                           // before the next TMA write here
         __syncwarp();
       }
-      float mc[2];
+      float mc[NT][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {                         // rows g and g + 8
-        float mx = m[h];
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int n = 0; n < WKEYS / 8; ++n) mx = max3f(mx, sc[n][2 * h], sc[n][2 * h + 1]);
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        mc[h] = mx == -INFINITY ? 0.f : mx * p.scale_log2;
-        const float f = ex2(m[h] * p.scale_log2 - mc[h]);   // m = -inf: 0
-        m[h] = mx;
-        l[h] *= f;
-        if (__any_sync(0xffffffffu, f != 1.f)) {
+        for (int h = 0; h < 2; ++h) {
+          float mx = m[t][h];
 #pragma unroll
-          for (int n = 0; n < D / 8; ++n) {
-            o[n][2 * h] *= f;
-            o[n][2 * h + 1] *= f;
+          for (int n = 0; n < WKEYS / 16; ++n) mx = max3f(mx, sc[n][t][h], sc[n][t][2 + h]);
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+          mc[t][h] = mx == -INFINITY ? 0.f : mx * p.scale_log2;
+          const float f = ex2(m[t][h] * p.scale_log2 - mc[t][h]);   // m = -inf: 0
+          m[t][h] = mx;
+          l[t][h] *= f;
+          if (__any_sync(0xffffffffu, f != 1.f)) {
+#pragma unroll
+            for (int dd = 0; dd < D / 16; ++dd) {
+              o[dd][t][h] *= f;
+              o[dd][t][2 + h] *= f;
+            }
           }
         }
-      }
       const uint32_t va = smem_u32(tile_v);
 #pragma unroll
       for (int n = 0; n < WKEYS / 16; ++n) {
-        uint32_t pa[4];
+        uint32_t pb[NT][2];                                 // P^T: head g, keys 2 quad .. and + 8
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float e0 = ex2(fmaf(sc[2 * n + t][2 * h], p.scale_log2, -mc[h]));
-            const float e1 = ex2(fmaf(sc[2 * n + t][2 * h + 1], p.scale_log2, -mc[h]));
-            l[h] += e0 + e1;                                // this lane's share of the row's sum
-            pa[2 * t + h] = pack_bf16x2(e0, e1);
+          for (int e = 0; e < 2; ++e) {
+            const float e0 = ex2(fmaf(sc[n][t][2 * e], p.scale_log2, -mc[t][0]));
+            const float e1 = ex2(fmaf(sc[n][t][2 * e + 1], p.scale_log2, -mc[t][1]));
+            l[t][0] += e0;                                  // this lane's share of the sums
+            l[t][1] += e1;
+            pb[t][e] = turn_8x8(pack_bf16x2(e0, e1));
           }
 #pragma unroll
         for (int dd = 0; dd < D / 16; ++dd) {
-          uint32_t b[4];
+          uint32_t a[4];
           ldsm_x4_trans(va + (dd / 4) * CHUNK * 128 +
-                            sw128(row0 + n * 16 + (mi & 1) * 8 + mr, (dd % 4) * 2 + (mi >> 1)), b);
-          mma_16816(o[2 * dd], pa, b[0], b[1]);
-          mma_16816(o[2 * dd + 1], pa, b[2], b[3]);
+                            sw128(row0 + n * 16 + (mi >> 1) * 8 + mr, (dd % 4) * 2 + (mi & 1)), a);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_16816(o[dd][t], a, pb[t][0], pb[t][1]);
         }
       }
       __syncwarp();
@@ -467,22 +500,26 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       // The ring is idle once every warp is here: it takes the warps' states, each thread sums
       // two columns of a row over the warps, in their order.
       if (!warps_all(ok)) return;                           // a wait ran out (status is set)
-      float* s_o = reinterpret_cast<float*>(ring);          // [DWARPS][ROWS][D]
+      constexpr int LD = D + 4;                             // a store's 32 lanes meet 32 banks
+      float* s_o = reinterpret_cast<float*>(ring);          // [DWARPS][NT * 8][LD]
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        const int row = g + 8 * h;
-        if (quad == 0) {
-          s_m[warp][row] = m[h] == -INFINITY ? (l[h] == 0.f ? -INFINITY : 0.f) : m[h] * p.scale_log2;
-          s_l[warp][row] = l[h];
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = t * 8 + quad * 2 + h;
+          const float sum = over_keys(l[t][h]);
+          if (g == 0) {
+            s_m[warp][row] = m[t][h] == -INFINITY ? (sum == 0.f ? -INFINITY : 0.f)
+                                                  : m[t][h] * p.scale_log2;
+            s_l[warp][row] = sum;
+          }
+          if (row >= rows) continue;
+#pragma unroll
+          for (int dd = 0; dd < D / 16; ++dd)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              s_o[(warp * NT * 8 + row) * LD + dd * 16 + g + e * 8] = o[dd][t][2 * e + h];
         }
-        if (row >= rows) continue;
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-          *reinterpret_cast<float2*>(s_o + (warp * ROWS + row) * D + quad * 2 + n * 8) =
-              make_float2(o[n][2 * h], o[n][2 * h + 1]);
-      }
       warps_all(true);
       for (int x = tid; x < rows * (D / 4); x += DWARPS * 32) {
         const int row = x / (D / 4), d = x % (D / 4) * 4;
@@ -495,7 +532,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         for (int w = 0; w < DWARPS; ++w) {
           if (s_m[w][row] == -INFINITY) continue;           // saw no key: o is not written
           const float f = ex2(s_m[w][row] - M);
-          const float4 v = *reinterpret_cast<const float4*>(s_o + (w * ROWS + row) * D + d);
+          const float4 v = *reinterpret_cast<const float4*>(s_o + (w * NT * 8 + row) * LD + d);
           acc.x = fmaf(v.x, f, acc.x);
           acc.y = fmaf(v.y, f, acc.y);
           acc.z = fmaf(v.z, f, acc.z);
@@ -519,23 +556,25 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     if (!ok) return;                                        // a wait ran out (status is set)
     const int64_t slot = (int64_t(blockIdx.x) + s.unit) * DWARPS + warp;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      const int row = g + 8 * h;
-      if (row >= rows) continue;
-      // None of its keys: only says so.  (Nothing but NaN scores: l = NaN, no maximum.)
-      const bool none = m[h] == -INFINITY && l[h] == 0.f;
-      if (quad == 0)
-        p.ml[slot * p.rows + row] =
-            none ? make_float2(-INFINITY, 0.f)
-                 : make_float2(m[h] == -INFINITY ? 0.f : m[h] * p.scale_log2, l[h]);
-      if (none) continue;
-      float* to = p.opart + (slot * p.rows + row) * D + quad * 2;
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n)
-        *reinterpret_cast<float2*>(to + n * 8) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-    }
+      for (int h = 0; h < 2; ++h) {
+        const int row = t * 8 + quad * 2 + h;
+        const float sum = over_keys(l[t][h]);
+        if (row >= rows) continue;
+        // None of its keys: only says so.  (Nothing but NaN scores: a sum of NaN, no maximum.)
+        const bool none = m[t][h] == -INFINITY && sum == 0.f;
+        if (g == 0)
+          p.ml[slot * p.rows + row] =
+              none ? make_float2(-INFINITY, 0.f)
+                   : make_float2(m[t][h] == -INFINITY ? 0.f : m[t][h] * p.scale_log2, sum);
+        if (none) continue;
+        float* to = p.opart + (slot * p.rows + row) * D + g;
+#pragma unroll
+        for (int dd = 0; dd < D / 16; ++dd)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) to[dd * 16 + e * 8] = o[dd][t][2 * e + h];
+      }
     at += s.n;
   }
 }
@@ -716,7 +755,7 @@ Layout layout_of(const enigma_sdpa_shared_prefix_desc& d) {
                                                           (tiles + 1) / 2)));
   }
   const int64_t p_slots = int64_t(d.heads_kv) * y.pairs * y.splits * 2;
-  y.ctas = y.direct ? int(d_units) : sms * (d.head_dim == 64 ? 3 : 2);
+  y.ctas = y.direct ? int(d_units) : sms * (d.head_dim == 64 ? DCfg<64>::CTAS : DCfg<128>::CTAS);
   const int64_t d_slots = !y.direct      ? (int64_t(y.ctas) + d_units) * DWARPS
                           : y.splits > 0 ? d_units
                                          : 0;
@@ -847,19 +886,22 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
   // A CTA that has the SM to itself needs the whole ring to cover the loads' latency.
   p.stages = y.direct && y.ctas <= enigma::sm_count() ? DCfg<D>::DEEP : DCfg<D>::STAGES;
   const int smem = p.stages * 2 * DCfg<D>::TILE + 1024 + (y.direct ? 0 : int(2 * d.batch + 1) * 4);
-  const auto kernel = y.direct ? paged_decode_kernel<D, true> : paged_decode_kernel<D, false>;
+  const auto kernel = y.rows <= 8 ? (y.direct ? paged_decode_kernel<D, true, 1>
+                                          : paged_decode_kernel<D, false, 1>)
+                              : (y.direct ? paged_decode_kernel<D, true, 2>
+                                          : paged_decode_kernel<D, false, 2>);
   {
     static std::atomic<uint64_t> ready{0};                  // devices where the attribute is set
     int dev = 0;
     e = cudaGetDevice(&dev);
     if (e == cudaSuccess && !(dev < 64 && (ready.load() >> dev & 1))) {
-      e = cudaFuncSetAttribute(paged_decode_kernel<D, true>,
-                               cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               DCfg<D>::DEEP * 2 * DCfg<D>::TILE + 1024);
-      if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(paged_decode_kernel<D, false>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 DCfg<D>::STAGES * 2 * DCfg<D>::TILE + 1024 + 8193 * 4);
+      const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+      const int unit = DCfg<D>::DEEP * 2 * DCfg<D>::TILE + 1024;
+      const int list = DCfg<D>::STAGES * 2 * DCfg<D>::TILE + 1024 + 8193 * 4;
+      e = cudaFuncSetAttribute(paged_decode_kernel<D, true, 1>, attr, unit);
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_decode_kernel<D, true, 2>, attr, unit);
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_decode_kernel<D, false, 1>, attr, list);
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_decode_kernel<D, false, 2>, attr, list);
       if (e == cudaSuccess && dev < 64) ready.fetch_or(uint64_t(1) << dev);
     }
     if (e != cudaSuccess) return e;
