@@ -72,13 +72,14 @@ namespace enigma {
 
 cudaError_t sdpa_packed_launch(const enigma_sdpa_packed_desc& d, cudaStream_t s) {
   cudaError_t e;
-  if (!tc_takes(d)) {
+  const bool tc = tc_takes(d);
+  if (!tc) {
     e = sdpa_packed_simt_launch(d, s);
   } else {
     note_kernel("attn_tc_kernel");
     e = d.head_dim == 128 ? launch<128>(d, s) : launch<64>(d, s);
   }
-  return e == cudaSuccess ? sdpa_packed_join_launch(d, s) : e;
+  return e == cudaSuccess ? sdpa_packed_join_launch(d, tc, s) : e;
 }
 
 }  // namespace enigma

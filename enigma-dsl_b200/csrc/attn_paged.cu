@@ -585,7 +585,7 @@ struct JoinParams {
   int64_t o_batch, o_head;
   int batch, heads_q, heads_kv, group;
   // prefix: pairs x splits items, two states each (0 splits: no prefix)
-  const float* p_opart;
+  const float* p_opart;                    // [slot][D / 8][128][8]
   const float2* p_ml;
   int pairs, splits, row_tiles, tokens;
   // own keys
@@ -611,6 +611,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const JoinParams p) {
   const int kvh = h / p.group, gh = h - kvh * p.group;
   const PrefixRows pr = prefix_rows(p.splits, p.tokens, p.row_tiles, p.pairs, p.group, b, kvh);
   const int64_t p_at = pr.at + gh;
+  const float* p_from = p.p_opart + p_at / BM * BM * D + (lane * V / 8 * BM + p_at % BM) * 8 +
+                        lane * V % 8;
   const int per_b = p.heads_kv * p.blocks, block = gh / p.rows, u = kvh * p.blocks + block;
   const int64_t unit = int64_t(b) * per_b + u;
   int n_d = 1;
@@ -640,7 +642,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const JoinParams p) {
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
       if (base + u >= n) break;
-      const float* from = (base + u < pr.n ? p.p_opart : p.d_opart) + row_at(base + u) * D + lane * V;
+      const float* from = base + u < pr.n ? p_from + int64_t(base + u) * pr.step * D
+                                          : p.d_opart + row_at(base + u) * D + lane * V;
       if constexpr (V == 4) {
         const float4 x = __ldcg(reinterpret_cast<const float4*>(from));
         v[u][0] = x.x, v[u][1] = x.y, v[u][2] = x.z, v[u][3] = x.w;

@@ -318,7 +318,7 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec, const int ro
 // for 72 pairs of tiles in 2 parts).  grid (groups, rows / 32).
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
-packed_join_kernel(const enigma_sdpa_packed_desc p) {
+packed_join_kernel(const enigma_sdpa_packed_desc p, const bool parts_blocked) {
   constexpr int R = 4;
   const int lane = threadIdx.x & 31, D = int(p.head_dim), G = int(p.heads_q / p.heads_kv);
   const int r0 = (int(blockIdx.y) * 8 + (threadIdx.x >> 5)) * R;   // first row, of 2 * 128
@@ -334,6 +334,10 @@ packed_join_kernel(const enigma_sdpa_packed_desc p) {
   if (!__any_sync(0xffffffffu, live)) return;
   const int n = g.parts;
   const int64_t step = 2 * 128, at = int64_t(g.slot + state) * 128;
+  // Element d of row r of a part: [d / 8][r][d % 8] (blocked) or [r][d].
+  const bool blocked = sizeof(T) == 2 && parts_blocked;     // fp32 parts never are
+  const int row = blocked ? 8 : D, v_step = blocked ? 4 * 128 * 8 : 32;
+  const int lane_at = blocked ? lane / 8 * 128 * 8 + lane % 8 : lane;
   griddep_wait();                                                  // the parts are written
   float M = -INFINITY, l = 0.f;
   float acc[R][V];
@@ -356,11 +360,11 @@ packed_join_kernel(const enigma_sdpa_packed_desc p) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         f[r] = __shfl_sync(0xffffffffu, w, r * 8 + y);
-        const float* from = opart + (at + row0 + r + (i0 + y) * step) * D;
+        const float* from = opart + (at + (i0 + y) * step) * D + (row0 + r) * row + lane_at;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           o[r][v] = 0.f;
-          if (f[r] != 0.f && lane + 32 * v < D) o[r][v] = from[lane + 32 * v];
+          if (f[r] != 0.f && lane + 32 * v < D) o[r][v] = from[v * v_step];
         }
       }
 #pragma unroll
@@ -380,9 +384,9 @@ packed_join_kernel(const enigma_sdpa_packed_desc p) {
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const float s = __shfl_sync(0xffffffffu, inv, r * 8);
-    const int64_t row = __shfl_sync(0xffffffffu, to, r * 8);
+    const int64_t to_row = __shfl_sync(0xffffffffu, to, r * 8);
     if (__shfl_sync(0xffffffffu, live ? 1 : 0, r * 8) == 0) continue;
-    T* out = static_cast<T*>(p.out) + row;
+    T* out = static_cast<T*>(p.out) + to_row;
 #pragma unroll
     for (int v = 0; v < V; ++v)
       if (lane + 32 * v < D) store(out + lane + 32 * v, acc[r][v] * s);
@@ -390,10 +394,10 @@ packed_join_kernel(const enigma_sdpa_packed_desc p) {
 }
 
 template <typename T>
-cudaError_t launch_join(const enigma_sdpa_packed_desc& d, const dim3 grid, cudaStream_t s) {
-  if (d.head_dim <= 64) return enigma::launch_dependent(packed_join_kernel<T, 2>, grid, 256, 0, s, d);
-  if (d.head_dim <= 128) return enigma::launch_dependent(packed_join_kernel<T, 4>, grid, 256, 0, s, d);
-  return enigma::launch_dependent(packed_join_kernel<T, 8>, grid, 256, 0, s, d);
+cudaError_t launch_join(const enigma_sdpa_packed_desc& d, const dim3 grid, bool blocked, cudaStream_t s) {
+  if (d.head_dim <= 64) return enigma::launch_dependent(packed_join_kernel<T, 2>, grid, 256, 0, s, d, blocked);
+  if (d.head_dim <= 128) return enigma::launch_dependent(packed_join_kernel<T, 4>, grid, 256, 0, s, d, blocked);
+  return enigma::launch_dependent(packed_join_kernel<T, 8>, grid, 256, 0, s, d, blocked);
 }
 
 template <typename T, int DP>
@@ -476,12 +480,12 @@ cudaError_t sdpa_packed_simt_launch(const enigma_sdpa_packed_desc& d, cudaStream
                                      : launch_packed<__nv_bfloat16>(d, s);
 }
 
-cudaError_t sdpa_packed_join_launch(const enigma_sdpa_packed_desc& d, cudaStream_t s) {
+cudaError_t sdpa_packed_join_launch(const enigma_sdpa_packed_desc& d, bool blocked, cudaStream_t s) {
   const int groups = d.header[enigma_serving::kGroups];
   if (groups == 0) return cudaSuccess;
   const dim3 grid(unsigned(groups), 2 * ENIGMA_PACKED_TILE_ROWS / 32);
-  return d.dtype == ENIGMA_DTYPE_F32 ? launch_join<float>(d, grid, s)
-                                     : launch_join<__nv_bfloat16>(d, grid, s);
+  return d.dtype == ENIGMA_DTYPE_F32 ? launch_join<float>(d, grid, blocked, s)
+                                     : launch_join<__nv_bfloat16>(d, grid, blocked, s);
 }
 
 cudaError_t sdpa_paged_simt_launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {

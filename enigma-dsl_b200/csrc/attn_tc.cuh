@@ -73,7 +73,7 @@ struct Params {
   float scale_log2;
   int group, tokens;               // G, tokens per row tile (G * tokens <= 128)
   uint32_t* status;
-  float* opart;                    // [slot][128][D] fp32, not normalised
+  float* opart;                    // [slot][D / 8][128][8] fp32, not normalised
   float2* ml;                      // [slot][128] (maximum in log2 units, sum)
   // packed prompts
   const int32_t *offsets, *list;   // each CTA's range of items, the items
@@ -188,6 +188,14 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const void* desc, uint64_
       ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(desc)), "r"(smem_u32(bar)), "r"(c0),
         "r"(c1), "r"(c2), "r"(c3)
       : "memory");
+}
+
+// 32 bytes, a sector.
+__device__ __forceinline__ void store_32b(float* to, const uint32_t* x) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]),
+                 "r"(x[6]), "r"(x[7])
+               : "memory");
 }
 
 // The same box fetched into L2 only.
@@ -669,16 +677,18 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           p.ml[row] = none || l == 0.f ? make_float2(-INFINITY, 0.f)
                                        : make_float2(m_used == -INFINITY ? 0.f : m_used * c, l);
         if (n_my > 0) {
+          // A warp's rows side by side, a sector each: with rows of D floats each of a warp's stores
+          // met 32 lines (32 sequences, 4096 shared and up to 512 own keys, 32 / 8 heads of 128:
+          // 21.7 -> 19.8 us; 1325 new tokens against 1 to 4096 keys, split: 60.6 -> 58.8).
+          float* to = p.opart + int64_t(w.slot + ti) * BM * D + r * 8;
 #pragma unroll 1
-          for (int k = 0; k < D; k += 16) {
-            uint32_t o[16];
-            tmem_ld16(o_addr + k, o);
+          for (int k = 0; k < D; k += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + k, o);
             tmem_wait_ld();
             if (live && !none) {
-              uint4* to = reinterpret_cast<uint4*>(p.opart + row * D + k);
 #pragma unroll
-              for (int t2 = 0; t2 < 4; ++t2)
-                to[t2] = make_uint4(o[4 * t2], o[4 * t2 + 1], o[4 * t2 + 2], o[4 * t2 + 3]);
+              for (int t2 = 0; t2 < 32; t2 += 8) store_32b(to + (k + t2) * BM, o + t2);
             }
           }
         }

@@ -72,7 +72,8 @@ cudaError_t qwen_decode_f32_launch(const enigma_qwen_decode_f32_desc& q, cudaStr
 // the CUDA-core kernels.
 cudaError_t sdpa_packed_launch(const enigma_sdpa_packed_desc& d, cudaStream_t s);
 cudaError_t sdpa_packed_simt_launch(const enigma_sdpa_packed_desc& d, cudaStream_t s);
-cudaError_t sdpa_packed_join_launch(const enigma_sdpa_packed_desc& d, cudaStream_t s);
+// blocked: the parts' layout is [slot][D / 8][128][8], else [slot][128][D].
+cudaError_t sdpa_packed_join_launch(const enigma_sdpa_packed_desc& d, bool blocked, cudaStream_t s);
 size_t sdpa_shared_prefix_workspace(const enigma_sdpa_shared_prefix_desc& d);
 cudaError_t sdpa_shared_prefix_launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s);
 cudaError_t sdpa_paged_simt_launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s);
