@@ -709,7 +709,7 @@ constexpr int64_t kFoldBytes = 128ll << 20, kDirectKeys = 1536;
 // Work of less is done one after the other: two streams cost four more host calls.  (32 sequences,
 // 4096 shared and up to 512 own keys, 8 kv heads of 128: 22.1 us side by side, 29.5 one after
 // the other; 128, 32768 and 1024: 117 / 134; 8, 2048 and 128: 12.6 / 13.6.)
-constexpr double kBesideUs = 3.0;
+constexpr double kBesideUs = 3.0, kStepUs = 1.9;
 
 struct Layout {
   int group, tokens, row_tiles, pairs, splits, prefix;    // prefix part
@@ -743,19 +743,26 @@ Layout layout_of(const enigma_sdpa_shared_prefix_desc& d) {
   const int64_t d_units = d.batch * d.heads_kv * y.blocks;
   if (tiles > 0 && !y.fold) {
     // The prefix is bound by the tensor cores, the own keys by memory, which a few SMs can keep
-    // busy: so each gets SMs by its work, side by side.  Per SM, a step of the prefix (128 keys for
-    // 256 rows) takes 1.9 us, own keys come at 0.1 MB/us; half of what the table has room for is taken
-    // as the own keys' number.  Parts of at least two tiles.
+    // busy: so each gets SMs by its work, side by side.  A step of the prefix (128 keys for 256 rows)
+    // takes 1.9 us; an SM draws 0.06 MB/us of own keys beside it, of which half of what the table has
+    // room for is taken as the number.  The number of parts, of two tiles or more, is the one
+    // whose later end is the earliest; over nine shapes within 1 % (6 % at most) of the best number
+    // measured for each, SMs in proportion to the two works 7 % (13 %).
     const int64_t units = int64_t(d.heads_kv) * y.pairs;
-    const double steps = double(d.heads_kv) * double(tiles) * (double(y.pairs) - (y.row_tiles % 2) * 0.5);
-    const double prefix = 1.9 * steps;
     const double own = double(d.batch * d.heads_kv) * double(most - y.prefix) / 2 *
-                       double(d.head_dim) * 4 / 1e5;
-    y.beside = y.direct && (prefix + own) / sms > kBesideUs;
-    const int64_t share = std::max<int64_t>(
-        sms / 4, y.beside ? int64_t(sms * prefix / (prefix + own) + 0.5) : sms);
-    y.splits = int(std::max<int64_t>(1, std::min<int64_t>(share / std::max<int64_t>(units, 1),
-                                                          (tiles + 1) / 2)));
+                       double(d.head_dim) * 4 / 6e4;
+    const int limit = int(std::max<int64_t>(1, std::min<int64_t>(sms / units, (tiles + 1) / 2)));
+    const double half = (y.row_tiles % 2) * 0.5;              // an odd tile fills half an item
+    y.beside = y.direct &&
+               (kStepUs * double(d.heads_kv) * tiles * (y.pairs - half) + own) / sms > kBesideUs;
+    y.splits = limit;
+    if (y.beside) {
+      double best = INFINITY;
+      for (int n = 1; n <= limit && n * units < sms; ++n) {
+        const double end = std::max(kStepUs * double((tiles + n - 1) / n), own / double(sms - n * units));
+        if (end < best) best = end, y.splits = n;
+      }
+    }
   }
   const int64_t p_slots = int64_t(d.heads_kv) * y.pairs * y.splits * 2;
   y.ctas = y.direct ? int(d_units) : sms * (d.head_dim == 64 ? DCfg<64>::CTAS : DCfg<128>::CTAS);
