@@ -198,14 +198,6 @@ __device__ __forceinline__ void store_32b(float* to, const uint32_t* x) {
                : "memory");
 }
 
-// The same box fetched into L2 only.
-__device__ __forceinline__ void prefetch_l2_4d(const void* desc, int32_t c0, int32_t c1, int32_t c2,
-                                               int32_t c3) {
-  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];"
-               ::"l"(reinterpret_cast<uint64_t>(desc)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-               : "memory");
-}
-
 // The number of a page, or `pages` (out of the tensor map's range: reads as zeros) where the
 // table holds none.
 __device__ __forceinline__ int page_at(const int32_t* table, const int32_t* slots, int n_slots,
@@ -319,23 +311,19 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         };
         ok = load_q(0, w.cnt0);
         if (!ok) break;
-        // Paged: lane x knows the page of box x of the next tiles, read AHEAD tiles ahead, and asks
-        // for the tile's bytes in L2 then: two stages cover L2's latency, not HBM's.  One lane
-        // issues all boxes: each lane its own costs 150 cycles a box.
-        constexpr int AHEAD = 3;
-        int at[AHEAD + 1];                   // pages of tiles j .. j + AHEAD
+        // Paged: lane x knows the page of box x of the next tiles; the table is read two tiles ahead.
+        // One lane issues all boxes, each lane its own was no faster; nor does it help to ask for
+        // later tiles' bytes in L2 (128 sequences, 32768 shared keys: 111 us with, 105 without).
+        int at_next = p.pages, at_after = p.pages;   // of tiles j, j + 1
         const bool looks = PAGED && lane < (BN >> p.box_shift);
         auto look_up = [&](int j) {          // the j-th tile of the item; none past its end
           if (!looks || j >= w.all) return p.pages;
           return page_at(p.table, p.slots, p.n_slots, p.width, p.pages, 0,
                          ((w.j0 + j) * BN + (lane << p.box_shift)) >> p.page_shift);
         };
-        auto row_of = [&](int j) {           // first row of this lane's box in its page
-          return ((w.j0 + j) * BN + (lane << p.box_shift)) & ((1 << p.page_shift) - 1);
-        };
         if (PAGED) {
-#pragma unroll
-          for (int x = 0; x <= AHEAD; ++x) at[x] = look_up(x);
+          at_next = look_up(0);
+          at_after = look_up(1);
         }
         for (int j = 0; j < w.all; ++j, ++jg) {
           const int s = jg % ST;
@@ -345,17 +333,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           int at_now = 0;
           if (PAGED) {
             boxes = (min(BN, w.lk - key0) + (1 << p.box_shift) - 1) >> p.box_shift;
-            at_now = at[0];
-#pragma unroll
-            for (int x = 0; x < AHEAD; ++x) at[x] = at[x + 1];
-            at[AHEAD] = look_up(j + AHEAD + 1);
-            if (at[AHEAD - 1] < p.pages) {   // tile j + AHEAD
-#pragma unroll
-              for (int a = 0; a < C::ATOMS; ++a) {
-                prefetch_l2_4d(&tmK, a * 64, row_of(j + AHEAD), w.kvh, at[AHEAD - 1]);
-                prefetch_l2_4d(&tmV, a * 64, row_of(j + AHEAD), w.kvh, at[AHEAD - 1]);
-              }
-            }
+            at_now = at_next;
+            at_next = at_after;
+            at_after = look_up(j + 2);
           }
           const uint32_t bytes = PAGED ? (uint32_t(boxes * C::ATOMS) * 128u) << p.box_shift
                                        : uint32_t(C::KV_BYTES);
