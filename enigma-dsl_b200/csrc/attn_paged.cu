@@ -5,6 +5,8 @@
 // keys are read once for few rows, which is bound by memory: paged_decode_kernel streams them.
 // Both leave partial results (maximum, sum, unnormalised O); paged_join_kernel joins them.
 #include <algorithm>
+#include <mutex>
+#include <new>
 
 #include "attn_tc.cuh"
 
@@ -794,18 +796,74 @@ bool pages_map(CUtensorMap* m, const void* base, const enigma_sdpa_shared_prefix
   return make_map(m, base, 4, dims, strides, box);
 }
 
-// The calling thread's two events on the current device, for a fork to the second stream and back
-// (a wait takes the event's state when it is made, so the next call may record it again).
-cudaError_t fork_events(cudaEvent_t** events) {
-  thread_local cudaEvent_t kept[64][2] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && dev >= 64) e = cudaErrorInvalidDevice;
-  for (int i = 0; i < 2 && e == cudaSuccess; ++i)
-    if (kept[dev][i] == nullptr) e = cudaEventCreateWithFlags(&kept[dev][i], cudaEventDisableTiming);
-  if (e == cudaSuccess) *events = kept[dev];
-  return e;
-}
+// A second stream and the events for a fork to it and back; one call holds it at a time.  A stream
+// that joined a capture belongs to it until the capture ends, so captured calls have their own: a
+// call outside the capture, or in another one, must not meet it.
+struct Side {
+  cudaStream_t stream;
+  cudaEvent_t fork, back;
+  Side* next;
+};
+std::mutex side_mu;
+Side* side_free[64][2];                                     // by device; not captured, captured
+
+class SideHold {
+ public:
+  ~SideHold() {
+    if (side_ == nullptr) return;
+    std::lock_guard<std::mutex> lk(side_mu);
+    side_->next = *list_;
+    *list_ = side_;
+  }
+  // For work that goes back to stream s.
+  cudaError_t take(cudaStream_t s) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && dev >= 64) e = cudaErrorInvalidDevice;
+    if (e != cudaSuccess) return e;
+    cudaStreamCaptureStatus state;
+    unsigned long long id = 0;
+    e = cudaStreamGetCaptureInfo(s, &state, &id);
+    if (e != cudaSuccess) return e;
+    const bool captured = state != cudaStreamCaptureStatusNone;
+    list_ = &side_free[dev][captured];
+    {
+      std::lock_guard<std::mutex> lk(side_mu);
+      for (Side** at = list_; *at != nullptr; at = &(*at)->next) {
+        if (captured) {                                     // free, or in the same capture
+          unsigned long long its = 0;
+          if (cudaStreamGetCaptureInfo((*at)->stream, &state, &its) != cudaSuccess ||
+              (state != cudaStreamCaptureStatusNone && its != id))
+            continue;
+        }
+        side_ = *at;
+        *at = side_->next;
+        return cudaSuccess;
+      }
+    }
+    Side* made = new (std::nothrow) Side{};
+    if (made == nullptr) return cudaErrorMemoryAllocation;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // this is no part of a capture
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    e = cudaStreamCreateWithFlags(&made->stream, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaEventCreateWithFlags(&made->fork, cudaEventDisableTiming);
+    if (e == cudaSuccess) e = cudaEventCreateWithFlags(&made->back, cudaEventDisableTiming);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e == cudaSuccess) {
+      side_ = made;
+      return e;
+    }
+    if (made->fork != nullptr) cudaEventDestroy(made->fork);
+    if (made->stream != nullptr) cudaStreamDestroy(made->stream);
+    delete made;
+    return e;
+  }
+  const Side& operator*() const { return *side_; }
+
+ private:
+  Side* side_ = nullptr;
+  Side** list_ = nullptr;
+};
 
 template <int D>
 cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
@@ -821,10 +879,10 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
   const float scale_log2 = d.scale * 1.4426950408889634f;
   const int page_shift = log2_of(d.page), box_shift = log2_of(box_rows);
   cudaError_t e;
-  cudaEvent_t* fork = nullptr;
+  SideHold side;
   if (y.beside) {
-    e = fork_events(&fork);
-    if (e == cudaSuccess) e = cudaEventRecord(fork[0], s);
+    e = side.take(s);
+    if (e == cudaSuccess) e = cudaEventRecord((*side).fork, s);
     if (e != cudaSuccess) return e;
   }
   if (y.splits > 0) {
@@ -917,16 +975,14 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
     if (e != cudaSuccess) return e;
   }
   if (y.beside) {
-    // On the library's second stream, after the work before this call and before the join, which
-    // waits for it even if the launch failed: a stream that captures must come back.
-    cudaStream_t side = enigma::aux_stream();
-    if (side == nullptr) return cudaErrorMemoryAllocation;
-    e = cudaStreamWaitEvent(side, fork[0], 0);
+    // On a second stream, after the work before this call and before the join, which waits for it
+    // even if the launch failed: a stream that captures must come back.
+    e = cudaStreamWaitEvent((*side).stream, (*side).fork, 0);
     if (e != cudaSuccess) return e;
-    kernel<<<unsigned(y.ctas), DTHREADS, smem, side>>>(mk, mv, p);
+    kernel<<<unsigned(y.ctas), DTHREADS, smem, (*side).stream>>>(mk, mv, p);
     e = cudaGetLastError();
-    cudaError_t back = cudaEventRecord(fork[1], side);
-    if (back == cudaSuccess) back = cudaStreamWaitEvent(s, fork[1], 0);
+    cudaError_t back = cudaEventRecord((*side).back, (*side).stream);
+    if (back == cudaSuccess) back = cudaStreamWaitEvent(s, (*side).back, 0);
     if (e == cudaSuccess) e = back;
   } else if (y.splits > 0) {
     e = enigma::launch_dependent(kernel, unsigned(y.ctas), DTHREADS, smem, s, mk, mv, p);

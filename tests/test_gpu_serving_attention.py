@@ -431,3 +431,36 @@ def test_shared_prefix_side_by_side_in_a_graph_and_on_streams(cuda):
             got.append(cuda_ops.sdpa_shared_prefix(q, kd, vd, td, ld, prefix_len=3000))
     torch.cuda.synchronize()
     assert all(torch.equal(g, short) for g in got)
+
+
+def test_shared_prefix_side_by_side_while_another_stream_captures(cuda):
+    """Two streams per call: a call that is not captured, made between two that are, stays out of the
+    graph, and the graph is whole."""
+    import torch
+    from enigma import cuda_ops
+    rng = np.random.default_rng(22)
+    k, v, table, lens = _paged_case(rng, 40, 3000, [1 + 11 * b for b in range(40)], 64, 4, 128, "bf16")
+    kd, vd = _dev(k, "bf16", cuda), _dev(v, "bf16", cuda)
+    td, ld = torch.from_numpy(table).to(cuda), torch.from_numpy(lens).to(cuda)
+    q = _dev(_values(rng, (40, 16, 128), "bf16"), "bf16", cuda)
+    want = cuda_ops.sdpa_shared_prefix(q, kd, vd, td, ld, prefix_len=3000)
+    workspaces = [torch.empty(64 << 20, dtype=torch.uint8, device=cuda) for _ in range(2)]
+    outs = [torch.zeros_like(want) for _ in range(3)]
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def call(out, workspace):
+        cuda_ops.sdpa_shared_prefix(q, kd, vd, td, ld, prefix_len=3000, out=out, workspace=workspace)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="relaxed"):
+        call(outs[0], workspaces[0])
+        with torch.cuda.stream(other):
+            call(outs[1], workspaces[1])
+        call(outs[2], workspaces[0])
+    torch.cuda.synchronize()
+    assert torch.equal(outs[1], want) and not outs[0].any() and not outs[2].any()
+    outs[1].zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[2], want) and not outs[1].any()
