@@ -599,15 +599,19 @@ struct JoinParams {
 
 // Joins a row's partial results,
 //   O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, M = max_i m_i (m in log2 units),
-// the prefix's in their order, then the own ones.  One warp per (sequence, query head).  It is all
-// latency (L2 answers in half a microsecond, and a row has a few dozen parts): 16 parts' rows are
-// in flight together, the first 16 already beside their (m, l).  A part that saw no key (m = -inf)
-// may hold anything.
-template <int D>
-__global__ void __launch_bounds__(128) paged_join_kernel(const JoinParams p) {
-  constexpr int V = D / 32;
-  const int lane = threadIdx.x & 31;
-  const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 5);     // batch * heads_q < 2^28
+// the prefix's in their order, then the own ones.  It is all latency (L2 answers in half a
+// microsecond): 16 parts' rows are in flight together, the first 16 already beside their (m, l).  A
+// part that saw no key (m = -inf) may hold anything.  A warp per (sequence, query head) where a row
+// has a few dozen parts; WARPS of them, joined in their order, where few rows have hundreds (one
+// sequence of 22250 keys, 15 / 3 heads of 64, 600 parts a row: 68 -> 14 us;
+// two of 40000 shared keys, 8 / 1 heads of 128: 38 -> 18).
+constexpr int kManyParts = 48, kJoinWarps = 16;
+
+template <int D, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) paged_join_kernel(const JoinParams p) {
+  constexpr int V = D / 32, BATCH = 16;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t id = WARPS == 1 ? blockIdx.x * 4 + warp : blockIdx.x;   // batch * heads_q < 2^28
   if (id >= uint32_t(p.batch) * uint32_t(p.heads_q)) return;
   const int b = int(id / uint32_t(p.heads_q)), h = int(id - uint32_t(b) * uint32_t(p.heads_q));
   const int kvh = h / p.group, gh = h - kvh * p.group;
@@ -633,19 +637,22 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const JoinParams p) {
       d_at = (int64_t(first) + unit) * DWARPS * p.rows + (gh - block * p.rows);
     }
   }
-  const int n = pr.n + n_d;
+  // This warp's parts [i0, i0 + n).
+  const int all = pr.n + n_d;
+  const int per = WARPS == 1 ? all : (all + WARPS * BATCH - 1) / (WARPS * BATCH) * BATCH;
+  const int i0 = WARPS == 1 ? 0 : warp * per, n = min(all - i0, per);
   auto row_at = [&](int i) {                       // row of part i in its workspace
     return i < pr.n ? p_at + int64_t(i) * pr.step : d_at + int64_t(i - pr.n) * p.rows;
   };
-  auto ml_at = [&](int i) { return __ldcg((i < pr.n ? p.p_ml : p.d_ml) + row_at(i)); };
-  constexpr int BATCH = 16;
+  auto ml_at = [&](int i) { return __ldcg((i0 + i < pr.n ? p.p_ml : p.d_ml) + row_at(i0 + i)); };
   float v[BATCH][V];
   auto fetch = [&](int base) {
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
       if (base + u >= n) break;
-      const float* from = base + u < pr.n ? p_from + int64_t(base + u) * pr.step * D
-                                          : p.d_opart + row_at(base + u) * D + lane * V;
+      const int i = i0 + base + u;
+      const float* from = i < pr.n ? p_from + int64_t(i) * pr.step * D
+                                   : p.d_opart + row_at(i) * D + lane * V;
       if constexpr (V == 4) {
         const float4 x = __ldcg(reinterpret_cast<const float4*>(from));
         v[u][0] = x.x, v[u][1] = x.y, v[u][2] = x.z, v[u][3] = x.w;
@@ -680,6 +687,25 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const JoinParams p) {
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if constexpr (WARPS > 1) {
+    __shared__ float s_m[WARPS], s_l[WARPS], s_acc[WARPS][D];
+    if (lane == 0) s_m[warp] = M, s_l[warp] = l;
+#pragma unroll
+    for (int x = 0; x < V; ++x) s_acc[warp][lane * V + x] = acc[x];
+    __syncthreads();
+    if (warp > 0) return;
+    for (int y = 1; y < WARPS; ++y) M = fmaxf(M, s_m[y]);
+    l = 0.f;
+#pragma unroll
+    for (int x = 0; x < V; ++x) acc[x] = 0.f;
+    for (int y = 0; y < WARPS; ++y) {
+      if (s_m[y] == -INFINITY) continue;           // no key among its parts
+      const float f = ex2(s_m[y] - M);
+      l = fmaf(s_l[y], f, l);
+#pragma unroll
+      for (int x = 0; x < V; ++x) acc[x] = fmaf(s_acc[y][lane * V + x], f, acc[x]);
+    }
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   __nv_bfloat16* out = p.out + b * p.o_batch + h * p.o_head + lane * V;
 #pragma unroll
@@ -1011,12 +1037,19 @@ cudaError_t launch(const enigma_sdpa_shared_prefix_desc& d, cudaStream_t s) {
   j.blocks = y.blocks;
   j.rows = y.rows;
   j.ctas = y.ctas;
-  const unsigned grid = unsigned((d.batch * d.heads_q + 3) / 4);
+  // Parts of a row: the prefix's (twice as many where one row tile has two softmax states), and four
+  // of each range that its unit's own keys lie in.
+  const int64_t rows = d.batch * d.heads_q, units = d.batch * d.heads_kv * y.blocks;
+  const int64_t parts = y.splits * (y.row_tiles % 2 + 1) +
+                        (y.direct ? 1 : (y.ctas / units + 1) * DWARPS);
+  const bool many = parts > kManyParts && rows <= 4 * enigma::sm_count();
+  const auto join = many ? paged_join_kernel<D, kJoinWarps> : paged_join_kernel<D, 1>;
+  const unsigned grid = unsigned(many ? rows : (rows + 3) / 4), threads = many ? kJoinWarps * 32 : 128;
   if (y.beside) {
-    paged_join_kernel<D><<<grid, 128, 0, s>>>(j);
+    join<<<grid, threads, 0, s>>>(j);
     return cudaGetLastError();
   }
-  return enigma::launch_dependent(paged_join_kernel<D>, grid, 128, 0, s, j);
+  return enigma::launch_dependent(join, grid, threads, 0, s, j);
 }
 
 }  // namespace

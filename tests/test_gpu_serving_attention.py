@@ -464,3 +464,26 @@ def test_shared_prefix_side_by_side_while_another_stream_captures(cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want) and torch.equal(outs[2], want) and not outs[1].any()
+
+
+@pytest.mark.parametrize("batch,prefix,own,page,heads,d", [
+    (1, 0, [22251], 16, (15, 3), 64),
+    (3, 0, [0, 1, 30000], 16, (8, 1), 128),
+    (2, 20000, [5, 300], 64, (8, 1), 128),
+    (4, 9000, [0, 1, 2, 130], 64, (16, 2), 64),
+    (2, 0, [9001, 64], 32, (40, 2), 128),
+])
+def test_shared_prefix_few_rows_of_many_parts(cuda, batch, prefix, own, page, heads, d):
+    """Few sequences with long caches: every SM has a part of each row."""
+    import torch
+    from enigma import cuda_ops
+    rng = np.random.default_rng(23)
+    hq, hk = heads
+    k, v, table, lens = _paged_case(rng, batch, prefix, own, page, hk, d, "bf16")
+    q = _values(rng, (batch, hq, d), "bf16")
+    td, ld = torch.from_numpy(table).to(cuda), torch.from_numpy(lens).to(cuda)
+    args = (_dev(q, "bf16", cuda), _dev(k, "bf16", cuda), _dev(v, "bf16", cuda), td, ld)
+    out = cuda_ops.sdpa_shared_prefix(*args, prefix_len=prefix)
+    assert torch.equal(out, cuda_ops.sdpa_shared_prefix(*args, prefix_len=prefix))
+    ref, mag, _, err = srv.paged(q, k, v, table, lens, prefix, d ** -0.5)
+    _hold(_np(out), ref, mag, err, int(lens.max()), "bf16")
