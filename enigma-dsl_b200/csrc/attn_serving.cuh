@@ -6,8 +6,9 @@
 namespace enigma_serving {
 
 // The plan of a packed batch (enigma_sdpa_packed_plan), as ints: the header, n_ctas + 1 offsets
-// (thread block c works through items [offset[c], offset[c + 1])), the items, the groups.
-enum PlanHeader { kItems, kCtas, kSlots, kGroups, kItemsAt, kGroupsAt, kInts, kReserved };
+// (thread block c works through items [offset[c], offset[c + 1])), the items, the groups.  kLongest:
+// 128-key tiles of the longest item.
+enum PlanHeader { kItems, kCtas, kSlots, kGroups, kItemsAt, kGroupsAt, kInts, kLongest };
 constexpr int kOffsetsAt = ENIGMA_PACKED_PLAN_HEADER;
 
 // One work item: the rows (token, query head of one kv head's group) of up to two consecutive

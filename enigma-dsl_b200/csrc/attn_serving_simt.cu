@@ -7,6 +7,8 @@
 
 namespace {
 
+using enigma_sm100::cluster_ctarank;
+using enigma_sm100::cluster_sync;
 using enigma_sm100::griddep_launch_dependents;
 using enigma_sm100::griddep_wait;
 using enigma_serving::PackedGroup;
@@ -119,11 +121,33 @@ __device__ __forceinline__ void rows_landed() {
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-template <typename T, int DP>
+// What CTA `rank` of the cluster has at this place of its shared memory.
+__device__ __forceinline__ float2 peer2(const float2* p, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(enigma_sm100::mapa_shared(enigma_sm100::smem_u32(p), uint32_t(rank)))
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 peer4(const float* p, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(enigma_sm100::mapa_shared(enigma_sm100::smem_u32(p), uint32_t(rank)))
+               : "memory");
+  return v;
+}
+
+// SPLIT: each block of rows is a cluster of `parts` CTAs, which share its keys (a kernel of its own:
+// one for both took 3 % longer where nothing is split).
+template <typename T, int DP, bool SPLIT>
 __global__ void __launch_bounds__(TT, TileCfg<DP>::CTAS)
-packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec, const int row_blocks) {
+packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec, const int row_blocks,
+                   const int n_parts) {
   using C = TileCfg<DP>;
   constexpr int TK = C::TK, LD = C::LD, KPT = C::KPT;
+  const int parts = SPLIT ? n_parts : 1;
   extern __shared__ float4 smem4[];
   griddep_launch_dependents();
   float* s_q = reinterpret_cast<float*>(smem4);           // [TR][LD]
@@ -132,7 +156,7 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec, const int ro
   float* s_p = s_v + TK * DP;                             // [TK][TR]
   const int tid = threadIdx.x;
   const PackedItem it = reinterpret_cast<const PackedItem*>(
-      p.plan + p.header[enigma_serving::kItemsAt])[blockIdx.x / row_blocks];
+      p.plan + p.header[enigma_serving::kItemsAt])[blockIdx.x / (row_blocks * parts)];
   const int G = int(p.heads_q / p.heads_kv), D = int(p.head_dim), kvh = it.kvh;
   // An item that does not lie inside the tensors is no work of theirs.
   if (it.q0 < 0 || it.q0 + int64_t(it.lq) > p.tokens_q || it.k0 < 0 ||
@@ -141,11 +165,16 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec, const int ro
     return;
   const int n = min(2 * it.tokens, it.lq - it.t0) * G;    // rows of the item
   // An item's row blocks side by side: the heaviest items start first.
-  const int r0 = int(blockIdx.x % row_blocks) * TR;
+  const int r0 = int(blockIdx.x / parts % row_blocks) * TR;
   if (r0 >= n) return;
   const int off = p.causal ? it.lk - it.lq + 1 : it.lk;   // a token's keys: min(lk, token + off)
   const int t_last = it.t0 + (min(r0 + TR, n) - 1) / G;
-  const int k_begin = it.j0 * 128, k_end = min(min(it.lk, t_last + off), it.j1 * 128);
+  int k_begin = it.j0 * 128, k_end = min(min(it.lk, t_last + off), it.j1 * 128);
+  if (SPLIT && k_begin < k_end) {        // this CTA's keys
+    const int rank = int(cluster_ctarank()), tiles = (k_end - k_begin + TK - 1) / TK;
+    k_end = min(k_end, k_begin + tiles * (rank + 1) / parts * TK);
+    k_begin += tiles * rank / parts * TK;
+  }
   const T* kb = static_cast<const T*>(p.k) + it.k0 * p.k_token + kvh * p.k_head;
   const T* vb = static_cast<const T*>(p.v) + it.k0 * p.v_token + kvh * p.v_head;
   // Keys past the end are zeros in K and V; their weights are zero too.
@@ -279,6 +308,66 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec, const int ro
   }
   float* opart = static_cast<float*>(p.workspace);
   float2* ml = reinterpret_cast<float2*>(opart + int64_t(p.header[enigma_serving::kSlots]) * 128 * D);
+  if (SPLIT) {
+    // Each CTA's state into its own shared memory, over Q and K; then each joins its share of the
+    // rows, reading the others' in their order.
+    float2* s_ml = reinterpret_cast<float2*>(s_k);        // [TR]
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+#pragma unroll
+      for (int x = 1; x < 16; x <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
+      const int row = rg * 8 + r;
+      // (Nothing but NaN scores: a sum of NaN, no maximum.)
+      if (cg == 0)
+        s_ml[row] = make_float2(m[r] == -INFINITY ? (l[r] == 0.f ? -INFINITY : 0.f) : m[r] * c_log2,
+                                l[r]);
+#pragma unroll
+      for (int c = 0; c < C::CPT; ++c)
+        s_q[row * LD + c / 4 * 64 + cg * 4 + c % 4] = (r & 1) ? o[r / 2][c].y : o[r / 2][c].x;
+    }
+    cluster_sync();
+    const int share = TR / parts, first = int(cluster_ctarank()) * share;
+    for (int x = tid; x < share * (DP / 4); x += TT) {
+      const int in_block = first + x / (DP / 4), d = x % (DP / 4) * 4, row = r0 + in_block;
+      if (row >= n || d >= D) continue;
+      float M = -INFINITY, L = 0.f;
+      for (int y = 0; y < parts; ++y) M = fmaxf(M, peer2(s_ml + in_block, y).x);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int y = 0; y < parts; ++y) {
+        const float2 a = peer2(s_ml + in_block, y);
+        if (a.x == -INFINITY) continue;                   // saw no key
+        const float f = exp2f(a.x - M);
+        const float4 v = peer4(s_q + in_block * LD + d, y);
+        acc.x = fmaf(v.x, f, acc.x);
+        acc.y = fmaf(v.y, f, acc.y);
+        acc.z = fmaf(v.z, f, acc.z);
+        acc.w = fmaf(v.w, f, acc.w);
+        L = fmaf(a.y, f, L);
+      }
+      const int64_t tok = int64_t(it.q0) + it.t0 + row / G;
+      const int h = kvh * G + row % G;
+      const int tile = row / (it.tokens * G), in_tile = row - tile * it.tokens * G;
+      const int64_t at = (int64_t(it.slot) + tile) * 128 + in_tile;
+      const bool final = it.slot < 0;
+      const float inv = !final ? 1.f : L == 0.f ? 0.f : 1.f / L;
+      const float vv[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+      T* out = static_cast<T*>(p.out) + tok * p.o_token + h * p.o_head + d;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (d + c >= D) continue;
+        if (final) store(out + c, vv[c]);
+        else opart[at * D + d + c] = vv[c];
+      }
+      if (d == 0) {
+        if (!final) ml[at] = make_float2(M, L);
+        else if (p.lse != nullptr)
+          p.lse[tok * p.heads_q + h] = (M + log2f(L)) * 0.6931471805599453f;
+      }
+    }
+    cluster_sync();                          // the others have read
+    return;
+  }
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
 #pragma unroll
@@ -403,9 +492,6 @@ cudaError_t launch_join(const enigma_sdpa_packed_desc& d, const dim3 grid, bool 
 template <typename T, int DP>
 cudaError_t launch_packed(const enigma_sdpa_packed_desc& d, cudaStream_t s) {
   using C = TileCfg<DP>;
-  const cudaError_t e = cudaFuncSetAttribute(
-      packed_simt_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-  if (e != cudaSuccess) return e;
   // Four elements at a time where every row starts on their boundary.
   const int64_t size = 4 * int64_t(sizeof(T));
   bool vec = true;
@@ -415,10 +501,32 @@ cudaError_t launch_packed(const enigma_sdpa_packed_desc& d, cudaStream_t s) {
   const int64_t group = d.heads_q / d.heads_kv;
   const int64_t rows = 2 * std::max<int64_t>(1, ENIGMA_PACKED_TILE_ROWS / group) * group;
   const int row_blocks = int((rows + TR - 1) / TR);
-  const int64_t grid = int64_t(d.header[enigma_serving::kItems]) * row_blocks;
-  if (grid > (int64_t(1) << 31) - 1) return cudaErrorInvalidConfiguration;
-  packed_simt_kernel<T, DP><<<unsigned(grid), TT, C::SMEM, s>>>(d, vec, row_blocks);
-  return cudaGetLastError();
+  const int64_t blocks = int64_t(d.header[enigma_serving::kItems]) * row_blocks;
+  if (blocks > (int64_t(1) << 31) - 1) return cudaErrorInvalidConfiguration;
+  // Where twice as many blocks would still be at most two rounds of what the SMs hold, clusters split
+  // each one's keys, into parts of 128 keys or more (30 tokens against 2000 keys, 8 / 2 heads of 64:
+  // 60 -> 30 us; 295 against 1258, 14 / 2 of 128: 129 -> 78, and unsplit with one round as the limit;
+  // four rounds: 96).
+  int parts = 1;
+  while (parts < 8 && blocks * parts * 2 <= 2 * int64_t(enigma::sm_count()) * C::CTAS &&
+         d.header[enigma_serving::kLongest] >= 2 * parts)
+    parts *= 2;
+  const auto kernel = parts > 1 ? packed_simt_kernel<T, DP, true> : packed_simt_kernel<T, DP, false>;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(unsigned(blocks * parts));
+  c.blockDim = dim3(TT);
+  c.dynamicSmemBytes = C::SMEM;
+  c.stream = s;
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeClusterDimension;
+  a[0].val.clusterDim.x = unsigned(parts);
+  a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
+  c.attrs = a;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, d, vec, row_blocks, parts);
 }
 
 template <typename T>

@@ -118,6 +118,7 @@ std::vector<int32_t> make_packed_plan(const int64_t* lens_q, const int64_t* lens
   out[kItemsAt] = int32_t(items_at);
   out[kGroupsAt] = int32_t(groups_at);
   out[kInts] = int32_t(out.size());
+  out[kLongest] = items.empty() ? 0 : int32_t(steps(items[0]));
   int32_t* to = out.data() + items_at;
   int done = 0;
   for (int c = 0; c < ctas; ++c) {

@@ -487,3 +487,31 @@ def test_shared_prefix_few_rows_of_many_parts(cuda, batch, prefix, own, page, he
     assert torch.equal(out, cuda_ops.sdpa_shared_prefix(*args, prefix_len=prefix))
     ref, mag, _, err = srv.paged(q, k, v, table, lens, prefix, d ** -0.5)
     _hold(_np(out), ref, mag, err, int(lens.max()), "bf16")
+
+
+@pytest.mark.parametrize("lq,lk", [
+    ([30], [2000]), ([1, 1, 1], [500, 3000, 20]), ([5, 0, 9], [1025, 700, 3]), ([40], [4000]),
+    ([64, 3], [257, 1])])
+@pytest.mark.parametrize("heads,d,dtype", [
+    ((8, 2), 64, "f32"), ((4, 4), 128, "f32"), ((3, 1), 200, "f32"), ((8, 2), 80, "bf16"),
+    ((2, 1), 33, "f32")])
+def test_packed_few_rows_of_many_keys(cuda, lq, lk, heads, d, dtype):
+    """Too few rows to fill the SMs: their keys are split inside one launch."""
+    import torch
+    from enigma import cuda_ops
+    hq, hk = heads
+    rng = np.random.default_rng(sum(lk) + d)
+    q = _values(rng, (sum(lq), hq, d), dtype)
+    k = _values(rng, (sum(lk), hk, d), dtype)
+    v = _values(rng, (sum(lk), hk, d), dtype)
+    plan = cuda_ops.PackedPlan(lq, lk, heads_q=hq, heads_kv=hk)
+    args = (_dev(q, dtype, cuda), _dev(k, dtype, cuda), _dev(v, dtype, cuda), plan)
+    out, lse = cuda_ops.sdpa_packed(*args, return_lse=True)
+    again, _ = cuda_ops.sdpa_packed(*args, return_lse=True)
+    assert torch.equal(out, again)
+    ref, mag, rlse, err = srv.packed(q, k, v, lq, lk, d ** -0.5)
+    _hold(_np(out), ref, mag, err, max(lk), dtype)
+    got, empty = _np(lse), np.isinf(rlse)
+    assert (got[empty] == -np.inf).all() and (_np(out)[empty] == 0).all()
+    tol = 4 * (err + (max(lk) + 16) * srv.U32) + 8 * srv.U32 * np.abs(np.where(empty, 0, rlse))
+    assert (np.abs(got[~empty] - rlse[~empty]) <= tol[~empty]).all()
