@@ -734,9 +734,9 @@ int log2_of(int64_t x) {
 }
 
 constexpr int64_t kFoldBytes = 128ll << 20, kDirectKeys = 1536;
-// Work of less is done one after the other: two streams cost four more host calls.  (32 sequences,
-// 4096 shared and up to 512 own keys, 8 kv heads of 128: 22.1 us side by side, 29.5 one after
-// the other; 128, 32768 and 1024: 117 / 134; 8, 2048 and 128: 12.6 / 13.6.)
+// Work of less is done one after the other: two streams cost four more host calls, 10 us.  (32
+// sequences, 4096 shared and up to 512 own keys, 8 kv heads of 128: 19 us side by side, 26 one after
+// the other; 128, 32768 and 1024: 104 / 129; 8, 2048 and 128: 12.1 / 13.4.)
 constexpr double kBesideUs = 3.0, kStepUs = 1.9;
 
 struct Layout {
@@ -758,8 +758,9 @@ Layout layout_of(const enigma_sdpa_shared_prefix_desc& d) {
   const int tiles = (y.prefix + BN - 1) / BN;
   // Short rows: one CTA per unit reads all its keys, the prefix's too, and writes the result; no
   // second launch, no partial results.  Measured (graph, us, so / with the prefix apart): 4 x 512
-  // shared keys, 2 kv heads of 64: 7.9 / 12.4; 16 x 512, 8 of 128: 9.8 / 14.6; 32 x 1024: 16.7 /
-  // 23.8; with longer rows a CTA's chain of chunks is: 8 x 2048: 26 / 12.8, 8 x 2048, 2 of 64: 27 / 13.8.
+  // shared keys, 2 kv heads of 64: 7.4 / 11.3; 16 x 512, 8 of 128: 8.2 / 12.1; 32 x 1024: 13.3 /
+  // 15.8; with longer rows a CTA's chain of chunks is what lasts: 8 x 1400: 13.7 / 11.7 (two launches
+  // more, 4 us of the host), 8 x 2048: 17.4 / 14.1, 8 x 2048, 2 of 64: 15.3 / 11.2.
   const int64_t most = d.table_width * d.page;
   y.fold = y.prefix > 0 && most <= kDirectKeys &&
            d.batch * y.prefix * d.heads_kv * d.head_dim * 4 <= kFoldBytes;
@@ -773,12 +774,13 @@ Layout layout_of(const enigma_sdpa_shared_prefix_desc& d) {
     // The prefix is bound by the tensor cores, the own keys by memory, which a few SMs can keep
     // busy: so each gets SMs by its work, side by side.  A step of the prefix (128 keys for 256 rows)
     // takes 1.9 us; an SM draws 0.06 MB/us of own keys beside it, of which half of what the table has
-    // room for is taken as the number.  The number of parts, of two tiles or more, is the one
+    // room for is taken as the number, and 0.3 us go to a unit's start.  The number of parts, of two tiles or more, is the one
     // whose later end is the earliest; over nine shapes within 1 % (6 % at most) of the best number
     // measured for each, SMs in proportion to the two works 7 % (13 %).
     const int64_t units = int64_t(d.heads_kv) * y.pairs;
-    const double own = double(d.batch * d.heads_kv) * double(most - y.prefix) / 2 *
-                       double(d.head_dim) * 4 / 6e4;
+    const double own = double(d_units) * 0.3 + double(d.batch * d.heads_kv) *
+                                                   double(most - y.prefix) / 2 *
+                                                   double(d.head_dim) * 4 / 6e4;
     const int limit = int(std::max<int64_t>(1, std::min<int64_t>(sms / units, (tiles + 1) / 2)));
     const double half = (y.row_tiles % 2) * 0.5;              // an odd tile fills half an item
     y.beside = y.direct &&
