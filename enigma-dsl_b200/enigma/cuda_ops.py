@@ -214,6 +214,12 @@ def _check_rows(name, dtype, *tensors):
     return _native.DTYPE_F32 if dtype == torch.float32 else _native.DTYPE_BF16
 
 
+def _contiguous_like(q):
+    """An uninitialised contiguous tensor of q's shape (new_empty takes a microsecond longer)."""
+    torch = _torch()
+    return torch.empty_like(q, memory_format=torch.contiguous_format)
+
+
 def _scratch(name, workspace, need, like):
     """(address, bytes) of the caller's workspace or of a new one, and what keeps it alive."""
     if workspace is None:
@@ -270,7 +276,7 @@ def sdpa_packed(q, k, v, plan: PackedPlan, scale: Optional[float] = None, out=No
             plan.heads.clear()
         plan.heads[key] = head
     if out is None:
-        out = q.new_empty(q.shape)
+        out = _contiguous_like(q)
         index = _same_device("sdpa_packed", q, k, v, plan.ints)
     else:
         index = _same_device("sdpa_packed", q, k, v, plan.ints, out)
@@ -339,7 +345,7 @@ def sdpa_shared_prefix(q, k_pages, v_pages, table, lens, prefix_len: int = 0, sl
         None if slots is None else (slots.shape, slots.stride(), slots.dtype),
         None if out is None else (out.shape, out.stride(), out.dtype), prefix_len, scale)
     if out is None:
-        out = q.new_empty(q.shape)
+        out = _contiguous_like(q)
     else:
         _same_device("sdpa_shared_prefix", q, out)
     ws, ws_bytes, keep = _scratch("sdpa_shared_prefix", workspace, need, q)
