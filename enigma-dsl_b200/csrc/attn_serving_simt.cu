@@ -551,14 +551,16 @@ paged_simt_kernel(const enigma_sdpa_shared_prefix_desc p) {
   const int64_t b = blockIdx.y;
   const int kvh = h / int(p.heads_q / p.heads_kv);
   const int64_t slot = p.slots != nullptr ? p.slots[b] : b;
-  const int64_t slot0 = p.slots != nullptr ? p.slots[0] : 0;
-  const bool there = slot >= 0 && slot < p.n_slots && slot0 >= 0 && slot0 < p.n_slots;
+  const int64_t slot0 = p.slots != nullptr ? p.slots[0] : 0;      // the prefix is read through it
+  const bool there = slot >= 0 && slot < p.n_slots, there0 = slot0 >= 0 && slot0 < p.n_slots;
   const int64_t len = there ? min(int64_t(max(p.lens[slot], 0)), p.table_width * p.page) : 0;
   Row<T> row;
   row.start(static_cast<const T*>(p.q) + b * p.q_batch + h * p.q_head, D, lane, p.scale);
   for (int64_t j = warp; j < len; j += kWarps) {
-    const int64_t s = j < p.prefix_len ? slot0 : slot;
-    const int at = p.table[s * p.table_width + j / p.page];
+    const bool shared = j < p.prefix_len;
+    const int at = shared && !there0
+                       ? -1
+                       : p.table[(shared ? slot0 : slot) * p.table_width + j / p.page];
     if (at < 0 || at >= p.pages) continue;                  // not a page: no key
     const int64_t off = (kvh * p.page + j % p.page) * D;
     row.key(static_cast<const T*>(p.k_pages) + at * p.k_page + off,

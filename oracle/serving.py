@@ -51,14 +51,16 @@ def packed(q, k, v, lens_q, lens_k, scale, causal=True):
 
 
 def paged(q, k_pages, v_pages, table, lens, prefix_len, scale, slots=None):
-    """q [B, Hq, D], pages [P, Hkv, page, D] -> out, magnitude, lse, score error."""
+    """q [B, Hq, D], pages [P, Hkv, page, D] -> out, magnitude, lse, score error.
+
+    A slot that does not exist has no keys."""
     hq, hk, page = q.shape[1], k_pages.shape[1], k_pages.shape[2]
     slots = range(len(q)) if slots is None else slots
     out, mag = np.zeros(q.shape), np.zeros(q.shape)
     lse, err = np.zeros(q.shape[:2]), np.zeros(q.shape[:2])
     first = list(slots)[0] if len(q) else 0
     for b, s in enumerate(slots):
-        n = int(lens[s])
+        n = int(lens[s]) if 0 <= s < len(table) else 0
         if n == 0:
             lse[b] = -np.inf
             continue

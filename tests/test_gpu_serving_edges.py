@@ -1,0 +1,62 @@
+"""Edge values of the serving operators on all their kernels: padded slots, tables with holes, NaN and
+what lies behind a length.  The same meaning whatever the type and the head size, against the 64-bit
+oracle under its derived bound (oracle.serving.bound)."""
+import numpy as np
+import pytest
+
+from oracle import numerics as orc
+from oracle import serving as srv
+
+pytestmark = pytest.mark.gpu
+
+# Heads of 64 and 128 in bf16 run on the tensor cores, the others on CUDA cores.
+KINDS = [("f32", 64), ("bf16", 96), ("bf16", 64), ("bf16", 128)]
+
+
+def _values(rng, shape, dtype):
+    x = rng.standard_normal(shape, dtype=np.float32)
+    return orc.bf16_round(x) if dtype == "bf16" else x
+
+
+def _dev(a, dtype, cuda):
+    import torch
+    t = torch.from_numpy(np.ascontiguousarray(a)).to(cuda)
+    return t.bfloat16() if dtype == "bf16" else t
+
+
+def _ints(x, cuda):
+    import torch
+    return torch.tensor(x, dtype=torch.int32, device=cuda)
+
+
+def _paged(cuda, dtype, q, k, v, table, lens, **args):
+    from enigma import cuda_ops
+    slots = args.pop("slots", None)
+    out = cuda_ops.sdpa_shared_prefix(
+        *(_dev(x, dtype, cuda) for x in (q, k, v)), _ints(table, cuda), _ints(lens, cuda),
+        slots=None if slots is None else _ints(slots, cuda), **args)
+    return out.float().cpu().numpy().astype(np.float64)
+
+
+def _hold(got, ref, mag, err, keys, dtype):
+    tol = srv.bound(ref, mag, err, keys, dtype == "bf16")
+    assert np.isfinite(got).all()
+    assert (np.abs(got - ref) <= tol).all(), (np.abs(got - ref) / tol).max()
+
+
+# Table widths in pages of 16: one launch reads the rows, or the prefix and own keys are apart.
+@pytest.mark.parametrize("width", [4, 120])
+@pytest.mark.parametrize("dtype,d", KINDS)
+def test_a_slot_that_does_not_exist_is_alone(cuda, dtype, d, width):
+    """A padded batch: only the padded rows are empty, in first place too."""
+    rng = np.random.default_rng(d + width)
+    k, v = (_values(rng, (9, 2, 16, d), dtype) for _ in range(2))
+    table = np.full((4, width), -1, np.int32)
+    table[:3, :3] = rng.permutation(9).reshape(3, 3)
+    lens = np.array([40, 17, 33, 0], np.int32)
+    q = _values(rng, (4, 8, d), dtype)
+    for slots in ([-1, 0, 2, 1], [4, 1, -7, 2], [0, -1, 1 << 30, 2]):
+        got = _paged(cuda, dtype, q, k, v, table, lens, slots=slots)
+        ref, mag, _, err = srv.paged(q, k, v, table, lens, 0, d ** -0.5, slots)
+        _hold(got, ref, mag, err, 40, dtype)
+        assert [bool((row == 0).all()) for row in got] == [not 0 <= s < 3 for s in slots]
