@@ -46,17 +46,36 @@ struct Row {
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const float m_new = fmaxf(m, s);
-    // A first key whose score is -inf keeps the empty state (no (-inf) - (-inf)).
-    const float base = m_new == -INFINITY ? 0.f : m_new;
-    const float corr = expf(m - base), p = expf(s - base);
-    l = l * corr + p;
+    float corr;
+    const float p = weigh(s, corr);
 #pragma unroll
     for (int t = 0; t < kMaxDPerLane; ++t) {
       const int d = lane + 32 * t;
       if (d < D) acc[t] = fmaf(acc[t], corr, p * load(v + d));
     }
+  }
+  // A key of zeros with a value of zeros: its score is 0 (NaN where q is not finite, as q . 0).
+  __device__ void zero_key() {
+    float s = 0.f;
+#pragma unroll
+    for (int t = 0; t < kMaxDPerLane; ++t) s = fmaf(q[t], 0.f, s);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    float corr;
+    weigh(s, corr);
+#pragma unroll
+    for (int t = 0; t < kMaxDPerLane; ++t) acc[t] *= corr;
+  }
+  // Takes a score into m and l: its weight, and what acc has to be multiplied by before it.
+  __device__ float weigh(float s, float& corr) {
+    const float m_new = fmaxf(m, s);
+    // A first key whose score is -inf keeps the empty state (no (-inf) - (-inf)).
+    const float base = m_new == -INFINITY ? 0.f : m_new;
+    const float p = expf(s - base);
+    corr = expf(m - base);
+    l = l * corr + p;
     m = m_new;
+    return p;
   }
 };
 
@@ -541,7 +560,8 @@ cudaError_t launch_packed(const enigma_sdpa_packed_desc& d, cudaStream_t s) {
 }
 
 // ============================================================================ paged
-// One CTA per (sequence, query head); its warps take every kWarps-th key and merge at the end.
+// One CTA per (sequence, query head); its warps take every kWarps-th key and merge at the end.  A key
+// without a page is one of zeros, as TMA reads it for the tensor-core kernels.
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32)
 paged_simt_kernel(const enigma_sdpa_shared_prefix_desc p) {
@@ -561,7 +581,10 @@ paged_simt_kernel(const enigma_sdpa_shared_prefix_desc p) {
     const int at = shared && !there0
                        ? -1
                        : p.table[(shared ? slot0 : slot) * p.table_width + j / p.page];
-    if (at < 0 || at >= p.pages) continue;                  // not a page: no key
+    if (at < 0 || at >= p.pages) {                          // not a page: reads as zeros
+      row.zero_key();
+      continue;
+    }
     const int64_t off = (kvh * p.page + j % p.page) * D;
     row.key(static_cast<const T*>(p.k_pages) + at * p.k_page + off,
             static_cast<const T*>(p.v_pages) + at * p.v_page + off, D, lane);

@@ -53,7 +53,8 @@ def packed(q, k, v, lens_q, lens_k, scale, causal=True):
 def paged(q, k_pages, v_pages, table, lens, prefix_len, scale, slots=None):
     """q [B, Hq, D], pages [P, Hkv, page, D] -> out, magnitude, lse, score error.
 
-    A slot that does not exist has no keys."""
+    A slot that does not exist has no keys; a key whose table entry is no page, or whose row does
+    not exist (prefix), is a key and a value of zeros."""
     hq, hk, page = q.shape[1], k_pages.shape[1], k_pages.shape[2]
     slots = range(len(q)) if slots is None else slots
     out, mag = np.zeros(q.shape), np.zeros(q.shape)
@@ -64,11 +65,14 @@ def paged(q, k_pages, v_pages, table, lens, prefix_len, scale, slots=None):
         if n == 0:
             lse[b] = -np.inf
             continue
-        at = [(table[first if j < prefix_len else s][j // page], j % page) for j in range(n)]
+        rows = [first if j < prefix_len else s for j in range(n)]
+        at = [(table[r][j // page] if 0 <= r < len(table) else -1, j % page)
+              for j, r in enumerate(rows)]
+        zeros = np.zeros(q.shape[2])
         for h in range(hq):
             kv = h // (hq // hk)
-            k = np.array([k_pages[p, kv, o] for p, o in at]).reshape(n, -1)
-            v = np.array([v_pages[p, kv, o] for p, o in at]).reshape(n, -1)
+            k, v = (np.array([x[p, kv, o] if 0 <= p < len(x) else zeros
+                              for p, o in at]).reshape(n, -1) for x in (k_pages, v_pages))
             o, m, e, x = attend(q[b:b + 1, h], k, v, scale, [n])
             out[b, h], mag[b, h], lse[b, h], err[b, h] = o[0], m[0], e[0], x[0]
     return out, mag, lse, err

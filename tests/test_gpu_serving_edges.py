@@ -60,3 +60,20 @@ def test_a_slot_that_does_not_exist_is_alone(cuda, dtype, d, width):
         ref, mag, _, err = srv.paged(q, k, v, table, lens, 0, d ** -0.5, slots)
         _hold(got, ref, mag, err, 40, dtype)
         assert [bool((row == 0).all()) for row in got] == [not 0 <= s < 3 for s in slots]
+
+
+@pytest.mark.parametrize("width", [4, 120])
+@pytest.mark.parametrize("dtype,d", KINDS)
+def test_a_key_without_a_page_reads_as_zeros(cuda, dtype, d, width):
+    """Holes in a table, page numbers outside the cache, a prefix behind a slot that does not exist:
+    keys and values of zeros, with a weight of their own."""
+    rng = np.random.default_rng(d + width + 1)
+    k, v = (_values(rng, (9, 2, 16, d), dtype) for _ in range(2))
+    table = np.full((3, width), -1, np.int32)
+    table[:, :3] = [[0, -1, 4], [5, 1 << 30, 2], [-1, 8, 9]]
+    lens = np.array([40, 33, 20], np.int32)
+    q = _values(rng, (3, 8, d), dtype)
+    for prefix, slots in ((0, None), (20, None), (20, [1, 0, 2]), (7, [-1, 2, 0]), (39, [9, 1, 0])):
+        got = _paged(cuda, dtype, q, k, v, table, lens, prefix_len=prefix, slots=slots)
+        ref, mag, _, err = srv.paged(q, k, v, table, lens, prefix, d ** -0.5, slots)
+        _hold(got, ref, mag, err, 40, dtype)
