@@ -598,11 +598,12 @@ paged_simt_kernel(const enigma_sdpa_shared_prefix_desc p) {
   __syncthreads();
   float M = -INFINITY, L = 0.f;
   for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w]);
-  for (int w = 0; w < kWarps; ++w) L += s_m[w] == -INFINITY ? 0.f : s_l[w] * expf(s_m[w] - M);
+  // A warp without keys has l = 0; one with nothing but NaN scores has no maximum either, but l = NaN.
+  for (int w = 0; w < kWarps; ++w) L += s_l[w] == 0.f ? 0.f : s_l[w] * expf(s_m[w] - M);
   for (int d = threadIdx.x; d < D; d += kWarps * 32) {
     float o = 0.f;
     for (int w = 0; w < kWarps; ++w)
-      if (s_m[w] != -INFINITY) o = fmaf(s_acc[w][d], expf(s_m[w] - M), o);
+      if (s_l[w] != 0.f) o = fmaf(s_acc[w][d], expf(s_m[w] - M), o);
     store(static_cast<T*>(p.out) + b * p.o_batch + h * p.o_head + d, L == 0.f ? 0.f : o / L);
   }
 }

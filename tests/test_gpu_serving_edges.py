@@ -77,3 +77,35 @@ def test_a_key_without_a_page_reads_as_zeros(cuda, dtype, d, width):
         got = _paged(cuda, dtype, q, k, v, table, lens, prefix_len=prefix, slots=slots)
         ref, mag, _, err = srv.paged(q, k, v, table, lens, prefix, d ** -0.5, slots)
         _hold(got, ref, mag, err, 40, dtype)
+
+
+@pytest.mark.parametrize("width", [4, 120])
+@pytest.mark.parametrize("dtype,d", KINDS)
+def test_nan_reaches_the_rows_that_see_it_paged(cuda, dtype, d, width):
+    """A NaN query, or a NaN in a key that is seen: NaN, not the softmax of the other keys.  The other
+    sequences' results are the same bits as without it."""
+    rng = np.random.default_rng(d + width + 2)
+    k, v = (_values(rng, (9, 2, 16, d), dtype) for _ in range(2))
+    table = np.full((3, width), -1, np.int32)
+    table[:, :3] = rng.permutation(9).reshape(3, 3)
+    q = _values(rng, (3, 8, d), dtype)
+    for lens in ([40, 17, 33], [5, 1, 48]):
+        for prefix in (0, 20):
+            clean = _paged(cuda, dtype, q, k, v, table, lens, prefix_len=prefix)
+            bad = q.copy()
+            bad[1, 2] = np.nan
+            got = _paged(cuda, dtype, bad, k, v, table, lens, prefix_len=prefix)
+            assert np.isnan(got[1, 2]).all()
+            others = np.ones((3, 8), bool)
+            others[1, 2] = False
+            assert (got[others] == clean[others]).all()
+        # Key 4 of sequence 0, kv head 1; with a prefix everybody who has that many keys sees it.
+        bad = k.copy()
+        bad[table[0, 0], 1, 4, 3] = np.nan
+        for prefix in (0, 20):
+            clean = _paged(cuda, dtype, q, k, v, table, lens, prefix_len=prefix)
+            got = _paged(cuda, dtype, q, bad, v, table, lens, prefix_len=prefix)
+            for b in range(3):
+                hit = b == 0 or (prefix > 0 and lens[b] > 4)
+                assert np.isnan(got[b, 4:]).all() if hit else (got[b] == clean[b]).all()
+                assert (got[b, :4] == clean[b, :4]).all()
