@@ -416,7 +416,8 @@ packed_simt_kernel(const enigma_sdpa_packed_desc p, const bool vec, const int ro
     }
     if (cg == 0) {
       if (!final) {
-        ml[at] = make_float2(m[r] * c_log2, l[r]);
+        // (Nothing but NaN scores: a sum of NaN, no maximum.  The part is not empty.)
+        ml[at] = make_float2(m[r] == -INFINITY && l[r] != 0.f ? 0.f : m[r] * c_log2, l[r]);
       } else if (p.lse != nullptr) {
         p.lse[tok * p.heads_q + h] = (m[r] * c_log2 + log2f(l[r])) * 0.6931471805599453f;
       }

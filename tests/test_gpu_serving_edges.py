@@ -109,3 +109,40 @@ def test_nan_reaches_the_rows_that_see_it_paged(cuda, dtype, d, width):
                 hit = b == 0 or (prefix > 0 and lens[b] > 4)
                 assert np.isnan(got[b, 4:]).all() if hit else (got[b] == clean[b]).all()
                 assert (got[b, :4] == clean[b, :4]).all()
+
+
+# Rows whose keys the plan splits, that are split inside one launch (CUDA cores), and that are not.
+@pytest.mark.parametrize("lens_q,lens_k", [([700, 45, 1024, 3], [700, 45, 1024, 3]),
+                                           ([5, 30], [7, 2000]), ([150], [150])])
+@pytest.mark.parametrize("dtype,d", KINDS)
+def test_nan_reaches_the_rows_that_see_it_packed(cuda, dtype, d, lens_q, lens_k):
+    """A NaN query or a NaN in a key that is seen gives NaN in the result and the log-sum-exp; the
+    rows that do not see it keep their bits."""
+    import torch
+    from enigma import cuda_ops
+    rng = np.random.default_rng(d + sum(lens_k))
+    tq, tk = sum(lens_q), sum(lens_k)
+    q, k, v = (_values(rng, (t, h, d), dtype) for t, h in ((tq, 14), (tk, 2), (tk, 2)))
+    plan = cuda_ops.PackedPlan(lens_q, lens_k, heads_q=14, heads_kv=2)
+
+    def run(*arrays):
+        return cuda_ops.sdpa_packed(*(_dev(x, dtype, cuda) for x in arrays), plan, return_lse=True)
+
+    clean, clean_lse = run(q, k, v)
+    at_q, at_k = np.cumsum([0] + lens_q), np.cumsum([0] + lens_k)
+    s = int(np.argmax(lens_k))                     # the longest sequence
+    for where in ("middle query", "last query", "first key", "late key"):
+        hit = torch.zeros(tq, 14, dtype=torch.bool, device=cuda)
+        bad_q, bad_k = q.copy(), k.copy()
+        if where.endswith("query"):
+            row = at_q[s] + (lens_q[s] - 1 if where.startswith("last") else lens_q[s] // 2)
+            bad_q[row, 3] = np.nan
+            hit[row, 3] = True
+        else:
+            j = 0 if where == "first key" else lens_k[s] * 3 // 4
+            bad_k[at_k[s] + j, 1, d // 2] = np.nan
+            first = max(0, j - (lens_k[s] - lens_q[s]))        # the first token that sees key j
+            hit[at_q[s] + first:at_q[s + 1], 7:] = True
+        out, lse = run(bad_q, bad_k, v)
+        assert out[hit].isnan().all() and lse[hit].isnan().all()
+        assert torch.equal(out[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit])
