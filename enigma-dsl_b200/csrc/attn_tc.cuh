@@ -484,7 +484,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     if (ti == 1 && lane == 0) mbar_arrive(&turn[0]);   // state 0 begins
     bool ok = true;
     for (int t = t_begin; t < t_end && ok; ++t) {
-      const Work w = make_work<PAGED>(p, t);
+      Work w = make_work<PAGED>(p, t);
       const int n_my = ti == 0 ? w.cnt0 : w.cnt1;
       const int tok = w.tok0 + (w.alt ? 0 : ti * p.tokens) + r_tok;
       const bool live = r_tok < p.tokens && tok < w.tok_end && (PAGED || tok < p.tokens_q);
@@ -493,6 +493,15 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         keys = PAGED ? min(w.lk, len_of(p.lens, p.slots, p.n_slots,
                                         int64_t(p.width) << p.page_shift, tok))
                      : min(w.lk, tok - w.seq0 + w.off);
+      }
+      // From here on the keys that any row of the item sees, where sequences end before the
+      // prefix does.  Looked for only where no row of this warp sees all of them.
+      if (PAGED && !__any_sync(0xffffffffu, live && keys == w.lk)) {
+        int most = 0;
+        const int end = min(w.tok0 + 2 * p.tokens, w.tok_end);
+        for (int b = w.tok0 + lane; b < end; b += 32)
+          most = max(most, len_of(p.lens, p.slots, p.n_slots, int64_t(p.width) << p.page_shift, b));
+        w.lk = min(w.lk, __reduce_max_sync(0xffffffffu, most));
       }
       float m_used = -INFINITY, l = 0.f;      // m in raw score units
       const int both = min(w.cnt0, w.cnt1);   // tiles that both states have: taken in turns
@@ -587,9 +596,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           if (pass > 0 || !__any_sync(0xffffffffu, need)) break;
           rebase(mx, need);
         }
-        // The sequence's last tile: what lies behind its end in V (a neighbour's tokens, a
-        // page's unwritten rows) may be NaN, and 0 * NaN would reach the sum.  Row r is
-        // cleared here, before P is released; the stage stays until PV has read it.
+        // What lies behind the last key that is seen (a neighbour's tokens, a page's unwritten
+        // rows) may be NaN in V, and 0 * NaN would reach the sum.  Row r is cleared here,
+        // before P is released; the stage stays until PV has read it.
         const int end = w.lk - (w.j0 + tile) * BN;
         if (end < BN) {
           const int st = jg + tile, s = st % ST;

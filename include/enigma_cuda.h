@@ -268,8 +268,9 @@ int32_t enigma_sdpa_packed(const enigma_sdpa_packed_desc* desc, void* stream);
  * sequence b uses row slots[b] (slots NULL: row b).  The first prefix_len keys are the same for
  * the whole batch: they are read once, through the row of sequence 0.  A sequence attends
  * to its first min(lens, table_width * page) keys; none gives zeros, and a slot that does not
- * exist has none.  A key whose table entry is no page is a key and a value of zeros.  scale is
- * positive, page 16, 32, 64 or 128, batch <= 4096.  workspace: caller-owned device memory of
+ * exist has none.  A key whose table entry is no page is a key and a value of zeros.  Keys that
+ * no sequence sees may hold anything; a prefix key that one sequence sees must be finite in v if
+ * another is too short to see it.  scale is positive, page 16, 32, 64 or 128, batch <= 4096.  workspace: caller-owned device memory of
  * enigma_sdpa_shared_prefix_workspace_bytes() bytes, 256-byte aligned. */
 typedef struct enigma_sdpa_shared_prefix_desc {
   int64_t batch, heads_q, heads_kv, head_dim, page, pages, table_width, n_slots, prefix_len;

@@ -146,3 +146,31 @@ def test_nan_reaches_the_rows_that_see_it_packed(cuda, dtype, d, lens_q, lens_k)
         out, lse = run(bad_q, bad_k, v)
         assert out[hit].isnan().all() and lse[hit].isnan().all()
         assert torch.equal(out[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit])
+
+
+@pytest.mark.parametrize("width,prefix", [(4, 60), (120, 60), (120, 700), (120, 1920)])
+@pytest.mark.parametrize("dtype,d", KINDS)
+@pytest.mark.parametrize("lens", [[40] * 5, [40, 0, 7, 33, 12], [0, 0, 50, 0, 1], [1] * 70 + [0, 690],
+                                  [300] * 40 + [5] * 40 + [129, 64], [128, 128], [0, 0]],
+                         ids=lambda x: f"{len(x)}-{max(x)}")
+def test_what_no_sequence_sees_of_the_prefix(cuda, dtype, d, width, prefix, lens):
+    """Sequences that end before the prefix does: what their pages hold behind that (unwritten rows,
+    NaN here) reaches nobody."""
+    lens = [min(n, width * 16) for n in lens]
+    rng = np.random.default_rng(d + width + prefix + len(lens))
+    most, held = max(lens), -(-max(max(lens), min(prefix, 800)) // 16)      # keys seen; pages held
+    k, v = (_values(rng, (held, 2, 16, d), dtype) for _ in range(2))
+    order = rng.permutation(held)
+    for x in (k, v):                               # in the order of the keys: NaN from key `most` on
+        y = np.empty((2, held * 16, d), np.float32)
+        y[:] = x.transpose(1, 0, 2, 3).reshape(2, held * 16, d)
+        y[:, most:] = np.nan
+        x[order] = y.reshape(2, held, 16, d).transpose(1, 0, 2, 3)
+    table = np.full((len(lens), width), -1, np.int32)
+    table[:, :min(width, held)] = order[:width]
+    q = _values(rng, (len(lens), 8, d), dtype)
+    slots = rng.permutation(len(lens))
+    for s in (None, slots):
+        got = _paged(cuda, dtype, q, k, v, table, lens, prefix_len=prefix, slots=s)
+        ref, mag, _, err = srv.paged(q, k, v, table, lens, prefix, d ** -0.5, s)
+        _hold(got, ref, mag, err, max(1, most), dtype)
