@@ -7,6 +7,7 @@ Inputs must be contiguous CUDA tensors; there is no CPU path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import math
@@ -30,9 +31,33 @@ def _torch():
 
 
 def ensure_device(device_index: int) -> None:
+    """Checks and prepares a device on first use; the caller's current device stays current."""
     if device_index not in _initialised:
-        _native.call("enigma_init", device_index)
+        with _torch().cuda.device(device_index):
+            _native.call("enigma_init", device_index)
         _initialised.add(device_index)
+
+
+def _launch(index: int, name: str, *args) -> None:
+    """Calls C entry `name` with device `index` current (the library launches on the current device,
+    whose streams, SM count and status word it takes), and raises if it fails."""
+    torch = _torch()
+    if torch._C._cuda_getDevice() == index:
+        status = getattr(_native.lib(), name)(*args)
+    else:
+        with torch.cuda.device(index):
+            status = getattr(_native.lib(), name)(*args)
+    if status:
+        _native.check(status, name)
+
+
+def _current(device):
+    """A context in which `device` is current, where it names a CUDA device by its number."""
+    torch = _torch()
+    device = torch.device(device)
+    if device.type != "cuda" or device.index is None:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device.index)
 
 
 def _stream_ptr(t) -> int:
@@ -40,7 +65,8 @@ def _stream_ptr(t) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
-def _check_cuda(*ts):
+def _check_cuda(*ts) -> int:
+    """Index of the CUDA device that all tensors are on, contiguous."""
     dev = None
     for t in ts:
         if not t.is_cuda:
@@ -51,7 +77,9 @@ def _check_cuda(*ts):
             dev = t.device
         elif t.device != dev:
             raise ValueError("all tensors must be on the same device")
-    ensure_device(dev.index if dev.index is not None else 0)
+    index = ts[0].get_device()
+    ensure_device(index)
+    return index
 
 
 def _dtype_code(t) -> int:
@@ -68,13 +96,13 @@ def rmsnorm(x, w, eps: float = 1e-6, out=None):
     torch = _torch()
     if out is None:
         out = torch.empty_like(x)
-    _check_cuda(x, w, out)
+    index = _check_cuda(x, w, out)
     hidden = x.shape[-1]
     if w.numel() != hidden or w.dtype != x.dtype or out.dtype != x.dtype:
         raise ValueError("rmsnorm: w must have hidden elements and x's dtype")
     rows = x.numel() // hidden if hidden else 0
-    _native.call("enigma_rmsnorm", _dtype_code(x), x.data_ptr(), w.data_ptr(), out.data_ptr(),
-                 rows, hidden, ctypes.c_float(eps), _stream_ptr(x))
+    _launch(index, "enigma_rmsnorm", _dtype_code(x), x.data_ptr(), w.data_ptr(), out.data_ptr(),
+            rows, hidden, ctypes.c_float(eps), _stream_ptr(x))
     return out
 
 
@@ -94,15 +122,15 @@ def gemm(a, b, out=None, accumulate: bool = False):
         if accumulate:
             raise ValueError("gemm: accumulate=True needs out")
         out = torch.empty((m, n), dtype=a.dtype, device=a.device)
-    _check_cuda(a, b, out)
+    index = _check_cuda(a, b, out)
     if a.dtype == torch.bfloat16:
         if accumulate:
             raise TypeError("gemm: accumulate is fp32-only")
-        _native.call("enigma_gemm_bf16", a.data_ptr(), b.data_ptr(), out.data_ptr(), m, n, k,
-                     _stream_ptr(a))
+        _launch(index, "enigma_gemm_bf16", a.data_ptr(), b.data_ptr(), out.data_ptr(), m, n, k,
+                _stream_ptr(a))
     elif a.dtype == torch.float32:
-        _native.call("enigma_gemm_f32", a.data_ptr(), b.data_ptr(), out.data_ptr(), m, n, k,
-                     int(accumulate), _stream_ptr(a))
+        _launch(index, "enigma_gemm_f32", a.data_ptr(), b.data_ptr(), out.data_ptr(), m, n, k,
+                int(accumulate), _stream_ptr(a))
     else:
         raise TypeError(f"gemm: unsupported dtype {a.dtype}")
     return out
@@ -124,12 +152,12 @@ def sdpa(q, k, v, scale: Optional[float] = None, causal: bool = False, out=None)
         scale = 1.0 / math.sqrt(d)
     if out is None:
         out = torch.empty_like(q)
-    _check_cuda(q, k, v, out)
+    index = _check_cuda(q, k, v, out)
     fn = "enigma_sdpa_bf16" if q.dtype == torch.bfloat16 else "enigma_sdpa_f32"
     if q.dtype not in (torch.bfloat16, torch.float32) or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError("sdpa: Q/K/V must all be bf16 or all fp32")
-    _native.call(fn, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), b, hq, hk, sq, sk,
-                 d, ctypes.c_float(scale), int(causal), _stream_ptr(q))
+    _launch(index, fn, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), b, hq, hk, sq, sk,
+            d, ctypes.c_float(scale), int(causal), _stream_ptr(q))
     return out
 
 
@@ -151,11 +179,13 @@ class PackedPlan:
         c_q, c_k = (ctypes.c_int64 * n)(*lens_q), (ctypes.c_int64 * n)(*lens_k)
         count = ctypes.c_int64()
         args = (c_q, c_k, n, heads_q, heads_kv, int(causal))
-        _native.call("enigma_sdpa_packed_plan", *args, None, 0, ctypes.byref(count))
-        ints = torch.empty(count.value, dtype=torch.int32)
-        _native.call("enigma_sdpa_packed_plan", *args,
-                     ctypes.cast(ints.data_ptr(), ctypes.POINTER(ctypes.c_int32)), count.value,
-                     ctypes.byref(count))
+        # The work is dealt out over the SMs of the plan's device (on the host: as many as a B200 has).
+        with _current(device):
+            _native.call("enigma_sdpa_packed_plan", *args, None, 0, ctypes.byref(count))
+            ints = torch.empty(count.value, dtype=torch.int32)
+            _native.call("enigma_sdpa_packed_plan", *args,
+                         ctypes.cast(ints.data_ptr(), ctypes.POINTER(ctypes.c_int32)), count.value,
+                         ctypes.byref(count))
         self.heads_q, self.heads_kv, self.causal = int(heads_q), int(heads_kv), bool(causal)
         self.tokens_q, self.tokens_k = sum(lens_q), sum(lens_k)
         self.header = tuple(ints[:_native.PACKED_PLAN_HEADER].tolist())
@@ -285,9 +315,7 @@ def sdpa_packed(q, k, v, plan: PackedPlan, scale: Optional[float] = None, out=No
     desc = head[0] + _PACKED_PTRS.pack(plan.ints.data_ptr(), q.data_ptr(), k.data_ptr(),
                                        v.data_ptr(), out.data_ptr(),
                                        lse.data_ptr() if return_lse else 0, ws, ws_bytes)
-    status = _native.lib().enigma_sdpa_packed(desc, _raw_stream(index))
-    if status:
-        _native.check(status, "enigma_sdpa_packed")
+    _launch(index, "enigma_sdpa_packed", desc, _raw_stream(index))
     return (out, lse) if return_lse else out
 
 
@@ -321,8 +349,8 @@ def _shared_head(index, q, k, v, table, lens, slots, out, prefix_len, scale):
                              *q[1][:2], *out[1][:2], k[1][0], v[1][0],
                              1.0 / math.sqrt(d) if scale is None else scale, dtype)
     need = ctypes.c_size_t()
-    _native.call("enigma_sdpa_shared_prefix_workspace_bytes", head + _SHARED_PTRS.pack(*([0] * 9)),
-                 ctypes.byref(need))
+    _launch(index, "enigma_sdpa_shared_prefix_workspace_bytes", head + _SHARED_PTRS.pack(*([0] * 9)),
+            ctypes.byref(need))
     return head, need.value
 
 
@@ -355,13 +383,11 @@ def sdpa_shared_prefix(q, k_pages, v_pages, table, lens, prefix_len: int = 0, sl
                                     0 if slots is None else slots.data_ptr(), q.data_ptr(),
                                     k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), ws,
                                     ws_bytes)
-    status = _native.lib().enigma_sdpa_shared_prefix(desc, _raw_stream(index))
-    if status:
-        _native.check(status, "enigma_sdpa_shared_prefix")
+    _launch(index, "enigma_sdpa_shared_prefix", desc, _raw_stream(index))
     return out
 
 
 def synchronize(device_index: int = 0) -> None:
     """Synchronize the device and raise if a kernel reported a device-side timeout."""
     ensure_device(device_index)
-    _native.call("enigma_synchronize", None)
+    _launch(device_index, "enigma_synchronize", None)

@@ -70,14 +70,16 @@ class DecodeLayer:
         self.w = weights
         self.k_cache, self.v_cache = k_cache, v_cache
         dev = k_cache.device
-        cuda_ops.ensure_device(dev.index or 0)
+        self._index = dev.index or 0
+        cuda_ops.ensure_device(self._index)
         self.position = cfg.cache_len
         self._cos = torch.empty(cfg.head_dim, dtype=torch.float32, device=dev)
         self._sin = torch.empty(cfg.head_dim, dtype=torch.float32, device=dev)
         self._set_rope()
         self.desc = self._desc()
         n = ctypes.c_size_t()
-        _native.call("enigma_decode_workspace_bytes", ctypes.byref(self.desc), ctypes.byref(n))
+        cuda_ops._launch(self._index, "enigma_decode_workspace_bytes", ctypes.byref(self.desc),
+                         ctypes.byref(n))
         self.workspace = torch.empty(n.value, dtype=torch.uint8, device=dev)
 
     @classmethod
@@ -126,11 +128,13 @@ class DecodeLayer:
         the default re-runs the same position (what a benchmark repeats).
         """
         import torch
+        from . import cuda_ops
         if out is None:
             out = torch.empty_like(x)
         s = torch.cuda.current_stream(x.device).cuda_stream
-        _native.call("enigma_decode_layer_bf16", ctypes.byref(self.desc), x.data_ptr(),
-                     out.data_ptr(), self.workspace.data_ptr(), self.workspace.numel(), s)
+        cuda_ops._launch(self._index, "enigma_decode_layer_bf16", ctypes.byref(self.desc),
+                         x.data_ptr(), out.data_ptr(), self.workspace.data_ptr(),
+                         self.workspace.numel(), s)
         if advance:
             if self.position + 1 >= self.cfg.cache_capacity:
                 raise EnigmaError("KV cache full")

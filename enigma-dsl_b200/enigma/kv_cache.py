@@ -98,9 +98,7 @@ class PagedKVCache:
         return values.contiguous()
 
     def _call(self, name, *args):
-        status = getattr(_native.lib(), name)(self._ref, *args, cuda_ops._raw_stream(self._index))
-        if status:
-            _native.check(status, name)
+        cuda_ops._launch(self._index, name, self._ref, *args, cuda_ops._raw_stream(self._index))
 
     def fork(self, parents, children) -> None:
         """Slot children[i] continues slot parents[i]: it lets go of what it held, shares the
