@@ -211,10 +211,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   __shared__ uint64_t full[C::DEEP][2], empty[C::DEEP];   // a stage's chunks for either team
   __shared__ float s_m[DWARPS][ROWS], s_l[DWARPS][ROWS];    // DIRECT
   __shared__ int s_warp[DWARPS + 1], s_pages[PAGES];
+  __shared__ int s_loads;                    // chunks asked for, when the producer is done; else -1
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t most = int64_t(p.width) << p.page_shift;
   griddep_launch_dependents();
 
+  if (tid == 0) s_loads = -1;
   if (tid < ST) {
     mbar_init(&full[tid][0], 1);
     mbar_init(&full[tid][1], 1);
@@ -355,11 +357,24 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       }
       at += s.n;
     }
+    if (lane == 0) *static_cast<volatile int*>(&s_loads) = wraps * ST + st;
     griddep_wait();
     return;
   }
 
   // ------------------------------------------------------------------ consumers
+  // A wait ran out (status is set): the copies in flight land before the block ends.
+  auto give_up = [&] {
+    int loads = -1;
+    for (uint32_t i = 0; i < kSpinLimit && loads < 0; ++i) {
+      loads = *static_cast<volatile int*>(&s_loads);
+      if ((i & 1023u) == 1023u) __nanosleep(64);
+    }
+    for (int n = max(0, loads - ST); n < loads; ++n) {
+      const int uses = ST % 2 == 0 ? n / ST : n / ST >> 1;  // of this barrier before (see below)
+      mbar_drain(&full[n % ST][n & 1], uses & 1);
+    }
+  };
   const int g = lane >> 2, quad = lane & 3;
   const int team = warp >> 1;                               // takes every second chunk
   int turn = 0, st = -1, wraps = 0;                         // whose chunk is next, its stage
@@ -501,7 +516,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     if (DIRECT) {
       // The ring is idle once every warp is here: it takes the warps' states, each thread sums
       // two columns of a row over the warps, in their order.
-      if (!warps_all(ok)) return;                           // a wait ran out (status is set)
+      if (!warps_all(ok)) return give_up();
       constexpr int LD = D + 4;                             // a store's 32 lanes meet 32 banks
       float* s_o = reinterpret_cast<float*>(ring);          // [DWARPS][NT * 8][LD]
 #pragma unroll
@@ -555,7 +570,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       }
       return;
     }
-    if (!ok) return;                                        // a wait ran out (status is set)
+    if (!ok) return give_up();
     const int64_t slot = (int64_t(blockIdx.x) + s.unit) * DWARPS + warp;
 #pragma unroll
     for (int t = 0; t < NT; ++t)

@@ -35,7 +35,8 @@
 // (467 us); P released once, or at 96 keys (470 us).
 //
 // P is rounded to bf16, the operand type of the PV product; sums, maxima and O stay fp32.
-// Every mbarrier wait is bounded (sm100.cuh).
+// Every mbarrier wait is bounded (sm100.cuh).  Whether or not one ran out, a block ends only when its
+// copies have landed and its products are done.
 #pragma once
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -241,7 +242,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   uint64_t* o_done = p_full + 4;             // [2]
   uint64_t* o_free = o_done + 2;             // [2] the epilogue has read O_i
   uint64_t* turn = o_free + 2;               // [2] state i may take the exponential units
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
+  uint64_t* idle = turn + 2;                 // [2] a wait ran out: the products of state i are done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 2);
+  __shared__ int loads[4], gave_up;          // K, V, Q_0, Q_1 tiles asked for; a wait ran out
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -270,8 +273,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       mbar_init(&o_done[i], 1);
       mbar_init(&o_free[i], 128);
       mbar_init(&turn[i], 4);
+      mbar_init(&idle[i], 1);
     }
     fence_barrier_init();
+    gave_up = 0;
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::TMEM_COLS);
@@ -287,6 +292,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     if (warp == 0) {
       // ------------------------------------------------------------ TMA producer
       int jg = 0;                            // key tiles loaded so far
+      int k_loads = 0, v_loads = 0;          // tiles asked for
       int q_items[2] = {0, 0};               // items with work per softmax state
       bool ok = true;
       const uint32_t q_bytes = uint32_t(p.group * p.tokens) * 128u;   // one atom of a Q tile
@@ -363,13 +369,21 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
             __syncwarp();
             return true;
           };
-          if (!load(&tmK, sK + s * C::KV_BYTES, &k_full[s], &k_empty[s]) ||
-              (j == 0 && !load_q(1, w.cnt1)) ||
-              !load(&tmV, sV + s * C::KV_BYTES, &v_full[s], &v_empty[s])) {
-            ok = false;
-            break;
-          }
+          ok = load(&tmK, sK + s * C::KV_BYTES, &k_full[s], &k_empty[s]);
+          if (!ok) break;
+          k_loads = jg + 1;
+          ok = (j > 0 || load_q(1, w.cnt1)) &&
+               load(&tmV, sV + s * C::KV_BYTES, &v_full[s], &v_empty[s]);
+          if (!ok) break;
+          v_loads = jg + 1;
         }
+      }
+      if (lane == 0) {
+        loads[0] = k_loads;
+        loads[1] = v_loads;
+        loads[2] = q_items[0];
+        loads[3] = q_items[1];
+        if (!ok) gave_up = 1;
       }
       __syncwarp();
     } else if (warp <= 2) {
@@ -398,7 +412,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           };
           int st = jg + (w.alt ? i : 0);
           const int step = w.alt ? 2 : 1;
-          auto issue_s = [&](int at) -> bool {
+          auto issue_s = [&](int at) {
             const int sk = at % ST;
             tc_fence_after();
             const uint64_t dk = dk0 + uint64_t((sk * C::KV_BYTES) >> 4);
@@ -408,7 +422,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
               mma_bf16_ss(s_tmem, dq + off, dk + off, idesc_s, kk != 0 ? 1u : 0u);
             }
             mma_commit(&s_full[i]);
-            return true;
           };
           if (n > 0) {
             ok = mbar_wait(&q_full[i], items_done & 1, p.status) &&
@@ -464,6 +477,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           }
           jg += w.all;
         }
+        if (!ok) gave_up = 1;
       }
       __syncwarp();
     }
@@ -689,10 +703,29 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         ++acc_items;
       }
     }
+    if (!ok) gave_up = 1;
   }
 
   tc_fence_before();
   __syncthreads();
+  if (gave_up != 0) {
+    // What was asked for and nobody waited for, before its shared memory and TMEM go back.
+    if (warp == 0) {
+      for (int n = max(0, loads[0] - ST); n < loads[0]; ++n)
+        mbar_drain(&k_full[n % ST], (n / ST) & 1);
+      for (int n = max(0, loads[1] - ST); n < loads[1]; ++n)
+        mbar_drain(&v_full[n % ST], (n / ST) & 1);
+      for (int i = 0; i < 2; ++i)
+        if (loads[2 + i] > 0) mbar_drain(&q_full[i], (loads[2 + i] - 1) & 1);
+    } else if (warp <= 2 && lane == 0) {
+      mma_commit(&idle[warp - 1]);
+      mbar_drain(&idle[warp - 1], 0);
+    } else if (warp >= 4) {
+      tmem_wait_st();
+    }
+    tc_fence_before();
+    __syncthreads();
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, C::TMEM_COLS);

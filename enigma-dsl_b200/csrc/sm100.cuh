@@ -83,6 +83,16 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t phase, uint32_
   return false;
 }
 
+// Bounded wait for what completes by itself (a copy in flight, products that were issued), before a
+// block gives its shared memory or TMEM back.  It does not look at the status word: a copy is still
+// in flight when some wait has run out.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t phase) {
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    if (mbar_try_wait(bar, phase)) return;
+    if ((i & 1023u) == 1023u) __nanosleep(64);
+  }
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const void* desc) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(desc)) : "memory");

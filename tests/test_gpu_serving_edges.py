@@ -174,3 +174,34 @@ def test_what_no_sequence_sees_of_the_prefix(cuda, dtype, d, width, prefix, lens
         got = _paged(cuda, dtype, q, k, v, table, lens, prefix_len=prefix, slots=s)
         ref, mag, _, err = srv.paged(q, k, v, table, lens, prefix, d ** -0.5, s)
         _hold(got, ref, mag, err, max(1, most), dtype)
+
+
+def test_waits_that_give_up(cuda):
+    """With a timeout already reported, waits may give up early: calls made then have no result, but
+    end in order, the report arrives, and the next calls are right."""
+    import torch
+    from enigma import _native, cuda_ops
+    rng = np.random.default_rng(31)
+    lens = [2000, 37, 900]
+    q, k, v = (_dev(_values(rng, (sum(lens), h, 128), "bf16"), "bf16", cuda) for h in (8, 2, 2))
+    plan = cuda_ops.PackedPlan(lens, heads_q=8, heads_kv=2)
+    pages = [_dev(_values(rng, (300, 2, 64, 128), "bf16"), "bf16", cuda) for _ in range(2)]
+    table = _ints([list(range(50)) + list(range(60 + 10 * b, 90 + 10 * b)) for b in range(20)], cuda)
+    rows = _ints([3200 + 90 * b for b in range(20)], cuda)
+
+    def calls():
+        return [cuda_ops.sdpa_packed(q, k, v, plan)] + [
+            cuda_ops.sdpa_shared_prefix(q[:20], *pages, table, n, prefix_len=p)
+            for n, p in ((rows, 3200), (rows, 0), (rows // 4, 0))]
+
+    want = calls()
+    torch.cuda.synchronize()
+    lib = _native.lib()
+    for _ in range(3):
+        _native.check(lib.enigma_check_timeout_path(10, None), "timeout probe")
+        calls()
+        with pytest.raises(_native.EnigmaCudaError, match="exceeded its limit"):
+            cuda_ops.synchronize(0)
+        got = calls()
+        cuda_ops.synchronize(0)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
