@@ -60,8 +60,6 @@ int32_t check_shared(const enigma_sdpa_shared_prefix_desc* d) {
     return bad("sdpa_shared_prefix: sizes must fit in int32");
   if (d->prefix_len < 0 || d->prefix_len > d->table_width * d->page)
     return bad("sdpa_shared_prefix: prefix_len must be in [0, table_width * page]");
-  if (d->slots == nullptr && d->batch > d->n_slots)
-    return bad("sdpa_shared_prefix: more sequences than table rows");
   return ENIGMA_OK;
 }
 
@@ -189,6 +187,8 @@ int32_t enigma_sdpa_shared_prefix(const enigma_sdpa_shared_prefix_desc* d, void*
   const int32_t e = check_shared(d);
   if (e != ENIGMA_OK) return e;
   if (!good_scale(d->scale)) return bad("sdpa_shared_prefix: scale must be positive and finite");
+  if (d->slots == nullptr && d->batch > d->n_slots)
+    return bad("sdpa_shared_prefix: more sequences than table rows");
   if (d->q_batch < 0 || d->q_head < 0 || d->o_batch < 0 || d->o_head < 0 || d->k_page < 0 ||
       d->v_page < 0)
     return bad("sdpa_shared_prefix: negative stride");

@@ -205,3 +205,16 @@ def test_waits_that_give_up(cuda):
         got = calls()
         cuda_ops.synchronize(0)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype,d", KINDS)
+def test_more_queries_than_table_rows(cuda, dtype, d):
+    """Slots may name a row more than once, and padding needs no row of its own."""
+    rng = np.random.default_rng(d + 3)
+    k, v = (_values(rng, (5, 2, 16, d), dtype) for _ in range(2))
+    table, lens, slots = [[3, 1], [3, 4]], [30, 18], [1, 0, 1, 1, -1, 0]
+    q = _values(rng, (6, 8, d), dtype)
+    for prefix in (0, 16):
+        got = _paged(cuda, dtype, q, k, v, np.array(table), lens, prefix_len=prefix, slots=slots)
+        ref, mag, _, err = srv.paged(q, k, v, np.array(table), lens, prefix, d ** -0.5, slots)
+        _hold(got, ref, mag, err, 30, dtype)
