@@ -299,12 +299,30 @@ cache_compact_kernel(const Map m) {
 struct Copy {
   uint8_t *k, *v;
   const int32_t *src, *dst, *fill;     // fill NULL: whole pages
-  const int32_t* count;                // device count, or NULL: n
+  const int32_t* count;                // on the device: copies to make
   int32_t* status;
   int64_t layer_bytes;                 // one layer of K (or V)
   int64_t head_bytes;                  // one head of a page
-  int n, layers, heads, pages, page, row_bytes;   // row_bytes: head_dim * element size
+  int layers, heads, pages, page, row_bytes;      // row_bytes: head_dim * element size
 };
+
+// Pages that a caller names: checked as a whole before any is copied; ws[0] = copies to make.
+__global__ void __launch_bounds__(MAP_THREADS)
+cache_copy_check_kernel(const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int n,
+                        int pages, int32_t* ws, int32_t* status) {
+  griddep_launch_dependents();
+  griddep_wait();
+  bool bad = false;
+  for (int i = threadIdx.x; i < n; i += MAP_THREADS) {
+    const int s = src[i], d = dst[i];
+    bad |= s < 0 || s >= pages || d < 0 || d >= pages;
+  }
+  bad = __syncthreads_or(bad);
+  if (threadIdx.x == 0) {
+    ws[0] = bad ? 0 : n;
+    if (bad) atomicOr(status, ENIGMA_CACHE_BAD_REQUEST);
+  }
+}
 
 // Units of one (copy, layer, K or V, head): fill * row_bytes contiguous bytes.  Bound by HBM; small
 // blocks and many of them, so that the hardware keeps all SMs' requests going: 128 threads, up
@@ -315,8 +333,7 @@ template <typename V>
 __global__ void __launch_bounds__(COPY_THREADS) cache_copy_kernel(const Copy c) {
   griddep_launch_dependents();
   griddep_wait();
-  const int n = c.count != nullptr ? *c.count : c.n;
-  const int64_t units = int64_t(n) * c.layers * 2 * c.heads;
+  const int64_t units = int64_t(*c.count) * c.layers * 2 * c.heads;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int head = int(u % c.heads);
     int64_t r = u / c.heads;
@@ -423,6 +440,7 @@ Map make_map(const enigma_kv_cache_desc& d) {
 
 bool a16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// *count copies (on the device), at most n.
 cudaError_t launch_copy(const enigma_kv_cache_desc& d, const int32_t* src, const int32_t* dst,
                         const int32_t* fill, const int32_t* count, int64_t n, cudaStream_t s) {
   Copy c;
@@ -436,7 +454,6 @@ cudaError_t launch_copy(const enigma_kv_cache_desc& d, const int32_t* src, const
   c.row_bytes = int(d.head_dim * d.elem_bytes);
   c.head_bytes = d.page * c.row_bytes;
   c.layer_bytes = d.pages * d.heads_kv * c.head_bytes;
-  c.n = int(n);
   c.layers = int(d.layers);
   c.heads = int(d.heads_kv);
   c.pages = int(d.pages);
@@ -508,7 +525,10 @@ cudaError_t kv_cache_compact(const enigma_kv_cache_desc& d, cudaStream_t s) {
 cudaError_t kv_cache_copy_pages(const enigma_kv_cache_desc& d, const int32_t* src,
                                 const int32_t* dst, int64_t n, cudaStream_t s) {
   note_kernel("cache_copy_kernel");
-  return launch_copy(d, src, dst, nullptr, nullptr, n, s);
+  const Map m = make_map(d);
+  const cudaError_t e = enigma::launch_dependent(cache_copy_check_kernel, 1, MAP_THREADS, 0, s, src,
+                                                 dst, n, d.pages, m.ws, d.status);
+  return e == cudaSuccess ? launch_copy(d, src, dst, nullptr, m.ws, n, s) : e;
 }
 
 cudaError_t kv_cache_write(const enigma_kv_cache_desc& d, int64_t layer, const void* new_k,

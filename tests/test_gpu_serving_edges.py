@@ -218,3 +218,31 @@ def test_more_queries_than_table_rows(cuda, dtype, d):
         got = _paged(cuda, dtype, q, k, v, np.array(table), lens, prefix_len=prefix, slots=slots)
         ref, mag, _, err = srv.paged(q, k, v, np.array(table), lens, prefix, d ** -0.5, slots)
         _hold(got, ref, mag, err, 30, dtype)
+
+
+def _cache(cuda, rng, pages=8):
+    import torch
+    from enigma.kv_cache import PagedKVCache
+    cache = PagedKVCache.empty(2, pages, 16, 2, 8, slots=4, max_len=64, dtype=torch.float32,
+                               device=cuda)
+    for x in (cache.k, cache.v):
+        x.copy_(torch.from_numpy(rng.standard_normal(x.shape, dtype=np.float32)))
+    return cache
+
+
+def test_copy_pages_is_whole_or_not_at_all(cuda):
+    """One page that does not exist among others that do: nothing is copied."""
+    import torch
+    from enigma import EnigmaError
+    cache = _cache(cuda, np.random.default_rng(41))
+    k, v = cache.k.clone(), cache.v.clone()
+    for src, dst in (([0, 99], [1, 2]), ([0, 1], [2, -1]), ([0, -1, 3], [4, 5, 6]),
+                     ([0, 1, 2, 3], [4, 5, 6, 8])):
+        cache.copy_pages(src, dst)
+        with pytest.raises(EnigmaError, match="does not exist"):
+            cache.check()
+        assert torch.equal(cache.k, k) and torch.equal(cache.v, v)
+    cache.copy_pages([0, 3], [7, 5])
+    cache.check()
+    k[:, 7], k[:, 5], v[:, 7], v[:, 5] = k[:, 0], k[:, 3], v[:, 0], v[:, 3]
+    assert torch.equal(cache.k, k) and torch.equal(cache.v, v)
