@@ -84,7 +84,9 @@ class PagedKVCache:
         """A request as an int32 device tensor (lists and host tensors are copied there)."""
         torch = cuda_ops._torch()
         if not isinstance(values, torch.Tensor):
-            values = torch.as_tensor(values, dtype=torch.int32)
+            values = torch.as_tensor(values)
+            if values.numel() == 0:
+                values = values.int()
         elif values.dtype is torch.int32 and values.get_device() == self._index \
                 and values.dim() == 1 and values.is_contiguous() \
                 and (like is None or values.shape == like.shape):
@@ -93,9 +95,15 @@ class PagedKVCache:
             raise ValueError(f"{name}: expected one number per sequence")
         if like is not None and values.shape != like.shape:
             raise ValueError(f"{name}: the request's parts differ in length")
-        if values.dtype != torch.int32 or values.device != self.k.device:
-            values = values.to(device=self.k.device, dtype=torch.int32)
-        return values.contiguous()
+        if values.dtype != torch.int32:
+            if values.dtype == torch.bool or values.is_floating_point() or values.is_complex():
+                raise TypeError(f"{name}: slots, lengths and pages are whole numbers")
+            # What an int32 does not hold stays out of range: refused here, or on the device.
+            wide, low, high = values.long(), -1 << 31, (1 << 31) - 1
+            if not wide.is_cuda and bool(((wide < low) | (wide > high)).any()):
+                raise ValueError(f"{name}: a number does not fit in int32")
+            values = wide.clamp(low, high).int()
+        return values.to(self.k.device).contiguous()
 
     def _call(self, name, *args):
         cuda_ops._launch(self._index, name, self._ref, *args, cuda_ops._raw_stream(self._index))

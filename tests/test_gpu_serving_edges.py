@@ -246,3 +246,31 @@ def test_copy_pages_is_whole_or_not_at_all(cuda):
     cache.check()
     k[:, 7], k[:, 5], v[:, 7], v[:, 5] = k[:, 0], k[:, 3], v[:, 0], v[:, 3]
     assert torch.equal(cache.k, k) and torch.equal(cache.v, v)
+
+
+def test_requests_are_whole_numbers_of_any_width(cuda):
+    """A slot that an int32 does not hold is not another slot; fractions and masks are no slots."""
+    import torch
+    from enigma import EnigmaError
+    cache = _cache(cuda, np.random.default_rng(42))
+    cache.reserve([0, 1], [20, 5])
+    for bad in (1 << 32, (1 << 32) + 1, -(1 << 33), 1 << 31):
+        cache.free(torch.tensor([bad], device=cuda))
+        with pytest.raises(EnigmaError, match="does not exist"):
+            cache.check()
+        for host in (torch.tensor([bad]), [bad], np.array([bad])):
+            with pytest.raises(ValueError, match="int32"):
+                cache.free(host)
+    cache.reserve([2], torch.tensor([(1 << 32) + 3], device=cuda))
+    with pytest.raises(EnigmaError, match="does not fit"):
+        cache.check()
+    for bad in ([0.7], torch.tensor([0.0], device=cuda), torch.tensor([True]), np.array([1.0])):
+        with pytest.raises(TypeError, match="whole numbers"):
+            cache.free(bad)
+    assert cache.lens.tolist() == [20, 5, 0, 0]
+    for good in ([1], torch.tensor([1]), np.array([1], np.uint8), torch.tensor([1], device=cuda),
+                 torch.tensor([1, 0], dtype=torch.int16, device=cuda)[:1], []):
+        cache.free(good)
+        cache.check()
+        assert cache.lens.tolist() == [20, 0 if len(good) else cache.lens[1].item(), 0, 0]
+        cache.reserve([1], [5])
