@@ -171,6 +171,7 @@ class PagedKVCache:
 
     def check(self) -> None:
         """Waits for the device and raises if a request since the last check was not met."""
+        cuda_ops._torch().cuda.synchronize(self._index)   # requests may run on any stream
         code = int(self.status.item())
         if code:
             self.status.zero_()

@@ -274,3 +274,20 @@ def test_requests_are_whole_numbers_of_any_width(cuda):
         cache.check()
         assert cache.lens.tolist() == [20, 0 if len(good) else cache.lens[1].item(), 0, 0]
         cache.reserve([1], [5])
+
+
+def test_check_waits_for_every_stream(cuda):
+    """A request on another stream that cannot be met is raised, though this stream is idle."""
+    import torch
+    from enigma import EnigmaError
+    cache = _cache(cuda, np.random.default_rng(43))
+    twice = _ints([1, 1], cuda)
+    side = torch.cuda.Stream()
+    for wait in (1000, 200_000_000):               # the first time loads what runs
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(wait)
+            cache.free(twice)
+        with pytest.raises(EnigmaError, match="a slot twice"):
+            cache.check()
+        cache.check()
