@@ -249,7 +249,8 @@ int32_t enigma_kv_cache_write(const enigma_kv_cache_desc* d, int64_t layer, cons
   if (e != ENIGMA_OK) return e;
   if (layer < 0 || layer >= d->layers) return bad("kv_cache: layer out of range");
   if (n < 0 || tokens < 0 || n > kInt31 || tokens > kInt31) return bad("kv_cache: request size");
-  if (n == 0 || tokens == 0) return ENIGMA_OK;
+  if (tokens == 0) return ENIGMA_OK;
+  if (n == 0) return bad("kv_cache: rows without a slot");
   if (new_k == nullptr || new_v == nullptr || strides4 == nullptr || slots == nullptr ||
       starts == nullptr || cu == nullptr)
     return bad("kv_cache: NULL request");

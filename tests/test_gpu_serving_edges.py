@@ -291,3 +291,15 @@ def test_check_waits_for_every_stream(cuda):
         with pytest.raises(EnigmaError, match="a slot twice"):
             cache.check()
         cache.check()
+
+
+def test_rows_without_a_slot_are_refused(cuda):
+    import torch
+    from enigma import _native
+    cache = _cache(cuda, np.random.default_rng(44))
+    rows = torch.zeros(3, 2, 8, device=cuda)
+    with pytest.raises(_native.EnigmaCudaError, match="without a slot"):
+        cache.write(0, rows, rows, [], [], [0])
+    cache.write(0, rows[:0], rows[:0], [], [], [0])          # nothing to write
+    cache.write(0, rows[:0], rows[:0], [1], [0], [0, 0])
+    cache.check()
