@@ -244,6 +244,16 @@ def _check_rows(name, dtype, *tensors):
     return _native.DTYPE_F32 if dtype == torch.float32 else _native.DTYPE_BF16
 
 
+def _dense(shape, stride) -> bool:
+    """Whether the elements lie one after the other; axes of length 1 may have any stride."""
+    step = 1
+    for n, s in zip(reversed(shape), reversed(stride)):
+        if n > 1 and s != step:
+            return 0 in shape
+        step *= n
+    return True
+
+
 def _contiguous_like(q):
     """An uninitialised contiguous tensor of q's shape (new_empty takes a microsecond longer)."""
     torch = _torch()
@@ -339,14 +349,14 @@ def _shared_head(index, q, k, v, table, lens, slots, out, prefix_len, scale):
     elif out[0] != q[0]:
         raise ValueError(f"{name}: out must have q's shape")
     dtype = _check_rows(name, q[2], q, k, v, out)
-    if k[1][1:] != (page * d, d, 1) or v[1][1:] != (page * d, d, 1):
+    if not _dense(k[0][1:], k[1][1:]) or not _dense(v[0][1:], v[1][1:]):
         raise ValueError(f"{name}: a page must be contiguous")
+    k_page, v_page = (x[1][0] if pages > 1 else hk * page * d for x in (k, v))
     for shape, stride, other in (table, lens) + (() if slots is None else (slots,)):
-        dense = stride[-1] == 1 and (len(shape) == 1 or stride[0] == shape[1])
-        if other != int32 or not (dense or 0 in shape):
+        if other != int32 or not _dense(shape, stride):
             raise ValueError(f"{name}: tables, lengths and slots are contiguous int32 tensors")
     head = _SHARED_HEAD.pack(b, hq, hk, d, page, pages, table[0][1], table[0][0], prefix_len,
-                             *q[1][:2], *out[1][:2], k[1][0], v[1][0],
+                             *q[1][:2], *out[1][:2], k_page, v_page,
                              1.0 / math.sqrt(d) if scale is None else scale, dtype)
     need = ctypes.c_size_t()
     _launch(index, "enigma_sdpa_shared_prefix_workspace_bytes", head + _SHARED_PTRS.pack(*([0] * 9)),

@@ -303,3 +303,27 @@ def test_rows_without_a_slot_are_refused(cuda):
     cache.write(0, rows[:0], rows[:0], [], [], [0])          # nothing to write
     cache.write(0, rows[:0], rows[:0], [1], [0], [0, 0])
     cache.check()
+
+
+@pytest.mark.parametrize("dtype,d", KINDS)
+def test_axes_of_length_one_have_any_stride(cuda, dtype, d):
+    """One row of a wider table, one length of several, one kv head seen through a transpose, one
+    page: contiguous whatever the stride of an axis that holds one element."""
+    import torch
+    from enigma import cuda_ops
+    rng = np.random.default_rng(d + 4)
+    k, v = (_dev(_values(rng, (4, 16, 1, d), dtype), dtype, cuda).transpose(1, 2) for _ in range(2))
+    q = _dev(_values(rng, (1, 4, d), dtype), dtype, cuda)
+    table, lens, slots = _ints([[2, 0, 3], [1, 2, 3]], cuda), _ints([30, 7], cuda), _ints([0, 5], cuda)
+    want = cuda_ops.sdpa_shared_prefix(q, k.contiguous(), v.contiguous(),
+                                       table[:1, :2].contiguous().clone(), lens[:1].clone())
+    ref, mag, _, err = srv.paged(q.float().cpu().numpy(), k.float().cpu().numpy(),
+                                 v.float().cpu().numpy(), [[2, 0]], [30], 0, d ** -0.5)
+    _hold(want.float().cpu().numpy().astype(np.float64), ref, mag, err, 30, dtype)
+    got = cuda_ops.sdpa_shared_prefix(q, k, v, table[:1, :2], lens[::2], slots=slots[::2])
+    assert torch.equal(got, want)
+    one = [x[2:3].as_strided((1, 1, 16, d), (7, 3, d, 1)) for x in (k, v)]
+    assert torch.equal(cuda_ops.sdpa_shared_prefix(q, *one, _ints([[0]], cuda), _ints([16], cuda)),
+                       cuda_ops.sdpa_shared_prefix(q, k, v, table[:1, :1], _ints([16], cuda)))
+    with pytest.raises(ValueError, match="int32"):
+        cuda_ops.sdpa_shared_prefix(q, k, v, table[:, :2], lens)
