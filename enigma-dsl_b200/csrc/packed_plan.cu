@@ -22,6 +22,9 @@ constexpr int64_t kItemCost = 2;
 // fp32 partial results.
 constexpr int64_t kMinPart = 4;
 
+// Ints that the items may take in all.
+constexpr int64_t kMaxInts = int64_t(1) << 30;
+
 int64_t steps(const PackedItem& it) { return std::max(0, it.j1 - it.j0); }
 
 }  // namespace
@@ -50,6 +53,8 @@ std::vector<int32_t> make_packed_plan(const int64_t* lens_q, const int64_t* lens
       total += (steps(p) + kItemCost) * heads_kv;
       longest = std::max(longest, steps(p) + kItemCost);
       pairs.push_back(p);
+      // Refused before the list is made: it may not fit in the host's memory either.
+      if (int64_t(pairs.size()) > kMaxInts / kItemInts / heads_kv) return {};
     }
     q0 += lq;
     k0 += lk;
@@ -87,10 +92,9 @@ std::vector<int32_t> make_packed_plan(const int64_t* lens_q, const int64_t* lens
         slots += 2;
         items.push_back(it);
       }
+      if (int64_t(items.size()) > kMaxInts / kItemInts) return {};
     }
   }
-  const int64_t limit = (int64_t(1) << 30);
-  if (int64_t(items.size()) > limit / kItemInts || slots > limit) return {};
   // Heaviest first (equal ones in order: neighbours share K and V), each to the least loaded.
   std::stable_sort(items.begin(), items.end(), [](const PackedItem& x, const PackedItem& y) {
     return steps(x) > steps(y);

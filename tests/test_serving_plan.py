@@ -111,3 +111,26 @@ def test_oracle_attend_is_softmax():
     np.testing.assert_allclose(out[0], w @ v / w.sum(), rtol=1e-12)
     np.testing.assert_allclose(lse[0], np.log(w.sum()), rtol=1e-12)
     assert (out[1] == 0).all() and lse[1] == -np.inf and (mag[0] >= np.abs(out[0])).all()
+
+
+def test_a_plan_that_is_too_large_is_refused_before_it_is_made():
+    """In a process that has no room for it: as an argument that is refused, not by running out."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import ctypes, resource
+resource.setrlimit(resource.RLIMIT_AS, (2 << 30, 2 << 30))
+from enigma import _native
+for heads, tokens in ((65535, (1 << 31) - 300), (65535, 1 << 20)):
+    length, n = (ctypes.c_int64 * 1)(tokens), ctypes.c_int64()
+    rc = _native.lib().enigma_sdpa_packed_plan(length, length, 1, heads, heads, 1, None, 0,
+                                               ctypes.byref(n))
+    print(rc, _native.last_error())
+"""
+    root = Path(__file__).resolve().parents[1] / "enigma-dsl_b200"
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                         timeout=120)
+    lines = out.stdout.splitlines()
+    assert out.returncode == 0 and len(lines) == 2, out.stderr
+    assert all(x.startswith("-4 ") and "too much work" in x for x in lines), lines
