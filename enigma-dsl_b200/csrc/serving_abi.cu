@@ -53,7 +53,7 @@ int32_t check_shared(const enigma_sdpa_shared_prefix_desc* d) {
   if (d->batch < 0 || d->batch > 4096) return bad("sdpa_shared_prefix: batch must be in [0, 4096]");
   if (d->page != 16 && d->page != 32 && d->page != 64 && d->page != 128)
     return bad("sdpa_shared_prefix: page must be 16, 32, 64 or 128");
-  if (d->pages <= 0 || d->table_width <= 0 || d->n_slots <= 0)
+  if (d->pages <= 0 || d->table_width <= 0 || d->n_slots < 0 || (d->n_slots == 0 && d->batch > 0))
     return bad("sdpa_shared_prefix: pages, table_width and n_slots must be positive");
   if (d->pages > kInt31 / (d->heads_kv * d->page) || d->table_width > (kInt31 - 256) / d->page ||
       d->n_slots > kInt31)

@@ -327,3 +327,18 @@ def test_axes_of_length_one_have_any_stride(cuda, dtype, d):
                        cuda_ops.sdpa_shared_prefix(q, k, v, table[:1, :1], _ints([16], cuda)))
     with pytest.raises(ValueError, match="int32"):
         cuda_ops.sdpa_shared_prefix(q, k, v, table[:, :2], lens)
+
+
+@pytest.mark.parametrize("dtype,d", KINDS)
+def test_an_empty_batch(cuda, dtype, d):
+    """No sequences, with or without table rows: an empty result."""
+    import torch
+    from enigma import cuda_ops
+    k = torch.zeros(4, 2, 16, d, device=cuda, dtype=torch.float32 if dtype == "f32" else torch.bfloat16)
+    q, table, lens = k.new_zeros(0, 8, d), _ints([[0, 1], [2, 3]], cuda), _ints([5, 20], cuda)
+    for rows in (2, 0):
+        for prefix in (0, 20):
+            out = cuda_ops.sdpa_shared_prefix(q, k, k, table[:rows], lens[:rows], prefix_len=prefix)
+            assert out.shape == (0, 8, d) and out.dtype == k.dtype
+    out = cuda_ops.sdpa_shared_prefix(q, k, k, table, lens, slots=lens[:0])
+    assert out.shape == (0, 8, d)
