@@ -46,36 +46,30 @@ struct Row {
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    float corr;
-    const float p = weigh(s, corr);
+    const float m_new = fmaxf(m, s);
+    // A first key whose score is -inf keeps the empty state (no (-inf) - (-inf)).
+    const float base = m_new == -INFINITY ? 0.f : m_new;
+    const float corr = expf(m - base), p = expf(s - base);
+    l = l * corr + p;
 #pragma unroll
     for (int t = 0; t < kMaxDPerLane; ++t) {
       const int d = lane + 32 * t;
       if (d < D) acc[t] = fmaf(acc[t], corr, p * load(v + d));
     }
+    m = m_new;
   }
-  // A key of zeros with a value of zeros: its score is 0 (NaN where q is not finite, as q . 0).
-  __device__ void zero_key() {
+  // n keys of zeros with values of zeros: their score is 0 (NaN where q is not finite, as q . 0).
+  __device__ void zero_keys(int n) {
     float s = 0.f;
 #pragma unroll
     for (int t = 0; t < kMaxDPerLane; ++t) s = fmaf(q[t], 0.f, s);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    float corr;
-    weigh(s, corr);
+    const float m_new = fmaxf(m, s), corr = expf(m - m_new);
+    l = l * corr + float(n) * expf(s - m_new);
 #pragma unroll
     for (int t = 0; t < kMaxDPerLane; ++t) acc[t] *= corr;
-  }
-  // Takes a score into m and l: its weight, and what acc has to be multiplied by before it.
-  __device__ float weigh(float s, float& corr) {
-    const float m_new = fmaxf(m, s);
-    // A first key whose score is -inf keeps the empty state (no (-inf) - (-inf)).
-    const float base = m_new == -INFINITY ? 0.f : m_new;
-    const float p = expf(s - base);
-    corr = expf(m - base);
-    l = l * corr + p;
     m = m_new;
-    return p;
   }
 };
 
@@ -577,19 +571,24 @@ paged_simt_kernel(const enigma_sdpa_shared_prefix_desc p) {
   const int64_t len = there ? min(int64_t(max(p.lens[slot], 0)), p.table_width * p.page) : 0;
   Row<T> row;
   row.start(static_cast<const T*>(p.q) + b * p.q_batch + h * p.q_head, D, lane, p.scale);
-  for (int64_t j = warp; j < len; j += kWarps) {
-    const bool shared = j < p.prefix_len;
-    const int at = shared && !there0
-                       ? -1
-                       : p.table[(shared ? slot0 : slot) * p.table_width + j / p.page];
+  int zeros = 0;                                            // keys of this warp without a page
+  int64_t j = warp;
+  if (!there0 && j < min(len, p.prefix_len)) {
+    zeros = int((min(len, p.prefix_len) - j + kWarps - 1) / kWarps);
+    j += int64_t(zeros) * kWarps;
+  }
+  for (; j < len; j += kWarps) {
+    const int64_t s = j < p.prefix_len ? slot0 : slot;
+    const int at = p.table[s * p.table_width + j / p.page];
     if (at < 0 || at >= p.pages) {                          // not a page: reads as zeros
-      row.zero_key();
+      ++zeros;
       continue;
     }
     const int64_t off = (kvh * p.page + j % p.page) * D;
     row.key(static_cast<const T*>(p.k_pages) + at * p.k_page + off,
             static_cast<const T*>(p.v_pages) + at * p.v_page + off, D, lane);
   }
+  if (zeros > 0) row.zero_keys(zeros);
 #pragma unroll
   for (int x = 0; x < kMaxDPerLane; ++x) s_acc[warp][lane + 32 * x] = row.acc[x];
   if (lane == 0) {
