@@ -771,16 +771,16 @@ Layout layout_of(const enigma_sdpa_shared_prefix_desc& d) {
   y.row_tiles = int((d.batch + y.tokens - 1) / y.tokens);
   y.pairs = (y.row_tiles + 1) / 2;
   const int tiles = (y.prefix + BN - 1) / BN;
-  // Short rows: one CTA per unit reads all its keys, the prefix's too, and writes the result; no
-  // second launch, no partial results.  Measured (graph, us, so / with the prefix apart): 4 x 512
+  // Short rows (by the table's width: lengths are on the device): one CTA per unit reads all its
+  // keys, the prefix's too, and writes the result; no second launch, no partial results.  Measured (graph, us, so / with the prefix apart): 4 x 512
   // shared keys, 2 kv heads of 64: 7.4 / 11.3; 16 x 512, 8 of 128: 8.2 / 12.1; 32 x 1024: 13.3 /
   // 15.8; with longer rows a CTA's chain of chunks is what lasts: 8 x 1400: 13.7 / 11.7 (two launches
   // more, 4 us of the host), 8 x 2048: 17.4 / 14.1, 8 x 2048, 2 of 64: 15.3 / 11.2.
   const int64_t most = d.table_width * d.page;
   y.fold = y.prefix > 0 && most <= kDirectKeys &&
            d.batch * y.prefix * d.heads_kv * d.head_dim * 4 <= kFoldBytes;
-  // A CTA per unit reads the own keys where no row has many of them; else they are split over the
-  // SMs.  Where the prefix is apart, a third launch joins the parts of both.
+  // A CTA per unit reads the own keys where no row has room for many of them; else they are split over
+  // the SMs (32 x 4096 shared and up to 512 own keys in a table of 4608: 19.5 us, of 8192: 37).  Where the prefix is apart, a third launch joins the parts of both.
   y.direct = y.fold || most - y.prefix <= kDirectKeys;
   y.blocks = (y.group + ROWS - 1) / ROWS;
   y.rows = (y.group + y.blocks - 1) / y.blocks;
@@ -789,9 +789,10 @@ Layout layout_of(const enigma_sdpa_shared_prefix_desc& d) {
     // The prefix is bound by the tensor cores, the own keys by memory, which a few SMs can keep
     // busy: so each gets SMs by its work, side by side.  A step of the prefix (128 keys for 256 rows)
     // takes 1.9 us; an SM draws 0.06 MB/us of own keys beside it, of which half of what the table has
-    // room for is taken as the number, and 0.3 us go to a unit's start.  The number of parts, of two tiles or more, is the one
-    // whose later end is the earliest; over nine shapes within 1 % (6 % at most) of the best number
-    // measured for each, SMs in proportion to the two works 7 % (13 %).
+    // room for is taken as the number, and 0.3 us go to a unit's start.  The number of parts, of two
+    // tiles or more, is the one whose later end is the earliest; over nine shapes, each table as wide
+    // as its longest sequence, within 1 % (6 % at most) of the best number measured for each, SMs in
+    // proportion to the two works 7 % (13 %).
     const int64_t units = int64_t(d.heads_kv) * y.pairs;
     const double own = double(d_units) * 0.3 + double(d.batch * d.heads_kv) *
                                                    double(most - y.prefix) / 2 *

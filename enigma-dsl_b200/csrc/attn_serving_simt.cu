@@ -78,11 +78,13 @@ struct Row {
 // with 8 rows x TK / 16 keys of S and 8 rows x DP / 16 columns of O.  Products run on the packed
 // fp32 FMA: S over pairs of the head dimension, so that neither operand has to be doubled, O over
 // pairs of rows.  K of the next tile is fetched while the softmax and P V run, V while S does.
-// Bound by what comes out of shared memory: a warp's 16-byte load is 512 bytes through the SM's
-// 128-byte port, even where lanes read the same, so S takes 12 loads = 48 cycles of it per warp for
-// 64 FMAs = 140 cycles of one of four FMA pipes (192 against 140 for the four), O the same (1772
-// tokens in 4 prompts, 14 / 2 heads of 64, causal: 126 us; 4096, 8 / 8: 547 us = 31 TFLOP/s).  Tiles
-// of 8 x 8 per thread load less, but registers leave too few warps: 10 to 20 % more time.
+// What comes out of shared memory holds the products up: a warp's 16-byte load is 512 bytes through
+// the SM's 128-byte port, even where lanes read the same, so S takes 12 loads = 48 cycles of it per
+// warp for 64 FMAs = 140 cycles of one of four FMA pipes (192 against 140 for the four), O the same.
+// 1772 tokens in 4 prompts, 14 / 2 heads of 64, causal: 126 us; 4096, 8 / 8: 547 us = 31 TFLOP/s, 2.4
+// times what the FMAs need, of which the port explains 1.37; the rest (two barriers and a softmax
+// between the products of a tile, 8 warps on an SM) is not taken apart.  Tiles of 8 x 8 per thread
+// load less, but registers leave too few warps: 10 to 20 % more time.
 constexpr int TR = 64, TT = 128;
 
 template <int DP>
@@ -556,7 +558,11 @@ cudaError_t launch_packed(const enigma_sdpa_packed_desc& d, cudaStream_t s) {
 
 // ============================================================================ paged
 // One CTA per (sequence, query head); its warps take every kWarps-th key and merge at the end.  A key
-// without a page is one of zeros, as TMA reads it for the tensor-core kernels.
+// without a page is one of zeros, as TMA reads it for the tensor-core kernels.  The simple form: every
+// query head reads K and V, the prefix too, for itself, a key costs a warp one dependent chain (dot
+// product, five shuffles, two exponentials, rescale), and long rows are not split.  That chain is the
+// time, not memory: 16 sequences of 1 to 8191 keys, 32 / 8 heads of 128, fp32: 1808 us against 82 for
+// the bytes; one of 22250 keys: 4809 against 28.
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32)
 paged_simt_kernel(const enigma_sdpa_shared_prefix_desc p) {

@@ -371,8 +371,10 @@ def sdpa_shared_prefix(q, k_pages, v_pages, table, lens, prefix_len: int = 0, sl
     q [B, Hq, D]; k_pages / v_pages [pages, Hkv, page, D] (one layer of a cache); table
     [n, width] int32 page numbers, lens [n] int32; sequence b uses row slots[b] (default: row
     b).  Sequence b attends to its first lens keys; those below prefix_len are the same for
-    the whole batch and are read once for all, through sequence 0's row.  A sequence without
-    keys gives zeros.  workspace: a uint8 tensor to use instead of an allocation per call (as
+    the whole batch and are read through sequence 0's row, for many sequences at once on the tensor
+    cores (bf16, heads of 64 or 128, aligned rows).  A sequence without keys gives zeros.  Which kernels run
+    depends on the table's width, the most keys that a row could hold: a table no wider than its
+    sequences need is faster.  workspace: a uint8 tensor to use instead of an allocation per call (as
     many bytes as enigma_sdpa_shared_prefix_workspace_bytes says).  Returns out [B, Hq, D].
     """
     index = _same_device("sdpa_shared_prefix", q, k_pages, v_pages, table, lens)

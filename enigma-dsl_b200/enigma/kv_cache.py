@@ -129,7 +129,10 @@ class PagedKVCache:
 
     def write(self, layer: int, new_k, new_v, slots, starts, cu) -> None:
         """Rows cu[i] .. cu[i + 1] of new_k / new_v [tokens, heads_kv, head_dim] are tokens
-        starts[i], starts[i] + 1, ... of slot slots[i] in `layer` (reserved before)."""
+        starts[i], starts[i] + 1, ... of slot slots[i] in `layer` (reserved before).
+
+        A slot may append whoever shares its pages; writing over tokens of a full page that a fork
+        shares changes them for all who hold the page."""
         shape, ks, vs = new_k.shape, new_k.stride(), new_v.stride()
         if len(shape) != 3 or shape != new_v.shape or shape[1:] != self._row:
             raise ValueError(f"write: expected rows [tokens, {self._row[0]}, {self._row[1]}]")

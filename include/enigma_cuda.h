@@ -266,9 +266,12 @@ int32_t enigma_sdpa_packed(const enigma_sdpa_packed_desc* desc, void* stream);
  * [pages, heads_kv, page, head_dim] (contiguous but for the page strides, in elements);
  * table [n_slots, table_width] int32 page numbers, lens [n_slots] int32 keys of each sequence;
  * sequence b uses row slots[b] (slots NULL: row b).  The first prefix_len keys are the same for
- * the whole batch: they are read once, through the row of sequence 0.  A sequence attends
- * to its first min(lens, table_width * page) keys; none gives zeros, and a slot that does not
- * exist has none.  A key whose table entry is no page is a key and a value of zeros.  Keys that
+ * the whole batch: they are read through the row of sequence 0.  bf16 with heads of 64 or 128,
+ * strides of multiples of 8 and 16-byte aligned buffers runs on the tensor cores, which read a
+ * prefix once for every 256 rows (sequence, query head) of a kv head, in tables of at most 1536
+ * keys once per sequence and kv head; other calls read it once per sequence and query head.  A
+ * sequence attends to its first min(lens, table_width * page) keys; none gives zeros, and a slot
+ * that does not exist has none.  A key whose table entry is no page is a key and a value of zeros.  Keys that
  * no sequence sees may hold anything; a prefix key that one sequence sees must be finite in v if
  * another is too short to see it.  scale is positive, page 16, 32, 64 or 128, batch <= 4096.  workspace: caller-owned device memory of
  * enigma_sdpa_shared_prefix_workspace_bytes() bytes, 256-byte aligned. */
@@ -298,9 +301,12 @@ int32_t enigma_sdpa_shared_prefix(const enigma_sdpa_shared_prefix_desc* desc, vo
  *   reserve  slots[i] grows to lens[i] tokens.
  *   write    rows of new_k / new_v (strides4: k token, k head, v token, v head, in elements)
  *            of one layer: rows cu[i] .. cu[i + 1] are tokens starts[i], ... of slots[i];
- *            a token without a page is left out and sets ENIGMA_CACHE_BAD_REQUEST.
+ *            a token without a page is left out and sets ENIGMA_CACHE_BAD_REQUEST.  A page that
+ *            forks share (a full one) is written for all of them: appending never meets one,
+ *            writing over earlier tokens may.
  *   compact  the n live pages take the numbers below n; rows are rewritten to match.
- *   copy_pages  whole pages src[i] -> dst[i], all layers; no page both source and destination.
+ *   copy_pages  whole pages src[i] -> dst[i], all layers; no page both source and destination
+ *            (that is not checked, numbers out of range are).
  * workspace: enigma_kv_cache_workspace_bytes() bytes; calls that share it run in one order. */
 #define ENIGMA_CACHE_FULL 1
 #define ENIGMA_CACHE_BAD_REQUEST 2
