@@ -57,6 +57,8 @@ cudaError_t launch(const enigma_sdpa_packed_desc& d, cudaStream_t s) {
   p.o_token = d.o_token;
   p.o_head = d.o_head;
   p.heads_q = int(d.heads_q);
+  p.heads_kv = int(d.heads_kv);
+  p.slots_end = std::max(1, d.header[kSlots]);
   p.causal = d.causal != 0;
   p.one = d.header[kItems] == d.header[kCtas];
   p.tokens_q = int(d.tokens_q);

@@ -439,7 +439,10 @@ packed_join_kernel(const enigma_sdpa_packed_desc p, const bool parts_blocked) {
   const int state = r0 / 128;
   const int row0 = r0 % 128, mine = row0 + (lane >> 3);            // this lane's row of (m, l)
   const int tok = g.tok0 + state * g.tokens + mine / G;
-  const bool live = mine < g.tokens * G && tok < g.tok_end && tok < p.tokens_q;
+  // (A group that does not lie inside the tensors or the parts is none of theirs.)
+  const bool live = mine < g.tokens * G && tok >= 0 && tok < g.tok_end && tok < p.tokens_q &&
+                    g.kvh >= 0 && g.kvh < p.heads_kv && g.slot >= 0 &&
+                    g.slot + 2 * int64_t(g.parts) <= p.header[enigma_serving::kSlots];
   if (!__any_sync(0xffffffffu, live)) return;
   const int n = g.parts;
   const int64_t step = 2 * 128, at = int64_t(g.slot + state) * 128;

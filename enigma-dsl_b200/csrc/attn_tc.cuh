@@ -82,6 +82,7 @@ struct Params {
   float* lse;
   int64_t o_token, o_head;
   int heads_q, causal, tokens_q, tokens_k;
+  int slots_end;                   // slots of partial results, at least 1
   int one;                         // each CTA has exactly one item
   // paged prefix
   const int32_t *table, *lens, *slots;
@@ -129,7 +130,9 @@ __device__ __forceinline__ Work make_work(const Params& p, int t) {
     // q0 lq k0 lk | t0 tokens j0 j1 | kvh slot - -
     w.seq0 = a.x;
     w.tok0 = a.x + b.x;
-    w.tok_end = a.x + a.y;
+    // An item that does not lie inside the tensors (a plan made for others) has no rows here.
+    const bool in = a.x >= 0 && b.x >= 0 && c.x >= 0 && c.x < p.heads_kv && c.y + 1 < p.slots_end;
+    w.tok_end = in ? a.x + a.y : w.tok0;
     w.k0 = a.z;
     w.lk = a.w;
     w.off = p.causal ? a.w - a.y + 1 : a.w;

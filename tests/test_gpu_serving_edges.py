@@ -342,3 +342,23 @@ def test_an_empty_batch(cuda, dtype, d):
             assert out.shape == (0, 8, d) and out.dtype == k.dtype
     out = cuda_ops.sdpa_shared_prefix(q, k, k, table, lens, slots=lens[:0])
     assert out.shape == (0, 8, d)
+
+
+@pytest.mark.parametrize("lens_q,lens_k", [([70, 5, 300], [70, 5, 300]), ([3, 20], [4000, 700])])
+@pytest.mark.parametrize("dtype,d", KINDS)
+def test_a_plan_for_more_heads_writes_no_others(cuda, dtype, d, lens_q, lens_k):
+    """The C entry is given a plan that was made for more kv heads than the tensors have: the heads
+    they have are computed, and nothing is written beside them."""
+    import torch
+    from enigma import cuda_ops
+    rng = np.random.default_rng(d + 5)
+    tq, tk = sum(lens_q), sum(lens_k)
+    q, k, v = (_dev(_values(rng, (t, 2, d), dtype), dtype, cuda) for t in (tq, tk, tk))
+    want = cuda_ops.sdpa_packed(q, k, v, cuda_ops.PackedPlan(lens_q, lens_k, heads_q=2, heads_kv=2))
+    plan = cuda_ops.PackedPlan(lens_q, lens_k, heads_q=8, heads_kv=8)
+    plan.heads_q = plan.heads_kv = 2
+    wide = torch.full((tq, 9, d), 5.0, dtype=q.dtype, device=cuda)       # room for 8 heads and more
+    got = cuda_ops.sdpa_packed(q, k, v, plan, out=wide[:, :2])
+    assert (wide[:, 2:] == 5).all()
+    tol = srv.bound(np.zeros(()), 4.0, np.zeros(1), max(lens_k), dtype == "bf16")
+    assert float((got.float() - want.float()).abs().max()) <= 2 * float(tol.max())
