@@ -94,6 +94,30 @@ cudaError_t kv_cache_compact(const enigma_kv_cache_desc& d, cudaStream_t s);
 cudaError_t kv_cache_copy_pages(const enigma_kv_cache_desc& d, const int32_t* src,
                                 const int32_t* dst, int64_t n, cudaStream_t s);
 
+// The whole pages that the last fork or compaction of this map copied, in other buffers that hold one
+// page for each of its pages (at most n).
+cudaError_t kv_cache_copy_listed(const enigma_kv_cache_desc& d, int64_t n, cudaStream_t s);
+
+// Rotary positions (rope.cu).
+cudaError_t rope_launch(const enigma_rope_desc& d, cudaStream_t s);
+
+// The cache in 8-bit codes (kv_cache_codes8.cu) and attention over it (attn_codes8.cu).
+cudaError_t kv_cache_q8_fork(const enigma_kv_cache_q8_desc& d, const int32_t* parents,
+                             const int32_t* children, int64_t n, cudaStream_t s);
+cudaError_t kv_cache_q8_compact(const enigma_kv_cache_q8_desc& d, cudaStream_t s);
+cudaError_t kv_cache_q8_copy_pages(const enigma_kv_cache_q8_desc& d, const int32_t* src,
+                                   const int32_t* dst, int64_t n, cudaStream_t s);
+cudaError_t kv_cache_q8_write(const enigma_kv_cache_q8_desc& d, int64_t layer, int dtype,
+                              const void* new_k, const void* new_v, const int64_t* strides4,
+                              const int32_t* slots, const int32_t* starts, const int32_t* cu,
+                              int64_t n, int64_t tokens, cudaStream_t s);
+cudaError_t kv_cache_q8_read(const enigma_kv_cache_q8_desc& d, int64_t layer, int dtype, void* out_k,
+                             void* out_v, const int64_t* strides4, const int32_t* slots,
+                             const int32_t* starts, const int32_t* cu, int64_t n, int64_t tokens,
+                             cudaStream_t s);
+size_t sdpa_quantized_workspace(const enigma_sdpa_quantized_desc& d);
+cudaError_t sdpa_quantized_launch(const enigma_sdpa_quantized_desc& d, cudaStream_t s);
+
 cudaError_t elementwise_launch(int op, int dtype, const void* a, const void* b, void* c, int64_t n,
                                cudaStream_t s);
 

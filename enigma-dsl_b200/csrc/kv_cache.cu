@@ -531,6 +531,11 @@ cudaError_t kv_cache_copy_pages(const enigma_kv_cache_desc& d, const int32_t* sr
   return e == cudaSuccess ? launch_copy(d, src, dst, nullptr, m.ws, n, s) : e;
 }
 
+cudaError_t kv_cache_copy_listed(const enigma_kv_cache_desc& d, int64_t n, cudaStream_t s) {
+  const Map m = make_map(d);
+  return launch_copy(d, m.src(), m.dst(), nullptr, m.ws, n, s);
+}
+
 cudaError_t kv_cache_write(const enigma_kv_cache_desc& d, int64_t layer, const void* new_k,
                            const void* new_v, const int64_t* strides4, const int32_t* slots,
                            const int32_t* starts, const int32_t* cu, int64_t n, int64_t tokens,

@@ -19,7 +19,10 @@ OK, ERR_LAUNCH, ERR_EXEC, ERR_TIMEOUT, ERR_BADARG, ERR_DEVICE = 0, -1, -2, -3, -
 DTYPE_F32, DTYPE_BF16 = 0, 1
 KERNEL_RMSNORM, KERNEL_GEMM, KERNEL_SDPA = 1, 2, 3
 PACKED_PLAN_HEADER = 8
-CACHE_FULL, CACHE_BAD_REQUEST = 1, 2
+CACHE_FULL, CACHE_BAD_REQUEST, CACHE_SHARED = 1, 2, 4
+SCALE_BLOCK = 16
+CODE_INT8, CODE_E4M3 = 0, 1
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 
 _STATUS_NAMES = {
     ERR_LAUNCH: "launch failed",
@@ -83,6 +86,14 @@ PROTOTYPES = {
     "enigma_kv_cache_write": [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp],
     "enigma_kv_cache_compact": [_vp, _vp],
     "enigma_kv_cache_copy_pages": [_vp, _vp, _vp, _i64, _vp],
+    "enigma_rope": [_vp, _vp],
+    "enigma_kv_cache_q8_fork": [_vp, _vp, _vp, _i64, _vp],
+    "enigma_kv_cache_q8_compact": [_vp, _vp],
+    "enigma_kv_cache_q8_copy_pages": [_vp, _vp, _vp, _i64, _vp],
+    "enigma_kv_cache_q8_write": [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp],
+    "enigma_kv_cache_q8_read": [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp],
+    "enigma_sdpa_quantized_workspace_bytes": [_vp, _c.POINTER(_sz)],
+    "enigma_sdpa_quantized": [_vp, _vp],
     "enigma_dispatch": [_i32, _c.POINTER(_vp), _i32, _c.POINTER(_i64), _i32, _c.POINTER(_f32),
                         _i32, _u32p, _u32p, _vp],
     "enigma_dispatch_timed": [_i32, _c.POINTER(_vp), _i32, _c.POINTER(_i64), _i32,

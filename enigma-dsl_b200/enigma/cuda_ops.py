@@ -399,6 +399,286 @@ def sdpa_shared_prefix(q, k_pages, v_pages, table, lens, prefix_len: int = 0, sl
     return out
 
 
+# enigma_sdpa_quantized_desc: sizes and strides, scale and types; then pointers.
+_CODES_HEAD = struct.Struct("16qf3i")
+_CODES_PTRS = struct.Struct("11Q")
+
+
+def _code_of(dtype) -> int:
+    torch = _torch()
+    if dtype == torch.int8:
+        return _native.CODE_INT8
+    if dtype == torch.float8_e4m3fn:
+        return _native.CODE_E4M3
+    raise TypeError(f"unsupported codes {dtype}: expected int8 or float8_e4m3fn")
+
+
+@functools.lru_cache(maxsize=1024)
+def _quantized_head(index, q, k, v, ks, vs, table, lens, slots, out, scale):
+    """Checks the (shape, stride, dtype) of a call and packs the desc's head; bytes of workspace."""
+    torch = _torch()
+    name = "sdpa_quantized"
+    if len(q[0]) != 3 or len(k[0]) != 4 or v[0] != k[0]:
+        raise ValueError(f"{name}: expected q [B, Hq, D] and pages [P, Hkv, page, D]")
+    b, hq, d = q[0]
+    pages, hk, page, dk = k[0]
+    if dk != d:
+        raise ValueError(f"{name}: K/V head_dim does not match Q")
+    if v[2] != k[2]:
+        raise TypeError(f"{name}: K and V must share a dtype")
+    code = _code_of(k[2])
+    parts = page // _native.SCALE_BLOCK
+    for x in (ks, vs):
+        if x[0] != (pages, hk, parts) or x[2] != torch.float32:
+            raise ValueError(f"{name}: scales are fp32 [P, Hkv, page / {_native.SCALE_BLOCK}]")
+    if len(table[0]) != 2 or len(lens[0]) != 1 or lens[0][0] != table[0][0]:
+        raise ValueError(f"{name}: expected table [n, width] and lens [n]")
+    if b > table[0][0] if slots is None else slots[0] != (b,):
+        raise ValueError(f"{name}: slots must name one row per sequence")
+    if out is None:
+        out = (q[0], (hq * d, d, 1), q[2])
+    elif out[0] != q[0]:
+        raise ValueError(f"{name}: out must have q's shape")
+    dtype = _check_rows(name, q[2], q, out)
+    _check_distinct(name, out)
+    if not all(_dense(x[0][1:], x[1][1:]) for x in (k, v, ks, vs)):
+        raise ValueError(f"{name}: a page and its scales must be contiguous")
+    strides = [x[1][0] if pages > 1 else math.prod(x[0]) for x in (k, v, ks, vs)]
+    for shape, stride, other in (table, lens) + (() if slots is None else (slots,)):
+        if other != torch.int32 or not _dense(shape, stride):
+            raise ValueError(f"{name}: tables, lengths and slots are contiguous int32 tensors")
+    head = _CODES_HEAD.pack(b, hq, hk, d, page, pages, table[0][1], table[0][0], *q[1][:2],
+                            *out[1][:2], *strides, 1.0 / math.sqrt(d) if scale is None else scale,
+                            dtype, code, 0)
+    need = ctypes.c_size_t()
+    _launch(index, "enigma_sdpa_quantized_workspace_bytes", head + _CODES_PTRS.pack(*([0] * 11)),
+            ctypes.byref(need))
+    return head, need.value
+
+
+def sdpa_quantized(q, k_pages, v_pages, k_scale, v_scale, table, lens, slots=None,
+                   scale: Optional[float] = None, out=None, workspace=None):
+    """One new token per sequence over a paged cache held in 8-bit codes.
+
+    q [B, Hq, D], bf16 or fp32; k_pages / v_pages [pages, Hkv, page, D], int8 or float8_e4m3fn (one
+    layer of a kv_cache.QuantizedKVCache); k_scale / v_scale [pages, Hkv, page / 16] fp32: code x of
+    a block of 16 tokens stands for x * scale.  table [n, width] int32 page numbers, lens [n] int32;
+    sequence b uses row slots[b] (default: row b) and attends to its first lens keys, all read as
+    its own (sequences that share pages find them in L2).  A sequence without keys gives zeros, a
+    key without a page is zeros.  D is a multiple of 16 up to 256, page 16, 32, 64 or 128.
+    workspace: a uint8 tensor to use instead of an allocation per call (as many bytes as
+    enigma_sdpa_quantized_workspace_bytes says).  Returns out [B, Hq, D] of q's type.
+    """
+    name = "sdpa_quantized"
+    index = _same_device(name, q, k_pages, v_pages, k_scale, v_scale, table, lens)
+    head, need = _quantized_head(
+        index, (q.shape, q.stride(), q.dtype), (k_pages.shape, k_pages.stride(), k_pages.dtype),
+        (v_pages.shape, v_pages.stride(), v_pages.dtype),
+        (k_scale.shape, k_scale.stride(), k_scale.dtype),
+        (v_scale.shape, v_scale.stride(), v_scale.dtype),
+        (table.shape, table.stride(), table.dtype), (lens.shape, lens.stride(), lens.dtype),
+        None if slots is None else (slots.shape, slots.stride(), slots.dtype),
+        None if out is None else (out.shape, out.stride(), out.dtype), scale)
+    if out is None:
+        out = _contiguous_like(q)
+    else:
+        _same_device(name, q, out)
+    ws, ws_bytes, keep = _scratch(name, workspace, need, q)
+    if slots is not None:
+        _same_device(name, q, slots)
+    desc = head + _CODES_PTRS.pack(table.data_ptr(), lens.data_ptr(),
+                                   0 if slots is None else slots.data_ptr(), q.data_ptr(),
+                                   k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(),
+                                   v_scale.data_ptr(), out.data_ptr(), ws, ws_bytes)
+    _launch(index, "enigma_sdpa_quantized", desc, _raw_stream(index))
+    return out
+
+
+def rope_frequencies(rotary_dim: int, theta: float = 1e6, scaling: Optional[dict] = None):
+    """(radians per position of each pair, factor on cos and sin), in Python's 64-bit floats.
+
+    Pair i of n / 2 turns by w_i = theta^(-2 i / n).  scaling stretches contexts:
+      {"type": "linear", "factor": f}: w_i / f;
+      {"type": "ntk", "factor": f}: theta f^(n / (n - 2)) in place of theta;
+      {"type": "yarn", "factor": f, "original_len": L, "beta_fast": 32, "beta_slow": 1}: pairs that
+        turn more than beta_fast times over L positions keep w_i, those below beta_slow get w_i / f,
+        linearly in i between the two (at i(beta) = n ln(L / 2 pi beta) / 2 ln theta, rounded
+        outwards); the factor is "attention_factor", by default 0.1 ln f + 1;
+      {"type": "bands", "factor": f, "original_len": L, "low": a, "high": b}: pairs that turn
+        more than b times over L keep w_i, those below a get w_i / f, linearly in the number of
+        turns between.
+    """
+    n = rotary_dim
+    if n < 0 or n % 2:
+        raise ValueError("rope: rotary_dim must be even")
+    if not theta > 1.0 or not math.isfinite(theta):
+        raise ValueError("rope: theta must be greater than 1")
+    spec = dict(scaling or {"type": "none"})
+    kind, f = spec.pop("type", None), float(spec.pop("factor", 1.0))
+    if not f > 0.0 or not math.isfinite(f):
+        raise ValueError("rope: the scaling's factor must be positive")
+
+    def take(*names, **defaults):
+        values = [spec.pop(x) for x in names if x in spec]
+        if len(values) != len(names):
+            raise ValueError(f"rope: {kind} scaling needs {', '.join(names)}")
+        values += [spec.pop(x, default) for x, default in defaults.items()]
+        if spec:
+            raise ValueError(f"rope: {kind} scaling does not take {', '.join(spec)}")
+        return [None if x is None else float(x) for x in values]
+
+    if kind == "ntk":
+        take()
+        if n > 2:
+            theta = theta * f ** (n / (n - 2))
+    w = [theta ** (-2.0 * i / n) for i in range(n // 2)]
+    if kind in ("none", "ntk"):
+        take()
+        return w, 1.0
+    if kind == "linear":
+        take()
+        return [x / f for x in w], 1.0
+    if kind == "yarn":
+        length, fast, slow, factor = take("original_len", beta_fast=32.0, beta_slow=1.0,
+                                          attention_factor=None)
+        if not (length > 0 and fast > 0 and slow > 0):
+            raise ValueError("rope: yarn scaling's numbers must be positive")
+        at = [n * math.log(length / (beta * 2 * math.pi)) / (2 * math.log(theta))
+              for beta in (fast, slow)]
+        lo, hi = max(math.floor(at[0]), 0), min(math.ceil(at[1]), n - 1)
+        ramp = [min(1.0, max(0.0, (i - lo) / max(hi - lo, 1e-3))) for i in range(n // 2)]
+        return ([x * (1 - r) + x / f * r for x, r in zip(w, ramp)],
+                0.1 * math.log(f) + 1 if factor is None else factor)
+    if kind == "bands":
+        length, low, high = take("original_len", "low", "high")
+        if not (length > 0 and high > low):
+            raise ValueError("rope: bands scaling needs original_len > 0 and high > low")
+        keep = [min(1.0, max(0.0, (length * x / (2 * math.pi) - low) / (high - low))) for x in w]
+        return [x * r + x / f * (1 - r) for x, r in zip(w, keep)], 1.0
+    raise ValueError(f"rope: no scaling is called {kind!r}")
+
+
+class RopeTable:
+    """What `rope` needs to know of a model: made once, used by every layer and call.
+
+    head_dim; rotary_dim: how many of a head's first elements turn (default: all); layout "half"
+    (element i pairs with i + rotary_dim / 2, as in the decode layer) or "interleaved" (2 i with
+    2 i + 1); theta and scaling as in `rope_frequencies`, or frequencies: radians per position of
+    each pair (then `factor` may be given too).
+    """
+
+    def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, theta: float = 1e6,
+                 layout: str = "half", scaling: Optional[dict] = None, frequencies=None,
+                 factor: float = 1.0, device="cuda"):
+        torch = _torch()
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        if layout not in ("half", "interleaved"):
+            raise ValueError("rope: layout is 'half' or 'interleaved'")
+        if not 0 < head_dim <= 4096 or not 0 <= rotary_dim <= head_dim or rotary_dim % 2:
+            raise ValueError("rope: rotary_dim must be even and at most head_dim, head_dim at most "
+                             "4096")
+        if frequencies is None:
+            frequencies, more = rope_frequencies(rotary_dim, theta, scaling)
+            factor = factor * more
+        elif scaling is not None:
+            raise ValueError("rope: scaling or frequencies, not both")
+        frequencies = [float(x) for x in frequencies]
+        if len(frequencies) != rotary_dim // 2:
+            raise ValueError("rope: one frequency for each pair")
+        if not all(map(math.isfinite, frequencies)) or not math.isfinite(factor):
+            raise ValueError("rope: frequencies and factor must be finite")
+        # Full turns per position, as 64-bit binary fractions (angles are modulo a full turn).
+        turns = [int(math.fmod(x / (2 * math.pi), 1.0) * 2.0 ** 64) % (1 << 64) for x in frequencies]
+        self.head_dim, self.rotary_dim = int(head_dim), int(rotary_dim)
+        self.layout, self.factor = layout, float(factor)
+        self.frequencies = frequencies
+        self.turns = torch.tensor([x - (1 << 64) if x >> 63 else x for x in turns],
+                                  dtype=torch.int64).to(device)
+        self.heads = {}          # checked calls' sizes, strides and types
+
+
+# enigma_rope_desc: sizes and strides, factor and types; then pointers.
+_ROPE_HEAD = struct.Struct("13qf5i")
+_ROPE_PTRS = struct.Struct("6Q")
+
+
+def _check_distinct(name, *tensors):
+    """Outputs whose elements are all places of their own: no axis repeats or overlaps another."""
+    for shape, stride, _ in tensors:
+        reach = 1
+        for s, n in sorted((s, n) for s, n in zip(stride, shape) if n > 1):
+            if s < reach and 0 not in shape:
+                raise ValueError(f"{name}: an output's elements overlap")
+            reach = s * (n - 1) + reach
+
+
+def _rope_head(table, q, k, positions, out_q, out_k, inverse):
+    """Checks the (shape, stride, dtype) of a call with this table and packs the desc's head."""
+    torch = _torch()
+    if k is None:
+        if out_k is not None:
+            raise ValueError("rope: out_k without k")
+        k, out_k = ((q[0][0], 0, q[0][-1]), (0, 0, 1), q[2]), None
+    if len(q[0]) != 3 or len(k[0]) != 3 or q[0][0] != k[0][0] or q[0][2] != k[0][2]:
+        raise ValueError("rope: expected q and k [tokens, heads, head_dim]")
+    tokens, hq, d = q[0]
+    if d != table.head_dim:
+        raise ValueError(f"rope: the table was made for heads of {table.head_dim}")
+    if positions[0] != (tokens,) or not _dense(positions[0], positions[1]):
+        raise ValueError("rope: positions must hold one number per token")
+    if positions[2] not in (torch.int32, torch.int64):
+        raise TypeError("rope: positions are int32 or int64")
+    outs = []
+    for x, out in ((q, out_q), (k, out_k)):
+        if out is None:
+            out = (x[0], (x[0][1] * d, d, 1), x[2])
+        elif out[0] != x[0]:
+            raise ValueError("rope: an output must have its input's shape")
+        outs.append(out)
+    dtype = _check_rows("rope", q[2], q, k, *outs)
+    _check_distinct("rope", *outs)
+    return _ROPE_HEAD.pack(tokens, hq, k[0][1], d, table.rotary_dim, *q[1][:2], *k[1][:2],
+                           *outs[0][1][:2], *outs[1][1][:2], table.factor, dtype,
+                           _native.ROPE_HALF if table.layout == "half"
+                           else _native.ROPE_INTERLEAVED, bool(inverse),
+                           8 if positions[2] == torch.int64 else 4, 0)
+
+
+def rope(q, k, positions, table: RopeTable, inverse: bool = False, out_q=None, out_k=None):
+    """Queries and keys turned to their positions, in one launch.
+
+    q [tokens, Hq, D], k [tokens, Hkv, D] or None, any token and head strides, e.g. slices of one
+    fused projection's output; positions [tokens], int32 or int64 on the device (negative ones turn
+    back).  inverse=True turns by the negative angle: the transpose, so it also takes a result's
+    gradient to its input's.  out_q / out_k: tensors to write, which may be q and k themselves but not
+    overlap them otherwise.  Angles are exact whatever the position.  Returns (q, k) turned, or q
+    alone without k.
+    """
+    key = ((q.shape, q.stride(), q.dtype), None if k is None else (k.shape, k.stride(), k.dtype),
+           (positions.shape, positions.stride(), positions.dtype),
+           None if out_q is None else (out_q.shape, out_q.stride(), out_q.dtype),
+           None if out_k is None else (out_k.shape, out_k.stride(), out_k.dtype), inverse)
+    head = table.heads.get(key)
+    if head is None:
+        head = _rope_head(table, *key)
+        if len(table.heads) >= 64:
+            table.heads.clear()
+        table.heads[key] = head
+    index = _same_device("rope", q, positions, table.turns)
+    if out_q is None:
+        out_q = _contiguous_like(q)
+    if k is not None and out_k is None:
+        out_k = _contiguous_like(k)
+    for x in (k, out_q, out_k):
+        if x is not None and x.get_device() != index:
+            raise ValueError("rope: all tensors must be on the same device")
+    desc = head + _ROPE_PTRS.pack(positions.data_ptr(), table.turns.data_ptr(), q.data_ptr(),
+                                  0 if k is None else k.data_ptr(), out_q.data_ptr(),
+                                  0 if k is None else out_k.data_ptr())
+    _launch(index, "enigma_rope", desc, _raw_stream(index))
+    return out_q if k is None else (out_q, out_k)
+
+
 def synchronize(device_index: int = 0) -> None:
     """Synchronize the device and raise if a kernel reported a device-side timeout."""
     ensure_device(device_index)

@@ -6,6 +6,10 @@ operations run on torch's current stream without reading anything back, so they 
 captured in a CUDA graph; what went wrong on the device (no free page, a slot named twice) is
 kept there until `check()` raises it.  `cuda_ops.sdpa_packed` fills a cache's first tokens
 with `write`, `cuda_ops.sdpa_shared_prefix` reads it (`attend`).
+
+`QuantizedKVCache` is the same cache in 8-bit codes with a scale for each 16 tokens of a page and
+head: half the bytes of bf16 to hold and to stream.  Rows are quantised as they are written, `attend`
+works on the codes (`cuda_ops.sdpa_quantized`), `read` gives rows back.
 """
 from __future__ import annotations
 
@@ -40,6 +44,10 @@ class PagedKVCache:
             raise ValueError("PagedKVCache: k and v must be [layers, pages, heads, page, head_dim]")
         cuda_ops._dtype_code(k)
         cuda_ops._check_cuda(k, v, table, lens, refs)
+        self._setup(k, v, table, lens, refs)
+
+    def _setup(self, k, v, table, lens, refs):
+        import torch
         if any(t.dtype != torch.int32 for t in (table, lens, refs)):
             raise ValueError("PagedKVCache: table, lens and refs are int32")
         layers, pages, heads, page, head_dim = k.shape
@@ -178,9 +186,153 @@ class PagedKVCache:
         code = int(self.status.item())
         if code:
             self.status.zero_()
+        if code & _native.CACHE_SHARED:
+            raise EnigmaError("paged cache: a write named a page that forks share")
         if code & _native.CACHE_BAD_REQUEST:
             raise EnigmaError("paged cache: a request named a slot or page that does not exist, "
                               "a slot twice, a parent as its child, or a length that does not "
                               "fit its row")
         if code & _native.CACHE_FULL:
             raise EnigmaError("paged cache: not enough free pages")
+
+
+class _QuantizedDesc(ctypes.Structure):
+    """Mirror of enigma_kv_cache_q8_desc (include/enigma_cuda.h)."""
+
+    _fields_ = [("cache", _CacheDesc), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("code", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class QuantizedKVCache(PagedKVCache):
+    """A paged cache in 8-bit codes: k, v [layers, pages, heads_kv, page, head_dim] int8 or
+    float8_e4m3fn, k_scale, v_scale [layers, pages, heads_kv, page / 16] fp32; a code x stands for
+    x * scale.  The page map and its operations are PagedKVCache's, pages move with their scales.
+
+    A scale is the least power of two that brings its block's largest magnitude to at most 127
+    (int8) or 448 (e4m3).  Appending to a partly filled block may raise its scale; its earlier tokens
+    are then rounded once more, and stay within one step of what was written, however often."""
+
+    def __init__(self, k, v, k_scale, v_scale, table, lens, refs):
+        import torch
+        if k.dim() != 5 or v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError("QuantizedKVCache: k and v must be [layers, pages, heads, page, head_dim]")
+        code = cuda_ops._code_of(k.dtype)
+        cuda_ops._check_cuda(k, v, k_scale, v_scale, table, lens, refs)
+        layers, pages, heads, page, head_dim = k.shape
+        if page not in (16, 32, 64, 128) or head_dim % 16 or not 0 < head_dim <= 256:
+            raise ValueError("QuantizedKVCache: page must be 16, 32, 64 or 128, head_dim a multiple "
+                             "of 16 up to 256")
+        scales = (layers, pages, heads, page // _native.SCALE_BLOCK)
+        if any(tuple(x.shape) != scales or x.dtype != torch.float32 for x in (k_scale, v_scale)):
+            raise ValueError("QuantizedKVCache: scales are fp32 [layers, pages, heads, page / "
+                             f"{_native.SCALE_BLOCK}]")
+        if k.data_ptr() % 16 or v.data_ptr() % 16:
+            raise ValueError("QuantizedKVCache: k and v must be 16-byte aligned")
+        self.k_scale, self.v_scale = k_scale, v_scale
+        self._setup(k, v, table, lens, refs)
+        self._q8 = _QuantizedDesc(self._desc, k_scale.data_ptr(), v_scale.data_ptr(), code, 0)
+        self._q8_ref = ctypes.byref(self._q8)
+
+    @classmethod
+    def empty(cls, layers: int, pages: int, page: int, heads_kv: int, head_dim: int, slots: int,
+              max_len: int, dtype=None, device="cuda"):
+        """A cache without tokens, for sequences of at most max_len tokens; dtype (of the codes):
+        torch.int8 (the default) or torch.float8_e4m3fn."""
+        import torch
+        dtype = torch.int8 if dtype is None else dtype
+        cuda_ops._code_of(dtype)
+        shape = (layers, pages, heads_kv, page, head_dim)
+        scales = (layers, pages, heads_kv, page // _native.SCALE_BLOCK)
+
+        def ints(fill, *size):
+            return torch.full(size, fill, dtype=torch.int32, device=device)
+
+        codes = [torch.zeros(shape, dtype=torch.int8, device=device).view(dtype) for _ in range(2)]
+        return cls(*codes, *(torch.zeros(scales, device=device) for _ in range(2)),
+                   ints(-1, slots, -(-max_len // page)), ints(0, slots), ints(0, pages))
+
+    def _call_q8(self, name, *args):
+        cuda_ops._launch(self._index, name, self._q8_ref, *args, cuda_ops._raw_stream(self._index))
+
+    def fork(self, parents, children) -> None:
+        parents = self._ints("fork", parents)
+        children = self._ints("fork", children, parents)
+        self._call_q8("enigma_kv_cache_q8_fork", parents.data_ptr(), children.data_ptr(),
+                      parents.shape[0])
+
+    def compact(self) -> None:
+        self._call_q8("enigma_kv_cache_q8_compact")
+
+    def copy_pages(self, src, dst) -> None:
+        src = self._ints("copy_pages", src)
+        dst = self._ints("copy_pages", dst, src)
+        self._call_q8("enigma_kv_cache_q8_copy_pages", src.data_ptr(), dst.data_ptr(), src.numel())
+
+    fork.__doc__ = PagedKVCache.fork.__doc__
+    compact.__doc__ = PagedKVCache.compact.__doc__
+    copy_pages.__doc__ = PagedKVCache.copy_pages.__doc__
+
+    def _rows(self, name, layer, k, v, slots, starts, cu):
+        """Checks a write's or read's rows; the request on the device and what C takes of the rows."""
+        if len(k.shape) != 3 or k.shape != v.shape or k.shape[1:] != self._row:
+            raise ValueError(f"{name}: expected rows [tokens, {self._row[0]}, {self._row[1]}]")
+        shape, ks, vs = k.shape, k.stride(), v.stride()
+        dtype = cuda_ops._check_rows(name, k.dtype, (shape, ks, k.dtype), (shape, vs, v.dtype))
+        cuda_ops._same_device(name, self.k, k, v)
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"{name}: layer {layer} of {self.layers}")
+        slots = self._ints(name, slots)
+        starts = self._ints(name, starts, slots)
+        cu = self._ints(name, cu)
+        n = slots.shape[0]
+        if cu.shape[0] != n + 1:
+            raise ValueError(f"{name}: cu holds one number more than there are slots")
+        # The request's tensors come back too: they live until the launch is queued.
+        return (layer, dtype, k.data_ptr(), v.data_ptr(), _STRIDES.pack(ks[0], ks[1], vs[0], vs[1]),
+                slots.data_ptr(), starts.data_ptr(), cu.data_ptr(), n, shape[0]), (slots, starts, cu)
+
+    def write(self, layer: int, new_k, new_v, slots, starts, cu) -> None:
+        """Rows cu[i] .. cu[i + 1] of new_k / new_v [tokens, heads_kv, head_dim], bf16 or fp32, are
+        tokens starts[i], starts[i] + 1, ... of slot slots[i] in `layer` (reserved before).
+
+        A slot's tokens are written in order; going back to an earlier token is fine and cuts off
+        what the block of 16 held behind.  Pages that forks share are not written (`check` says so;
+        appending never meets one), nor is a block that two entries of one call name.  A value that is
+        not finite makes its block of 16 tokens NaN."""
+        args, keep = self._rows("write", layer, new_k, new_v, slots, starts, cu)
+        self._call_q8("enigma_kv_cache_q8_write", *args)
+
+    def read(self, layer: int, slots, starts, cu, tokens: Optional[int] = None, dtype=None,
+             out_k=None, out_v=None):
+        """Tokens starts[i], starts[i] + 1, ... of slot slots[i] in `layer` as rows cu[i] .. cu[i + 1]
+        of k, v [tokens, heads_kv, head_dim], e.g. earlier context for `cuda_ops.sdpa_packed`.
+
+        tokens: the number of rows, by default cu's last number (which must then be on the host);
+        dtype bf16 (the default; it holds every code times a power of two) or fp32; out_k / out_v:
+        tensors to write instead.  A token that the slot does not hold gives zeros; rows that no entry
+        names are not written (they stay what they were in out_k and out_v)."""
+        import torch
+        if (out_k is None) != (out_v is None):
+            raise ValueError("read: out_k and out_v come together")
+        if out_k is None:
+            if tokens is None:
+                if isinstance(cu, torch.Tensor) and cu.is_cuda:
+                    raise ValueError("read: tokens must be given where cu is on the device")
+                tokens = int(cu[-1]) if len(cu) else 0
+            dtype = torch.bfloat16 if dtype is None else dtype
+            shape = (int(tokens), *self._row)
+            out_k, out_v = (torch.empty(shape, dtype=dtype, device=self.k.device) for _ in range(2))
+        elif tokens not in (None, out_k.shape[0]) or dtype not in (None, out_k.dtype):
+            raise ValueError("read: out_k and out_v have another size or type")
+        args, keep = self._rows("read", layer, out_k, out_v, slots, starts, cu)
+        cuda_ops._check_distinct("read", *((x.shape, x.stride(), None) for x in (out_k, out_v)))
+        self._call_q8("enigma_kv_cache_q8_read", *args)
+        return out_k, out_v
+
+    def attend(self, layer: int, q, slots=None, scale: Optional[float] = None, out=None,
+               workspace=None):
+        """cuda_ops.sdpa_quantized over one layer of this cache."""
+        return cuda_ops.sdpa_quantized(q, self.k[layer], self.v[layer], self.k_scale[layer],
+                                       self.v_scale[layer], self.table, self.lens,
+                                       slots=None if slots is None else self._ints("attend", slots),
+                                       scale=scale, out=out, workspace=workspace)

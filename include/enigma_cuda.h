@@ -333,6 +333,99 @@ int32_t enigma_kv_cache_compact(const enigma_kv_cache_desc* desc, void* stream);
 int32_t enigma_kv_cache_copy_pages(const enigma_kv_cache_desc* desc, const int32_t* src,
                                    const int32_t* dst, int64_t n, void* stream);
 
+/* ---- rotary positions, and the paged cache in 8-bit codes ----
+ * (No counterpart in the reference, whose decode example turns one token's heads by two given
+ * tables inside its kernel, examples/qwen_megakernel.py:228-269.) */
+
+/* Turns queries q [tokens, heads_q, head_dim] and keys k [tokens, heads_k, head_dim] (heads_k 0:
+ * queries alone) to their positions in one launch.  Pair i of a head's first rotary_dim elements
+ * (x[i], x[i + rotary_dim / 2]) in the half layout, (x[2i], x[2i + 1]) interleaved, turns by
+ * positions[token] * turns[i] / 2^64 of a full turn and is multiplied by `factor`; the elements
+ * behind are copied.  inverse != 0 turns back: the transpose of the same map, so its gradient.
+ * Positions are int32 or int64 (position_bytes); turns [rotary_dim / 2] is a device array, a
+ * frequency w in radians being round(w / 2 pi * 2^64) modulo 2^64.  Token and head strides in
+ * elements, head_dim contiguous; an output may be its input, but not overlap it otherwise. */
+#define ENIGMA_ROPE_HALF 0
+#define ENIGMA_ROPE_INTERLEAVED 1
+typedef struct enigma_rope_desc {
+  int64_t tokens, heads_q, heads_k, head_dim, rotary_dim;
+  int64_t q_token, q_head, k_token, k_head, oq_token, oq_head, ok_token, ok_head;
+  float factor;
+  int32_t dtype, layout, inverse, position_bytes, reserved;
+  const void* positions;
+  const uint64_t* turns;
+  const void *q, *k;
+  void *out_q, *out_k;
+} enigma_rope_desc;
+int32_t enigma_rope(const enigma_rope_desc* desc, void* stream);
+
+/* A paged cache whose pages hold 8-bit codes (cache.elem_bytes 1; whole numbers in [-127, 127] or
+ * e4m3 floats) with one fp32 scale for each ENIGMA_SCALE_BLOCK tokens of a page and head:
+ * k_scale, v_scale [layers, pages, heads_kv, page / ENIGMA_SCALE_BLOCK]; a code stands for code *
+ * scale.  head_dim is a multiple of 16 up to 256, page 16, 32, 64 or 128; pages are 16-byte aligned.
+ * enigma_kv_cache_free and enigma_kv_cache_reserve take `cache` itself; fork, compact and
+ * copy_pages are those of enigma_kv_cache_* with the scales moved along.
+ *   write  as enigma_kv_cache_write, from rows of type dtype.  The scale of a block is the least
+ *          power of two 2^e under which the block's largest magnitude (2^-110 if that is more) is at most
+ *          127, or 448, and a code is the value over the scale, rounded to nearest (ties to
+ *          even).  A write that starts behind a block's first token keeps the block's earlier
+ *          tokens: its scale is the larger of the block's and the new tokens', and where it
+ *          grows the earlier codes are rounded to it.  What a block held behind the last
+ *          written token is lost.  A value that is not finite makes its block's scale NaN, until
+ *          a write starts the block anew.  A page that forks share is not written
+ *          (ENIGMA_CACHE_SHARED), nor is a block that two entries of a request name
+ *          (ENIGMA_CACHE_BAD_REQUEST).
+ *   read   rows cu[i] .. cu[i + 1] of out_k / out_v [tokens, heads_kv, head_dim] of type dtype
+ *          (strides4 as in write) get the tokens starts[i], ... of slots[i]; a token that the slot does
+ *          not hold gives zeros; rows before cu[0] and behind cu[n] are left as they were. */
+#define ENIGMA_SCALE_BLOCK 16
+#define ENIGMA_CODE_INT8 0
+#define ENIGMA_CODE_E4M3 1
+#define ENIGMA_CACHE_SHARED 4
+typedef struct enigma_kv_cache_q8_desc {
+  enigma_kv_cache_desc cache;
+  float *k_scale, *v_scale;
+  int32_t code, reserved;
+} enigma_kv_cache_q8_desc;
+int32_t enigma_kv_cache_q8_fork(const enigma_kv_cache_q8_desc* desc, const int32_t* parents,
+                                const int32_t* children, int64_t n, void* stream);
+int32_t enigma_kv_cache_q8_compact(const enigma_kv_cache_q8_desc* desc, void* stream);
+int32_t enigma_kv_cache_q8_copy_pages(const enigma_kv_cache_q8_desc* desc, const int32_t* src,
+                                      const int32_t* dst, int64_t n, void* stream);
+int32_t enigma_kv_cache_q8_write(const enigma_kv_cache_q8_desc* desc, int64_t layer, int32_t dtype,
+                                 const void* new_k, const void* new_v, const int64_t* strides4,
+                                 const int32_t* slots, const int32_t* starts, const int32_t* cu,
+                                 int64_t n, int64_t tokens, void* stream);
+int32_t enigma_kv_cache_q8_read(const enigma_kv_cache_q8_desc* desc, int64_t layer, int32_t dtype,
+                                void* out_k, void* out_v, const int64_t* strides4,
+                                const int32_t* slots, const int32_t* starts, const int32_t* cu,
+                                int64_t n, int64_t tokens, void* stream);
+
+/* One new token per sequence over pages of 8-bit codes: q, out [batch, heads_q, head_dim] of type
+ * dtype; k_pages, v_pages [pages, heads_kv, page, head_dim] codes, contiguous but for the page
+ * strides (k_page, v_page, in codes, multiples of 16); k_scale, v_scale [pages, heads_kv, page /
+ * ENIGMA_SCALE_BLOCK], contiguous but for theirs (ks_page, vs_page); scales are any finite numbers.
+ *   out = sum_j softmax_j(scale k_scale_j q . k_j) v_scale_j v_j
+ * over the first min(lens, table_width * page) keys; tables, lens and slots as in
+ * enigma_sdpa_shared_prefix: no keys, or a slot that does not exist, give zeros, and a key whose
+ * table entry is no page is a key and a value of zeros.  A code or scale that is seen and is NaN
+ * gives NaN; what no sequence sees may hold anything.  scale is positive, batch <= 4096, head_dim
+ * a multiple of 16 up to 256, page 16, 32, 64 or 128.  workspace: caller-owned device memory of
+ * enigma_sdpa_quantized_workspace_bytes() bytes, 256-byte aligned. */
+typedef struct enigma_sdpa_quantized_desc {
+  int64_t batch, heads_q, heads_kv, head_dim, page, pages, table_width, n_slots;
+  int64_t q_batch, q_head, o_batch, o_head, k_page, v_page, ks_page, vs_page;
+  float scale;
+  int32_t dtype, code, reserved;
+  const int32_t *table, *lens, *slots;
+  const void *q, *k_pages, *v_pages;
+  const float *k_scale, *v_scale;
+  void *out, *workspace;
+  size_t workspace_bytes;
+} enigma_sdpa_quantized_desc;
+int32_t enigma_sdpa_quantized_workspace_bytes(const enigma_sdpa_quantized_desc* desc, size_t* bytes);
+int32_t enigma_sdpa_quantized(const enigma_sdpa_quantized_desc* desc, void* stream);
+
 /* ---- generic dispatch by kernel id: replaces enigma_dispatch /
  *      enigma_dispatch_timed (libenigma_runtime.swift:132-214).
  *      grid / threads are Metal-style totals (threads per axis, not groups),

@@ -154,3 +154,109 @@ class Pages:
     def copy_pages(self, src, dst):
         for a, b in zip(src, dst):
             self.k[:, b], self.v[:, b] = self.k[:, a], self.v[:, a]
+
+
+def rope(x, positions, frequencies, factor, layout, inverse=False):
+    """x [tokens, heads, D] turned in 64 bits, and |a| + |b| of each element's pair (0: copied)."""
+    x = np.asarray(x, np.float64)
+    out, mag = x.copy(), np.zeros(x.shape)
+    n = 2 * len(frequencies)
+    for i, w in enumerate(frequencies):
+        a, b = (i, i + n // 2) if layout == "half" else (2 * i, 2 * i + 1)
+        angle = np.asarray(positions, np.float64)[:, None] * w
+        c, s = factor * np.cos(angle), factor * np.sin(-angle if inverse else angle)
+        out[..., a] = x[..., a] * c - x[..., b] * s
+        out[..., b] = x[..., b] * c + x[..., a] * s
+        mag[..., a] = mag[..., b] = abs(factor) * (np.abs(x[..., a]) + np.abs(x[..., b]))
+    return out, mag
+
+
+BLOCK = 16            # tokens of a page that share a scale
+TOP = {"int8": 127.0, "e4m3": 448.0}
+
+
+def to_code(y, code):
+    """y rounded to the nearest code (ties to even), as the number that the code is."""
+    y = np.asarray(y, np.float64)
+    if code == "int8":
+        return np.rint(y)
+    step = np.exp2(np.maximum(np.floor(np.log2(np.maximum(np.abs(y), 2.0 ** -60))), -6) - 3)
+    return np.rint(y / step) * step
+
+
+def scale_of(top, code):
+    """The least power of two that brings `top` (2^-110 at least) into the codes' range."""
+    m, e = np.frexp(np.maximum(top, 2.0 ** -110) / TOP[code])       # 2^e > it >= 2^(e - 1)
+    return np.exp2(np.where(m == 0.5, e - 1, e))
+
+
+class QuantizedPages(Pages):
+    """Pages whose k and v hold codes (as numbers), with a scale per block."""
+
+    def __init__(self, k, v, k_scale, v_scale, table, lens, refs, code):
+        super().__init__(np.asarray(k, np.float64), np.asarray(v, np.float64), table, lens, refs)
+        self.scales = [np.array(x, np.float64) for x in (k_scale, v_scale)]
+        self.code = code
+
+    def _moved(self, pairs):
+        for a, b in pairs:
+            for x in self.scales:
+                x[:, b] = x[:, a]
+
+    def fork(self, parents, children):
+        super().fork(parents, children)
+        self._moved((self.table[a, self.lens[a] // self.page], self.table[c, self.lens[a] // self.page])
+                    for a, c in zip(parents, children) if self.lens[a] % self.page)
+
+    def compact(self):
+        live = [int(p) for p in np.flatnonzero(self.refs > 0)]
+        holes = [p for p in range(len(live)) if self.refs[p] == 0]
+        self._moved(zip([p for p in live if p >= len(live)], holes))
+        super().compact()
+
+    def copy_pages(self, src, dst):
+        super().copy_pages(src, dst)
+        self._moved(zip(src, dst))
+
+    def write(self, layer, new_k, new_v, slots, starts, cu):
+        for codes, scales, rows in ((self.k, self.scales[0], new_k), (self.v, self.scales[1], new_v)):
+            rows = np.asarray(rows, np.float64)
+            for i, s in enumerate(slots):
+                t, pos = cu[i], int(starts[i])
+                while t < cu[i + 1]:
+                    r = pos % BLOCK
+                    n = min(BLOCK - r, cu[i + 1] - t)
+                    p, j, o = self.table[s, pos // self.page], pos % self.page // BLOCK, pos % self.page - r
+                    x = rows[t:t + n].transpose(1, 0, 2)
+                    finite = np.isfinite(x).all((1, 2))
+                    top = np.where(finite, np.abs(np.where(finite[:, None, None], x, 0)).max((1, 2)), 0)
+                    scale = np.where(finite, scale_of(top, self.code), np.nan)
+                    old = scales[layer, p, :, j]
+                    if r:
+                        scale = np.where(np.isnan(old), np.nan, np.maximum(scale, old))
+                        held = codes[layer, p, :, o:o + r]
+                        grown = np.where(np.isnan(scale), 1.0, old / scale)[:, None, None]
+                        codes[layer, p, :, o:o + r] = to_code(held * grown, self.code)
+                    unit = np.where(np.isnan(scale), np.inf, scale)[:, None, None]
+                    y = np.where(np.isfinite(x), x, 0) / unit                  # a NaN block: codes 0
+                    codes[layer, p, :, o + r:o + r + n] = to_code(y, self.code)
+                    scales[layer, p, :, j] = scale
+                    t, pos = t + n, pos + n
+
+    def values(self, layer):
+        """(k, v) of a layer as the values that the codes stand for."""
+        return tuple(x[layer] * np.repeat(s[layer], BLOCK, -1)[..., None]
+                     for x, s in zip((self.k, self.v), self.scales))
+
+    def read(self, layer, slots, starts, cu, out_k, out_v):
+        k, v = self.values(layer)
+        for i, s in enumerate(slots):
+            for t in range(cu[i], cu[i + 1]):
+                pos = int(starts[i]) + t - cu[i]
+                p = -1
+                if 0 <= s < len(self.table) and 0 <= pos < self.lens[s] \
+                        and pos // self.page < self.table.shape[1]:
+                    p = self.table[s, pos // self.page]
+                has = 0 <= p < len(k)
+                out_k[t] = k[p, :, pos % self.page] if has else 0
+                out_v[t] = v[p, :, pos % self.page] if has else 0
