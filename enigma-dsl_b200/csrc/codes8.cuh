@@ -26,6 +26,19 @@ __device__ __forceinline__ uint32_t halves_of(uint32_t two) {
   return r;
 }
 
+// Four codes as two pairs of halves.
+template <bool E4M3>
+__device__ __forceinline__ void halves_of4(uint32_t four, uint32_t* lo, uint32_t* hi) {
+  if (E4M3) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(*lo), "=r"(*hi) : "r"(four));
+  } else {
+    const uint32_t u = four ^ 0x80808080u;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*lo) : "r"(__byte_perm(u, 0x64646464u, 0x4140)), "r"(0x64806480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*hi) : "r"(__byte_perm(u, 0x64646464u, 0x4342)), "r"(0x64806480u));
+  }
+}
+
 __device__ __forceinline__ float2 floats_of(uint32_t halves) {
   float2 f;
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
