@@ -17,11 +17,16 @@
 // The order of a product's inner index is free as long as both operands share it, and so is which
 // rows stand where: so a lane's operands are 16 consecutive bytes of a key's row in both products,
 // no fragment needs a transposing load, and V's pairs of keys are made by byte permutations before
-// they are converted.  Scores take s_k in fp32.  s_v goes into P relative to the chunk's larger
-// one, which is applied to the chunk's product in fp32, as is exp2(chunk's maximum - running maximum):
-// P is at most 2^15, its largest value exactly, so rounding it to fp16 costs 2^-11 of the weight, or
-// 2^-40 of the chunk's largest.  fp32 queries and P are two fp16 numbers each (2^-22, or the same
-// 2^-40).  Queries are brought to [2^11, 2^12) by a power of two per head.
+// they are converted.  Scores take s_k in fp32, P takes s_v.
+//
+// bf16: O accumulates in the products' own registers.  P = exp2(s - m) s_v / v0 2^9 with a reference m
+// that follows the running maximum once a score passes it by 4, and v0 the largest |s_v|, followed
+// once another passes it fourfold: P < 2^15, so most chunks change no reference, need no maximum
+// over the lanes and rescale nothing.  Rounding P to fp16 costs 2^-11 of the weight, or 2^-34 of a weight
+// of one.  fp32: queries and P are two fp16 numbers each (2^-22); a chunk's P is relative to its own
+// largest score and s_v, times 2^15, and what brings it to the running maximum is applied to the
+// chunk's product in fp32, so that small weights keep theirs whatever came before (2^-40 of the
+// chunk's largest).  Queries are brought to [2^11, 2^12) by a power of two per head.
 #include <algorithm>
 #include <atomic>
 
@@ -33,19 +38,25 @@ namespace {
 using namespace enigma_codes8;
 using namespace enigma_sm100;
 
-constexpr int WARPS = 8;
-constexpr int THREADS = WARPS * 32;
-constexpr int SLOTS = WARPS + 2;         // pieces of a block in the workspace: its warps' first ones,
-constexpr int BEFORE = WARPS;            // what it has of a unit that began in another block,
-constexpr int AFTER = WARPS + 1;         // and of one that goes on in the next
+// The work list's unit starts count as STARTS chunks: loading its queries and writing its result takes
+// a warp about as long.  Each warp of a block gets at least LEAST entries, if the list has as many for
+// one block: so a block has a chunk or more, and a unit's pieces are in consecutive blocks.
+constexpr int STARTS = 1;
+constexpr int LEAST = 3;
 
-template <int DT, int NT>
+template <typename T, int DT, int NT>
 struct Cfg {
+  // As many warps as their registers leave room for: O, queries and a chunk's operands.
+  static constexpr int WARPS = DT * NT * int(sizeof(T)) <= 128 ? 16 : DT * NT * int(sizeof(T)) <= 256 ? 12 : 8;
+  static constexpr int THREADS = WARPS * 32;
+  static constexpr int SLOTS = WARPS + 2;                // pieces of a block in the workspace: its warps'
+  static constexpr int BEFORE = WARPS;                   // first ones, what it has of a unit that began
+  static constexpr int AFTER = WARPS + 1;                // in another block, and of one that goes on
   static constexpr int KEYS = DT == 256 ? 16 : 32;       // of a chunk
   static constexpr int MT = KEYS / 16;                    // 16-key tiles, scale blocks
   static constexpr int TILE = KEYS * DT;                  // bytes of K or V
-  static constexpr int STAGES = DT == 64 ? 6 : 3;
-  static constexpr int RING = STAGES * 2 * TILE;          // 24 KB a warp
+  static constexpr int STAGES = (192 << 10) / (WARPS * 2 * TILE);
+  static constexpr int RING = STAGES * 2 * TILE;          // of a warp
   static constexpr int TILES = DT / 16;                   // 16-element tiles of O
   static constexpr int HEADS = 8 * NT;
   static constexpr int PIECE = (TILES * NT * 4) * 32;     // floats of O in fragment order
@@ -63,6 +74,7 @@ struct Attend {
   int whole;                             // a block per unit: nothing to join
   float scale_log2;
   bool q_vec, o_vec;                     // rows of q, out on 16 bytes
+  int fast;                              // rows of DT codes: copies at constant offsets
   float* pieces;                         // [block][SLOTS][SLOT]
   int2* links;                           // [block]: unit that goes on behind it, blocks it spans
 };
@@ -70,6 +82,12 @@ struct Attend {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;"
                ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// The same with offsets that the instruction holds.
+template <int TO, int FROM>
+__device__ __forceinline__ void cp_async16_at(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0+%2], [%1+%3], 16;"
+               ::"r"(dst), "l"(src), "n"(TO), "n"(FROM) : "memory");
 }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -96,6 +114,15 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same from zero.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                              uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t turn_8x8(uint32_t x) {   // an 8 x 8 fragment, transposed
   uint32_t y;
@@ -153,10 +180,10 @@ __device__ __forceinline__ int len_at(const Attend& a, int b) {
   return int(min(int64_t(max(a.lens[slot], 0)), int64_t(a.width) << a.page_shift));
 }
 
-// A place in the work list: chunk j of the n of a unit.
+// A place in the work list: chunk j of the n of a unit; entries left in the warp's range.
 struct Place {
-  int b, u, j, n, len;
-  int64_t row;                           // first entry of the sequence's table row
+  int b, u, j, n, len, left;
+  const int32_t* row;                    // the sequence's table row
 };
 
 __device__ __forceinline__ void store1(float* p, float x) { *p = x; }
@@ -175,6 +202,16 @@ __device__ __forceinline__ void store_pair(T* p, float x, float y, bool vec) {
   }
 }
 
+// N copies of 16 bytes a lane, STEP bytes apart in memory and, but for the swizzle's form, in the tile.
+template <int N, int FORMS, int STEP, int Y = 0>
+__device__ __forceinline__ void copy_rows(const uint32_t (&to)[FORMS], uint32_t plus, const uint8_t* from) {
+  if constexpr (Y < N) {
+    constexpr int TO = Y / FORMS * FORMS * STEP;
+    cp_async16_at<TO, Y * STEP>(to[Y % FORMS] + plus, from);
+    copy_rows<N, FORMS, STEP, Y + 1>(to, plus, from);
+  }
+}
+
 // First element of O's tile m that lane (g, t) has, in rows g and g + 8: e and e + 1.
 template <int DT>
 __device__ __forceinline__ int element_of(int m, int g) {
@@ -190,20 +227,21 @@ __device__ __forceinline__ T* out_row(const Attend& a, int b, int u, int head) {
 
 // T: of queries and results; DT: the head's elements, rounded up; NT: tiles of 8 query heads.
 template <typename T, bool E4M3, int DT, int NT>
-__global__ void __launch_bounds__(THREADS, 1) attend_codes8_kernel(const Attend a) {
-  using C = Cfg<DT, NT>;
+__global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kernel(const Attend a) {
+  using C = Cfg<T, DT, NT>;
   constexpr bool SPLIT = sizeof(T) == 4;
-  constexpr int MT = C::MT, KEYS = C::KEYS;
-  extern __shared__ __align__(128) uint8_t smem[];       // rings, chunks before each b, lengths
-  __shared__ float s_scale[WARPS][C::STAGES][2 * MT];
-  __shared__ float s_m[WARPS][C::HEADS], s_l[WARPS][C::HEADS];   // of the pieces in the rings
+  constexpr int MT = C::MT, KEYS = C::KEYS, WARPS = C::WARPS, THREADS = C::THREADS;
+  constexpr int PARTS = SPLIT ? 4 : 2;   // registers of an operand: two halves of the inner index
+  extern __shared__ __align__(128) uint8_t smem[];       // rings, list entries before each b, last chunks
+  __shared__ __align__(16) float s_scale[WARPS][C::STAGES][2 * MT];
+  __shared__ float s_m[2 * WARPS][C::HEADS], s_l[2 * WARPS][C::HEADS], s_w[2 * WARPS][C::HEADS];
   __shared__ int s_unit[2 * WARPS], s_ends[2 * WARPS];   // pieces in order: a warp's first, its last
   __shared__ int s_warp[WARPS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * C::RING;
   const uint32_t ring_at = smem_u32(ring);
   int* s_starts = reinterpret_cast<int*>(smem + WARPS * C::RING);        // [batch + 1]
-  int* s_len = s_starts + a.batch + 1;                                    // [batch]
+  uint8_t* s_rest = reinterpret_cast<uint8_t*>(s_starts + a.batch + 1);   // [batch] keys of the last chunk
   const int per_b = a.heads_kv * a.blocks;
   griddep_launch_dependents();
   if (tid < 2 * WARPS) s_unit[tid] = -1;
@@ -212,9 +250,15 @@ __global__ void __launch_bounds__(THREADS, 1) attend_codes8_kernel(const Attend 
       reinterpret_cast<uint4*>(smem)[x] = make_uint4(0, 0, 0, 0);
   griddep_wait();
 
-  // The warp's range [x0, x1) of the list (whole: of the block's unit), per of them a warp.
-  int64_t x0, x1, per;
+  // The warp's part of the list (whole: of the block's unit, chunks alone).
   Place in;
+  in.left = 0;
+  int64_t total = 0, used = 1;           // entries in all, blocks that take some
+  auto set_sequence = [&](Place& p) {
+    p.n = s_starts[p.b + 1] - s_starts[p.b] - STARTS;
+    p.len = (p.n - 1) * KEYS + s_rest[p.b];
+    p.row = a.table + int64_t(a.slots ? a.slots[p.b] : p.b) * a.width;
+  };
   if (a.whole) {
     in.b = int(blockIdx.x) / per_b;
     in.u = int(blockIdx.x) - in.b * per_b;
@@ -226,10 +270,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_codes8_kernel(const Attend 
         store1(out_row<T>(a, in.b, in.u, hb + x / a.d) + x % a.d, 0.f);
       return;
     }
-    per = (in.n + WARPS - 1) / WARPS;
-    x0 = min(warp * per, int64_t(in.n));
-    x1 = min(x0 + per, int64_t(in.n));
-    in.j = int(x0);
+    in.row = a.table + int64_t(a.slots ? a.slots[in.b] : in.b) * a.width;
+    in.j = int(int64_t(in.n) * warp / WARPS);
+    in.left = int(int64_t(in.n) * (warp + 1) / WARPS) - in.j;
     __syncthreads();
   } else {
     int run = 0;
@@ -237,9 +280,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_codes8_kernel(const Attend 
       const int b = b0 + tid;
       int v = 0;
       if (b < a.batch) {
-        const int len = len_at(a, b);
-        s_len[b] = len;
-        v = (len + KEYS - 1) / KEYS;
+        const int len = len_at(a, b), n = (len + KEYS - 1) / KEYS;
+        s_rest[b] = uint8_t(len - (n - 1) * KEYS);
+        v = n > 0 ? n + STARTS : 0;
       }
       int x = v;
 #pragma unroll
@@ -259,11 +302,12 @@ __global__ void __launch_bounds__(THREADS, 1) attend_codes8_kernel(const Attend 
     }
     if (tid == 0) s_starts[a.batch] = run;
     __syncthreads();
-    const int64_t total = int64_t(run) * per_b;
-    per = (total + int64_t(gridDim.x) * WARPS - 1) / (int64_t(gridDim.x) * WARPS);
-    x0 = min((int64_t(blockIdx.x) * WARPS + warp) * per, total);
-    x1 = min(x0 + per, total);
-    if (x0 < x1) {
+    total = int64_t(run) * per_b;
+    used = max(int64_t(1), min(int64_t(gridDim.x), total / (LEAST * WARPS)));
+    const int64_t w = int64_t(blockIdx.x) * WARPS + warp, of = used * WARPS;
+    const int64_t x0 = total * w / of;
+    if (blockIdx.x < used) in.left = int(total * (w + 1) / of - x0);
+    if (in.left > 0) {
       int lo = 0, hi = a.batch;          // the last b with starts[b] * per_b <= x0
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -271,88 +315,116 @@ __global__ void __launch_bounds__(THREADS, 1) attend_codes8_kernel(const Attend 
         else hi = mid;
       }
       in.b = lo;
-      in.len = s_len[lo];
-      in.n = s_starts[lo + 1] - s_starts[lo];
+      set_sequence(in);
       const int64_t within = x0 - int64_t(s_starts[lo]) * per_b;
-      in.u = int(within / in.n);
-      in.j = int(within - int64_t(in.u) * in.n);
+      in.u = int(within / (in.n + STARTS));
+      const int entry = int(within - int64_t(in.u) * (in.n + STARTS));
+      in.j = max(entry - STARTS, 0);
+      in.left -= max(STARTS - entry, 0);
     }
     // Sequences without keys are in nobody's range.
     for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
-      if (s_len[b] == 0)
+      if (s_starts[b + 1] == s_starts[b])
         for (int x = tid; x < a.heads_kv * a.group * a.d; x += THREADS)
           store1(static_cast<T*>(a.out) + b * a.o_batch + int64_t(x / a.d) * a.o_head + x % a.d, 0.f);
   }
 
-  auto find_row = [&](Place& p) {
-    p.row = int64_t(a.slots ? a.slots[p.b] : p.b) * a.width;
+  auto query_row = [&](const Place& p, int head) {
+    const int kvh = p.u / a.blocks;
+    return static_cast<const T*>(a.q) + p.b * a.q_batch +
+           int64_t(kvh * a.group + (p.u - kvh * a.blocks) * C::HEADS + head) * a.q_head;
   };
-  auto advance = [&](Place& p) {         // (called only where another chunk of the range follows)
+  auto heads_of = [&](const Place& p) { return min(C::HEADS, a.group - p.u % a.blocks * C::HEADS); };
+  // The next chunk of the range, if there is one (left > 0).
+  auto advance = [&](Place& p) {
+    --p.left;
     if (++p.j < p.n) return;
+    p.left -= STARTS;
+    if (p.left <= 0) return;
     p.j = 0;
     if (++p.u < per_b) return;
     p.u = 0;
-    do {
-      ++p.b;
-      p.n = s_starts[p.b + 1] - s_starts[p.b];
-    } while (p.n == 0);
-    p.len = s_len[p.b];
-    find_row(p);
+    do ++p.b; while (s_starts[p.b + 1] == s_starts[p.b]);
+    set_sequence(p);
   };
-  // Asks for a chunk's codes and scales; keys behind the last and without a page are zeros.
+
+  // Asks for a chunk's codes and scales; keys behind the last and without a page are zeros.  A lane's
+  // copies go to places that differ by constants, but for the swizzle, which takes two forms.
   const int page_mask = (1 << a.page_shift) - 1, parts = (page_mask + 1) / kScaleBlock;
   const int chunks = a.d >> 4;           // 16-byte chunks of a row
+  constexpr int PER = DT / 16, ROWS = 32 / PER;              // of a row; rows that the lanes copy at once
+  constexpr int FORMS = ROWS == 8 ? 1 : 8 / ROWS;            // the swizzles take the rows' low three bits
+  const int lane_r = lane / PER, lane_c = lane % PER;
+  uint32_t k_to[FORMS], v_to[FORMS];
+#pragma unroll
+  for (int y = 0; y < FORMS; ++y) {
+    k_to[y] = ring_at + k_at<DT>(y * ROWS + lane_r, lane_c);
+    v_to[y] = ring_at + C::TILE + v_at<DT>(y * ROWS + lane_r, lane_c);
+  }
   auto issue = [&](const Place& p, int stage) {
-    const int kvh = p.u / a.blocks;
-    const uint32_t kd = ring_at + stage * 2 * C::TILE, vd = kd + C::TILE;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int key0 = p.j * KEYS + 16 * i, live = min(16, p.len - key0);
-      const int page = live > 0 ? a.table[p.row + (key0 >> a.page_shift)] : -1;
+    const int kvh = p.u / a.blocks, key0 = p.j * KEYS, live = p.len - key0;
+    const uint32_t to = stage * 2 * C::TILE;
+    const bool one = MT == 1 || a.page_shift >= 5;           // all keys of the chunk in a page
+    for (int i = 0; i < MT; i += one ? MT : 1) {
+      const int n = one ? KEYS : 16, from0 = 16 * i, here = live - from0;
+      const int page = here > 0 ? p.row[(key0 + from0) >> a.page_shift] : -1;
       const bool has = page >= 0 && page < a.pages;
-      const int in_page = key0 & page_mask;
-      const int64_t at = has ? (int64_t(kvh) * (page_mask + 1) + in_page) * a.d : 0;
-      const uint8_t* k = a.k + (has ? page * a.k_page + at : 0);
-      const uint8_t* v = a.v + (has ? page * a.v_page + at : 0);
-      constexpr int PER = DT / 16, ROWS = 32 / PER;          // chunks of a row, rows at once
-      const int c = lane % PER;
-#pragma unroll
-      for (int r0 = 0; r0 < 16; r0 += ROWS) {
-        const int r = r0 + lane / PER;
-        const uint32_t bytes = has && r < live ? 16 : 0;
-        const int64_t from = bytes ? int64_t(r) * a.d + c * 16 : 0;
-        if (c < chunks) {
-          cp_async16(kd + k_at<DT>(16 * i + r, c), k + from, bytes);
-          cp_async16(vd + v_at<DT>(16 * i + r, c), v + from, bytes);
+      const int in_page = (key0 + from0) & page_mask;
+      const int64_t at = (int64_t(kvh) * (page_mask + 1) + in_page) * a.d;
+      if (a.fast && one && has && here >= KEYS) {
+        const uint8_t* k = a.k + page * a.k_page + at + lane * 16;
+        const uint8_t* v = a.v + page * a.v_page + at + lane * 16;
+        copy_rows<KEYS / ROWS, FORMS, ROWS * DT>(k_to, to, k);
+        copy_rows<KEYS / ROWS, FORMS, ROWS * DT>(v_to, to, v);
+      } else if (a.fast && has && here >= n) {
+        const uint8_t* k = a.k + page * a.k_page + at + lane * 16;
+        const uint8_t* v = a.v + page * a.v_page + at + lane * 16;
+        copy_rows<16 / ROWS, FORMS, ROWS * DT>(k_to, to + from0 * DT, k);
+        copy_rows<16 / ROWS, FORMS, ROWS * DT>(v_to, to + from0 * DT, v);
+      } else {
+        const uint8_t* k = a.k + (has ? page * a.k_page + at : 0);
+        const uint8_t* v = a.v + (has ? page * a.v_page + at : 0);
+#pragma unroll 1
+        for (int r = lane_r; r < n; r += ROWS) {
+          const uint32_t bytes = has && r < here ? 16 : 0;
+          const int64_t from = bytes ? int64_t(r) * a.d + lane_c * 16 : 0;
+          if (lane_c < chunks) {
+            cp_async16(ring_at + to + k_at<DT>(from0 + r, lane_c), k + from, bytes);
+            cp_async16(ring_at + to + C::TILE + v_at<DT>(from0 + r, lane_c), v + from, bytes);
+          }
         }
       }
-      if (lane < 2) {
-        const float* s = lane ? a.vs : a.ks;
-        const int64_t where = page * (lane ? a.vs_page : a.ks_page) + kvh * parts + in_page / kScaleBlock;
-        cp_async4(smem_u32(&s_scale[warp][stage][lane * MT + i]), s + (has ? where : 0), has ? 4 : 0);
+      const int x = lane % MT;
+      if (lane < 2 * MT && (one || x == i)) {
+        const bool is_v = lane >= MT, there = has && (one ? 16 * x < here : true);
+        const int64_t where = page * (is_v ? a.vs_page : a.ks_page) + kvh * parts +
+                              in_page / kScaleBlock + (one ? x : 0);
+        cp_async4(smem_u32(&s_scale[warp][stage][lane]), (is_v ? a.vs : a.ks) + (there ? where : 0),
+                  there ? 4 : 0);
       }
     }
   };
 
-  uint32_t qf[NT][DT / 16][SPLIT ? 4 : 2];               // queries: both halves of the inner index
-  float cq[NT][2];                                       // what brings a head's scores to log2 units
+  uint32_t qf[NT][DT / 16][PARTS];       // queries
+  float cq[NT][2];                       // what brings a head's scores to log2 units
   float m[NT][2], l[NT][2], o[C::TILES][NT][4];
+  float v0 = 0.f, to_v0 = 0.f;           // bf16: O is in units of v0 2^-9, to_v0 = 2^9 / v0
   auto load_queries = [&](const Place& p) {
-    const int kvh = p.u / a.blocks, hb = (p.u - kvh * a.blocks) * C::HEADS;
+    const int heads = heads_of(p);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int head = hb + nt * 8 + g;
-      const T* row = static_cast<const T*>(a.q) + p.b * a.q_batch + int64_t(kvh * a.group + head) * a.q_head;
+      const T* row = query_row(p, nt * 8 + g);
       float x[DT / 64][16];
       uint32_t top = 0;
 #pragma unroll
       for (int jj = 0; jj < DT / 64; ++jj) {
         const int e = 64 * jj + 16 * t;
-        const bool there = head < a.group && e < a.d;
-        if (there && a.q_vec) {
+        const bool there = nt * 8 + g < heads && e < a.d;
+        if (a.q_vec) {
 #pragma unroll
           for (int i = 0; i < int(sizeof(T)); ++i) {         // 16 elements: 2 or 4 times 16 bytes
-            const uint4 w = *reinterpret_cast<const uint4*>(row + e + i * (16 / int(sizeof(T))));
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (there) w = *reinterpret_cast<const uint4*>(row + e + i * (16 / int(sizeof(T))));
             const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
@@ -385,7 +457,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_codes8_kernel(const Attend 
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float lo = x[jj][4 * s + 2 * i] * up, hi = x[jj][4 * s + 2 * i + 1] * up;
-            if (SPLIT) qf[nt][4 * jj + s][i] = split_halves(lo, hi, &qf[nt][4 * jj + s][(2 + i) % (SPLIT ? 4 : 2)]);
+            if (SPLIT) qf[nt][4 * jj + s][i] = split_halves(lo, hi, &qf[nt][4 * jj + s][(2 + i) % PARTS]);
             else qf[nt][4 * jj + s][i] = pack_halves(lo, hi);
           }
 #pragma unroll
@@ -398,18 +470,15 @@ __global__ void __launch_bounds__(THREADS, 1) attend_codes8_kernel(const Attend 
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[x][nt][i] = 0.f;
     }
+    v0 = to_v0 = 0.f;
   };
 
   auto compute = [&](const Place& p, int stage) {
     const uint32_t kd = ring_at + stage * 2 * C::TILE, vd = kd + C::TILE;
-    const float* sc = s_scale[warp][stage];
+    float sc[2 * MT];                    // s_k, s_v of the chunk's blocks
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) sc[i] = s_scale[warp][stage][i];
     float s[MT][NT][4];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) s[i][nt][x] = 0.f;
 #pragma unroll
     for (int jj = 0; jj < DT / 64; ++jj) {
       if (64 * jj >= a.d) break;
@@ -425,9 +494,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_codes8_kernel(const Attend 
           halves_of4<E4M3>(ys[z], &f[1], &f[3]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma_f16(s[i][nt], f, qf[nt][4 * jj + z][0], qf[nt][4 * jj + z][1]);
-            if (SPLIT) mma_f16(s[i][nt], f, qf[nt][4 * jj + z][2 % (SPLIT ? 4 : 2)],
-                               qf[nt][4 * jj + z][3 % (SPLIT ? 4 : 2)]);
+            if (jj + z == 0) mma_f16_first(s[i][nt], f, qf[nt][0][0], qf[nt][0][1]);
+            else mma_f16(s[i][nt], f, qf[nt][4 * jj + z][0], qf[nt][4 * jj + z][1]);
+            if (SPLIT) mma_f16(s[i][nt], f, qf[nt][4 * jj + z][2 % PARTS], qf[nt][4 * jj + z][3 % PARTS]);
           }
         }
       }
@@ -455,73 +524,136 @@ __global__ void __launch_bounds__(THREADS, 1) attend_codes8_kernel(const Attend 
           }
         }
       }
-    const bool last = (p.j + 1) * KEYS > p.len;              // some of its keys do not count
-    float top_v = 0.f, ratio[MT];
+    float top_v = 0.f;
 #pragma unroll
     for (int i = 0; i < MT; ++i) top_v = fmaxf(top_v, fabsf(sc[MT + i]));
+    // Scores in log2 units, and each lane's largest.
+    float top[NT][2];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const float x = sc[MT + i];
-      ratio[i] = x == 0.f ? 0.f : fabsf(x) == top_v ? copysignf(1.f, x) : x / top_v;
-    }
-    uint32_t pf[MT][NT][SPLIT ? 4 : 2];
-    float fresh[NT][2];
-    bool grown = false;
-    float shrink[NT][2];
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+      for (int i = 0; i < MT; ++i) {
+        const float c[2] = {sc[i] * cq[nt][0], sc[i] * cq[nt][1]};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[i][nt][x] *= c[x & 1];
+      }
+    if ((p.j + 1) * KEYS > p.len) {                          // some keys do not count
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          s[i][nt][x] *= sc[i] * cq[nt][x & 1];
-          if (last && p.j * KEYS + 16 * i + g + 8 * (x >> 1) >= p.len) s[i][nt][x] = -INFINITY;
-          top[x & 1] = fmaxf(top[x & 1], s[i][nt][x]);
-        }
+        for (int x = 0; x < 2; ++x)
+          if (p.j * KEYS + 16 * i + g + 8 * x >= p.len)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[i][nt][2 * x] = s[i][nt][2 * x + 1] = -INFINITY;
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        top[x] = max_over_keys(top[x]);
-        const float now = fmaxf(m[nt][x], top[x]), base = base_of(now);
-        grown |= now != m[nt][x];
-        shrink[nt][x] = ex2(m[nt][x] - base);
-        fresh[nt][x] = ex2(top[x] - base);
-        m[nt][x] = now;
-        top[x] = 15.f - base_of(top[x]);
+        top[nt][x] = fmaxf(s[0][nt][x], s[0][nt][2 + x]);
+#pragma unroll
+        for (int i = 1; i < MT; ++i) top[nt][x] = fmaxf(top[nt][x], fmaxf(s[i][nt][x], s[i][nt][2 + x]));
       }
+    uint32_t pf[MT][NT][PARTS];
+    float fresh[NT][2];                  // fp32: what brings the chunk's product to O's units
+    if (SPLIT) {
+      float ratio[MT];
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        float w[4];
+        const float x = sc[MT + i];
+        ratio[i] = x == 0.f ? 0.f : fabsf(x) == top_v ? copysignf(1.f, x) : x / top_v;
+      }
+      bool grown = false;
+      float shrink[NT][2];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          w[x] = ex2(s[i][nt][x] + top[x & 1]);
-          sum[x & 1] += w[x];
-          w[x] *= ratio[i];
+      for (int nt = 0; nt < NT; ++nt) {
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float here = max_over_keys(top[nt][x]);
+          const float now = fmaxf(m[nt][x], here), base = base_of(now);
+          grown |= now != m[nt][x];
+          shrink[nt][x] = ex2(m[nt][x] - base);
+          fresh[nt][x] = ex2(here - base);
+          m[nt][x] = now;
+          top[nt][x] = 15.f - base_of(here);
         }
-        if (SPLIT) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          float w[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            w[x] = ex2(s[i][nt][x] + top[nt][x & 1]);
+            sum[x & 1] += w[x];
+            w[x] *= ratio[i];
+          }
           uint32_t r0, r1;
           pf[i][nt][0] = turn_8x8(split_halves(w[0], w[1], &r0));
           pf[i][nt][1] = turn_8x8(split_halves(w[2], w[3], &r1));
-          pf[i][nt][2 % (SPLIT ? 4 : 2)] = turn_8x8(r0);
-          pf[i][nt][3 % (SPLIT ? 4 : 2)] = turn_8x8(r1);
-        } else {
-          pf[i][nt][0] = turn_8x8(pack_halves(w[0], w[1]));
-          pf[i][nt][1] = turn_8x8(pack_halves(w[2], w[3]));
+          pf[i][nt][2 % PARTS] = turn_8x8(r0);
+          pf[i][nt][3 % PARTS] = turn_8x8(r1);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          l[nt][x] = l[nt][x] * shrink[nt][x] + sum[x] * fresh[nt][x];
+          fresh[nt][x] *= top_v;
         }
       }
+      if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        l[nt][x] = l[nt][x] * shrink[nt][x] + sum[x] * fresh[nt][x];
-        fresh[nt][x] *= top_v;
+        for (int x = 0; x < C::TILES; ++x)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[x][nt][i] *= shrink[nt][i & 1];
       }
-    }
-    if (__any_sync(0xffffffffu, grown)) {
+    } else {
+      bool past = top_v > 4.f * v0;
 #pragma unroll
-      for (int x = 0; x < C::TILES; ++x)
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) past |= top[nt][x] > m[nt][x] + 4.f;
+      if (__any_sync(0xffffffffu, past)) {                   // new references
+        float shrink[NT][2], change = 1.f;
+        if (top_v > v0) {
+          const float was = v0;
+          v0 = fmaxf(top_v, 0x1p-100f);
+          to_v0 = 512.f / v0;
+          change = was / v0;
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[x][nt][i] *= shrink[nt][i & 1];
+          for (int x = 0; x < 2; ++x) {
+            const float now = fmaxf(m[nt][x], max_over_keys(top[nt][x]));
+            shrink[nt][x] = ex2(m[nt][x] - base_of(now));
+            m[nt][x] = now;
+            l[nt][x] *= shrink[nt][x];
+            shrink[nt][x] *= change;
+          }
+#pragma unroll
+        for (int x = 0; x < C::TILES; ++x)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[x][nt][i] *= shrink[nt][i & 1];
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float base[2] = {base_of(m[nt][0]), base_of(m[nt][1])};
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const float r = sc[MT + i] * to_v0;
+          float w[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            w[x] = ex2(s[i][nt][x] - base[x & 1]);
+            l[nt][x & 1] += w[x];
+          }
+          pf[i][nt][0] = turn_8x8(pack_halves(w[0] * r, w[1] * r));
+          pf[i][nt][1] = turn_8x8(pack_halves(w[2] * r, w[3] * r));
+        }
+      }
     }
 #pragma unroll
     for (int z = 0; z < WORDS; ++z)
@@ -529,36 +661,40 @@ __global__ void __launch_bounds__(THREADS, 1) attend_codes8_kernel(const Attend 
       for (int half = 0; half < 2; ++half) {
         float acc[NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) acc[nt][x] = 0.f;
-#pragma unroll
         for (int i = 0; i < MT; ++i) {
           uint32_t f[4];
           halves_of4<E4M3>(__byte_perm(vw[i][0][z], vw[i][1][z], half ? 0x7362 : 0x5140), &f[0], &f[1]);
           halves_of4<E4M3>(__byte_perm(vw[i][2][z], vw[i][3][z], half ? 0x7362 : 0x5140), &f[2], &f[3]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma_f16(acc[nt], f, pf[i][nt][0], pf[i][nt][1]);
-            if (SPLIT) mma_f16(acc[nt], f, pf[i][nt][2 % (SPLIT ? 4 : 2)], pf[i][nt][3 % (SPLIT ? 4 : 2)]);
+            if (!SPLIT) {
+              mma_f16(o[2 * z + half][nt], f, pf[i][nt][0], pf[i][nt][1]);
+              continue;
+            }
+            if (i == 0) mma_f16_first(acc[nt], f, pf[i][nt][0], pf[i][nt][1]);
+            else mma_f16(acc[nt], f, pf[i][nt][0], pf[i][nt][1]);
+            mma_f16(acc[nt], f, pf[i][nt][2 % PARTS], pf[i][nt][3 % PARTS]);
           }
         }
+        if (SPLIT)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            o[2 * z + half][nt][x] = fmaf(acc[nt][x], fresh[nt][x & 1], o[2 * z + half][nt][x]);
+            for (int x = 0; x < 4; ++x)
+              o[2 * z + half][nt][x] = fmaf(acc[nt][x], fresh[nt][x & 1], o[2 * z + half][nt][x]);
       }
   };
 
-  if (x0 < x1) {
-    find_row(in);
+  if (in.left > 0) {
     Place at = in;
-    int64_t asked = x0;
     auto next = [&](int stage) {
-      if (asked < x1) {
+      if (in.left > 0) {
         issue(in, stage);
-        if (++asked < x1) advance(in);
+        const int u = in.u, b = in.b;
+        advance(in);
+        if (in.left > 0 && (in.u != u || in.b != b) && g < heads_of(in))   // its queries, ahead
+          for (int x = t * 64; x < a.d * int(sizeof(T)); x += 256)
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(reinterpret_cast<const uint8_t*>(query_row(in, g)) + x));
       }
       cp_commit();
     };
@@ -566,7 +702,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_codes8_kernel(const Attend 
     for (int s = 0; s < C::STAGES - 1; ++s) next(s);
     int st = 0, to = C::STAGES - 1;
     bool fresh = true, began = false;
-    for (int64_t x = x0; x < x1; ++x) {
+    while (at.left > 0) {
       if (fresh) {
         load_queries(at);
         began = at.j == 0;
@@ -578,136 +714,129 @@ __global__ void __launch_bounds__(THREADS, 1) attend_codes8_kernel(const Attend 
       compute(at, st);
       st = st + 1 == C::STAGES ? 0 : st + 1;
       to = to + 1 == C::STAGES ? 0 : to + 1;
-      const bool end = at.j + 1 == at.n, over = x + 1 == x1;
+      const bool end = at.j + 1 == at.n;
+      const bool over = at.left - 1 - (end && !a.whole ? STARTS : 0) <= 0;
       if (end || over) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int y = 0; y < 2; ++y) l[nt][y] = sum_over_keys(l[nt][y]);
+        const float unit = SPLIT ? 1.f : v0 * (1.f / 512.f);
         if (began && end) {              // all of the unit
-          const int hb = at.u % a.blocks * C::HEADS;
+          const int heads = heads_of(at), hb = at.u % a.blocks * C::HEADS;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-              const int head = hb + nt * 8 + 2 * t + y;
-              if (head >= a.group) continue;
-              T* row = out_row<T>(a, at.b, at.u, head);
-              const float sum = l[nt][y], inv = 1.f / sum;
+              const int head = nt * 8 + 2 * t + y;
+              if (head >= heads) continue;
+              T* row = out_row<T>(a, at.b, at.u, hb + head);
+              const float f = l[nt][y] == 0.f ? 0.f : unit / l[nt][y];
 #pragma unroll
               for (int mt = 0; mt < C::TILES; ++mt) {
                 const int e = element_of<DT>(mt, g);
-                if (e < a.d)
-                  store_pair(row + e, sum == 0.f ? 0.f : o[mt][nt][y] * inv,
-                             sum == 0.f ? 0.f : o[mt][nt][2 + y] * inv, a.o_vec);
+                if (e < a.d) store_pair(row + e, o[mt][nt][y] * f, o[mt][nt][2 + y] * f, a.o_vec);
               }
             }
         } else {
           // A first piece that others follow goes to the workspace, a last one where the copies were.
           __syncwarp();
+          const int i = 2 * warp + over;
           float* to_o = over ? reinterpret_cast<float*>(ring)
-                             : a.pieces + (int64_t(blockIdx.x) * SLOTS + warp) * C::SLOT;
-          float* to_m = over ? s_m[warp] : to_o + C::PIECE;
-          float* to_l = over ? s_l[warp] : to_m + C::HEADS;
+                             : a.pieces + (int64_t(blockIdx.x) * C::SLOTS + warp) * C::SLOT;
 #pragma unroll
           for (int mt = 0; mt < C::TILES; ++mt)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int y = 0; y < 4; ++y) to_o[((mt * NT + nt) * 4 + y) * 32 + lane] = o[mt][nt][y];
+              for (int y = 0; y < 4; ++y) to_o[((mt * NT + nt) * 4 + y) * 32 + lane] = o[mt][nt][y] * unit;
           if (g == 0)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int y = 0; y < 2; ++y) {
-                to_m[nt * 8 + 2 * t + y] = m[nt][y];
-                to_l[nt * 8 + 2 * t + y] = l[nt][y];
+                s_m[i][nt * 8 + 2 * t + y] = m[nt][y];
+                s_l[i][nt * 8 + 2 * t + y] = l[nt][y];
               }
           if (lane == 0) {
-            s_unit[2 * warp + over] = at.b * per_b + at.u;
-            s_ends[2 * warp + over] = (began ? 1 : 0) | (end ? 2 : 0);
+            s_unit[i] = at.b * per_b + at.u;
+            s_ends[i] = (began ? 1 : 0) | (end ? 2 : 0);
           }
         }
         fresh = true;
       }
-      if (!over) advance(at);
+      advance(at);
     }
   }
   __syncthreads();
 
   // The warps' pieces, unit by unit.
   if (!a.whole && tid == 0) a.links[blockIdx.x] = make_int2(0, 0);
-  for (int i0 = 0; i0 < 2 * WARPS;) {
-    const int unit = s_unit[i0];
-    if (unit < 0) {
-      ++i0;
-      continue;
+  const int mine = lane < 2 * WARPS ? s_unit[lane] : -1;
+  uint32_t rest = __ballot_sync(0xffffffffu, mine >= 0);
+  while (rest != 0) {
+    const int first = __ffs(rest) - 1, unit = s_unit[first];
+    const uint32_t these = __ballot_sync(0xffffffffu, mine == unit);
+    rest &= ~these;
+    const bool began = s_ends[first] & 1, end = s_ends[31 - __clz(these)] & 2, done = began && end;
+    float* to = a.pieces + (int64_t(blockIdx.x) * C::SLOTS + (began ? C::AFTER : C::BEFORE)) * C::SLOT;
+    for (int h = warp; h < C::HEADS; h += WARPS) {           // lane: piece
+      const bool one = these >> lane & 1;
+      const float pm = one ? s_m[lane % (2 * WARPS)][h] : -INFINITY;
+      const float pl = one ? s_l[lane % (2 * WARPS)][h] : 0.f;
+      float top = pm;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float w = ex2(pm - base_of(top));
+      float sum = one ? pl * w : 0.f;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      if (one) s_w[lane % (2 * WARPS)][h] = !done ? w : sum == 0.f ? 0.f : w / sum;
+      if (!done && lane == 0) {
+        to[C::PIECE + h] = top;
+        to[C::PIECE + C::HEADS + h] = sum;
+      }
     }
-    int i1 = i0 + 1, tail = i0;
-    while (i1 < 2 * WARPS && (s_unit[i1] < 0 || s_unit[i1] == unit)) {
-      if (s_unit[i1] >= 0) tail = i1;
-      ++i1;
-    }
-    const bool began = s_ends[i0] & 1, end = s_ends[tail] & 2;
+    __syncthreads();
     const int b = unit / per_b, u = unit - b * per_b, hb = u % a.blocks * C::HEADS;
-    float* to = a.pieces + (int64_t(blockIdx.x) * SLOTS + (began ? AFTER : BEFORE)) * C::SLOT;
     for (int x = warp; x < C::TILES * NT; x += WARPS) {
       const int mt = x / NT, nt = x % NT, h0 = nt * 8 + 2 * t;
-      float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int i = i0; i <= tail; ++i) {
-        if (s_unit[i] < 0) continue;
-        const float* piece = a.pieces + (int64_t(blockIdx.x) * SLOTS + (i >> 1)) * C::SLOT;
-        const float* pm = i & 1 ? s_m[i >> 1] : piece + C::PIECE;
-        top[0] = fmaxf(top[0], pm[h0]);
-        top[1] = fmaxf(top[1], pm[h0 + 1]);
-      }
-      for (int i = i0; i <= tail; ++i) {
-        if (s_unit[i] < 0) continue;
-        const float* piece = a.pieces + (int64_t(blockIdx.x) * SLOTS + (i >> 1)) * C::SLOT;
-        const float* pm = i & 1 ? s_m[i >> 1] : piece + C::PIECE;
-        const float* pl = i & 1 ? s_l[i >> 1] : piece + C::PIECE + C::HEADS;
-        const float* po = i & 1 ? reinterpret_cast<const float*>(smem + (i >> 1) * C::RING) : piece;
-        float w[2];
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          w[y] = ex2(pm[h0 + y] - base_of(top[y]));
-          sum[y] += pl[h0 + y] * w[y];
-        }
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      for (uint32_t bits = these; bits != 0; bits &= bits - 1) {
+        const int i = __ffs(bits) - 1;
+        const float* po = i & 1 ? reinterpret_cast<const float*>(smem + (i >> 1) * C::RING)
+                                : a.pieces + (int64_t(blockIdx.x) * C::SLOTS + (i >> 1)) * C::SLOT;
+        const float w[2] = {s_w[i][h0], s_w[i][h0 + 1]};
 #pragma unroll
         for (int y = 0; y < 4; ++y) acc[y] += po[((mt * NT + nt) * 4 + y) * 32 + lane] * w[y & 1];
       }
-      if (began && end) {
+      if (done) {
         const int e = element_of<DT>(mt, g);
 #pragma unroll
         for (int y = 0; y < 2; ++y)
           if (hb + h0 + y < a.group && e < a.d)
-            store_pair(out_row<T>(a, b, u, hb + h0 + y) + e, sum[y] == 0.f ? 0.f : acc[y] / sum[y],
-                       sum[y] == 0.f ? 0.f : acc[2 + y] / sum[y], a.o_vec);
+            store_pair(out_row<T>(a, b, u, hb + h0 + y) + e, acc[y], acc[2 + y], a.o_vec);
       } else {
 #pragma unroll
         for (int y = 0; y < 4; ++y) to[((mt * NT + nt) * 4 + y) * 32 + lane] = acc[y];
-        if (mt == 0 && g == 0)
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            to[C::PIECE + h0 + y] = top[y];
-            to[C::PIECE + C::HEADS + h0 + y] = sum[y];
-          }
       }
     }
     if (began && !end && tid == 0) {     // (the last unit of the block: written after the zero above)
-      const int64_t n = s_starts[b + 1] - s_starts[b];
-      const int64_t stop = int64_t(s_starts[b]) * per_b + (u + 1) * n;
-      a.links[blockIdx.x] = make_int2(unit, int((stop - 1) / (per * WARPS)) - int(blockIdx.x) + 1);
+      const int64_t entries = s_starts[b + 1] - s_starts[b];
+      const int64_t stop = int64_t(s_starts[b]) * per_b + (u + 1) * entries;
+      const int last = int((stop * used - 1) / total);                   // the block that has its end
+      a.links[blockIdx.x] = make_int2(unit, last - int(blockIdx.x) + 1);
     }
-    i0 = i1;
+    if (rest != 0) __syncthreads();      // s_w is written again
   }
 }
 
 // Block (c, x): tile x of O of the unit that began in block c and went on behind it.  Its warps take
 // every eighth part, then the block joins the warps.
 template <typename T, int DT, int NT>
-__global__ void __launch_bounds__(THREADS) join_codes8_kernel(const Attend a) {
-  using C = Cfg<DT, NT>;
+__global__ void __launch_bounds__(256) join_codes8_kernel(const Attend a) {
+  using C = Cfg<T, DT, NT>;
+  constexpr int WARPS = 8;
   __shared__ float s_o[WARPS][4][32], s_m[WARPS][8], s_l[WARPS][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int mt = int(blockIdx.y) / NT, nt = int(blockIdx.y) % NT, h0 = nt * 8 + 2 * t;
@@ -719,7 +848,7 @@ __global__ void __launch_bounds__(THREADS) join_codes8_kernel(const Attend a) {
 #pragma unroll 4
   for (int i = warp; i < link.y; i += WARPS) {
     const float* piece =
-        a.pieces + (int64_t(blockIdx.x + i) * SLOTS + (i == 0 ? AFTER : BEFORE)) * C::SLOT;
+        a.pieces + (int64_t(blockIdx.x + i) * C::SLOTS + (i == 0 ? C::AFTER : C::BEFORE)) * C::SLOT;
     float x[4], pm[2], pl[2];
 #pragma unroll
     for (int y = 0; y < 4; ++y) x[y] = piece[((mt * NT + nt) * 4 + y) * 32 + lane];
@@ -786,29 +915,38 @@ size_t slot_floats(const enigma_sdpa_quantized_desc& d) {
   return heads * dt + 2 * heads;
 }
 
+template <typename T>
+size_t slots_of(const enigma_sdpa_quantized_desc& d) {
+  if (d.head_dim > 128) return Cfg<T, 256, 1>::SLOTS;
+  if constexpr (sizeof(T) == 2)
+    if (tiles_of(d) == 2) return d.head_dim > 64 ? Cfg<T, 128, 2>::SLOTS : Cfg<T, 64, 2>::SLOTS;
+  return d.head_dim > 64 ? Cfg<T, 128, 1>::SLOTS : Cfg<T, 64, 1>::SLOTS;
+}
+
 template <typename T, bool E4M3, int DT, int NT>
 cudaError_t launch(const enigma_sdpa_quantized_desc& d, Attend a, cudaStream_t s) {
-  using C = Cfg<DT, NT>;
+  using C = Cfg<T, DT, NT>;
   a.blocks = (a.group + C::HEADS - 1) / C::HEADS;
   a.whole = whole(d) ? 1 : 0;
+  a.fast = a.d == DT;
   const int sms = enigma::sm_count();
-  const size_t smem = size_t(WARPS) * C::RING + (a.whole ? 0 : (2 * size_t(d.batch) + 1) * 4);
+  const size_t smem = size_t(C::WARPS) * C::RING + (a.whole ? 0 : size_t(d.batch) * 5 + 4);
   auto* kernel = attend_codes8_kernel<T, E4M3, DT, NT>;
   static std::atomic<uint64_t> ready{0};                     // devices where the attribute is set
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && !(dev < 64 && (ready.load() >> dev & 1))) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             WARPS * C::RING + (2 * 4096 + 1) * 4);
+                             C::WARPS * C::RING + 4096 * 5 + 4);
     if (e == cudaSuccess && dev < 64) ready.fetch_or(uint64_t(1) << dev);
   }
   if (e != cudaSuccess) return e;
   a.links = static_cast<int2*>(d.workspace);
   a.pieces = static_cast<float*>(d.workspace) + (sms * 2 + 63) / 64 * 64;
   const unsigned grid = a.whole ? unsigned(units_of(d)) : unsigned(sms);
-  e = enigma::launch_dependent(kernel, grid, THREADS, smem, s, a);
+  e = enigma::launch_dependent(kernel, grid, C::THREADS, smem, s, a);
   if (e != cudaSuccess || a.whole) return e;
-  return enigma::launch_dependent(join_codes8_kernel<T, DT, NT>, dim3(grid, C::TILES * NT), THREADS, 0, s,
+  return enigma::launch_dependent(join_codes8_kernel<T, DT, NT>, dim3(grid, C::TILES * NT), 256, 0, s,
                                   a);
 }
 
@@ -828,7 +966,8 @@ namespace enigma {
 size_t sdpa_quantized_workspace(const enigma_sdpa_quantized_desc& d) {
   if (d.batch == 0 || whole(d)) return 0;
   const size_t sms = size_t(sm_count());
-  return ((sms * 2 + 63) / 64 * 64 + sms * SLOTS * slot_floats(d)) * sizeof(float);
+  const size_t slots = d.dtype == ENIGMA_DTYPE_F32 ? slots_of<float>(d) : slots_of<__nv_bfloat16>(d);
+  return ((sms * 2 + 63) / 64 * 64 + sms * slots * slot_floats(d)) * sizeof(float);
 }
 
 cudaError_t sdpa_quantized_launch(const enigma_sdpa_quantized_desc& d, cudaStream_t s) {

@@ -329,20 +329,22 @@ def _attend(cuda, rng, cache, want, heads_q, dtype, slots=None, scale=None, laye
     out = cache.attend(layer, _dev(q, dtype, cuda), slots=slots, scale=scale, **kw)
     k, v = want.values(layer)
     ref = srv.paged(q, k, v, want.table, want.lens, 0, 1 / np.sqrt(d) if scale is None else scale, slots)
-    return _np(out), (*ref, _floor(want, layer))
+    return _np(out), (*ref, _floor(want, dtype, layer))
 
 
-def _floor(want, layer=0):
+def _floor(want, dtype, layer=0):
     """What rounding a weight to fp16 may cost a key where the relative bound is less.
 
-    A key's weight over the largest of its chunk, times s_v over the larger s_v of the chunk, times
-    2^15, is rounded to a number (in fp32: to what is left by a first one) whose distance from it is
-    half the least fp16, 2^-25, where it is not relative.  Multiplied back by 2^-15, the chunk's s_v
-    and the key's code, and divided by a sum of weights that is 1 or more (its largest is 1), that
-    is 2^-40 max|s_v| max|code| for each key.  It counts for an element to which only keys of
-    small weight contribute, the others' codes being zero."""
+    Half the least fp16 is 2^-25.  bf16: a key's weight, in units of one that is at most 2^4 times
+    less than the largest weight, times s_v over a v0 that is at most the largest |s_v|, times 2^9, is
+    rounded; multiplied back by v0 2^-9 and the key's code, and divided by a sum of weights that is
+    1 or more in those units (they are the weight of a key that was seen), that is at most 2^-34
+    max|s_v| max|code| for each key.  fp32: the weight over the largest of its chunk, times s_v over
+    the chunk's larger one, times 2^15, in two numbers, of which the second is rounded so: 2^-40.  It
+    counts for an element to which only keys of small weight contribute, the others' codes being zero."""
     codes = want.v[layer]
-    return 2.0 ** -40 * np.abs(want.scales[1][layer]).max() * np.abs(codes).max()
+    return 2.0 ** (-34 if dtype == "bf16" else -40) * np.abs(want.scales[1][layer]).max() \
+        * np.abs(codes).max()
 
 
 def _hold(got, ref, keys, dtype):
@@ -528,7 +530,7 @@ def test_attend_strided(cuda, dtype, gap, d):
     assert cache.attend(2, q, out=view, scale=0.2).data_ptr() == view.data_ptr()
     k, v = want.values(2)
     n = wide[:, gap:].reshape(b, hq + 2 * hk, d)[:, :hq]
-    _hold(_np(view), (*srv.paged(n, k, v, want.table, want.lens, 0, 0.2), _floor(want, 2)), 200, dtype)
+    _hold(_np(view), (*srv.paged(n, k, v, want.table, want.lens, 0, 0.2), _floor(want, dtype, 2)), 200, dtype)
     assert (out[:, :gap + d] == 7).all()
     # Every second page of a larger pool: a page stride of its own.
     pool = [x[0] for x in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
@@ -538,7 +540,7 @@ def test_attend_strided(cuda, dtype, gap, d):
         doubled.append(y[::2])
     got = cuda_ops.sdpa_quantized(q, *doubled, cache.table, cache.lens, scale=0.2)
     k, v = want.values(0)
-    _hold(_np(got), (*srv.paged(n, k, v, want.table, want.lens, 0, 0.2), _floor(want)), 200, dtype)
+    _hold(_np(got), (*srv.paged(n, k, v, want.table, want.lens, 0, 0.2), _floor(want, dtype)), 200, dtype)
     one = cuda_ops.sdpa_quantized(q[1:2], *doubled, cache.table[1:2], cache.lens[1:2], scale=0.2)
     assert (one == got[1:2]).all() or np.abs(_np(one) - _np(got[1:2])).max() < 0.1
 
@@ -699,5 +701,5 @@ def test_together(cuda, code, heads_q, heads_kv, d, layout, rotary):
             assert (np.abs(_np(x) - ref) <= tol).all()
         _same(cache, want)
         ref = srv.paged(_np(q), *want.values(layer), want.table, want.lens, 0, 1 / np.sqrt(d), [3, 4, 5])
-        _hold(_np(out), (*ref, _floor(want, layer)), max(at) + 1, "bf16")
+        _hold(_np(out), (*ref, _floor(want, "bf16", layer)), max(at) + 1, "bf16")
     cache.check()
