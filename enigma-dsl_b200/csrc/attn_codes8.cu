@@ -47,12 +47,12 @@ constexpr int LEAST = 3;
 template <typename T, int DT, int NT>
 struct Cfg {
   // As many warps as their registers leave room for: O, queries and a chunk's operands.
-  static constexpr int WARPS = DT * NT * int(sizeof(T)) <= 128 ? 16 : DT * NT * int(sizeof(T)) <= 256 ? 12 : 8;
+  static constexpr int WARPS = NT == 1 && DT < 256 || DT * NT <= 128 ? 12 : 8;
   static constexpr int THREADS = WARPS * 32;
   static constexpr int SLOTS = WARPS + 2;                // pieces of a block in the workspace: its warps'
   static constexpr int BEFORE = WARPS;                   // first ones, what it has of a unit that began
   static constexpr int AFTER = WARPS + 1;                // in another block, and of one that goes on
-  static constexpr int KEYS = DT == 256 ? 16 : 32;       // of a chunk
+  static constexpr int KEYS = 4096 / DT;                  // of a chunk: 4 KB of K, as much of V
   static constexpr int MT = KEYS / 16;                    // 16-key tiles, scale blocks
   static constexpr int TILE = KEYS * DT;                  // bytes of K or V
   static constexpr int STAGES = (192 << 10) / (WARPS * 2 * TILE);
@@ -180,6 +180,11 @@ __device__ __forceinline__ int len_at(const Attend& a, int b) {
   return int(min(int64_t(max(a.lens[slot], 0)), int64_t(a.width) << a.page_shift));
 }
 
+// x / y, in 32 bits where that is enough (a 64-bit division takes several times as long).
+__device__ __forceinline__ int64_t quotient(int64_t x, uint32_t y) {
+  return x >> 32 ? x / y : int64_t(uint32_t(x) / y);
+}
+
 // A place in the work list: chunk j of the n of a unit; entries left in the warp's range.
 struct Place {
   int b, u, j, n, len, left;
@@ -225,17 +230,23 @@ __device__ __forceinline__ T* out_row(const Attend& a, int b, int u, int head) {
   return static_cast<T*>(a.out) + b * a.o_batch + int64_t(kvh * a.group + head) * a.o_head;
 }
 
+// What a block's warps left, in order: a warp's first piece, its last.
+template <typename C>
+struct Pieces {
+  float m[2 * C::WARPS][C::HEADS], l[2 * C::WARPS][C::HEADS], w[2 * C::WARPS][C::HEADS];
+  int unit[2 * C::WARPS], ends[2 * C::WARPS];            // -1: none; 1: has its unit's first key, 2: the last
+};
+
 // T: of queries and results; DT: the head's elements, rounded up; NT: tiles of 8 query heads.
 template <typename T, bool E4M3, int DT, int NT>
-__global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kernel(const Attend a) {
+__global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kernel(const __grid_constant__ Attend a) {
   using C = Cfg<T, DT, NT>;
   constexpr bool SPLIT = sizeof(T) == 4;
   constexpr int MT = C::MT, KEYS = C::KEYS, WARPS = C::WARPS, THREADS = C::THREADS;
   constexpr int PARTS = SPLIT ? 4 : 2;   // registers of an operand: two halves of the inner index
   extern __shared__ __align__(128) uint8_t smem[];       // rings, list entries before each b, last chunks
   __shared__ __align__(16) float s_scale[WARPS][C::STAGES][2 * MT];
-  __shared__ float s_m[2 * WARPS][C::HEADS], s_l[2 * WARPS][C::HEADS], s_w[2 * WARPS][C::HEADS];
-  __shared__ int s_unit[2 * WARPS], s_ends[2 * WARPS];   // pieces in order: a warp's first, its last
+  __shared__ Pieces<C> s_pieces;
   __shared__ int s_warp[WARPS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * C::RING;
@@ -244,7 +255,7 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
   uint8_t* s_rest = reinterpret_cast<uint8_t*>(s_starts + a.batch + 1);   // [batch] keys of the last chunk
   const int per_b = a.heads_kv * a.blocks;
   griddep_launch_dependents();
-  if (tid < 2 * WARPS) s_unit[tid] = -1;
+  if (tid < 2 * WARPS) s_pieces.unit[tid] = -1;
   if (a.d < DT)                          // columns that no copy fills
     for (int x = tid; x < WARPS * C::RING / 16; x += THREADS)
       reinterpret_cast<uint4*>(smem)[x] = make_uint4(0, 0, 0, 0);
@@ -303,10 +314,12 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
     if (tid == 0) s_starts[a.batch] = run;
     __syncthreads();
     total = int64_t(run) * per_b;
-    used = max(int64_t(1), min(int64_t(gridDim.x), total / (LEAST * WARPS)));
-    const int64_t w = int64_t(blockIdx.x) * WARPS + warp, of = used * WARPS;
-    const int64_t x0 = total * w / of;
-    if (blockIdx.x < used) in.left = int(total * (w + 1) / of - x0);
+    used = max(int64_t(1), min(int64_t(gridDim.x), quotient(total, LEAST * WARPS)));
+    const uint32_t w = blockIdx.x * WARPS + warp, of = uint32_t(used) * WARPS;
+    const int64_t each = quotient(total, of);
+    const uint32_t more = uint32_t(total - each * of);       // (below of: grids are small)
+    const int64_t x0 = each * w + w * more / of;
+    if (blockIdx.x < used) in.left = int(each + (w + 1) * more / of - w * more / of);
     if (in.left > 0) {
       int lo = 0, hi = a.batch;          // the last b with starts[b] * per_b <= x0
       while (hi - lo > 1) {
@@ -317,7 +330,7 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
       in.b = lo;
       set_sequence(in);
       const int64_t within = x0 - int64_t(s_starts[lo]) * per_b;
-      in.u = int(within / (in.n + STARTS));
+      in.u = int(quotient(within, in.n + STARTS));
       const int entry = int(within - int64_t(in.u) * (in.n + STARTS));
       in.j = max(entry - STARTS, 0);
       in.left -= max(STARTS - entry, 0);
@@ -364,7 +377,7 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
   auto issue = [&](const Place& p, int stage) {
     const int kvh = p.u / a.blocks, key0 = p.j * KEYS, live = p.len - key0;
     const uint32_t to = stage * 2 * C::TILE;
-    const bool one = MT == 1 || a.page_shift >= 5;           // all keys of the chunk in a page
+    const bool one = page_mask + 1 >= KEYS;                  // all keys of the chunk in a page
     for (int i = 0; i < MT; i += one ? MT : 1) {
       const int n = one ? KEYS : 16, from0 = 16 * i, here = live - from0;
       const int page = here > 0 ? p.row[(key0 + from0) >> a.page_shift] : -1;
@@ -708,6 +721,8 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
         began = at.j == 0;
         fresh = false;
       }
+      // (Asking for a chunk as soon as the codes before it are in registers, in the middle of a chunk's
+      // work, has more in flight but is slower: 292 against 272 us for 192 long contexts.)
       cp_wait<C::STAGES - 2>();
       __syncwarp();                      // every lane's copies, and nobody reads the stage before
       next(to);
@@ -755,12 +770,12 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int y = 0; y < 2; ++y) {
-                s_m[i][nt * 8 + 2 * t + y] = m[nt][y];
-                s_l[i][nt * 8 + 2 * t + y] = l[nt][y];
+                s_pieces.m[i][nt * 8 + 2 * t + y] = m[nt][y];
+                s_pieces.l[i][nt * 8 + 2 * t + y] = l[nt][y];
               }
           if (lane == 0) {
-            s_unit[i] = at.b * per_b + at.u;
-            s_ends[i] = (began ? 1 : 0) | (end ? 2 : 0);
+            s_pieces.unit[i] = at.b * per_b + at.u;
+            s_pieces.ends[i] = (began ? 1 : 0) | (end ? 2 : 0);
           }
         }
         fresh = true;
@@ -770,20 +785,23 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
   }
   __syncthreads();
 
-  // The warps' pieces, unit by unit.
+  // The pieces of each unit: to the result, or to a piece of the block's.
   if (!a.whole && tid == 0) a.links[blockIdx.x] = make_int2(0, 0);
-  const int mine = lane < 2 * WARPS ? s_unit[lane] : -1;
-  uint32_t rest = __ballot_sync(0xffffffffu, mine >= 0);
-  while (rest != 0) {
-    const int first = __ffs(rest) - 1, unit = s_unit[first];
-    const uint32_t these = __ballot_sync(0xffffffffu, mine == unit);
+  const int mine = lane < 2 * WARPS ? s_pieces.unit[lane] : -1;
+  const uint32_t all = __ballot_sync(0xffffffffu, mine >= 0);
+  float* own = a.pieces + int64_t(blockIdx.x) * C::SLOTS * C::SLOT;
+  // Weights: a warp per (unit, head), a lane per piece.
+  int turn = warp;
+  for (uint32_t rest = all; rest != 0;) {
+    const int first = __ffs(rest) - 1;
+    const uint32_t these = __ballot_sync(0xffffffffu, mine == s_pieces.unit[first]);
     rest &= ~these;
-    const bool began = s_ends[first] & 1, end = s_ends[31 - __clz(these)] & 2, done = began && end;
-    float* to = a.pieces + (int64_t(blockIdx.x) * C::SLOTS + (began ? C::AFTER : C::BEFORE)) * C::SLOT;
-    for (int h = warp; h < C::HEADS; h += WARPS) {           // lane: piece
+    const bool began = s_pieces.ends[first] & 1, done = began && (s_pieces.ends[31 - __clz(these)] & 2);
+    int h = turn;
+    for (; h < C::HEADS; h += WARPS) {
       const bool one = these >> lane & 1;
-      const float pm = one ? s_m[lane % (2 * WARPS)][h] : -INFINITY;
-      const float pl = one ? s_l[lane % (2 * WARPS)][h] : 0.f;
+      const float pm = one ? s_pieces.m[lane % (2 * WARPS)][h] : -INFINITY;
+      const float pl = one ? s_pieces.l[lane % (2 * WARPS)][h] : 0.f;
       float top = pm;
 #pragma unroll
       for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
@@ -791,43 +809,65 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
       float sum = one ? pl * w : 0.f;
 #pragma unroll
       for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      if (one) s_w[lane % (2 * WARPS)][h] = !done ? w : sum == 0.f ? 0.f : w / sum;
+      if (one) s_pieces.w[lane % (2 * WARPS)][h] = !done ? w : sum == 0.f ? 0.f : w / sum;
       if (!done && lane == 0) {
-        to[C::PIECE + h] = top;
-        to[C::PIECE + C::HEADS + h] = sum;
+        float* to = own + (began ? C::AFTER : C::BEFORE) * C::SLOT + C::PIECE;
+        to[h] = top;
+        to[C::HEADS + h] = sum;
       }
     }
-    __syncthreads();
-    const int b = unit / per_b, u = unit - b * per_b, hb = u % a.blocks * C::HEADS;
-    for (int x = warp; x < C::TILES * NT; x += WARPS) {
+    turn = h - C::HEADS;                 // the warps that had nothing to do come first in the next unit
+  }
+  __syncthreads();
+  // Results: a warp per (unit, tile of O), four pieces at a time.
+  turn = warp;
+  for (uint32_t rest = all; rest != 0;) {
+    const int first = __ffs(rest) - 1, unit = s_pieces.unit[first];
+    const uint32_t these = __ballot_sync(0xffffffffu, mine == unit);
+    rest &= ~these;
+    const bool began = s_pieces.ends[first] & 1, end = s_pieces.ends[31 - __clz(these)] & 2;
+    const int b = unit / per_b, u = unit - b * per_b;
+    int x = turn;
+    for (; x < C::TILES * NT; x += WARPS) {
       const int mt = x / NT, nt = x % NT, h0 = nt * 8 + 2 * t;
       float acc[4] = {0.f, 0.f, 0.f, 0.f};
-      for (uint32_t bits = these; bits != 0; bits &= bits - 1) {
-        const int i = __ffs(bits) - 1;
-        const float* po = i & 1 ? reinterpret_cast<const float*>(smem + (i >> 1) * C::RING)
-                                : a.pieces + (int64_t(blockIdx.x) * C::SLOTS + (i >> 1)) * C::SLOT;
-        const float w[2] = {s_w[i][h0], s_w[i][h0 + 1]};
+      for (uint32_t bits = these; bits != 0;) {
+        float v[4][4], w[4][2];
 #pragma unroll
-        for (int y = 0; y < 4; ++y) acc[y] += po[((mt * NT + nt) * 4 + y) * 32 + lane] * w[y & 1];
+        for (int z = 0; z < 4; ++z) {
+          const int i = bits != 0 ? __ffs(bits) - 1 : first;             // (none left: nothing of the first)
+          const float* po = (i & 1 ? reinterpret_cast<const float*>(smem + (i >> 1) * C::RING)
+                                   : own + (i >> 1) * C::SLOT) + x * 128 + lane;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) v[z][y] = po[y * 32];
+          w[z][0] = bits != 0 ? s_pieces.w[i][h0] : 0.f;
+          w[z][1] = bits != 0 ? s_pieces.w[i][h0 + 1] : 0.f;
+          bits &= bits - 1;
+        }
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) acc[y] += v[z][y] * w[z][y & 1];
       }
-      if (done) {
-        const int e = element_of<DT>(mt, g);
+      if (began && end) {
+        const int hb = u % a.blocks * C::HEADS, e = element_of<DT>(mt, g);
 #pragma unroll
         for (int y = 0; y < 2; ++y)
           if (hb + h0 + y < a.group && e < a.d)
             store_pair(out_row<T>(a, b, u, hb + h0 + y) + e, acc[y], acc[2 + y], a.o_vec);
       } else {
+        float* to = own + (began ? C::AFTER : C::BEFORE) * C::SLOT + x * 128 + lane;
 #pragma unroll
-        for (int y = 0; y < 4; ++y) to[((mt * NT + nt) * 4 + y) * 32 + lane] = acc[y];
+        for (int y = 0; y < 4; ++y) to[y * 32] = acc[y];
       }
     }
+    turn = x - C::TILES * NT;
     if (began && !end && tid == 0) {     // (the last unit of the block: written after the zero above)
       const int64_t entries = s_starts[b + 1] - s_starts[b];
       const int64_t stop = int64_t(s_starts[b]) * per_b + (u + 1) * entries;
       const int last = int((stop * used - 1) / total);                   // the block that has its end
       a.links[blockIdx.x] = make_int2(unit, last - int(blockIdx.x) + 1);
     }
-    if (rest != 0) __syncthreads();      // s_w is written again
   }
 }
 
@@ -842,14 +882,13 @@ __global__ void __launch_bounds__(256) join_codes8_kernel(const Attend a) {
   const int mt = int(blockIdx.y) / NT, nt = int(blockIdx.y) % NT, h0 = nt * 8 + 2 * t;
   griddep_launch_dependents();
   griddep_wait();
+  // The first part is asked for before it is known whether there is one.
   const int2 link = a.links[blockIdx.x];
-  if (link.y == 0) return;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int i = warp; i < link.y; i += WARPS) {
-    const float* piece =
-        a.pieces + (int64_t(blockIdx.x + i) * C::SLOTS + (i == 0 ? C::AFTER : C::BEFORE)) * C::SLOT;
-    float x[4], pm[2], pl[2];
+  float x[4], pm[2], pl[2];
+  auto load = [&](int i) {
+    const int block = min(int(blockIdx.x) + i, int(gridDim.x) - 1);
+    const float* piece = a.pieces + (int64_t(block) * C::SLOTS + (i == 0 ? C::AFTER : C::BEFORE)) * C::SLOT;
 #pragma unroll
     for (int y = 0; y < 4; ++y) x[y] = piece[((mt * NT + nt) * 4 + y) * 32 + lane];
 #pragma unroll
@@ -857,14 +896,27 @@ __global__ void __launch_bounds__(256) join_codes8_kernel(const Attend a) {
       pm[y] = piece[C::PIECE + h0 + y];
       pl[y] = piece[C::PIECE + C::HEADS + h0 + y];
     }
+  };
+  load(warp);
+  if (link.y == 0) return;
+  for (int i = warp; i < link.y;) {
+    const float y0 = x[0], y1 = x[1], y2 = x[2], y3 = x[3];
+    const float qm[2] = {pm[0], pm[1]}, ql[2] = {pl[0], pl[1]};
+    i += WARPS;
+    if (i < link.y) load(i);
+    float was[2], is[2];
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
-      const float top = fmaxf(m[y], pm[y]), was = ex2(m[y] - base_of(top)), is = ex2(pm[y] - base_of(top));
+      const float top = fmaxf(m[y], qm[y]);
+      was[y] = ex2(m[y] - base_of(top));
+      is[y] = ex2(qm[y] - base_of(top));
       m[y] = top;
-      l[y] = l[y] * was + pl[y] * is;
-      acc[y] = acc[y] * was + x[y] * is;
-      acc[2 + y] = acc[2 + y] * was + x[2 + y] * is;
+      l[y] = l[y] * was[y] + ql[y] * is[y];
     }
+    acc[0] = acc[0] * was[0] + y0 * is[0];
+    acc[1] = acc[1] * was[1] + y1 * is[1];
+    acc[2] = acc[2] * was[0] + y2 * is[0];
+    acc[3] = acc[3] * was[1] + y3 * is[1];
   }
 #pragma unroll
   for (int y = 0; y < 4; ++y) s_o[warp][y][lane] = acc[y];
