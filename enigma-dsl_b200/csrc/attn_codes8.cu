@@ -233,8 +233,9 @@ __device__ __forceinline__ T* out_row(const Attend& a, int b, int u, int head) {
 // What a block's warps left, in order: a warp's first piece, its last.
 template <typename C>
 struct Pieces {
-  float m[2 * C::WARPS][C::HEADS], l[2 * C::WARPS][C::HEADS], w[2 * C::WARPS][C::HEADS];
+  alignas(16) float2 ml[2 * C::WARPS][C::HEADS];          // maximum, sum
   int unit[2 * C::WARPS], ends[2 * C::WARPS];            // -1: none; 1: has its unit's first key, 2: the last
+  int2 at[2 * C::WARPS];                                  // sequence, and unit of the sequence
 };
 
 // T: of queries and results; DT: the head's elements, rounded up; NT: tiles of 8 query heads.
@@ -721,14 +722,14 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
         began = at.j == 0;
         fresh = false;
       }
-      // (Asking for a chunk as soon as the codes before it are in registers, in the middle of a chunk's
-      // work, has more in flight but is slower: 292 against 272 us for 192 long contexts.)
       cp_wait<C::STAGES - 2>();
       __syncwarp();                      // every lane's copies, and nobody reads the stage before
+      // (Asking for a chunk as soon as the codes before it are in registers, in the middle of a chunk's
+      // work, has more in flight but is slower: 292 against 272 us for 192 long contexts.)
       next(to);
+      to = to + 1 == C::STAGES ? 0 : to + 1;
       compute(at, st);
       st = st + 1 == C::STAGES ? 0 : st + 1;
-      to = to + 1 == C::STAGES ? 0 : to + 1;
       const bool end = at.j + 1 == at.n;
       const bool over = at.left - 1 - (end && !a.whole ? STARTS : 0) <= 0;
       if (end || over) {
@@ -769,13 +770,12 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int y = 0; y < 2; ++y) {
-                s_pieces.m[i][nt * 8 + 2 * t + y] = m[nt][y];
-                s_pieces.l[i][nt * 8 + 2 * t + y] = l[nt][y];
-              }
+              for (int y = 0; y < 2; ++y)
+                s_pieces.ml[i][nt * 8 + 2 * t + y] = make_float2(m[nt][y], l[nt][y]);
           if (lane == 0) {
             s_pieces.unit[i] = at.b * per_b + at.u;
             s_pieces.ends[i] = (began ? 1 : 0) | (end ? 2 : 0);
+            s_pieces.at[i] = make_int2(at.b, at.u);
           }
         }
         fresh = true;
@@ -790,78 +790,87 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
   const int mine = lane < 2 * WARPS ? s_pieces.unit[lane] : -1;
   const uint32_t all = __ballot_sync(0xffffffffu, mine >= 0);
   float* own = a.pieces + int64_t(blockIdx.x) * C::SLOTS * C::SLOT;
-  // Weights: a warp per (unit, head), a lane per piece.
+  // A warp per (unit, tile of O): the lane's two heads' largest maximum, then what each piece adds.
   int turn = warp;
-  for (uint32_t rest = all; rest != 0;) {
-    const int first = __ffs(rest) - 1;
-    const uint32_t these = __ballot_sync(0xffffffffu, mine == s_pieces.unit[first]);
-    rest &= ~these;
-    const bool began = s_pieces.ends[first] & 1, done = began && (s_pieces.ends[31 - __clz(these)] & 2);
-    int h = turn;
-    for (; h < C::HEADS; h += WARPS) {
-      const bool one = these >> lane & 1;
-      const float pm = one ? s_pieces.m[lane % (2 * WARPS)][h] : -INFINITY;
-      const float pl = one ? s_pieces.l[lane % (2 * WARPS)][h] : 0.f;
-      float top = pm;
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      const float w = ex2(pm - base_of(top));
-      float sum = one ? pl * w : 0.f;
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      if (one) s_pieces.w[lane % (2 * WARPS)][h] = !done ? w : sum == 0.f ? 0.f : w / sum;
-      if (!done && lane == 0) {
-        float* to = own + (began ? C::AFTER : C::BEFORE) * C::SLOT + C::PIECE;
-        to[h] = top;
-        to[C::HEADS + h] = sum;
-      }
-    }
-    turn = h - C::HEADS;                 // the warps that had nothing to do come first in the next unit
-  }
-  __syncthreads();
-  // Results: a warp per (unit, tile of O), four pieces at a time.
-  turn = warp;
   for (uint32_t rest = all; rest != 0;) {
     const int first = __ffs(rest) - 1, unit = s_pieces.unit[first];
     const uint32_t these = __ballot_sync(0xffffffffu, mine == unit);
     rest &= ~these;
+    const int2 where = s_pieces.at[first];
+    const int b = where.x, u = where.y;
     const bool began = s_pieces.ends[first] & 1, end = s_pieces.ends[31 - __clz(these)] & 2;
-    const int b = unit / per_b, u = unit - b * per_b;
     int x = turn;
     for (; x < C::TILES * NT; x += WARPS) {
       const int mt = x / NT, nt = x % NT, h0 = nt * 8 + 2 * t;
-      float acc[4] = {0.f, 0.f, 0.f, 0.f};
-      for (uint32_t bits = these; bits != 0;) {
-        float v[4][4], w[4][2];
+      float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t bits = these;
+      if (__popc(these) > 6) {           // many: all last pieces at once, those of other units as nothing
+        float4 ml[WARPS];
 #pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          const int i = bits != 0 ? __ffs(bits) - 1 : first;             // (none left: nothing of the first)
-          const float* po = (i & 1 ? reinterpret_cast<const float*>(smem + (i >> 1) * C::RING)
-                                   : own + (i >> 1) * C::SLOT) + x * 128 + lane;
-#pragma unroll
-          for (int y = 0; y < 4; ++y) v[z][y] = po[y * 32];
-          w[z][0] = bits != 0 ? s_pieces.w[i][h0] : 0.f;
-          w[z][1] = bits != 0 ? s_pieces.w[i][h0 + 1] : 0.f;
-          bits &= bits - 1;
+        for (int w = 0; w < WARPS; ++w) {
+          ml[w] = *reinterpret_cast<const float4*>(&s_pieces.ml[2 * w + 1][h0]);
+          if (!(these >> (2 * w + 1) & 1)) ml[w] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+          top[0] = fmaxf(top[0], ml[w].x);
+          top[1] = fmaxf(top[1], ml[w].z);
         }
+        const float base[2] = {base_of(top[0]), base_of(top[1])};
 #pragma unroll
-        for (int z = 0; z < 4; ++z)
+        for (int w = 0; w < WARPS; ++w) {
+          const bool one = these >> (2 * w + 1) & 1;
+          const float* po = reinterpret_cast<const float*>(smem + w * C::RING) + x * 128 + lane;
+          const float f[2] = {ex2(ml[w].x - base[0]), ex2(ml[w].z - base[1])};
+          sum[0] += ml[w].y * f[0];
+          sum[1] += ml[w].w * f[1];
 #pragma unroll
-          for (int y = 0; y < 4; ++y) acc[y] += v[z][y] * w[z][y & 1];
+          for (int y = 0; y < 4; ++y) acc[y] += (one ? po[y * 32] : 0.f) * f[y & 1];
+        }
+        bits &= 0x55555555u;             // (a unit has at most one piece that others followed)
+      }
+      // One after the other, the next one's loads ahead.
+      float v[4];
+      float4 ml = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+      auto load = [&](int i) {
+        const float* po = i & 1 ? reinterpret_cast<const float*>(smem + (i >> 1) * C::RING)
+                                : own + (i >> 1) * C::SLOT;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) v[y] = po[x * 128 + y * 32 + lane];
+        ml = *reinterpret_cast<const float4*>(&s_pieces.ml[i][h0]);
+      };
+      if (bits != 0) load(__ffs(bits) - 1);
+#pragma unroll 1
+      while (bits != 0) {
+        const float now[2] = {fmaxf(top[0], ml.x), fmaxf(top[1], ml.z)};
+        const float base[2] = {base_of(now[0]), base_of(now[1])};
+        const float was[2] = {ex2(top[0] - base[0]), ex2(top[1] - base[1])};
+        const float is[2] = {ex2(ml.x - base[0]), ex2(ml.z - base[1])};
+        sum[0] = sum[0] * was[0] + ml.y * is[0];
+        sum[1] = sum[1] * was[1] + ml.w * is[1];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) acc[y] = acc[y] * was[y & 1] + v[y] * is[y & 1];
+        top[0] = now[0];
+        top[1] = now[1];
+        bits &= bits - 1;
+        if (bits != 0) load(__ffs(bits) - 1);
       }
       if (began && end) {
         const int hb = u % a.blocks * C::HEADS, e = element_of<DT>(mt, g);
 #pragma unroll
         for (int y = 0; y < 2; ++y)
-          if (hb + h0 + y < a.group && e < a.d)
-            store_pair(out_row<T>(a, b, u, hb + h0 + y) + e, acc[y], acc[2 + y], a.o_vec);
+          if (hb + h0 + y < a.group && e < a.d) {
+            const float f = sum[y] == 0.f ? 0.f : 1.f / sum[y];
+            store_pair(out_row<T>(a, b, u, hb + h0 + y) + e, acc[y] * f, acc[2 + y] * f, a.o_vec);
+          }
       } else {
-        float* to = own + (began ? C::AFTER : C::BEFORE) * C::SLOT + x * 128 + lane;
+        float* to = own + (began ? C::AFTER : C::BEFORE) * C::SLOT;
 #pragma unroll
-        for (int y = 0; y < 4; ++y) to[y * 32] = acc[y];
+        for (int y = 0; y < 4; ++y) to[x * 128 + lane + y * 32] = acc[y];
+        if (mt == 0 && g == 0)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            reinterpret_cast<float2*>(to + C::PIECE)[h0 + y] = make_float2(top[y], sum[y]);
       }
     }
-    turn = x - C::TILES * NT;
+    turn = x - C::TILES * NT;            // the warps that had nothing to do come first in the next unit
     if (began && !end && tid == 0) {     // (the last unit of the block: written after the zero above)
       const int64_t entries = s_starts[b + 1] - s_starts[b];
       const int64_t stop = int64_t(s_starts[b]) * per_b + (u + 1) * entries;
@@ -893,8 +902,9 @@ __global__ void __launch_bounds__(256) join_codes8_kernel(const Attend a) {
     for (int y = 0; y < 4; ++y) x[y] = piece[((mt * NT + nt) * 4 + y) * 32 + lane];
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
-      pm[y] = piece[C::PIECE + h0 + y];
-      pl[y] = piece[C::PIECE + C::HEADS + h0 + y];
+      const float2 ml = reinterpret_cast<const float2*>(piece + C::PIECE)[h0 + y];
+      pm[y] = ml.x;
+      pl[y] = ml.y;
     }
   };
   load(warp);
