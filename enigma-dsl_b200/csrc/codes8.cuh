@@ -46,19 +46,22 @@ __device__ __forceinline__ float2 floats_of(uint32_t halves) {
   return f;
 }
 
-// Four values in the codes' units, rounded to codes (to nearest, ties to even).  No value of a block
-// passes the codes' range but one that is not a number, whose block reads as NaN.
+// Four values times `unit` (one over their scale) rounded to codes: to nearest, ties to even.  No value of a
+// block passes the codes' range but one that is not a number, whose block reads as NaN.
 template <bool E4M3>
-__device__ __forceinline__ uint32_t codes_of(float a, float b, float c, float d) {
+__device__ __forceinline__ uint32_t codes_of(float a, float b, float c, float d, float unit) {
   if (E4M3) {
     uint16_t lo, hi;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b * unit), "f"(a * unit));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d * unit), "f"(c * unit));
     return uint32_t(lo) | uint32_t(hi) << 16;
   }
-  const uint32_t x = uint32_t(__float2int_rn(a)) & 255u, y = uint32_t(__float2int_rn(b)) & 255u;
-  const uint32_t z = uint32_t(__float2int_rn(c)) & 255u, w = uint32_t(__float2int_rn(d)) & 255u;
-  return x | y << 8 | z << 16 | w << 24;
+  // 1.5 * 2^23 + x is x rounded to a whole number, in the low bits (conversions to integers run at a
+  // quarter of the rate of additions).
+  constexpr float kWhole = 0x1.8p23f;
+  const uint32_t x = __float_as_uint(fmaf(a, unit, kWhole)), y = __float_as_uint(fmaf(b, unit, kWhole));
+  const uint32_t z = __float_as_uint(fmaf(c, unit, kWhole)), w = __float_as_uint(fmaf(d, unit, kWhole));
+  return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
 }
 
 // The scale of values whose largest magnitude has these bits (finite): the least power of two 2^e

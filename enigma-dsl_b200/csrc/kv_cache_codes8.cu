@@ -18,6 +18,50 @@ using namespace enigma_sm100;
 
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+// Elements of a row that are moved at once, 16 bytes of them.
+template <typename T>
+constexpr int kVec = 16 / int(sizeof(T));
+
+// Four elements from 16 or 8 loaded bytes, from element 4 y on.
+__device__ __forceinline__ void four_of(const uint4& v, int, float (&x)[4], float) {
+  x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y);
+  x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
+}
+__device__ __forceinline__ void four_of(const uint4& v, int y, float (&x)[4], __nv_bfloat16) {
+  const uint32_t a = y ? v.z : v.x, b = y ? v.w : v.y;
+  x[0] = __uint_as_float(a << 16); x[1] = __uint_as_float(a & 0xffff0000u);
+  x[2] = __uint_as_float(b << 16); x[3] = __uint_as_float(b & 0xffff0000u);
+}
+
+// 16 bytes of a row, whatever its alignment.
+template <typename T, bool VEC>
+__device__ __forceinline__ uint4 load_vec(const T* p) {
+  if (VEC) return *reinterpret_cast<const uint4*>(p);
+  uint4 v;
+  if (sizeof(T) == 4) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+    v = make_uint4(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16, h[4] | uint32_t(h[5]) << 16,
+                   h[6] | uint32_t(h[7]) << 16);
+  }
+  return v;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_vec(T* p, const uint4& v) {
+  if (VEC) {
+    *reinterpret_cast<uint4*>(p) = v;
+  } else if (sizeof(T) == 4) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else {
+    uint16_t* h = reinterpret_cast<uint16_t*>(p);
+    h[0] = uint16_t(v.x); h[1] = uint16_t(v.x >> 16); h[2] = uint16_t(v.y); h[3] = uint16_t(v.y >> 16);
+    h[4] = uint16_t(v.z); h[5] = uint16_t(v.z >> 16); h[6] = uint16_t(v.w); h[7] = uint16_t(v.w >> 16);
+  }
+}
+
 // Entry of packed row t: the last i in [0, n) with cu[i] <= t, found 32 ways at once.
 __device__ __forceinline__ int entry_of(const int32_t* cu, int n, int t) {
   const int lane = threadIdx.x & 31;
@@ -32,221 +76,400 @@ __device__ __forceinline__ int entry_of(const int32_t* cu, int n, int t) {
   return lo;
 }
 
-__device__ __forceinline__ void load4(const float* p, float (&x)[4], bool vec) {
-  if (vec) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-  } else {
+struct Rows {
+  const int32_t *table, *slots, *starts, *cu;
+  int64_t k_token, k_head, v_token, v_head;
+  int n, tokens, heads, slots_total, pages, width, page_shift, d;
+};
+
+// An entry of a request, and its rows [first, end).
+struct Entry {
+  int index, slot, start, first, end;
+};
+
+// The entries of the packed rows t0 .. t0 + 15, for lanes 0 to 15 (and again for the others): a search
+// for the first, then one look at it and the 31 entries behind; where more of those begin within
+// these rows (empty ones may), a search for each row.
+__device__ __forceinline__ Entry entries_of(const Rows& r, int t0) {
+  const int lane = threadIdx.x & 31, x = lane % kScaleBlock;
+  const int e0 = entry_of(r.cu, r.n, t0), j = min(e0 + lane, r.n - 1);
+  const int first = r.cu[j], end = r.cu[j + 1], slot = r.slots[j], start = r.starts[j];
+  int at = 0;                            // the row's entry - e0
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = p[i];
+  for (int y = 0; y < kScaleBlock; ++y) {
+    const uint32_t past = __ballot_sync(0xffffffffu, lane > 0 && e0 + lane < r.n && first <= t0 + y);
+    if (x == y) at = past ? 31 - __clz(past) : 0;
   }
-}
-__device__ __forceinline__ void load4(const __nv_bfloat16* p, float (&x)[4], bool vec) {
-  uint2 v;
-  if (vec) {
-    v = *reinterpret_cast<const uint2*>(p);
-  } else {
-    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-    v = make_uint2(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16);
+  Entry e;
+  e.index = e0 + at;
+  e.first = __shfl_sync(0xffffffffu, first, at);
+  e.end = __shfl_sync(0xffffffffu, end, at);
+  e.slot = __shfl_sync(0xffffffffu, slot, at);
+  e.start = __shfl_sync(0xffffffffu, start, at);
+  if (__any_sync(0xffffffffu, at == 31)) {                   // perhaps further on
+    int mine = 0;
+    for (int y = 0; y < kScaleBlock; ++y) {
+      const int i = entry_of(r.cu, r.n, t0 + y);
+      if (x == y) mine = i;
+    }
+    e = {mine, r.slots[mine], r.starts[mine], r.cu[mine], r.cu[mine + 1]};
   }
-  x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
-  x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+  return e;
 }
 
 struct Write {
+  Rows r;
   uint8_t *k, *v;                        // the layer's pages
   float *ks, *vs;                        // and scales
   const void *new_k, *new_v;
-  const int32_t *table, *refs, *slots, *starts, *cu;
+  const int32_t* refs;
   int32_t* status;
-  int64_t k_token, k_head, v_token, v_head;
-  int n, tokens, heads, slots_total, pages, width, page, d;
-  bool vec;                              // rows can be read four elements at a time
 };
 
 // The rows of one block that one entry of the request writes.
 struct Part {
   int t, rows, r0;                       // first packed row, their number, first row in the block
-  int64_t block;                         // (page * heads) * blocks of a page + block in the page
+  int entry, slot;
+  int64_t block;                         // of the first head: (page * heads) * blocks of a page + block in it
+  int64_t first;                         // position of the block's first row in the sequence
 };
 
-// Blocks (c, y): the parts that begin in packed rows [16 c, 16 c + 16), 8 gridDim.y warps over their
-// (part, K or V, head) triples.  A part begins with its entry, or on a block's first token.
-template <typename T, bool E4M3>
-__global__ void __launch_bounds__(256) write_codes8_kernel(const Write w) {
+// One block of one head: what is new of it, and where it is.
+template <typename T>
+struct Block {
+  const T* rows;                         // the first new row
+  int64_t token;                         // from one row to the next
+  uint8_t* codes;
+  float* scale;
+  int n, r0;                             // new rows, the first one's place in the block; n 0: none
+};
+
+// Blocks by a warp: the scale that old and new rows need, and their codes.  NV: vectors of 16 bytes that a
+// lane has of a block's new rows; those of all N blocks are loaded at once.
+template <typename T, bool E4M3, bool VEC, int NV, int N>
+__device__ __forceinline__ void write_blocks(const Block<T> (&b)[N], int d) {
+  constexpr int E = kVec<T>;
+  const int lane = threadIdx.x & 31, cols = d / E, step_r = 32 / cols, step_c = 32 - step_r * cols;
+  const int r_first = lane / cols, c_first = lane - r_first * cols;
+  float held[N];
+  uint4 x[N][NV];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    held[k] = b[k].r0 > 0 ? *b[k].scale : 0.f;
+    int r = r_first, c = c_first;        // (a row past the last is the last again)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      x[k][i] = load_vec<T, VEC>(b[k].rows + max(min(r, b[k].n - 1), 0) * b[k].token + c * E);
+      r += step_r;
+      c += step_c;
+      if (c >= cols) c -= cols, ++r;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    if (b[k].n == 0) continue;
+    uint32_t top = 0;                    // bits of the largest magnitude
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t v[4] = {x[k][i].x, x[k][i].y, x[k][i].z, x[k][i].w};
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        top = E == 8 ? __vmaxu2(top, v[y] & 0x7fff7fffu) : max(top, v[y] & 0x7fffffffu);
+    }
+    if (E == 8) top = max(top & 0xffff0000u, top << 16);
+    top = __reduce_max_sync(0xffffffffu, top);
+    const bool finite = top < 0x7f800000u && fabsf(held[k]) < INFINITY;
+    const float scale = finite ? fmaxf(held[k], scale_of<E4M3>(top)) : __uint_as_float(0x7fffffffu);
+    const float inverse = finite ? 1.f / scale : 0.f;
+    if (finite && held[k] < scale) {     // (r0 = 0: there are no old rows)
+      for (int w = lane; w < b[k].r0 * (d / 4); w += 32) {
+        uint32_t* word = reinterpret_cast<uint32_t*>(b[k].codes) + w;
+        uint32_t lo, hi;
+        halves_of4<E4M3>(*word, &lo, &hi);
+        const float2 p = floats_of(lo), q = floats_of(hi);
+        const float h = held[k];
+        *word = codes_of<E4M3>(p.x * h, p.y * h, q.x * h, q.y * h, inverse);
+      }
+    }
+    int r = r_first, c = c_first;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      uint32_t out[E / 4];
+#pragma unroll
+      for (int y = 0; y < E / 4; ++y) {
+        float f[4];
+        four_of(x[k][i], y, f, T(0.f));
+        out[y] = finite ? codes_of<E4M3>(f[0], f[1], f[2], f[3], inverse) : 0u;
+      }
+      if (r < b[k].n) {
+        uint32_t* to = reinterpret_cast<uint32_t*>(b[k].codes + (b[k].r0 + r) * d + c * E);
+        if (E == 8) *reinterpret_cast<uint2*>(to) = make_uint2(out[0], out[E / 4 - 1]);
+        else *to = out[0];
+      }
+      r += step_r;
+      c += step_c;
+      if (c >= cols) c -= cols, ++r;
+    }
+    if (lane == 0) *b[k].scale = scale;
+  }
+}
+
+constexpr int WWARPS = 8;
+
+// Blocks (c, y): the parts that begin in packed rows [16 c, 16 c + 16), WWARPS gridDim.y warps over their
+// (part, K or V, head) triples.  A part begins with its entry, or on a block's first token.  Bound
+// by memory for prompts; the request's look-ups, five loads that wait for one another, are made
+// once for 16 rows, a lane each, and hidden by the other blocks of the SM.
+template <typename T, bool E4M3, bool VEC, int NV>
+__global__ void __launch_bounds__(WWARPS * 32, (NV <= 8 ? 32 : NV == 16 ? 16 : 8) / WWARPS) write_codes8_kernel(const __grid_constant__ Write w) {
   __shared__ Part s_part[kScaleBlock];
-  __shared__ int s_found[kScaleBlock];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x < kScaleBlock) s_found[threadIdx.x] = 0;
+  __shared__ uint32_t s_found;
+  __shared__ int s_few;                                    // no part has more than 32 vectors
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t0 = int(blockIdx.x) * kScaleBlock;
+  const Rows& r = w.r;
+  const int page = 1 << r.page_shift, per_page = page / kScaleBlock;
   griddep_launch_dependents();
   griddep_wait();
-  __syncthreads();
-  const int per_page = w.page / kScaleBlock;
-  for (int x = warp; x < kScaleBlock; x += 8) {
-    const int t = int(blockIdx.x) * kScaleBlock + x;
-    if (t >= w.tokens) break;
-    const int i = entry_of(w.cu, w.n, t);
-    const int first = w.cu[i], end = min(w.cu[i + 1], w.tokens), slot = w.slots[i];
-    const int64_t start = w.starts[i], pos = start + t - first;
+  if (warp == 0) {
+    const int x = lane % kScaleBlock, t = t0 + x;
+    const Entry e = entries_of(r, t0);
     int fail = 0;
-    if (t < first || t >= end || slot < 0 || slot >= w.slots_total || pos < 0 ||
-        pos / w.page >= w.width)
-      fail = ENIGMA_CACHE_BAD_REQUEST;
-    const int r0 = int(pos % kScaleBlock);
-    if (fail == 0 && t != max(first, 0) && r0 != 0) continue;            // in the middle of a part
-    int at = -1;
-    if (fail == 0) {
-      at = w.table[int64_t(slot) * w.width + pos / w.page];
-      if (at < 0 || at >= w.pages) fail = ENIGMA_CACHE_BAD_REQUEST;
-      else if (w.refs[at] > 1) fail = ENIGMA_CACHE_SHARED;
-    }
-    if (fail == 0) {
-      // Another entry of the same slot that touches this block would change it at the same time.
-      const int64_t b0 = pos - r0, b1 = b0 + kScaleBlock;
-      bool twice = false;
-      for (int j = lane; j < w.n; j += 32)
-        if (j != i && w.slots[j] == slot) {
-          const int64_t s = w.starts[j], e = s + w.cu[j + 1] - int64_t(w.cu[j]);
-          twice |= s < e && s < b1 && e > b0;
-        }
-      if (__any_sync(0xffffffffu, twice)) fail = ENIGMA_CACHE_BAD_REQUEST;
-    }
-    if (lane == 0) {
-      if (fail != 0) {
-        atomicOr(w.status, fail);
-      } else {
-        Part p;
-        p.t = t;
-        p.rows = min(kScaleBlock - r0, end - t);
-        p.r0 = r0;
-        p.block = int64_t(at) * w.heads * per_page + pos % w.page / kScaleBlock;
-        s_part[x] = p;
-        s_found[x] = 1;
+    Part p;
+    bool found = false;
+    if (t < r.tokens && lane < kScaleBlock) {
+      const int first = e.first, end = min(e.end, r.tokens);
+      p.slot = e.slot;
+      const int64_t pos = int64_t(e.start) + t - first;
+      if (t < first || t >= end || p.slot < 0 || p.slot >= r.slots_total || pos < 0 ||
+          pos >> r.page_shift >= r.width)
+        fail = ENIGMA_CACHE_BAD_REQUEST;
+      p.t = t;
+      p.r0 = int(pos & (kScaleBlock - 1));
+      p.rows = min(kScaleBlock - p.r0, end - t);
+      p.entry = e.index;
+      p.first = pos - p.r0;
+      if (fail == 0 && (t == max(first, 0) || p.r0 == 0)) {              // else in the middle of a part
+        const int at = r.table[int64_t(p.slot) * r.width + (pos >> r.page_shift)];
+        if (at < 0 || at >= r.pages) fail = ENIGMA_CACHE_BAD_REQUEST;
+        else if (w.refs[at] > 1) fail = ENIGMA_CACHE_SHARED;
+        found = fail == 0;
+        p.block = int64_t(at) * r.heads * per_page + (pos & (page - 1)) / kScaleBlock;
       }
+      if (fail != 0) atomicOr(w.status, fail);
+    }
+    const uint32_t all = __ballot_sync(0xffffffffu, found);
+    if (found) s_part[__popc(all & ((1u << lane) - 1u))] = p;
+    const bool few = __all_sync(0xffffffffu, !found || p.rows * r.d <= 32 * kVec<T>);
+    if (lane == 0) {
+      s_found = (1u << __popc(all)) - 1u;
+      s_few = few;
     }
   }
   __syncthreads();
-  // The parts that there are, in the order of their rows: the same list in every block of a column.
-  const uint32_t found = __ballot_sync(0xffffffffu, lane < kScaleBlock && s_found[lane % kScaleBlock]);
-  const int quads = w.d / 4, step_r = 32 / quads, step_c = 32 % quads;
-  const int units = __popc(found) * 2 * w.heads;
-  for (int u = int(blockIdx.y) * 8 + warp; u < units; u += 8 * int(gridDim.y)) {
-    const Part p = s_part[__fns(found, 0, u / (2 * w.heads) + 1)];
-    const int rest = u % (2 * w.heads), head = rest >> 1;
+  const int parts = __popc(s_found);
+  // Another entry of the same slot that touches the block would change it at the same time.
+  if (r.n > 1) {
+    __syncthreads();
+    for (int j = threadIdx.x; j < r.n; j += WWARPS * 32) {
+      const int slot = r.slots[j];
+      for (int x = 0; x < parts; ++x)
+        if (s_part[x].slot == slot && s_part[x].entry != j) {
+          const int64_t s = r.starts[j], e = s + r.cu[j + 1] - int64_t(r.cu[j]);
+          if (s < e && s < s_part[x].first + kScaleBlock && e > s_part[x].first) {
+            atomicAnd(&s_found, ~(1u << x));
+            atomicOr(w.status, ENIGMA_CACHE_BAD_REQUEST);
+          }
+        }
+    }
+    __syncthreads();
+  }
+  const uint32_t found = s_found;
+  const int units = parts * 2 * r.heads;
+  auto block_of = [&](int u) {
+    Block<T> b;
+    const int x = min(u, units - 1) / (2 * r.heads), rest = min(u, units - 1) - x * 2 * r.heads;
+    const int head = rest >> 1;
+    const Part& p = s_part[x];
     const bool is_v = rest & 1;
-    const T* rows = is_v ? static_cast<const T*>(w.new_v) + p.t * w.v_token + head * w.v_head
-                         : static_cast<const T*>(w.new_k) + p.t * w.k_token + head * w.k_head;
-    const int64_t token = is_v ? w.v_token : w.k_token;
     const int64_t block = p.block + int64_t(head) * per_page;
-    uint8_t* codes = (is_v ? w.v : w.k) + block * kScaleBlock * w.d;
-    float* scale_at = (is_v ? w.vs : w.ks) + block;
-    const float held = p.r0 > 0 ? *scale_at : 0.f;
-    uint32_t top = 0;
-    for (int r = lane / quads, c = lane % quads; r < p.rows;) {
-      float x[4];
-      load4(rows + r * token + 4 * c, x, w.vec);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-      r += step_r;
-      c += step_c;
-      if (c >= quads) c -= quads, ++r;
+    b.token = is_v ? r.v_token : r.k_token;
+    b.rows = static_cast<const T*>(is_v ? w.new_v : w.new_k) + p.t * b.token +
+             head * (is_v ? r.v_head : r.k_head);
+    b.codes = (is_v ? w.v : w.k) + block * kScaleBlock * r.d;
+    b.scale = (is_v ? w.vs : w.ks) + block;
+    b.n = u < units && (found >> x & 1) ? p.rows : 0;
+    b.r0 = p.r0;
+    return b;
+  };
+  if (units == 0) return;
+  const int stride = WWARPS * int(gridDim.y);
+  if (s_few) {                           // single tokens: four blocks at once, a vector a lane
+    for (int u = int(blockIdx.y) * WWARPS + warp; u < units; u += 4 * stride) {
+      const Block<T> b[4] = {block_of(u), block_of(u + stride), block_of(u + 2 * stride),
+                             block_of(u + 3 * stride)};
+      write_blocks<T, E4M3, VEC, 1, 4>(b, r.d);
     }
-    top = __reduce_max_sync(0xffffffffu, top);
-    const bool finite = top < 0x7f800000u && fabsf(held) < INFINITY;
-    const float scale = finite ? fmaxf(held, scale_of<E4M3>(top)) : __uint_as_float(0x7fffffffu);
-    const float inverse = finite ? 1.f / scale : 0.f;
-    if (finite && held < scale) {                                        // (r0 = 0: there are none)
-      for (int x = lane; x < p.r0 * quads; x += 32) {
-        uint32_t* word = reinterpret_cast<uint32_t*>(codes) + x;
-        const float2 lo = floats_of(halves_of<E4M3>(*word & 0xffffu));
-        const float2 hi = floats_of(halves_of<E4M3>(*word >> 16));
-        *word = codes_of<E4M3>(lo.x * held * inverse, lo.y * held * inverse, hi.x * held * inverse,
-                               hi.y * held * inverse);
-      }
+  } else {
+    for (int u = int(blockIdx.y) * WWARPS + warp; u < units; u += stride) {
+      const Block<T> b[1] = {block_of(u)};
+      write_blocks<T, E4M3, VEC, NV, 1>(b, r.d);
     }
-    for (int r = lane / quads, c = lane % quads; r < p.rows;) {
-      float x[4];
-      load4(rows + r * token + 4 * c, x, w.vec);
-      *reinterpret_cast<uint32_t*>(codes + (p.r0 + r) * w.d + 4 * c) =
-          finite ? codes_of<E4M3>(x[0] * inverse, x[1] * inverse, x[2] * inverse, x[3] * inverse) : 0u;
-      r += step_r;
-      c += step_c;
-      if (c >= quads) c -= quads, ++r;
-    }
-    if (lane == 0) *scale_at = scale;
   }
 }
 
 struct Read {
+  Rows r;
   const uint8_t *k, *v;
   const float *ks, *vs;
   void *out_k, *out_v;
-  const int32_t *table, *lens, *slots, *starts, *cu;
-  int64_t k_token, k_head, v_token, v_head;
-  int n, tokens, heads, slots_total, pages, width, page, d;
-  bool vec;
+  const int32_t* lens;
 };
 
-__device__ __forceinline__ void store4(float* p, const float (&x)[4], bool vec) {
-  if (vec) {
-    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = x[i];
-  }
-}
-__device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&x)[4], bool vec) {
-  if (vec) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = __float2bfloat16_rn(x[i]);
-  }
-}
-
-// A warp per packed row; rows before the first entry and behind the last are left as they were, a
+// A block has 16 packed rows: their look-ups as above, then a warp per row, its lanes along the heads,
+// READ vectors at once.  Rows before the first entry and behind the last are left as they were, a
 // token that the slot does not hold is zeros.
-template <typename T, bool E4M3>
-__global__ void __launch_bounds__(256) read_codes8_kernel(const Read w) {
-  const int lane = threadIdx.x & 31;
-  const int quads = w.d / 4, row = w.heads * quads, per_page = w.page / kScaleBlock;
+constexpr int READ = 4;
+template <typename T, bool E4M3, bool VEC>
+__global__ void __launch_bounds__(256) read_codes8_kernel(const __grid_constant__ Read w) {
+  constexpr int E = kVec<T>;
+  __shared__ int64_t s_line[kScaleBlock];                  // of the first head: page * heads * page size + row
+  __shared__ int s_kind[kScaleBlock];                      // 0: no row, 1: zeros, 2: a token
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t0 = int(blockIdx.x) * kScaleBlock;
+  const Rows& r = w.r;
+  const int page = 1 << r.page_shift, per_page = page / kScaleBlock;
   griddep_launch_dependents();
   griddep_wait();
-  for (int t = int(blockIdx.x) * 8 + (threadIdx.x >> 5); t < w.tokens; t += int(gridDim.x) * 8) {
-    const int i = entry_of(w.cu, w.n, t);
-    if (t < w.cu[i] || t >= w.cu[i + 1]) continue;
-    const int slot = w.slots[i];
-    const int64_t pos = int64_t(w.starts[i]) + t - w.cu[i];
-    int at = -1;
-    if (slot >= 0 && slot < w.slots_total && pos >= 0 && pos < w.lens[slot] &&
-        pos / w.page < w.width)
-      at = w.table[int64_t(slot) * w.width + pos / w.page];
-    const bool has = at >= 0 && at < w.pages;
-    for (int x = lane; x < 2 * row; x += 32) {
-      const bool is_v = x >= row;
-      const int y = is_v ? x - row : x, h = y / quads, c = y - h * quads;
-      float f[4] = {0.f, 0.f, 0.f, 0.f};
-      if (has) {
-        const int64_t line = (int64_t(at) * w.heads + h) * w.page + pos % w.page;
-        const uint32_t word = reinterpret_cast<const uint32_t*>((is_v ? w.v : w.k) + line * w.d)[c];
-        const float s = (is_v ? w.vs : w.ks)[(int64_t(at) * w.heads + h) * per_page +
-                                             pos % w.page / kScaleBlock];
-        const float2 lo = floats_of(halves_of<E4M3>(word & 0xffffu));
-        const float2 hi = floats_of(halves_of<E4M3>(word >> 16));
-        f[0] = lo.x * s; f[1] = lo.y * s; f[2] = hi.x * s; f[3] = hi.y * s;
+  if (warp == 0) {
+    const int t = t0 + lane % kScaleBlock;
+    const Entry e = entries_of(r, t0);
+    if (lane < kScaleBlock) {
+      int kind = 0;
+      if (t < r.tokens && t >= e.first && t < e.end) {
+        const int slot = e.slot;
+        const int64_t pos = int64_t(e.start) + t - e.first;
+        kind = 1;
+        if (slot >= 0 && slot < r.slots_total && pos >= 0 && pos >> r.page_shift < r.width) {
+          const int at = r.table[int64_t(slot) * r.width + (pos >> r.page_shift)];
+          if (pos < w.lens[slot] && at >= 0 && at < r.pages) {
+            kind = 2;
+            s_line[lane] = int64_t(at) * r.heads * page + (pos & (page - 1));
+          }
+        }
       }
-      store4((is_v ? static_cast<T*>(w.out_v) + t * w.v_token + h * w.v_head
-                   : static_cast<T*>(w.out_k) + t * w.k_token + h * w.k_head) + 4 * c, f, w.vec);
+      s_kind[lane] = kind;
+    }
+  }
+  __syncthreads();
+  const int cols = r.d / E, items = r.heads * cols, step_h = 32 / cols, step_c = 32 - step_h * cols;
+  const int h_first = lane / cols, c_first = lane - h_first * cols;
+  for (int x = warp; x < 2 * kScaleBlock; x += 8) {        // row, K or V
+    const int kind = s_kind[x >> 1];
+    if (kind == 0) continue;
+    const bool is_v = x & 1;
+    const int t = t0 + (x >> 1);
+    const int64_t line = kind == 2 ? s_line[x >> 1] : 0;
+    const uint8_t* codes = (is_v ? w.v : w.k) + line * r.d;
+    const float* scales = (is_v ? w.vs : w.ks) + line / kScaleBlock;   // (a page's lines are whole blocks)
+    T* out = static_cast<T*>(is_v ? w.out_v : w.out_k) + t * (is_v ? r.v_token : r.k_token);
+    const int64_t out_head = is_v ? r.v_head : r.k_head;
+    int h = h_first, c = c_first;
+    for (int i0 = lane; i0 < items; i0 += 32 * READ) {
+      uint32_t code[READ][E / 4];
+      float scale[READ];
+      int hs[READ], cs[READ];
+#pragma unroll
+      for (int y = 0; y < READ; ++y) {                     // (a head past the last is the last again)
+        hs[y] = h;
+        cs[y] = c;
+        const int head = min(h, r.heads - 1);
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(codes + int64_t(head) * page * r.d + c * E);
+        if (E == 8) {
+          const uint2 v = *reinterpret_cast<const uint2*>(from);
+          code[y][0] = v.x;
+          code[y][E / 4 - 1] = v.y;
+        } else {
+          code[y][0] = *from;
+        }
+        scale[y] = scales[head * per_page];
+        h += step_h;
+        c += step_c;
+        if (c >= cols) c -= cols, ++h;
+      }
+#pragma unroll
+      for (int y = 0; y < READ; ++y) {
+        uint32_t words[4];
+#pragma unroll
+        for (int z = 0; z < E / 4; ++z) {
+          uint32_t lo, hi;
+          halves_of4<E4M3>(code[y][z], &lo, &hi);
+          const float2 a = floats_of(lo), b = floats_of(hi);
+          const float f[4] = {a.x * scale[y], a.y * scale[y], b.x * scale[y], b.y * scale[y]};
+          if (E == 8) {
+            words[(2 * z) & 3] = pack_bf16x2(f[0], f[1]);
+            words[(2 * z + 1) & 3] = pack_bf16x2(f[2], f[3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) words[e] = __float_as_uint(f[e]);
+          }
+        }
+        uint4 v = make_uint4(words[0], words[1], words[2], words[3]);
+        if (kind == 1) v = make_uint4(0, 0, 0, 0);
+        if (hs[y] < r.heads) store_vec<T, VEC>(out + hs[y] * out_head + cs[y] * E, v);
+      }
     }
   }
 }
 
-// Rows of four elements that can be moved at once.
+// Rows that can be moved 16 bytes at a time.
 bool vectors(int dtype, const void* k, const void* v, const int64_t* strides4) {
-  const size_t es = dtype == ENIGMA_DTYPE_F32 ? 4 : 2;
-  bool ok = aligned(k, 4 * es) && aligned(v, 4 * es);
-  for (int i = 0; i < 4; ++i) ok = ok && strides4[i] % 4 == 0;
+  bool ok = aligned(k, 16) && aligned(v, 16);
+  for (int i = 0; i < 4; ++i) ok = ok && strides4[i] * (dtype == ENIGMA_DTYPE_F32 ? 4 : 2) % 16 == 0;
   return ok;
+}
+
+Rows rows_of(const enigma_kv_cache_desc& c, const int64_t* strides4, const int32_t* slots,
+             const int32_t* starts, const int32_t* cu, int64_t n, int64_t tokens) {
+  Rows r;
+  r.table = c.table;
+  r.slots = slots;
+  r.starts = starts;
+  r.cu = cu;
+  r.k_token = strides4[0];
+  r.k_head = strides4[1];
+  r.v_token = strides4[2];
+  r.v_head = strides4[3];
+  r.n = int(n);
+  r.tokens = int(tokens);
+  r.heads = int(c.heads_kv);
+  r.slots_total = int(c.slots);
+  r.pages = int(c.pages);
+  r.width = int(c.table_width);
+  r.page_shift = c.page == 16 ? 4 : c.page == 32 ? 5 : c.page == 64 ? 6 : 7;
+  r.d = int(c.head_dim);
+  return r;
+}
+
+template <typename T, bool E4M3, bool VEC>
+cudaError_t launch_write(const Write& w, cudaStream_t s) {
+  const int64_t columns = (int64_t(w.r.tokens) + kScaleBlock - 1) / kScaleBlock;
+  // Blocks that share a column's parts: one where the columns fill the GPU; where they do not, as many
+  // as leave each warp four (part, K or V, head) if every row is a part.
+  const int64_t most = (int64_t(kScaleBlock) * 2 * w.r.heads + 4 * WWARPS - 1) / (4 * WWARPS);
+  const int64_t share = std::max<int64_t>(1, std::min(most, enigma::sm_count() * 64 / WWARPS / columns));
+  const dim3 grid{unsigned(columns), unsigned(std::min<int64_t>(share, 65535))};
+  const int vectors = w.r.d * int(sizeof(T)) / 32;         // of a lane, if all 16 rows are new
+  auto* kernel = vectors <= 4   ? write_codes8_kernel<T, E4M3, VEC, 4>
+                 : vectors <= 8 ? write_codes8_kernel<T, E4M3, VEC, 8>
+                                : write_codes8_kernel<T, E4M3, VEC, 16>;
+  if constexpr (sizeof(T) == 4)
+    if (vectors > 16) kernel = write_codes8_kernel<T, E4M3, VEC, 32>;
+  return enigma::launch_dependent(kernel, grid, WWARPS * 32, 0, s, w);
+}
+
+template <typename T, bool E4M3, bool VEC>
+cudaError_t launch_read(const Read& w, cudaStream_t s) {
+  const unsigned grid = unsigned((int64_t(w.r.tokens) + kScaleBlock - 1) / kScaleBlock);
+  return enigma::launch_dependent(read_codes8_kernel<T, E4M3, VEC>, grid, 256, 0, s, w);
 }
 
 // The scales as pages of one row per head, which move with their codes.
@@ -289,37 +512,22 @@ cudaError_t kv_cache_q8_write(const enigma_kv_cache_q8_desc& d, int64_t layer, i
   const enigma_kv_cache_desc& c = d.cache;
   const int64_t blocks = c.pages * c.heads_kv * (c.page / kScaleBlock);       // of a layer
   Write w;
+  w.r = rows_of(c, strides4, slots, starts, cu, n, tokens);
   w.k = static_cast<uint8_t*>(c.k) + layer * blocks * kScaleBlock * c.head_dim;
   w.v = static_cast<uint8_t*>(c.v) + layer * blocks * kScaleBlock * c.head_dim;
   w.ks = d.k_scale + layer * blocks;
   w.vs = d.v_scale + layer * blocks;
   w.new_k = new_k;
   w.new_v = new_v;
-  w.table = c.table;
   w.refs = c.refs;
-  w.slots = slots;
-  w.starts = starts;
-  w.cu = cu;
   w.status = c.status;
-  w.k_token = strides4[0];
-  w.k_head = strides4[1];
-  w.v_token = strides4[2];
-  w.v_head = strides4[3];
-  w.n = int(n);
-  w.tokens = int(tokens);
-  w.heads = int(c.heads_kv);
-  w.slots_total = int(c.slots);
-  w.pages = int(c.pages);
-  w.width = int(c.table_width);
-  w.page = int(c.page);
-  w.d = int(c.head_dim);
-  w.vec = vectors(dtype, new_k, new_v, strides4);
-  const dim3 grid(unsigned((tokens + kScaleBlock - 1) / kScaleBlock), 4);
-  const bool f32 = dtype == ENIGMA_DTYPE_F32, e4m3 = d.code == ENIGMA_CODE_E4M3;
-  if (f32 && e4m3) return launch_dependent(write_codes8_kernel<float, true>, grid, 256, 0, s, w);
-  if (f32) return launch_dependent(write_codes8_kernel<float, false>, grid, 256, 0, s, w);
-  if (e4m3) return launch_dependent(write_codes8_kernel<__nv_bfloat16, true>, grid, 256, 0, s, w);
-  return launch_dependent(write_codes8_kernel<__nv_bfloat16, false>, grid, 256, 0, s, w);
+  const bool vec = vectors(dtype, new_k, new_v, strides4), e4m3 = d.code == ENIGMA_CODE_E4M3;
+  using B = __nv_bfloat16;
+  if (dtype == ENIGMA_DTYPE_F32)
+    return e4m3 ? (vec ? launch_write<float, true, true>(w, s) : launch_write<float, true, false>(w, s))
+                : (vec ? launch_write<float, false, true>(w, s) : launch_write<float, false, false>(w, s));
+  return e4m3 ? (vec ? launch_write<B, true, true>(w, s) : launch_write<B, true, false>(w, s))
+              : (vec ? launch_write<B, false, true>(w, s) : launch_write<B, false, false>(w, s));
 }
 
 cudaError_t kv_cache_q8_read(const enigma_kv_cache_q8_desc& d, int64_t layer, int dtype, void* out_k,
@@ -330,36 +538,21 @@ cudaError_t kv_cache_q8_read(const enigma_kv_cache_q8_desc& d, int64_t layer, in
   const enigma_kv_cache_desc& c = d.cache;
   const int64_t blocks = c.pages * c.heads_kv * (c.page / kScaleBlock);
   Read w;
+  w.r = rows_of(c, strides4, slots, starts, cu, n, tokens);
   w.k = static_cast<const uint8_t*>(c.k) + layer * blocks * kScaleBlock * c.head_dim;
   w.v = static_cast<const uint8_t*>(c.v) + layer * blocks * kScaleBlock * c.head_dim;
   w.ks = d.k_scale + layer * blocks;
   w.vs = d.v_scale + layer * blocks;
   w.out_k = out_k;
   w.out_v = out_v;
-  w.table = c.table;
   w.lens = c.lens;
-  w.slots = slots;
-  w.starts = starts;
-  w.cu = cu;
-  w.k_token = strides4[0];
-  w.k_head = strides4[1];
-  w.v_token = strides4[2];
-  w.v_head = strides4[3];
-  w.n = int(n);
-  w.tokens = int(tokens);
-  w.heads = int(c.heads_kv);
-  w.slots_total = int(c.slots);
-  w.pages = int(c.pages);
-  w.width = int(c.table_width);
-  w.page = int(c.page);
-  w.d = int(c.head_dim);
-  w.vec = vectors(dtype, out_k, out_v, strides4);
-  const unsigned grid = unsigned(std::min<int64_t>((tokens + 7) / 8, int64_t(sm_count()) * 32));
-  const bool f32 = dtype == ENIGMA_DTYPE_F32, e4m3 = d.code == ENIGMA_CODE_E4M3;
-  if (f32 && e4m3) return launch_dependent(read_codes8_kernel<float, true>, grid, 256, 0, s, w);
-  if (f32) return launch_dependent(read_codes8_kernel<float, false>, grid, 256, 0, s, w);
-  if (e4m3) return launch_dependent(read_codes8_kernel<__nv_bfloat16, true>, grid, 256, 0, s, w);
-  return launch_dependent(read_codes8_kernel<__nv_bfloat16, false>, grid, 256, 0, s, w);
+  const bool vec = vectors(dtype, out_k, out_v, strides4), e4m3 = d.code == ENIGMA_CODE_E4M3;
+  using B = __nv_bfloat16;
+  if (dtype == ENIGMA_DTYPE_F32)
+    return e4m3 ? (vec ? launch_read<float, true, true>(w, s) : launch_read<float, true, false>(w, s))
+                : (vec ? launch_read<float, false, true>(w, s) : launch_read<float, false, false>(w, s));
+  return e4m3 ? (vec ? launch_read<B, true, true>(w, s) : launch_read<B, true, false>(w, s))
+              : (vec ? launch_read<B, false, true>(w, s) : launch_read<B, false, false>(w, s));
 }
 
 }  // namespace enigma
