@@ -362,59 +362,69 @@ __global__ void __launch_bounds__(256) read_codes8_kernel(const __grid_constant_
   __syncthreads();
   const int cols = r.d / E, items = r.heads * cols, step_h = 32 / cols, step_c = 32 - step_h * cols;
   const int h_first = lane / cols, c_first = lane - h_first * cols;
-  for (int x = warp; x < 2 * kScaleBlock; x += 8) {        // row, K or V
-    const int kind = s_kind[x >> 1];
+  for (int x = warp; x < kScaleBlock; x += 8) {            // a row: K and V together
+    const int kind = s_kind[x];
     if (kind == 0) continue;
-    const bool is_v = x & 1;
-    const int t = t0 + (x >> 1);
-    const int64_t line = kind == 2 ? s_line[x >> 1] : 0;
-    const uint8_t* codes = (is_v ? w.v : w.k) + line * r.d;
-    const float* scales = (is_v ? w.vs : w.ks) + line / kScaleBlock;   // (a page's lines are whole blocks)
-    T* out = static_cast<T*>(is_v ? w.out_v : w.out_k) + t * (is_v ? r.v_token : r.k_token);
-    const int64_t out_head = is_v ? r.v_head : r.k_head;
+    const int t = t0 + x;
+    const int64_t line = kind == 2 ? s_line[x] : 0;
+    const uint8_t* codes[2] = {w.k + line * r.d, w.v + line * r.d};
+    const float* scales[2] = {w.ks + line / kScaleBlock, w.vs + line / kScaleBlock};   // (pages are whole blocks)
+    T* out[2] = {static_cast<T*>(w.out_k) + t * r.k_token, static_cast<T*>(w.out_v) + t * r.v_token};
+    const int64_t out_head[2] = {r.k_head, r.v_head};
     int h = h_first, c = c_first;
     for (int i0 = lane; i0 < items; i0 += 32 * READ) {
-      uint32_t code[READ][E / 4];
-      float scale[READ];
-      int hs[READ], cs[READ];
+      uint32_t code[2][READ][E / 4];
+      float scale[2][READ];
+      const int h0 = h, c0 = c;
 #pragma unroll
       for (int y = 0; y < READ; ++y) {                     // (a head past the last is the last again)
-        hs[y] = h;
-        cs[y] = c;
         const int head = min(h, r.heads - 1);
-        const uint32_t* from = reinterpret_cast<const uint32_t*>(codes + int64_t(head) * page * r.d + c * E);
-        if (E == 8) {
-          const uint2 v = *reinterpret_cast<const uint2*>(from);
-          code[y][0] = v.x;
-          code[y][E / 4 - 1] = v.y;
-        } else {
-          code[y][0] = *from;
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const uint32_t* from = reinterpret_cast<const uint32_t*>(codes[z] + int64_t(head) * page * r.d + c * E);
+          if (E == 8) {
+            const uint2 v = *reinterpret_cast<const uint2*>(from);
+            code[z][y][0] = v.x;
+            code[z][y][E / 4 - 1] = v.y;
+          } else {
+            code[z][y][0] = *from;
+          }
+          scale[z][y] = scales[z][head * per_page];
         }
-        scale[y] = scales[head * per_page];
         h += step_h;
         c += step_c;
         if (c >= cols) c -= cols, ++h;
       }
+      h = h0;
+      c = c0;
 #pragma unroll
       for (int y = 0; y < READ; ++y) {
-        uint32_t words[4];
 #pragma unroll
-        for (int z = 0; z < E / 4; ++z) {
-          uint32_t lo, hi;
-          halves_of4<E4M3>(code[y][z], &lo, &hi);
-          const float2 a = floats_of(lo), b = floats_of(hi);
-          const float f[4] = {a.x * scale[y], a.y * scale[y], b.x * scale[y], b.y * scale[y]};
-          if (E == 8) {
-            words[(2 * z) & 3] = pack_bf16x2(f[0], f[1]);
-            words[(2 * z + 1) & 3] = pack_bf16x2(f[2], f[3]);
-          } else {
+        for (int z = 0; z < 2; ++z) {
+          uint32_t words[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) words[e] = __float_as_uint(f[e]);
+          for (int i = 0; i < E / 4; ++i) {
+            uint32_t lo, hi;
+            halves_of4<E4M3>(code[z][y][i], &lo, &hi);
+            const float2 a = floats_of(lo), b = floats_of(hi);
+            const float f = scale[z][y];
+            if (E == 8) {
+              words[(2 * i) & 3] = pack_bf16x2(a.x * f, a.y * f);
+              words[(2 * i + 1) & 3] = pack_bf16x2(b.x * f, b.y * f);
+            } else {
+              words[0] = __float_as_uint(a.x * f);
+              words[1] = __float_as_uint(a.y * f);
+              words[2] = __float_as_uint(b.x * f);
+              words[3] = __float_as_uint(b.y * f);
+            }
           }
+          uint4 v = make_uint4(words[0], words[1], words[2], words[3]);
+          if (kind == 1) v = make_uint4(0, 0, 0, 0);
+          if (h < r.heads) store_vec<T, VEC>(out[z] + h * out_head[z] + c * E, v);
         }
-        uint4 v = make_uint4(words[0], words[1], words[2], words[3]);
-        if (kind == 1) v = make_uint4(0, 0, 0, 0);
-        if (hs[y] < r.heads) store_vec<T, VEC>(out + hs[y] * out_head + cs[y] * E, v);
+        h += step_h;
+        c += step_c;
+        if (c >= cols) c -= cols, ++h;
       }
     }
   }

@@ -479,17 +479,23 @@ def sdpa_quantized(q, k_pages, v_pages, k_scale, v_scale, table, lens, slots=Non
         (table.shape, table.stride(), table.dtype), (lens.shape, lens.stride(), lens.dtype),
         None if slots is None else (slots.shape, slots.stride(), slots.dtype),
         None if out is None else (out.shape, out.stride(), out.dtype), scale)
+    return _sdpa_quantized(index, head, need, [x.data_ptr() for x in (
+        k_pages, v_pages, k_scale, v_scale, table, lens)], q, slots, out, workspace)
+
+
+def _sdpa_quantized(index, head, need, pages, q, slots, out, workspace):
+    """The launch, of checked sizes and types: `pages` holds the addresses of K's and V's pages, their
+    scales, the table and the lengths, on device `index`."""
+    name = "sdpa_quantized"
     if out is None:
         out = _contiguous_like(q)
-    else:
-        _same_device(name, q, out)
+    for t in (q, out, slots):
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{name}: all tensors must be on the same device")
     ws, ws_bytes, keep = _scratch(name, workspace, need, q)
-    if slots is not None:
-        _same_device(name, q, slots)
-    desc = head + _CODES_PTRS.pack(table.data_ptr(), lens.data_ptr(),
-                                   0 if slots is None else slots.data_ptr(), q.data_ptr(),
-                                   k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(),
-                                   v_scale.data_ptr(), out.data_ptr(), ws, ws_bytes)
+    k, v, ks, vs, table, lens = pages
+    desc = head + _CODES_PTRS.pack(table, lens, 0 if slots is None else slots.data_ptr(), q.data_ptr(),
+                                   k, v, ks, vs, out.data_ptr(), ws, ws_bytes)
     _launch(index, "enigma_sdpa_quantized", desc, _raw_stream(index))
     return out
 

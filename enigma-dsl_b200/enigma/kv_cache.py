@@ -232,6 +232,7 @@ class QuantizedKVCache(PagedKVCache):
         self._setup(k, v, table, lens, refs)
         self._q8 = _QuantizedDesc(self._desc, k_scale.data_ptr(), v_scale.data_ptr(), code, 0)
         self._q8_ref = ctypes.byref(self._q8)
+        self._heads = {}         # checked calls' sizes, strides and types
 
     @classmethod
     def empty(cls, layers: int, pages: int, page: int, heads_kv: int, head_dim: int, slots: int,
@@ -272,24 +273,41 @@ class QuantizedKVCache(PagedKVCache):
     compact.__doc__ = PagedKVCache.compact.__doc__
     copy_pages.__doc__ = PagedKVCache.copy_pages.__doc__
 
-    def _rows(self, name, layer, k, v, slots, starts, cu):
-        """Checks a write's or read's rows; the request on the device and what C takes of the rows."""
-        if len(k.shape) != 3 or k.shape != v.shape or k.shape[1:] != self._row:
+    def _checked(self, key, check):
+        """What `check(*key)` packs, made once for these sizes, strides and types."""
+        head = self._heads.get(key)
+        if head is None:
+            head = check(*key)
+            if len(self._heads) >= 256:
+                self._heads.clear()
+            self._heads[key] = head
+        return head
+
+    def _rows_head(self, name, layer, k, v):
+        """Checks the (shape, stride, dtype) of a write's or read's rows; their type, strides, number."""
+        (shape, ks, kind), vs = k, v[1]
+        if len(shape) != 3 or shape != v[0] or shape[1:] != self._row:
             raise ValueError(f"{name}: expected rows [tokens, {self._row[0]}, {self._row[1]}]")
-        shape, ks, vs = k.shape, k.stride(), v.stride()
-        dtype = cuda_ops._check_rows(name, k.dtype, (shape, ks, k.dtype), (shape, vs, v.dtype))
-        cuda_ops._same_device(name, self.k, k, v)
+        dtype = cuda_ops._check_rows(name, kind, k, v)
+        if name == "read":
+            cuda_ops._check_distinct(name, k, v)
         if not 0 <= layer < self.layers:
             raise ValueError(f"{name}: layer {layer} of {self.layers}")
+        return dtype, _STRIDES.pack(ks[0], ks[1], vs[0], vs[1]), shape[0]
+
+    def _rows_call(self, name, entry, layer, k, v, slots, starts, cu):
+        dtype, strides, tokens = self._checked(
+            (name, layer, (k.shape, k.stride(), k.dtype), (v.shape, v.stride(), v.dtype)),
+            self._rows_head)
+        cuda_ops._same_device(name, self.k, k, v)
         slots = self._ints(name, slots)
         starts = self._ints(name, starts, slots)
         cu = self._ints(name, cu)
         n = slots.shape[0]
         if cu.shape[0] != n + 1:
             raise ValueError(f"{name}: cu holds one number more than there are slots")
-        # The request's tensors come back too: they live until the launch is queued.
-        return (layer, dtype, k.data_ptr(), v.data_ptr(), _STRIDES.pack(ks[0], ks[1], vs[0], vs[1]),
-                slots.data_ptr(), starts.data_ptr(), cu.data_ptr(), n, shape[0]), (slots, starts, cu)
+        self._call_q8(entry, layer, dtype, k.data_ptr(), v.data_ptr(), strides, slots.data_ptr(),
+                      starts.data_ptr(), cu.data_ptr(), n, tokens)
 
     def write(self, layer: int, new_k, new_v, slots, starts, cu) -> None:
         """Rows cu[i] .. cu[i + 1] of new_k / new_v [tokens, heads_kv, head_dim], bf16 or fp32, are
@@ -299,8 +317,7 @@ class QuantizedKVCache(PagedKVCache):
         what the block of 16 held behind.  Pages that forks share are not written (`check` says so;
         appending never meets one), nor is a block that two entries of one call name.  A value that is
         not finite makes its block of 16 tokens NaN."""
-        args, keep = self._rows("write", layer, new_k, new_v, slots, starts, cu)
-        self._call_q8("enigma_kv_cache_q8_write", *args)
+        self._rows_call("write", "enigma_kv_cache_q8_write", layer, new_k, new_v, slots, starts, cu)
 
     def read(self, layer: int, slots, starts, cu, tokens: Optional[int] = None, dtype=None,
              out_k=None, out_v=None):
@@ -320,19 +337,28 @@ class QuantizedKVCache(PagedKVCache):
                     raise ValueError("read: tokens must be given where cu is on the device")
                 tokens = int(cu[-1]) if len(cu) else 0
             dtype = torch.bfloat16 if dtype is None else dtype
-            shape = (int(tokens), *self._row)
-            out_k, out_v = (torch.empty(shape, dtype=dtype, device=self.k.device) for _ in range(2))
+            out_k, out_v = torch.empty((2, int(tokens), *self._row), dtype=dtype,
+                                       device=self.k.device).unbind()
         elif tokens not in (None, out_k.shape[0]) or dtype not in (None, out_k.dtype):
             raise ValueError("read: out_k and out_v have another size or type")
-        args, keep = self._rows("read", layer, out_k, out_v, slots, starts, cu)
-        cuda_ops._check_distinct("read", *((x.shape, x.stride(), None) for x in (out_k, out_v)))
-        self._call_q8("enigma_kv_cache_q8_read", *args)
+        self._rows_call("read", "enigma_kv_cache_q8_read", layer, out_k, out_v, slots, starts, cu)
         return out_k, out_v
 
     def attend(self, layer: int, q, slots=None, scale: Optional[float] = None, out=None,
                workspace=None):
         """cuda_ops.sdpa_quantized over one layer of this cache."""
-        return cuda_ops.sdpa_quantized(q, self.k[layer], self.v[layer], self.k_scale[layer],
-                                       self.v_scale[layer], self.table, self.lens,
-                                       slots=None if slots is None else self._ints("attend", slots),
-                                       scale=scale, out=out, workspace=workspace)
+        slots = None if slots is None else self._ints("attend", slots)
+        head, need, pages = self._checked(
+            (layer, (q.shape, q.stride(), q.dtype), None if slots is None else slots.shape,
+             None if out is None else (out.shape, out.stride(), out.dtype), scale), self._attend_head)
+        return cuda_ops._sdpa_quantized(self._index, head, need, pages, q, slots, out, workspace)
+
+    def _attend_head(self, layer, q, slots, out, scale):
+        """Checks the (shape, stride, dtype) of an attend; the desc's head, bytes of workspace, and the
+        addresses of what is read of the cache."""
+        parts = [x[layer] for x in (self.k, self.v, self.k_scale, self.v_scale)] + [self.table, self.lens]
+        described = [(x.shape, x.stride(), x.dtype) for x in parts]
+        head, need = cuda_ops._quantized_head(
+            self._index, q, *described, None if slots is None else (slots, (1,), self.table.dtype),
+            out, scale)
+        return head, need, [x.data_ptr() for x in parts]
