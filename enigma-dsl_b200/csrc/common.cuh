@@ -107,13 +107,9 @@ cudaError_t kv_cache_q8_fork(const enigma_kv_cache_q8_desc& d, const int32_t* pa
 cudaError_t kv_cache_q8_compact(const enigma_kv_cache_q8_desc& d, cudaStream_t s);
 cudaError_t kv_cache_q8_copy_pages(const enigma_kv_cache_q8_desc& d, const int32_t* src,
                                    const int32_t* dst, int64_t n, cudaStream_t s);
-cudaError_t kv_cache_q8_write(const enigma_kv_cache_q8_desc& d, int64_t layer, int dtype,
-                              const void* new_k, const void* new_v, const int64_t* strides4,
-                              const int32_t* slots, const int32_t* starts, const int32_t* cu,
-                              int64_t n, int64_t tokens, cudaStream_t s);
-cudaError_t kv_cache_q8_read(const enigma_kv_cache_q8_desc& d, int64_t layer, int dtype, void* out_k,
-                             void* out_v, const int64_t* strides4, const int32_t* slots,
-                             const int32_t* starts, const int32_t* cu, int64_t n, int64_t tokens,
+cudaError_t kv_cache_q8_write(const enigma_kv_cache_q8_desc& d, const enigma_kv_cache_rows& rows,
+                              cudaStream_t s);
+cudaError_t kv_cache_q8_read(const enigma_kv_cache_q8_desc& d, const enigma_kv_cache_rows& rows,
                              cudaStream_t s);
 size_t sdpa_quantized_workspace(const enigma_sdpa_quantized_desc& d);
 cudaError_t sdpa_quantized_launch(const enigma_sdpa_quantized_desc& d, cudaStream_t s);

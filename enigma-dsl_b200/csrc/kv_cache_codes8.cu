@@ -431,25 +431,23 @@ __global__ void __launch_bounds__(256) read_codes8_kernel(const __grid_constant_
 }
 
 // Rows that can be moved 16 bytes at a time.
-bool vectors(int dtype, const void* k, const void* v, const int64_t* strides4) {
-  bool ok = aligned(k, 16) && aligned(v, 16);
-  for (int i = 0; i < 4; ++i) ok = ok && strides4[i] * (dtype == ENIGMA_DTYPE_F32 ? 4 : 2) % 16 == 0;
-  return ok;
+bool vectors(const enigma_kv_cache_rows& w) {
+  const int64_t all = w.k_token | w.k_head | w.v_token | w.v_head, es = w.dtype == ENIGMA_DTYPE_F32 ? 4 : 2;
+  return aligned(w.k, 16) && aligned(w.v, 16) && all * es % 16 == 0;
 }
 
-Rows rows_of(const enigma_kv_cache_desc& c, const int64_t* strides4, const int32_t* slots,
-             const int32_t* starts, const int32_t* cu, int64_t n, int64_t tokens) {
+Rows rows_of(const enigma_kv_cache_desc& c, const enigma_kv_cache_rows& w) {
   Rows r;
   r.table = c.table;
-  r.slots = slots;
-  r.starts = starts;
-  r.cu = cu;
-  r.k_token = strides4[0];
-  r.k_head = strides4[1];
-  r.v_token = strides4[2];
-  r.v_head = strides4[3];
-  r.n = int(n);
-  r.tokens = int(tokens);
+  r.slots = w.slots;
+  r.starts = w.starts;
+  r.cu = w.cu;
+  r.k_token = w.k_token;
+  r.k_head = w.k_head;
+  r.v_token = w.v_token;
+  r.v_head = w.v_head;
+  r.n = int(w.n);
+  r.tokens = int(w.tokens);
   r.heads = int(c.heads_kv);
   r.slots_total = int(c.slots);
   r.pages = int(c.pages);
@@ -514,51 +512,47 @@ cudaError_t kv_cache_q8_copy_pages(const enigma_kv_cache_q8_desc& d, const int32
   return e == cudaSuccess ? kv_cache_copy_pages(scales_of(d), src, dst, n, s) : e;
 }
 
-cudaError_t kv_cache_q8_write(const enigma_kv_cache_q8_desc& d, int64_t layer, int dtype,
-                              const void* new_k, const void* new_v, const int64_t* strides4,
-                              const int32_t* slots, const int32_t* starts, const int32_t* cu,
-                              int64_t n, int64_t tokens, cudaStream_t s) {
+cudaError_t kv_cache_q8_write(const enigma_kv_cache_q8_desc& d, const enigma_kv_cache_rows& rows,
+                              cudaStream_t s) {
   note_kernel("write_codes8_kernel");
   const enigma_kv_cache_desc& c = d.cache;
   const int64_t blocks = c.pages * c.heads_kv * (c.page / kScaleBlock);       // of a layer
   Write w;
-  w.r = rows_of(c, strides4, slots, starts, cu, n, tokens);
-  w.k = static_cast<uint8_t*>(c.k) + layer * blocks * kScaleBlock * c.head_dim;
-  w.v = static_cast<uint8_t*>(c.v) + layer * blocks * kScaleBlock * c.head_dim;
-  w.ks = d.k_scale + layer * blocks;
-  w.vs = d.v_scale + layer * blocks;
-  w.new_k = new_k;
-  w.new_v = new_v;
+  w.r = rows_of(c, rows);
+  w.k = static_cast<uint8_t*>(c.k) + rows.layer * blocks * kScaleBlock * c.head_dim;
+  w.v = static_cast<uint8_t*>(c.v) + rows.layer * blocks * kScaleBlock * c.head_dim;
+  w.ks = d.k_scale + rows.layer * blocks;
+  w.vs = d.v_scale + rows.layer * blocks;
+  w.new_k = rows.k;
+  w.new_v = rows.v;
   w.refs = c.refs;
   w.status = c.status;
-  const bool vec = vectors(dtype, new_k, new_v, strides4), e4m3 = d.code == ENIGMA_CODE_E4M3;
+  const bool vec = vectors(rows), e4m3 = d.code == ENIGMA_CODE_E4M3;
   using B = __nv_bfloat16;
-  if (dtype == ENIGMA_DTYPE_F32)
+  if (rows.dtype == ENIGMA_DTYPE_F32)
     return e4m3 ? (vec ? launch_write<float, true, true>(w, s) : launch_write<float, true, false>(w, s))
                 : (vec ? launch_write<float, false, true>(w, s) : launch_write<float, false, false>(w, s));
   return e4m3 ? (vec ? launch_write<B, true, true>(w, s) : launch_write<B, true, false>(w, s))
               : (vec ? launch_write<B, false, true>(w, s) : launch_write<B, false, false>(w, s));
 }
 
-cudaError_t kv_cache_q8_read(const enigma_kv_cache_q8_desc& d, int64_t layer, int dtype, void* out_k,
-                             void* out_v, const int64_t* strides4, const int32_t* slots,
-                             const int32_t* starts, const int32_t* cu, int64_t n, int64_t tokens,
+cudaError_t kv_cache_q8_read(const enigma_kv_cache_q8_desc& d, const enigma_kv_cache_rows& rows,
                              cudaStream_t s) {
   note_kernel("read_codes8_kernel");
   const enigma_kv_cache_desc& c = d.cache;
   const int64_t blocks = c.pages * c.heads_kv * (c.page / kScaleBlock);
   Read w;
-  w.r = rows_of(c, strides4, slots, starts, cu, n, tokens);
-  w.k = static_cast<const uint8_t*>(c.k) + layer * blocks * kScaleBlock * c.head_dim;
-  w.v = static_cast<const uint8_t*>(c.v) + layer * blocks * kScaleBlock * c.head_dim;
-  w.ks = d.k_scale + layer * blocks;
-  w.vs = d.v_scale + layer * blocks;
-  w.out_k = out_k;
-  w.out_v = out_v;
+  w.r = rows_of(c, rows);
+  w.k = static_cast<const uint8_t*>(c.k) + rows.layer * blocks * kScaleBlock * c.head_dim;
+  w.v = static_cast<const uint8_t*>(c.v) + rows.layer * blocks * kScaleBlock * c.head_dim;
+  w.ks = d.k_scale + rows.layer * blocks;
+  w.vs = d.v_scale + rows.layer * blocks;
+  w.out_k = rows.k;
+  w.out_v = rows.v;
   w.lens = c.lens;
-  const bool vec = vectors(dtype, out_k, out_v, strides4), e4m3 = d.code == ENIGMA_CODE_E4M3;
+  const bool vec = vectors(rows), e4m3 = d.code == ENIGMA_CODE_E4M3;
   using B = __nv_bfloat16;
-  if (dtype == ENIGMA_DTYPE_F32)
+  if (rows.dtype == ENIGMA_DTYPE_F32)
     return e4m3 ? (vec ? launch_read<float, true, true>(w, s) : launch_read<float, true, false>(w, s))
                 : (vec ? launch_read<float, false, true>(w, s) : launch_read<float, false, false>(w, s));
   return e4m3 ? (vec ? launch_read<B, true, true>(w, s) : launch_read<B, true, false>(w, s))

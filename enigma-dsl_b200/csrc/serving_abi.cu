@@ -123,22 +123,23 @@ int32_t check_q8(const enigma_kv_cache_q8_desc* d) {
 }
 
 // The rows of a write or read.
-int32_t check_rows(const enigma_kv_cache_q8_desc* d, int64_t layer, int32_t dtype, const void* k,
-                   const void* v, const int64_t* strides4, const int32_t* slots,
-                   const int32_t* starts, const int32_t* cu, int64_t n, int64_t tokens) {
-  if (layer < 0 || layer >= d->cache.layers) return bad("kv_cache_q8: layer out of range");
-  if (dtype != ENIGMA_DTYPE_F32 && dtype != ENIGMA_DTYPE_BF16) return bad("kv_cache_q8: dtype");
-  if (n < 0 || tokens < 0 || n > kInt31 - 256 || tokens > kInt31 - 256)
+int32_t check_rows(const enigma_kv_cache_q8_desc* d, const enigma_kv_cache_rows* w) {
+  if (w == nullptr) return bad("kv_cache_q8: rows is NULL");
+  if (w->layer < 0 || w->layer >= d->cache.layers) return bad("kv_cache_q8: layer out of range");
+  if (w->dtype != ENIGMA_DTYPE_F32 && w->dtype != ENIGMA_DTYPE_BF16) return bad("kv_cache_q8: dtype");
+  if (w->n < 0 || w->tokens < 0 || w->n > kInt31 - 256 || w->tokens > kInt31 - 256)
     return bad("kv_cache_q8: request size");
-  if (tokens == 0) return ENIGMA_OK;
-  if (n == 0) return bad("kv_cache_q8: rows without a slot");
-  if (k == nullptr || v == nullptr || strides4 == nullptr || slots == nullptr ||
-      starts == nullptr || cu == nullptr)
+  if (w->tokens == 0) return ENIGMA_OK;
+  if (w->n == 0) return bad("kv_cache_q8: rows without a slot");
+  if (w->k == nullptr || w->v == nullptr || w->slots == nullptr || w->starts == nullptr ||
+      w->cu == nullptr)
     return bad("kv_cache_q8: NULL request");
-  for (int i = 0; i < 4; ++i)
-    if (strides4[i] < 0) return bad("kv_cache_q8: negative stride");
-  const size_t es = dtype == ENIGMA_DTYPE_F32 ? 4 : 2;
-  if (!aligned(k, es) || !aligned(v, es)) return bad("kv_cache_q8: misaligned buffer");
+  if (w->k_token < 0 || w->k_head < 0 || w->v_token < 0 || w->v_head < 0)
+    return bad("kv_cache_q8: negative stride");
+  const size_t es = w->dtype == ENIGMA_DTYPE_F32 ? 4 : 2;
+  if (!aligned(w->k, es) || !aligned(w->v, es) || !aligned(w->slots, 4) || !aligned(w->starts, 4) ||
+      !aligned(w->cu, 4))
+    return bad("kv_cache_q8: misaligned buffer");
   return ENIGMA_OK;
 }
 
@@ -398,30 +399,20 @@ int32_t enigma_kv_cache_q8_copy_pages(const enigma_kv_cache_q8_desc* d, const in
                        "kv_cache_q8_copy_pages");
 }
 
-int32_t enigma_kv_cache_q8_write(const enigma_kv_cache_q8_desc* d, int64_t layer, int32_t dtype,
-                                 const void* new_k, const void* new_v, const int64_t* strides4,
-                                 const int32_t* slots, const int32_t* starts, const int32_t* cu,
-                                 int64_t n, int64_t tokens, void* stream) {
+int32_t enigma_kv_cache_q8_write(const enigma_kv_cache_q8_desc* d, const enigma_kv_cache_rows* rows,
+                                 void* stream) {
   int32_t e = check_q8(d);
-  if (e == ENIGMA_OK)
-    e = check_rows(d, layer, dtype, new_k, new_v, strides4, slots, starts, cu, n, tokens);
-  if (e != ENIGMA_OK || tokens == 0) return e;
-  return launch_status(enigma::kv_cache_q8_write(*d, layer, dtype, new_k, new_v, strides4, slots,
-                                                 starts, cu, n, tokens, as_stream(stream)),
-                       "kv_cache_q8_write");
+  if (e == ENIGMA_OK) e = check_rows(d, rows);
+  if (e != ENIGMA_OK || rows->tokens == 0) return e;
+  return launch_status(enigma::kv_cache_q8_write(*d, *rows, as_stream(stream)), "kv_cache_q8_write");
 }
 
-int32_t enigma_kv_cache_q8_read(const enigma_kv_cache_q8_desc* d, int64_t layer, int32_t dtype,
-                                void* out_k, void* out_v, const int64_t* strides4,
-                                const int32_t* slots, const int32_t* starts, const int32_t* cu,
-                                int64_t n, int64_t tokens, void* stream) {
+int32_t enigma_kv_cache_q8_read(const enigma_kv_cache_q8_desc* d, const enigma_kv_cache_rows* rows,
+                                void* stream) {
   int32_t e = check_q8(d);
-  if (e == ENIGMA_OK)
-    e = check_rows(d, layer, dtype, out_k, out_v, strides4, slots, starts, cu, n, tokens);
-  if (e != ENIGMA_OK || tokens == 0) return e;
-  return launch_status(enigma::kv_cache_q8_read(*d, layer, dtype, out_k, out_v, strides4, slots,
-                                                starts, cu, n, tokens, as_stream(stream)),
-                       "kv_cache_q8_read");
+  if (e == ENIGMA_OK) e = check_rows(d, rows);
+  if (e != ENIGMA_OK || rows->tokens == 0) return e;
+  return launch_status(enigma::kv_cache_q8_read(*d, *rows, as_stream(stream)), "kv_cache_q8_read");
 }
 
 int32_t enigma_sdpa_quantized_workspace_bytes(const enigma_sdpa_quantized_desc* d, size_t* bytes) {

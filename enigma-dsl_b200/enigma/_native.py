@@ -90,8 +90,8 @@ PROTOTYPES = {
     "enigma_kv_cache_q8_fork": [_vp, _vp, _vp, _i64, _vp],
     "enigma_kv_cache_q8_compact": [_vp, _vp],
     "enigma_kv_cache_q8_copy_pages": [_vp, _vp, _vp, _i64, _vp],
-    "enigma_kv_cache_q8_write": [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp],
-    "enigma_kv_cache_q8_read": [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp],
+    "enigma_kv_cache_q8_write": [_vp, _vp, _vp],
+    "enigma_kv_cache_q8_read": [_vp, _vp, _vp],
     "enigma_sdpa_quantized_workspace_bytes": [_vp, _c.POINTER(_sz)],
     "enigma_sdpa_quantized": [_vp, _vp],
     "enigma_dispatch": [_i32, _c.POINTER(_vp), _i32, _c.POINTER(_i64), _i32, _c.POINTER(_f32),

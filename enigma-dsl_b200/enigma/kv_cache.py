@@ -32,6 +32,10 @@ class _CacheDesc(ctypes.Structure):
 
 
 _STRIDES = struct.Struct("4q")
+# enigma_kv_cache_rows (include/enigma_cuda.h): layer, entries, tokens; strides and type; pointers.
+_ROWS = struct.Struct("3q")
+_ROWS_KIND = struct.Struct("4q2i")
+_ROWS_PTRS = struct.Struct("5Q")
 
 
 class PagedKVCache:
@@ -284,7 +288,7 @@ class QuantizedKVCache(PagedKVCache):
         return head
 
     def _rows_head(self, name, layer, k, v):
-        """Checks the (shape, stride, dtype) of a write's or read's rows; their type, strides, number."""
+        """Checks the (shape, stride, dtype) of a write's or read's rows; strides and type, their number."""
         (shape, ks, kind), vs = k, v[1]
         if len(shape) != 3 or shape != v[0] or shape[1:] != self._row:
             raise ValueError(f"{name}: expected rows [tokens, {self._row[0]}, {self._row[1]}]")
@@ -293,21 +297,36 @@ class QuantizedKVCache(PagedKVCache):
             cuda_ops._check_distinct(name, k, v)
         if not 0 <= layer < self.layers:
             raise ValueError(f"{name}: layer {layer} of {self.layers}")
-        return dtype, _STRIDES.pack(ks[0], ks[1], vs[0], vs[1]), shape[0]
+        return _ROWS_KIND.pack(ks[0], ks[1], vs[0], vs[1], dtype, 0), shape[0]
 
     def _rows_call(self, name, entry, layer, k, v, slots, starts, cu):
-        dtype, strides, tokens = self._checked(
+        kind, tokens = self._checked(
             (name, layer, (k.shape, k.stride(), k.dtype), (v.shape, v.stride(), v.dtype)),
             self._rows_head)
         cuda_ops._same_device(name, self.k, k, v)
-        slots = self._ints(name, slots)
-        starts = self._ints(name, starts, slots)
-        cu = self._ints(name, cu)
+        if not self._are_ints(slots, starts, cu):
+            slots = self._ints(name, slots)
+            starts = self._ints(name, starts)
+            cu = self._ints(name, cu)
         n = slots.shape[0]
+        if starts.shape[0] != n:
+            raise ValueError(f"{name}: the request's parts differ in length")
         if cu.shape[0] != n + 1:
             raise ValueError(f"{name}: cu holds one number more than there are slots")
-        self._call_q8(entry, layer, dtype, k.data_ptr(), v.data_ptr(), strides, slots.data_ptr(),
-                      starts.data_ptr(), cu.data_ptr(), n, tokens)
+        self._call_q8(entry, _ROWS.pack(layer, n, tokens) + kind + _ROWS_PTRS.pack(
+            k.data_ptr(), v.data_ptr(), slots.data_ptr(), starts.data_ptr(), cu.data_ptr()))
+
+    def _are_ints(self, *parts) -> bool:
+        """Whether a request's parts are what `_ints` would make of them."""
+        int32, index = cuda_ops._torch().int32, self._index
+        try:
+            for x in parts:
+                if x.dtype is not int32 or x.get_device() != index or x.dim() != 1 \
+                        or not x.is_contiguous():
+                    return False
+        except (AttributeError, TypeError):                  # a list, an array
+            return False
+        return True
 
     def write(self, layer: int, new_k, new_v, slots, starts, cu) -> None:
         """Rows cu[i] .. cu[i + 1] of new_k / new_v [tokens, heads_kv, head_dim], bf16 or fp32, are

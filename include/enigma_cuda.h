@@ -365,7 +365,7 @@ int32_t enigma_rope(const enigma_rope_desc* desc, void* stream);
  * scale.  head_dim is a multiple of 16 up to 256, page 16, 32, 64 or 128; pages are 16-byte aligned.
  * enigma_kv_cache_free and enigma_kv_cache_reserve take `cache` itself; fork, compact and
  * copy_pages are those of enigma_kv_cache_* with the scales moved along.
- *   write  as enigma_kv_cache_write, from rows of type dtype.  The scale of a block is the least
+ *   write  as enigma_kv_cache_write, from rows of any type.  The scale of a block is the least
  *          power of two 2^e under which the block's largest magnitude (2^-110 if that is more) is at most
  *          127, or 448, and a code is the value over the scale, rounded to nearest (ties to
  *          even).  A write that starts behind a block's first token keeps the block's earlier
@@ -375,8 +375,7 @@ int32_t enigma_rope(const enigma_rope_desc* desc, void* stream);
  *          a write starts the block anew.  A page that forks share is not written
  *          (ENIGMA_CACHE_SHARED), nor is a block that two entries of a request name
  *          (ENIGMA_CACHE_BAD_REQUEST).
- *   read   rows cu[i] .. cu[i + 1] of out_k / out_v [tokens, heads_kv, head_dim] of type dtype
- *          (strides4 as in write) get the tokens starts[i], ... of slots[i]; a token that the slot does
+ *   read   rows cu[i] .. cu[i + 1] get the tokens starts[i], ... of slots[i]; a token that the slot does
  *          not hold gives zeros; rows before cu[0] and behind cu[n] are left as they were. */
 #define ENIGMA_SCALE_BLOCK 16
 #define ENIGMA_CODE_INT8 0
@@ -392,14 +391,18 @@ int32_t enigma_kv_cache_q8_fork(const enigma_kv_cache_q8_desc* desc, const int32
 int32_t enigma_kv_cache_q8_compact(const enigma_kv_cache_q8_desc* desc, void* stream);
 int32_t enigma_kv_cache_q8_copy_pages(const enigma_kv_cache_q8_desc* desc, const int32_t* src,
                                       const int32_t* dst, int64_t n, void* stream);
-int32_t enigma_kv_cache_q8_write(const enigma_kv_cache_q8_desc* desc, int64_t layer, int32_t dtype,
-                                 const void* new_k, const void* new_v, const int64_t* strides4,
-                                 const int32_t* slots, const int32_t* starts, const int32_t* cu,
-                                 int64_t n, int64_t tokens, void* stream);
-int32_t enigma_kv_cache_q8_read(const enigma_kv_cache_q8_desc* desc, int64_t layer, int32_t dtype,
-                                void* out_k, void* out_v, const int64_t* strides4,
-                                const int32_t* slots, const int32_t* starts, const int32_t* cu,
-                                int64_t n, int64_t tokens, void* stream);
+/* Rows [tokens, heads_kv, head_dim] of one layer and the n entries of a request: what a write puts
+ * into the cache, or where a read puts them.  Strides in elements. */
+typedef struct enigma_kv_cache_rows {
+  int64_t layer, n, tokens, k_token, k_head, v_token, v_head;
+  int32_t dtype, reserved;
+  void *k, *v;
+  const int32_t *slots, *starts, *cu;
+} enigma_kv_cache_rows;
+int32_t enigma_kv_cache_q8_write(const enigma_kv_cache_q8_desc* desc, const enigma_kv_cache_rows* rows,
+                                 void* stream);
+int32_t enigma_kv_cache_q8_read(const enigma_kv_cache_q8_desc* desc, const enigma_kv_cache_rows* rows,
+                                void* stream);
 
 /* One new token per sequence over pages of 8-bit codes: q, out [batch, heads_q, head_dim] of type
  * dtype; k_pages, v_pages [pages, heads_kv, page, head_dim] codes, contiguous but for the page

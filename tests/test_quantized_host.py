@@ -228,6 +228,13 @@ def test_c_rope_refuses():
             assert lib.enigma_rope(ctypes.byref(d), None) == _native.ERR_BADARG, (key, x)
 
 
+class _Rows(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("layer", "n", "tokens", "k_token", "k_head", "v_token",
+                                              "v_head")] + \
+        [(n, ctypes.c_int32) for n in ("dtype", "reserved")] + \
+        [(n, ctypes.c_void_p) for n in ("k", "v", "slots", "starts", "cu")]
+
+
 def test_c_cache_refuses():
     from enigma import _native
     from enigma.kv_cache import _CacheDesc, _QuantizedDesc
@@ -252,16 +259,16 @@ def test_c_cache_refuses():
         assert lib.enigma_kv_cache_q8_compact(d, None) == bad
         assert lib.enigma_kv_cache_q8_fork(d, 64, 64, 0, None) == bad
         assert lib.enigma_kv_cache_q8_copy_pages(d, 64, 64, 0, None) == bad
-    strides = (ctypes.c_int64 * 4)(128, 64, 128, 64)
-    below = (ctypes.c_int64 * 4)(128, 64, -1, 64)
+    good = dict(layer=0, n=1, tokens=1, k_token=128, k_head=64, v_token=128, v_head=64, dtype=1, k=64, v=64,
+                slots=64, starts=64, cu=64)
     for fn in (lib.enigma_kv_cache_q8_write, lib.enigma_kv_cache_q8_read):
-        assert fn(desc(), 0, 1, 64, 64, strides, 64, 64, 64, 1, 0, None) == 0
-        for args in ((1, 1, 64, 64, strides, 64, 64, 64, 1, 1), (0, 2, 64, 64, strides, 64, 64, 64, 1, 1),
-                     (0, 1, 0, 64, strides, 64, 64, 64, 1, 1), (0, 1, 65, 64, strides, 64, 64, 64, 1, 1),
-                     (0, 1, 64, 64, below, 64, 64, 64, 1, 1), (0, 1, 64, 64, strides, 0, 64, 64, 1, 1),
-                     (0, 1, 64, 64, strides, 64, 64, 64, 0, 1), (0, 1, 64, 64, strides, 64, 64, 64, 1, -1),
-                     (0, 1, 64, 64, strides, 64, 64, 64, 1, 1 << 31)):
-            assert fn(desc(), *args, None) == bad, args
+        assert fn(desc(), ctypes.byref(_Rows(**{**good, "tokens": 0})), None) == 0
+        assert fn(desc(), None, None) == bad and fn(None, ctypes.byref(_Rows(**good)), None) == bad
+        for key, values in dict(layer=[-1, 1], n=[0, -1, 1 << 31], tokens=[-1, 1 << 31], k_token=[-1],
+                                k_head=[-1], v_token=[-1], v_head=[-1], dtype=[2], k=[0, 65], v=[0, 65],
+                                slots=[0, 66], starts=[0, 66], cu=[0, 66]).items():
+            for x in values:
+                assert fn(desc(), ctypes.byref(_Rows(**{**good, key: x})), None) == bad, (key, x)
     for n in (-1, 5):
         assert lib.enigma_kv_cache_q8_copy_pages(desc(), 64, 64, n, None) == bad
     assert lib.enigma_kv_cache_q8_fork(desc(), 64, 64, 3, None) == bad
