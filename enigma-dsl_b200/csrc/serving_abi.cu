@@ -1,6 +1,7 @@
 // serving_abi.cu — C-ABI entry points of the serving operators (packed prompt attention, paged
-// attention with a shared prefix, page operations, rotary positions, the cache in 8-bit codes).  Validation happens here; the kernels
-// check what only the device knows (page numbers, slots, lengths).
+// attention with a shared prefix, page operations, rotary positions, the cache in 8-bit codes).
+// Validation happens here; the kernels check what only the device knows (page numbers, slots,
+// lengths).
 #include <algorithm>
 #include <exception>
 #include <vector>
@@ -113,6 +114,7 @@ int32_t check_q8(const enigma_kv_cache_q8_desc* d) {
   int32_t e = check_cache(&d->cache, true, true);
   if (e != ENIGMA_OK) return e;
   if (d->cache.elem_bytes != 1) return bad("kv_cache_q8: elem_bytes must be 1");
+  if (d->cache.heads_kv > 65535) return bad("kv_cache_q8: heads_kv must be at most 65535");
   e = check_codes(d->cache.head_dim, d->cache.page, d->code);
   if (e != ENIGMA_OK) return e;
   if (d->k_scale == nullptr || d->v_scale == nullptr) return bad("kv_cache_q8: NULL buffer");
@@ -156,6 +158,10 @@ int32_t check_quantized(const enigma_sdpa_quantized_desc* d) {
   if (d->pages > kInt31 / (d->heads_kv * d->page) || d->table_width > (kInt31 - 256) / d->page ||
       d->n_slots > kInt31)
     return bad("sdpa_quantized: sizes must fit in int32");
+  // The kernel counts a batch's chunks of 16 keys or more in 32 bits, a thread's share of all heads' too.
+  const int64_t chunks = d->batch * (d->table_width * d->page / 16 + 2);
+  if (chunks > kInt31 || double(chunks) * double(d->heads_q) > 1e12)
+    return bad("sdpa_quantized: more keys than one call takes");
   return ENIGMA_OK;
 }
 

@@ -367,17 +367,22 @@ class QuantizedKVCache(PagedKVCache):
                workspace=None):
         """cuda_ops.sdpa_quantized over one layer of this cache."""
         slots = None if slots is None else self._ints("attend", slots)
-        head, need, pages = self._checked(
+        head, need, steps = self._checked(
             (layer, (q.shape, q.stride(), q.dtype), None if slots is None else slots.shape,
              None if out is None else (out.shape, out.stride(), out.dtype), scale), self._attend_head)
+        pages = [x.data_ptr() + step for x, step in zip(
+            (self.k, self.v, self.k_scale, self.v_scale, self.table, self.lens), steps)]
         return cuda_ops._sdpa_quantized(self._index, head, need, pages, q, slots, out, workspace)
 
     def _attend_head(self, layer, q, slots, out, scale):
-        """Checks the (shape, stride, dtype) of an attend; the desc's head, bytes of workspace, and the
-        addresses of what is read of the cache."""
-        parts = [x[layer] for x in (self.k, self.v, self.k_scale, self.v_scale)] + [self.table, self.lens]
-        described = [(x.shape, x.stride(), x.dtype) for x in parts]
+        """Checks the (shape, stride, dtype) of an attend; the desc's head, bytes of workspace, and where
+        in the cache's tensors the layer begins."""
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"attend: layer {layer} of {self.layers}")
+        pools = (self.k, self.v, self.k_scale, self.v_scale)
+        described = [(x.shape, x.stride(), x.dtype)
+                     for x in [y[layer] for y in pools] + [self.table, self.lens]]
         head, need = cuda_ops._quantized_head(
             self._index, q, *described, None if slots is None else (slots, (1,), self.table.dtype),
             out, scale)
-        return head, need, [x.data_ptr() for x in parts]
+        return head, need, [layer * x.stride(0) * x.element_size() for x in pools] + [0, 0]

@@ -413,8 +413,9 @@ int32_t enigma_kv_cache_q8_read(const enigma_kv_cache_q8_desc* desc, const enigm
  * enigma_sdpa_shared_prefix: no keys, or a slot that does not exist, give zeros, and a key whose
  * table entry is no page is a key and a value of zeros.  A code or scale that is seen and is NaN
  * gives NaN; what no sequence sees may hold anything.  scale is positive, batch <= 4096, head_dim
- * a multiple of 16 up to 256, page 16, 32, 64 or 128.  workspace: caller-owned device memory of
- * enigma_sdpa_quantized_workspace_bytes() bytes, 256-byte aligned. */
+ * a multiple of 16 up to 256, page 16, 32, 64 or 128; batch * table_width * page / 16 fits in int32.
+ * workspace: caller-owned device memory of enigma_sdpa_quantized_workspace_bytes() bytes, 256-byte
+ * aligned. */
 typedef struct enigma_sdpa_quantized_desc {
   int64_t batch, heads_q, heads_kv, head_dim, page, pages, table_width, n_slots;
   int64_t q_batch, q_head, o_batch, o_head, k_page, v_page, ks_page, vs_page;

@@ -189,6 +189,8 @@ def test_cache_refuses(calls):  # noqa: F811
                                             out_v=rows)),
             (ValueError, lambda: cache.attend(0, _on_one(3, 4, 64))),              # more than rows
             (ValueError, lambda: cache.attend(0, _on_one(2, 4, 32))),
+            (ValueError, lambda: cache.attend(1, _on_one(2, 4, 64))),
+            (ValueError, lambda: cache.attend(-1, _on_one(2, 4, 64))),
             (ValueError, lambda: cache.attend(0, _on_one(2, 3, 64))),
             (TypeError, lambda: cache.attend(0, _on_one(2, 4, 64, dtype=torch.float16))),
             (ValueError, lambda: cache.attend(0, _on_one(2, 4, 64), out=_on_one(2, 4, 32))),
@@ -254,7 +256,7 @@ def test_c_cache_refuses():
     assert lib.enigma_kv_cache_fork(ctypes.byref(c), 64, 64, 0, None) == bad
     assert lib.enigma_kv_cache_compact(ctypes.byref(c), None) == bad
     assert lib.enigma_kv_cache_copy_pages(ctypes.byref(c), 64, 64, 0, None) == bad
-    for d in (None, desc(scale=0), desc(scale=66), desc(code=2), desc(elem_bytes=2), desc(page=48),
+    for d in (None, desc(scale=0), desc(scale=66), desc(code=2), desc(elem_bytes=2), desc(page=48), desc(heads_kv=65536),
               desc(head_dim=24), desc(head_dim=512), desc(k=72), desc(v=0), desc(workspace_bytes=8)):
         assert lib.enigma_kv_cache_q8_compact(d, None) == bad
         assert lib.enigma_kv_cache_q8_fork(d, 64, 64, 0, None) == bad
@@ -306,6 +308,11 @@ def test_c_attend_refuses():
         for x in values:
             d = _Attend(**{**good, key: x})
             assert lib.enigma_sdpa_quantized(ctypes.byref(d), None) == bad, (key, x)
+    many = dict(batch=4096, n_slots=1 << 20)                             # chunks past 32 bits
+    for kw in (dict(many, table_width=1 << 25), dict(many, table_width=1 << 18, heads_q=60000, heads_kv=60000,
+                                                     pages=1, page=16)):
+        d = _Attend(**{**good, **kw})
+        assert lib.enigma_sdpa_quantized(ctypes.byref(d), None) == bad, kw
     d = _Attend(**{**good, "slots": 0, "batch": 3})                      # more sequences than rows
     assert lib.enigma_sdpa_quantized(ctypes.byref(d), None) == bad
 
