@@ -3,13 +3,22 @@
 //   out = sum_j softmax_j(c s_k(j) q . k_j) s_v(j) v_j  over the sequence's first len keys.
 //
 // Bound by memory: a key costs 2 D bytes and a few scales, read once for all query heads of its kv
-// head.  The work is the flattened list of (unit, chunk of KEYS keys), unit = (sequence, kv head, up to
-// 8 NT of its query heads); warp w of W takes the contiguous range [w n, (w + 1) n), n = ceil(T / W), so
-// every SM streams as much, whatever the lengths are.  Each warp has a ring of its own in shared memory
-// that it fills with cp.async (16 bytes a lane) and empties by itself: no barrier until the end, and
-// nothing to wait for but its own copies.  A unit that lies within one warp's range is finished
-// there.  The others leave pieces (maximum, sum, unnormalised O): the block joins its warps' pieces
-// after its only barrier, and what goes past a block's ends is joined by join_codes8_kernel.
+// head.  The work is the flattened list of T entries, a unit's start and its chunks of KEYS keys, unit =
+// (sequence, kv head, up to H of its query heads); warp w of W takes the contiguous range
+// [w T / W, (w + 1) T / W), so every SM streams as much, whatever the lengths are.  Each warp has a ring
+// of its own in shared memory that it fills with cp.async (16 bytes a lane) and empties by itself: no
+// barrier until the end, and nothing to wait for but its own copies.  A unit that lies within one
+// warp's range is finished there.  The others leave pieces (maximum, sum, unnormalised O): the block
+// joins its warps' pieces after its only barrier, and what goes past a block's ends is joined by
+// join_codes8_kernel.
+// Measured, replayed from a graph: 192 contexts of 500 to 8000 keys, 8 kv heads of 128, bf16: 272 us, 6.2
+// TB/s of codes and scales.  16 of 1 to 8191 keys: 35.4 us, 3.8 TB/s, of which the keys take 20; the rest
+// is the launches (2 us), the ranges (2), the joins in the blocks (3) and behind them (3), and the
+// first chunk's way.  64 of 2049 keys, 2 heads of 64: 11.1 us.  One of 131071, fp32: 56 us, 4.8 TB/s, bound by
+// instructions: each product is made twice, P's exponentials and splits are as many as in bf16.
+// The matrix instructions are the warp's, not the SM's asynchronous ones: a decode step has one to 16
+// rows a key, and what counts is that codes go from their copy to an operand without another pass
+// through shared memory.
 //
 // Both products are m16n8k16 with fp16 operands and fp32 sums, which hold every code exactly; keys
 // or the head's elements are the 16-row side, the query heads (8) the narrow one:
@@ -23,10 +32,12 @@
 // that follows the running maximum once a score passes it by 4, and v0 the largest |s_v|, followed
 // once another passes it fourfold: P < 2^15, so most chunks change no reference, need no maximum
 // over the lanes and rescale nothing.  Rounding P to fp16 costs 2^-11 of the weight, or 2^-34 of a weight
-// of one.  fp32: queries and P are two fp16 numbers each (2^-22); a chunk's P is relative to its own
-// largest score and s_v, times 2^15, and what brings it to the running maximum is applied to the
-// chunk's product in fp32, so that small weights keep theirs whatever came before (2^-40 of the
-// chunk's largest).  Queries are brought to [2^11, 2^12) by a power of two per head.
+// of one.  fp32: queries and P are two fp16 numbers each (2^-22), for up to 4 heads in columns beside each
+// other, so that one product serves both (one context of 131071: 56 us, 65 with two products); a
+// chunk's P is relative to its own largest score and s_v, times 2^15, and what brings it to the running
+// maximum is applied to the chunk's product in fp32, so that small weights keep theirs whatever came
+// before (2^-40 of the chunk's largest).  Queries are brought to [2^11, 2^12) by a power of two per
+// head.
 #include <algorithm>
 #include <atomic>
 
@@ -39,14 +50,17 @@ using namespace enigma_codes8;
 using namespace enigma_sm100;
 
 // The work list's unit starts count as STARTS chunks: loading its queries and writing its result takes
-// a warp about as long.  Each warp of a block gets at least LEAST entries, if the list has as many for
-// one block: so a block has a chunk or more, and a unit's pieces are in consecutive blocks.
+// a warp about as long.  A block gets LEAST entries or more, if the list has as many: so it has a chunk,
+// and a unit's pieces are in consecutive blocks.
 constexpr int STARTS = 1;
-constexpr int LEAST = 3;
+constexpr int LEAST = 2;
 
-template <typename T, int DT, int NT>
+template <typename T, int DT, int H>
 struct Cfg {
-  // As many warps as their registers leave room for: O, queries and a chunk's operands.
+  static constexpr int NT = (H + 7) / 8;                  // tiles of 8 columns
+  // As many warps as their registers leave room for: O, queries and a chunk's operands.  12 against 8:
+  // 192 long contexts of heads of 128 272 us, 281; 16 ragged ones 35.4, 38; fp32 heads of 64, 32 x 4096
+  // keys, 37, 40.  Two tiles of heads of 128 need 8: 42 us (64 x 4096 keys, 2 kv heads), 57 with 10.
   static constexpr int WARPS = NT == 1 && DT < 256 || DT * NT <= 128 ? 12 : 8;
   static constexpr int THREADS = WARPS * 32;
   static constexpr int SLOTS = WARPS + 2;                // pieces of a block in the workspace: its warps'
@@ -58,9 +72,9 @@ struct Cfg {
   static constexpr int STAGES = (192 << 10) / (WARPS * 2 * TILE);
   static constexpr int RING = STAGES * 2 * TILE;          // of a warp
   static constexpr int TILES = DT / 16;                   // 16-element tiles of O
-  static constexpr int HEADS = 8 * NT;
+  static constexpr int HEADS = H, COLS = 8 * NT;
   static constexpr int PIECE = (TILES * NT * 4) * 32;     // floats of O in fragment order
-  static constexpr int SLOT = PIECE + 2 * HEADS;          // and maxima and sums
+  static constexpr int SLOT = PIECE + 2 * COLS;           // and maxima and sums
 };
 
 struct Attend {
@@ -233,18 +247,19 @@ __device__ __forceinline__ T* out_row(const Attend& a, int b, int u, int head) {
 // What a block's warps left, in order: a warp's first piece, its last.
 template <typename C>
 struct Pieces {
-  alignas(16) float2 ml[2 * C::WARPS][C::HEADS];          // maximum, sum
+  alignas(16) float2 ml[2 * C::WARPS][C::COLS];           // maximum, sum
   int unit[2 * C::WARPS], ends[2 * C::WARPS];            // -1: none; 1: has its unit's first key, 2: the last
   int2 at[2 * C::WARPS];                                  // sequence, and unit of the sequence
 };
 
-// T: of queries and results; DT: the head's elements, rounded up; NT: tiles of 8 query heads.
-template <typename T, bool E4M3, int DT, int NT>
-__global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kernel(const __grid_constant__ Attend a) {
-  using C = Cfg<T, DT, NT>;
-  constexpr bool SPLIT = sizeof(T) == 4;
-  constexpr int MT = C::MT, KEYS = C::KEYS, WARPS = C::WARPS, THREADS = C::THREADS;
-  constexpr int PARTS = SPLIT ? 4 : 2;   // registers of an operand: two halves of the inner index
+// T: of queries and results; DT: the head's elements, rounded up; H: query heads of a unit.
+template <typename T, bool E4M3, int DT, int H>
+__global__ void __launch_bounds__(Cfg<T, DT, H>::THREADS, 1) attend_codes8_kernel(const __grid_constant__ Attend a) {
+  using C = Cfg<T, DT, H>;
+  constexpr bool SPLIT = sizeof(T) == 4, BESIDE = H == 4;
+  static_assert(!BESIDE || SPLIT);
+  constexpr int MT = C::MT, NT = C::NT, KEYS = C::KEYS, WARPS = C::WARPS, THREADS = C::THREADS;
+  constexpr int PARTS = SPLIT && !BESIDE ? 4 : 2;            // registers of an operand: two halves of the inner index
   extern __shared__ __align__(128) uint8_t smem[];       // rings, list entries before each b, last chunks
   __shared__ __align__(16) float s_scale[WARPS][C::STAGES][2 * MT];
   __shared__ Pieces<C> s_pieces;
@@ -315,7 +330,7 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
     if (tid == 0) s_starts[a.batch] = run;
     __syncthreads();
     total = int64_t(run) * per_b;
-    used = max(int64_t(1), min(int64_t(gridDim.x), quotient(total, LEAST * WARPS)));
+    used = max(int64_t(1), min(int64_t(gridDim.x), quotient(total, LEAST)));
     const uint32_t w = blockIdx.x * WARPS + warp, of = uint32_t(used) * WARPS;
     const int64_t each = quotient(total, of);
     const uint32_t more = uint32_t(total - each * of);       // (below of: grids are small)
@@ -427,13 +442,14 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
     const int heads = heads_of(p);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const T* row = query_row(p, nt * 8 + g);
+      const int head = BESIDE ? g & 3 : nt * 8 + g;
+      const T* row = query_row(p, head);
       float x[DT / 64][16];
       uint32_t top = 0;
 #pragma unroll
       for (int jj = 0; jj < DT / 64; ++jj) {
         const int e = 64 * jj + 16 * t;
-        const bool there = nt * 8 + g < heads && e < a.d;
+        const bool there = head < heads && e < a.d;
         if (a.q_vec) {
 #pragma unroll
           for (int i = 0; i < int(sizeof(T)); ++i) {         // 16 elements: 2 or 4 times 16 bytes
@@ -471,8 +487,10 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float lo = x[jj][4 * s + 2 * i] * up, hi = x[jj][4 * s + 2 * i + 1] * up;
-            if (SPLIT) qf[nt][4 * jj + s][i] = split_halves(lo, hi, &qf[nt][4 * jj + s][(2 + i) % PARTS]);
-            else qf[nt][4 * jj + s][i] = pack_halves(lo, hi);
+            uint32_t rest;
+            qf[nt][4 * jj + s][i] = SPLIT ? split_halves(lo, hi, &rest) : pack_halves(lo, hi);
+            if (BESIDE && g >= 4) qf[nt][4 * jj + s][i] = rest;
+            if (PARTS == 4) qf[nt][4 * jj + s][(2 + i) % PARTS] = rest;
           }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -510,7 +528,7 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
           for (int nt = 0; nt < NT; ++nt) {
             if (jj + z == 0) mma_f16_first(s[i][nt], f, qf[nt][0][0], qf[nt][0][1]);
             else mma_f16(s[i][nt], f, qf[nt][4 * jj + z][0], qf[nt][4 * jj + z][1]);
-            if (SPLIT) mma_f16(s[i][nt], f, qf[nt][4 * jj + z][2 % PARTS], qf[nt][4 * jj + z][3 % PARTS]);
+            if (PARTS == 4) mma_f16(s[i][nt], f, qf[nt][4 * jj + z][2 % PARTS], qf[nt][4 * jj + z][3 % PARTS]);
           }
         }
       }
@@ -549,7 +567,10 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
       for (int i = 0; i < MT; ++i) {
         const float c[2] = {sc[i] * cq[nt][0], sc[i] * cq[nt][1]};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) s[i][nt][x] *= c[x & 1];
+        for (int x = 0; x < 4; ++x) {
+          if (BESIDE) s[i][nt][x] += __shfl_xor_sync(0xffffffffu, s[i][nt][x], 2);
+          s[i][nt][x] *= c[x & 1];
+        }
       }
     if ((p.j + 1) * KEYS > p.len) {                          // some keys do not count
 #pragma unroll
@@ -601,11 +622,14 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
             sum[x & 1] += w[x];
             w[x] *= ratio[i];
           }
-          uint32_t r0, r1;
-          pf[i][nt][0] = turn_8x8(split_halves(w[0], w[1], &r0));
-          pf[i][nt][1] = turn_8x8(split_halves(w[2], w[3], &r1));
-          pf[i][nt][2 % PARTS] = turn_8x8(r0);
-          pf[i][nt][3 % PARTS] = turn_8x8(r1);
+          uint32_t r0, r1, h0 = split_halves(w[0], w[1], &r0), h1 = split_halves(w[2], w[3], &r1);
+          if (BESIDE && t >= 2) h0 = r0, h1 = r1;
+          pf[i][nt][0] = turn_8x8(h0);
+          pf[i][nt][1] = turn_8x8(h1);
+          if (PARTS == 4) {
+            pf[i][nt][2 % PARTS] = turn_8x8(r0);
+            pf[i][nt][3 % PARTS] = turn_8x8(r1);
+          }
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -687,7 +711,7 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
             }
             if (i == 0) mma_f16_first(acc[nt], f, pf[i][nt][0], pf[i][nt][1]);
             else mma_f16(acc[nt], f, pf[i][nt][0], pf[i][nt][1]);
-            mma_f16(acc[nt], f, pf[i][nt][2 % PARTS], pf[i][nt][3 % PARTS]);
+            if (PARTS == 4) mma_f16(acc[nt], f, pf[i][nt][2 % PARTS], pf[i][nt][3 % PARTS]);
           }
         }
         if (SPLIT)
@@ -737,6 +761,11 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int y = 0; y < 2; ++y) l[nt][y] = sum_over_keys(l[nt][y]);
+        if (BESIDE)                      // both parts of P
+#pragma unroll
+          for (int mt = 0; mt < C::TILES; ++mt)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) o[mt][0][y] += __shfl_xor_sync(0xffffffffu, o[mt][0][y], 2);
         const float unit = SPLIT ? 1.f : v0 * (1.f / 512.f);
         if (began && end) {              // all of the unit
           const int heads = heads_of(at), hb = at.u % a.blocks * C::HEADS;
@@ -856,7 +885,7 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
         const int hb = u % a.blocks * C::HEADS, e = element_of<DT>(mt, g);
 #pragma unroll
         for (int y = 0; y < 2; ++y)
-          if (hb + h0 + y < a.group && e < a.d) {
+          if (h0 + y < C::HEADS && hb + h0 + y < a.group && e < a.d) {
             const float f = sum[y] == 0.f ? 0.f : 1.f / sum[y];
             store_pair(out_row<T>(a, b, u, hb + h0 + y) + e, acc[y] * f, acc[2 + y] * f, a.o_vec);
           }
@@ -882,10 +911,10 @@ __global__ void __launch_bounds__(Cfg<T, DT, NT>::THREADS, 1) attend_codes8_kern
 
 // Block (c, x): tile x of O of the unit that began in block c and went on behind it.  Its warps take
 // every eighth part, then the block joins the warps.
-template <typename T, int DT, int NT>
+template <typename T, int DT, int H>
 __global__ void __launch_bounds__(256) join_codes8_kernel(const Attend a) {
-  using C = Cfg<T, DT, NT>;
-  constexpr int WARPS = 8;
+  using C = Cfg<T, DT, H>;
+  constexpr int WARPS = 8, NT = C::NT;
   __shared__ float s_o[WARPS][4][32], s_m[WARPS][8], s_l[WARPS][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int mt = int(blockIdx.y) / NT, nt = int(blockIdx.y) % NT, h0 = nt * 8 + 2 * t;
@@ -949,51 +978,62 @@ __global__ void __launch_bounds__(256) join_codes8_kernel(const Attend a) {
   }
   const int per_b = a.heads_kv * a.blocks, b = link.x / per_b, u = link.x - b * per_b;
   const int head = u % a.blocks * C::HEADS + h0 + y, e = element_of<DT>(mt, g);
-  if (head < a.group && e < a.d)
+  if (h0 + y < C::HEADS && head < a.group && e < a.d)
     store_pair(out_row<T>(a, b, u, head) + e, sum == 0.f ? 0.f : e0 / sum, sum == 0.f ? 0.f : e1 / sum,
                a.o_vec);
 }
 
-// Tiles of 8 query heads that a unit takes: two for groups of more than 8, where their registers
-// fit (fp32 queries and heads of 256 have as much in one).
-int tiles_of(const enigma_sdpa_quantized_desc& d) {
-  return d.heads_q / d.heads_kv > 8 && d.head_dim <= 128 && d.dtype == ENIGMA_DTYPE_BF16 ? 2 : 1;
+// Query heads that a unit takes.  16 where the group is larger than 8, so that codes are read and
+// converted once for two tiles (64 x 4096 keys, 2 kv heads for 32: of 128 42 us against 49, of 64 23
+// against 29), but where registers have no room for them: heads of 256, and fp32.  4 in fp32 where the
+// group is no larger: both parts of a query and of P in one tile (one context of 131071: 56 us, 65).
+int unit_heads(const enigma_sdpa_quantized_desc& d) {
+  const int64_t group = d.heads_q / d.heads_kv;
+  if (d.dtype == ENIGMA_DTYPE_F32) return group > 4 ? 8 : 4;
+  return group > 8 && d.head_dim <= 128 ? 16 : 8;
 }
 
 int64_t units_of(const enigma_sdpa_quantized_desc& d) {
-  const int64_t heads = 8 * tiles_of(d), group = d.heads_q / d.heads_kv;
+  const int64_t heads = unit_heads(d), group = d.heads_q / d.heads_kv;
   return d.batch * d.heads_kv * ((group + heads - 1) / heads);
 }
 
-// A block per unit, or the even split and a join.
+// A block per unit, or the even split and a join.  The host knows the table's width, not the lengths: a
+// block per unit, which saves the ranges and the joins, where the longest unit there may be is
+// small, the larger the fewer SMs it leaves idle.  us, heads of 128, all of the longest length or
+// of 1 to it:
+//   8 units (heads of 64) of 128 KB: 7.8, 7.6 (split 8.6, 8.6); 256 KB: 10.2, 10.2 (9.0, 9.0)
+//   64 of 256 KB: 11.7, 11.3 (13.3, 11.3);           512 KB: 17.2, 16.6 (15.8, 13.7)
+//   128 of 512 KB: 18.0, 17.0 (21.7, 17.6);          1 MB: 30.1, 27.2 (33.8, 23.6)
 bool whole(const enigma_sdpa_quantized_desc& d) {
   const int64_t sms = enigma::sm_count(), units = units_of(d);
   const int64_t bytes = 2 * d.head_dim * d.page * d.table_width;         // of the longest unit there may be
-  return units <= sms && bytes * (sms - units) / sms <= (110 << 10);
+  return units <= sms && bytes * (5 * sms - 4 * units) / (5 * sms) <= (170 << 10);
 }
 
-size_t slot_floats(const enigma_sdpa_quantized_desc& d) {
-  const size_t dt = d.head_dim <= 64 ? 64 : d.head_dim <= 128 ? 128 : 256, heads = 8 * tiles_of(d);
-  return heads * dt + 2 * heads;
+// Floats of the workspace that a block's pieces take.
+template <typename T, int H>
+size_t block_floats(const enigma_sdpa_quantized_desc& d) {
+  if (d.head_dim <= 64) return size_t(Cfg<T, 64, H>::SLOTS) * Cfg<T, 64, H>::SLOT;
+  if constexpr (H <= 8)
+    if (d.head_dim > 128) return size_t(Cfg<T, 256, H>::SLOTS) * Cfg<T, 256, H>::SLOT;
+  return size_t(Cfg<T, 128, H>::SLOTS) * Cfg<T, 128, H>::SLOT;
+}
+size_t block_floats(const enigma_sdpa_quantized_desc& d) {
+  const int heads = unit_heads(d);
+  if (d.dtype == ENIGMA_DTYPE_F32) return heads == 4 ? block_floats<float, 4>(d) : block_floats<float, 8>(d);
+  return heads == 16 ? block_floats<__nv_bfloat16, 16>(d) : block_floats<__nv_bfloat16, 8>(d);
 }
 
-template <typename T>
-size_t slots_of(const enigma_sdpa_quantized_desc& d) {
-  if (d.head_dim > 128) return Cfg<T, 256, 1>::SLOTS;
-  if constexpr (sizeof(T) == 2)
-    if (tiles_of(d) == 2) return d.head_dim > 64 ? Cfg<T, 128, 2>::SLOTS : Cfg<T, 64, 2>::SLOTS;
-  return d.head_dim > 64 ? Cfg<T, 128, 1>::SLOTS : Cfg<T, 64, 1>::SLOTS;
-}
-
-template <typename T, bool E4M3, int DT, int NT>
+template <typename T, bool E4M3, int DT, int H>
 cudaError_t launch(const enigma_sdpa_quantized_desc& d, Attend a, cudaStream_t s) {
-  using C = Cfg<T, DT, NT>;
+  using C = Cfg<T, DT, H>;
   a.blocks = (a.group + C::HEADS - 1) / C::HEADS;
   a.whole = whole(d) ? 1 : 0;
   a.fast = a.d == DT;
   const int sms = enigma::sm_count();
   const size_t smem = size_t(C::WARPS) * C::RING + (a.whole ? 0 : size_t(d.batch) * 5 + 4);
-  auto* kernel = attend_codes8_kernel<T, E4M3, DT, NT>;
+  auto* kernel = attend_codes8_kernel<T, E4M3, DT, H>;
   static std::atomic<uint64_t> ready{0};                     // devices where the attribute is set
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -1008,17 +1048,25 @@ cudaError_t launch(const enigma_sdpa_quantized_desc& d, Attend a, cudaStream_t s
   const unsigned grid = a.whole ? unsigned(units_of(d)) : unsigned(sms);
   e = enigma::launch_dependent(kernel, grid, C::THREADS, smem, s, a);
   if (e != cudaSuccess || a.whole) return e;
-  return enigma::launch_dependent(join_codes8_kernel<T, DT, NT>, dim3(grid, C::TILES * NT), 256, 0, s,
+  return enigma::launch_dependent(join_codes8_kernel<T, DT, H>, dim3(grid, C::TILES * C::NT), 256, 0, s,
                                   a);
 }
 
-template <typename T, bool E4M3>
+template <typename T, bool E4M3, int H>
 cudaError_t launch_sizes(const enigma_sdpa_quantized_desc& d, const Attend& a, cudaStream_t s) {
-  if (d.head_dim > 128) return launch<T, E4M3, 256, 1>(d, a, s);
-  if (sizeof(T) == 2 && tiles_of(d) == 2)
-    return d.head_dim > 64 ? launch<__nv_bfloat16, E4M3, 128, 2>(d, a, s)
-                           : launch<__nv_bfloat16, E4M3, 64, 2>(d, a, s);
-  return d.head_dim > 64 ? launch<T, E4M3, 128, 1>(d, a, s) : launch<T, E4M3, 64, 1>(d, a, s);
+  if (d.head_dim <= 64) return launch<T, E4M3, 64, H>(d, a, s);
+  if constexpr (H <= 8)
+    if (d.head_dim > 128) return launch<T, E4M3, 256, H>(d, a, s);
+  return launch<T, E4M3, 128, H>(d, a, s);
+}
+
+template <bool E4M3>
+cudaError_t launch_heads(const enigma_sdpa_quantized_desc& d, const Attend& a, cudaStream_t s) {
+  const int heads = unit_heads(d);
+  if (d.dtype == ENIGMA_DTYPE_F32)
+    return heads == 4 ? launch_sizes<float, E4M3, 4>(d, a, s) : launch_sizes<float, E4M3, 8>(d, a, s);
+  return heads == 16 ? launch_sizes<__nv_bfloat16, E4M3, 16>(d, a, s)
+                     : launch_sizes<__nv_bfloat16, E4M3, 8>(d, a, s);
 }
 
 }  // namespace
@@ -1028,8 +1076,7 @@ namespace enigma {
 size_t sdpa_quantized_workspace(const enigma_sdpa_quantized_desc& d) {
   if (d.batch == 0 || whole(d)) return 0;
   const size_t sms = size_t(sm_count());
-  const size_t slots = d.dtype == ENIGMA_DTYPE_F32 ? slots_of<float>(d) : slots_of<__nv_bfloat16>(d);
-  return ((sms * 2 + 63) / 64 * 64 + sms * slots * slot_floats(d)) * sizeof(float);
+  return ((sms * 2 + 63) / 64 * 64 + sms * block_floats(d)) * sizeof(float);
 }
 
 cudaError_t sdpa_quantized_launch(const enigma_sdpa_quantized_desc& d, cudaStream_t s) {
@@ -1067,8 +1114,7 @@ cudaError_t sdpa_quantized_launch(const enigma_sdpa_quantized_desc& d, cudaStrea
             d.q_head * es % 16 == 0;
   a.o_vec = reinterpret_cast<uintptr_t>(d.out) % 16 == 0 && d.o_batch * es % 16 == 0 &&
             d.o_head * es % 16 == 0;
-  if (f32) return e4m3 ? launch_sizes<float, true>(d, a, s) : launch_sizes<float, false>(d, a, s);
-  return e4m3 ? launch_sizes<__nv_bfloat16, true>(d, a, s) : launch_sizes<__nv_bfloat16, false>(d, a, s);
+  return e4m3 ? launch_heads<true>(d, a, s) : launch_heads<false>(d, a, s);
 }
 
 }  // namespace enigma
