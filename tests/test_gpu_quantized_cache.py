@@ -390,6 +390,36 @@ def test_attend_long(cuda, heads_q, heads_kv, d, lens, dtype, code):
     _hold(got, ref, max(lens), dtype)
 
 
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("heads_q,heads_kv,d,lens", [
+    (4, 1, 64, [700, 33]), (6, 3, 256, [600, 5, 0]), (1, 1, 80, [1, 900]), (3, 1, 128, [50, 64]),
+    (8, 2, 256, [17, 2]), (9, 1, 64, [300]), (12, 1, 128, [1000, 1])])
+def test_attend_few_heads(cuda, heads_q, heads_kv, d, lens, code):
+    """Groups that fill no tile of heads, in short and wide tables, by themselves and among others."""
+    rng = np.random.default_rng(heads_q + d)
+    pages = sum(-(-n // 32) for n in lens) + 1
+    for dtype in ("bf16", "f32"):
+        for width in (-(-max(lens) // 32), 800):
+            cache, want = _make(cuda, rng, 1, pages, heads_kv, 32, d, len(lens), width, lens, code)
+            got, ref = _attend(cuda, rng, cache, want, heads_q, dtype)
+            _hold(got, ref, max(lens), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("heads_q,heads_kv,d", [(14, 2, 64), (8, 4, 128), (4, 1, 256)])
+def test_attend_little_work(cuda, dtype, heads_q, heads_kv, d):
+    """Fewer chunks than the GPU has warps, or hardly more: units that end and begin anywhere in a
+    block's share, in tables wide enough for far more."""
+    rng = np.random.default_rng(d)
+    for n in (1, 2, 5, 17, 60, 149, 400):
+        lens = [int(x) for x in rng.integers(0, 200, n) * (rng.random(n) < 0.8)]
+        lens[-1] = 1 + n
+        cache, want = _make(cuda, rng, 1, sum(-(-x // 16) for x in lens), heads_kv, 16, d, n, 2000, lens,
+                            "int8")
+        got, ref = _attend(cuda, rng, cache, want, heads_q, dtype)
+        _hold(got, ref, max(lens), dtype)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_attend_large_batches(cuda, dtype):
     """More sequences than SMs, most of a few keys; and the same slot named many times."""
