@@ -4,9 +4,12 @@ The prompts, of different lengths, run packed through every layer once (`sdpa_pa
 keys and values go into a paged cache (`PagedKVCache.reserve`, `write`). Each prompt is forked into
 its samples, which share its pages; every new token is one row per sample, and a prompt's samples
 read the prompt's keys once for all (`attend`). At the end the samples are freed and the pages
-that prompts still hold move together (`free`, `compact`).
+that prompts still hold move together (`free`, `compact`). Queries and keys are turned to their
+positions in place (`rope`). With --codes the cache holds 8-bit codes (`QuantizedKVCache`): half the
+size, and every sample reads the prompt for itself.
 
     python examples/parallel_sampling.py --prompts 3 --samples 8 --tokens 32
+    python examples/parallel_sampling.py --codes int8
 """
 from __future__ import annotations
 
@@ -19,7 +22,7 @@ from pathlib import Path
 sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "enigma-dsl_b200"))
 
 from enigma import cuda_ops  # noqa: E402
-from enigma.kv_cache import PagedKVCache  # noqa: E402
+from enigma.kv_cache import PagedKVCache, QuantizedKVCache  # noqa: E402
 
 
 @dataclass
@@ -64,16 +67,8 @@ class Decoder:
         inv = cfg.rope_theta ** (-torch.arange(half, device=self.device, dtype=torch.float64)
                                  * 2.0 / cfg.head_dim)
         angle = torch.arange(cfg.max_len, device=self.device, dtype=torch.float64)[:, None] * inv
-        self.cos, self.sin = angle.cos().float(), angle.sin().float()
-
-    def rotate(self, x, positions):
-        """Rotary positions on [tokens, heads, head_dim], in place (a view of the projection)."""
-        half = self.cfg.head_dim // 2
-        cos, sin = self.cos[positions][:, None], self.sin[positions][:, None]
-        a, b = x[..., :half].float(), x[..., half:].float()
-        x[..., :half] = (a * cos - b * sin).to(x.dtype)
-        x[..., half:] = (b * cos + a * sin).to(x.dtype)
-        return x
+        self.cos, self.sin = angle.cos().float(), angle.sin().float()    # what `rope` turns by
+        self.rope = cuda_ops.RopeTable(cfg.head_dim, theta=cfg.rope_theta, device=self.device)
 
     def forward(self, tokens, positions, attention, last=None):
         """Logits (fp32) of the rows `last`, or of all; attention(layer, q, k, v) -> o."""
@@ -84,7 +79,8 @@ class Decoder:
             qkv = cuda_ops.gemm(cuda_ops.rmsnorm(x, w["norm"], cfg.eps), w["qkv"])
             q, k, v = qkv.view(len(x), -1, cfg.head_dim).split(
                 [cfg.heads_q, cfg.heads_kv, cfg.heads_kv], dim=1)
-            o = attention(i, self.rotate(q, positions), self.rotate(k, positions), v)
+            cuda_ops.rope(q, k, positions, self.rope, out_q=q, out_k=k)  # views of the projection
+            o = attention(i, q, k, v)
             x = x + cuda_ops.gemm(o.reshape(len(x), -1), w["o"])
             up = cuda_ops.gemm(cuda_ops.rmsnorm(x, w["post"], cfg.eps), w["gate_up"])
             gate, up = up.chunk(2, dim=1)
@@ -98,20 +94,21 @@ class Decoder:
 
 class Sampler:
     """Prompts and their samples over one cache: slot p is prompt p, then prompt by prompt its
-    samples."""
+    samples.  codes: None for a bf16 cache, or the type of an 8-bit one (torch.int8,
+    torch.float8_e4m3fn)."""
 
-    def __init__(self, model: Decoder, prompts, samples: int, new_tokens: int):
+    def __init__(self, model: Decoder, prompts, samples: int, new_tokens: int, codes=None):
         import torch
         cfg = model.cfg
-        self.model, self.samples = model, samples
+        self.model, self.samples, self.codes = model, samples, codes
         self.lens = [len(p) for p in prompts]
         n = len(prompts)
         longest = max(self.lens) + new_tokens
         # A sample's own pages: a copy of the prompt's last, and room for its new tokens.
         pages = sum(-(-x // cfg.page) for x in self.lens) + n * samples * (-(-new_tokens // cfg.page) + 1)
-        self.cache = PagedKVCache.empty(cfg.layers, pages, cfg.page, cfg.heads_kv, cfg.head_dim,
-                                        slots=n * (1 + samples), max_len=longest,
-                                        device=model.device)
+        kind, more = (PagedKVCache, {}) if codes is None else (QuantizedKVCache, dict(dtype=codes))
+        self.cache = kind.empty(cfg.layers, pages, cfg.page, cfg.heads_kv, cfg.head_dim,
+                                slots=n * (1 + samples), max_len=longest, device=model.device, **more)
         self.tokens = torch.cat([torch.as_tensor(p, device=model.device) for p in prompts])
         self.sample_slots = torch.arange(n, n * (1 + samples), dtype=torch.int32,
                                          device=model.device)
@@ -149,6 +146,8 @@ class Sampler:
 
         def attention(layer, q, k, v):
             cache.write(layer, k, v, slots, starts, cu)
+            if self.codes is not None:
+                return cache.attend(layer, q, slots=slots)
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
             for p, prompt_len in enumerate(self.lens):
                 mine = slice(p * self.samples, (p + 1) * self.samples)
@@ -173,13 +172,15 @@ def main(argv=None):
     ap.add_argument("--samples", type=int, default=8)
     ap.add_argument("--tokens", type=int, default=32, help="new tokens per sample")
     ap.add_argument("--temperature", type=float, default=1.0)
+    ap.add_argument("--codes", choices=["int8", "e4m3"], help="an 8-bit cache of these codes")
     args = ap.parse_args(argv)
+    codes = {None: None, "int8": torch.int8, "e4m3": torch.float8_e4m3fn}[args.codes]
     cfg = Config()
     model = Decoder(cfg)
     gen = torch.Generator(device="cuda").manual_seed(1)
     prompts = [torch.randint(0, cfg.vocab, (300 + 611 * p,), generator=gen, device="cuda")
                for p in range(args.prompts)]
-    run = Sampler(model, prompts, args.samples, args.tokens)
+    run = Sampler(model, prompts, args.samples, args.tokens, codes)
     logits = run.prefill().repeat_interleave(args.samples, dim=0)
     out = []
     torch.cuda.synchronize()
