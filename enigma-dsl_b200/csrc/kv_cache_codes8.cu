@@ -219,19 +219,34 @@ constexpr int WWARPS = 8;
 // Blocks (c, y): the parts that begin in packed rows [16 c, 16 c + 16), WWARPS gridDim.y warps over their
 // (part, K or V, head) triples.  A part begins with its entry, or on a block's first token.  Bound
 // by memory for prompts; the request's look-ups, five loads that wait for one another, are made
-// once for 16 rows, a lane each, and hidden by the other blocks of the SM.
+// once for 16 rows, a lane each, and hidden by the other blocks of the SM.  8 heads of 128, bf16, replayed:
+// 32768 tokens 42 us (4.8 TB/s of rows and codes), 8192 12.7; 256 single tokens 6.2 us, nearly all of it
+// the look-ups.  4096 single tokens take 24 us, 20 without the look for clashes, which every block
+// makes among all entries (47 where each slot was compared with each part).
 template <typename T, bool E4M3, bool VEC, int NV>
 __global__ void __launch_bounds__(WWARPS * 32, (NV <= 8 ? 32 : NV == 16 ? 16 : 8) / WWARPS) write_codes8_kernel(const __grid_constant__ Write w) {
   __shared__ Part s_part[kScaleBlock];
-  __shared__ uint32_t s_found;
+  __shared__ uint32_t s_found, s_twice;                    // parts there are, parts that another entry changes
+  __shared__ uint32_t s_own;                               // entries (the block's first, ...) that clash with no part
+  __shared__ int s_first;                                  // the block's first entry
   __shared__ int s_few;                                    // no part has more than 32 vectors
+  __shared__ __align__(16) uint32_t s_slots[128];          // bit s % 4096: slot s may be a part's
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t0 = int(blockIdx.x) * kScaleBlock;
   const Rows& r = w.r;
   const int page = 1 << r.page_shift, per_page = page / kScaleBlock;
   griddep_launch_dependents();
   griddep_wait();
+  constexpr int AHEAD = 4;               // entries' slots that a thread loads at once, at first while
+  int slots[AHEAD];                      // the parts are looked up
+  auto load_slots = [&](int j) {         // (an entry past the last is the last again)
+#pragma unroll
+    for (int y = 0; y < AHEAD; ++y) slots[y] = r.slots[min(j + y * WWARPS * 32, r.n - 1)];
+  };
+  if (r.n > 1) load_slots(threadIdx.x);
   if (warp == 0) {
     const int x = lane % kScaleBlock, t = t0 + x;
+    reinterpret_cast<uint4*>(s_slots)[lane] = make_uint4(0, 0, 0, 0);
+    __syncwarp();
     const Entry e = entries_of(r, t0);
     int fail = 0;
     Part p;
@@ -258,10 +273,25 @@ __global__ void __launch_bounds__(WWARPS * 32, (NV <= 8 ? 32 : NV == 16 ? 16 : 8
       if (fail != 0) atomicOr(w.status, fail);
     }
     const uint32_t all = __ballot_sync(0xffffffffu, found);
-    if (found) s_part[__popc(all & ((1u << lane) - 1u))] = p;
+    if (found) {
+      s_part[__popc(all & ((1u << lane) - 1u))] = p;
+      if (r.n > 1) atomicOr(&s_slots[p.slot >> 5 & 127], 1u << (p.slot & 31));
+    }
+    // Parts of one slot are of one entry as a rule, which clashes with none of them then.
+    const int e0 = __shfl_sync(0xffffffffu, e.index, 0);
+    uint32_t own = 0;
+    if (r.n > 1) {
+      const uint32_t by_slot = __match_any_sync(0xffffffffu, found ? p.slot : -1 - lane);
+      const uint32_t by_entry = __match_any_sync(0xffffffffu, found ? p.entry : -1 - lane);
+      own = __reduce_or_sync(0xffffffffu, found && by_slot == by_entry && p.entry - e0 < 32
+                                              ? 1u << (p.entry - e0) : 0u);
+    }
     const bool few = __all_sync(0xffffffffu, !found || p.rows * r.d <= 32 * kVec<T>);
     if (lane == 0) {
       s_found = (1u << __popc(all)) - 1u;
+      s_twice = 0;
+      s_own = own;
+      s_first = e0;
       s_few = few;
     }
   }
@@ -269,21 +299,28 @@ __global__ void __launch_bounds__(WWARPS * 32, (NV <= 8 ? 32 : NV == 16 ? 16 : 8
   const int parts = __popc(s_found);
   // Another entry of the same slot that touches the block would change it at the same time.
   if (r.n > 1) {
-    __syncthreads();
-    for (int j = threadIdx.x; j < r.n; j += WWARPS * 32) {
-      const int slot = r.slots[j];
-      for (int x = 0; x < parts; ++x)
-        if (s_part[x].slot == slot && s_part[x].entry != j) {
-          const int64_t s = r.starts[j], e = s + r.cu[j + 1] - int64_t(r.cu[j]);
-          if (s < e && s < s_part[x].first + kScaleBlock && e > s_part[x].first) {
-            atomicAnd(&s_found, ~(1u << x));
-            atomicOr(w.status, ENIGMA_CACHE_BAD_REQUEST);
+    for (int j0 = threadIdx.x; j0 < r.n;) {
+#pragma unroll
+      for (int y = 0; y < AHEAD; ++y) {
+        const int j = j0 + y * WWARPS * 32, slot = slots[y];
+        if (j >= r.n || !(s_slots[slot >> 5 & 127] >> (slot & 31) & 1)) continue;
+        if (uint32_t(j - s_first) < 32 && (s_own >> (j - s_first) & 1)) continue;
+#pragma unroll 1
+        for (int x = 0; x < parts; ++x)
+          if (s_part[x].slot == slot && s_part[x].entry != j) {
+            const int64_t s = r.starts[j], e = s + r.cu[j + 1] - int64_t(r.cu[j]);
+            if (s < e && s < s_part[x].first + kScaleBlock && e > s_part[x].first) {
+              atomicOr(&s_twice, 1u << x);
+              atomicOr(w.status, ENIGMA_CACHE_BAD_REQUEST);
+            }
           }
-        }
+      }
+      j0 += AHEAD * WWARPS * 32;
+      if (j0 < r.n) load_slots(j0);
     }
     __syncthreads();
   }
-  const uint32_t found = s_found;
+  const uint32_t found = s_found & ~s_twice;
   const int units = parts * 2 * r.heads;
   auto block_of = [&](int u) {
     Block<T> b;
@@ -326,8 +363,9 @@ struct Read {
 };
 
 // A block has 16 packed rows: their look-ups as above, then a warp per row, its lanes along the heads,
-// READ vectors at once.  Rows before the first entry and behind the last are left as they were, a
-// token that the slot does not hold is zeros.
+// READ vectors of K and of V at once.  Rows before the first entry and behind the last are left as they
+// were, a token that the slot does not hold is zeros.  Bound by memory: 32768 tokens of 8 heads of 128,
+// bf16, 36 us (5.5 TB/s of codes and rows), 8192 9.1; 256 single tokens 5.3 us, the look-ups.
 constexpr int READ = 4;
 template <typename T, bool E4M3, bool VEC>
 __global__ void __launch_bounds__(256) read_codes8_kernel(const __grid_constant__ Read w) {

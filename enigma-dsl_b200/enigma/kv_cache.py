@@ -356,8 +356,9 @@ class QuantizedKVCache(PagedKVCache):
                     raise ValueError("read: tokens must be given where cu is on the device")
                 tokens = int(cu[-1]) if len(cu) else 0
             dtype = torch.bfloat16 if dtype is None else dtype
-            out_k, out_v = torch.empty((2, int(tokens), *self._row), dtype=dtype,
-                                       device=self.k.device).unbind()
+            device = self.k.device
+            out_k = torch.empty(int(tokens), *self._row, dtype=dtype, device=device)
+            out_v = torch.empty(int(tokens), *self._row, dtype=dtype, device=device)
         elif tokens not in (None, out_k.shape[0]) or dtype not in (None, out_k.dtype):
             raise ValueError("read: out_k and out_v have another size or type")
         self._rows_call("read", "enigma_kv_cache_q8_read", layer, out_k, out_v, slots, starts, cu)

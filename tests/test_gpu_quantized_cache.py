@@ -249,6 +249,48 @@ def test_many_entries(cuda):
     np.testing.assert_array_equal(_np(v), ref[1])
 
 
+@pytest.mark.parametrize("n,near", [(40, True), (300, True), (2500, False), (9000, True)])
+def test_entries_that_clash(cuda, n, near):
+    """Among many entries some name a block that another does, next to it or far away, before or behind:
+    neither is written.  Slots that differ by a multiple of a power of two, the same slot in another
+    block, and entries without rows clash with nobody."""
+    from enigma import EnigmaError
+    rng = np.random.default_rng(n)
+    total = 9000
+    cache, want = _make(cuda, rng, 1, total * 2 + 3, 1, 16, 16, total, 2, [20] * total, "int8")
+    slots = rng.permutation(total)[:n] if n < total else np.arange(total)
+    slots[:8] = [5 + 1024 * i for i in range(8)] if n < total else slots[:8]
+    slots[8:] = [s if s not in slots[:8] else 9 for s in slots[8:]] if n < total else slots[8:]
+    starts, lens = rng.integers(0, 12, n), rng.integers(0, 4, n)
+    lens[:8] = 1
+    for _ in range(max(3, n // 50)):
+        i = int(rng.integers(0, n))
+        j = min(n - 1, i + int(rng.integers(1, 12))) if near else int(rng.integers(0, n))
+        slots[j] = slots[i]
+        starts[j] = rng.integers(0, 30)                     # the same block, the next, or across their border
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    x, t = _written(cuda, rng, int(cu[-1]), 1, 16)
+    blocks = [[(slots[i], b) for b in range(starts[i] // 16, (starts[i] + lens[i] - 1) // 16 + 1)]
+              if lens[i] else [] for i in range(n)]
+    count = {}
+    for bs in blocks:
+        for b in bs:
+            count[b] = count.get(b, 0) + 1
+    clash = any(c > 1 for c in count.values())
+    cache.write(0, t, t, slots, starts, cu)
+    for i in range(n):                                      # block by block: the others of an entry are met
+        for s, b in blocks[i]:
+            if count[s, b] == 1:
+                lo, hi = max(starts[i], 16 * b), min(starts[i] + lens[i], 16 * b + 16)
+                rows = x[cu[i] + lo - starts[i]:cu[i] + hi - starts[i]]
+                want.write(0, rows, rows, [s], [lo], [0, hi - lo])
+    if clash:
+        with pytest.raises(EnigmaError, match="twice"):
+            cache.check()
+    cache.check()
+    _same(cache, want)
+
+
 @pytest.mark.parametrize("code", CODES)
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("layers,pages,heads,page,d", SHAPES)
