@@ -368,16 +368,14 @@ class QuantizedKVCache(PagedKVCache):
                workspace=None):
         """cuda_ops.sdpa_quantized over one layer of this cache."""
         slots = None if slots is None else self._ints("attend", slots)
-        head, need, steps = self._checked(
+        head, need, pages = self._checked(
             (layer, (q.shape, q.stride(), q.dtype), None if slots is None else slots.shape,
              None if out is None else (out.shape, out.stride(), out.dtype), scale), self._attend_head)
-        pages = [x.data_ptr() + step for x, step in zip(
-            (self.k, self.v, self.k_scale, self.v_scale, self.table, self.lens), steps)]
         return cuda_ops._sdpa_quantized(self._index, head, need, pages, q, slots, out, workspace)
 
     def _attend_head(self, layer, q, slots, out, scale):
-        """Checks the (shape, stride, dtype) of an attend; the desc's head, bytes of workspace, and where
-        in the cache's tensors the layer begins."""
+        """Checks the (shape, stride, dtype) of an attend; the desc's head, bytes of workspace, and the
+        addresses of the layer's pages, scales, the table and the lengths."""
         if not 0 <= layer < self.layers:
             raise ValueError(f"attend: layer {layer} of {self.layers}")
         pools = (self.k, self.v, self.k_scale, self.v_scale)
@@ -386,4 +384,5 @@ class QuantizedKVCache(PagedKVCache):
         head, need = cuda_ops._quantized_head(
             self._index, q, *described, None if slots is None else (slots, (1,), self.table.dtype),
             out, scale)
-        return head, need, [layer * x.stride(0) * x.element_size() for x in pools] + [0, 0]
+        return head, need, (*(x.data_ptr() + layer * x.stride(0) * x.element_size() for x in pools),
+                            self.table.data_ptr(), self.lens.data_ptr())
