@@ -228,8 +228,8 @@ constexpr int WWARPS = 8;
 // (part, K or V, head) triples.  A part begins with its entry, or on a block's first token.  Bound
 // by memory for prompts; the request's look-ups, five loads that wait for one another, are made
 // once for 16 rows, a lane each, and hidden by the other blocks of the SM.  8 heads of 128, bf16, replayed:
-// 32768 tokens 42 us (4.8 TB/s of rows and codes), 8192 12.5; 256 single tokens 6.3 us, nearly all of it
-// the look-ups.  4096 single tokens take 24 us, 20 without the look for clashes, which every block
+// 32768 tokens 40 us (5.0 TB/s of rows and codes), 8192 12.4; 256 single tokens 6.3 us, nearly all of it
+// the look-ups.  4096 single tokens take 23 us, 19 without the look for clashes, which every block
 // makes among all entries (47 where each slot was compared with each part).
 // A block's rows of more than 8 vectors a lane are shared by P warps: their registers then leave room for as
 // many warps as those of shorter rows (5448 fp32 tokens of 8 heads of 256: 23 us, 38 with a warp
@@ -244,6 +244,7 @@ __global__ void __launch_bounds__(WWARPS * 32, 32 / WWARPS) write_codes8_kernel(
   __shared__ uint32_t s_tops[2][WWARPS];
   __shared__ __align__(16) uint32_t s_slots[128];          // bit s % 4096: slot s may be a part's
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t0 = int(blockIdx.x) * kScaleBlock;
+  const int threads = int(blockDim.x), warps = threads >> 5;
   const Rows& r = w.r;
   const int page = 1 << r.page_shift, per_page = page / kScaleBlock;
   griddep_launch_dependents();
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(WWARPS * 32, 32 / WWARPS) write_codes8_kernel(
   int slots[AHEAD];                      // the parts are looked up
   auto load_slots = [&](int j) {         // (an entry past the last is the last again)
 #pragma unroll
-    for (int y = 0; y < AHEAD; ++y) slots[y] = r.slots[min(j + y * WWARPS * 32, r.n - 1)];
+    for (int y = 0; y < AHEAD; ++y) slots[y] = r.slots[min(j + y * threads, r.n - 1)];
   };
   if (r.n > 1) load_slots(threadIdx.x);
   if (warp == 0) {
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(WWARPS * 32, 32 / WWARPS) write_codes8_kernel(
     for (int j0 = threadIdx.x; j0 < r.n;) {
 #pragma unroll
       for (int y = 0; y < AHEAD; ++y) {
-        const int j = j0 + y * WWARPS * 32, slot = slots[y];
+        const int j = j0 + y * threads, slot = slots[y];
         if (j >= r.n || !(s_slots[slot >> 5 & 127] >> (slot & 31) & 1)) continue;
         if (uint32_t(j - s_first) < 32 && (s_own >> (j - s_first) & 1)) continue;
 #pragma unroll 1
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(WWARPS * 32, 32 / WWARPS) write_codes8_kernel(
             }
           }
       }
-      j0 += AHEAD * WWARPS * 32;
+      j0 += AHEAD * threads;
       if (j0 < r.n) load_slots(j0);
     }
     __syncthreads();
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(WWARPS * 32, 32 / WWARPS) write_codes8_kernel(
     return b;
   };
   if (units == 0) return;
-  const int stride = WWARPS * int(gridDim.y), u0 = int(blockIdx.y) * WWARPS + warp;
+  const int stride = warps * int(gridDim.y), u0 = int(blockIdx.y) * warps + warp;
   if (s_few == 1) {                      // single tokens: four blocks at once, a vector a lane
     for (int u = u0; u < units; u += 4 * stride) {
       const Block<T> b[4] = {block_of(u), block_of(u + stride), block_of(u + 2 * stride),
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(WWARPS * 32, 32 / WWARPS) write_codes8_kernel(
     }
   } else {
     int turn = 0;
-    for (int u = u0 / P; u < units; u += stride / P) {       // (P divides WWARPS)
+    for (int u = u0 / P; u < units; u += stride / P) {       // (P divides `warps`)
       const Block<T> b[1] = {block_of(u)};
       write_blocks<T, E4M3, VEC, NV, 1, P>(b, r.d, warp % P, &s_tops[turn][warp / P * P]);
       if (b[0].n > 0) turn ^= 1;         // (where the warps met)
@@ -386,7 +387,7 @@ struct Read {
 // were, a token that the slot does not hold is zeros.  Bound by memory: 32768 tokens of 8 heads of 128,
 // bf16, 36 us (5.6 TB/s of codes and rows), 8192 9.0; 256 single tokens 4.5 us, the look-ups.
 template <typename T, bool E4M3, bool VEC, int READ>
-__global__ void __launch_bounds__(256) read_codes8_kernel(const __grid_constant__ Read w) {
+__global__ void __launch_bounds__(WWARPS * 32) read_codes8_kernel(const __grid_constant__ Read w) {
   constexpr int E = kVec<T>;
   __shared__ int64_t s_line[kScaleBlock];                  // of the first head: page * heads * page size + row
   __shared__ int s_kind[kScaleBlock];                      // 0: no row, 1: zeros, 2: a token
@@ -419,7 +420,7 @@ __global__ void __launch_bounds__(256) read_codes8_kernel(const __grid_constant_
   const int cols = r.d / E, items = r.heads * cols, step_h = 32 / cols, step_c = 32 - step_h * cols;
   const int h_first = lane / cols, c_first = lane - h_first * cols;
   const int pieces = (items + 32 * READ - 1) / (32 * READ) * kScaleBlock;          // of all rows: K and V together
-  for (int i = int(blockIdx.y) * 8 + warp; i < pieces; i += 8 * int(gridDim.y)) {
+  for (int i = int(blockIdx.y) * WWARPS + warp; i < pieces; i += WWARPS * int(gridDim.y)) {
     const int x = i % kScaleBlock, kind = s_kind[x];
     if (kind == 0) continue;
     const int t = t0 + x;
@@ -517,23 +518,40 @@ Rows rows_of(const enigma_kv_cache_desc& c, const enigma_kv_cache_rows& w) {
   return r;
 }
 
+// Blocks that share a column, 16 packed rows whose look-ups each of them makes: one where the columns alone
+// fill the GPU with `per_sm` blocks an SM, else as many as fill it, or twice as many where a warp
+// still has two of the column's `tasks` then; never more than have one of at most `most`, nor more than
+// eight whose warps then have four or less.  (8192 tokens, 8 heads of 128, written: 12.3 us with one, 12.5 with
+// two; 4096: 10.4, 8.0, four 8.4; 8192 tokens of 32 heads read: 42, 38; 5448 fp32 tokens of 8 heads of
+// 256 written: 32, 27, three 24; 64 single tokens of 2 heads of 64: 7.3, 5.8, eight 5.0; 256 of 8 of 128: 18,
+// 11, eight 6.4, 32 7.1.)
+dim3 shared(int64_t columns, int64_t per_sm, int64_t tasks, int64_t most) {
+  const int64_t fill = enigma::sm_count() * per_sm / columns;
+  const int64_t twice = std::min(tasks / (2 * WWARPS), enigma::sm_count() * per_sm * 2 / columns);
+  const int64_t enough = std::min(most / WWARPS, std::max<int64_t>(8, most / (4 * WWARPS)));
+  const int64_t share = std::max<int64_t>(1, std::max(std::min(enough, fill), twice));
+  return dim3(unsigned(columns), unsigned(std::min<int64_t>(share, 65535)));
+}
+
 template <typename T, bool E4M3, bool VEC>
 cudaError_t launch_write(const Write& w, cudaStream_t s) {
   const int vectors = w.r.d * int(sizeof(T)) / 32;         // of a lane, if a warp has all of 16 new rows
   const int warps = vectors <= 8 ? 1 : vectors <= 16 ? 2 : 4;
   const int64_t columns = (int64_t(w.r.tokens) + kScaleBlock - 1) / kScaleBlock;
-  // Blocks that share a column's parts: one where the columns fill the GPU with 32 warps an SM (8192 tokens
-  // of 2 heads of 64 4.7 us, 5.9 in twice as many blocks); where they do not, as many as leave each
-  // warp four (part, K or V, head) if every row is a part.
-  const int64_t most = (int64_t(kScaleBlock) * 2 * w.r.heads * warps + 4 * WWARPS - 1) / (4 * WWARPS);
-  const int64_t share = std::max<int64_t>(1, std::min(most, enigma::sm_count() * 32 / WWARPS / columns));
-  const dim3 grid{unsigned(columns), unsigned(std::min<int64_t>(share, 65535))};
+  // (Part, K or V, head) triples of a column: where it is one part, and where the entries are as short as they
+  // may be and begin anywhere.
+  const int64_t units = int64_t(2) * w.r.heads * warps;
+  const int64_t parts = w.r.n == 1 ? 1 : std::min<int64_t>(kScaleBlock, 2 + w.r.n / columns);
+  const dim3 grid = shared(columns, 4, units, units * parts);
+  // Long requests take blocks of 4 warps, of which fewer wait for the look-ups: 32768 tokens of 2 heads of 64
+  // 8.8 us, 12.9 with 8, of 8 heads of 128 40, 42; but 12000 21 against 17.
+  const unsigned threads = columns > enigma::sm_count() * 12 ? 128 : 256;
   auto* kernel = vectors <= 4 ? write_codes8_kernel<T, E4M3, VEC, 4, 1>
                  : warps == 1 ? write_codes8_kernel<T, E4M3, VEC, 8, 1>
                               : write_codes8_kernel<T, E4M3, VEC, 8, 2>;
   if constexpr (sizeof(T) == 4)
     if (warps == 4) kernel = write_codes8_kernel<T, E4M3, VEC, 8, 4>;
-  return enigma::launch_dependent(kernel, grid, WWARPS * 32, 0, s, w);
+  return enigma::launch_dependent(kernel, grid, threads, 0, s, w);
 }
 
 template <typename T, bool E4M3, bool VEC>
@@ -549,12 +567,8 @@ cudaError_t launch_read(const Read& w, cudaStream_t s) {
       kernel = read_codes8_kernel<T, E4M3, VEC, 8>;
       at_once = 8;
     }
-  // Blocks that share 16 rows: one where those fill the GPU, else up to one for 8 pieces (64 fp32 rows of 8
-  // heads of 256: 4.8 us, 9.0 in blocks of 16 rows).
-  const int64_t most = 2 * ((items + 32 * at_once - 1) / (32 * at_once));
-  const int64_t share = std::max<int64_t>(1, std::min(most, (at_once == 1 ? 8 : 4) * enigma::sm_count() / columns));
-  return enigma::launch_dependent(kernel, dim3(unsigned(columns), unsigned(std::min<int64_t>(share, 65535))), 256, 0,
-                                  s, w);
+  const int64_t pieces = kScaleBlock * ((items + 32 * at_once - 1) / (32 * at_once));
+  return enigma::launch_dependent(kernel, shared(columns, at_once == 1 ? 8 : 4, pieces, pieces), 256, 0, s, w);
 }
 
 // The scales as pages of one row per head, which move with their codes.
