@@ -40,6 +40,7 @@
 // head.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "attn_serving.cuh"
 #include "codes8.cuh"
@@ -66,7 +67,9 @@ struct Cfg {
   static constexpr int SLOTS = WARPS + 2;                // pieces of a block in the workspace: its warps'
   static constexpr int BEFORE = WARPS;                   // first ones, what it has of a unit that began
   static constexpr int AFTER = WARPS + 1;                // in another block, and of one that goes on
-  static constexpr int KEYS = 4096 / DT;                  // of a chunk: 4 KB of K, as much of V
+  static constexpr int MAIN = DT < 128 ? 64 : DT;         // elements of a row's first part, and pieces of
+  static constexpr int TAILS = (DT - MAIN) / 16;          // 16 behind it, which tiles hold apart
+  static constexpr int KEYS = TAILS ? 32 : 4096 / DT;     // of a chunk: up to 4 KB of K, as much of V
   static constexpr int MT = KEYS / 16;                    // 16-key tiles, scale blocks
   static constexpr int TILE = KEYS * DT;                  // bytes of K or V
   static constexpr int STAGES = (192 << 10) / (WARPS * 2 * TILE);
@@ -122,6 +125,16 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
   return v;
 }
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+  return v;
+}
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
@@ -174,7 +187,7 @@ __device__ __forceinline__ float sum_over_keys(float x) {
 // 0 where nothing was seen, so that no difference of infinities is taken.
 __device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.f : top; }
 
-// Where chunk c (16 bytes) of row r is in a tile.  Eight lanes that load at once must find eight
+// Where chunk c (16 bytes) of row r is in a tile (of its first part: DT is MAIN here).  Eight lanes that load at once must find eight
 // different 16-byte columns of a 128-byte line: of K, lanes of two neighbouring rows and four
 // neighbouring chunks; of V, of two neighbouring chunks and every second of eight rows.
 template <int DT>
@@ -221,20 +234,20 @@ __device__ __forceinline__ void store_pair(T* p, float x, float y, bool vec) {
   }
 }
 
-// N copies of 16 bytes a lane, STEP bytes apart in memory and, but for the swizzle's form, in the tile.
-template <int N, int FORMS, int STEP, int Y = 0>
+// N copies of 16 bytes a lane, STEP bytes apart in memory and, but for the swizzle's form, INTO in the tile.
+template <int N, int FORMS, int STEP, int INTO, int Y = 0>
 __device__ __forceinline__ void copy_rows(const uint32_t (&to)[FORMS], uint32_t plus, const uint8_t* from) {
   if constexpr (Y < N) {
-    constexpr int TO = Y / FORMS * FORMS * STEP;
+    constexpr int TO = Y / FORMS * FORMS * INTO;
     cp_async16_at<TO, Y * STEP>(to[Y % FORMS] + plus, from);
-    copy_rows<N, FORMS, STEP, Y + 1>(to, plus, from);
+    copy_rows<N, FORMS, STEP, INTO, Y + 1>(to, plus, from);
   }
 }
 
 // First element of O's tile m that lane (g, t) has, in rows g and g + 8: e and e + 1.
 template <int DT>
 __device__ __forceinline__ int element_of(int m, int g) {
-  if (DT == 64) return 8 * g + 2 * m;
+  if (DT < 128) return m < 4 ? 8 * g + 2 * m : 16 * m + 2 * g;
   return DT == 128 || m < 8 ? 16 * g + 2 * m : 128 + 16 * g + 2 * (m - 8);
 }
 
@@ -258,6 +271,7 @@ __global__ void __launch_bounds__(Cfg<T, DT, H>::THREADS, 1) attend_codes8_kerne
   using C = Cfg<T, DT, H>;
   constexpr bool SPLIT = sizeof(T) == 4, BESIDE = H == 4;
   static_assert(!BESIDE || SPLIT);
+  constexpr int MAIN = C::MAIN, TAILS = C::TAILS, TAIL = C::KEYS * 16;   // (bytes of a tail in a tile)
   constexpr int MT = C::MT, NT = C::NT, KEYS = C::KEYS, WARPS = C::WARPS, THREADS = C::THREADS;
   constexpr int PARTS = SPLIT && !BESIDE ? 4 : 2;            // registers of an operand: two halves of the inner index
   extern __shared__ __align__(128) uint8_t smem[];       // rings, list entries before each b, last chunks
@@ -381,15 +395,17 @@ __global__ void __launch_bounds__(Cfg<T, DT, H>::THREADS, 1) attend_codes8_kerne
   // copies go to places that differ by constants, but for the swizzle, which takes two forms.
   const int page_mask = (1 << a.page_shift) - 1, parts = (page_mask + 1) / kScaleBlock;
   const int chunks = a.d >> 4;           // 16-byte chunks of a row
-  constexpr int PER = DT / 16, ROWS = 32 / PER;              // of a row; rows that the lanes copy at once
+  constexpr int PER = MAIN / 16, ROWS = 32 / PER;              // of a row; rows that the lanes copy at once
   constexpr int FORMS = ROWS == 8 ? 1 : 8 / ROWS;            // the swizzles take the rows' low three bits
   const int lane_r = lane / PER, lane_c = lane % PER;
   uint32_t k_to[FORMS], v_to[FORMS];
 #pragma unroll
   for (int y = 0; y < FORMS; ++y) {
-    k_to[y] = ring_at + k_at<DT>(y * ROWS + lane_r, lane_c);
-    v_to[y] = ring_at + C::TILE + v_at<DT>(y * ROWS + lane_r, lane_c);
+    k_to[y] = ring_at + k_at<MAIN>(y * ROWS + lane_r, lane_c);
+    v_to[y] = ring_at + C::TILE + v_at<MAIN>(y * ROWS + lane_r, lane_c);
   }
+  const int lane_from = lane_r * DT + lane_c * 16;
+  const uint32_t tail_to = ring_at + KEYS * MAIN + lane * 16;
   auto issue = [&](const Place& p, int stage) {
     const int kvh = p.u / a.blocks, key0 = p.j * KEYS, live = p.len - key0;
     const uint32_t to = stage * 2 * C::TILE;
@@ -401,15 +417,26 @@ __global__ void __launch_bounds__(Cfg<T, DT, H>::THREADS, 1) attend_codes8_kerne
       const int in_page = (key0 + from0) & page_mask;
       const int64_t at = (int64_t(kvh) * (page_mask + 1) + in_page) * a.d;
       if (a.fast && one && has && here >= KEYS) {
-        const uint8_t* k = a.k + page * a.k_page + at + lane * 16;
-        const uint8_t* v = a.v + page * a.v_page + at + lane * 16;
-        copy_rows<KEYS / ROWS, FORMS, ROWS * DT>(k_to, to, k);
-        copy_rows<KEYS / ROWS, FORMS, ROWS * DT>(v_to, to, v);
+        const uint8_t* k = a.k + page * a.k_page + at;
+        const uint8_t* v = a.v + page * a.v_page + at;
+        copy_rows<KEYS / ROWS, FORMS, ROWS * DT, ROWS * MAIN>(k_to, to, k + lane_from);
+        copy_rows<KEYS / ROWS, FORMS, ROWS * DT, ROWS * MAIN>(v_to, to, v + lane_from);
+#pragma unroll
+        for (int c = 0; c < TAILS; ++c) {                    // (chunks of 32 keys: a lane a row)
+          cp_async16(tail_to + to + c * TAIL, k + lane * DT + MAIN + 16 * c, 16);
+          cp_async16(tail_to + to + C::TILE + c * TAIL, v + lane * DT + MAIN + 16 * c, 16);
+        }
       } else if (a.fast && has && here >= n) {
-        const uint8_t* k = a.k + page * a.k_page + at + lane * 16;
-        const uint8_t* v = a.v + page * a.v_page + at + lane * 16;
-        copy_rows<16 / ROWS, FORMS, ROWS * DT>(k_to, to + from0 * DT, k);
-        copy_rows<16 / ROWS, FORMS, ROWS * DT>(v_to, to + from0 * DT, v);
+        const uint8_t* k = a.k + page * a.k_page + at;
+        const uint8_t* v = a.v + page * a.v_page + at;
+        copy_rows<16 / ROWS, FORMS, ROWS * DT, ROWS * MAIN>(k_to, to + from0 * MAIN, k + lane_from);
+        copy_rows<16 / ROWS, FORMS, ROWS * DT, ROWS * MAIN>(v_to, to + from0 * MAIN, v + lane_from);
+        if (TAILS && lane < 16)
+#pragma unroll
+          for (int c = 0; c < TAILS; ++c) {
+            cp_async16(tail_to + to + from0 * 16 + c * TAIL, k + lane * DT + MAIN + 16 * c, 16);
+            cp_async16(tail_to + to + from0 * 16 + C::TILE + c * TAIL, v + lane * DT + MAIN + 16 * c, 16);
+          }
       } else {
         const uint8_t* k = a.k + (has ? page * a.k_page + at : 0);
         const uint8_t* v = a.v + (has ? page * a.v_page + at : 0);
@@ -418,10 +445,18 @@ __global__ void __launch_bounds__(Cfg<T, DT, H>::THREADS, 1) attend_codes8_kerne
           const uint32_t bytes = has && r < here ? 16 : 0;
           const int64_t from = bytes ? int64_t(r) * a.d + lane_c * 16 : 0;
           if (lane_c < chunks) {
-            cp_async16(ring_at + to + k_at<DT>(from0 + r, lane_c), k + from, bytes);
-            cp_async16(ring_at + to + C::TILE + v_at<DT>(from0 + r, lane_c), v + from, bytes);
+            cp_async16(ring_at + to + k_at<MAIN>(from0 + r, lane_c), k + from, bytes);
+            cp_async16(ring_at + to + C::TILE + v_at<MAIN>(from0 + r, lane_c), v + from, bytes);
           }
         }
+        if (TAILS && lane < n)
+#pragma unroll
+          for (int c = 0; c < TAILS; ++c) {                  // (n is at most 32 here)
+            const uint32_t bytes = has && lane < here ? 16 : 0;
+            const int from = bytes ? lane * DT + MAIN + 16 * c : 0;
+            cp_async16(tail_to + to + from0 * 16 + c * TAIL, k + from, bytes);
+            cp_async16(tail_to + to + from0 * 16 + C::TILE + c * TAIL, v + from, bytes);
+          }
       }
       const int x = lane % MT;
       if (lane < 2 * MT && (one || x == i)) {
@@ -444,10 +479,10 @@ __global__ void __launch_bounds__(Cfg<T, DT, H>::THREADS, 1) attend_codes8_kerne
     for (int nt = 0; nt < NT; ++nt) {
       const int head = BESIDE ? g & 3 : nt * 8 + g;
       const T* row = query_row(p, head);
-      float x[DT / 64][16];
+      float x[MAIN / 64][16], tail[TAILS + 1][4];
       uint32_t top = 0;
 #pragma unroll
-      for (int jj = 0; jj < DT / 64; ++jj) {
+      for (int jj = 0; jj < MAIN / 64; ++jj) {
         const int e = 64 * jj + 16 * t;
         const bool there = head < heads && e < a.d;
         if (a.q_vec) {
@@ -473,6 +508,13 @@ __global__ void __launch_bounds__(Cfg<T, DT, H>::THREADS, 1) attend_codes8_kerne
 #pragma unroll
         for (int y = 0; y < 16; ++y) top = max(top, __float_as_uint(x[jj][y]) & 0x7fffffffu);
       }
+#pragma unroll
+      for (int c = 0; c < TAILS; ++c)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          tail[c][y] = head < heads ? float(row[MAIN + 16 * c + 4 * t + y]) : 0.f;
+          top = max(top, __float_as_uint(tail[c][y]) & 0x7fffffffu);
+        }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int e = max(27, int(top >> 23));                 // biased; 2^-100 at least
@@ -480,18 +522,21 @@ __global__ void __launch_bounds__(Cfg<T, DT, H>::THREADS, 1) attend_codes8_kerne
       const float back = __uint_as_float(uint32_t(max(e - 11, 1)) << 23) * a.scale_log2;
 #pragma unroll
       for (int i = 0; i < 2; ++i) cq[nt][i] = __shfl_sync(0xffffffffu, back, (2 * t + i) * 4);
+      auto pack = [&](int k16, int i, float lo, float hi) {
+        uint32_t rest;
+        qf[nt][k16][i] = SPLIT ? split_halves(lo * up, hi * up, &rest) : pack_halves(lo * up, hi * up);
+        if (BESIDE && g >= 4) qf[nt][k16][i] = rest;
+        if (PARTS == 4) qf[nt][k16][(2 + i) % PARTS] = rest;
+      };
 #pragma unroll
-      for (int jj = 0; jj < DT / 64; ++jj)
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
+        for (int jj = 0; jj < MAIN / 64; ++jj)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float lo = x[jj][4 * s + 2 * i] * up, hi = x[jj][4 * s + 2 * i + 1] * up;
-            uint32_t rest;
-            qf[nt][4 * jj + s][i] = SPLIT ? split_halves(lo, hi, &rest) : pack_halves(lo, hi);
-            if (BESIDE && g >= 4) qf[nt][4 * jj + s][i] = rest;
-            if (PARTS == 4) qf[nt][4 * jj + s][(2 + i) % PARTS] = rest;
-          }
+          for (int s = 0; s < 4; ++s) pack(4 * jj + s, i, x[jj][4 * s + 2 * i], x[jj][4 * s + 2 * i + 1]);
+#pragma unroll
+        for (int c = 0; c < TAILS; ++c) pack(MAIN / 16 + c, i, tail[c][2 * i], tail[c][2 * i + 1]);
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         m[nt][i] = -INFINITY;
@@ -511,50 +556,63 @@ __global__ void __launch_bounds__(Cfg<T, DT, H>::THREADS, 1) attend_codes8_kerne
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) sc[i] = s_scale[warp][stage][i];
     float s[MT][NT][4];
+    // 16 elements of tile i's keys, words x of key g and y of key g + 8.
+    auto add_scores = [&](int i, int k16, uint32_t x, uint32_t y) {
+      uint32_t f[4];
+      halves_of4<E4M3>(x, &f[0], &f[2]);
+      halves_of4<E4M3>(y, &f[1], &f[3]);
 #pragma unroll
-    for (int jj = 0; jj < DT / 64; ++jj) {
+      for (int nt = 0; nt < NT; ++nt) {
+        if (k16 == 0) mma_f16_first(s[i][nt], f, qf[nt][0][0], qf[nt][0][1]);
+        else mma_f16(s[i][nt], f, qf[nt][k16][0], qf[nt][k16][1]);
+        if (PARTS == 4) mma_f16(s[i][nt], f, qf[nt][k16][2 % PARTS], qf[nt][k16][3 % PARTS]);
+      }
+    };
+#pragma unroll
+    for (int jj = 0; jj < MAIN / 64; ++jj) {
       if (64 * jj >= a.d) break;
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const uint4 x = lds128(kd + k_at<DT>(16 * i + g, 4 * jj + t));
-        const uint4 y = lds128(kd + k_at<DT>(16 * i + g + 8, 4 * jj + t));
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          uint32_t f[4];
-          halves_of4<E4M3>(xs[z], &f[0], &f[2]);
-          halves_of4<E4M3>(ys[z], &f[1], &f[3]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            if (jj + z == 0) mma_f16_first(s[i][nt], f, qf[nt][0][0], qf[nt][0][1]);
-            else mma_f16(s[i][nt], f, qf[nt][4 * jj + z][0], qf[nt][4 * jj + z][1]);
-            if (PARTS == 4) mma_f16(s[i][nt], f, qf[nt][4 * jj + z][2 % PARTS], qf[nt][4 * jj + z][3 % PARTS]);
-          }
-        }
+        const uint4 x = lds128(kd + k_at<MAIN>(16 * i + g, 4 * jj + t));
+        const uint4 y = lds128(kd + k_at<MAIN>(16 * i + g + 8, 4 * jj + t));
+        add_scores(i, 4 * jj, x.x, y.x);
+        add_scores(i, 4 * jj + 1, x.y, y.y);
+        add_scores(i, 4 * jj + 2, x.z, y.z);
+        add_scores(i, 4 * jj + 3, x.w, y.w);
       }
     }
+#pragma unroll
+    for (int c = 0; c < TAILS; ++c)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const uint32_t at = kd + KEYS * MAIN + c * TAIL + (16 * i + g) * 16 + 4 * t;
+        add_scores(i, MAIN / 16 + c, lds32(at), lds32(at + 8 * 16));
+      }
     // V's codes while the scores are weighed: keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of each tile.
-    constexpr int WORDS = DT / 32;
-    uint32_t vw[MT][4][WORDS];
+    constexpr int WORDS = MAIN / 32;
+    uint32_t vw[MT][4][WORDS + TAILS];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int z = 0; z < 4; ++z) {
         const int r = 16 * i + 2 * t + (z & 1) + 8 * (z >> 1);
-        if (DT == 64) {
-          const uint2 w = lds64(vd + v_at<DT>(r, g >> 1) + (g & 1) * 8);
+        if (MAIN == 64) {
+          const uint2 w = lds64(vd + v_at<MAIN>(r, g >> 1) + (g & 1) * 8);
           vw[i][z][0] = w.x;
           vw[i][z][1] = w.y;
         } else {
 #pragma unroll
-          for (int h = 0; h < DT / 128; ++h) {
-            const uint4 w = lds128(vd + v_at<DT>(r, g + 8 * h));
+          for (int h = 0; h < MAIN / 128; ++h) {
+            const uint4 w = lds128(vd + v_at<MAIN>(r, g + 8 * h));
             vw[i][z][(4 * h) % WORDS] = w.x;
             vw[i][z][(4 * h + 1) % WORDS] = w.y;
             vw[i][z][(4 * h + 2) % WORDS] = w.z;
             vw[i][z][(4 * h + 3) % WORDS] = w.w;
           }
         }
+#pragma unroll
+        for (int c = 0; c < TAILS; ++c)
+          vw[i][z][WORDS + c] = lds16(vd + KEYS * MAIN + c * TAIL + r * 16 + 2 * g);
       }
     float top_v = 0.f;
 #pragma unroll
@@ -693,34 +751,38 @@ __global__ void __launch_bounds__(Cfg<T, DT, H>::THREADS, 1) attend_codes8_kerne
         }
       }
     }
+    // A tile of O: two bytes of each key's word z.
+    auto add_tile = [&](int tile, int z, uint32_t bytes) {
+      float acc[NT][4];
 #pragma unroll
-    for (int z = 0; z < WORDS; ++z)
+      for (int i = 0; i < MT; ++i) {
+        uint32_t f[4];
+        halves_of4<E4M3>(__byte_perm(vw[i][0][z], vw[i][1][z], bytes), &f[0], &f[1]);
+        halves_of4<E4M3>(__byte_perm(vw[i][2][z], vw[i][3][z], bytes), &f[2], &f[3]);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float acc[NT][4];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          uint32_t f[4];
-          halves_of4<E4M3>(__byte_perm(vw[i][0][z], vw[i][1][z], half ? 0x7362 : 0x5140), &f[0], &f[1]);
-          halves_of4<E4M3>(__byte_perm(vw[i][2][z], vw[i][3][z], half ? 0x7362 : 0x5140), &f[2], &f[3]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            if (!SPLIT) {
-              mma_f16(o[2 * z + half][nt], f, pf[i][nt][0], pf[i][nt][1]);
-              continue;
-            }
-            if (i == 0) mma_f16_first(acc[nt], f, pf[i][nt][0], pf[i][nt][1]);
-            else mma_f16(acc[nt], f, pf[i][nt][0], pf[i][nt][1]);
-            if (PARTS == 4) mma_f16(acc[nt], f, pf[i][nt][2 % PARTS], pf[i][nt][3 % PARTS]);
+        for (int nt = 0; nt < NT; ++nt) {
+          if (!SPLIT) {
+            mma_f16(o[tile][nt], f, pf[i][nt][0], pf[i][nt][1]);
+            continue;
           }
+          if (i == 0) mma_f16_first(acc[nt], f, pf[i][nt][0], pf[i][nt][1]);
+          else mma_f16(acc[nt], f, pf[i][nt][0], pf[i][nt][1]);
+          if (PARTS == 4) mma_f16(acc[nt], f, pf[i][nt][2 % PARTS], pf[i][nt][3 % PARTS]);
         }
-        if (SPLIT)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              o[2 * z + half][nt][x] = fmaf(acc[nt][x], fresh[nt][x & 1], o[2 * z + half][nt][x]);
       }
+      if (SPLIT)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[tile][nt][x] = fmaf(acc[nt][x], fresh[nt][x & 1], o[tile][nt][x]);
+    };
+#pragma unroll
+    for (int z = 0; z < WORDS; ++z) {
+      add_tile(2 * z, z, 0x5140);
+      add_tile(2 * z + 1, z, 0x7362);
+    }
+#pragma unroll
+    for (int c = 0; c < TAILS; ++c) add_tile(2 * WORDS + c, WORDS + c, 0x5140);
   };
 
   if (in.left > 0) {
@@ -1011,18 +1073,38 @@ bool whole(const enigma_sdpa_quantized_desc& d) {
   return units <= sms && bytes * (5 * sms - 4 * units) / (5 * sms) <= (170 << 10);
 }
 
-// Floats of the workspace that a block's pieces take.
-template <typename T, int H>
-size_t block_floats(const enigma_sdpa_quantized_desc& d) {
-  if (d.head_dim <= 64) return size_t(Cfg<T, 64, H>::SLOTS) * Cfg<T, 64, H>::SLOT;
+// Calls f with the elements of a head that the kernel is made for: 80 and 96 by themselves (38 x 4096 keys, 8 heads of
+// 80: 58 us, 75 as heads of 128), others rounded up.
+template <int H, typename F>
+auto with_elements(int64_t head_dim, F f) {
+  using std::integral_constant;
+  if (head_dim <= 64) return f(integral_constant<int, 64>{});
+  if (head_dim == 80) return f(integral_constant<int, 80>{});
+  if (head_dim == 96) return f(integral_constant<int, 96>{});
   if constexpr (H <= 8)
-    if (d.head_dim > 128) return size_t(Cfg<T, 256, H>::SLOTS) * Cfg<T, 256, H>::SLOT;
-  return size_t(Cfg<T, 128, H>::SLOTS) * Cfg<T, 128, H>::SLOT;
+    if (head_dim > 128) return f(integral_constant<int, 256>{});
+  return f(integral_constant<int, 128>{});
 }
-size_t block_floats(const enigma_sdpa_quantized_desc& d) {
+
+// Calls f with the type of queries and the heads of a unit.
+template <typename F>
+auto with_heads(const enigma_sdpa_quantized_desc& d, F f) {
+  using std::integral_constant;
   const int heads = unit_heads(d);
-  if (d.dtype == ENIGMA_DTYPE_F32) return heads == 4 ? block_floats<float, 4>(d) : block_floats<float, 8>(d);
-  return heads == 16 ? block_floats<__nv_bfloat16, 16>(d) : block_floats<__nv_bfloat16, 8>(d);
+  if (d.dtype == ENIGMA_DTYPE_F32)
+    return heads == 4 ? f(0.f, integral_constant<int, 4>{}) : f(0.f, integral_constant<int, 8>{});
+  return heads == 16 ? f(__nv_bfloat16{}, integral_constant<int, 16>{})
+                     : f(__nv_bfloat16{}, integral_constant<int, 8>{});
+}
+
+// Floats of the workspace that a block's pieces take.
+size_t block_floats(const enigma_sdpa_quantized_desc& d) {
+  return with_heads(d, [&](auto type, auto heads) {
+    return with_elements<heads.value>(d.head_dim, [&](auto elements) {
+      using C = Cfg<decltype(type), elements.value, heads.value>;
+      return size_t(C::SLOTS) * C::SLOT;
+    });
+  });
 }
 
 template <typename T, bool E4M3, int DT, int H>
@@ -1052,21 +1134,13 @@ cudaError_t launch(const enigma_sdpa_quantized_desc& d, Attend a, cudaStream_t s
                                   a);
 }
 
-template <typename T, bool E4M3, int H>
-cudaError_t launch_sizes(const enigma_sdpa_quantized_desc& d, const Attend& a, cudaStream_t s) {
-  if (d.head_dim <= 64) return launch<T, E4M3, 64, H>(d, a, s);
-  if constexpr (H <= 8)
-    if (d.head_dim > 128) return launch<T, E4M3, 256, H>(d, a, s);
-  return launch<T, E4M3, 128, H>(d, a, s);
-}
-
 template <bool E4M3>
-cudaError_t launch_heads(const enigma_sdpa_quantized_desc& d, const Attend& a, cudaStream_t s) {
-  const int heads = unit_heads(d);
-  if (d.dtype == ENIGMA_DTYPE_F32)
-    return heads == 4 ? launch_sizes<float, E4M3, 4>(d, a, s) : launch_sizes<float, E4M3, 8>(d, a, s);
-  return heads == 16 ? launch_sizes<__nv_bfloat16, E4M3, 16>(d, a, s)
-                     : launch_sizes<__nv_bfloat16, E4M3, 8>(d, a, s);
+cudaError_t launch_any(const enigma_sdpa_quantized_desc& d, const Attend& a, cudaStream_t s) {
+  return with_heads(d, [&](auto type, auto heads) {
+    return with_elements<heads.value>(d.head_dim, [&](auto elements) {
+      return launch<decltype(type), E4M3, elements.value, heads.value>(d, a, s);
+    });
+  });
 }
 
 }  // namespace
@@ -1114,7 +1188,7 @@ cudaError_t sdpa_quantized_launch(const enigma_sdpa_quantized_desc& d, cudaStrea
             d.q_head * es % 16 == 0;
   a.o_vec = reinterpret_cast<uintptr_t>(d.out) % 16 == 0 && d.o_batch * es % 16 == 0 &&
             d.o_head * es % 16 == 0;
-  return e4m3 ? launch_heads<true>(d, a, s) : launch_heads<false>(d, a, s);
+  return e4m3 ? launch_any<true>(d, a, s) : launch_any<false>(d, a, s);
 }
 
 }  // namespace enigma

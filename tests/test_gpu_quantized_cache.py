@@ -447,6 +447,21 @@ def test_attend_few_heads(cuda, heads_q, heads_kv, d, lens, code):
             _hold(got, ref, max(lens), dtype)
 
 
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("heads_q,heads_kv", [(32, 2), (14, 2), (8, 2), (3, 3)])
+@pytest.mark.parametrize("d", [80, 96, 112])
+def test_attend_heads_between(cuda, d, heads_q, heads_kv, code):
+    """Heads between 64 and 128 elements: chunks that lie in a page, cross pages, end early."""
+    rng = np.random.default_rng(heads_q + d)
+    for page, lens in ((16, [1, 31, 32, 33, 100]), (64, [600, 0, 47, 2000]), (128, [9000, 5])):
+        pages = sum(-(-n // page) for n in lens) + 1
+        for dtype in ("bf16", "f32"):
+            cache, want = _make(cuda, rng, 1, pages, heads_kv, page, d, len(lens),
+                                -(-max(lens) // page) + 1, lens, code)
+            got, ref = _attend(cuda, rng, cache, want, heads_q, dtype)
+            _hold(got, ref, max(lens), dtype)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("heads_q,heads_kv,d", [(14, 2, 64), (8, 4, 128), (4, 1, 256)])
 def test_attend_little_work(cuda, dtype, heads_q, heads_kv, d):
