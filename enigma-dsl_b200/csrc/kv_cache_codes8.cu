@@ -546,9 +546,11 @@ cudaError_t launch_write(const Write& w, cudaStream_t s) {
   // Long requests take blocks of 4 warps, of which fewer wait for the look-ups: 32768 tokens of 2 heads of 64
   // 8.8 us, 12.9 with 8, of 8 heads of 128 40, 42; but 12000 21 against 17.
   const unsigned threads = columns > enigma::sm_count() * 12 ? 128 : 256;
-  auto* kernel = vectors <= 4 ? write_codes8_kernel<T, E4M3, VEC, 4, 1>
-                 : warps == 1 ? write_codes8_kernel<T, E4M3, VEC, 8, 1>
-                              : write_codes8_kernel<T, E4M3, VEC, 8, 2>;
+  auto* kernel = vectors <= 4    ? write_codes8_kernel<T, E4M3, VEC, 4, 1>
+                 : vectors == 5  ? write_codes8_kernel<T, E4M3, VEC, 5, 1>             // (heads of 80)
+                 : warps == 1    ? write_codes8_kernel<T, E4M3, VEC, 8, 1>
+                 : vectors == 10 ? write_codes8_kernel<T, E4M3, VEC, 5, 2>
+                                 : write_codes8_kernel<T, E4M3, VEC, 8, 2>;
   if constexpr (sizeof(T) == 4)
     if (warps == 4) kernel = write_codes8_kernel<T, E4M3, VEC, 8, 4>;
   return enigma::launch_dependent(kernel, grid, threads, 0, s, w);

@@ -84,14 +84,16 @@ __device__ __forceinline__ void turn_pairs(Vec<__nv_bfloat16, E>& x, Vec<__nv_bf
 
 // A warp takes a token, or the heads of one part of it where tokens are few.  It makes the angles
 // once, into shared memory; then a lane keeps one unit's (E pairs in the half layout, a vector of
-// either half; E / 2 interleaved ones; or E elements that are copied) and turns that unit of every
-// head, or of every second, third, ... where a head has less than 32 units: neighbouring lanes touch
-// neighbouring memory.  Bound by memory: BATCH heads' loads are in flight at once, the first through
-// the making of the angles.  They are straight-line code, heads past the last being the last again:
-// loads under a condition, or asked for one by one as others arrive, waited for one another (8192
-// tokens of 40 heads of 128: 42 to 83 us).
-// 5 heads (30 us at that size; 2, 3, 4: 30.5, 30.1, 31.3), or 2 where a warp has no more rounds (64 tokens of
-// 16 heads of 64: 2.7 against 2.9 us).
+// either half, or two vectors of the elements that are copied, from either half of those; interleaved
+// a vector of E / 2 pairs or of copied ones) and turns that unit of every head, or of every second,
+// third, ... where a head has less than 32 units: neighbouring lanes touch neighbouring memory.  Bound by
+// memory: 8192 tokens of 40 heads of 128, bf16, 28.1 us, 6.0 TB/s; half of each head turned 26.4 for
+// 150 MB (39.7 where copied elements had a lane for each vector).  BATCH heads' loads are in flight at
+// once, the first through the making of the angles.  They are straight-line code, heads past the last
+// being the last again: loads under a condition, or asked for one by one as others arrive, waited for
+// one another (42 to 83 us).
+// 5 heads (30 us then; 2, 3, 4: 30.5, 30.1, 31.3), or 2 where a warp has no more rounds (64 tokens of
+// 16 heads of 64: 2.5 against 2.9 us).
 constexpr int WARPS = 4;
 constexpr int ANGLE_BYTES = 48 << 10;    // of a block
 
@@ -102,7 +104,7 @@ __global__ void __launch_bounds__(WARPS * 32) rope_kernel(const __grid_constant_
   constexpr int PAIRS = TWO ? E : E / 2;
   extern __shared__ __align__(16) float2 s_angles[];
   const int pairs = r.rotary / 2, turned = pairs / PAIRS;
-  const int units = turned + (r.d - r.rotary) / E;
+  const int rest = r.d - r.rotary, units = turned + (TWO ? (rest / E + 1) / 2 : rest / E);
   const int lane = threadIdx.x & 31, warps = int(blockDim.x) >> 5;
   float2* angles = s_angles + (threadIdx.x >> 5) * ((pairs + 1) & ~1);
   const int groups = max(1, 32 / units);                 // heads at once
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(WARPS * 32) rope_kernel(const __grid_constant_
     const int u = min(u0 + lane - group * units, units - 1);
     const bool has = units <= 32 ? lane < groups * units : u0 + lane < units, turn = u < turned;
     const int e0 = !turn ? r.rotary + (u - turned) * E : HALF || !TWO ? u * E : 2 * u;
-    const int apart = !turn ? 0 : HALF ? pairs : 1;
+    const int apart = !turn ? rest / 2 : HALF ? pairs : 1;
     const T* q = static_cast<const T*>(r.q) + t * r.q_token + e0;
     const T* k = static_cast<const T*>(r.k) + t * r.k_token + e0 - r.heads_q * r.k_head;
     T* out_q = static_cast<T*>(r.out_q) + t * r.oq_token + e0;
@@ -150,7 +152,7 @@ __global__ void __launch_bounds__(WARPS * 32) rope_kernel(const __grid_constant_
         const int h = h0 + i * groups + group;
         const bool is_q = h < r.heads_q;
         T* to = (is_q ? out_q : out_k) + h * (is_q ? r.oq_head : r.ok_head);
-        const V was = x[i];
+        const V was = x[i], was_y = y[i];
         turn_pairs<E, PAIRS>(x[i], y[i], angle);
         if (!has || h >= h_hi) continue;
         if (turn) {
@@ -158,6 +160,7 @@ __global__ void __launch_bounds__(WARPS * 32) rope_kernel(const __grid_constant_
           if (TWO) *reinterpret_cast<V*>(to + apart) = y[i];
         } else if (to != (is_q ? q : k) + h * (is_q ? r.q_head : r.k_head)) {
           *reinterpret_cast<V*>(to) = was;                   // (bits that no arithmetic has seen)
+          if (TWO) *reinterpret_cast<V*>(to + apart) = was_y;
         }
       }
     }
@@ -168,7 +171,7 @@ __global__ void __launch_bounds__(WARPS * 32) rope_kernel(const __grid_constant_
 int vector_of(const enigma_rope_desc& d) {
   const int64_t es = d.dtype == ENIGMA_DTYPE_F32 ? 4 : 2;
   const bool half = d.layout == ENIGMA_ROPE_HALF;
-  int64_t all = half ? d.rotary_dim / 2 : d.rotary_dim;
+  int64_t all = half ? d.rotary_dim / 2 | (d.head_dim - d.rotary_dim) / 2 : d.rotary_dim;
   all |= d.head_dim | d.rotary_dim | d.q_token | d.q_head | d.oq_token | d.oq_head;
   uintptr_t at = reinterpret_cast<uintptr_t>(d.q) | reinterpret_cast<uintptr_t>(d.out_q);
   if (d.heads_k > 0) {
@@ -183,7 +186,8 @@ int vector_of(const enigma_rope_desc& d) {
 template <typename T, int E>
 cudaError_t launch(const enigma_rope_desc& d, Rope r, cudaStream_t s) {
   const bool half = d.layout == ENIGMA_ROPE_HALF;
-  const int64_t units = (half || E == 1 ? r.rotary / 2 / E : r.rotary / E) + (r.d - r.rotary) / E;
+  const int64_t rest = (r.d - r.rotary) / E;
+  const int64_t units = half || E == 1 ? r.rotary / 2 / E + (rest + 1) / 2 : r.rotary / E + rest;
   // Parts of a token where there are fewer than 16 warps an SM, of at least one round of heads.
   const int64_t sms = enigma::sm_count(), groups = std::max<int64_t>(1, 32 / units);
   const int64_t rounds = (r.heads + groups - 1) / groups;
