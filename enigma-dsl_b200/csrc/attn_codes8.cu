@@ -187,9 +187,10 @@ __device__ __forceinline__ float sum_over_keys(float x) {
 // 0 where nothing was seen, so that no difference of infinities is taken.
 __device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.f : top; }
 
-// Where chunk c (16 bytes) of row r is in a tile (of its first part: DT is MAIN here).  Eight lanes that load at once must find eight
-// different 16-byte columns of a 128-byte line: of K, lanes of two neighbouring rows and four
-// neighbouring chunks; of V, of two neighbouring chunks and every second of eight rows.
+// Where chunk c (16 bytes) of row r is in a tile (of its first part: DT is MAIN here).  Eight lanes that
+// load at once must find eight different 16-byte columns of a 128-byte line: of K, lanes of two
+// neighbouring rows and four neighbouring chunks; of V, of two neighbouring chunks and every second
+// of eight rows.
 template <int DT>
 __device__ __forceinline__ uint32_t k_at(int r, int c) {
   if (DT == 64) return uint32_t(r * 64 + c * 16);
@@ -267,13 +268,14 @@ struct Pieces {
 
 // T: of queries and results; DT: the head's elements, rounded up; H: query heads of a unit.
 template <typename T, bool E4M3, int DT, int H>
-__global__ void __launch_bounds__(Cfg<T, DT, H>::THREADS, 1) attend_codes8_kernel(const __grid_constant__ Attend a) {
+__global__ void __launch_bounds__(Cfg<T, DT, H>::THREADS, 1)
+    attend_codes8_kernel(const __grid_constant__ Attend a) {
   using C = Cfg<T, DT, H>;
   constexpr bool SPLIT = sizeof(T) == 4, BESIDE = H == 4;
   static_assert(!BESIDE || SPLIT);
   constexpr int MAIN = C::MAIN, TAILS = C::TAILS, TAIL = C::KEYS * 16;   // (bytes of a tail in a tile)
   constexpr int MT = C::MT, NT = C::NT, KEYS = C::KEYS, WARPS = C::WARPS, THREADS = C::THREADS;
-  constexpr int PARTS = SPLIT && !BESIDE ? 4 : 2;            // registers of an operand: two halves of the inner index
+  constexpr int PARTS = SPLIT && !BESIDE ? 4 : 2;            // registers of an operand: inner index, two parts
   extern __shared__ __align__(128) uint8_t smem[];       // rings, list entries before each b, last chunks
   __shared__ __align__(16) float s_scale[WARPS][C::STAGES][2 * MT];
   __shared__ Pieces<C> s_pieces;
@@ -1073,8 +1075,8 @@ bool whole(const enigma_sdpa_quantized_desc& d) {
   return units <= sms && bytes * (5 * sms - 4 * units) / (5 * sms) <= (170 << 10);
 }
 
-// Calls f with the elements of a head that the kernel is made for: 80 and 96 by themselves (38 x 4096 keys, 8 heads of
-// 80: 58 us, 75 as heads of 128), others rounded up.
+// Calls f with the elements of a head that the kernel is made for: 80 and 96 by themselves (38 x 4096
+// keys, 8 heads of 80: 58 us, 75 as heads of 128), others rounded up.
 template <int H, typename F>
 auto with_elements(int64_t head_dim, F f) {
   using std::integral_constant;

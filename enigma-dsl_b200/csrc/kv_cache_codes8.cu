@@ -238,7 +238,7 @@ template <typename T, bool E4M3, bool VEC, int NV, int P>
 __global__ void __launch_bounds__(WWARPS * 32, 32 / WWARPS) write_codes8_kernel(const __grid_constant__ Write w) {
   __shared__ Part s_part[kScaleBlock];
   __shared__ uint32_t s_found, s_twice;                    // parts there are, parts that another entry changes
-  __shared__ uint32_t s_own;                               // entries (the block's first, ...) that clash with no part
+  __shared__ uint32_t s_own;                               // entries from s_first on that clash with no part
   __shared__ int s_first;                                  // the block's first entry
   __shared__ int s_few;                                    // no part has more than 32 vectors: 1; 64: 2
   __shared__ uint32_t s_tops[2][WWARPS];
@@ -382,10 +382,11 @@ struct Read {
   const int32_t* lens;
 };
 
-// Blocks (c, y): packed rows [16 c, 16 c + 16): their look-ups as above, then a warp per row or piece of one,
-// its lanes along the heads, READ vectors of K and of V at once.  Rows before the first entry and behind the last are left as they
-// were, a token that the slot does not hold is zeros.  Bound by memory: 32768 tokens of 8 heads of 128,
-// bf16, 36 us (5.6 TB/s of codes and rows), 8192 9.0; 256 single tokens 4.5 us, the look-ups.
+// Blocks (c, y): packed rows [16 c, 16 c + 16): their look-ups as above, then a warp per row or piece of
+// one, its lanes along the heads, READ vectors of K and of V at once.  Rows before the first entry and
+// behind the last are left as they were, a token that the slot does not hold is zeros.  Bound by memory:
+// 32768 tokens of 8 heads of 128, bf16, 36 us (5.6 TB/s of codes and rows), 8192 9.0; 256 single tokens
+// 4.5 us, the look-ups.
 template <typename T, bool E4M3, bool VEC, int READ>
 __global__ void __launch_bounds__(WWARPS * 32) read_codes8_kernel(const __grid_constant__ Read w) {
   constexpr int E = kVec<T>;
