@@ -12,7 +12,7 @@
 // joins its warps' pieces after its only barrier, and what goes past a block's ends is joined by
 // join_codes8_kernel.
 // Measured, replayed from a graph: 192 contexts of 500 to 8000 keys, 8 kv heads of 128, bf16: 272 us, 6.2
-// TB/s of codes and scales.  16 of 1 to 8191 keys: 35.4 us, 3.8 TB/s, of which the keys take 20; the rest
+// TB/s of codes and scales.  16 of 1 to 8191 keys: 33.4 us, 4.0 TB/s, of which the keys take 20; the rest
 // is the launches (2 us), the ranges (2), the joins in the blocks (3) and behind them (3), and the
 // first chunk's way.  64 of 2049 keys, 2 heads of 64: 11.1 us.  One of 131071, fp32: 56 us, 4.8 TB/s, bound by
 // instructions: each product is made twice, P's exponentials and splits are as many as in bf16.
@@ -50,17 +50,18 @@ namespace {
 using namespace enigma_codes8;
 using namespace enigma_sm100;
 
-// The work list's unit starts count as STARTS chunks: loading its queries and writing its result takes
-// a warp about as long.  A block gets LEAST entries or more, if the list has as many: so it has a chunk,
-// and a unit's pieces are in consecutive blocks.
-constexpr int STARTS = 1;
-constexpr int LEAST = 2;
-
 template <typename T, int DT, int H>
 struct Cfg {
   static constexpr int NT = (H + 7) / 8;                  // tiles of 8 columns
+  // The work list's unit starts count as STARTS chunks: loading its queries and writing its result takes a
+  // warp about as long (16 of 1 to 8191 keys, heads of 128: 33.4 us, 35.4 with one, 33.6 with three, but
+  // 192 long contexts 0.9 % longer with three; heads of 256, 42.4, 43.8 with two).  A block gets LEAST
+  // entries or more, if the list has as many: so it has a chunk, and a unit's pieces are in consecutive
+  // blocks.
+  static constexpr int STARTS = DT > 128 ? 4 : 2;
+  static constexpr int LEAST = STARTS + 2;
   // As many warps as their registers leave room for: O, queries and a chunk's operands.  12 against 8:
-  // 192 long contexts of heads of 128 272 us, 281; 16 ragged ones 35.4, 38; fp32 heads of 64, 32 x 4096
+  // 192 long contexts of heads of 128 272 us, 281; 16 ragged ones 35, 38; fp32 heads of 64, 32 x 4096
   // keys, 37, 40.  Two tiles of heads of 128 need 8: 42 us (64 x 4096 keys, 2 kv heads), 57 with 10.
   static constexpr int WARPS = NT == 1 && DT < 256 || DT * NT <= 128 ? 12 : 8;
   static constexpr int THREADS = WARPS * 32;
@@ -273,6 +274,7 @@ __global__ void __launch_bounds__(Cfg<T, DT, H>::THREADS, 1)
   using C = Cfg<T, DT, H>;
   constexpr bool SPLIT = sizeof(T) == 4, BESIDE = H == 4;
   static_assert(!BESIDE || SPLIT);
+  constexpr int STARTS = C::STARTS, LEAST = C::LEAST;
   constexpr int MAIN = C::MAIN, TAILS = C::TAILS, TAIL = C::KEYS * 16;   // (bytes of a tail in a tile)
   constexpr int MT = C::MT, NT = C::NT, KEYS = C::KEYS, WARPS = C::WARPS, THREADS = C::THREADS;
   constexpr int PARTS = SPLIT && !BESIDE ? 4 : 2;            // registers of an operand: inner index, two parts

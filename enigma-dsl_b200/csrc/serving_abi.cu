@@ -158,8 +158,9 @@ int32_t check_quantized(const enigma_sdpa_quantized_desc* d) {
   if (d->pages > kInt31 / (d->heads_kv * d->page) || d->table_width > (kInt31 - 256) / d->page ||
       d->n_slots > kInt31)
     return bad("sdpa_quantized: sizes must fit in int32");
-  // The kernel counts a batch's chunks of 16 keys or more in 32 bits, a thread's share of all heads' too.
-  const int64_t chunks = d->batch * (d->table_width * d->page / 16 + 2);
+  // The kernel counts a batch's chunks of 16 keys or more, and up to four for a sequence's start, in 32
+  // bits, a thread's share of all heads' too.
+  const int64_t chunks = d->batch * (d->table_width * d->page / 16 + 5);
   if (chunks > kInt31 || double(chunks) * double(d->heads_q) > 1e12)
     return bad("sdpa_quantized: more keys than one call takes");
   return ENIGMA_OK;
