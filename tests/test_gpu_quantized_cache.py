@@ -249,6 +249,33 @@ def test_many_entries(cuda):
     np.testing.assert_array_equal(_np(v), ref[1])
 
 
+@pytest.mark.parametrize("heads,d,dtype,lens", [
+    (1, 64, "bf16", [29000, 3]), (2, 16, "bf16", [7, 40000]), (1, 256, "f32", [28999]),
+    (1, 256, "bf16", [28500, 500]), (24, 32, "bf16", [600, 31]), (32, 128, "f32", [100, 1, 17])])
+def test_long_requests_and_many_heads(cuda, heads, d, dtype, lens):
+    """Requests that fill the GPU many times over, and rows of many heads; from the middle of a block."""
+    rng = np.random.default_rng(heads + d)
+    page, n = 128, len(lens)
+    cache, want = _make(cuda, rng, 1, sum(x // page + 2 for x in lens), heads, page, d, n,
+                        max(lens) // page + 2, [], "int8")
+    slots, starts = list(range(n)), [5] * n
+    cache.reserve(slots, [x + 5 for x in lens])
+    want.reserve(slots, [x + 5 for x in lens])
+    for at, count in (([0] * n, starts), (starts, lens)):
+        cu = np.concatenate([[0], np.cumsum(count)])
+        x = _values(rng, (int(cu[-1]), heads, d), dtype)
+        t = _dev(x, dtype, cuda)
+        cache.write(0, t, t, slots, at, cu)
+        want.write(0, x, x, slots, at, cu)
+    cache.check()
+    _same(cache, want)
+    got = cache.read(0, slots, starts, cu, dtype=t.dtype)
+    ref = np.zeros((2, *x.shape))
+    want.read(0, slots, starts, cu, *ref)
+    for y, r in zip(got, ref):
+        np.testing.assert_array_equal(_np(y), r)
+
+
 @pytest.mark.parametrize("n,near", [(40, True), (300, True), (2500, False), (9000, True)])
 def test_entries_that_clash(cuda, n, near):
     """Among many entries some name a block that another does, next to it or far away, before or behind:
@@ -546,6 +573,39 @@ def test_attend_unseen_values_do_not_reach(cuda, code, dtype, page):
     # Numbers of pages behind a sequence's last key.
     for s, n in enumerate(lens):
         cache.table[s, -(-n // page):] = [-7, 1 << 30, 3][s % 3]
+    assert (cache.attend(0, q) == clean).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [80, 96, 128, 256])
+@pytest.mark.parametrize("heads_q", [6, 32])
+def test_attend_unseen_and_nan_other_heads(cuda, d, heads_q, dtype):
+    """The same for other head sizes and groups: what is behind the last key reaches nobody, NaN in an
+    element of a value that is seen reaches that element of that sequence's kv head alone."""
+    import torch
+    rng = np.random.default_rng(d)
+    lens = [1, 31, 32, 50, 0, 700]
+    cache, want = _make(cuda, rng, 1, 60, 2, 32, d, 6, 40, lens, "e4m3")
+    q = _dev(_values(rng, (6, heads_q, d), dtype), dtype, cuda)
+    clean = cache.attend(0, q)
+    used = torch.zeros(60, 32, dtype=torch.bool)
+    for s, n in enumerate(lens):
+        for j in range(n):
+            used[want.table[s, j // 32], j % 32] = True
+    unseen = ~used.to(cuda)[None, :, None, :, None]
+    for x in (cache.k, cache.v):
+        raw = x.view(torch.int8)
+        raw.copy_(torch.where(unseen, torch.full_like(raw, 127), raw))   # NaN
+    assert (cache.attend(0, q) == clean).all()
+    group = heads_q // 2
+    for s, j, e in ((3, 49, d - 1), (5, 333, d - 16), (0, 0, 0), (5, 0, 63)):
+        p, r = int(want.table[s, j // 32]), j % 32
+        raw = cache.v.view(torch.int8)
+        was = int(raw[0, p, 1, r, e])
+        raw[0, p, 1, r, e] = 127
+        nan = torch.isnan(cache.attend(0, q))
+        raw[0, p, 1, r, e] = was
+        assert nan[s, group:, e].all() and int(nan.sum()) == group
     assert (cache.attend(0, q) == clean).all()
 
 
