@@ -61,8 +61,8 @@ struct Cfg {
   static constexpr int STARTS = DT > 128 ? 4 : 2;
   static constexpr int LEAST = STARTS + 2;
   // As many warps as their registers leave room for: O, queries and a chunk's operands.  12 against 8:
-  // 192 long contexts of heads of 128 272 us, 281; 16 ragged ones 35, 38; fp32 heads of 64, 32 x 4096
-  // keys, 37, 40.  Two tiles of heads of 128 need 8: 42 us (64 x 4096 keys, 2 kv heads), 57 with 10.
+  // 192 long contexts of heads of 128 272 us, 288; 16 ragged ones 33, 36; fp32 heads of 64, 47 x 4096
+  // keys, 49, 54.  Two tiles of heads of 128 need 8: 42 us (64 x 4096 keys, 2 kv heads), 57 with 10.
   static constexpr int WARPS = NT == 1 && DT < 256 || DT * NT <= 128 ? 12 : 8;
   static constexpr int THREADS = WARPS * 32;
   static constexpr int SLOTS = WARPS + 2;                // pieces of a block in the workspace: its warps'
@@ -1050,8 +1050,8 @@ __global__ void __launch_bounds__(256) join_codes8_kernel(const Attend a) {
 }
 
 // Query heads that a unit takes.  16 where the group is larger than 8, so that codes are read and
-// converted once for two tiles (64 x 4096 keys, 2 kv heads for 32: of 128 42 us against 49, of 64 23
-// against 29), but where registers have no room for them: heads of 256, and fp32.  4 in fp32 where the
+// converted once for two tiles (2 kv heads for 32: 95 x 4096 keys of 128 58 us against 69, 190 of 64 57
+// against 70), but where registers have no room for them: heads of 256, and fp32.  4 in fp32 where the
 // group is no larger: both parts of a query and of P in one tile (one context of 131071: 56 us, 65).
 int unit_heads(const enigma_sdpa_quantized_desc& d) {
   const int64_t group = d.heads_q / d.heads_kv;
@@ -1068,9 +1068,9 @@ int64_t units_of(const enigma_sdpa_quantized_desc& d) {
 // block per unit, which saves the ranges and the joins, where the longest unit there may be is
 // small, the larger the fewer SMs it leaves idle.  us, heads of 128, all of the longest length or
 // of 1 to it:
-//   8 units (heads of 64) of 128 KB: 7.8, 7.6 (split 8.6, 8.6); 256 KB: 10.2, 10.2 (9.0, 9.0)
-//   64 of 256 KB: 11.7, 11.3 (13.3, 11.3);           512 KB: 17.2, 16.6 (15.8, 13.7)
-//   128 of 512 KB: 18.0, 17.0 (21.7, 17.6);          1 MB: 30.1, 27.2 (33.8, 23.6)
+//   8 units (heads of 64) of 128 KB: 7.8, 7.6 (split 8.6, 8.4); 256 KB: 10.2, 10.0 (9.0, 8.8)
+//   64 of 256 KB: 11.7, 11.3 (13.3, 10.9);           512 KB: 17.0, 16.6 (15.8, 13.7)
+//   128 of 512 KB: 17.8, 17.0 (21.5, 17.0);          1 MB: 29.9, 27.2 (33.8, 22.1)
 bool whole(const enigma_sdpa_quantized_desc& d) {
   const int64_t sms = enigma::sm_count(), units = units_of(d);
   const int64_t bytes = 2 * d.head_dim * d.page * d.table_width;         // of the longest unit there may be
