@@ -670,14 +670,16 @@ def rope(q, k, positions, table: RopeTable, inverse: bool = False, out_q=None, o
         if len(table.heads) >= 64:
             table.heads.clear()
         table.heads[key] = head
-    index = _same_device("rope", q, positions, table.turns)
+    index = q.get_device()
+    if (positions.get_device() != index or table.turns.get_device() != index or index not in _initialised
+            or k is not None and k.get_device() != index
+            or out_q is not None and out_q.get_device() != index
+            or out_k is not None and out_k.get_device() != index):
+        _same_device("rope", q, *(x for x in (positions, table.turns, k, out_q, out_k) if x is not None))
     if out_q is None:
         out_q = _contiguous_like(q)
     if k is not None and out_k is None:
         out_k = _contiguous_like(k)
-    for x in (k, out_q, out_k):
-        if x is not None and x.get_device() != index:
-            raise ValueError("rope: all tensors must be on the same device")
     desc = head + _ROPE_PTRS.pack(positions.data_ptr(), table.turns.data_ptr(), q.data_ptr(),
                                   0 if k is None else k.data_ptr(), out_q.data_ptr(),
                                   0 if k is None else out_k.data_ptr())
