@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(WWARPS * 32, 32 / WWARPS) write_codes8_kernel(
   const int page = 1 << r.page_shift, per_page = page / kScaleBlock;
   griddep_launch_dependents();
   griddep_wait();
-  constexpr int AHEAD = 4;               // entries' slots that a thread loads at once, at first while
+  constexpr int AHEAD = 2;               // entries' slots that a thread loads at once, at first while
   int slots[AHEAD];                      // the parts are looked up
   auto load_slots = [&](int j) {         // (an entry past the last is the last again)
 #pragma unroll
