@@ -364,9 +364,11 @@ class QuantizedKVCache(PagedKVCache):
         self._rows_call("read", "enigma_kv_cache_q8_read", layer, out_k, out_v, slots, starts, cu)
         return out_k, out_v
 
-    def attend(self, layer: int, q, slots=None, scale: Optional[float] = None, out=None,
+    def attend(self, layer: int, q, slots=None, *, scale: Optional[float] = None, out=None,
                workspace=None):
-        """cuda_ops.sdpa_quantized over one layer of this cache."""
+        """cuda_ops.sdpa_quantized over one layer of this cache.  Every sequence reads its keys for
+        itself: there is no prefix_len, which PagedKVCache.attend takes after slots, so what follows
+        slots is named."""
         slots = None if slots is None else self._ints("attend", slots)
         head, need, pages = self._checked(
             (layer, (q.shape, q.stride(), q.dtype), None if slots is None else slots.shape,
