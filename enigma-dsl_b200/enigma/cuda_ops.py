@@ -509,7 +509,7 @@ def rope_frequencies(rotary_dim: int, theta: float = 1e6, scaling: Optional[dict
       {"type": "yarn", "factor": f, "original_len": L, "beta_fast": 32, "beta_slow": 1}: pairs that
         turn more than beta_fast times over L positions keep w_i, those below beta_slow get w_i / f,
         linearly in i between the two (at i(beta) = n ln(L / 2 pi beta) / 2 ln theta, rounded
-        outwards); the factor is "attention_factor", by default 0.1 ln f + 1;
+        outwards); the factor is "attention_factor", by default 0.1 ln f + 1, or 1 for f up to 1;
       {"type": "bands", "factor": f, "original_len": L, "low": a, "high": b}: pairs that turn
         more than b times over L keep w_i, those below a get w_i / f, linearly in the number of
         turns between.
@@ -554,7 +554,7 @@ def rope_frequencies(rotary_dim: int, theta: float = 1e6, scaling: Optional[dict
         lo, hi = max(math.floor(at[0]), 0), min(math.ceil(at[1]), n - 1)
         ramp = [min(1.0, max(0.0, (i - lo) / max(hi - lo, 1e-3))) for i in range(n // 2)]
         return ([x * (1 - r) + x / f * r for x, r in zip(w, ramp)],
-                0.1 * math.log(f) + 1 if factor is None else factor)
+                0.1 * math.log(max(f, 1.0)) + 1 if factor is None else factor)
     if kind == "bands":
         length, low, high = take("original_len", "low", "high")
         if not (length > 0 and high > low):

@@ -20,3 +20,16 @@ def test_attend_takes_no_prefix_by_position(calls):  # noqa: F811
     assert not any(name.startswith("enigma_sdpa") for name, _ in calls.calls)
     cache.attend(0, q, slots, scale=0.1, out=torch.zeros_like(q))
     assert calls.calls[-1][0] == "enigma_sdpa_quantized"
+
+
+def test_yarn_factor_of_no_stretch():
+    """The default factor on cos and sin is 0.1 ln f + 1 where a context is stretched, and 1 where it is
+    not (f up to 1); a factor that is given stands."""
+    import math
+    from enigma.cuda_ops import RopeTable, rope_frequencies
+    for f, want in ((0.5, 1.0), (0.999, 1.0), (1.0, 1.0), (1.5, 0.1 * math.log(1.5) + 1),
+                    (32.0, 0.1 * math.log(32.0) + 1)):
+        scaling = dict(type="yarn", factor=f, original_len=4096)
+        assert rope_frequencies(64, 1e4, scaling)[1] == pytest.approx(want, rel=1e-15)
+        assert RopeTable(64, theta=1e4, scaling=scaling, device="cpu").factor == pytest.approx(want, rel=1e-15)
+        assert rope_frequencies(64, 1e4, dict(scaling, attention_factor=0.75))[1] == 0.75
