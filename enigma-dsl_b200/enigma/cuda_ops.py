@@ -523,6 +523,8 @@ def rope_frequencies(rotary_dim: int, theta: float = 1e6, scaling: Optional[dict
     kind, f = spec.pop("type", None), float(spec.pop("factor", 1.0))
     if not f > 0.0 or not math.isfinite(f):
         raise ValueError("rope: the scaling's factor must be positive")
+    if kind == "none" and f != 1.0:
+        raise ValueError("rope: a factor without a scaling to use it")
 
     def take(*names, **defaults):
         values = [spec.pop(x) for x in names if x in spec]

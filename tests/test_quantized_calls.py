@@ -33,3 +33,10 @@ def test_yarn_factor_of_no_stretch():
         assert rope_frequencies(64, 1e4, scaling)[1] == pytest.approx(want, rel=1e-15)
         assert RopeTable(64, theta=1e4, scaling=scaling, device="cpu").factor == pytest.approx(want, rel=1e-15)
         assert rope_frequencies(64, 1e4, dict(scaling, attention_factor=0.75))[1] == 0.75
+
+
+def test_a_factor_that_nothing_would_use_is_refused():
+    from enigma.cuda_ops import rope_frequencies
+    with pytest.raises(ValueError, match="factor"):
+        rope_frequencies(64, 1e4, {"type": "none", "factor": 8})
+    assert rope_frequencies(64, 1e4, {"type": "none", "factor": 1}) == rope_frequencies(64, 1e4)
