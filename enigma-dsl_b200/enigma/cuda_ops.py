@@ -551,6 +551,8 @@ def rope_frequencies(rotary_dim: int, theta: float = 1e6, scaling: Optional[dict
                                           attention_factor=None)
         if not (length > 0 and fast > 0 and slow > 0):
             raise ValueError("rope: yarn scaling's numbers must be positive")
+        if fast < slow:
+            raise ValueError("rope: yarn scaling needs beta_fast of at least beta_slow")
         at = [n * math.log(length / (beta * 2 * math.pi)) / (2 * math.log(theta))
               for beta in (fast, slow)]
         lo, hi = max(math.floor(at[0]), 0), min(math.ceil(at[1]), n - 1)

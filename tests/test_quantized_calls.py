@@ -40,3 +40,13 @@ def test_a_factor_that_nothing_would_use_is_refused():
     with pytest.raises(ValueError, match="factor"):
         rope_frequencies(64, 1e4, {"type": "none", "factor": 8})
     assert rope_frequencies(64, 1e4, {"type": "none", "factor": 1}) == rope_frequencies(64, 1e4)
+
+
+def test_yarn_borders_in_the_wrong_order_are_refused():
+    """Pairs that turn more than beta_fast times stay, those below beta_slow are stretched: with beta_fast
+    below beta_slow some pairs would be both."""
+    from enigma.cuda_ops import rope_frequencies
+    scaling = dict(type="yarn", factor=4.0, original_len=4096)
+    with pytest.raises(ValueError, match="beta"):
+        rope_frequencies(64, 1e4, dict(scaling, beta_fast=1.0, beta_slow=32.0))
+    rope_frequencies(64, 1e4, dict(scaling, beta_fast=4.0, beta_slow=4.0))
