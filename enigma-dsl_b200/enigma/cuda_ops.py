@@ -625,12 +625,15 @@ def _check_distinct(name, *tensors):
 def _rope_head(table, q, k, positions, out_q, out_k, inverse):
     """Checks the (shape, stride, dtype) of a call with this table and packs the desc's head."""
     torch = _torch()
+    shapes = "rope: expected q and k [tokens, heads, head_dim]"
+    if len(q[0]) != 3:
+        raise ValueError(shapes)
     if k is None:
         if out_k is not None:
             raise ValueError("rope: out_k without k")
         k, out_k = ((q[0][0], 0, q[0][-1]), (0, 0, 1), q[2]), None
-    if len(q[0]) != 3 or len(k[0]) != 3 or q[0][0] != k[0][0] or q[0][2] != k[0][2]:
-        raise ValueError("rope: expected q and k [tokens, heads, head_dim]")
+    if len(k[0]) != 3 or q[0][0] != k[0][0] or q[0][2] != k[0][2]:
+        raise ValueError(shapes)
     tokens, hq, d = q[0]
     if d != table.head_dim:
         raise ValueError(f"rope: the table was made for heads of {table.head_dim}")

@@ -50,3 +50,14 @@ def test_yarn_borders_in_the_wrong_order_are_refused():
     with pytest.raises(ValueError, match="beta"):
         rope_frequencies(64, 1e4, dict(scaling, beta_fast=1.0, beta_slow=32.0))
     rope_frequencies(64, 1e4, dict(scaling, beta_fast=4.0, beta_slow=4.0))
+
+
+def test_queries_without_heads_are_refused(calls):  # noqa: F811
+    """A wrong number of axes is a ValueError whether keys come along or not."""
+    from enigma import cuda_ops
+    from test_quantized_host import _table
+    for q in (_on_one(64), _on_one(64)[0], _on_one(5, 64)):
+        for k in (None, _on_one(5, 2, 64)):
+            with pytest.raises(ValueError):
+                cuda_ops.rope(q, k, _ints(5), _table())
+    assert not any(name == "enigma_rope" for name, _ in calls.calls)
