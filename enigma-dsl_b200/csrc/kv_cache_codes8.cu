@@ -1,8 +1,8 @@
 // kv_cache_codes8.cu — a paged cache in 8-bit codes: rows quantised as they are written, and read back.
 //
 // Codes and scales are those of codes8.cuh.  A write that starts inside a block of 16 tokens keeps
-// the block's earlier tokens: the scale becomes the larger of the block's and what the new tokens
-// need, and if it grows the earlier codes are rounded to it.  A write that starts a block, or
+// the block's earlier tokens: the scale becomes the larger (in magnitude) of the block's and what the new
+// tokens need, and if it grows the earlier codes are rounded to it.  A write that starts a block, or
 // goes on behind it, sets the scale from the new tokens alone: what the page held before, or a
 // sequence that was cut short, does not count.  So a sequence's tokens are written in order, and
 // what stands in a block behind the last written token means nothing.  A value that is not finite
@@ -186,10 +186,13 @@ __device__ __forceinline__ void write_blocks(const Block<T> (&b)[N], int d, int 
 #pragma unroll
       for (int y = 0; y < P; ++y) top = max(top, tops[y]);
     }
-    const bool finite = top < 0x7f800000u && fabsf(held[k]) < INFINITY;
-    const float scale = finite ? fmaxf(held[k], scale_of<E4M3>(top)) : __uint_as_float(0x7fffffffu);
+    // Scales compare by magnitude: a block of a cache made elsewhere may have a negative one, which stays as it
+    // is where it is large enough.
+    const float need = scale_of<E4M3>(top);
+    const bool finite = top < 0x7f800000u && fabsf(held[k]) < INFINITY, grows = fabsf(held[k]) < need;
+    const float scale = !finite ? __uint_as_float(0x7fffffffu) : grows ? need : held[k];
     const float inverse = finite ? 1.f / scale : 0.f;
-    if (finite && held[k] < scale) {     // (r0 = 0: there are no old rows)
+    if (finite && grows) {               // (r0 = 0: there are no old rows)
       for (int w = lane + 32 * q; w < b[k].r0 * (d / 4); w += 32 * P) {
         uint32_t* word = reinterpret_cast<uint32_t*>(b[k].codes) + w;
         uint32_t lo, hi;

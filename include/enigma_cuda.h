@@ -369,7 +369,9 @@ int32_t enigma_rope(const enigma_rope_desc* desc, void* stream);
  *          power of two 2^e under which the block's largest magnitude (2^-110 if that is more) is at most
  *          127, or 448, and a code is the value over the scale, rounded to nearest (ties to
  *          even).  A write that starts behind a block's first token keeps the block's earlier
- *          tokens: its scale is the larger of the block's and the new tokens', and where it
+ *          tokens: its scale is the larger of the block's and the new tokens' (in magnitude: the
+ *          block's may be any finite number, and stays where it is the larger one, the new codes
+ *          being rounded from products with its fp32 reciprocal), and where it
  *          grows the earlier codes are rounded to it.  What a block held behind the last
  *          written token is lost.  A value that is not finite makes its block's scale NaN, until
  *          a write starts the block anew.  A page that forks share is not written

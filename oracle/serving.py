@@ -233,7 +233,7 @@ class QuantizedPages(Pages):
                     scale = np.where(finite, scale_of(top, self.code), np.nan)
                     old = scales[layer, p, :, j]
                     if r:
-                        scale = np.where(np.isnan(old), np.nan, np.maximum(scale, old))
+                        scale = np.where(np.isnan(old), np.nan, np.where(np.abs(old) < scale, scale, old))
                         held = codes[layer, p, :, o:o + r]
                         grown = np.where(np.isnan(scale), 1.0, old / scale)[:, None, None]
                         codes[layer, p, :, o:o + r] = to_code(held * grown, self.code)
