@@ -63,3 +63,113 @@ def test_append_behind_any_scale(cuda, code):
                                                                  -6) - 3)
             off = np.abs(values[p][:, :lens] - true)
             assert (off <= np.abs(got[0, p][..., None]) * (step / 2 + y * 2.0 ** -22)).all()
+
+
+# ------------------------------------------------------------------------- rows of any alignment
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype,gap", [("bf16", 1), ("bf16", 3), ("bf16", 4), ("f32", 1), ("f32", 3)])
+@pytest.mark.parametrize("heads,page,d", [(2, 16, 64), (3, 64, 128), (1, 32, 16), (2, 128, 80), (2, 64, 96),
+                                          (1, 16, 144), (2, 32, 160), (1, 64, 256)])
+def test_write_rows_off_16_bytes(cuda, heads, page, d, dtype, gap, code):
+    """Rows that start and lie anywhere: single tokens, short parts, whole blocks, each alone in a request
+    (so that a block has them in one, two or more vectors a lane) and together."""
+    rng = np.random.default_rng(heads + d + gap)
+    cache, want = _make(cuda, rng, 1, 40, heads, page, d, 6, 4 * 128 // page, [5, 17, 0, 2 * page], code)
+    for counts in ([1, 1, 1, 1], [2, 3, 5, 1], [page + 9, 0, 33, 16], [1, 20, 3, 40]):
+        slots = [3, 0, 1, 2]
+        starts = [int(want.lens[s]) for s in slots]
+        lens = [a + b for a, b in zip(starts, counts)]
+        if max(lens) > want.table.shape[1] * page:
+            break
+        cache.reserve(slots, lens)
+        want.reserve(slots, lens)
+        cu = np.concatenate([[0], np.cumsum(counts)])
+        wide = _values(rng, (int(cu[-1]), 2 * heads * d + gap), dtype)
+        t = _dev(wide, dtype, cuda)[:, gap:].unflatten(1, (2 * heads, d))
+        rows = wide[:, gap:].reshape(-1, 2 * heads, d)
+        cache.write(0, t[:, :heads], t[:, heads:], slots, starts, cu)
+        want.write(0, rows[:, :heads], rows[:, heads:], slots, starts, cu)
+        cache.check()
+        _same(cache, want)
+
+
+# ------------------------------------------------------------------- heads of 48, and of 144 to 240
+WIDE = [48, 144, 160, 176, 208, 240]
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("d", WIDE)
+def test_write_and_read_other_heads(cuda, d, page, dtype, code):
+    import torch
+    rng = np.random.default_rng(d + page)
+    heads = 2
+    cache, want = _make(cuda, rng, 1, 30, heads, page, d, 4, 128 // page + 2, [5, 33], code)
+    for counts in ([1, 1, 70], [2, 3, 1], [30, 17, 16]):
+        slots = [0, 1, 3]
+        starts = [int(want.lens[s]) for s in slots]
+        lens = [a + b for a, b in zip(starts, counts)]
+        cache.reserve(slots, lens)
+        want.reserve(slots, lens)
+        cu = np.concatenate([[0], np.cumsum(counts)])
+        x = _values(rng, (int(cu[-1]), heads, d), dtype)
+        cache.write(0, _dev(x, dtype, cuda), _dev(x, dtype, cuda), slots, starts, cu)
+        want.write(0, x, x, slots, starts, cu)
+        cache.check()
+        _same(cache, want)
+    cu = np.concatenate([[0], np.cumsum([int(want.lens[s]) + 2 for s in slots])])
+    ref = np.zeros((2, int(cu[-1]), heads, d))
+    want.read(0, slots, [0, 0, 0], cu, *ref)
+    kind = torch.bfloat16 if dtype == "bf16" else torch.float32
+    for y, r in zip(cache.read(0, slots, [0, 0, 0], cu, dtype=kind), ref):
+        np.testing.assert_array_equal(_np(y), r)
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("heads_q,heads_kv", [(8, 2), (14, 2), (20, 1), (3, 3)])
+@pytest.mark.parametrize("d", WIDE)
+def test_attend_other_heads(cuda, d, heads_q, heads_kv, code):
+    """Pages of one block and of several, short and long contexts, tables as wide as the contexts need and
+    wider."""
+    rng = np.random.default_rng(heads_q + d)
+    for page, lens, more in ((16, [1, 15, 16, 17, 33, 100], 0), (64, [700, 0, 47], 1), (128, [2500, 5], 300)):
+        pages = sum(-(-n // page) for n in lens) + 2
+        for dtype in ("bf16", "f32"):
+            cache, want = _make(cuda, rng, 1, pages, heads_kv, page, d, len(lens),
+                                -(-max(lens) // page) + more, lens, code)
+            got, ref = _attend(cuda, rng, cache, want, heads_q, dtype)
+            _hold(got, ref, max(lens), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [48, 144, 240])
+def test_attend_unseen_and_nan_other_widths(cuda, d, dtype):
+    """What is behind the last key reaches nobody; NaN in an element of a value that is seen reaches that
+    element of that sequence's kv head alone; results between other columns leave those as they were."""
+    import torch
+    rng = np.random.default_rng(d + 1)
+    lens, heads_q = [1, 31, 50, 0, 700], 6
+    cache, want = _make(cuda, rng, 1, 60, 2, 32, d, 5, 40, lens, "e4m3")
+    q = _dev(_values(rng, (5, heads_q, d), dtype), dtype, cuda)
+    clean = cache.attend(0, q)
+    used = torch.zeros(60, 32, dtype=torch.bool)
+    for s, n in enumerate(lens):
+        for j in range(n):
+            used[want.table[s, j // 32], j % 32] = True
+    unseen = ~used.to(cuda)[None, :, None, :, None]
+    for x in (cache.k, cache.v):
+        raw = x.view(torch.int8)
+        raw.copy_(torch.where(unseen, torch.full_like(raw, 127), raw))   # NaN
+    assert (cache.attend(0, q) == clean).all()
+    for s, j, e in ((2, 49, d - 1), (4, 333, d - 16), (0, 0, 0)):
+        p, r = int(want.table[s, j // 32]), j % 32
+        raw = cache.v.view(torch.int8)
+        was = int(raw[0, p, 1, r, e])
+        raw[0, p, 1, r, e] = 127
+        nan = torch.isnan(cache.attend(0, q))
+        raw[0, p, 1, r, e] = was
+        assert nan[s, heads_q // 2:, e].all() and int(nan.sum()) == heads_q // 2
+    wide = torch.full((5, heads_q, d + 3), 7.0, dtype=q.dtype, device=cuda)
+    cache.attend(0, q, out=wide[..., 1:1 + d])
+    assert (wide[..., 1:1 + d] == clean).all() and (wide[..., 0] == 7).all() and (wide[..., 1 + d:] == 7).all()
