@@ -6,7 +6,9 @@
 // elements behind are copied.  The turn back (the transpose, which is also the gradient) has -sin.
 //
 // Angles: turns[i] is w_i / 2 pi as a 64-bit binary fraction, so p * turns[i] modulo 2^64 is the
-// angle modulo a full turn, exactly, for any position; rounding starts at its conversion to fp32.
+// angle modulo a full turn without any rounding of its own, for any position.  What is off is the
+// frequency (made from 64-bit floats: 2^-52 of itself, and half a unit) and the angle's conversion to
+// fp32 (pi 2^-24 radians), which is the larger part up to p * w_i of about 2^29.
 // (An fp32 product p * w_i is off by p * w_i * 2^-24 radians: 0.06 at a position of a million.)
 #include <algorithm>
 

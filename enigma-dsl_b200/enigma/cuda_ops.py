@@ -598,7 +598,8 @@ class RopeTable:
         if not all(map(math.isfinite, frequencies)) or not math.isfinite(factor):
             raise ValueError("rope: frequencies and factor must be finite")
         # Full turns per position, as 64-bit binary fractions (angles are modulo a full turn).
-        turns = [int(math.fmod(x / (2 * math.pi), 1.0) * 2.0 ** 64) % (1 << 64) for x in frequencies]
+        turns = [round(math.fmod(x / (2 * math.pi), 1.0) * 2.0 ** 64) % (1 << 64)
+                 for x in frequencies]
         self.head_dim, self.rotary_dim = int(head_dim), int(rotary_dim)
         self.layout, self.factor = layout, float(factor)
         self.frequencies = frequencies
@@ -664,8 +665,8 @@ def rope(q, k, positions, table: RopeTable, inverse: bool = False, out_q=None, o
     fused projection's output; positions [tokens], int32 or int64 on the device (negative ones turn
     back).  inverse=True turns by the negative angle: the transpose, so it also takes a result's
     gradient to its input's.  out_q / out_k: tensors to write, which may be q and k themselves but not
-    overlap them otherwise.  Angles are exact whatever the position.  Returns (q, k) turned, or q
-    alone without k.
+    overlap them otherwise.  An angle is off by at most 2^-52 of position * frequency, less than its
+    rounding to fp32 up to positions of about 2^29.  Returns (q, k) turned, or q alone without k.
     """
     key = ((q.shape, q.stride(), q.dtype), None if k is None else (k.shape, k.stride(), k.dtype),
            (positions.shape, positions.stride(), positions.dtype),

@@ -61,3 +61,16 @@ def test_queries_without_heads_are_refused(calls):  # noqa: F811
             with pytest.raises(ValueError):
                 cuda_ops.rope(q, k, _ints(5), _table())
     assert not any(name == "enigma_rope" for name, _ in calls.calls)
+
+
+def test_turns_are_rounded_to_nearest():
+    """A frequency's share of a full turn as a 64-bit fraction is off by half a unit, and by the rounding of
+    its 64-bit float (2^-52 of it): also where it is so small that the unit counts."""
+    import math
+    from fractions import Fraction
+    from enigma.cuda_ops import RopeTable
+    w = [x * 10.0 ** -e for e in range(6, 20) for x in (1.0, -1.7, 2.3, 7.9)]
+    t = RopeTable(2 * len(w), frequencies=w, device="cpu")
+    for x, got in zip(w, t.turns.tolist()):
+        want = Fraction(x) / Fraction(2 * math.pi) * 2 ** 64
+        assert abs(got - want) <= abs(want) * Fraction(1, 2 ** 52) + Fraction(1, 2), x
