@@ -42,7 +42,6 @@
 #include <atomic>
 #include <type_traits>
 
-#include "attn_serving.cuh"
 #include "codes8.cuh"
 
 namespace {

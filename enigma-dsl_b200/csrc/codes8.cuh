@@ -12,27 +12,14 @@ namespace enigma_codes8 {
 
 constexpr int kScaleBlock = ENIGMA_SCALE_BLOCK;
 
-// Two codes (low byte first) as halves; both kinds are exact in fp16.
-template <bool E4M3>
-__device__ __forceinline__ uint32_t halves_of(uint32_t two) {
-  uint32_t r;
-  if (E4M3) {
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(uint16_t(two)));
-  } else {
-    // 0x6400 + u is the half 1024 + u: the code's byte with its sign bit turned is code + 128.
-    const uint32_t u = __byte_perm(two ^ 0x8080u, 0x64646464u, 0x4140);
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0x64806480u));
-  }
-  return r;
-}
-
-// Four codes as two pairs of halves.
+// Four codes (low byte first) as two pairs of halves; both kinds are exact in fp16.
 template <bool E4M3>
 __device__ __forceinline__ void halves_of4(uint32_t four, uint32_t* lo, uint32_t* hi) {
   if (E4M3) {
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t"
         "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(*lo), "=r"(*hi) : "r"(four));
   } else {
+    // 0x6400 + u is the half 1024 + u: the code's byte with its sign bit turned is code + 128.
     const uint32_t u = four ^ 0x80808080u;
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*lo) : "r"(__byte_perm(u, 0x64646464u, 0x4140)), "r"(0x64806480u));
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(*hi) : "r"(__byte_perm(u, 0x64646464u, 0x4342)), "r"(0x64806480u));
