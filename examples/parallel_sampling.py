@@ -14,6 +14,7 @@ size, and every sample reads the prompt for itself.
 from __future__ import annotations
 
 import argparse
+import functools
 import sys
 import time
 from dataclasses import dataclass
@@ -63,12 +64,21 @@ class Decoder:
                        for _ in range(cfg.layers)]
         self.embed = torch.randn(cfg.vocab, cfg.hidden, generator=gen, device=self.device).bfloat16()
         self.head = weight(cfg.hidden, cfg.vocab)
-        half = cfg.head_dim // 2
-        inv = cfg.rope_theta ** (-torch.arange(half, device=self.device, dtype=torch.float64)
-                                 * 2.0 / cfg.head_dim)
-        angle = torch.arange(cfg.max_len, device=self.device, dtype=torch.float64)[:, None] * inv
-        self.cos, self.sin = angle.cos().float(), angle.sin().float()    # what `rope` turns by
         self.rope = cuda_ops.RopeTable(cfg.head_dim, theta=cfg.rope_theta, device=self.device)
+
+    def _angles(self):
+        import torch
+        w = torch.tensor(self.rope.frequencies, dtype=torch.float64, device=self.device)
+        return torch.arange(self.cfg.max_len, dtype=torch.float64, device=self.device)[:, None] * w
+
+    # [max_len, head_dim / 2], for a decoder in plain torch to compare with: `rope` needs neither.
+    @functools.cached_property
+    def cos(self):
+        return self._angles().cos().float()
+
+    @functools.cached_property
+    def sin(self):
+        return self._angles().sin().float()
 
     def forward(self, tokens, positions, attention, last=None):
         """Logits (fp32) of the rows `last`, or of all; attention(layer, q, k, v) -> o."""

@@ -74,3 +74,26 @@ def test_turns_are_rounded_to_nearest():
     for x, got in zip(w, t.turns.tolist()):
         want = Fraction(x) / Fraction(2 * math.pi) * 2 ** 64
         assert abs(got - want) <= abs(want) * Fraction(1, 2 ** 52) + Fraction(1, 2), x
+
+
+def test_example_keeps_no_tables_of_angles():
+    """The sampling example turns by its RopeTable; cos and sin of the whole context are made only where a
+    plain decoder asks for them, and are the same turns."""
+    import importlib.util
+    import math
+    import sys
+    from pathlib import Path
+    path = Path(__file__).resolve().parents[1] / "examples" / "parallel_sampling.py"
+    spec = importlib.util.spec_from_file_location("parallel_sampling_host", path)
+    ex = sys.modules[spec.name] = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    cfg = ex.Config(layers=1, hidden=64, heads_q=2, heads_kv=1, head_dim=32, intermediate=64, vocab=16,
+                    max_len=100)
+    model = ex.Decoder(cfg, device="cpu")
+    held = [n for n, x in vars(model).items() if isinstance(x, torch.Tensor) and cfg.max_len in x.shape]
+    assert held == []
+    w = torch.tensor(model.rope.frequencies, dtype=torch.float64)
+    angle = torch.arange(100.0, dtype=torch.float64)[:, None] * w
+    assert (model.cos - angle.cos()).abs().max() <= 2 ** -24 and (model.sin - angle.sin()).abs().max() <= 2 ** -24
+    turns = (model.rope.turns.double() * 2.0 ** -63 * math.pi)               # radians a position, to 2^-52
+    assert torch.allclose(turns.cos(), model.cos[1].double(), rtol=0, atol=2 ** -22)
