@@ -462,7 +462,8 @@ def sdpa_quantized(q, k_pages, v_pages, k_scale, v_scale, table, lens, slots=Non
 
     q [B, Hq, D], bf16 or fp32; k_pages / v_pages [pages, Hkv, page, D], int8 or float8_e4m3fn (one
     layer of a kv_cache.QuantizedKVCache); k_scale / v_scale [pages, Hkv, page / 16] fp32: code x of
-    a block of 16 tokens stands for x * scale.  table [n, width] int32 page numbers, lens [n] int32;
+    a block of 16 tokens stands for x * scale (finite; a weight times its scale is held to 2^-34 of the
+    largest |v_scale| beside it in bf16, 2^-40 in fp32).  table [n, width] int32 page numbers, lens [n] int32;
     sequence b uses row slots[b] (default: row b) and attends to its first lens keys, all read as
     its own (sequences that share pages find them in L2).  A sequence without keys gives zeros, a
     key without a page is zeros.  D is a multiple of 16 up to 256, page 16, 32, 64 or 128.

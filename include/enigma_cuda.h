@@ -409,7 +409,8 @@ int32_t enigma_kv_cache_q8_read(const enigma_kv_cache_q8_desc* desc, const enigm
 /* One new token per sequence over pages of 8-bit codes: q, out [batch, heads_q, head_dim] of type
  * dtype; k_pages, v_pages [pages, heads_kv, page, head_dim] codes, contiguous but for the page
  * strides (k_page, v_page, in codes, multiples of 16); k_scale, v_scale [pages, heads_kv, page /
- * ENIGMA_SCALE_BLOCK], contiguous but for theirs (ks_page, vs_page); scales are any finite numbers.
+ * ENIGMA_SCALE_BLOCK], contiguous but for theirs (ks_page, vs_page); scales are any finite numbers
+ * (a weight times its v_scale is held to 2^-34 of the largest |v_scale| seen with it, 2^-40 in fp32).
  *   out = sum_j softmax_j(scale k_scale_j q . k_j) v_scale_j v_j
  * over the first min(lens, table_width * page) keys; tables, lens and slots as in
  * enigma_sdpa_shared_prefix: no keys, or a slot that does not exist, give zeros, and a key whose
