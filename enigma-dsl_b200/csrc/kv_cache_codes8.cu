@@ -252,8 +252,10 @@ __global__ void __launch_bounds__(WWARPS * 32, 32 / WWARPS) write_codes8_kernel(
   const int page = 1 << r.page_shift, per_page = page / kScaleBlock;
   griddep_launch_dependents();
   griddep_wait();
-  constexpr int AHEAD = 2;               // entries' slots that a thread loads at once, at first while
-  int slots[AHEAD];                      // the parts are looked up
+  // Entries' slots that a thread loads at once, at first while the parts are looked up.  (Four: 4096 single tokens
+  // 22.9 against 23.4 us, 1024 9.0 both, but 16 prompts written and read 48.3 against 47.9.)
+  constexpr int AHEAD = 2;
+  int slots[AHEAD];
   auto load_slots = [&](int j) {         // (an entry past the last is the last again)
 #pragma unroll
     for (int y = 0; y < AHEAD; ++y) slots[y] = r.slots[min(j + y * threads, r.n - 1)];

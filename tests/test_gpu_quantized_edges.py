@@ -173,3 +173,80 @@ def test_attend_unseen_and_nan_other_widths(cuda, d, dtype):
     wide = torch.full((5, heads_q, d + 3), 7.0, dtype=q.dtype, device=cuda)
     cache.attend(0, q, out=wide[..., 1:1 + d])
     assert (wide[..., 1:1 + d] == clean).all() and (wide[..., 0] == 7).all() and (wide[..., 1 + d:] == 7).all()
+
+
+# --------------------------------------------------------------------------- far rows, replayed maps
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rows_past_32_bits(cuda, dtype):
+    """Rows of rope, write, read and attention that lie more than 2^31 elements apart."""
+    import torch
+    from enigma import cuda_ops
+    from enigma.kv_cache import QuantizedKVCache
+    rng = np.random.default_rng(41)
+    kind = torch.bfloat16 if dtype == "bf16" else torch.float32
+    n, heads, d, far = 3, 4, 64, 1_100_000_000              # the last row begins past 2^31 elements
+    pool = torch.empty(2 * far + heads * d, dtype=kind, device=cuda)
+    rows = pool.as_strided((n, heads, d), (far, d, 1))
+    x = _values(rng, (n, heads, d), dtype)
+    near = _dev(x, dtype, cuda)
+    rows.copy_(near)
+    table = cuda_ops.RopeTable(d)
+    at = torch.tensor([5, 1, 900], dtype=torch.int32, device=cuda)
+    want = cuda_ops.rope(near, None, at, table)
+    assert (cuda_ops.rope(rows, None, at, table) == want).all()
+    assert (cuda_ops.rope(rows, None, at, table, out_q=rows) == want).all()
+    caches = [QuantizedKVCache.empty(1, 2, 16, heads, d, 1, 32, device=cuda) for _ in range(2)]
+    for cache, t in zip(caches, (rows, want)):
+        cache.reserve([0], [n])
+        cache.write(0, t, t, [0], [0], [0, n])
+        cache.check()
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert (getattr(caches[0], name) == getattr(caches[1], name)).all()
+    plain = caches[1].attend(0, want, slots=[0] * n)
+    assert (caches[0].attend(0, rows, slots=[0] * n) == plain).all()
+    got = caches[0].attend(0, want, slots=[0] * n, out=rows)
+    assert got.data_ptr() == rows.data_ptr() and (rows == plain).all()
+    other = torch.empty_like(want)
+    caches[0].read(0, [0], [0], [0, n], out_k=rows, out_v=other)
+    k, _ = caches[1].read(0, [0], [0], [0, n], dtype=kind)
+    assert (rows == k).all() and (other == k).all()
+
+
+@pytest.mark.parametrize("code", CODES)
+def test_maps_replayed(cuda, code):
+    """Forks, a write behind them and a compaction as one captured graph, replayed: pages and scales as the
+    same requests give them one by one."""
+    import torch
+    rng = np.random.default_rng(42)
+    cache, want = _make(cuda, rng, 2, 40, 3, 32, 64, 6, 4, [70, 33, 96], code)
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    parents, children, gone = ints(0, 1, 0), ints(3, 4, 5), ints(4)
+    slots, starts, cu = ints(3, 5), ints(70, 70), ints(0, 2, 7)
+    lens = ints(72, 75)
+    x = _values(rng, (7, 3, 64), "bf16")
+    t = _dev(x, "bf16", cuda)
+
+    def requests(c, a, b, s, n, r, begin, packed, g):
+        c.fork(a, b)
+        c.reserve(s, n)
+        c.write(1, r, r, s, begin, packed)
+        c.free(g)
+        c.compact()
+
+    def plain():
+        requests(want, [0, 1, 0], [3, 4, 5], [3, 5], [72, 75], x, [70, 70], [0, 2, 7], [4])
+
+    requests(cache, parents, children, slots, lens, t, starts, cu, gone)
+    plain()
+    cache.check()
+    _same(cache, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        requests(cache, parents, children, slots, lens, t, starts, cu, gone)
+    for i in range(3):
+        t.mul_(2.0)
+        x = x * np.float32(2)
+        graph.replay()
+        plain()
+        cache.check()
+        _same(cache, want)
